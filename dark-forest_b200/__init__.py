@@ -33,6 +33,7 @@ DF_ERR_WORKSPACE = 5
 DF_ERR_STATIC_SCRATCH = 6
 DF_ERR_DEVICE_BOUNDS = 9
 STATIC_SCRATCH_MAX_ROWS = 2097152
+CACHE_WORKSPACE_BYTES = 33554432  # what cache_attention is lent
 VARIANT_AUTO, VARIANT_SIMT, VARIANT_TENSOR = 0, 1, 2
 OPT_FWD_PERSIST, OPT_FUSE_DELTA, OPT_BWD_OVERLAP, OPT_SCHED_TABLE, OPT_DISABLE_TENSOR, OPT_PDL, OPT_CE_VARIANT, OPT_LN_STAGED = range(8)
 
@@ -93,6 +94,12 @@ PROTOTYPES = {
     "df_adamw_update": (ctypes.c_int, [_P] * 4 + [_U64] + [_F32] * 7 + [_P]),
     "df_adamw_plan": (_U64, [_P, _U32]),
     "df_adamw_update_multi": (ctypes.c_int, [_P, _U32, _U64] + [_F32] * 7 + [_P]),
+    "df_cache_plan": (ctypes.c_int, [_P] * 10 + [_U32] * 5 + [_P]),
+    "df_cache_release": (ctypes.c_int, [_P] * 7 + [_U32] * 4 + [_P]),
+    "df_cache_append": (ctypes.c_int, [_P] * 7 + [_U32] * 5 + [_U64] * 2 + [_U32] * 2 + [_P]),
+    "df_cache_attention": (ctypes.c_int, [_P] * 11 + [_U64] + [_U32] * 8 + [_U64, _F32, _U32, _U32, _P]),
+    "df_token_logprobs": (ctypes.c_int, [_P] * 7 + [_U32] * 2 + [_U64, _U32, _F32, _U32, _P]),
+    "df_token_logprobs_backward": (ctypes.c_int, [_P] * 7 + [_U32] * 2 + [_U64] * 2 + [_F32, _U32, _P]),
     "df_attn_init": (ctypes.c_int, []),
     "df_attn_backward_profile": (ctypes.c_int, [_P] * 10 + [_U32] * 4 + [_F32, _U32, _P, _P, _P]),
     "df_attn_set_option": (ctypes.c_int, [ctypes.c_int, ctypes.c_int]),
@@ -310,6 +317,48 @@ def chunked_logit_ce(logits, targets, loss, total_rows, grad_logits=None, stream
     """Softmax + cross-entropy over a chunk: logits [rows, cols] fp32 (overwritten with probabilities when
     grad_logits is given), targets [rows] int32/uint32 token ids, loss [1] fp32 accumulator. grad_logits None: eval form."""
     return _calls.chunked_logit_ce(logits, targets, loss, total_rows, grad_logits, stream)
+
+
+# ------------------------------------------------------------------------------------------
+# A batch of requests over a paged cache in 8 bits. Codes [pages, kv_heads, page_size, d_head] in torch.int8 or
+# torch.float8_e4m3fn, scales [pages, kv_heads] fp32; lengths, tables, slots and counts are int32 tensors on the GPU and
+# are never waited for, so that a step can be captured in a graph. include/darkforest_kernels.h has the definitions.
+# ------------------------------------------------------------------------------------------
+def cache_plan(lens, new_tokens, block_table, free_pages, free_count, page_size, n_tokens, lens_out=None, starts=None, slots=None, positions=None,
+               state=None, stream=None):
+    """Block tables, slots and positions of a step's new tokens: lens, new_tokens [requests], block_table [requests, width] (extended in
+    place), free_pages a stack of which the first free_count[0] entries are free pages, n_tokens the size of the slot map (the sum of new_tokens, or
+    more). Returns (lens_out, starts, slots, positions, state); state[0] = free pages left, state[1] = 0, or why nothing was granted."""
+    return _calls.cache_plan(lens, new_tokens, block_table, free_pages, free_count, page_size, n_tokens, lens_out, starts, slots, positions, state, stream)
+
+
+def cache_release(lens, finished, block_table, free_pages, free_count, page_size, lens_out=None, count_out=None, stream=None):
+    """The pages of requests with finished != 0 go back on the stack free_pages (in place). Returns (lens_out, count_out)."""
+    return _calls.cache_release(lens, finished, block_table, free_pages, free_count, page_size, lens_out, count_out, stream)
+
+
+def cache_append(k, v, slots, k_cache, v_cache, k_scale, v_scale, stream=None):
+    """Quantises k, v [tokens, kv_heads * d_head] (fp32 or bf16; rows may be strided) into the cache at slots, in place; returns the
+    cache's four tensors."""
+    return _calls.cache_append(k, v, slots, k_cache, v_cache, k_scale, v_scale, stream)
+
+
+def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, starts, n_heads, scale, workspace, out=None, lse=None, stream=None):
+    """Attention of q [tokens, n_heads * d_head] (fp32 or bf16; rows may be strided), request after request as starts [requests + 1] says,
+    over the requests' cached tokens (lens [requests], the new ones included). workspace: a zeroed tensor of CACHE_WORKSPACE_BYTES
+    that is kept from call to call. Returns (out, lse [tokens, n_heads])."""
+    return _calls.cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, starts, n_heads, scale, workspace, out, lse, stream)
+
+
+def token_logprobs(logits, targets, scale=1.0, top_k=0, logp=None, entropy=None, lse=None, top_ids=None, top_logp=None, stream=None):
+    """Log probabilities of targets [rows] (int32) under scale * logits [rows, cols] (fp32 or bf16; rows may be strided), with the rows'
+    entropy, logsumexp and top_k best columns. Returns (logp, entropy, lse, top_ids, top_logp)."""
+    return _calls.token_logprobs(logits, targets, scale, top_k, logp, entropy, lse, top_ids, top_logp, stream)
+
+
+def token_logprobs_backward(logits, targets, lse, entropy, grad_logp, grad_entropy=None, scale=1.0, d_logits=None, stream=None):
+    """Gradient of token_logprobs' logp and entropy with respect to the logits, in their type (grad_logp or grad_entropy may be None)."""
+    return _calls.token_logprobs_backward(logits, targets, lse, entropy, grad_logp, grad_entropy, scale, d_logits, stream)
 
 
 # ------------------------------------------------------------------------------------------

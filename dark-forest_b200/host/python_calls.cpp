@@ -30,7 +30,9 @@ namespace {
   X(df_attn_merge_partials) X(df_attn_accumulate) X(df_linear_qkv_forward) X(df_linear_forward) X(df_linear_gelu_forward)    \
   X(df_chunked_logit_ce) X(df_layernorm_forward) X(df_layernorm_backward) X(df_gelu_forward) X(df_gelu_backward)             \
   X(df_adamw_update) X(df_adamw_update_multi) X(launch_fused_attention) X(launch_fused_mha_forward)                          \
-  X(launch_attention_backward) X(launch_fused_mha_backward) X(df_attn_last_status) X(df_attn_status_string)
+  X(launch_attention_backward) X(launch_fused_mha_backward) X(df_attn_last_status) X(df_attn_status_string)                  \
+  X(df_cache_plan) X(df_cache_release) X(df_cache_append) X(df_cache_attention) X(df_token_logprobs)                        \
+  X(df_token_logprobs_backward)
 
 struct Functions {
 #define X(name) decltype(&::name) name = nullptr;
@@ -357,6 +359,174 @@ PyObject *chunked_logit_ce(Args a) {  // logits targets loss total_rows grad_log
   return a[2];
 }
 
+// ---------------------------------------------------------------- cache in 8 bits, log probabilities
+[[noreturn]] void refuse(const char *what, const char *why) {
+  raise(attention_error, (std::string(what) + ": " + why).c_str());
+}
+
+// A tensor argument of a known type and shape (-1: any size), on the GPU and contiguous.
+template <typename T>
+T *typed(PyObject *o, at::ScalarType type, std::initializer_list<int64_t> shape, const char *what) {
+  T *p = ptr<T>(o);
+  const at::Tensor &t = tensor(o);
+  if (t.scalar_type() != type) refuse(what, "wrong dtype");
+  if (t.dim() != static_cast<int64_t>(shape.size())) refuse(what, "wrong number of dimensions");
+  int i = 0;
+  for (int64_t n : shape) {
+    if (n >= 0 && t.size(i) != n) refuse(what, "wrong size");
+    ++i;
+  }
+  return p;
+}
+int32_t *ints(PyObject *o, std::initializer_list<int64_t> shape, const char *what) { return typed<int32_t>(o, at::kInt, shape, what); }
+float *floats(PyObject *o, std::initializer_list<int64_t> shape, const char *what) { return typed<float>(o, at::kFloat, shape, what); }
+
+uint32_t below_2_31(int64_t n, const char *what) {
+  if (n > 0x7fffffffll) refuse(what, "too large");
+  return static_cast<uint32_t>(n);
+}
+
+// A two-dimensional fp32 or bf16 tensor whose rows may lie apart (their elements together).
+struct Rows {
+  const void *data;
+  uint32_t rows, cols, bf16;
+  uint64_t stride;
+};
+Rows strided_rows(PyObject *o, const char *what) {
+  const at::Tensor &t = tensor(o);
+  if (!t.is_cuda()) refuse(what, "must live on a CUDA device (no CPU path)");
+  if (t.dim() != 2) refuse(what, "expected a two-dimensional tensor");
+  if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16) refuse(what, "expected float32 or bfloat16");
+  if (t.size(1) > 1 && t.stride(1) != 1) refuse(what, "the elements of a row must lie together");
+  if (t.size(0) > 1 && t.stride(0) < t.size(1)) refuse(what, "rows overlap");
+  return {t.data_ptr(), below_2_31(t.size(0), what), below_2_31(t.size(1), what), t.scalar_type() == at::kBFloat16 ? 1u : 0u,
+          static_cast<uint64_t>(t.size(0) > 1 ? t.stride(0) : t.size(1))};
+}
+
+struct Cache {
+  uint8_t *k, *v;
+  float *k_scale, *v_scale;
+  uint32_t pages, heads, page_size, d, format;
+};
+Cache cache(PyObject *k, PyObject *v, PyObject *k_scale, PyObject *v_scale) {
+  const at::Tensor &t = tensor(k);
+  const at::ScalarType type = t.scalar_type();
+  if (type != at::kChar && type != at::kFloat8_e4m3fn) refuse("k_cache", "expected int8 or float8_e4m3fn");
+  if (t.dim() != 4) refuse("k_cache", "expected [pages, kv_heads, page_size, d_head]");
+  Cache c;
+  c.k = typed<uint8_t>(k, type, {-1, -1, -1, -1}, "k_cache");
+  c.v = typed<uint8_t>(v, type, {t.size(0), t.size(1), t.size(2), t.size(3)}, "v_cache");
+  c.k_scale = floats(k_scale, {t.size(0), t.size(1)}, "k_scale");
+  c.v_scale = floats(v_scale, {t.size(0), t.size(1)}, "v_scale");
+  c.pages = below_2_31(t.size(0), "k_cache");
+  c.heads = below_2_31(t.size(1), "k_cache");
+  c.page_size = below_2_31(t.size(2), "k_cache");
+  c.d = below_2_31(t.size(3), "k_cache");
+  c.format = type == at::kChar ? DF_CACHE_INT8 : DF_CACHE_E4M3;
+  return c;
+}
+
+void given_or_ints(Out &out, PyObject *given, PyObject *model, std::initializer_list<int64_t> shape, const char *what) {
+  given_or_empty(out, given, model, shape, at::kInt);
+  ints(out.get(), shape, what);
+}
+void given_or_floats(Out &out, PyObject *given, PyObject *model, std::initializer_list<int64_t> shape, const char *what) {
+  given_or_empty(out, given, model, shape);
+  floats(out.get(), shape, what);
+}
+
+PyObject *cache_plan(Args a) {  // lens new_tokens block_table free_pages free_count page_size n_tokens lens_out starts slots positions state stream
+  int32_t *lens = ints(a[0], {-1}, "lens");
+  const int64_t n = tensor(a[0]).size(0), tokens = static_cast<int64_t>(whole(a[6]));
+  if (tokens < 0) refuse("n_tokens", "negative");
+  int32_t *new_tokens = ints(a[1], {n}, "new_tokens"), *table = ints(a[2], {n, -1}, "block_table");
+  int32_t *free_pages = ints(a[3], {-1}, "free_pages"), *free_count = ints(a[4], {1}, "free_count");
+  Out lens_out, starts, slots, positions, state;
+  given_or_ints(lens_out, a[7], a[0], {n}, "lens_out");
+  given_or_ints(starts, a[8], a[0], {n + 1}, "starts");
+  given_or_ints(slots, a[9], a[0], {tokens}, "slots");
+  given_or_ints(positions, a[10], a[0], {tokens}, "positions");
+  given_or_ints(state, a[11], a[0], {2}, "state");
+  call(fn.df_cache_plan, a[12], lens, new_tokens, table, free_pages, free_count, ptr<int32_t>(lens_out.get()), ptr<int32_t>(starts.get()),
+       ptr<int32_t>(slots.get()), ptr<int32_t>(positions.get()), ptr<int32_t>(state.get()), below_2_31(n, "lens"), below_2_31(tokens, "n_tokens"),
+       below_2_31(tensor(a[2]).size(1), "block_table"), u32(a[5]), below_2_31(tensor(a[3]).size(0), "free_pages"));
+  return tuple_of({&lens_out, &starts, &slots, &positions, &state});
+}
+
+PyObject *cache_release(Args a) {  // lens finished block_table free_pages free_count page_size lens_out count_out stream
+  int32_t *lens = ints(a[0], {-1}, "lens");
+  const int64_t n = tensor(a[0]).size(0);
+  int32_t *finished = ints(a[1], {n}, "finished"), *table = ints(a[2], {n, -1}, "block_table");
+  int32_t *free_pages = ints(a[3], {-1}, "free_pages"), *free_count = ints(a[4], {1}, "free_count");
+  Out lens_out, count_out;
+  given_or_ints(lens_out, a[6], a[0], {n}, "lens_out");
+  given_or_ints(count_out, a[7], a[0], {1}, "count_out");
+  call(fn.df_cache_release, a[8], lens, finished, table, free_pages, free_count, ptr<int32_t>(lens_out.get()), ptr<int32_t>(count_out.get()),
+       below_2_31(n, "lens"), below_2_31(tensor(a[2]).size(1), "block_table"), u32(a[5]), below_2_31(tensor(a[3]).size(0), "free_pages"));
+  return tuple_of({&lens_out, &count_out});
+}
+
+PyObject *cache_append(Args a) {  // k v slots k_cache v_cache k_scale v_scale stream
+  const Rows k = strided_rows(a[0], "k"), v = strided_rows(a[1], "v");
+  const Cache c = cache(a[3], a[4], a[5], a[6]);
+  if (static_cast<uint64_t>(k.cols) != static_cast<uint64_t>(c.heads) * c.d) refuse("k", "expected kv_heads * d_head columns");
+  if (v.rows != k.rows || v.cols != k.cols || v.bf16 != k.bf16) refuse("v", "shape or dtype differs from k");
+  int32_t *slots = ints(a[2], {k.rows}, "slots");
+  call(fn.df_cache_append, a[7], k.data, v.data, slots, static_cast<void *>(c.k), static_cast<void *>(c.v), c.k_scale, c.v_scale, k.rows, c.heads, c.d,
+       c.page_size, c.pages, k.stride, v.stride, k.bf16, c.format);
+  return PyTuple_Pack(4, a[3], a[4], a[5], a[6]);
+}
+
+PyObject *cache_attention(Args a) {  // q k_cache v_cache k_scale v_scale block_table lens starts n_heads scale workspace out lse stream
+  const Rows q = strided_rows(a[0], "q");
+  const Cache c = cache(a[1], a[2], a[3], a[4]);
+  int32_t *lens = ints(a[6], {-1}, "lens");
+  const int64_t n = tensor(a[6]).size(0);
+  int32_t *table = ints(a[5], {n, -1}, "block_table"), *starts = ints(a[7], {n + 1}, "starts");
+  const uint32_t heads = u32(a[8]);
+  if (static_cast<uint64_t>(q.cols) != static_cast<uint64_t>(heads) * c.d) refuse("q", "expected n_heads * d_head columns");
+  uint8_t *workspace = ptr<uint8_t>(a[10]);
+  Out out, lse;
+  const at::ScalarType type = q.bf16 ? at::kBFloat16 : at::kFloat;
+  given_or_empty(out, a[11], a[0], {static_cast<int64_t>(q.rows), static_cast<int64_t>(q.cols)}, type);
+  void *o = typed<void>(out.get(), type, {q.rows, q.cols}, "out");
+  given_or_floats(lse, a[12], a[0], {q.rows, heads}, "lse");
+  call(fn.df_cache_attention, a[13], q.data, static_cast<const void *>(c.k), static_cast<const void *>(c.v), c.k_scale, c.v_scale, table, lens, starts, o,
+       ptr(lse.get()), static_cast<void *>(workspace), static_cast<uint64_t>(tensor(a[10]).nbytes()), below_2_31(n, "lens"), q.rows, heads, c.heads, c.d,
+       c.page_size, c.pages, below_2_31(tensor(a[5]).size(1), "block_table"), q.stride, real(a[9]), q.bf16, c.format);
+  return tuple_of({&out, &lse});
+}
+
+PyObject *token_logprobs(Args a) {  // logits targets scale top_k logp entropy lse top_ids top_logp stream
+  const Rows z = strided_rows(a[0], "logits");
+  int32_t *targets = ints(a[1], {z.rows}, "targets");
+  const int64_t top = static_cast<int64_t>(whole(a[3]));
+  if (top < 0 || top > DF_LOGPROBS_MAX_TOP) refuse("top_k", "out of range");
+  Out logp, entropy, lse, ids, best;
+  given_or_floats(logp, a[4], a[0], {z.rows}, "logp");
+  given_or_floats(entropy, a[5], a[0], {z.rows}, "entropy");
+  given_or_floats(lse, a[6], a[0], {z.rows}, "lse");
+  given_or_ints(ids, a[7], a[0], {z.rows, top}, "top_ids");
+  given_or_floats(best, a[8], a[0], {z.rows, top}, "top_logp");
+  call(fn.df_token_logprobs, a[9], z.data, targets, ptr(logp.get()), ptr(entropy.get()), ptr(lse.get()), ptr<int32_t>(ids.get()), ptr(best.get()), z.rows, z.cols,
+       z.stride, static_cast<uint32_t>(top), real(a[2]), z.bf16);
+  return tuple_of({&logp, &entropy, &lse, &ids, &best});
+}
+
+PyObject *token_logprobs_backward(Args a) {  // logits targets lse entropy grad_logp grad_entropy scale d_logits stream
+  const Rows z = strided_rows(a[0], "logits");
+  int32_t *targets = ints(a[1], {z.rows}, "targets");
+  float *lse = floats(a[2], {z.rows}, "lse"), *entropy = floats(a[3], {z.rows}, "entropy");
+  float *g = a[4] == Py_None ? nullptr : floats(a[4], {z.rows}, "grad_logp"), *h = a[5] == Py_None ? nullptr : floats(a[5], {z.rows}, "grad_entropy");
+  Out d;
+  given_or_empty(d, a[7], a[0], {static_cast<int64_t>(z.rows), static_cast<int64_t>(z.cols)}, z.bf16 ? at::kBFloat16 : at::kFloat);
+  const Rows to = strided_rows(d.get(), "d_logits");
+  if (to.rows != z.rows || to.cols != z.cols || to.bf16 != z.bf16) refuse("d_logits", "shape or dtype differs from the logits");
+  call(fn.df_token_logprobs_backward, a[8], z.data, targets, lse, entropy, g, h, const_cast<void *>(to.data), z.rows, z.cols, z.stride, to.stride, real(a[6]),
+       z.bf16);
+  return d.release();
+}
+
 // ---------------------------------------------------------------- LayerNorm, GELU, AdamW
 PyObject *layernorm(Args a) {  // x gamma beta out means rstds stream
   const Shape2 x = shape2(a[0]);
@@ -494,6 +664,8 @@ PyMethodDef methods[] = {
     ENTRY(backward_block, 14), ENTRY(backward_block_bf16, 15), ENTRY(delta, 5), ENTRY(delta_bf16, 5), ENTRY(decode, 12),
     ENTRY(merge_partials, 6), ENTRY(accumulate, 3), ENTRY(linear_qkv, 11), ENTRY(linear, 6), ENTRY(linear_gelu, 7), ENTRY(chunked_logit_ce, 6),
     ENTRY(layernorm, 7), ENTRY(layernorm_backward, 9), ENTRY(gelu, 3), ENTRY(gelu_backward, 4), ENTRY(adamw_update, 12), ENTRY(adamw_step, 11),
+    ENTRY(cache_plan, 13), ENTRY(cache_release, 9), ENTRY(cache_append, 8), ENTRY(cache_attention, 14), ENTRY(token_logprobs, 10),
+    ENTRY(token_logprobs_backward, 9),
     ENTRY(context_forward, 9), ENTRY(context_backward, 13), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "df_python_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -185,6 +185,38 @@ extern "C" {
         logits: *mut f32, targets: *const u32, grad_logits: *mut f32, loss: *mut f32, chunk_rows: u32, cols: u32,
         total_rows: u32, stream: *mut c_void
     ) -> i32;
+    pub fn df_cache_plan(
+        lens: *const i32, new_tokens: *const i32, block_table: *mut i32, free_pages: *const i32, free_count:
+        *const i32, lens_out: *mut i32, starts: *mut i32, slots: *mut i32, positions: *mut i32, state: *mut i32,
+        n_requests: u32, n_tokens: u32, table_width: u32, page_size: u32, n_pages: u32, stream: *mut c_void
+    ) -> i32;
+    pub fn df_cache_release(
+        lens: *const i32, finished: *const i32, block_table: *const i32, free_pages: *mut i32, free_count:
+        *const i32, lens_out: *mut i32, count_out: *mut i32, n_requests: u32, table_width: u32, page_size: u32,
+        n_pages: u32, stream: *mut c_void
+    ) -> i32;
+    pub fn df_cache_append(
+        k: *const c_void, v: *const c_void, slots: *const i32, k_cache: *mut c_void, v_cache: *mut c_void,
+        k_scale: *mut f32, v_scale: *mut f32, n_tokens: u32, n_kv_heads: u32, d_head: u32, page_size: u32,
+        n_pages: u32, k_row_stride: u64, v_row_stride: u64, kv_bf16: u32, format: u32, stream: *mut c_void
+    ) -> i32;
+    pub fn df_cache_attention(
+        q: *const c_void, k_cache: *const c_void, v_cache: *const c_void, k_scale: *const f32, v_scale: *const
+        f32, block_table: *const i32, lens: *const i32, starts: *const i32, out: *mut c_void, lse: *mut f32,
+        workspace: *mut c_void, workspace_bytes: u64, n_requests: u32, n_tokens: u32, n_heads: u32, n_kv_heads:
+        u32, d_head: u32, page_size: u32, n_pages: u32, table_width: u32, q_row_stride: u64, scale: f32, q_bf16:
+        u32, format: u32, stream: *mut c_void
+    ) -> i32;
+    pub fn df_token_logprobs(
+        logits: *const c_void, targets: *const i32, logp: *mut f32, entropy: *mut f32, lse: *mut f32, top_ids:
+        *mut i32, top_logp: *mut f32, rows: u32, cols: u32, row_stride: u64, top_k: u32, scale: f32,
+        logits_bf16: u32, stream: *mut c_void
+    ) -> i32;
+    pub fn df_token_logprobs_backward(
+        logits: *const c_void, targets: *const i32, lse: *const f32, entropy: *const f32, grad_logp: *const f32,
+        grad_entropy: *const f32, d_logits: *mut c_void, rows: u32, cols: u32, row_stride: u64, d_row_stride:
+        u64, scale: f32, logits_bf16: u32, stream: *mut c_void
+    ) -> i32;
     pub fn launch_layernorm(
         x: *const f32, gamma: *const f32, beta: *const f32, out: *mut f32, means: *mut f32, rstds: *mut f32, batch: u32,
         features: u32

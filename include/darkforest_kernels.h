@@ -387,6 +387,74 @@ DF_API void launch_chunked_ce_eval(float *logits, const uint32_t *targets, float
 DF_API int df_chunked_logit_ce(float *logits, const uint32_t *targets, float *grad_logits, float *loss, uint32_t chunk_rows,
                         uint32_t cols, uint32_t total_rows, void *stream);
 
+/* ---- serving a batch of requests over a paged cache held in 8 bits (no counterpart in the reference, whose decode forms
+ * above read one sequence's fp32 or bf16 cache) ----
+ * Cache: k_cache, v_cache are codes [n_pages][n_kv_heads][page_size][d_head], one byte each, k_scale, v_scale [n_pages][n_kv_heads]
+ * fp32; an element is code * scale of its page and head. `format` DF_CACHE_INT8: the code is a signed byte; DF_CACHE_E4M3: an 8-bit float
+ * (1 sign, 4 exponent and 3 fraction bits, finite up to 448; the two codes 0x7f and 0xff, which df_cache_append never writes, read as +-480).
+ * Token t of request r lies in page block_table[r * table_width + t / page_size], row t % page_size; its slot is page * page_size + row.
+ * d_head is a multiple of 16 up to 128, page_size a multiple of 16 up to 256 (anything else: DF_ERR_UNSUPPORTED), n_pages * page_size below 2^31.
+ * Lengths, tables, slots and counts are read on the GPU: no call waits for them, so a captured graph replays with new ones.
+ *
+ *   df_cache_plan       One step's block tables, slot map and positions. Request r holds lens[r] tokens and brings new_tokens[r] >= 0 (negative
+ *       values count as 0). Pages that it needs beyond ceil(lens[r] / page_size) are taken in request order from the end of
+ *       free_pages[0 .. *free_count) and written into its row of block_table; earlier entries stay. lens_out[r] = lens[r] + new_tokens[r];
+ *       starts[n_requests + 1]: exclusive sums of new_tokens; slots, positions [n_tokens]: the new tokens' slots and places in their
+ *       sequences, request after request (-1 behind the last one). state[0]: free pages left, state[1]: 0. All or nothing: where the pages do not suffice
+ *       (state[1] = pages missing), or a request outgrows its table row or n_tokens (state[1] = -1 - r, the first such request), nothing is
+ *       granted: lens_out = lens, slots and positions -1, table and free pages as before. At most 16384 requests. lens_out must
+ *       not be lens. free_pages has n_pages entries.
+ *   df_cache_release    Requests with finished[r] != 0 give their ceil(lens[r] / page_size) pages back: they are appended to free_pages behind
+ *       *free_count, in order; lens_out[r] = 0, *count_out = the new count. The others keep their length. Outputs must not be inputs, free_pages aside.
+ *   df_cache_append     Rows k, v [n_tokens] of n_kv_heads * d_head elements (fp32, or bf16 with kv_bf16; row strides in elements) go to slots[n_tokens];
+ *       slots outside the cache (-1) are left out. The tokens of a page lie together and in order, and behind the rows that the page already has (as
+ *       df_cache_plan lays them out). The scale of a page and head is the smallest power of two, 2^-126 or above, that holds its
+ *       largest element (127 or 448 times the scale); it only grows while a page fills, and then the page's older codes are rounded once more,
+ *       so that a stored element is within one step of its scale of what was given, however the page was filled. All of it is
+ *       exact or rounded to nearest even. An infinity or NaN makes the scale NaN, and with it whatever attends to the page.
+ *   df_cache_attention  Rows of q [n_tokens][n_heads * d_head] (fp32, or bf16 with q_bf16; out alike), request after request as starts[n_requests + 1]
+ *       says, against the requests' cached tokens: with q_len = starts[r + 1] - starts[r], row j of request r sees its tokens 0 .. lens[r] - q_len + j
+ *       (its own is in the cache already). Query head h reads K/V head h / (n_heads / n_kv_heads). lse [n_tokens][n_heads]: natural logsumexp of the
+ *       scaled scores, may be NULL. Rows that see nothing: out = 0, lse = -inf. Rows outside every request are left as they are.
+ *       workspace: DF_CACHE_WORKSPACE_BYTES, 16-byte aligned, zeroed once by the caller; every call leaves it ready for the next.
+ *       Calls that can overlap need a workspace each. */
+#define DF_CACHE_INT8 0
+#define DF_CACHE_E4M3 1
+#define DF_CACHE_WORKSPACE_BYTES 33554432u
+DF_API int df_cache_plan(const int32_t *lens, const int32_t *new_tokens, int *block_table, const int32_t *free_pages,
+                  const int32_t *free_count, int *lens_out, int *starts, int *slots, int *positions, int *state,
+                  uint32_t n_requests, uint32_t n_tokens, uint32_t table_width, uint32_t page_size, uint32_t n_pages, void *stream);
+DF_API int df_cache_release(const int32_t *lens, const int32_t *finished, const int32_t *block_table, int *free_pages,
+                     const int32_t *free_count, int *lens_out, int *count_out, uint32_t n_requests, uint32_t table_width,
+                     uint32_t page_size, uint32_t n_pages, void *stream);
+DF_API int df_cache_append(const void *k, const void *v, const int32_t *slots, void *k_cache, void *v_cache, float *k_scale,
+                    float *v_scale, uint32_t n_tokens, uint32_t n_kv_heads, uint32_t d_head, uint32_t page_size,
+                    uint32_t n_pages, uint64_t k_row_stride, uint64_t v_row_stride, uint32_t kv_bf16, uint32_t format,
+                    void *stream);
+DF_API int df_cache_attention(const void *q, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale,
+                       const int32_t *block_table, const int32_t *lens, const int32_t *starts, void *out, float *lse,
+                       void *workspace, uint64_t workspace_bytes, uint32_t n_requests, uint32_t n_tokens, uint32_t n_heads,
+                       uint32_t n_kv_heads, uint32_t d_head, uint32_t page_size, uint32_t n_pages, uint32_t table_width,
+                       uint64_t q_row_stride, float scale, uint32_t q_bf16, uint32_t format, void *stream);
+
+/* ---- log probabilities of given tokens (no counterpart in the reference) ----
+ * logits [rows] of cols elements (fp32, or bf16 with logits_bf16; row stride in elements); z = scale * logits (scale > 0: one over the temperature).
+ *   df_token_logprobs   per row: lse = log sum exp z, logp = z[target] - lse, entropy = -sum p log p (nats), and the top_k (0 .. 32, at most cols)
+ *       largest columns, equal ones in the order of their index, with their log probabilities: top_ids, top_logp [rows][top_k]. A target outside
+ *       0 .. cols - 1 (a padded row) gives logp 0. -inf logits are columns that cannot come: they add nothing to lse and entropy and stand last. A row of
+ *       nothing else has lse -inf, entropy 0 and log probabilities of -inf; a NaN or +inf in a row makes its results NaN (NaN and +inf
+ *       stand first among the alternatives).
+ *   df_token_logprobs_backward   d_logits = scale * (grad_logp * (onehot(target) - p) - grad_entropy * p * (log p + entropy)), from lse and entropy as
+ *       above; grad_logp and grad_entropy [rows] may each be NULL. A row with a target outside the columns has no part of grad_logp. d_logits has
+ *       the logits' type and may be the logits themselves (with the same row stride). */
+#define DF_LOGPROBS_MAX_TOP 32
+DF_API int df_token_logprobs(const void *logits, const int32_t *targets, float *logp, float *entropy, float *lse, int *top_ids,
+                      float *top_logp, uint32_t rows, uint32_t cols, uint64_t row_stride, uint32_t top_k, float scale,
+                      uint32_t logits_bf16, void *stream);
+DF_API int df_token_logprobs_backward(const void *logits, const int32_t *targets, const float *lse, const float *entropy,
+                               const float *grad_logp, const float *grad_entropy, void *d_logits, uint32_t rows, uint32_t cols,
+                               uint64_t row_stride, uint64_t d_row_stride, float scale, uint32_t logits_bf16, void *stream);
+
 /* ---- variant selection and status ---- */
 #define DF_VARIANT_AUTO 0     /* tensor-core kernel where the shape allows (TF32 at d_head 64, full fp32 by bf16 parts at others), SIMT otherwise */
 #define DF_VARIANT_SIMT 1     /* force the shape-generic SIMT kernels                      */
