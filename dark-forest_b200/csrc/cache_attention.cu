@@ -3,9 +3,30 @@
 // For query row (token j of request r, head h), with kv = h / (n_heads / n_kv_heads) and last = lens[r] - q_len + j:
 //   s_t = scale * k_scale[page(t), kv] * (q . k_code_t),  t = 0 .. last        m = max s, l = sum exp(s_t - m)
 //   out = sum exp(s_t - m) / l * v_scale[page(t), kv] * v_code_t               lse = m + log l
-// One pass with a running maximum and sum per row.
+// One pass over the cache with a running maximum and sum per row; nothing but codes leaves HBM.
+//
+// What bounds it. With few query rows, HBM: a token of a head costs 2 d bytes and (rows) * 4 d operations. At 8 bits an SM gets 23 codes a cycle,
+// more than its fp32 lanes could widen and multiply one by one, so both products run on the tensor cores, on codes widened to half
+// precision in registers (every code is a half exactly). m16n8k16 instructions take it: their operand layouts leave the order of the contracted
+// index free, so that a lane reads whole 16-byte pieces of rows and no element is moved between lanes:
+//   scores   A = 16 rows of q, B = 8 tokens: lane (g, c) = (lane / 4, lane % 4) holds the dims c * DP/4 ... of token g; k-step kt is its word kt.
+//   output   A = weights, in the accumulators' own layout, B = 16 tokens x 8 dims: lane (g, c) holds the dims g * DP/8 ... of its four tokens;
+//            n-tile i is its byte i. The accumulators of lane (g, c) are then row g's dims c * DP/4 ..., like its part of q.
+// Precision. An fp32 query row, times a power of two that brings its largest element to 1 .. 2, enters as two halves (22 bits), and so do the
+// weights exp(s - m) * 2^15: the 16 rows of an instruction are then 8 rows and their second parts, and the two accumulators are added. A bf16 row
+// fits one half, its weights are rounded to 11 bits (the result has 8): 16 rows. The products of 16 tokens, which share one v_scale, are
+// added to the row's fp32 sums.
+//
+// Work. A CTA is one warp that loads (tensor-map copies of 16 tokens, 128-byte swizzle: the reads above are then free of bank conflicts at
+// head sizes 64 and 128) and four that compute, over a ring of stages of 64 tokens. A request with no more rows (query tokens times heads per K/V head)
+// than a warp takes is computed with its tokens dealt to the four warps; one with more has its rows dealt to them, and every warp goes over
+// all tokens. The whole step is one line of units (64 tokens of one head and row tile; four units where rows are dealt, which takes four times as
+// long); the grid's CTAs take equal parts of it, whatever the requests' lengths. A segment (request, row tile, head) that is cut leaves partial (m, l, out)
+// states in the workspace, and the CTA that finishes its last part adds them in their order. Every CTA forms the sums over the requests itself.
 #include <float.h>
 #include <math.h>
+
+#include <mutex>
 
 #include "cache_codes.cuh"
 #include "sm100_ptx.cuh"
@@ -13,89 +34,753 @@
 namespace df {
 namespace {
 
+using ptx::ex2_approx;
+
+constexpr uint32_t kStageTokens = 64, kStages = 4, kComputeWarps = 4, kThreads = 32 * (kComputeWarps + 1);
+constexpr float kWeightBits = 15.0f;  // weights are held times 2^15, so that halves reach down to 2^-39 of the largest one
+constexpr uint32_t kMaxGrid = 448;
+constexpr uint32_t kSplitUnits = 6;  // what cutting segments costs, in units
+constexpr uint32_t kCounterBytes = 4096;  // a counter per CTA, at the workspace's beginning
+
 struct AttendParams {
   const void *q;
-  const uint8_t *k, *v;
   const float *k_scale, *v_scale;
   const int32_t *table, *lens, *starts;
   void *out;
   float *lse;
+  unsigned int *counters;
+  float *partial;
+  unsigned int *status;
   unsigned long long q_stride;
-  uint32_t n_requests, n_tokens, heads, kv_heads, D, P, n_pages, width;
-  float scale;
+  uint32_t n_requests, n_tokens, heads, kv_heads, group, D, P, n_pages, width;
+  uint32_t q_aligned, out_aligned;  // 16-byte boundaries
+  float scale_log2;
 };
 
+// Rows that one warp takes, and the size of a partial state.
 template <bool BF16>
-__device__ __forceinline__ float load1(const void *base, size_t e) {
-  if (BF16) return __uint_as_float((uint32_t)__ldg(static_cast<const uint16_t *>(base) + e) << 16);
-  return __ldg(static_cast<const float *>(base) + e);
+constexpr uint32_t kRows = BF16 ? 16 : 8;
+template <bool BF16, int DP>
+constexpr uint32_t kPartialFloats = kComputeWarps * kRows<BF16> * (DP + 2);
+
+struct Request {
+  uint32_t first, rows, q_len, len, tiles, row_tiles, weight;
+};
+
+template <uint32_t ROWS>
+__device__ __forceinline__ Request request_of(const AttendParams &p, uint32_t r) {
+  Request q;
+  const long long most = (long long)p.width * p.P;
+  q.len = (uint32_t)min((long long)max(__ldg(p.lens + r), 0), most);
+  const int b = max(0, min(__ldg(p.starts + r), (int)p.n_tokens)), e = max(b, min(__ldg(p.starts + r + 1), (int)p.n_tokens));
+  q.first = (uint32_t)b;
+  q.q_len = (uint32_t)(e - b);
+  q.rows = q.q_len * p.group;
+  const bool wide = q.rows > ROWS;
+  q.row_tiles = q.rows == 0 ? 0u : wide ? (q.rows + kComputeWarps * ROWS - 1) / (kComputeWarps * ROWS) : 1u;
+  q.tiles = max(1u, (q.len + kStageTokens - 1) / kStageTokens);
+  q.weight = wide ? kComputeWarps : 1u;
+  return q;
+}
+
+// What a CTA does of one segment.
+struct Part {
+  Request rq;
+  uint32_t r, h, row0;           // K/V head; first row of the row tile
+  uint32_t t0, t1;               // stages [t0, t1)
+  uint32_t limit;                // tokens that the tile's last row sees
+  uint32_t parts, first_cta;     // of the whole segment
+};
+
+// The line of units (or, where no segment is cut, of segments) and this CTA's place on it.
+struct Line {
+  unsigned long long at, end, base;  // base: of request r
+  unsigned long long per_cta;
+  uint32_t r;
+  bool whole;  // counted in segments
+};
+
+template <uint32_t ROWS>
+__device__ __forceinline__ bool next_part(const AttendParams &p, Line &line, Part &part) {
+  while (line.at < line.end) {
+    Request q = request_of<ROWS>(p, line.r);
+    unsigned long long span = line.whole ? 1ull : (unsigned long long)q.tiles * q.weight;
+    while (line.at >= line.base + span * q.row_tiles * p.kv_heads) {  // on to the request that holds line.at (it is below the line's end)
+      line.base += span * q.row_tiles * p.kv_heads;
+      q = request_of<ROWS>(p, ++line.r);
+      span = line.whole ? 1ull : (unsigned long long)q.tiles * q.weight;
+    }
+    const uint32_t idx = (uint32_t)((line.at - line.base) / span);
+    const unsigned long long s0 = line.base + idx * span, s1 = s0 + span;
+    part.rq = q;
+    part.r = line.r;
+    part.h = idx % p.kv_heads;
+    part.row0 = idx / p.kv_heads * (kComputeWarps * ROWS);
+    part.parts = 1;
+    part.first_cta = blockIdx.x;
+    part.t0 = 0;
+    part.t1 = q.tiles;
+    if (line.whole) {
+      line.at = s1;
+    } else {
+      const unsigned long long stop = min(s1, line.end);
+      part.t0 = (uint32_t)((line.at - s0) / q.weight);
+      if (stop < s1) part.t1 = (uint32_t)((stop - s0) / q.weight);
+      // A boundary between CTAs counts down to whole stages; so the first CTA that a segment reaches may have none of it (a unit is a
+      // quarter of a stage where rows are dealt, and a CTA has at least four units), every other one has some.
+      uint32_t c0 = (uint32_t)(s0 / line.per_cta);
+      const uint32_t c1 = (uint32_t)((s1 - 1) / line.per_cta);
+      if (((c0 + 1ull) * line.per_cta - s0) / q.weight == 0) ++c0;
+      part.first_cta = c0;
+      part.parts = c1 - c0 + 1;
+      line.at = stop;
+      if (part.t1 <= part.t0) continue;
+    }
+    const uint32_t tile_rows = q.weight == 1 ? ROWS : kComputeWarps * ROWS;
+    const uint32_t last_row = min(q.rows, part.row0 + tile_rows) - 1;
+    const long long see = (long long)q.len - q.q_len + last_row / p.group + 1;
+    part.limit = (uint32_t)max(0ll, min(see, (long long)q.len));
+    part.t1 = max(part.t0, min(part.t1, (part.limit + kStageTokens - 1) / kStageTokens));
+    return true;
+  }
+  return false;
+}
+
+// ---------------------------------------------------------------- widening codes to pairs of halves
+// Bytes (0, 2) and (1, 3) of a word.
+template <int FORMAT>
+__device__ __forceinline__ void widen_alternate(uint32_t w, uint32_t &even, uint32_t &odd) {
+  if (FORMAT == DF_CACHE_INT8) {  // 1024 + (code + 128) is a half with the code in its last bits
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4240), b = __byte_perm(u, 0x64646464u, 0x4341);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), bias), y = __hsub2(*reinterpret_cast<__half2 *>(&b), bias);
+    even = *reinterpret_cast<const uint32_t *>(&x);
+    odd = *reinterpret_cast<const uint32_t *>(&y);
+  } else {  // times 2^-8 (cache_codes.cuh)
+    even = ((w << 7) & 0x3f803f80u) | ((w << 8) & 0x80008000u);
+    odd = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
+  }
+}
+// Byte i of two words each, for the four i: pair[i] = (a.byte i, b.byte i).
+template <int FORMAT>
+__device__ __forceinline__ void widen_pairs(uint32_t a, uint32_t b, uint32_t (&pair)[4]) {
+  if (FORMAT == DF_CACHE_INT8) {
+    const uint32_t lo = __byte_perm(a, b, 0x5140) ^ 0x80808080u, hi = __byte_perm(a, b, 0x7362) ^ 0x80808080u;  // a0 b0 a1 b1, a2 b2 a3 b3
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    pair[0] = __byte_perm(lo, 0x64646464u, 0x4140);
+    pair[1] = __byte_perm(lo, 0x64646464u, 0x4342);
+    pair[2] = __byte_perm(hi, 0x64646464u, 0x4140);
+    pair[3] = __byte_perm(hi, 0x64646464u, 0x4342);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&pair[i]), bias);
+      pair[i] = *reinterpret_cast<const uint32_t *>(&x);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t t = __byte_perm(a, b, (uint32_t)(i | (i << 4) | ((4 + i) << 8) | ((4 + i) << 12)));  // a.i a.i b.i b.i
+      pair[i] = ((t >> 1) & 0x3f803f80u) | (t & 0x80008000u);
+    }
+  }
+}
+
+__device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t halves(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// a pair of floats as halves and what they leave
+__device__ __forceinline__ void split_halves(float x, float y, uint32_t &first, uint32_t &second) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  first = *reinterpret_cast<const uint32_t *>(&h);
+  second = halves(x - f.x, y - f.y);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void load_row4(const void *q, unsigned long long e, bool aligned, float (&x)[4]) {
+  if (BF16) {
+    const uint16_t *p = static_cast<const uint16_t *>(q) + e;
+    uint32_t lo, hi;
+    if (aligned) {
+      const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
+      lo = w.x;
+      hi = w.y;
+    } else {
+      lo = __ldg(p) | ((uint32_t)__ldg(p + 1) << 16);
+      hi = __ldg(p + 2) | ((uint32_t)__ldg(p + 3) << 16);
+    }
+    x[0] = __uint_as_float(lo << 16);
+    x[1] = __uint_as_float(lo & 0xffff0000u);
+    x[2] = __uint_as_float(hi << 16);
+    x[3] = __uint_as_float(hi & 0xffff0000u);
+  } else {
+    const float *p = static_cast<const float *>(q) + e;
+    if (aligned) {
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __ldg(p + i);
+    }
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ void store_row4(void *out, size_t e, bool aligned, const float (&x)[4]) {
+  if (BF16) {
+    uint32_t w[2];
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[0]) : "f"(x[1]), "f"(x[0]));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[1]) : "f"(x[3]), "f"(x[2]));
+    uint16_t *p = static_cast<uint16_t *>(out) + e;
+    if (aligned) {
+      *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+    }
+  } else {
+    float *p = static_cast<float *>(out) + e;
+    if (aligned) {
+      *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = x[i];
+    }
+  }
+}
+
+// Sums (m, l, o[4]) states one after another.
+struct Running {
+  float m = -FLT_MAX, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  __device__ __forceinline__ void add(float m2, float l2, const float4 &o2) {
+    const float top = fmaxf(m, m2), a = ex2_approx(m - top), b = ex2_approx(m2 - top);
+    m = top;
+    l = l * a + l2 * b;
+    o[0] = o[0] * a + o2.x * b;
+    o[1] = o[1] * a + o2.y * b;
+    o[2] = o[2] * a + o2.z * b;
+    o[3] = o[3] * a + o2.w * b;
+  }
+};
+
+__device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // the compute warps; all of them come to each
+
+template <int DP>
+constexpr uint32_t kSubBytes = 16 * DP;  // a box of 16 tokens, or less where D < DP: whole swizzle periods
+template <int DP>
+constexpr uint32_t kRingBytes = kStages * 2 * (kStageTokens / 16) * kSubBytes<DP>;
+template <bool BF16, int DP>
+constexpr uint32_t kSmemBytes = 1024 + kRingBytes<DP> + kComputeWarps * kRows<BF16> * DP * 4;
+
+template <bool BF16, int FORMAT, int DP>
+__global__ void __launch_bounds__(kThreads, 2)
+k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttendParams p) {
+  constexpr uint32_t ROWS = kRows<BF16>;
+  constexpr int KT = DP / 16, NT = DP / 8, RW = BF16 ? 2 : 1;  // k-steps, n-tiles, rows of a lane
+  constexpr float kCodeScale = FORMAT == DF_CACHE_E4M3 ? 256.0f : 1.0f;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ float2 s_scale[kStages][kStageTokens / 16];  // k_scale, v_scale of a stage's boxes
+  __shared__ float s_m[kComputeWarps][ROWS], s_l[kComputeWarps][ROWS];
+  __shared__ uint64_t s_full[kStages], s_empty[kStages];
+  __shared__ unsigned long long s_sum[kThreads / 32][2], s_place[2];
+  __shared__ uint32_t s_most[kThreads / 32], s_request, s_last, s_abort;
+  const uint32_t t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const uint32_t ring = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  float *merge = reinterpret_cast<float *>(smem_raw + (ring - ptx::smem_u32(smem_raw)) + kRingBytes<DP>);  // [warp][row][DP]
+  if (t == 0) {
+    for (uint32_t s = 0; s < kStages; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&s_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&s_empty[s]), kComputeWarps);
+    }
+    ptx::mbar_init_fence();
+    s_abort = 0;
+    ptx::tma_prefetch_desc(&k_map);
+    ptx::tma_prefetch_desc(&v_map);
+  }
+  ptx::pdl_wait();
+
+  // ---- the line: sums over the requests, and the request at which this CTA begins
+  const uint32_t per = (p.n_requests + kThreads - 1) / kThreads, r0 = min(p.n_requests, t * per), r1 = min(p.n_requests, r0 + per);
+  unsigned long long units = 0, segments = 0;
+  uint32_t most = 0;
+  for (uint32_t r = r0; r < r1; ++r) {
+    const Request q = request_of<ROWS>(p, r);
+    const unsigned long long n = (unsigned long long)q.row_tiles * p.kv_heads;
+    segments += n;
+    units += n * q.tiles * q.weight;
+    if (n) most = max(most, q.tiles * q.weight);
+  }
+  unsigned long long in_units = units, in_segments = segments;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long a = __shfl_up_sync(0xffffffffu, in_units, o), b = __shfl_up_sync(0xffffffffu, in_segments, o);
+    if (lane >= (uint32_t)o) { in_units += a; in_segments += b; }
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 31) { s_sum[warp][0] = in_units; s_sum[warp][1] = in_segments; s_most[warp] = most; }
+  __syncthreads();
+  unsigned long long all_units = 0, all_segments = 0, my_units = 0, my_segments = 0;
+  for (uint32_t w = 0; w < kThreads / 32; ++w) {
+    if (w == warp) { my_units = all_units + in_units - units; my_segments = all_segments + in_segments - segments; }
+    all_units += s_sum[w][0];
+    all_segments += s_sum[w][1];
+    most = max(most, s_most[w]);
+  }
+  Line line;
+  const unsigned long long G = gridDim.x, seg_per = (all_segments + G - 1) / G, unit_per = max(8ull, (all_units + G - 1) / G);
+  line.whole = seg_per * most <= unit_per + kSplitUnits;
+  line.per_cta = line.whole ? seg_per : unit_per;
+  const unsigned long long total = line.whole ? all_segments : all_units;
+  line.at = line.per_cta * blockIdx.x;
+  line.end = min(total, line.at + line.per_cta);
+  if (line.at >= line.end) return;  // (the whole CTA)
+  unsigned long long base = line.whole ? my_segments : my_units;
+  const unsigned long long mine = line.whole ? segments : units;
+  if (line.at >= base && line.at < base + mine) {
+    for (uint32_t r = r0; r < r1; ++r) {
+      const Request q = request_of<ROWS>(p, r);
+      const unsigned long long n = (unsigned long long)q.row_tiles * p.kv_heads * (line.whole ? 1u : q.tiles * q.weight);
+      if (line.at < base + n) {
+        s_request = r;
+        s_place[0] = base;
+        break;
+      }
+      base += n;
+    }
+  }
+  __syncthreads();
+  line.r = s_request;
+  line.base = s_place[0];
+
+  const uint32_t a_full = ptx::smem_u32(&s_full[0]), a_empty = ptx::smem_u32(&s_empty[0]);
+  const uint32_t chunks = p.D / 16;  // 16-byte pieces of a row
+  Part part;
+  uint32_t stage = 0;  // stages so far, this CTA
+  if (warp == kComputeWarps) {
+    // ---------------------------------------------------------------- the loading warp
+    // Eight stages at a time: lane i looks up the page and scales of box i % 4 of stage i / 4 of the group.
+    const uint32_t box_bytes = 16 * p.D;
+    while (next_part<ROWS>(p, line, part)) {
+      const int32_t *row = p.table + (size_t)part.r * p.width;
+      for (uint32_t g = part.t0; g < part.t1; g += 8) {
+        const uint32_t token = (g + lane / 4) * kStageTokens + lane % 4 * 16;
+        const bool in = token < part.limit && g + lane / 4 < part.t1;
+        uint32_t slice = p.n_pages * p.kv_heads, line0 = 0;  // behind the last slice: zeros
+        float2 scale = make_float2(0.0f, 0.0f);
+        if (in) {
+          const uint32_t page = (uint32_t)__ldg(row + token / p.P);
+          if (page < p.n_pages) {
+            slice = page * p.kv_heads + part.h;
+            scale = make_float2(__ldg(p.k_scale + slice), __ldg(p.v_scale + slice));
+          }
+          line0 = token % p.P * p.D / 128;
+        }
+        const uint32_t ballot = __ballot_sync(0xffffffffu, in);
+        for (uint32_t s = 0; s < min(8u, part.t1 - g); ++s, ++stage) {
+          const uint32_t slot = stage % kStages;
+          if (stage >= kStages && !ptx::mbar_wait_warp(a_empty + 8 * slot, (stage / kStages - 1) & 1, &s_abort)) {
+            if (lane == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
+            goto loaded;
+          }
+          const bool mine_now = lane / 4 == s;
+          if (mine_now) s_scale[slot][lane % 4] = scale;
+          __syncwarp();
+          const uint32_t boxes = __popc((ballot >> (4 * s)) & 15u);
+          if (lane == 0) ptx::mbar_arrive_expect_tx(a_full + 8 * slot, 2 * boxes * box_bytes);
+          __syncwarp();
+          if (mine_now && in) {
+            const uint32_t dst = ring + (slot * 2 * 4 + lane % 4) * kSubBytes<DP>;
+            ptx::tma_load_3d(dst, &k_map, a_full + 8 * slot, 0, (int)line0, (int)slice);
+            ptx::tma_load_3d(dst + 4 * kSubBytes<DP>, &v_map, a_full + 8 * slot, 0, (int)line0, (int)slice);
+          }
+        }
+      }
+    }
+  loaded:
+    if (s_abort) {  // copies in flight write to this CTA's shared memory: none may be left when it goes
+      for (uint32_t s = stage > kStages ? stage - kStages : 0; s < stage; ++s)
+        for (uint32_t polls = 0; polls < (1u << 16) && !ptx::mbar_try_wait(a_full + 8 * (s % kStages), (s / kStages) & 1); ++polls) {
+        }
+    }
+    return;
+  }
+
+  // ---------------------------------------------------------------- the computing warps
+  const uint32_t g = lane >> 2, c = lane & 3;
+  bool ok = true;
+  while (next_part<ROWS>(p, line, part)) {
+    const bool wide = part.rq.weight != 1;
+    const uint32_t warp_row = part.row0 + (wide ? warp * ROWS : 0);
+    // rows of this lane
+    uint32_t see[RW], a[KT][4];
+    bool valid[RW];
+    float norm[RW], m[RW], l[RW], o[RW][NT * 2];
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+      const uint32_t row = warp_row + g + 8 * i;
+      valid[i] = row < part.rq.rows;
+      const uint32_t j = row / p.group, head = part.h * p.group + row % p.group;
+      const long long n = (long long)part.rq.len - part.rq.q_len + j + 1;
+      see[i] = valid[i] ? (uint32_t)max(0ll, min(n, (long long)part.rq.len)) : 0u;
+      const unsigned long long e = (unsigned long long)(part.rq.first + j) * p.q_stride + (unsigned long long)head * p.D + c * (DP / 4);
+      float x[KT][4];
+      float top = 0.0f;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        if (valid[i] && c * (DP / 4) + kt * 4 < p.D) {
+          load_row4<BF16>(p.q, e + kt * 4, p.q_aligned, x[kt]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[kt][k] = 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = fmaxf(top, fabsf(x[kt][k]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the largest element to 1 .. 2 (an infinity or zero stays)
+      const uint32_t exponent = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+      const bool keep = top == 0.0f || top == INFINITY;
+      const float down = keep ? 1.0f : __uint_as_float((254u - exponent) << 23);
+      norm[i] = (keep ? 1.0f : __uint_as_float(exponent << 23)) * (kCodeScale * p.scale_log2);  // the scale after the product: q itself fits its halves
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        if (BF16) {
+          a[kt][i] = halves(x[kt][0] * down, x[kt][2] * down);
+          a[kt][2 + i] = halves(x[kt][1] * down, x[kt][3] * down);
+        } else {
+          split_halves(x[kt][0] * down, x[kt][2] * down, a[kt][0], a[kt][1]);
+          split_halves(x[kt][1] * down, x[kt][3] * down, a[kt][2], a[kt][3]);
+        }
+      }
+      m[i] = -FLT_MAX;
+      l[i] = 0.0f;
+#pragma unroll
+      for (int n2 = 0; n2 < NT * 2; ++n2) o[i][n2] = 0.0f;
+    }
+    // what the warp's rows see, at least and at most: rows are in the order of their tokens
+    const uint32_t last_row = min(part.rq.rows, warp_row + ROWS) - 1;
+    const long long lo = (long long)part.rq.len - part.rq.q_len + warp_row / p.group + 1, hi = (long long)part.rq.len - part.rq.q_len + last_row / p.group + 1;
+    const uint32_t see_all = (uint32_t)max(0ll, min(lo, (long long)part.rq.len));
+    const uint32_t see_any = warp_row < part.rq.rows ? (uint32_t)max(0ll, min(hi, (long long)part.rq.len)) : 0u;
+
+    for (uint32_t tile = part.t0; tile < part.t1; ++tile, ++stage) {
+      const uint32_t slot = stage % kStages;
+      if (ok) ok = ptx::mbar_wait_warp(a_full + 8 * slot, (stage / kStages) & 1, &s_abort);
+      const uint32_t stage_at = ring + slot * 2 * 4 * kSubBytes<DP>;
+      for (uint32_t sub = wide ? 0 : warp; ok && sub < (wide ? 4u : warp + 1); ++sub) {
+        const uint32_t token0 = tile * kStageTokens + sub * 16;
+        if (token0 >= see_any) break;
+        const float2 scale = s_scale[slot][sub];
+        const uint32_t k_at = stage_at + sub * kSubBytes<DP>, v_at = k_at + 4 * kSubBytes<DP>;
+        // Tokens of a lane's accumulators: tile j, columns 2c and 2c + 1. With 64-byte rows the order below keeps two rows of a 128-byte
+        // line together, which the swizzle then spreads over all banks.
+        auto token_of = [&](uint32_t j, uint32_t col) { return DP == 128 ? 8 * j + col : 4 * (col >> 1) + 2 * j + (col & 1); };
+        auto piece = [&](uint32_t at, uint32_t token, uint32_t chunk) {  // address of a 16-byte piece
+          const uint32_t x = token * chunks + chunk;
+          return at + ((x * 16) ^ ((x & 0x38u) << 1));
+        };
+        // ---- scores
+        float acc[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t w[KT];
+          const uint32_t token = token_of(j, g);
+#pragma unroll
+          for (int k4 = 0; k4 < KT / 4; ++k4) {
+            const uint32_t chunk = c * (KT / 4) + k4;
+            if (chunk < chunks) {
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(w[4 * k4]), "=r"(w[4 * k4 + 1]), "=r"(w[4 * k4 + 2]), "=r"(w[4 * k4 + 3])
+                           : "r"(piece(k_at, token, chunk)));
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[4 * k4 + k] = 0u;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[j][k] = 0.0f;
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            uint32_t b0, b1;
+            widen_alternate<FORMAT>(w[kt], b0, b1);
+            mma_half(acc[j], a[kt], b0, b1);
+          }
+        }
+        // ---- weights
+        const bool masked = token0 + 16 > see_all;
+        uint32_t pa[4];
+        float v_row[RW];
+        bool grew = false;
+        float before[RW];
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+          const float f = scale.x * norm[i];
+          float s[2][2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              s[j][k] = (BF16 ? acc[j][2 * i + k] : acc[j][k] + acc[j][2 + k]) * f;
+              if (masked && token0 + token_of(j, 2 * c + k) >= see[i]) s[j][k] = -INFINITY;
+            }
+          float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          before[i] = m[i];
+          grew |= top > m[i];
+          m[i] = fmaxf(m[i], top);
+          const float shift = m[i] - kWeightBits;
+          float w[2][2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) w[j][k] = ex2_approx(s[j][k] - shift);
+          if (before[i] != m[i]) l[i] *= ex2_approx(before[i] - m[i]);
+          l[i] += (w[0][0] + w[0][1]) + (w[1][0] + w[1][1]);
+          if (BF16) {
+            pa[i] = halves(w[0][0], w[0][1]);
+            pa[2 + i] = halves(w[1][0], w[1][1]);
+          } else {
+            split_halves(w[0][0], w[0][1], pa[0], pa[1]);
+            split_halves(w[1][0], w[1][1], pa[2], pa[3]);
+          }
+          // a row that sees none of these tokens takes nothing of them, whatever their scale is (it may be NaN)
+          v_row[i] = token0 < see[i] ? scale.y : 0.0f;
+        }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+          for (int i = 0; i < RW; ++i) {
+            const float f = ex2_approx(before[i] - m[i]);
+#pragma unroll
+            for (int n = 0; n < NT * 2; ++n) o[i][n] *= f;
+          }
+        }
+        // ---- output
+        uint32_t w[4][NT / 4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t token = token_of(k >> 1, 2 * c + (k & 1));
+          if constexpr (DP == 128) {
+            if (g < chunks) {
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(w[k][0]), "=r"(w[k][1]), "=r"(w[k][2]), "=r"(w[k][3])
+                           : "r"(piece(v_at, token, g)));
+            } else {
+              w[k][0] = w[k][1] = w[k][2] = w[k][3] = 0u;
+            }
+          } else {
+            if ((g >> 1) < chunks) {
+              asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[k][0]), "=r"(w[k][1]) : "r"(piece(v_at, token, g >> 1) + 8 * (g & 1)));
+            } else {
+              w[k][0] = w[k][1] = 0u;
+            }
+          }
+        }
+#pragma unroll
+        for (int n4 = 0; n4 < NT / 4; ++n4) {
+          uint32_t b0[4], b1[4];
+          widen_pairs<FORMAT>(w[0][n4], w[1][n4], b0);
+          widen_pairs<FORMAT>(w[2][n4], w[3][n4], b1);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma_half(d, pa, b0[k], b1[k]);
+            const int n = n4 * 4 + k;  // columns 2c, 2c + 1: dims 2c * DP/8 + n and (2c + 1) * DP/8 + n
+            if (BF16) {
+#pragma unroll
+              for (int i = 0; i < RW; ++i) {
+                o[i][n] = fmaf(v_row[i], d[2 * i], o[i][n]);
+                o[i][NT + n] = fmaf(v_row[i], d[2 * i + 1], o[i][NT + n]);
+              }
+            } else {
+              o[0][n] = fmaf(v_row[0], d[0] + d[2], o[0][n]);
+              o[0][NT + n] = fmaf(v_row[0], d[1] + d[3], o[0][NT + n]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(a_empty + 8 * slot);
+    }
+    if (!ok && lane == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+#pragma unroll
+      for (int n = 0; n < NT * 2; ++n) o[i][n] *= kCodeScale;
+    }
+
+    // ---- the result, or this part of it: o[i][0 .. DP/4) are row i's dims c * DP/4 ...
+    const bool split = part.parts > 1;
+    const uint32_t rows = wide ? min(part.rq.rows - part.row0, kComputeWarps * ROWS) : part.rq.rows;
+    auto state_of = [&](uint32_t cta) {  // the first CTA of a segment has it last, every other one first
+      return p.partial + (size_t)(2 * cta + (cta == part.first_cta ? 1 : 0)) * kPartialFloats<BF16, DP>;
+    };
+    auto finish_row = [&](size_t row, uint32_t dim, const float (&x)[4], float mm, float ll) {  // four dims of a finished row
+      const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+      const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+      if (dim < p.D) store_row4<BF16>(p.out, row * p.D + dim, p.out_aligned, y);
+      if (dim == 0 && p.lse) p.lse[row] = ll == 0.0f ? -INFINITY : (mm - kWeightBits + log2f(ll)) * kLn2;
+    };
+    auto global_row = [&](uint32_t row) {
+      const uint32_t rr = part.row0 + row;
+      return (size_t)(part.rq.first + rr / p.group) * p.heads + part.h * p.group + rr % p.group;
+    };
+    float *mine_state = state_of(blockIdx.x), *mine_o = mine_state + 2 * kComputeWarps * ROWS;
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < RW; ++i) {
+        const uint32_t row = warp * ROWS + g + 8 * i;
+#pragma unroll
+        for (int n = 0; n < DP / 4; n += 4) {
+          const float x[4] = {o[i][n], o[i][n + 1], o[i][n + 2], o[i][n + 3]};
+          const uint32_t dim = c * (DP / 4) + n;
+          if (!split && valid[i]) finish_row(global_row(row), dim, x, m[i], l[i]);
+          if (split && valid[i]) *reinterpret_cast<float4 *>(mine_o + row * DP + dim) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+        if (split && valid[i] && c == 0) *reinterpret_cast<float2 *>(mine_state + 2 * row) = make_float2(m[i], l[i]);
+      }
+    } else {
+      // the four warps' states of the same rows
+#pragma unroll
+      for (int i = 0; i < RW; ++i) {
+        const uint32_t row = g + 8 * i;
+        if (valid[i]) {
+          if (c == 0) { s_m[warp][row] = m[i]; s_l[warp][row] = l[i]; }
+#pragma unroll
+          for (int n = 0; n < DP / 4; n += 4)
+            *reinterpret_cast<float4 *>(merge + (warp * ROWS + row) * DP + c * (DP / 4) + n) = make_float4(o[i][n], o[i][n + 1], o[i][n + 2], o[i][n + 3]);
+        }
+      }
+      compute_barrier();
+      for (uint32_t e = t; e < rows * (DP / 4); e += 32 * kComputeWarps) {
+        const uint32_t row = e / (DP / 4), dim = e % (DP / 4) * 4;
+        Running sum;
+#pragma unroll
+        for (uint32_t w = 0; w < kComputeWarps; ++w)
+          sum.add(s_m[w][row], s_l[w][row], *reinterpret_cast<const float4 *>(merge + (w * ROWS + row) * DP + dim));
+        if (!split) {
+          finish_row(global_row(row), dim, sum.o, sum.m, sum.l);
+        } else {
+          *reinterpret_cast<float4 *>(mine_o + row * DP + dim) = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
+          if (dim == 0) *reinterpret_cast<float2 *>(mine_state + 2 * row) = make_float2(sum.m, sum.l);
+        }
+      }
+    }
+    if (split) {
+      __threadfence();
+      compute_barrier();
+      if (t == 0) {
+        s_last = atomicAdd(p.counters + part.first_cta, 1u) + 1 == part.parts;
+        if (s_last) p.counters[part.first_cta] = 0;  // ready for the next call
+        __threadfence();
+      }
+      compute_barrier();
+      if (s_last) {
+        __threadfence();
+        const uint32_t elements = rows * (DP / 4), ways = max(1u, 32 * kComputeWarps / elements);
+        // thread: four dims of a row, and every `ways`-th part where there are fewer of them than threads
+        const uint32_t e0 = ways > 1 ? t % elements : t, way = ways > 1 ? t / elements : 0;
+        for (uint32_t e = e0; e < elements && way < ways; e += 32 * kComputeWarps) {
+          const uint32_t row = e / (DP / 4), dim = e % (DP / 4) * 4;
+          Running sum;
+#pragma unroll 4
+          for (uint32_t i = way; i < part.parts; i += ways) {
+            const float *state = state_of(part.first_cta + i);
+            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(state + 2 * row));
+            sum.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4 *>(state + 2 * kComputeWarps * ROWS + row * DP + dim)));
+          }
+          if (ways == 1) {
+            finish_row(global_row(row), dim, sum.o, sum.m, sum.l);
+          } else {  // elements * ways <= 128 threads, six floats each
+            float *at = merge + (way * elements + e) * 8;
+            *reinterpret_cast<float4 *>(at) = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
+            at[4] = sum.m;
+            at[5] = sum.l;
+          }
+        }
+        if (ways > 1) {
+          compute_barrier();
+          if (t < elements) {
+            Running sum;
+            for (uint32_t w = 0; w < ways; ++w) {
+              const float *at = merge + (w * elements + t) * 8;
+              sum.add(at[4], at[5], *reinterpret_cast<const float4 *>(at));
+            }
+            finish_row(global_row(t / (DP / 4)), t % (DP / 4) * 4, sum.o, sum.m, sum.l);
+          }
+        }
+      }
+    }
+    compute_barrier();  // the merge buffer and s_last are free again
+  }
+}
+
+struct DeviceInfo {
+  std::once_flag once;
+  uint32_t grid = 0;
+};
+
+// CTAs that the device keeps resident, asked once per kernel and device.
+template <bool BF16, int FORMAT, int DP>
+uint32_t resident_ctas() {
+  static DeviceInfo table[64];
+  int dev = 0;
+  if (check_cuda(cudaGetDevice(&dev)) != DF_OK || dev < 0 || dev >= 64) return 0;
+  DeviceInfo &d = table[dev];
+  std::call_once(d.once, [&]() {
+    auto kernel = k_cache_attention<BF16, FORMAT, DP>;
+    int per_sm = 0, n_sm = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes<BF16, DP>) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, (int)kThreads, kSmemBytes<BF16, DP>) != cudaSuccess ||
+        cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return;
+    d.grid = (uint32_t)(per_sm * n_sm);
+  });
+  return d.grid;
+}
+
+// The pool as lines of 128 bytes: a slice (page, head) is P * D / 128 of them, 16 tokens D / 8.
+bool encode_pool_map(CUtensorMap *map, const void *pool, const AttendParams &p) {
+  PFN_encodeTiled encode = get_encode_tiled();
+  if (!encode) return false;
+  const cuuint64_t lines = (cuuint64_t)p.P * p.D / 128;
+  const cuuint64_t dims[3] = {128, lines, (cuuint64_t)p.n_pages * p.kv_heads};
+  const cuuint64_t strides[2] = {128, lines * 128};
+  const cuuint32_t box[3] = {128, p.D / 8, 1}, step[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool BF16, int FORMAT, int DP>
+int launch(AttendParams &p, const void *k_cache, const void *v_cache, cudaStream_t s) {
+  constexpr uint32_t kFits = (DF_CACHE_WORKSPACE_BYTES - kCounterBytes) / (2 * kPartialFloats<BF16, DP> * 4);
+  static_assert(kFits >= 2 * 148 && kMaxGrid * 4 <= kCounterBytes, "workspace");
+  uint32_t grid = resident_ctas<BF16, FORMAT, DP>();
+  if (grid == 0) return DF_ERR_CUDA;
+  grid = grid < kFits ? grid : kFits;
+  grid = grid < kMaxGrid ? grid : kMaxGrid;
+  CUtensorMap k_map, v_map;
+  if (!encode_pool_map(&k_map, k_cache, p) || !encode_pool_map(&v_map, v_cache, p)) return DF_ERR_CUDA;
+  const int st = check_cuda(launch_kernel(k_cache_attention<BF16, FORMAT, DP>, dim3(grid), dim3(kThreads), kSmemBytes<BF16, DP>, s, k_map, v_map, p));
+  note_launch();
+  return st;
 }
 
 template <bool BF16, int FORMAT>
-__global__ void __launch_bounds__(128) k_cache_attention(const AttendParams p) {
-  ptx::pdl_wait();
-  __shared__ float sm_m[4], sm_l[4], sm_o[4][128];
-  const uint32_t token = blockIdx.x, h = blockIdx.y, kv = h / (p.heads / p.kv_heads);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint32_t r = 0;
-  for (; r < p.n_requests; ++r)
-    if ((int)token >= __ldg(p.starts + r) && (int)token < __ldg(p.starts + r + 1)) break;
-  if (r == p.n_requests) return;
-  const long long len = min((long long)max(__ldg(p.lens + r), 0), (long long)p.width * p.P);
-  const long long see = len - __ldg(p.starts + r + 1) + (long long)token + 1;  // keys that the row sees
-  float q[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -FLT_MAX, l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t d = lane + 32 * i;
-    q[i] = d < p.D ? load1<BF16>(p.q, (size_t)token * p.q_stride + (size_t)h * p.D + d) * (p.scale * kLog2e) : 0.0f;
-  }
-  for (long long t = warp; t < see; t += 4) {
-    const uint32_t page = (uint32_t)__ldg(p.table + (size_t)r * p.width + t / p.P);
-    const bool in = page < p.n_pages;
-    const size_t slice = (size_t)(in ? page : 0) * p.kv_heads + kv, at = (slice * p.P + t % p.P) * p.D;
-    float dot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t d = lane + 32 * i;
-      if (d < p.D && in) dot = fmaf(q[i], cache_value<FORMAT>(__ldg(p.k + at + d)), dot);
-    }
-#pragma unroll
-    for (int o2 = 16; o2 > 0; o2 >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o2);
-    const float s = dot * (in ? __ldg(p.k_scale + slice) : 0.0f);
-    const float top = fmaxf(m, s), alpha = exp2f(m - top), e = exp2f(s - top);
-    const float w = e * (in ? __ldg(p.v_scale + slice) : 0.0f);
-    m = top;
-    l = fmaf(l, alpha, e);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t d = lane + 32 * i;
-      if (d < p.D) o[i] = fmaf(w, in ? cache_value<FORMAT>(__ldg(p.v + at + d)) : 0.0f, o[i] * alpha);
-    }
-  }
-  if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) sm_o[warp][lane + 32 * i] = o[i];
-  __syncthreads();
-  const uint32_t d = threadIdx.x;
-  float M = -FLT_MAX, L = 0.0f, O = 0.0f;
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w]);
-  for (int w = 0; w < 4; ++w) {
-    const float f = exp2f(sm_m[w] - M);
-    L = fmaf(sm_l[w], f, L);
-    O = fmaf(sm_o[w][d], f, O);
-  }
-  if (d < p.D) {
-    const float x = L == 0.0f ? 0.0f : O / L;
-    const size_t e = ((size_t)token * p.heads + h) * p.D + d;
-    if (BF16) {
-      uint16_t b;
-      asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(b) : "f"(x));
-      static_cast<uint16_t *>(p.out)[e] = b;
-    } else {
-      static_cast<float *>(p.out)[e] = x;
-    }
-  }
-  if (d == 0 && p.lse) p.lse[(size_t)token * p.heads + h] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
+int launch_for_head(AttendParams &p, const void *k_cache, const void *v_cache, cudaStream_t s) {
+  return p.D <= 64 ? launch<BF16, FORMAT, 64>(p, k_cache, v_cache, s) : launch<BF16, FORMAT, 128>(p, k_cache, v_cache, s);
 }
 
 int finish(int st) {
@@ -114,22 +799,44 @@ extern "C" int df_cache_attention(const void *q, const void *k_cache, const void
                                   uint32_t d_head, uint32_t page_size, uint32_t n_pages, uint32_t table_width, uint64_t q_row_stride, float scale,
                                   uint32_t q_bf16, uint32_t format, void *stream) {
   DF_RANGE("df_cache_attention");
-  if (!cache_shape_valid(n_kv_heads, d_head, page_size, n_pages) || n_tokens >= (1u << 31) || n_requests >= (1u << 31)) return finish(DF_ERR_INVALID_ARG);
+  if (!cache_shape_valid(n_kv_heads, d_head, page_size, n_pages) || n_requests >= (1u << 31)) return finish(DF_ERR_INVALID_ARG);
   if (format != DF_CACHE_INT8 && format != DF_CACHE_E4M3) return finish(DF_ERR_INVALID_ARG);
-  if (n_heads == 0 || n_heads % n_kv_heads != 0 || n_heads > 65535u || !isfinite(scale)) return finish(DF_ERR_INVALID_ARG);
+  if (n_heads == 0 || n_heads % n_kv_heads != 0 || !isfinite(scale) || (uint64_t)n_tokens * n_heads >= (1ull << 31)) return finish(DF_ERR_INVALID_ARG);
   if (n_tokens > 1 && q_row_stride < (uint64_t)n_heads * d_head) return finish(DF_ERR_INVALID_ARG);
   if (!cache_shape_supported(d_head, page_size)) return finish(DF_ERR_UNSUPPORTED);
   if (n_tokens == 0 || n_requests == 0) return DF_OK;
-  if (!q || !lens || !starts || !out || (n_pages && (!k_cache || !v_cache || !k_scale || !v_scale)) || (table_width && !block_table))
+  if (!q || !lens || !starts || !out || n_pages == 0 || !k_cache || !v_cache || !k_scale || !v_scale || (table_width && !block_table))
     return finish(DF_ERR_INVALID_ARG);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return finish(DF_ERR_INVALID_ARG);
   if (workspace_bytes < DF_CACHE_WORKSPACE_BYTES) return finish(DF_ERR_WORKSPACE);
   if (((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15u) != 0) return finish(DF_ERR_UNSUPPORTED);
-  const AttendParams p = {q, static_cast<const uint8_t *>(k_cache), static_cast<const uint8_t *>(v_cache), k_scale, v_scale, block_table, lens, starts, out, lse,
-                          q_row_stride, n_requests, n_tokens, n_heads, n_kv_heads, d_head, page_size, n_pages, table_width, scale};
-  auto kernel = q_bf16 ? (format == DF_CACHE_INT8 ? k_cache_attention<true, DF_CACHE_INT8> : k_cache_attention<true, DF_CACHE_E4M3>)
-                       : (format == DF_CACHE_INT8 ? k_cache_attention<false, DF_CACHE_INT8> : k_cache_attention<false, DF_CACHE_E4M3>);
-  const int st = check_cuda(launch_kernel(kernel, dim3(n_tokens, n_heads), dim3(128), 0, static_cast<cudaStream_t>(stream), p));
-  note_launch();
-  return finish(st);
+  AttendParams p = {};
+  p.q = q;
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.table = block_table;
+  p.lens = lens;
+  p.starts = starts;
+  p.out = out;
+  p.lse = lse;
+  p.counters = static_cast<unsigned int *>(workspace);
+  p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kCounterBytes);
+  p.status = device_status_ptr();
+  p.q_stride = q_row_stride;
+  p.n_requests = n_requests;
+  p.n_tokens = n_tokens;
+  p.heads = n_heads;
+  p.kv_heads = n_kv_heads;
+  p.group = n_heads / n_kv_heads;
+  p.D = d_head;
+  p.P = page_size;
+  p.n_pages = n_pages;
+  p.width = table_width;
+  p.q_aligned = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(q_row_stride * (q_bf16 ? 2 : 4))) & 15u) == 0;
+  p.out_aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  p.scale_log2 = scale * kLog2e;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (q_bf16)
+    return finish(format == DF_CACHE_INT8 ? launch_for_head<true, DF_CACHE_INT8>(p, k_cache, v_cache, s) : launch_for_head<true, DF_CACHE_E4M3>(p, k_cache, v_cache, s));
+  return finish(format == DF_CACHE_INT8 ? launch_for_head<false, DF_CACHE_INT8>(p, k_cache, v_cache, s) : launch_for_head<false, DF_CACHE_E4M3>(p, k_cache, v_cache, s));
 }
