@@ -36,7 +36,7 @@ namespace {
 
 using ptx::ex2_approx;
 
-constexpr uint32_t kStageTokens = 64, kStages = 4, kComputeWarps = 4, kThreads = 32 * (kComputeWarps + 1);
+constexpr uint32_t kStageTokens = 64, kComputeWarps = 4, kThreads = 32 * (kComputeWarps + 1);
 constexpr float kWeightBits = 15.0f;  // weights are held times 2^15, so that halves reach down to 2^-39 of the largest one
 constexpr uint32_t kMaxGrid = 448;
 constexpr uint32_t kSplitUnits = 6;  // what cutting segments costs, in units
@@ -64,7 +64,8 @@ template <bool BF16, int DP>
 constexpr uint32_t kPartialFloats = kComputeWarps * kRows<BF16> * (DP + 2);
 
 struct Request {
-  uint32_t first, rows, q_len, len, tiles, row_tiles, weight;
+  uint32_t first, rows, q_len, len, tiles, row_tiles;
+  uint32_t weight;  // warps that the rows of a tile are dealt to (1, 2, 4; the tokens to the others): units of a stage
 };
 
 template <uint32_t ROWS>
@@ -76,10 +77,9 @@ __device__ __forceinline__ Request request_of(const AttendParams &p, uint32_t r)
   q.first = (uint32_t)b;
   q.q_len = (uint32_t)(e - b);
   q.rows = q.q_len * p.group;
-  const bool wide = q.rows > ROWS;
-  q.row_tiles = q.rows == 0 ? 0u : wide ? (q.rows + kComputeWarps * ROWS - 1) / (kComputeWarps * ROWS) : 1u;
+  q.weight = q.rows <= ROWS ? 1u : q.rows <= 2 * ROWS ? 2u : kComputeWarps;
+  q.row_tiles = (q.rows + q.weight * ROWS - 1) / (q.weight * ROWS);
   q.tiles = max(1u, (q.len + kStageTokens - 1) / kStageTokens);
-  q.weight = wide ? kComputeWarps : 1u;
   return q;
 }
 
@@ -115,7 +115,7 @@ __device__ __forceinline__ bool next_part(const AttendParams &p, Line &line, Par
     part.rq = q;
     part.r = line.r;
     part.h = idx % p.kv_heads;
-    part.row0 = idx / p.kv_heads * (kComputeWarps * ROWS);
+    part.row0 = idx / p.kv_heads * (q.weight * ROWS);
     part.parts = 1;
     part.first_cta = blockIdx.x;
     part.t0 = 0;
@@ -136,8 +136,7 @@ __device__ __forceinline__ bool next_part(const AttendParams &p, Line &line, Par
       line.at = stop;
       if (part.t1 <= part.t0) continue;
     }
-    const uint32_t tile_rows = q.weight == 1 ? ROWS : kComputeWarps * ROWS;
-    const uint32_t last_row = min(q.rows, part.row0 + tile_rows) - 1;
+    const uint32_t last_row = min(q.rows, part.row0 + q.weight * ROWS) - 1;
     const long long see = (long long)q.len - q.q_len + last_row / p.group + 1;
     part.limit = (uint32_t)max(0ll, min(see, (long long)q.len));
     part.t1 = max(part.t0, min(part.t1, (part.limit + kStageTokens - 1) / kStageTokens));
@@ -147,50 +146,46 @@ __device__ __forceinline__ bool next_part(const AttendParams &p, Line &line, Par
 }
 
 // ---------------------------------------------------------------- widening codes to pairs of halves
-// Bytes (0, 2) and (1, 3) of a word.
+// int8: 1024 + (code + 128) is a half with the code in its last bits. e4m3: an instruction.
+__device__ __forceinline__ uint32_t half_of_biased(uint32_t biased) {  // two halves 1024 + (code + 128)
+  const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&biased), bias);
+  return *reinterpret_cast<const uint32_t *>(&x);
+}
+__device__ __forceinline__ void halves_of_e4m3(uint32_t w, uint32_t &low, uint32_t &high) {  // bytes (0, 1) and (2, 3)
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(low), "=r"(high) : "r"(w));
+}
+// The four codes of a word as two pairs: bytes (0, 1) and (2, 3).
 template <int FORMAT>
-__device__ __forceinline__ void widen_alternate(uint32_t w, uint32_t &even, uint32_t &odd) {
-  if (FORMAT == DF_CACHE_INT8) {  // 1024 + (code + 128) is a half with the code in its last bits
+__device__ __forceinline__ void widen_word(uint32_t w, uint32_t &first, uint32_t &second) {
+  if (FORMAT == DF_CACHE_INT8) {
     const uint32_t u = w ^ 0x80808080u;
-    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
-    uint32_t a = __byte_perm(u, 0x64646464u, 0x4240), b = __byte_perm(u, 0x64646464u, 0x4341);
-    const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), bias), y = __hsub2(*reinterpret_cast<__half2 *>(&b), bias);
-    even = *reinterpret_cast<const uint32_t *>(&x);
-    odd = *reinterpret_cast<const uint32_t *>(&y);
-  } else {  // times 2^-8 (cache_codes.cuh)
-    even = ((w << 7) & 0x3f803f80u) | ((w << 8) & 0x80008000u);
-    odd = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
+    first = half_of_biased(__byte_perm(u, 0x64646464u, 0x4140));
+    second = half_of_biased(__byte_perm(u, 0x64646464u, 0x4342));
+  } else {
+    halves_of_e4m3(w, first, second);
   }
 }
 // Byte i of two words each, for the four i: pair[i] = (a.byte i, b.byte i).
 template <int FORMAT>
 __device__ __forceinline__ void widen_pairs(uint32_t a, uint32_t b, uint32_t (&pair)[4]) {
-  if (FORMAT == DF_CACHE_INT8) {
-    const uint32_t lo = __byte_perm(a, b, 0x5140) ^ 0x80808080u, hi = __byte_perm(a, b, 0x7362) ^ 0x80808080u;  // a0 b0 a1 b1, a2 b2 a3 b3
-    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    pair[0] = __byte_perm(lo, 0x64646464u, 0x4140);
-    pair[1] = __byte_perm(lo, 0x64646464u, 0x4342);
-    pair[2] = __byte_perm(hi, 0x64646464u, 0x4140);
-    pair[3] = __byte_perm(hi, 0x64646464u, 0x4342);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&pair[i]), bias);
-      pair[i] = *reinterpret_cast<const uint32_t *>(&x);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t t = __byte_perm(a, b, (uint32_t)(i | (i << 4) | ((4 + i) << 8) | ((4 + i) << 12)));  // a.i a.i b.i b.i
-      pair[i] = ((t >> 1) & 0x3f803f80u) | (t & 0x80008000u);
-    }
-  }
+  const uint32_t lo = __byte_perm(a, b, 0x5140), hi = __byte_perm(a, b, 0x7362);  // a0 b0 a1 b1, a2 b2 a3 b3
+  widen_word<FORMAT>(lo, pair[0], pair[1]);
+  widen_word<FORMAT>(hi, pair[2], pair[3]);
 }
 
 __device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_half_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // onto zeros
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 __device__ __forceinline__ uint32_t halves(float lo, float hi) {
@@ -276,26 +271,31 @@ __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 12
 
 template <int DP>
 constexpr uint32_t kSubBytes = 16 * DP;  // a box of 16 tokens, or less where D < DP: whole swizzle periods
-template <int DP>
-constexpr uint32_t kRingBytes = kStages * 2 * (kStageTokens / 16) * kSubBytes<DP>;
+// Stages of the ring: three CTAs of an SM share its 227 KB (fp32 rows), or two (bf16 rows, which need more registers).
 template <bool BF16, int DP>
-constexpr uint32_t kSmemBytes = 1024 + kRingBytes<DP> + kComputeWarps * kRows<BF16> * DP * 4;
+constexpr uint32_t kStagesOf = BF16 ? (DP == 128 ? 5 : 8) : (DP == 128 ? 3 : 6);
+template <bool BF16, int DP>
+constexpr uint32_t kRingBytes = kStagesOf<BF16, DP> * 2 * (kStageTokens / 16) * kSubBytes<DP>;
+template <bool BF16, int DP>
+constexpr uint32_t kSmemBytes = 1024 + kRingBytes<BF16, DP> + kComputeWarps * 8 * DP * 4;
 
 template <bool BF16, int FORMAT, int DP>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, BF16 ? 2 : 3)
 k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttendParams p) {
-  constexpr uint32_t ROWS = kRows<BF16>;
+  constexpr uint32_t ROWS = kRows<BF16>, kStages = kStagesOf<BF16, DP>;
   constexpr int KT = DP / 16, NT = DP / 8, RW = BF16 ? 2 : 1;  // k-steps, n-tiles, rows of a lane
-  constexpr float kCodeScale = FORMAT == DF_CACHE_E4M3 ? 256.0f : 1.0f;
   extern __shared__ uint8_t smem_raw[];
   __shared__ float2 s_scale[kStages][kStageTokens / 16];  // k_scale, v_scale of a stage's boxes
-  __shared__ float s_m[kComputeWarps][ROWS], s_l[kComputeWarps][ROWS];
+  __shared__ float s_m[kComputeWarps][8], s_l[kComputeWarps][8];
+  __shared__ Line s_line[kComputeWarps];
+  __shared__ Part s_part[kComputeWarps];
   __shared__ uint64_t s_full[kStages], s_empty[kStages];
   __shared__ unsigned long long s_sum[kThreads / 32][2], s_place[2];
   __shared__ uint32_t s_most[kThreads / 32], s_request, s_last, s_abort;
   const uint32_t t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const uint32_t ring = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
-  float *merge = reinterpret_cast<float *>(smem_raw + (ring - ptx::smem_u32(smem_raw)) + kRingBytes<DP>);  // [warp][row][DP]
+  uint8_t *ring_bytes = smem_raw + (ring - ptx::smem_u32(smem_raw));
+  float *merge = reinterpret_cast<float *>(ring_bytes + kRingBytes<BF16, DP>);  // [warp]: q as operands [k-step][lane][4 words], later a state [8 rows][DP]
   if (t == 0) {
     for (uint32_t s = 0; s < kStages; ++s) {
       ptx::mbar_init(ptx::smem_u32(&s_full[s]), 1);
@@ -363,47 +363,65 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 
   const uint32_t a_full = ptx::smem_u32(&s_full[0]), a_empty = ptx::smem_u32(&s_empty[0]);
   const uint32_t chunks = p.D / 16;  // 16-byte pieces of a row
-  Part part;
   uint32_t stage = 0;  // stages so far, this CTA
   if (warp == kComputeWarps) {
     // ---------------------------------------------------------------- the loading warp
-    // Eight stages at a time: lane i looks up the page and scales of box i % 4 of stage i / 4 of the group.
+    // Eight stages at a time: lane i has the page and scales of box i % 4 of stage i / 4. They are looked up a group ahead: the table's
+    // entry before the present group is loaded, the scales behind it.
+    struct Group {
+      uint32_t stages, slice, line, boxes;  // boxes: a bit per lane that has one
+      int32_t page;
+      float2 scale;
+    } now, then;
     const uint32_t box_bytes = 16 * p.D;
-    while (next_part<ROWS>(p, line, part)) {
-      const int32_t *row = p.table + (size_t)part.r * p.width;
-      for (uint32_t g = part.t0; g < part.t1; g += 8) {
-        const uint32_t token = (g + lane / 4) * kStageTokens + lane % 4 * 16;
-        const bool in = token < part.limit && g + lane / 4 < part.t1;
-        uint32_t slice = p.n_pages * p.kv_heads, line0 = 0;  // behind the last slice: zeros
-        float2 scale = make_float2(0.0f, 0.0f);
-        if (in) {
-          const uint32_t page = (uint32_t)__ldg(row + token / p.P);
-          if (page < p.n_pages) {
-            slice = page * p.kv_heads + part.h;
-            scale = make_float2(__ldg(p.k_scale + slice), __ldg(p.v_scale + slice));
-          }
-          line0 = token % p.P * p.D / 128;
+    uint32_t tile = 0, head = 0;
+    Part part;
+    part.t1 = 0;
+    auto look_up = [&](Group &gr) {
+      gr.stages = 0;
+      if (tile >= part.t1) {
+        do {
+          if (!next_part<ROWS>(p, line, part)) return;
+        } while (part.t0 >= part.t1);  // a part that sees nothing
+        tile = part.t0;
+      }
+      head = part.h;
+      const uint32_t token = (tile + lane / 4) * kStageTokens + lane % 4 * 16;
+      const bool in = token < part.limit && tile + lane / 4 < part.t1;
+      gr.page = in ? __ldg(p.table + (size_t)part.r * p.width + token / p.P) : -1;
+      gr.line = token % p.P * p.D / 128;
+      gr.boxes = __ballot_sync(0xffffffffu, in);
+      gr.stages = min(8u, part.t1 - tile);
+      tile += gr.stages;
+    };
+    auto look_up_scales = [&](Group &gr) {
+      const bool in = (uint32_t)gr.page < p.n_pages;
+      gr.slice = in ? (uint32_t)gr.page * p.kv_heads + head : p.n_pages * p.kv_heads;  // behind the last slice: zeros
+      gr.scale = in ? make_float2(__ldg(p.k_scale + gr.slice), __ldg(p.v_scale + gr.slice)) : make_float2(0.0f, 0.0f);
+    };
+    look_up(now);
+    look_up_scales(now);
+    while (now.stages) {
+      look_up(then);
+      for (uint32_t s = 0; s < now.stages; ++s, ++stage) {
+        const uint32_t slot = stage % kStages;
+        if (stage >= kStages && !ptx::mbar_wait_warp(a_empty + 8 * slot, (stage / kStages - 1) & 1, &s_abort)) {
+          if (lane == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
+          goto loaded;
         }
-        const uint32_t ballot = __ballot_sync(0xffffffffu, in);
-        for (uint32_t s = 0; s < min(8u, part.t1 - g); ++s, ++stage) {
-          const uint32_t slot = stage % kStages;
-          if (stage >= kStages && !ptx::mbar_wait_warp(a_empty + 8 * slot, (stage / kStages - 1) & 1, &s_abort)) {
-            if (lane == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
-            goto loaded;
-          }
-          const bool mine_now = lane / 4 == s;
-          if (mine_now) s_scale[slot][lane % 4] = scale;
-          __syncwarp();
-          const uint32_t boxes = __popc((ballot >> (4 * s)) & 15u);
-          if (lane == 0) ptx::mbar_arrive_expect_tx(a_full + 8 * slot, 2 * boxes * box_bytes);
-          __syncwarp();
-          if (mine_now && in) {
-            const uint32_t dst = ring + (slot * 2 * 4 + lane % 4) * kSubBytes<DP>;
-            ptx::tma_load_3d(dst, &k_map, a_full + 8 * slot, 0, (int)line0, (int)slice);
-            ptx::tma_load_3d(dst + 4 * kSubBytes<DP>, &v_map, a_full + 8 * slot, 0, (int)line0, (int)slice);
-          }
+        const bool my_turn = lane / 4 == s;
+        if (my_turn) s_scale[slot][lane % 4] = now.scale;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_expect_tx(a_full + 8 * slot, 2 * box_bytes * __popc((now.boxes >> (4 * s)) & 15u));
+        __syncwarp();
+        if (my_turn && (now.boxes >> lane & 1)) {
+          const uint32_t dst = ring + (slot * 2 * 4 + lane % 4) * kSubBytes<DP>;
+          ptx::tma_load_3d(dst, &k_map, a_full + 8 * slot, 0, (int)now.line, (int)now.slice);
+          ptx::tma_load_3d(dst + 4 * kSubBytes<DP>, &v_map, a_full + 8 * slot, 0, (int)now.line, (int)now.slice);
         }
       }
+      if (then.stages) look_up_scales(then);
+      now = then;
     }
   loaded:
     if (s_abort) {  // copies in flight write to this CTA's shared memory: none may be left when it goes
@@ -417,13 +435,46 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   // ---------------------------------------------------------------- the computing warps
   const uint32_t g = lane >> 2, c = lane & 3;
   bool ok = true;
-  while (next_part<ROWS>(p, line, part)) {
-    const bool wide = part.rq.weight != 1;
-    const uint32_t warp_row = part.row0 + (wide ? warp * ROWS : 0);
+  uint8_t *q_at = ring_bytes + kRingBytes<BF16, DP> + warp * (8 * DP * 4) + lane * 16;
+  // Tokens of a lane's accumulators: tile j, columns 2c and 2c + 1. With 64-byte rows the order below keeps two rows of a 128-byte
+  // line together, which the swizzle then spreads over all banks.
+  auto token_of = [&](uint32_t j, uint32_t col) { return DP == 128 ? 8 * j + col : 4 * (col >> 1) + 2 * j + (col & 1); };
+  auto piece = [&](uint32_t token, uint32_t chunk) {  // where a box has a 16-byte piece
+    const uint32_t x = token * chunks + min(chunk, chunks - 1);
+    return (x * 16) ^ ((x & 0x38u) << 1);
+  };
+  // Behind the row's end (D < DP) its last piece is read again: it meets zeros of q, or makes dims that are not stored.
+  uint32_t k_off[2][KT / 4], v_off[4];
+#pragma unroll
+  for (int k4 = 0; k4 < KT / 4; ++k4) {
+    k_off[0][k4] = piece(token_of(0, g), c * (KT / 4) + k4);
+    k_off[1][k4] = piece(token_of(1, g), c * (KT / 4) + k4);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v_off[k] = DP == 128 ? piece(token_of(k >> 1, 2 * c + (k & 1)), g) : piece(token_of(k >> 1, 2 * c + (k & 1)), g >> 1) + 8 * (g & 1);
+  // A warp's place on the line and its present part lie in shared memory: registers are for the loop over the tokens.
+  if (lane == 0) s_line[warp] = line;
+  for (;;) {
+    __syncwarp();
+    Line next = s_line[warp];
+    __syncwarp();
+    Part found;
+    if (!next_part<ROWS>(p, next, found)) break;
+    if (lane == 0) {
+      s_line[warp] = next;
+      s_part[warp] = found;
+    }
+    __syncwarp();
+    const Part &part = s_part[warp];
+    const uint32_t tile0 = found.t0, tile1 = found.t1;
+    const uint32_t weight = part.rq.weight, row_warp = warp & (weight - 1), token_warp = weight == 1 ? warp : weight == 2 ? warp >> 1 : 0u;
+    const uint32_t warp_row = part.row0 + row_warp * ROWS;
     // rows of this lane
-    uint32_t see[RW], a[KT][4];
+    uint32_t see[RW];
     bool valid[RW];
-    float norm[RW], m[RW], l[RW], o[RW][NT * 2];
+    float norm[RW], m[RW], l[RW];
+    float2 o[RW][NT];  // columns 2c, 2c + 1 of n-tile n: dims 2c * DP/8 + n and (2c + 1) * DP/8 + n
+    __syncwarp();  // the region below was read as a merge buffer by this warp's lanes alone, behind a barrier
 #pragma unroll
     for (int i = 0; i < RW; ++i) {
       const uint32_t row = warp_row + g + 8 * i;
@@ -451,160 +502,181 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       const uint32_t exponent = min(max(__float_as_uint(top) >> 23, 1u), 253u);
       const bool keep = top == 0.0f || top == INFINITY;
       const float down = keep ? 1.0f : __uint_as_float((254u - exponent) << 23);
-      norm[i] = (keep ? 1.0f : __uint_as_float(exponent << 23)) * (kCodeScale * p.scale_log2);  // the scale after the product: q itself fits its halves
+      norm[i] = (keep ? 1.0f : __uint_as_float(exponent << 23)) * p.scale_log2;  // the scale after the product: q itself fits its halves
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        if (BF16) {
-          a[kt][i] = halves(x[kt][0] * down, x[kt][2] * down);
-          a[kt][2 + i] = halves(x[kt][1] * down, x[kt][3] * down);
+        uint32_t a[2][2];
+        if (BF16) {  // this row's two of the four operand words
+          a[0][0] = halves(x[kt][0] * down, x[kt][1] * down);
+          a[0][1] = halves(x[kt][2] * down, x[kt][3] * down);
+          *reinterpret_cast<uint32_t *>(q_at + kt * 512 + 4 * i) = a[0][0];
+          *reinterpret_cast<uint32_t *>(q_at + kt * 512 + 4 * (2 + i)) = a[0][1];
         } else {
-          split_halves(x[kt][0] * down, x[kt][2] * down, a[kt][0], a[kt][1]);
-          split_halves(x[kt][1] * down, x[kt][3] * down, a[kt][2], a[kt][3]);
+          split_halves(x[kt][0] * down, x[kt][1] * down, a[0][0], a[0][1]);
+          split_halves(x[kt][2] * down, x[kt][3] * down, a[1][0], a[1][1]);
+          *reinterpret_cast<uint4 *>(q_at + kt * 512) = make_uint4(a[0][0], a[0][1], a[1][0], a[1][1]);
         }
       }
       m[i] = -FLT_MAX;
       l[i] = 0.0f;
 #pragma unroll
-      for (int n2 = 0; n2 < NT * 2; ++n2) o[i][n2] = 0.0f;
+      for (int n2 = 0; n2 < NT; ++n2) o[i][n2] = make_float2(0.0f, 0.0f);
     }
     // what the warp's rows see, at least and at most: rows are in the order of their tokens
     const uint32_t last_row = min(part.rq.rows, warp_row + ROWS) - 1;
     const long long lo = (long long)part.rq.len - part.rq.q_len + warp_row / p.group + 1, hi = (long long)part.rq.len - part.rq.q_len + last_row / p.group + 1;
     const uint32_t see_all = (uint32_t)max(0ll, min(lo, (long long)part.rq.len));
     const uint32_t see_any = warp_row < part.rq.rows ? (uint32_t)max(0ll, min(hi, (long long)part.rq.len)) : 0u;
+    const bool second_rows = !BF16 || warp_row + 8 < part.rq.rows;  // bf16: whether rows 8 .. 15 of the warp are there
 
-    for (uint32_t tile = part.t0; tile < part.t1; ++tile, ++stage) {
+    // Two boxes, 32 tokens, at a time. Where tokens are dealt to four warps, two of them share a stage and the pairs take turns; to two, each
+    // takes a half. Every warp waits for every stage and gives it back, also one that has nothing to do with it: a wait names its phase by a
+    // parity, and a warp that had passed over a stage of a slot would take that stage for the next one.
+    const uint32_t pair0 = weight == kComputeWarps ? 0u : token_warp & 1, pair1 = weight == kComputeWarps ? 2u : pair0 + 1;
+    for (uint32_t tile = tile0; tile < tile1; ++tile, ++stage) {
       const uint32_t slot = stage % kStages;
-      if (ok) ok = ptx::mbar_wait_warp(a_full + 8 * slot, (stage / kStages) & 1, &s_abort);
-      const uint32_t stage_at = ring + slot * 2 * 4 * kSubBytes<DP>;
-      for (uint32_t sub = wide ? 0 : warp; ok && sub < (wide ? 4u : warp + 1); ++sub) {
-        const uint32_t token0 = tile * kStageTokens + sub * 16;
+      ok = ok && ptx::mbar_wait_warp(a_full + 8 * slot, (stage / kStages) & 1, &s_abort);
+      if (!ok) continue;
+      const uint8_t *stage_at = ring_bytes + slot * 2 * 4 * kSubBytes<DP>;
+      const bool idle = weight == 1 && ((tile - tile0) & 1) != token_warp >> 1;
+      for (uint32_t pair = idle ? pair1 : pair0; pair < pair1; ++pair) {
+        const uint32_t token0 = tile * kStageTokens + pair * 32;
         if (token0 >= see_any) break;
-        const float2 scale = s_scale[slot][sub];
-        const uint32_t k_at = stage_at + sub * kSubBytes<DP>, v_at = k_at + 4 * kSubBytes<DP>;
-        // Tokens of a lane's accumulators: tile j, columns 2c and 2c + 1. With 64-byte rows the order below keeps two rows of a 128-byte
-        // line together, which the swizzle then spreads over all banks.
-        auto token_of = [&](uint32_t j, uint32_t col) { return DP == 128 ? 8 * j + col : 4 * (col >> 1) + 2 * j + (col & 1); };
-        auto piece = [&](uint32_t at, uint32_t token, uint32_t chunk) {  // address of a 16-byte piece
-          const uint32_t x = token * chunks + chunk;
-          return at + ((x * 16) ^ ((x & 0x38u) << 1));
-        };
+        const float2 scale[2] = {s_scale[slot][2 * pair], s_scale[slot][2 * pair + 1]};
+        const uint8_t *k_at = stage_at + 2 * pair * kSubBytes<DP>, *v_at = k_at + 4 * kSubBytes<DP>;
         // ---- scores
-        float acc[2][4];
+        float acc[4][4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t w[KT];
-          const uint32_t token = token_of(j, g);
+        for (int k4 = 0; k4 < KT / 4; ++k4) {
+          uint32_t w[4][4];
 #pragma unroll
-          for (int k4 = 0; k4 < KT / 4; ++k4) {
-            const uint32_t chunk = c * (KT / 4) + k4;
-            if (chunk < chunks) {
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(w[4 * k4]), "=r"(w[4 * k4 + 1]), "=r"(w[4 * k4 + 2]), "=r"(w[4 * k4 + 3])
-                           : "r"(piece(k_at, token, chunk)));
-            } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) w[4 * k4 + k] = 0u;
-            }
+          for (int nt = 0; nt < 4; ++nt) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(k_at + (nt >> 1) * kSubBytes<DP> + k_off[nt & 1][k4]);
+            w[nt][0] = v.x; w[nt][1] = v.y; w[nt][2] = v.z; w[nt][3] = v.w;
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) acc[j][k] = 0.0f;
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint4 q4 = *reinterpret_cast<const uint4 *>(q_at + (k4 * 4 + kk) * 512);
+            const uint32_t a[4] = {q4.x, q4.y, q4.z, q4.w};
 #pragma unroll
-          for (int kt = 0; kt < KT; ++kt) {
-            uint32_t b0, b1;
-            widen_alternate<FORMAT>(w[kt], b0, b1);
-            mma_half(acc[j], a[kt], b0, b1);
+            for (int nt = 0; nt < 4; ++nt) {
+              uint32_t b0, b1;
+              widen_word<FORMAT>(w[nt][kk], b0, b1);
+              if (k4 == 0 && kk == 0) mma_half_first(acc[nt], a, b0, b1);
+              else mma_half(acc[nt], a, b0, b1);
+            }
           }
         }
         // ---- weights
-        const bool masked = token0 + 16 > see_all;
-        uint32_t pa[4];
-        float v_row[RW];
+        const bool masked = token0 + 32 > see_all;
+        // The two boxes' weights meet one scale of V, the larger one; a row that sees none of a box's tokens takes nothing of
+        // it, whatever its scale is (it may be NaN).
+        const float v_scale = fmaxf(scale[0].y, scale[1].y);
+        const bool v_alike = scale[0].y == scale[1].y && !masked;
+        uint32_t pa[2][4];
+        float v_row[RW], before[RW];
         bool grew = false;
-        float before[RW];
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
-          const float f = scale.x * norm[i];
-          float s[2][2];
+          before[i] = m[i];
+          v_row[i] = 0.0f;
+          if (BF16 && i == 1 && !second_rows) {
+            pa[0][1] = pa[0][3] = pa[1][1] = pa[1][3] = 0u;
+            continue;
+          }
+          const float f[2] = {scale[0].x * norm[i], scale[1].x * norm[i]};
+          float s[4][2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              s[j][k] = (BF16 ? acc[j][2 * i + k] : acc[j][k] + acc[j][2 + k]) * f;
-              if (masked && token0 + token_of(j, 2 * c + k) >= see[i]) s[j][k] = -INFINITY;
-            }
-          float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+            for (int k = 0; k < 2; ++k) s[nt][k] = (BF16 ? acc[nt][2 * i + k] : acc[nt][k] + acc[nt][2 + k]) * f[nt >> 1];
+          if (masked) {
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+                if (token0 + 16 * (nt >> 1) + token_of(nt & 1, 2 * c + k) >= see[i]) s[nt][k] = -INFINITY;
+          }
+          float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          before[i] = m[i];
           grew |= top > m[i];
           m[i] = fmaxf(m[i], top);
           const float shift = m[i] - kWeightBits;
-          float w[2][2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) w[j][k] = ex2_approx(s[j][k] - shift);
-          if (before[i] != m[i]) l[i] *= ex2_approx(before[i] - m[i]);
-          l[i] += (w[0][0] + w[0][1]) + (w[1][0] + w[1][1]);
-          if (BF16) {
-            pa[i] = halves(w[0][0], w[0][1]);
-            pa[2 + i] = halves(w[1][0], w[1][1]);
-          } else {
-            split_halves(w[0][0], w[0][1], pa[0], pa[1]);
-            split_halves(w[1][0], w[1][1], pa[2], pa[3]);
+            for (int k = 0; k < 2; ++k) s[nt][k] = ex2_approx(s[nt][k] - shift);
+          l[i] = fmaf(l[i], ex2_approx(before[i] - m[i]), ((s[0][0] + s[0][1]) + (s[1][0] + s[1][1])) + ((s[2][0] + s[2][1]) + (s[3][0] + s[3][1])));
+          v_row[i] = token0 < see[i] ? v_scale : 0.0f;
+          if (!v_alike) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const float share = token0 + 16 * b < see[i] && v_scale != 0.0f ? __fdividef(scale[b].y, v_scale) : 0.0f;
+#pragma unroll
+              for (int nt = 2 * b; nt < 2 * b + 2; ++nt)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) s[nt][k] *= share;
+            }
           }
-          // a row that sees none of these tokens takes nothing of them, whatever their scale is (it may be NaN)
-          v_row[i] = token0 < see[i] ? scale.y : 0.0f;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (BF16) {
+              pa[b][i] = halves(s[2 * b][0], s[2 * b][1]);
+              pa[b][2 + i] = halves(s[2 * b + 1][0], s[2 * b + 1][1]);
+            } else {
+              split_halves(s[2 * b][0], s[2 * b][1], pa[b][0], pa[b][1]);
+              split_halves(s[2 * b + 1][0], s[2 * b + 1][1], pa[b][2], pa[b][3]);
+            }
+          }
         }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
           for (int i = 0; i < RW; ++i) {
             const float f = ex2_approx(before[i] - m[i]);
 #pragma unroll
-            for (int n = 0; n < NT * 2; ++n) o[i][n] *= f;
+            for (int n = 0; n < NT; ++n) o[i][n] = make_float2(o[i][n].x * f, o[i][n].y * f);
           }
         }
         // ---- output
-        uint32_t w[4][NT / 4];
+        uint32_t w[2][4][NT / 4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t token = token_of(k >> 1, 2 * c + (k & 1));
-          if constexpr (DP == 128) {
-            if (g < chunks) {
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(w[k][0]), "=r"(w[k][1]), "=r"(w[k][2]), "=r"(w[k][3])
-                           : "r"(piece(v_at, token, g)));
-            } else {
-              w[k][0] = w[k][1] = w[k][2] = w[k][3] = 0u;
-            }
-          } else {
-            if ((g >> 1) < chunks) {
-              asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[k][0]), "=r"(w[k][1]) : "r"(piece(v_at, token, g >> 1) + 8 * (g & 1)));
-            } else {
-              w[k][0] = w[k][1] = 0u;
-            }
-          }
-        }
-#pragma unroll
-        for (int n4 = 0; n4 < NT / 4; ++n4) {
-          uint32_t b0[4], b1[4];
-          widen_pairs<FORMAT>(w[0][n4], w[1][n4], b0);
-          widen_pairs<FORMAT>(w[2][n4], w[3][n4], b1);
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma_half(d, pa, b0[k], b1[k]);
-            const int n = n4 * 4 + k;  // columns 2c, 2c + 1: dims 2c * DP/8 + n and (2c + 1) * DP/8 + n
-            if (BF16) {
-#pragma unroll
-              for (int i = 0; i < RW; ++i) {
-                o[i][n] = fmaf(v_row[i], d[2 * i], o[i][n]);
-                o[i][NT + n] = fmaf(v_row[i], d[2 * i + 1], o[i][NT + n]);
-              }
+            const uint8_t *at = v_at + b * kSubBytes<DP> + v_off[k];
+            if constexpr (DP == 128) {
+              const uint4 v = *reinterpret_cast<const uint4 *>(at);
+              w[b][k][0] = v.x; w[b][k][1] = v.y; w[b][k][2] = v.z; w[b][k][3] = v.w;
             } else {
-              o[0][n] = fmaf(v_row[0], d[0] + d[2], o[0][n]);
-              o[0][NT + n] = fmaf(v_row[0], d[1] + d[3], o[0][NT + n]);
+              const uint2 v = *reinterpret_cast<const uint2 *>(at);
+              w[b][k][0] = v.x; w[b][k][1] = v.y;
+            }
+            // behind the last token that a row sees a box may hold any bytes, and an 8-bit float may be NaN
+            if (FORMAT == DF_CACHE_E4M3 && masked && token0 + 16 * b + token_of(k >> 1, 2 * c + (k & 1)) >= see_any) {
+#pragma unroll
+              for (int n4 = 0; n4 < NT / 4; ++n4) w[b][k][n4] = 0u;
+            }
+          }
+#pragma unroll
+        for (int n4 = 0; n4 < NT / 4; ++n4) {
+          uint32_t b0[2][4], b1[2][4];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            widen_pairs<FORMAT>(w[b][0][n4], w[b][1][n4], b0[b]);
+            widen_pairs<FORMAT>(w[b][2][n4], w[b][3][n4], b1[b]);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float d[4];
+            mma_half_first(d, pa[0], b0[0][k], b1[0][k]);
+            mma_half(d, pa[1], b0[1][k], b1[1][k]);
+            const int n = n4 * 4 + k;
+            if (BF16) {
+              o[0][n] = ptx::fma2(make_float2(v_row[0], v_row[0]), make_float2(d[0], d[1]), o[0][n]);
+              if (second_rows) o[RW - 1][n] = ptx::fma2(make_float2(v_row[RW - 1], v_row[RW - 1]), make_float2(d[2], d[3]), o[RW - 1][n]);
+            } else {
+              o[0][n] = ptx::fma2(make_float2(v_row[0], v_row[0]), ptx::add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])), o[0][n]);
             }
           }
         }
@@ -617,19 +689,22 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     for (int i = 0; i < RW; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-#pragma unroll
-      for (int n = 0; n < NT * 2; ++n) o[i][n] *= kCodeScale;
     }
+    // four of the lane's DP / 4 dims of row i, from the n-th on
+    auto four = [&](int i, int n) {
+      return n < NT ? make_float4(o[i][n].x, o[i][n + 1].x, o[i][n + 2].x, o[i][n + 3].x)
+                    : make_float4(o[i][n - NT].y, o[i][n - NT + 1].y, o[i][n - NT + 2].y, o[i][n - NT + 3].y);
+    };
 
-    // ---- the result, or this part of it: o[i][0 .. DP/4) are row i's dims c * DP/4 ...
+    // ---- the result, or this part of it
     const bool split = part.parts > 1;
-    const uint32_t rows = wide ? min(part.rq.rows - part.row0, kComputeWarps * ROWS) : part.rq.rows;
+    const uint32_t rows = min(part.rq.rows - part.row0, weight * ROWS);
     auto state_of = [&](uint32_t cta) {  // the first CTA of a segment has it last, every other one first
       return p.partial + (size_t)(2 * cta + (cta == part.first_cta ? 1 : 0)) * kPartialFloats<BF16, DP>;
     };
-    auto finish_row = [&](size_t row, uint32_t dim, const float (&x)[4], float mm, float ll) {  // four dims of a finished row
+    auto finish_row = [&](size_t row, uint32_t dim, const float4 &x, float mm, float ll) {  // four dims of a finished row
       const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-      const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+      const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
       if (dim < p.D) store_row4<BF16>(p.out, row * p.D + dim, p.out_aligned, y);
       if (dim == 0 && p.lse) p.lse[row] = ll == 0.0f ? -INFINITY : (mm - kWeightBits + log2f(ll)) * kLn2;
     };
@@ -638,44 +713,45 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       return (size_t)(part.rq.first + rr / p.group) * p.heads + part.h * p.group + rr % p.group;
     };
     float *mine_state = state_of(blockIdx.x), *mine_o = mine_state + 2 * kComputeWarps * ROWS;
-    if (wide) {
+    if (weight == kComputeWarps) {
 #pragma unroll
       for (int i = 0; i < RW; ++i) {
+        if (!valid[i]) continue;
         const uint32_t row = warp * ROWS + g + 8 * i;
 #pragma unroll
         for (int n = 0; n < DP / 4; n += 4) {
-          const float x[4] = {o[i][n], o[i][n + 1], o[i][n + 2], o[i][n + 3]};
           const uint32_t dim = c * (DP / 4) + n;
-          if (!split && valid[i]) finish_row(global_row(row), dim, x, m[i], l[i]);
-          if (split && valid[i]) *reinterpret_cast<float4 *>(mine_o + row * DP + dim) = make_float4(x[0], x[1], x[2], x[3]);
+          if (split) *reinterpret_cast<float4 *>(mine_o + row * DP + dim) = four(i, n);
+          else finish_row(global_row(row), dim, four(i, n), m[i], l[i]);
         }
-        if (split && valid[i] && c == 0) *reinterpret_cast<float2 *>(mine_state + 2 * row) = make_float2(m[i], l[i]);
+        if (split && c == 0) *reinterpret_cast<float2 *>(mine_state + 2 * row) = make_float2(m[i], l[i]);
       }
     } else {
-      // the four warps' states of the same rows
+      // the states of the warps that shared the tokens, eight rows of a warp at a time; a warp's is where its part of q was
 #pragma unroll
       for (int i = 0; i < RW; ++i) {
-        const uint32_t row = g + 8 * i;
+        if (8u * i >= rows) break;
         if (valid[i]) {
-          if (c == 0) { s_m[warp][row] = m[i]; s_l[warp][row] = l[i]; }
+          if (c == 0) { s_m[warp][g] = m[i]; s_l[warp][g] = l[i]; }
 #pragma unroll
-          for (int n = 0; n < DP / 4; n += 4)
-            *reinterpret_cast<float4 *>(merge + (warp * ROWS + row) * DP + c * (DP / 4) + n) = make_float4(o[i][n], o[i][n + 1], o[i][n + 2], o[i][n + 3]);
+          for (int n = 0; n < DP / 4; n += 4) *reinterpret_cast<float4 *>(merge + (warp * 8 + g) * DP + c * (DP / 4) + n) = four(i, n);
         }
-      }
-      compute_barrier();
-      for (uint32_t e = t; e < rows * (DP / 4); e += 32 * kComputeWarps) {
-        const uint32_t row = e / (DP / 4), dim = e % (DP / 4) * 4;
-        Running sum;
-#pragma unroll
-        for (uint32_t w = 0; w < kComputeWarps; ++w)
-          sum.add(s_m[w][row], s_l[w][row], *reinterpret_cast<const float4 *>(merge + (w * ROWS + row) * DP + dim));
-        if (!split) {
-          finish_row(global_row(row), dim, sum.o, sum.m, sum.l);
-        } else {
-          *reinterpret_cast<float4 *>(mine_o + row * DP + dim) = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
-          if (dim == 0) *reinterpret_cast<float2 *>(mine_state + 2 * row) = make_float2(sum.m, sum.l);
+        compute_barrier();
+        for (uint32_t e = t; e < weight * 8 * (DP / 4); e += 32 * kComputeWarps) {
+          const uint32_t w0 = e / (8 * (DP / 4)), r8 = e / (DP / 4) % 8, row = w0 * ROWS + r8 + 8 * i, dim = e % (DP / 4) * 4;
+          if (row >= rows) break;
+          Running sum;
+          for (uint32_t w = w0; w < kComputeWarps; w += weight)
+            sum.add(s_m[w][r8], s_l[w][r8], *reinterpret_cast<const float4 *>(merge + (w * 8 + r8) * DP + dim));
+          const float4 x = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
+          if (!split) {
+            finish_row(global_row(row), dim, x, sum.m, sum.l);
+          } else {
+            *reinterpret_cast<float4 *>(mine_o + row * DP + dim) = x;
+            if (dim == 0) *reinterpret_cast<float2 *>(mine_state + 2 * row) = make_float2(sum.m, sum.l);
+          }
         }
+        if (i + 1 < RW) compute_barrier();
       }
     }
     if (split) {
@@ -702,7 +778,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             sum.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4 *>(state + 2 * kComputeWarps * ROWS + row * DP + dim)));
           }
           if (ways == 1) {
-            finish_row(global_row(row), dim, sum.o, sum.m, sum.l);
+            finish_row(global_row(row), dim, make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]), sum.m, sum.l);
           } else {  // elements * ways <= 128 threads, six floats each
             float *at = merge + (way * elements + e) * 8;
             *reinterpret_cast<float4 *>(at) = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
@@ -718,7 +794,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
               const float *at = merge + (w * elements + t) * 8;
               sum.add(at[4], at[5], *reinterpret_cast<const float4 *>(at));
             }
-            finish_row(global_row(t / (DP / 4)), t % (DP / 4) * 4, sum.o, sum.m, sum.l);
+            finish_row(global_row(t / (DP / 4)), t % (DP / 4) * 4, make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]), sum.m, sum.l);
           }
         }
       }

@@ -391,7 +391,7 @@ DF_API int df_chunked_logit_ce(float *logits, const uint32_t *targets, float *gr
  * above read one sequence's fp32 or bf16 cache) ----
  * Cache: k_cache, v_cache are codes [n_pages][n_kv_heads][page_size][d_head], one byte each, k_scale, v_scale [n_pages][n_kv_heads]
  * fp32; an element is code * scale of its page and head. `format` DF_CACHE_INT8: the code is a signed byte; DF_CACHE_E4M3: an 8-bit float
- * (1 sign, 4 exponent and 3 fraction bits, finite up to 448; the two codes 0x7f and 0xff, which df_cache_append never writes, read as +-480).
+ * (1 sign, 4 exponent and 3 fraction bits, finite up to 448; the codes 0x7f and 0xff, which df_cache_append never writes, are NaN).
  * Token t of request r lies in page block_table[r * table_width + t / page_size], row t % page_size; its slot is page * page_size + row.
  * d_head is a multiple of 16 up to 128, page_size a multiple of 16 up to 256 (anything else: DF_ERR_UNSUPPORTED), n_pages * page_size below 2^31.
  * Lengths, tables, slots and counts are read on the GPU: no call waits for them, so a captured graph replays with new ones.
