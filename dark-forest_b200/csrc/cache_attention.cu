@@ -27,6 +27,7 @@
 #include <math.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "cache_codes.cuh"
 #include "sm100_ptx.cuh"
@@ -38,7 +39,7 @@ using ptx::ex2_approx;
 
 constexpr uint32_t kStageTokens = 64, kComputeWarps = 4, kThreads = 32 * (kComputeWarps + 1);
 constexpr float kWeightBits = 15.0f;  // weights are held times 2^15, so that halves reach down to 2^-39 of the largest one
-constexpr uint32_t kMaxGrid = 448;
+constexpr uint32_t kMaxGrid = 640;
 constexpr uint32_t kSplitUnits = 6;  // what cutting segments costs, in units
 constexpr uint32_t kCounterBytes = 4096;  // a counter per CTA, at the workspace's beginning
 
@@ -57,11 +58,14 @@ struct AttendParams {
   float scale_log2;
 };
 
+// How query rows fill the 16 rows of an instruction: 8 fp32 rows and their second parts; 8 bf16 rows, the other half empty (few rows: what
+// the kernel waits for is latency, and half the accumulators let more warps in); 16 bf16 rows.
+enum Mode { kFp32, kBf16Few, kBf16 };
 // Rows that one warp takes, and the size of a partial state.
-template <bool BF16>
-constexpr uint32_t kRows = BF16 ? 16 : 8;
-template <bool BF16, int DP>
-constexpr uint32_t kPartialFloats = kComputeWarps * kRows<BF16> * (DP + 2);
+template <Mode MODE>
+constexpr uint32_t kRows = MODE == kBf16 ? 16 : 8;
+template <Mode MODE, int DP>
+constexpr uint32_t kPartialFloats = kComputeWarps * kRows<MODE> * (DP + 2);
 
 struct Request {
   uint32_t first, rows, q_len, len, tiles, row_tiles;
@@ -271,19 +275,22 @@ __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 12
 
 template <int DP>
 constexpr uint32_t kSubBytes = 16 * DP;  // a box of 16 tokens, or less where D < DP: whole swizzle periods
-// Stages of the ring: three CTAs of an SM share its 227 KB (fp32 rows), or two (bf16 rows, which need more registers).
-template <bool BF16, int DP>
-constexpr uint32_t kStagesOf = BF16 ? (DP == 128 ? 5 : 8) : (DP == 128 ? 3 : 6);
-template <bool BF16, int DP>
-constexpr uint32_t kRingBytes = kStagesOf<BF16, DP> * 2 * (kStageTokens / 16) * kSubBytes<DP>;
-template <bool BF16, int DP>
-constexpr uint32_t kSmemBytes = 1024 + kRingBytes<BF16, DP> + kComputeWarps * 8 * DP * 4;
+// CTAs of an SM, by the registers that they need, and stages of the ring, by the shared memory that is left to each.
+template <Mode MODE>
+constexpr int kCtas = MODE == kBf16 ? 2 : 3;
+template <Mode MODE, int DP>
+constexpr uint32_t kStagesOf = MODE == kBf16 ? (DP == 128 ? 5 : 8) : (DP == 128 ? 3 : 6);
+template <Mode MODE, int DP>
+constexpr uint32_t kRingBytes = kStagesOf<MODE, DP> * 2 * (kStageTokens / 16) * kSubBytes<DP>;
+template <Mode MODE, int DP>
+constexpr uint32_t kSmemBytes = 1024 + kRingBytes<MODE, DP> + kComputeWarps * 8 * DP * 4;
 
-template <bool BF16, int FORMAT, int DP>
-__global__ void __launch_bounds__(kThreads, BF16 ? 2 : 3)
+template <Mode MODE, int FORMAT, int DP>
+__global__ void __launch_bounds__(kThreads, kCtas<MODE>)
 k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttendParams p) {
-  constexpr uint32_t ROWS = kRows<BF16>, kStages = kStagesOf<BF16, DP>;
-  constexpr int KT = DP / 16, NT = DP / 8, RW = BF16 ? 2 : 1;  // k-steps, n-tiles, rows of a lane
+  constexpr uint32_t ROWS = kRows<MODE>, kStages = kStagesOf<MODE, DP>;
+  constexpr bool BF16 = MODE != kFp32;
+  constexpr int KT = DP / 16, NT = DP / 8, RW = MODE == kBf16 ? 2 : 1;  // k-steps, n-tiles, rows of a lane
   extern __shared__ uint8_t smem_raw[];
   __shared__ float2 s_scale[kStages][kStageTokens / 16];  // k_scale, v_scale of a stage's boxes
   __shared__ float s_m[kComputeWarps][8], s_l[kComputeWarps][8];
@@ -295,7 +302,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   const uint32_t t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const uint32_t ring = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t *ring_bytes = smem_raw + (ring - ptx::smem_u32(smem_raw));
-  float *merge = reinterpret_cast<float *>(ring_bytes + kRingBytes<BF16, DP>);  // [warp]: q as operands [k-step][lane][4 words], later a state [8 rows][DP]
+  float *merge = reinterpret_cast<float *>(ring_bytes + kRingBytes<MODE, DP>);  // [warp]: q as operands [k-step][lane][4 words], later a state [8 rows][DP]
   if (t == 0) {
     for (uint32_t s = 0; s < kStages; ++s) {
       ptx::mbar_init(ptx::smem_u32(&s_full[s]), 1);
@@ -435,7 +442,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   // ---------------------------------------------------------------- the computing warps
   const uint32_t g = lane >> 2, c = lane & 3;
   bool ok = true;
-  uint8_t *q_at = ring_bytes + kRingBytes<BF16, DP> + warp * (8 * DP * 4) + lane * 16;
+  uint8_t *q_at = ring_bytes + kRingBytes<MODE, DP> + warp * (8 * DP * 4) + lane * 16;
   // Tokens of a lane's accumulators: tile j, columns 2c and 2c + 1. With 64-byte rows the order below keeps two rows of a 128-byte
   // line together, which the swizzle then spreads over all banks.
   auto token_of = [&](uint32_t j, uint32_t col) { return DP == 128 ? 8 * j + col : 4 * (col >> 1) + 2 * j + (col & 1); };
@@ -509,8 +516,12 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         if (BF16) {  // this row's two of the four operand words
           a[0][0] = halves(x[kt][0] * down, x[kt][1] * down);
           a[0][1] = halves(x[kt][2] * down, x[kt][3] * down);
-          *reinterpret_cast<uint32_t *>(q_at + kt * 512 + 4 * i) = a[0][0];
-          *reinterpret_cast<uint32_t *>(q_at + kt * 512 + 4 * (2 + i)) = a[0][1];
+          if (MODE == kBf16Few) {
+            *reinterpret_cast<uint2 *>(q_at + kt * 512) = make_uint2(a[0][0], a[0][1]);
+          } else {
+            *reinterpret_cast<uint32_t *>(q_at + kt * 512 + 4 * i) = a[0][0];
+            *reinterpret_cast<uint32_t *>(q_at + kt * 512 + 4 * (2 + i)) = a[0][1];
+          }
         } else {
           split_halves(x[kt][0] * down, x[kt][1] * down, a[0][0], a[0][1]);
           split_halves(x[kt][2] * down, x[kt][3] * down, a[1][0], a[1][1]);
@@ -527,7 +538,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     const long long lo = (long long)part.rq.len - part.rq.q_len + warp_row / p.group + 1, hi = (long long)part.rq.len - part.rq.q_len + last_row / p.group + 1;
     const uint32_t see_all = (uint32_t)max(0ll, min(lo, (long long)part.rq.len));
     const uint32_t see_any = warp_row < part.rq.rows ? (uint32_t)max(0ll, min(hi, (long long)part.rq.len)) : 0u;
-    const bool second_rows = !BF16 || warp_row + 8 < part.rq.rows;  // bf16: whether rows 8 .. 15 of the warp are there
+    const bool second_rows = RW == 2 && warp_row + 8 < part.rq.rows;  // whether rows 8 .. 15 of the warp are there
 
     // Two boxes, 32 tokens, at a time. Where tokens are dealt to four warps, two of them share a stage and the pairs take turns; to two, each
     // takes a half. Every warp waits for every stage and gives it back, also one that has nothing to do with it: a wait names its phase by a
@@ -538,6 +549,11 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       ok = ok && ptx::mbar_wait_warp(a_full + 8 * slot, (stage / kStages) & 1, &s_abort);
       if (!ok) continue;
       const uint8_t *stage_at = ring_bytes + slot * 2 * 4 * kSubBytes<DP>;
+      auto give_back = [&]() {
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(a_empty + 8 * slot);
+      };
+      bool given_back = false;
       const bool idle = weight == 1 && ((tile - tile0) & 1) != token_warp >> 1;
       for (uint32_t pair = idle ? pair1 : pair0; pair < pair1; ++pair) {
         const uint32_t token0 = tile * kStageTokens + pair * 32;
@@ -556,8 +572,14 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           }
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
-            const uint4 q4 = *reinterpret_cast<const uint4 *>(q_at + (k4 * 4 + kk) * 512);
-            const uint32_t a[4] = {q4.x, q4.y, q4.z, q4.w};
+            uint32_t a[4];
+            if (MODE == kBf16Few) {
+              const uint2 q2 = *reinterpret_cast<const uint2 *>(q_at + (k4 * 4 + kk) * 512);
+              a[0] = q2.x; a[1] = 0u; a[2] = q2.y; a[3] = 0u;
+            } else {
+              const uint4 q4 = *reinterpret_cast<const uint4 *>(q_at + (k4 * 4 + kk) * 512);
+              a[0] = q4.x; a[1] = q4.y; a[2] = q4.z; a[3] = q4.w;
+            }
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt) {
               uint32_t b0, b1;
@@ -567,8 +589,32 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             }
           }
         }
-        // ---- weights
+        // ---- V's bytes: the stage is given back before the longer half of the work on it
         const bool masked = token0 + 32 > see_all;
+        uint32_t w[2][4][NT / 4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint8_t *at = v_at + b * kSubBytes<DP> + v_off[k];
+            if constexpr (DP == 128) {
+              const uint4 v = *reinterpret_cast<const uint4 *>(at);
+              w[b][k][0] = v.x; w[b][k][1] = v.y; w[b][k][2] = v.z; w[b][k][3] = v.w;
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2 *>(at);
+              w[b][k][0] = v.x; w[b][k][1] = v.y;
+            }
+            // behind the last token that a row sees a box may hold any bytes, and an 8-bit float may be NaN
+            if (FORMAT == DF_CACHE_E4M3 && masked && token0 + 16 * b + token_of(k >> 1, 2 * c + (k & 1)) >= see_any) {
+#pragma unroll
+              for (int n4 = 0; n4 < NT / 4; ++n4) w[b][k][n4] = 0u;
+            }
+          }
+        if (pair + 1 == pair1) {
+          give_back();
+          given_back = true;
+        }
+        // ---- weights
         // The two boxes' weights meet one scale of V, the larger one; a row that sees none of a box's tokens takes nothing of
         // it, whatever its scale is (it may be NaN).
         const float v_scale = fmaxf(scale[0].y, scale[1].y);
@@ -580,10 +626,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         for (int i = 0; i < RW; ++i) {
           before[i] = m[i];
           v_row[i] = 0.0f;
-          if (BF16 && i == 1 && !second_rows) {
-            pa[0][1] = pa[0][3] = pa[1][1] = pa[1][3] = 0u;
-            continue;
-          }
+          if (MODE == kBf16Few || (i == 1 && !second_rows)) pa[0][1] = pa[0][3] = pa[1][1] = pa[1][3] = 0u;
+          if (i == 1 && !second_rows) continue;
           const float f[2] = {scale[0].x * norm[i], scale[1].x * norm[i]};
           float s[4][2];
 #pragma unroll
@@ -639,25 +683,6 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           }
         }
         // ---- output
-        uint32_t w[2][4][NT / 4];
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint8_t *at = v_at + b * kSubBytes<DP> + v_off[k];
-            if constexpr (DP == 128) {
-              const uint4 v = *reinterpret_cast<const uint4 *>(at);
-              w[b][k][0] = v.x; w[b][k][1] = v.y; w[b][k][2] = v.z; w[b][k][3] = v.w;
-            } else {
-              const uint2 v = *reinterpret_cast<const uint2 *>(at);
-              w[b][k][0] = v.x; w[b][k][1] = v.y;
-            }
-            // behind the last token that a row sees a box may hold any bytes, and an 8-bit float may be NaN
-            if (FORMAT == DF_CACHE_E4M3 && masked && token0 + 16 * b + token_of(k >> 1, 2 * c + (k & 1)) >= see_any) {
-#pragma unroll
-              for (int n4 = 0; n4 < NT / 4; ++n4) w[b][k][n4] = 0u;
-            }
-          }
 #pragma unroll
         for (int n4 = 0; n4 < NT / 4; ++n4) {
           uint32_t b0[2][4], b1[2][4];
@@ -667,22 +692,21 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             widen_pairs<FORMAT>(w[b][2][n4], w[b][3][n4], b1[b]);
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float d[4];
-            mma_half_first(d, pa[0], b0[0][k], b1[0][k]);
-            mma_half(d, pa[1], b0[1][k], b1[1][k]);
-            const int n = n4 * 4 + k;
-            if (BF16) {
-              o[0][n] = ptx::fma2(make_float2(v_row[0], v_row[0]), make_float2(d[0], d[1]), o[0][n]);
-              if (second_rows) o[RW - 1][n] = ptx::fma2(make_float2(v_row[RW - 1], v_row[RW - 1]), make_float2(d[2], d[3]), o[RW - 1][n]);
-            } else {
-              o[0][n] = ptx::fma2(make_float2(v_row[0], v_row[0]), ptx::add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])), o[0][n]);
+            for (int k = 0; k < 4; ++k) {
+              float d[4];
+              mma_half_first(d, pa[0], b0[0][k], b1[0][k]);
+              mma_half(d, pa[1], b0[1][k], b1[1][k]);
+              const int n = n4 * 4 + k;
+              if (BF16) {
+                o[0][n] = ptx::fma2(make_float2(v_row[0], v_row[0]), make_float2(d[0], d[1]), o[0][n]);
+                if (RW == 2 && second_rows) o[RW - 1][n] = ptx::fma2(make_float2(v_row[RW - 1], v_row[RW - 1]), make_float2(d[2], d[3]), o[RW - 1][n]);
+              } else {
+                o[0][n] = ptx::fma2(make_float2(v_row[0], v_row[0]), ptx::add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])), o[0][n]);
+              }
             }
-          }
         }
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(a_empty + 8 * slot);
+      if (!given_back) give_back();
     }
     if (!ok && lane == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
 #pragma unroll
@@ -700,7 +724,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     const bool split = part.parts > 1;
     const uint32_t rows = min(part.rq.rows - part.row0, weight * ROWS);
     auto state_of = [&](uint32_t cta) {  // the first CTA of a segment has it last, every other one first
-      return p.partial + (size_t)(2 * cta + (cta == part.first_cta ? 1 : 0)) * kPartialFloats<BF16, DP>;
+      return p.partial + (size_t)(2 * cta + (cta == part.first_cta ? 1 : 0)) * kPartialFloats<MODE, DP>;
     };
     auto finish_row = [&](size_t row, uint32_t dim, const float4 &x, float mm, float ll) {  // four dims of a finished row
       const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
@@ -809,17 +833,17 @@ struct DeviceInfo {
 };
 
 // CTAs that the device keeps resident, asked once per kernel and device.
-template <bool BF16, int FORMAT, int DP>
+template <Mode MODE, int FORMAT, int DP>
 uint32_t resident_ctas() {
   static DeviceInfo table[64];
   int dev = 0;
   if (check_cuda(cudaGetDevice(&dev)) != DF_OK || dev < 0 || dev >= 64) return 0;
   DeviceInfo &d = table[dev];
   std::call_once(d.once, [&]() {
-    auto kernel = k_cache_attention<BF16, FORMAT, DP>;
+    auto kernel = k_cache_attention<MODE, FORMAT, DP>;
     int per_sm = 0, n_sm = 0;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes<BF16, DP>) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, (int)kThreads, kSmemBytes<BF16, DP>) != cudaSuccess ||
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes<MODE, DP>) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, (int)kThreads, kSmemBytes<MODE, DP>) != cudaSuccess ||
         cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
       return;
     d.grid = (uint32_t)(per_sm * n_sm);
@@ -839,24 +863,24 @@ bool encode_pool_map(CUtensorMap *map, const void *pool, const AttendParams &p) 
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool BF16, int FORMAT, int DP>
+template <Mode MODE, int FORMAT, int DP>
 int launch(AttendParams &p, const void *k_cache, const void *v_cache, cudaStream_t s) {
-  constexpr uint32_t kFits = (DF_CACHE_WORKSPACE_BYTES - kCounterBytes) / (2 * kPartialFloats<BF16, DP> * 4);
+  constexpr uint32_t kFits = (DF_CACHE_WORKSPACE_BYTES - kCounterBytes) / (2 * kPartialFloats<MODE, DP> * 4);
   static_assert(kFits >= 2 * 148 && kMaxGrid * 4 <= kCounterBytes, "workspace");
-  uint32_t grid = resident_ctas<BF16, FORMAT, DP>();
+  uint32_t grid = resident_ctas<MODE, FORMAT, DP>();
   if (grid == 0) return DF_ERR_CUDA;
   grid = grid < kFits ? grid : kFits;
   grid = grid < kMaxGrid ? grid : kMaxGrid;
   CUtensorMap k_map, v_map;
   if (!encode_pool_map(&k_map, k_cache, p) || !encode_pool_map(&v_map, v_cache, p)) return DF_ERR_CUDA;
-  const int st = check_cuda(launch_kernel(k_cache_attention<BF16, FORMAT, DP>, dim3(grid), dim3(kThreads), kSmemBytes<BF16, DP>, s, k_map, v_map, p));
+  const int st = check_cuda(launch_kernel(k_cache_attention<MODE, FORMAT, DP>, dim3(grid), dim3(kThreads), kSmemBytes<MODE, DP>, s, k_map, v_map, p));
   note_launch();
   return st;
 }
 
-template <bool BF16, int FORMAT>
+template <Mode MODE, int FORMAT>
 int launch_for_head(AttendParams &p, const void *k_cache, const void *v_cache, cudaStream_t s) {
-  return p.D <= 64 ? launch<BF16, FORMAT, 64>(p, k_cache, v_cache, s) : launch<BF16, FORMAT, 128>(p, k_cache, v_cache, s);
+  return p.D <= 64 ? launch<MODE, FORMAT, 64>(p, k_cache, v_cache, s) : launch<MODE, FORMAT, 128>(p, k_cache, v_cache, s);
 }
 
 int finish(int st) {
@@ -912,7 +936,13 @@ extern "C" int df_cache_attention(const void *q, const void *k_cache, const void
   p.out_aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
   p.scale_log2 = scale * kLog2e;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (q_bf16)
-    return finish(format == DF_CACHE_INT8 ? launch_for_head<true, DF_CACHE_INT8>(p, k_cache, v_cache, s) : launch_for_head<true, DF_CACHE_E4M3>(p, k_cache, v_cache, s));
-  return finish(format == DF_CACHE_INT8 ? launch_for_head<false, DF_CACHE_INT8>(p, k_cache, v_cache, s) : launch_for_head<false, DF_CACHE_E4M3>(p, k_cache, v_cache, s));
+  // Eight bf16 rows to a warp while requests have no more on average: what the kernel is then bound by is the latency of a
+  // warp's steps, and with half the accumulators twice the warps fit an SM.
+  const bool few = (uint64_t)n_tokens * p.group <= 8ull * n_requests;
+  auto run = [&](auto format_constant) {
+    constexpr int FORMAT = decltype(format_constant)::value;
+    if (!q_bf16) return launch_for_head<kFp32, FORMAT>(p, k_cache, v_cache, s);
+    return few ? launch_for_head<kBf16Few, FORMAT>(p, k_cache, v_cache, s) : launch_for_head<kBf16, FORMAT>(p, k_cache, v_cache, s);
+  };
+  return finish(format == DF_CACHE_INT8 ? run(std::integral_constant<int, DF_CACHE_INT8>{}) : run(std::integral_constant<int, DF_CACHE_E4M3>{}));
 }
