@@ -55,6 +55,7 @@ struct AttendParams {
   unsigned long long q_stride;
   uint32_t n_requests, n_tokens, heads, kv_heads, group, D, P, n_pages, width;
   uint32_t q_aligned, out_aligned;  // 16-byte boundaries
+  uint32_t whole;  // the line would be too long in units
   float scale_log2;
 };
 
@@ -69,7 +70,7 @@ constexpr uint32_t kPartialFloats = kComputeWarps * kRows<MODE> * (DP + 2);
 
 struct Request {
   uint32_t first, rows, q_len, len, tiles, row_tiles;
-  uint32_t weight;  // warps that the rows of a tile are dealt to (1, 2, 4; the tokens to the others): units of a stage
+  uint32_t weight_log2;  // warps that the rows of a tile are dealt to (1, 2, 4; the tokens to the others): units of a stage
 };
 
 template <uint32_t ROWS>
@@ -81,8 +82,8 @@ __device__ __forceinline__ Request request_of(const AttendParams &p, uint32_t r)
   q.first = (uint32_t)b;
   q.q_len = (uint32_t)(e - b);
   q.rows = q.q_len * p.group;
-  q.weight = q.rows <= ROWS ? 1u : q.rows <= 2 * ROWS ? 2u : kComputeWarps;
-  q.row_tiles = (q.rows + q.weight * ROWS - 1) / (q.weight * ROWS);
+  q.weight_log2 = q.rows <= ROWS ? 0u : q.rows <= 2 * ROWS ? 1u : 2u;
+  q.row_tiles = (q.rows + (ROWS << q.weight_log2) - 1) / ROWS >> q.weight_log2;
   q.tiles = max(1u, (q.len + kStageTokens - 1) / kStageTokens);
   return q;
 }
@@ -96,11 +97,11 @@ struct Part {
   uint32_t parts, first_cta;     // of the whole segment
 };
 
-// The line of units (or, where no segment is cut, of segments) and this CTA's place on it.
+// The line of units (or, where no segment is cut, of segments) and this CTA's place on it. Its length is below 2^31 (the launcher sees to
+// it), so that its divisions are of 32 bits: those of 64 took a part's first microseconds.
 struct Line {
-  unsigned long long at, end, base;  // base: of request r
-  unsigned long long per_cta;
-  uint32_t r;
+  uint32_t at, end, base;  // base: of request r
+  uint32_t per_cta, r;
   bool whole;  // counted in segments
 };
 
@@ -108,41 +109,40 @@ template <uint32_t ROWS>
 __device__ __forceinline__ bool next_part(const AttendParams &p, Line &line, Part &part) {
   while (line.at < line.end) {
     Request q = request_of<ROWS>(p, line.r);
-    unsigned long long span = line.whole ? 1ull : (unsigned long long)q.tiles * q.weight;
+    uint32_t span = line.whole ? 1u : q.tiles << q.weight_log2;
     while (line.at >= line.base + span * q.row_tiles * p.kv_heads) {  // on to the request that holds line.at (it is below the line's end)
       line.base += span * q.row_tiles * p.kv_heads;
       q = request_of<ROWS>(p, ++line.r);
-      span = line.whole ? 1ull : (unsigned long long)q.tiles * q.weight;
+      span = line.whole ? 1u : q.tiles << q.weight_log2;
     }
-    const uint32_t idx = (uint32_t)((line.at - line.base) / span);
-    const unsigned long long s0 = line.base + idx * span, s1 = s0 + span;
+    const uint32_t idx = line.whole ? line.at - line.base : (line.at - line.base) / span;
+    const uint32_t s0 = line.base + idx * span, s1 = s0 + span;
+    const uint32_t row_tile = q.row_tiles == 1 ? 0u : idx / p.kv_heads;
     part.rq = q;
     part.r = line.r;
-    part.h = idx % p.kv_heads;
-    part.row0 = idx / p.kv_heads * (q.weight * ROWS);
+    part.h = idx - row_tile * p.kv_heads;
+    part.row0 = row_tile * (ROWS << q.weight_log2);
     part.parts = 1;
     part.first_cta = blockIdx.x;
     part.t0 = 0;
     part.t1 = q.tiles;
-    if (line.whole) {
-      line.at = s1;
-    } else {
-      const unsigned long long stop = min(s1, line.end);
-      part.t0 = (uint32_t)((line.at - s0) / q.weight);
-      if (stop < s1) part.t1 = (uint32_t)((stop - s0) / q.weight);
+    const uint32_t from = line.at, stop = min(s1, line.end);
+    line.at = stop;
+    if (from != s0 || stop != s1) {  // cut
+      part.t0 = (from - s0) >> q.weight_log2;
+      if (stop < s1) part.t1 = (stop - s0) >> q.weight_log2;
       // A boundary between CTAs counts down to whole stages; so the first CTA that a segment reaches may have none of it (a unit is a
       // quarter of a stage where rows are dealt, and a CTA has at least four units), every other one has some.
-      uint32_t c0 = (uint32_t)(s0 / line.per_cta);
-      const uint32_t c1 = (uint32_t)((s1 - 1) / line.per_cta);
-      if (((c0 + 1ull) * line.per_cta - s0) / q.weight == 0) ++c0;
+      uint32_t c0 = s0 / line.per_cta;
+      const uint32_t c1 = (s1 - 1) / line.per_cta;
+      if (((c0 + 1) * line.per_cta - s0) >> q.weight_log2 == 0) ++c0;
       part.first_cta = c0;
       part.parts = c1 - c0 + 1;
-      line.at = stop;
       if (part.t1 <= part.t0) continue;
     }
-    const uint32_t last_row = min(q.rows, part.row0 + q.weight * ROWS) - 1;
-    const long long see = (long long)q.len - q.q_len + last_row / p.group + 1;
-    part.limit = (uint32_t)max(0ll, min(see, (long long)q.len));
+    const uint32_t last_row = min(q.rows, part.row0 + (ROWS << q.weight_log2)) - 1;
+    const int see = (int)q.len - (int)q.q_len + (int)(p.group == 1 ? last_row : last_row / p.group) + 1;
+    part.limit = (uint32_t)max(0, min(see, (int)q.len));
     part.t1 = max(part.t0, min(part.t1, (part.limit + kStageTokens - 1) / kStageTokens));
     return true;
   }
@@ -297,8 +297,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   __shared__ Line s_line[kComputeWarps];
   __shared__ Part s_part[kComputeWarps];
   __shared__ uint64_t s_full[kStages], s_empty[kStages];
-  __shared__ unsigned long long s_sum[kThreads / 32][2], s_place[2];
-  __shared__ uint32_t s_most[kThreads / 32], s_request, s_last, s_abort;
+  __shared__ uint32_t s_units[kThreads], s_segments[kThreads], s_most[kThreads / 32], s_last, s_abort;
   const uint32_t t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const uint32_t ring = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t *ring_bytes = smem_raw + (ring - ptx::smem_u32(smem_raw));
@@ -317,56 +316,51 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 
   // ---- the line: sums over the requests, and the request at which this CTA begins
   const uint32_t per = (p.n_requests + kThreads - 1) / kThreads, r0 = min(p.n_requests, t * per), r1 = min(p.n_requests, r0 + per);
-  unsigned long long units = 0, segments = 0;
-  uint32_t most = 0;
+  uint32_t units = 0, segments = 0, most = 0;
   for (uint32_t r = r0; r < r1; ++r) {
     const Request q = request_of<ROWS>(p, r);
-    const unsigned long long n = (unsigned long long)q.row_tiles * p.kv_heads;
+    const uint32_t n = q.row_tiles * p.kv_heads;
     segments += n;
-    units += n * q.tiles * q.weight;
-    if (n) most = max(most, q.tiles * q.weight);
+    units += n * (q.tiles << q.weight_log2);
+    if (n) most = max(most, q.tiles << q.weight_log2);
   }
-  unsigned long long in_units = units, in_segments = segments;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long a = __shfl_up_sync(0xffffffffu, in_units, o), b = __shfl_up_sync(0xffffffffu, in_segments, o);
-    if (lane >= (uint32_t)o) { in_units += a; in_segments += b; }
+    const uint32_t a = __shfl_up_sync(0xffffffffu, units, o), b = __shfl_up_sync(0xffffffffu, segments, o);
+    if (lane >= (uint32_t)o) { units += a; segments += b; }
   }
   most = __reduce_max_sync(0xffffffffu, most);
-  if (lane == 31) { s_sum[warp][0] = in_units; s_sum[warp][1] = in_segments; s_most[warp] = most; }
+  s_units[t] = units;
+  s_segments[t] = segments;
+  if (lane == 0) s_most[warp] = most;
   __syncthreads();
-  unsigned long long all_units = 0, all_segments = 0, my_units = 0, my_segments = 0;
+  uint32_t all_units = 0, all_segments = 0;
+  most = 0;
+#pragma unroll
   for (uint32_t w = 0; w < kThreads / 32; ++w) {
-    if (w == warp) { my_units = all_units + in_units - units; my_segments = all_segments + in_segments - segments; }
-    all_units += s_sum[w][0];
-    all_segments += s_sum[w][1];
+    all_units += s_units[32 * w + 31];
+    all_segments += s_segments[32 * w + 31];
     most = max(most, s_most[w]);
   }
   Line line;
-  const unsigned long long G = gridDim.x, seg_per = (all_segments + G - 1) / G, unit_per = max(8ull, (all_units + G - 1) / G);
-  line.whole = seg_per * most <= unit_per + kSplitUnits;
+  const uint32_t G = gridDim.x, seg_per = (all_segments + G - 1) / G, unit_per = max(8u, (all_units + G - 1) / G);
+  line.whole = p.whole || (unsigned long long)seg_per * most <= unit_per + kSplitUnits;
   line.per_cta = line.whole ? seg_per : unit_per;
-  const unsigned long long total = line.whole ? all_segments : all_units;
+  const uint32_t total = line.whole ? all_segments : all_units;
+  if ((unsigned long long)line.per_cta * blockIdx.x >= total) return;  // (the whole CTA)
   line.at = line.per_cta * blockIdx.x;
   line.end = min(total, line.at + line.per_cta);
-  if (line.at >= line.end) return;  // (the whole CTA)
-  unsigned long long base = line.whole ? my_segments : my_units;
-  const unsigned long long mine = line.whole ? segments : units;
-  if (line.at >= base && line.at < base + mine) {
-    for (uint32_t r = r0; r < r1; ++r) {
-      const Request q = request_of<ROWS>(p, r);
-      const unsigned long long n = (unsigned long long)q.row_tiles * p.kv_heads * (line.whole ? 1u : q.tiles * q.weight);
-      if (line.at < base + n) {
-        s_request = r;
-        s_place[0] = base;
-        break;
-      }
-      base += n;
-    }
+  // the warp, then the lane, then the request of those lane's that line.at falls to: every warp looks for itself
+  {
+    const uint32_t *sums = line.whole ? s_segments : s_units;
+    uint32_t base = 0, w = 0;
+    while (line.at >= base + sums[32 * w + 31]) base += sums[32 * w++ + 31];
+    const uint32_t mine = base + sums[32 * w + lane];
+    const uint32_t owner = __ffs(__ballot_sync(0xffffffffu, line.at < mine)) - 1;
+    const uint32_t before = __shfl_sync(0xffffffffu, mine, max(owner, 1u) - 1);
+    line.base = owner == 0 ? base : before;
+    line.r = (32 * w + owner) * per;  // next_part goes on to the request
   }
-  __syncthreads();
-  line.r = s_request;
-  line.base = s_place[0];
 
   const uint32_t a_full = ptx::smem_u32(&s_full[0]), a_empty = ptx::smem_u32(&s_empty[0]);
   const uint32_t chunks = p.D / 16;  // 16-byte pieces of a row
@@ -474,8 +468,10 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     __syncwarp();
     const Part &part = s_part[warp];
     const uint32_t tile0 = found.t0, tile1 = found.t1;
-    const uint32_t weight = part.rq.weight, row_warp = warp & (weight - 1), token_warp = weight == 1 ? warp : weight == 2 ? warp >> 1 : 0u;
+    const uint32_t weight = 1u << part.rq.weight_log2, row_warp = warp & (weight - 1), token_warp = warp >> part.rq.weight_log2;
     const uint32_t warp_row = part.row0 + row_warp * ROWS;
+    const int behind = (int)part.rq.len - (int)part.rq.q_len + 1, most_seen = (int)part.rq.len;
+    auto see_of = [&](uint32_t j) { return (uint32_t)max(0, min(behind + (int)j, most_seen)); };  // tokens that query token j sees
     // rows of this lane
     uint32_t see[RW];
     bool valid[RW];
@@ -486,9 +482,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     for (int i = 0; i < RW; ++i) {
       const uint32_t row = warp_row + g + 8 * i;
       valid[i] = row < part.rq.rows;
-      const uint32_t j = row / p.group, head = part.h * p.group + row % p.group;
-      const long long n = (long long)part.rq.len - part.rq.q_len + j + 1;
-      see[i] = valid[i] ? (uint32_t)max(0ll, min(n, (long long)part.rq.len)) : 0u;
+      const uint32_t j = p.group == 1 ? row : row / p.group, head = part.h * p.group + row - j * p.group;
+      see[i] = valid[i] ? see_of(j) : 0u;
       const unsigned long long e = (unsigned long long)(part.rq.first + j) * p.q_stride + (unsigned long long)head * p.D + c * (DP / 4);
       float x[KT][4];
       float top = 0.0f;
@@ -535,9 +530,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     }
     // what the warp's rows see, at least and at most: rows are in the order of their tokens
     const uint32_t last_row = min(part.rq.rows, warp_row + ROWS) - 1;
-    const long long lo = (long long)part.rq.len - part.rq.q_len + warp_row / p.group + 1, hi = (long long)part.rq.len - part.rq.q_len + last_row / p.group + 1;
-    const uint32_t see_all = (uint32_t)max(0ll, min(lo, (long long)part.rq.len));
-    const uint32_t see_any = warp_row < part.rq.rows ? (uint32_t)max(0ll, min(hi, (long long)part.rq.len)) : 0u;
+    const uint32_t see_all = see_of(p.group == 1 ? warp_row : warp_row / p.group);
+    const uint32_t see_any = warp_row < part.rq.rows ? see_of(p.group == 1 ? last_row : last_row / p.group) : 0u;
     const bool second_rows = RW == 2 && warp_row + 8 < part.rq.rows;  // whether rows 8 .. 15 of the warp are there
 
     // Two boxes, 32 tokens, at a time. Where tokens are dealt to four warps, two of them share a stage and the pairs take turns; to two, each
@@ -734,7 +728,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     };
     auto global_row = [&](uint32_t row) {
       const uint32_t rr = part.row0 + row;
-      return (size_t)(part.rq.first + rr / p.group) * p.heads + part.h * p.group + rr % p.group;
+      const uint32_t j = p.group == 1 ? rr : rr / p.group;
+      return (size_t)(part.rq.first + j) * p.heads + part.h * p.group + rr - j * p.group;
     };
     float *mine_state = state_of(blockIdx.x), *mine_o = mine_state + 2 * kComputeWarps * ROWS;
     if (weight == kComputeWarps) {
@@ -779,16 +774,15 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       }
     }
     if (split) {
-      __threadfence();
       compute_barrier();
-      if (t == 0) {
-        s_last = atomicAdd(p.counters + part.first_cta, 1u) + 1 == part.parts;
+      if (t == 0) {  // releases what the barrier has gathered, and acquires what the CTAs before have released
+        unsigned int arrived;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(arrived) : "l"(p.counters + part.first_cta) : "memory");
+        s_last = arrived + 1 == part.parts;
         if (s_last) p.counters[part.first_cta] = 0;  // ready for the next call
-        __threadfence();
       }
       compute_barrier();
       if (s_last) {
-        __threadfence();
         const uint32_t elements = rows * (DP / 4), ways = max(1u, 32 * kComputeWarps / elements);
         // thread: four dims of a row, and every `ways`-th part where there are fewer of them than threads
         const uint32_t e0 = ways > 1 ? t % elements : t, way = ways > 1 ? t / elements : 0;
@@ -899,7 +893,8 @@ extern "C" int df_cache_attention(const void *q, const void *k_cache, const void
                                   uint32_t d_head, uint32_t page_size, uint32_t n_pages, uint32_t table_width, uint64_t q_row_stride, float scale,
                                   uint32_t q_bf16, uint32_t format, void *stream) {
   DF_RANGE("df_cache_attention");
-  if (!cache_shape_valid(n_kv_heads, d_head, page_size, n_pages) || n_requests >= (1u << 31)) return finish(DF_ERR_INVALID_ARG);
+  if (!cache_shape_valid(n_kv_heads, d_head, page_size, n_pages) || (uint64_t)n_requests * n_kv_heads >= (1ull << 30))
+    return finish(DF_ERR_INVALID_ARG);
   if (format != DF_CACHE_INT8 && format != DF_CACHE_E4M3) return finish(DF_ERR_INVALID_ARG);
   if (n_heads == 0 || n_heads % n_kv_heads != 0 || !isfinite(scale) || (uint64_t)n_tokens * n_heads >= (1ull << 31)) return finish(DF_ERR_INVALID_ARG);
   if (n_tokens > 1 && q_row_stride < (uint64_t)n_heads * d_head) return finish(DF_ERR_INVALID_ARG);
@@ -932,6 +927,9 @@ extern "C" int df_cache_attention(const void *q, const void *k_cache, const void
   p.P = page_size;
   p.n_pages = n_pages;
   p.width = table_width;
+  // what the line's units can add up to: segments (row tiles of at least eight rows, times K/V heads) of at most the table's width
+  const uint64_t longest = ((uint64_t)table_width * page_size + kStageTokens - 1) / kStageTokens * kComputeWarps;
+  p.whole = ((uint64_t)n_tokens * p.group / 8 + n_requests) * n_kv_heads * (longest ? longest : 1) >= (1ull << 31);
   p.q_aligned = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(q_row_stride * (q_bf16 ? 2 : 4))) & 15u) == 0;
   p.out_aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
   p.scale_log2 = scale * kLog2e;
