@@ -40,7 +40,6 @@ using ptx::ex2_approx;
 constexpr uint32_t kStageTokens = 64, kComputeWarps = 4, kThreads = 32 * (kComputeWarps + 1);
 constexpr float kWeightBits = 15.0f;  // weights are held times 2^15, so that halves reach down to 2^-39 of the largest one
 constexpr uint32_t kMaxGrid = 640;
-constexpr uint32_t kSplitUnits = 6;  // what cutting segments costs, in units
 constexpr uint32_t kCounterBytes = 4096;  // a counter per CTA, at the workspace's beginning
 
 struct AttendParams {
@@ -97,6 +96,18 @@ struct Part {
   uint32_t parts, first_cta;     // of the whole segment
 };
 
+// What a segment costs besides its stages (its rows of q, the sums over warps, its results), in units: 5 to 8 us beside 1.2 us for a stage of 128-byte
+// tokens with every SM busy. Counted at the segment's beginning; without it CTAs with several short segments ended 20 us after the others
+// (32 ragged requests: 94 us, 77 with it).
+template <int DP>
+constexpr uint32_t kSegmentUnits = DP == 128 ? 6 : 10;
+template <int DP>
+__device__ __forceinline__ uint32_t span_of(const Request &q) { return (q.tiles << q.weight_log2) + kSegmentUnits<DP>; }
+template <int DP>
+__device__ __forceinline__ uint32_t tile_at(const Request &q, uint32_t x) {  // stages of a segment in front of its unit x
+  return x <= kSegmentUnits<DP> ? 0u : (x - kSegmentUnits<DP>) >> q.weight_log2;
+}
+
 // The line of units (or, where no segment is cut, of segments) and this CTA's place on it. Its length is below 2^31 (the launcher sees to
 // it), so that its divisions are of 32 bits: those of 64 took a part's first microseconds.
 struct Line {
@@ -105,15 +116,15 @@ struct Line {
   bool whole;  // counted in segments
 };
 
-template <uint32_t ROWS>
+template <uint32_t ROWS, int DP>
 __device__ __forceinline__ bool next_part(const AttendParams &p, Line &line, Part &part) {
   while (line.at < line.end) {
     Request q = request_of<ROWS>(p, line.r);
-    uint32_t span = line.whole ? 1u : q.tiles << q.weight_log2;
+    uint32_t span = line.whole ? 1u : span_of<DP>(q);
     while (line.at >= line.base + span * q.row_tiles * p.kv_heads) {  // on to the request that holds line.at (it is below the line's end)
       line.base += span * q.row_tiles * p.kv_heads;
       q = request_of<ROWS>(p, ++line.r);
-      span = line.whole ? 1u : q.tiles << q.weight_log2;
+      span = line.whole ? 1u : span_of<DP>(q);
     }
     const uint32_t idx = line.whole ? line.at - line.base : (line.at - line.base) / span;
     const uint32_t s0 = line.base + idx * span, s1 = s0 + span;
@@ -129,13 +140,13 @@ __device__ __forceinline__ bool next_part(const AttendParams &p, Line &line, Par
     const uint32_t from = line.at, stop = min(s1, line.end);
     line.at = stop;
     if (from != s0 || stop != s1) {  // cut
-      part.t0 = (from - s0) >> q.weight_log2;
-      if (stop < s1) part.t1 = (stop - s0) >> q.weight_log2;
-      // A boundary between CTAs counts down to whole stages; so the first CTA that a segment reaches may have none of it (a unit is a
-      // quarter of a stage where rows are dealt, and a CTA has at least four units), every other one has some.
+      part.t0 = tile_at<DP>(q, from - s0);
+      if (stop < s1) part.t1 = tile_at<DP>(q, stop - s0);
+      // A boundary between CTAs counts down to whole stages; so the first CTA that a segment reaches may have none of it, every other one has
+      // some (a CTA has at least four units more than a segment's beginning takes).
       uint32_t c0 = s0 / line.per_cta;
       const uint32_t c1 = (s1 - 1) / line.per_cta;
-      if (((c0 + 1) * line.per_cta - s0) >> q.weight_log2 == 0) ++c0;
+      if (tile_at<DP>(q, (c0 + 1) * line.per_cta - s0) == 0) ++c0;
       part.first_cta = c0;
       part.parts = c1 - c0 + 1;
       if (part.t1 <= part.t0) continue;
@@ -204,34 +215,40 @@ __device__ __forceinline__ void split_halves(float x, float y, uint32_t &first, 
   second = halves(x - f.x, y - f.y);
 }
 
+// Four elements of a row of q, as they lie there.
 template <bool BF16>
-__device__ __forceinline__ void load_row4(const void *q, unsigned long long e, bool aligned, float (&x)[4]) {
-  if (BF16) {
-    const uint16_t *p = static_cast<const uint16_t *>(q) + e;
-    uint32_t lo, hi;
-    if (aligned) {
-      const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
-      lo = w.x;
-      hi = w.y;
+struct Raw4 {
+  uint32_t w[BF16 ? 2 : 4];
+  __device__ __forceinline__ void load(const void *q, unsigned long long e, bool aligned) {
+    if constexpr (BF16) {
+      const uint16_t *p = static_cast<const uint16_t *>(q) + e;
+      if (aligned) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+        w[0] = v.x; w[1] = v.y;
+      } else {
+        w[0] = __ldg(p) | ((uint32_t)__ldg(p + 1) << 16);
+        w[1] = __ldg(p + 2) | ((uint32_t)__ldg(p + 3) << 16);
+      }
     } else {
-      lo = __ldg(p) | ((uint32_t)__ldg(p + 1) << 16);
-      hi = __ldg(p + 2) | ((uint32_t)__ldg(p + 3) << 16);
-    }
-    x[0] = __uint_as_float(lo << 16);
-    x[1] = __uint_as_float(lo & 0xffff0000u);
-    x[2] = __uint_as_float(hi << 16);
-    x[3] = __uint_as_float(hi & 0xffff0000u);
-  } else {
-    const float *p = static_cast<const float *>(q) + e;
-    if (aligned) {
-      const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
-      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
+      const uint32_t *p = static_cast<const uint32_t *>(q) + e;
+      if (aligned) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __ldg(p + i);
+        for (int i = 0; i < 4; ++i) w[i] = __ldg(p + i);
+      }
     }
   }
-}
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (uint32_t &x : w) x = 0u;
+  }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (BF16) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else return __uint_as_float(w[i]);
+  }
+};
 
 template <bool BF16>
 __device__ __forceinline__ void store_row4(void *out, size_t e, bool aligned, const float (&x)[4]) {
@@ -321,8 +338,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     const Request q = request_of<ROWS>(p, r);
     const uint32_t n = q.row_tiles * p.kv_heads;
     segments += n;
-    units += n * (q.tiles << q.weight_log2);
-    if (n) most = max(most, q.tiles << q.weight_log2);
+    units += n * span_of<DP>(q);
+    if (n) most = max(most, span_of<DP>(q));
   }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -343,8 +360,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     most = max(most, s_most[w]);
   }
   Line line;
-  const uint32_t G = gridDim.x, seg_per = (all_segments + G - 1) / G, unit_per = max(8u, (all_units + G - 1) / G);
-  line.whole = p.whole || (unsigned long long)seg_per * most <= unit_per + kSplitUnits;
+  const uint32_t G = gridDim.x, seg_per = (all_segments + G - 1) / G, unit_per = max(kSegmentUnits<DP> + 8u, (all_units + G - 1) / G);
+  line.whole = p.whole || (unsigned long long)seg_per * most <= unit_per + kSegmentUnits<DP>;  // cutting costs another end
   line.per_cta = line.whole ? seg_per : unit_per;
   const uint32_t total = line.whole ? all_segments : all_units;
   if ((unsigned long long)line.per_cta * blockIdx.x >= total) return;  // (the whole CTA)
@@ -382,7 +399,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       gr.stages = 0;
       if (tile >= part.t1) {
         do {
-          if (!next_part<ROWS>(p, line, part)) return;
+          if (!next_part<ROWS, DP>(p, line, part)) return;
         } while (part.t0 >= part.t1);  // a part that sees nothing
         tile = part.t0;
       }
@@ -460,7 +477,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     Line next = s_line[warp];
     __syncwarp();
     Part found;
-    if (!next_part<ROWS>(p, next, found)) break;
+    if (!next_part<ROWS, DP>(p, next, found)) break;
     if (lane == 0) {
       s_line[warp] = next;
       s_part[warp] = found;
@@ -478,6 +495,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     float norm[RW], m[RW], l[RW];
     float2 o[RW][NT];  // columns 2c, 2c + 1 of n-tile n: dims 2c * DP/8 + n and (2c + 1) * DP/8 + n
     __syncwarp();  // the region below was read as a merge buffer by this warp's lanes alone, behind a barrier
+    Raw4<BF16> raw[RW][KT];  // all loads first: they come from DRAM
 #pragma unroll
     for (int i = 0; i < RW; ++i) {
       const uint32_t row = warp_row + g + 8 * i;
@@ -485,19 +503,19 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       const uint32_t j = p.group == 1 ? row : row / p.group, head = part.h * p.group + row - j * p.group;
       see[i] = valid[i] ? see_of(j) : 0u;
       const unsigned long long e = (unsigned long long)(part.rq.first + j) * p.q_stride + (unsigned long long)head * p.D + c * (DP / 4);
-      float x[KT][4];
-      float top = 0.0f;
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        if (valid[i] && c * (DP / 4) + kt * 4 < p.D) {
-          load_row4<BF16>(p.q, e + kt * 4, p.q_aligned, x[kt]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) x[kt][k] = 0.0f;
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top = fmaxf(top, fabsf(x[kt][k]));
+        if (valid[i] && c * (DP / 4) + kt * 4 < p.D) raw[i][kt].load(p.q, e + kt * 4, p.q_aligned);
+        else raw[i][kt].zero();
       }
+    }
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+      float top = 0.0f;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = fmaxf(top, fabsf(raw[i][kt].at(k)));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // the largest element to 1 .. 2 (an infinity or zero stays)
@@ -509,8 +527,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       for (int kt = 0; kt < KT; ++kt) {
         uint32_t a[2][2];
         if (BF16) {  // this row's two of the four operand words
-          a[0][0] = halves(x[kt][0] * down, x[kt][1] * down);
-          a[0][1] = halves(x[kt][2] * down, x[kt][3] * down);
+          a[0][0] = halves(raw[i][kt].at(0) * down, raw[i][kt].at(1) * down);
+          a[0][1] = halves(raw[i][kt].at(2) * down, raw[i][kt].at(3) * down);
           if (MODE == kBf16Few) {
             *reinterpret_cast<uint2 *>(q_at + kt * 512) = make_uint2(a[0][0], a[0][1]);
           } else {
@@ -518,8 +536,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             *reinterpret_cast<uint32_t *>(q_at + kt * 512 + 4 * (2 + i)) = a[0][1];
           }
         } else {
-          split_halves(x[kt][0] * down, x[kt][1] * down, a[0][0], a[0][1]);
-          split_halves(x[kt][2] * down, x[kt][3] * down, a[1][0], a[1][1]);
+          split_halves(raw[i][kt].at(0) * down, raw[i][kt].at(1) * down, a[0][0], a[0][1]);
+          split_halves(raw[i][kt].at(2) * down, raw[i][kt].at(3) * down, a[1][0], a[1][1]);
           *reinterpret_cast<uint4 *>(q_at + kt * 512) = make_uint4(a[0][0], a[0][1], a[1][0], a[1][1]);
         }
       }
@@ -746,6 +764,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         if (split && c == 0) *reinterpret_cast<float2 *>(mine_state + 2 * row) = make_float2(m[i], l[i]);
       }
     } else {
+      // Four dims of a row, at a place that keeps the lanes of a store in different banks.
+      auto spread = [&](uint32_t row, uint32_t d4) { return d4 ^ (((d4 >> (DP == 128 ? 3 : 2)) ^ (row << 2)) & (DP / 16 - 1)); };
       // the states of the warps that shared the tokens, eight rows of a warp at a time; a warp's is where its part of q was
 #pragma unroll
       for (int i = 0; i < RW; ++i) {
@@ -753,7 +773,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         if (valid[i]) {
           if (c == 0) { s_m[warp][g] = m[i]; s_l[warp][g] = l[i]; }
 #pragma unroll
-          for (int n = 0; n < DP / 4; n += 4) *reinterpret_cast<float4 *>(merge + (warp * 8 + g) * DP + c * (DP / 4) + n) = four(i, n);
+          for (int n = 0; n < DP / 16; ++n) *reinterpret_cast<float4 *>(merge + (warp * 8 + g) * DP + 4 * spread(g, c * (DP / 16) + n)) = four(i, 4 * n);
         }
         compute_barrier();
         for (uint32_t e = t; e < weight * 8 * (DP / 4); e += 32 * kComputeWarps) {
@@ -761,7 +781,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           if (row >= rows) break;
           Running sum;
           for (uint32_t w = w0; w < kComputeWarps; w += weight)
-            sum.add(s_m[w][r8], s_l[w][r8], *reinterpret_cast<const float4 *>(merge + (w * 8 + r8) * DP + dim));
+            sum.add(s_m[w][r8], s_l[w][r8], *reinterpret_cast<const float4 *>(merge + (w * 8 + r8) * DP + 4 * spread(r8, dim / 4)));
           const float4 x = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
           if (!split) {
             finish_row(global_row(row), dim, x, sum.m, sum.l);
@@ -929,7 +949,7 @@ extern "C" int df_cache_attention(const void *q, const void *k_cache, const void
   p.width = table_width;
   // what the line's units can add up to: segments (row tiles of at least eight rows, times K/V heads) of at most the table's width
   const uint64_t longest = ((uint64_t)table_width * page_size + kStageTokens - 1) / kStageTokens * kComputeWarps;
-  p.whole = ((uint64_t)n_tokens * p.group / 8 + n_requests) * n_kv_heads * (longest ? longest : 1) >= (1ull << 31);
+  p.whole = ((uint64_t)n_tokens * p.group / 8 + n_requests) * n_kv_heads * (longest + 16) >= (1ull << 31);
   p.q_aligned = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(q_row_stride * (q_bf16 ? 2 : 4))) & 15u) == 0;
   p.out_aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
   p.scale_log2 = scale * kLog2e;
