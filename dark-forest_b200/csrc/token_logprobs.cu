@@ -7,15 +7,16 @@
 // may be -inf). All sums in fp32.
 //
 // Both directions are bound by HBM: the forward reads every logit once, the gradient reads and writes it once. In the forward a row is cut
-// into slices, one for each CTA of a cluster, and a slice lies in the shared memory of its CTA, at most kUsual 16-byte groups a thread (52 KB: four CTAs
-// of an SM load and compute at different times) unless the row is longer than eight such slices. The CTAs' parts (maximum, sums, best
+// into slices, one for each CTA of a cluster, and a slice lies in the shared memory of its CTA, at most kUsual 16-byte groups a thread (104 KB: two CTAs
+// of an SM load and compute at different times; four of half the size spent as much on their ends as on their elements) unless the row is longer than eight such slices. The CTAs' parts (maximum, sums, best
 // keys) meet in the shared memory of the cluster's first.
-// Alternatives without sorting a row: the ceil(k / 8)-th largest of its lanes' maxima is found in each of eight warps; the smallest of
+// Alternatives without sorting a row: the ceil(k / 16)-th largest of its lanes' maxima is found in each of sixteen warps; the smallest of
 // these is a bound that at least k elements of the slice reach, and for logits in no particular order a few dozen do. Only the lanes whose maximum
 // reaches it are looked through, by their whole warp, and what is found is put in a list and ranked by counting (key: the value's order, then the
 // lower index). Where more than the list's length reach the bound (equal logits, masked rows) the k best are taken one after another.
 // Rows beyond 8 CTAs of kMost groups (442368 fp32 columns, 884736 bf16) are walked in global memory by one CTA each.
 #include <cooperative_groups.h>
+#include <cuda_bf16.h>
 #include <float.h>
 #include <math.h>
 
@@ -31,9 +32,9 @@ namespace {
 
 using ptx::ex2_approx;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxSlices = 8, kList = 320, kTop = DF_LOGPROBS_MAX_TOP;
-constexpr uint32_t kMost = 54, kUsual = 13;  // groups of a thread: one CTA of an SM, four of them
-static_assert(kMaxSlices * kTop <= kList, "the first CTA ranks all CTAs' alternatives in one list");
+constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxSlices = 8, kList = 256, kTop = DF_LOGPROBS_MAX_TOP;
+constexpr uint32_t kMost = 27, kUsual = 13;  // groups of a thread: one CTA of an SM, two of them
+static_assert(kMaxSlices * kTop <= kThreads, "a thread for each of the CTAs' alternatives");
 
 template <bool BF16>
 __device__ __forceinline__ float load1(const void *base, size_t e) {
@@ -55,6 +56,7 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t order) {
   return order == 0xffffffffu ? NAN : __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
 }
+__device__ __forceinline__ float bound_of(uint32_t order) { return order < 0x00800000u ? -INFINITY : value_of(order); }  // (the last bit may be off)
 __device__ __forceinline__ unsigned long long key_of(float x, uint32_t i) { return ((unsigned long long)order_of(x) << 32) | (0xffffffffu - i); }
 
 struct LogprobParams {
@@ -91,25 +93,35 @@ __device__ __forceinline__ float element(const uint4 &v, int e) {
   return __uint_as_float(w[e]);
 }
 
-// exp(z - m) and its product with z - m
-__device__ __forceinline__ void add_element(float x, float scale, float m, float &sum, float &weighted) {
-  const float y = fmaf(x, scale, -m), e = ex2_approx(y * kLog2e);
-  sum += e;
-  weighted = fmaf(e, fmaxf(y, -1000.0f), weighted);  // e = 0 where y is below
-}
+// Two elements' exp(z - m) and its product with z - m, in units of log 2: y = (x - max x) * (scale * log2 e). The difference first: it is exact where it
+// matters, and neither a large maximum nor its product with the scale can round it away or overflow.
+struct Sums2 {
+  float2 sum = {0.0f, 0.0f}, weighted = {0.0f, 0.0f};
+  __device__ __forceinline__ void add(float a, float b, float2 scale_log2, float2 minus_top) {
+    float2 y = ptx::mul2(ptx::add2(make_float2(a, b), minus_top), scale_log2);
+    const float2 e = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+    y = make_float2(fmaxf(y.x, -2000.0f), fmaxf(y.y, -2000.0f));  // -inf: its e is 0, the product 0 too
+    sum = ptx::add2(sum, e);
+    weighted = ptx::fma2(e, y, weighted);
+  }
+  __device__ __forceinline__ void add(const Sums2 &o) {
+    sum = ptx::add2(sum, o.sum);
+    weighted = ptx::add2(weighted, o.weighted);
+  }
+};
 
-// Writes a finished row. x in units of the logits; `top` = max of scale * x, -inf for a row that cannot come at all.
+// A finished row: its largest logit (-inf where nothing can come), and sums in units of log 2.
 struct RowResult {
   float top, sum, weighted;
   bool bad;  // a NaN or +inf
-  __device__ __forceinline__ float log_sum() const { return bad ? NAN : logf(sum); }
-  // z - m first: their difference is exact where it matters, while m + log S would round log S away beside a large m
-  __device__ __forceinline__ float logp(float x, float scale) const { return bad ? NAN : top == -INFINITY ? -INFINITY : (x * scale - top) - log_sum(); }
+  __device__ __forceinline__ float logp(float x, float scale) const {
+    return bad ? NAN : top == -INFINITY ? -INFINITY : fmaf(x - top, scale, -log2f(sum) * kLn2);
+  }
   template <bool BF16>
   __device__ __forceinline__ void write(const LogprobParams &p, uint32_t row, const void *grow) const {
     const int32_t target = __ldg(p.targets + row);
-    p.lse[row] = bad ? NAN : top == -INFINITY ? -INFINITY : top + log_sum();
-    p.entropy[row] = bad ? NAN : top == -INFINITY ? 0.0f : log_sum() - weighted / sum;
+    p.lse[row] = bad ? NAN : top == -INFINITY ? -INFINITY : fmaf(top, p.scale, log2f(sum) * kLn2);
+    p.entropy[row] = bad ? NAN : top == -INFINITY ? 0.0f : (log2f(sum) - weighted / sum) * kLn2;
     p.logp[row] = target >= 0 && (uint32_t)target < p.cols ? logp(load1<BF16>(grow, target), p.scale) : 0.0f;
   }
   __device__ __forceinline__ void write_top(const LogprobParams &p, uint32_t row, uint32_t k, unsigned long long key) const {
@@ -140,7 +152,7 @@ __device__ __forceinline__ void rank_list(const unsigned long long *list, uint32
 }
 
 template <bool BF16>
-__global__ void __launch_bounds__(kThreads, 4) k_token_logprobs(const LogprobParams p) {
+__global__ void __launch_bounds__(kThreads, 2) k_token_logprobs(const LogprobParams p) {
   ptx::pdl_wait();
   constexpr int E = RowSplit<BF16>::kElements;
   extern __shared__ __align__(16) uint4 body_smem[];  // [groups][kThreads]
@@ -169,12 +181,20 @@ __global__ void __launch_bounds__(kThreads, 4) k_token_logprobs(const LogprobPar
 
   // ---- maximum (NaN apart)
   float top = x_extra;
+  auto bf2 = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162 *>(&w); };
+  const uint32_t low2 = 0xff80ff80u;  // -inf, twice
+  __nv_bfloat162 top2 = bf2(low2);
 #pragma unroll 4
   for (uint32_t i = 0; i < groups; ++i) {
     const uint4 v = body_smem[i * kThreads + t];
+    if (BF16) {
+      top2 = __hmax2(top2, __hmax2(__hmax2(bf2(v.x), bf2(v.y)), __hmax2(bf2(v.z), bf2(v.w))));
+    } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) top = fmaxf(top, element<BF16>(v, e));
+      for (int e = 0; e < E; ++e) top = fmaxf(top, element<BF16>(v, e));
+    }
   }
+  if (BF16) top = fmaxf(top, fmaxf(__low2float(top2), __high2float(top2)));
   const float mine = top;  // of this thread
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -190,23 +210,23 @@ __global__ void __launch_bounds__(kThreads, 4) k_token_logprobs(const LogprobPar
     if (lane == 0) sm.bound[warp] = bound & ~1u;
   }
   __syncthreads();
-  top = sm.red[0][0];
+  top = sm.red[0][lane % kWarps];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.red[0][w]);
+  for (int o = kWarps / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 
   // ---- sums
-  const float m = top == -INFINITY ? 0.0f : top * p.scale;
-  float sum = 0.0f, weighted = 0.0f;
-  add_element(x_extra, p.scale, m, sum, weighted);
+  const float2 scale2 = make_float2(p.scale * kLog2e, p.scale * kLog2e), minus_top = top == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-top, -top);
+  Sums2 sums;
+  sums.add(x_extra, -INFINITY, scale2, minus_top);
 #pragma unroll 2
   for (uint32_t i = 0; i < groups; ++i) {  // a group by itself first: a thread's sum is then of some dozens of terms, not hundreds
     const uint4 v = body_smem[i * kThreads + t];
-    float group_sum = 0.0f, group_weighted = 0.0f;
+    Sums2 group;
 #pragma unroll
-    for (int e = 0; e < E; ++e) add_element(element<BF16>(v, e), p.scale, m, group_sum, group_weighted);
-    sum += group_sum;
-    weighted += group_weighted;
+    for (int e = 0; e < E; e += 2) group.add(element<BF16>(v, e), element<BF16>(v, e + 1), scale2, minus_top);
+    sums.add(group);
   }
+  float sum = sums.sum.x + sums.sum.y, weighted = sums.weighted.x + sums.weighted.y;
   const bool nan_here = isnan(sum);  // this thread has a NaN (or +inf, or there is one in the slice)
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -217,18 +237,15 @@ __global__ void __launch_bounds__(kThreads, 4) k_token_logprobs(const LogprobPar
 
   // ---- the slice's best
   if (p.top_k) {
-    uint32_t bound = full_warps ? 0xffffffffu : 0u;  // fewer than 32 groups: everything
-    for (uint32_t w = 0; w < full_warps; ++w) bound = min(bound, sm.bound[w]);
+    const float bound = full_warps ? bound_of(__reduce_min_sync(0xffffffffu, lane < full_warps ? sm.bound[lane] : 0xffffffffu)) : -INFINITY;  // else everything
     auto consider = [&](float x, uint32_t i) {
-      const uint32_t order = order_of(x);
-      if (order >= bound) {
+      if (!(x < bound)) {  // a NaN is nobody's maximum, but comes first
         const uint32_t at = atomicAdd(&sm.n_list, 1u);
-        if (at < kList) sm.list[at] = ((unsigned long long)order << 32) | (0xffffffffu - i);
+        if (at < kList) sm.list[at] = key_of(x, i);
       }
     };
     if (extra < p.cols) consider(x_extra, extra);
-    // a NaN is nobody's maximum, but comes first
-    uint32_t look = __ballot_sync(0xffffffffu, groups > 0 && (order_of(mine) >= bound || nan_here));
+    uint32_t look = __ballot_sync(0xffffffffu, groups > 0 && (mine >= bound || nan_here));
     while (look) {
       const uint32_t owner = __ffs(look) - 1, n = __shfl_sync(0xffffffffu, groups, owner);
       look &= look - 1;
@@ -241,12 +258,12 @@ __global__ void __launch_bounds__(kThreads, 4) k_token_logprobs(const LogprobPar
     }
   }
   __syncthreads();
-  sum = sm.red[1][0];
-  weighted = sm.red[2][0];
+  sum = sm.red[1][lane % kWarps];
+  weighted = sm.red[2][lane % kWarps];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) {
-    sum += sm.red[1][w];
-    weighted += sm.red[2][w];
+  for (int o = kWarps / 2; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    weighted += __shfl_xor_sync(0xffffffffu, weighted, o);
   }
   const bool bad = isnan(sum) || top == INFINITY;  // a NaN or +inf reaches the sum
 
@@ -256,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_token_logprobs(const LogprobPar
     cluster.barrier_wait();
     first = cluster.map_shared_rank(&sm, 0);
   }
-  if (t == 0) first->part[slice] = make_float4(top == -INFINITY ? -INFINITY : m, sum, weighted, bad ? 1.0f : 0.0f);
+  if (t == 0) first->part[slice] = make_float4(top, sum, weighted, bad ? 1.0f : 0.0f);
   unsigned long long *best = first->best + slice * p.top_k;
   if (p.top_k) {
     const uint32_t n = sm.n_list;
@@ -294,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_token_logprobs(const LogprobPar
   } else {
     __syncthreads();
   }
+  if (t >= max(32u, p.slices * p.top_k)) return;
   RowResult r = {-INFINITY, 0.0f, 0.0f, false};
   for (uint32_t s = 0; s < p.slices; ++s) {
     r.top = fmaxf(r.top, sm.part[s].x);
@@ -302,9 +320,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_token_logprobs(const LogprobPar
   for (uint32_t s = 0; s < p.slices; ++s) {
     const float4 q = sm.part[s];
     if (q.x == -INFINITY) continue;  // nothing of this slice can come
-    const float down = q.x - r.top, f = ex2_approx(down * kLog2e);
+    const float down = (q.x - r.top) * (p.scale * kLog2e), f = ex2_approx(down);
     r.sum = fmaf(q.y, f, r.sum);
-    r.weighted = fmaf(fmaf(q.y, fmaxf(down, -1000.0f), q.z), f, r.weighted);  // y to the slice's maximum becomes y + down
+    r.weighted = fmaf(fmaf(q.y, fmaxf(down, -2000.0f), q.z), f, r.weighted);  // y to the slice's maximum becomes y + down
   }
   if (t == 0) r.write<BF16>(p, row, grow);
   if (p.top_k) {
@@ -351,13 +369,14 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs_any(const LogprobPa
   }
   r.bad = __syncthreads_or(r.bad);
   top = block_reduce(top, [](float a, float b) { return fmaxf(a, b); }, red);
-  r.top = top == -INFINITY ? -INFINITY : top * p.scale;
-  const float m = top == -INFINITY ? 0.0f : r.top;
+  r.top = top;
+  const float2 scale2 = make_float2(p.scale * kLog2e, p.scale * kLog2e), minus_top = top == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-top, -top);
   for (uint32_t i0 = t; i0 < p.cols; i0 += 32 * kThreads) {  // 32 terms by themselves first: thousands in a row would lose the last bits
-    float some = 0.0f, some_weighted = 0.0f;
-    for (uint32_t i = i0; i < min(p.cols, i0 + 32 * kThreads); i += kThreads) add_element(load1<BF16>(grow, i), p.scale, m, some, some_weighted);
-    r.sum += some;
-    r.weighted += some_weighted;
+    Sums2 some;
+    for (uint32_t i = i0; i < min(p.cols, i0 + 32 * kThreads); i += 2 * kThreads)
+      some.add(load1<BF16>(grow, i), i + kThreads < p.cols ? load1<BF16>(grow, i + kThreads) : -INFINITY, scale2, minus_top);
+    r.sum += some.sum.x + some.sum.y;
+    r.weighted += some.weighted.x + some.weighted.y;
   }
   r.sum = block_reduce(r.sum, add, red);
   r.weighted = block_reduce(r.weighted, add, red);
