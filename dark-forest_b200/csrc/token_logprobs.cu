@@ -6,21 +6,18 @@
 // The entropy is formed from differences to the maximum, so that nothing large cancels; a column with exp(z - m) = 0 adds nothing (its z - m
 // may be -inf). All sums in fp32.
 //
-// Both directions are bound by HBM: the forward reads every logit once, the gradient reads and writes it once. In the forward a row is cut
-// into slices, one for each CTA of a cluster, and a slice lies in the shared memory of its CTA, at most kUsual 16-byte groups a thread (104 KB: two CTAs
-// of an SM load and compute at different times; four of half the size spent as much on their ends as on their elements) unless the row is longer than eight such slices. The CTAs' parts (maximum, sums, best
-// keys) meet in the shared memory of the cluster's first.
-// Alternatives without sorting a row: the ceil(k / 16)-th largest of its lanes' maxima is found in each of sixteen warps; the smallest of
-// these is a bound that at least k elements of the slice reach, and for logits in no particular order a few dozen do. Only the lanes whose maximum
-// reaches it are looked through, by their whole warp, and what is found is put in a list and ranked by counting (key: the value's order, then the
-// lower index). Where more than the list's length reach the bound (equal logits, masked rows) the k best are taken one after another.
-// Rows beyond 8 CTAs of kMost groups (442368 fp32 columns, 884736 bf16) are walked in global memory by one CTA each.
+// Both directions are bound by HBM: the forward reads every logit once, the gradient reads and writes it once. In the forward a CTA, or where there are few
+// rows a cluster of them, walks a row once, kChunk 16-byte groups a thread at a time, with a running maximum and sums per thread; the CTAs' parts
+// (maximum, sums, best keys) meet in the shared memory of the cluster's first. Holding the row in shared memory instead (four CTAs or two of an SM) took
+// 50 to 66 us at 1024 x 50257 bf16, 32 us this way: loads of one row then ran beside the sums of one other at best.
+// Alternatives without sorting a row: each of the sixteen warps names its two largest lane maxima; the k-th largest of these 32 is a bound that at
+// least k elements reach, and for logits in no particular order few others do. Only the lanes whose maximum reaches it are looked through
+// again, by their whole warp (out of L2), and what is found is put in a list and ranked by counting (key: the value's order, then the lower index).
+// Where more than the list's length reach the bound (equal logits, masked rows) the k best are taken one after another.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <float.h>
 #include <math.h>
-
-#include <mutex>
 
 #include "df_common.cuh"
 #include "sm100_ptx.cuh"
@@ -33,7 +30,7 @@ namespace {
 using ptx::ex2_approx;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxSlices = 8, kList = 256, kTop = DF_LOGPROBS_MAX_TOP;
-constexpr uint32_t kMost = 27, kUsual = 13;  // groups of a thread: one CTA of an SM, two of them
+constexpr int kChunk = 4;  // groups of a thread that are loaded at once
 static_assert(kMaxSlices * kTop <= kThreads, "a thread for each of the CTAs' alternatives");
 
 template <bool BF16>
@@ -104,10 +101,6 @@ struct Sums2 {
     sum = ptx::add2(sum, e);
     weighted = ptx::fma2(e, y, weighted);
   }
-  __device__ __forceinline__ void add(const Sums2 &o) {
-    sum = ptx::add2(sum, o.sum);
-    weighted = ptx::add2(weighted, o.weighted);
-  }
 };
 
 // A finished row: its largest logit (-inf where nothing can come), and sums in units of log 2.
@@ -137,7 +130,7 @@ struct SliceSmem {
   float4 part[kMaxSlices];                     // (first CTA) maximum, sum, weighted sum, bad
   float red[3][kWarps];
   unsigned long long red_key[kWarps];
-  uint32_t bound[kWarps];
+  uint32_t bound[2 * kWarps];
   uint32_t n_list;
 };
 
@@ -151,11 +144,17 @@ __device__ __forceinline__ void rank_list(const unsigned long long *list, uint32
   }
 }
 
+// Sums relative to `from` become sums relative to `to` (which is not below it).
+__device__ __forceinline__ void rebase(float from, float to, float scale_log2, float &sum, float &weighted) {
+  const float down = fmaxf((from - to) * scale_log2, -2000.0f), f = ex2_approx(down);  // from = -inf: sums are 0
+  weighted = fmaf(sum, down, weighted) * f;  // y to the old maximum becomes y + down
+  sum *= f;
+}
+
 template <bool BF16>
-__global__ void __launch_bounds__(kThreads, 2) k_token_logprobs(const LogprobParams p) {
+__global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const LogprobParams p) {
   ptx::pdl_wait();
   constexpr int E = RowSplit<BF16>::kElements;
-  extern __shared__ __align__(16) uint4 body_smem[];  // [groups][kThreads]
   __shared__ SliceSmem sm;
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -170,64 +169,78 @@ __global__ void __launch_bounds__(kThreads, 2) k_token_logprobs(const LogprobPar
   uint32_t extra = p.cols;  // the scalar element of this thread, if any
   if (slice == 0 && t < split.head) extra = t;
   if (slice == p.slices - 1 && t >= 32 && t - 32 < p.cols - split.body_end()) extra = split.body_end() + (t - 32);
-  const uint32_t groups = g1 > g0 + t ? (g1 - g0 - t + kThreads - 1) / kThreads : 0;  // of this thread
-  const uint32_t dst = ptx::smem_u32(body_smem + t);
-  for (uint32_t i = 0; i < groups; ++i)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * (kThreads * 16u)), "l"(body + g0 + i * kThreads + t) : "memory");
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  const float x_extra = extra < p.cols ? load1<BF16>(grow, extra) : -INFINITY;
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncwarp();
+  const float scale_log2 = p.scale * kLog2e;
+  const float2 scale2 = make_float2(scale_log2, scale_log2);
+  auto pair_of = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162 *>(&w); };
 
-  // ---- maximum (NaN apart)
-  float top = x_extra;
-  auto bf2 = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162 *>(&w); };
-  const uint32_t low2 = 0xff80ff80u;  // -inf, twice
-  __nv_bfloat162 top2 = bf2(low2);
-#pragma unroll 4
-  for (uint32_t i = 0; i < groups; ++i) {
-    const uint4 v = body_smem[i * kThreads + t];
+  // ---- one walk: maximum (NaN apart) and sums of this thread's elements
+  const float x_extra = extra < p.cols ? load1<BF16>(grow, extra) : -INFINITY;
+  float mine = -INFINITY, sum = 0.0f, weighted = 0.0f;
+  for (uint32_t g = g0 + t; g < g1; g += kChunk * kThreads) {
+    constexpr uint32_t kNone = BF16 ? 0xff80ff80u : 0xff800000u;  // -inf
+    uint4 v[kChunk];
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) v[i] = g + i * kThreads < g1 ? __ldg(body + g + i * kThreads) : make_uint4(kNone, kNone, kNone, kNone);
+    float top = -INFINITY;
     if (BF16) {
-      top2 = __hmax2(top2, __hmax2(__hmax2(bf2(v.x), bf2(v.y)), __hmax2(bf2(v.z), bf2(v.w))));
+      __nv_bfloat162 top2 = pair_of(kNone);
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i)
+        top2 = __hmax2(top2, __hmax2(__hmax2(pair_of(v[i].x), pair_of(v[i].y)), __hmax2(pair_of(v[i].z), pair_of(v[i].w))));
+      top = fmaxf(__low2float(top2), __high2float(top2));
     } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) top = fmaxf(top, element<BF16>(v, e));
+      for (int i = 0; i < kChunk; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) top = fmaxf(top, element<BF16>(v[i], e));
     }
+    if (top > mine) {
+      rebase(mine, top, scale_log2, sum, weighted);
+      mine = top;
+    }
+    const float2 minus_top = mine == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-mine, -mine);
+    Sums2 sums;  // a chunk by itself first: a thread's sums are then of some dozens of terms, not hundreds
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i)
+#pragma unroll
+      for (int e = 0; e < E; e += 2) sums.add(element<BF16>(v[i], e), element<BF16>(v[i], e + 1), scale2, minus_top);
+    sum += sums.sum.x + sums.sum.y;
+    weighted += sums.weighted.x + sums.weighted.y;
   }
-  if (BF16) top = fmaxf(top, fmaxf(__low2float(top2), __high2float(top2)));
-  const float mine = top;  // of this thread
+  const bool any = g0 + t < g1;                     // groups for this thread
+  const float body_most = mine;
+  const bool nan_here = any && isnan(sum);          // a NaN or +inf among them
+  if (extra < p.cols) {
+    const float top = fmaxf(mine, x_extra);
+    rebase(mine, top, scale_log2, sum, weighted);
+    mine = top;
+    Sums2 one;
+    one.add(x_extra, -INFINITY, scale2, mine == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-mine, -mine));
+    sum += one.sum.x;
+    weighted += one.weighted.x;
+  }
+  // ---- the CTA's
+  float top = mine;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) sm.red[0][warp] = top;
   const uint32_t full_warps = min((g1 - g0) / 32, (uint32_t)kWarps);  // every lane of them has a maximum
-  if (p.top_k && warp < full_warps) {  // this warp's bound: its ceil(k / full_warps)-th largest lane maximum
-    uint32_t left = order_of(mine) | 1u, bound = 0;  // (the last bit off: a lane that is out has 0)
-    for (uint32_t n = 0; n < (p.top_k + full_warps - 1) / full_warps; ++n) {
+  const uint32_t named = full_warps == 0 ? 0u : full_warps == kWarps ? 2u : (p.top_k + full_warps - 1) / full_warps;
+  if (p.top_k && warp < full_warps) {  // this warp's largest lane maxima
+    uint32_t left = order_of(body_most) | 1u, bound = 0;  // (the last bit off: a lane that is out has 0)
+    for (uint32_t n = 0; n < named; ++n) {
       bound = __reduce_max_sync(0xffffffffu, left);
       const uint32_t holds = __ballot_sync(0xffffffffu, left == bound);
       if (lane == __ffs(holds) - 1) left = 0;
+      if (lane == 0 && n < 2) sm.bound[n * kWarps + warp] = bound & ~1u;
     }
-    if (lane == 0) sm.bound[warp] = bound & ~1u;
+    if (lane == 0 && full_warps < kWarps) sm.bound[warp] = bound & ~1u;
   }
   __syncthreads();
   top = sm.red[0][lane % kWarps];
 #pragma unroll
   for (int o = kWarps / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-
-  // ---- sums
-  const float2 scale2 = make_float2(p.scale * kLog2e, p.scale * kLog2e), minus_top = top == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-top, -top);
-  Sums2 sums;
-  sums.add(x_extra, -INFINITY, scale2, minus_top);
-#pragma unroll 2
-  for (uint32_t i = 0; i < groups; ++i) {  // a group by itself first: a thread's sum is then of some dozens of terms, not hundreds
-    const uint4 v = body_smem[i * kThreads + t];
-    Sums2 group;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) group.add(element<BF16>(v, e), element<BF16>(v, e + 1), scale2, minus_top);
-    sums.add(group);
-  }
-  float sum = sums.sum.x + sums.sum.y, weighted = sums.weighted.x + sums.weighted.y;
-  const bool nan_here = isnan(sum);  // this thread has a NaN (or +inf, or there is one in the slice)
+  if (mine != top && top != -INFINITY) rebase(mine, top, scale_log2, sum, weighted);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -237,7 +250,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_token_logprobs(const LogprobPar
 
   // ---- the slice's best
   if (p.top_k) {
-    const float bound = full_warps ? bound_of(__reduce_min_sync(0xffffffffu, lane < full_warps ? sm.bound[lane] : 0xffffffffu)) : -INFINITY;  // else everything
+    float bound = -INFINITY;  // fewer than 32 groups: everything
+    if (full_warps == kWarps) {  // the k-th largest of 32: the smallest that fewer than k are above
+      const uint32_t order = sm.bound[lane];
+      uint32_t above = 0;
+#pragma unroll 8
+      for (int j = 0; j < 32; ++j) above += sm.bound[j] > order ? 1u : 0u;
+      bound = bound_of(__reduce_min_sync(0xffffffffu, above < p.top_k ? order : 0xffffffffu));
+    } else if (full_warps) {  // at least k lanes have a maximum that reaches the smallest of these
+      bound = bound_of(__reduce_min_sync(0xffffffffu, lane < full_warps ? sm.bound[lane] : 0xffffffffu));
+    }
     auto consider = [&](float x, uint32_t i) {
       if (!(x < bound)) {  // a NaN is nobody's maximum, but comes first
         const uint32_t at = atomicAdd(&sm.n_list, 1u);
@@ -245,15 +267,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_token_logprobs(const LogprobPar
       }
     };
     if (extra < p.cols) consider(x_extra, extra);
-    uint32_t look = __ballot_sync(0xffffffffu, groups > 0 && (mine >= bound || nan_here));
+    uint32_t look = __ballot_sync(0xffffffffu, any && (body_most >= bound || nan_here));
     while (look) {
-      const uint32_t owner = __ffs(look) - 1, n = __shfl_sync(0xffffffffu, groups, owner);
+      const uint32_t owner = __ffs(look) - 1;
       look &= look - 1;
-      for (uint32_t i = lane; i < n; i += 32) {
-        const uint32_t at = i * kThreads + warp * 32 + owner;
-        const uint4 v = body_smem[at];
+      for (uint32_t g = g0 + warp * 32 + owner + lane * kThreads; g < g1; g += 32 * kThreads) {
+        const uint4 v = __ldg(body + g);
 #pragma unroll
-        for (int e = 0; e < E; ++e) consider(element<BF16>(v, e), split.head + (g0 + at) * E + e);
+        for (int e = 0; e < E; ++e) consider(element<BF16>(v, e), split.head + g * E + e);
       }
     }
   }
@@ -289,10 +310,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_token_logprobs(const LogprobPar
           if (key < last && key > most) most = key;
         };
         if (extra < p.cols) consider(x_extra, extra);
-        for (uint32_t i = 0; i < groups; ++i) {
-          const uint4 v = body_smem[i * kThreads + t];
+        for (uint32_t g = g0 + t; g < g1; g += kThreads) {
+          const uint4 v = __ldg(body + g);
 #pragma unroll
-          for (int e = 0; e < E; ++e) consider(element<BF16>(v, e), split.head + (g0 + i * kThreads + t) * E + e);
+          for (int e = 0; e < E; ++e) consider(element<BF16>(v, e), split.head + g * E + e);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -320,9 +341,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_token_logprobs(const LogprobPar
   for (uint32_t s = 0; s < p.slices; ++s) {
     const float4 q = sm.part[s];
     if (q.x == -INFINITY) continue;  // nothing of this slice can come
-    const float down = (q.x - r.top) * (p.scale * kLog2e), f = ex2_approx(down);
-    r.sum = fmaf(q.y, f, r.sum);
-    r.weighted = fmaf(fmaf(q.y, fmaxf(down, -2000.0f), q.z), f, r.weighted);  // y to the slice's maximum becomes y + down
+    float sum_s = q.y, weighted_s = q.z;
+    rebase(q.x, r.top, scale_log2, sum_s, weighted_s);
+    r.sum += sum_s;
+    r.weighted += weighted_s;
   }
   if (t == 0) r.write<BF16>(p, row, grow);
   if (p.top_k) {
@@ -336,60 +358,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_token_logprobs(const LogprobPar
         for (uint32_t j = 0; j < n; ++j) rank += sm.best[j] > key ? 1u : 0u;
       if (key && rank < p.top_k) r.write_top(p, row, rank, key);
     }
-  }
-}
-
-template <typename T, typename Op>
-__device__ __forceinline__ T block_reduce(T v, Op op, T *red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  T r = red[0];
-  for (int w = 1; w < kWarps; ++w) r = op(r, red[w]);
-  return r;
-}
-
-// Rows of any length: passes over global memory (they come out of L2 after the first).
-template <bool BF16>
-__global__ void __launch_bounds__(kThreads) k_token_logprobs_any(const LogprobParams p) {
-  ptx::pdl_wait();
-  __shared__ float red[kWarps];
-  __shared__ unsigned long long red_key[kWarps];
-  const uint32_t row = blockIdx.x, t = threadIdx.x;
-  const void *grow = row_at<BF16>(p.logits, row, p.stride);
-  auto add = [](float a, float b) { return a + b; };
-  RowResult r = {-INFINITY, 0.0f, 0.0f, false};
-  float top = -INFINITY;
-  for (uint32_t i = t; i < p.cols; i += kThreads) {
-    const float x = load1<BF16>(grow, i);
-    r.bad |= isnan(x) || x == INFINITY;
-    top = fmaxf(top, x);
-  }
-  r.bad = __syncthreads_or(r.bad);
-  top = block_reduce(top, [](float a, float b) { return fmaxf(a, b); }, red);
-  r.top = top;
-  const float2 scale2 = make_float2(p.scale * kLog2e, p.scale * kLog2e), minus_top = top == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-top, -top);
-  for (uint32_t i0 = t; i0 < p.cols; i0 += 32 * kThreads) {  // 32 terms by themselves first: thousands in a row would lose the last bits
-    Sums2 some;
-    for (uint32_t i = i0; i < min(p.cols, i0 + 32 * kThreads); i += 2 * kThreads)
-      some.add(load1<BF16>(grow, i), i + kThreads < p.cols ? load1<BF16>(grow, i + kThreads) : -INFINITY, scale2, minus_top);
-    r.sum += some.sum.x + some.sum.y;
-    r.weighted += some.weighted.x + some.weighted.y;
-  }
-  r.sum = block_reduce(r.sum, add, red);
-  r.weighted = block_reduce(r.weighted, add, red);
-  if (t == 0) r.write<BF16>(p, row, grow);
-  unsigned long long last = ~0ull;
-  for (uint32_t k = 0; k < p.top_k; ++k) {
-    unsigned long long best = 0;
-    for (uint32_t i = t; i < p.cols; i += kThreads) {
-      const unsigned long long key = key_of(load1<BF16>(grow, i), i);
-      if (key < last && key > best) best = key;
-    }
-    last = block_reduce(best, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; }, red_key);
-    if (t == 0) r.write_top(p, row, k, last);
   }
 }
 
@@ -470,41 +438,18 @@ int finish(int st) {
   return st;
 }
 
-struct DeviceInfo {
-  std::once_flag once;
-  bool ok = false;
-};
-
-// Shared memory of a whole SM for the longest slices; asked for once per kernel and device.
-template <bool BF16>
-bool prepare() {
-  static DeviceInfo table[64];
-  int dev = 0;
-  if (check_cuda(cudaGetDevice(&dev)) != DF_OK || dev < 0 || dev >= 64) return false;
-  DeviceInfo &d = table[dev];
-  std::call_once(d.once, [&]() {
-    d.ok = cudaFuncSetAttribute(k_token_logprobs<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kMost * kThreads * 16)) == cudaSuccess;
-  });
-  return d.ok;
-}
-
-// Slices of a row: as few CTAs as hold it at four to an SM; more while the rows alone do not give every SM two CTAs; beyond eight slices' worth of
-// columns the slices grow to an SM each.
+// One CTA a row; more, up to eight, while the rows alone do not give every SM three and a CTA still has a chunk.
 template <bool BF16>
 int launch_forward(LogprobParams &p, cudaStream_t s) {
   const uint32_t n = p.cols / RowSplit<BF16>::kElements + 1;
   const int n_sm = sm_count();
-  if (n_sm == 0 || !prepare<BF16>()) return DF_ERR_CUDA;
-  auto groups_of = [&](uint32_t slices) { return (n + slices * kThreads - 1) / (slices * kThreads); };
+  if (n_sm == 0) return DF_ERR_CUDA;
   uint32_t slices = 1;
-  while (slices < kMaxSlices && (groups_of(slices) > kUsual || ((uint64_t)p.rows * slices < 2u * (uint64_t)n_sm && groups_of(slices) > 2))) slices *= 2;
+  while (slices < kMaxSlices && (uint64_t)p.rows * slices < 3u * (uint64_t)n_sm && n > slices * (kChunk * kThreads)) slices *= 2;
   p.slices = slices;
-  p.groups = groups_of(slices);
-  int st;
-  if (p.groups > kMost || (uint64_t)p.rows * slices > 0x7fffffffull)
-    st = check_cuda(launch_kernel(k_token_logprobs_any<BF16>, dim3(p.rows), dim3(kThreads), 0, s, p));
-  else
-    st = check_cuda(launch_clusters(k_token_logprobs<BF16>, slices, dim3(p.rows * slices), dim3(kThreads), (size_t)p.groups * kThreads * 16, s, p));
+  p.groups = (n + slices * kThreads - 1) / (slices * kThreads);
+  if ((uint64_t)p.rows * slices > 0x7fffffffull) return DF_ERR_UNSUPPORTED;
+  const int st = check_cuda(launch_clusters(k_token_logprobs<BF16>, slices, dim3(p.rows * slices), dim3(kThreads), 0, s, p));
   note_launch();
   return st;
 }
