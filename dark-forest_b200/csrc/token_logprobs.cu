@@ -10,7 +10,7 @@
 // rows a cluster of them, walks a row once, kChunk 16-byte groups a thread at a time, with a running maximum and sums per thread; the CTAs' parts
 // (maximum, sums, best keys) meet in the shared memory of the cluster's first. Holding the row in shared memory instead (four CTAs or two of an SM) took
 // 50 to 66 us at 1024 x 50257 bf16, 32 us this way: loads of one row then ran beside the sums of one other at best.
-// Alternatives without sorting a row: each of the sixteen warps names its two largest lane maxima; the k-th largest of these 32 is a bound that at
+// Alternatives without sorting a row: each of the eight warps names its four largest lane maxima; the k-th largest of these 32 is a bound that at
 // least k elements reach, and for logits in no particular order few others do. Only the lanes whose maximum reaches it are looked through
 // again, by their whole warp (out of L2), and what is found is put in a list and ranked by counting (key: the value's order, then the lower index).
 // Where more than the list's length reach the bound (equal logits, masked rows) the k best are taken one after another.
@@ -29,7 +29,7 @@ namespace {
 
 using ptx::ex2_approx;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxSlices = 8, kList = 256, kTop = DF_LOGPROBS_MAX_TOP;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kNamed = 32 / kWarps, kMaxSlices = 8, kList = 256, kTop = DF_LOGPROBS_MAX_TOP;
 constexpr int kChunk = 4;  // groups of a thread that are loaded at once
 static_assert(kMaxSlices * kTop <= kThreads, "a thread for each of the CTAs' alternatives");
 
@@ -130,7 +130,8 @@ struct SliceSmem {
   float4 part[kMaxSlices];                     // (first CTA) maximum, sum, weighted sum, bad
   float red[3][kWarps];
   unsigned long long red_key[kWarps];
-  uint32_t bound[2 * kWarps];
+  uint32_t bound[32];
+  uint8_t owner[kWarps][32];
   uint32_t n_list;
 };
 
@@ -152,7 +153,7 @@ __device__ __forceinline__ void rebase(float from, float to, float scale_log2, f
 }
 
 template <bool BF16>
-__global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const LogprobParams p) {
+__global__ void __launch_bounds__(kThreads, 6) k_token_logprobs(const LogprobParams p) {
   ptx::pdl_wait();
   constexpr int E = RowSplit<BF16>::kElements;
   __shared__ SliceSmem sm;
@@ -225,14 +226,14 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const LogprobPar
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) sm.red[0][warp] = top;
   const uint32_t full_warps = min((g1 - g0) / 32, (uint32_t)kWarps);  // every lane of them has a maximum
-  const uint32_t named = full_warps == 0 ? 0u : full_warps == kWarps ? 2u : (p.top_k + full_warps - 1) / full_warps;
+  const uint32_t named = full_warps == 0 ? 0u : full_warps == kWarps ? (uint32_t)kNamed : (p.top_k + full_warps - 1) / full_warps;
   if (p.top_k && warp < full_warps) {  // this warp's largest lane maxima
     uint32_t left = order_of(body_most) | 1u, bound = 0;  // (the last bit off: a lane that is out has 0)
     for (uint32_t n = 0; n < named; ++n) {
       bound = __reduce_max_sync(0xffffffffu, left);
       const uint32_t holds = __ballot_sync(0xffffffffu, left == bound);
       if (lane == __ffs(holds) - 1) left = 0;
-      if (lane == 0 && n < 2) sm.bound[n * kWarps + warp] = bound & ~1u;
+      if (lane == 0 && n < kNamed) sm.bound[n * kWarps + warp] = bound & ~1u;
     }
     if (lane == 0 && full_warps < kWarps) sm.bound[warp] = bound & ~1u;
   }
@@ -267,15 +268,17 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const LogprobPar
       }
     };
     if (extra < p.cols) consider(x_extra, extra);
-    uint32_t look = __ballot_sync(0xffffffffu, any && (body_most >= bound || nan_here));
-    while (look) {
-      const uint32_t owner = __ffs(look) - 1;
-      look &= look - 1;
-      for (uint32_t g = g0 + warp * 32 + owner + lane * kThreads; g < g1; g += 32 * kThreads) {
-        const uint4 v = __ldg(body + g);
+    // the warp's lanes over all groups of the lanes to be looked through at once: one after another they cost a trip to L2 each
+    const bool look = any && (body_most >= bound || nan_here);
+    const uint32_t looking = __ballot_sync(0xffffffffu, look), turns = (g1 - g0 + kThreads - 1) / kThreads;
+    if (look) sm.owner[warp][__popc(looking & ((1u << lane) - 1))] = (uint8_t)lane;
+    __syncwarp();
+    for (uint32_t i = lane; i < __popc(looking) * turns; i += 32) {
+      const uint32_t n = i / turns, g = g0 + warp * 32 + sm.owner[warp][n] + (i - n * turns) * kThreads;
+      if (g >= g1) continue;
+      const uint4 v = __ldg(body + g);
 #pragma unroll
-        for (int e = 0; e < E; ++e) consider(element<BF16>(v, e), split.head + g * E + e);
-      }
+      for (int e = 0; e < E; ++e) consider(element<BF16>(v, e), split.head + g * E + e);
     }
   }
   __syncthreads();
