@@ -10,10 +10,11 @@
 // rows a cluster of them, walks a row once, kChunk 16-byte groups a thread at a time, with a running maximum and sums per thread; the CTAs' parts
 // (maximum, sums, best keys) meet in the shared memory of the cluster's first. Holding the row in shared memory instead (four CTAs or two of an SM) took
 // 50 to 66 us at 1024 x 50257 bf16, 32 us this way: loads of one row then ran beside the sums of one other at best.
-// Alternatives without sorting a row: each of the eight warps names its four largest lane maxima; the k-th largest of these 32 is a bound that at
-// least k elements reach, and for logits in no particular order few others do. Only the lanes whose maximum reaches it are looked through
-// again, by their whole warp (out of L2), and what is found is put in a list and ranked by counting (key: the value's order, then the lower index).
-// Where more than the list's length reach the bound (equal logits, masked rows) the k best are taken one after another.
+// Alternatives without sorting a row: each of the 4 (16) warps names its 8 (2) largest lane maxima; the k-th largest of these 32 is a bound that at
+// least k elements reach, and for logits in no particular order few others do. A thread also keeps the maxima of up to kParts parts of
+// its elements; only parts that reach the bound are read again (out of L2), and what is found is put in a list and ranked by counting (key: the value's
+// order, then the lower index). Where more than the list's length reach the bound (equal logits, masked rows) the larger ones are listed and the
+// first of the equal ones added in their order.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <float.h>
@@ -29,9 +30,8 @@ namespace {
 
 using ptx::ex2_approx;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kNamed = 32 / kWarps, kMaxSlices = 8, kList = 256, kTop = DF_LOGPROBS_MAX_TOP;
+constexpr int kMaxSlices = 8, kList = 256, kLook = 256, kParts = 16, kTop = DF_LOGPROBS_MAX_TOP;
 constexpr int kChunk = 4;  // groups of a thread that are loaded at once
-static_assert(kMaxSlices * kTop <= kThreads, "a thread for each of the CTAs' alternatives");
 
 template <bool BF16>
 __device__ __forceinline__ float load1(const void *base, size_t e) {
@@ -53,7 +53,6 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t order) {
   return order == 0xffffffffu ? NAN : __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
 }
-__device__ __forceinline__ float bound_of(uint32_t order) { return order < 0x00800000u ? -INFINITY : value_of(order); }  // (the last bit may be off)
 __device__ __forceinline__ unsigned long long key_of(float x, uint32_t i) { return ((unsigned long long)order_of(x) << 32) | (0xffffffffu - i); }
 
 struct LogprobParams {
@@ -124,18 +123,23 @@ struct RowResult {
 };
 
 // What a CTA knows of its slice, and in the cluster's first CTA what the others send.
+template <int kThreads>
 struct SliceSmem {
+  static constexpr int kWarps = kThreads / 32;
+  float most[kParts][kThreads];                // the threads' elements in up to kParts parts: their maxima
   unsigned long long list[kList];
   unsigned long long best[kMaxSlices * kTop];  // (first CTA) every CTA's best, in order
   float4 part[kMaxSlices];                     // (first CTA) maximum, sum, weighted sum, bad
   float red[3][kWarps];
   unsigned long long red_key[kWarps];
   uint32_t bound[32];
-  uint8_t owner[kWarps][32];
-  uint32_t n_list;
+  uint32_t look[kLook];  // parts that reach the bound
+  uint32_t taken[kWarps];
+  uint32_t n_list, n_look;
 };
 
 // The k best of `n` keys in `list`, in order, to `out`: a thread's key comes where as many are larger. All keys differ.
+template <int kThreads>
 __device__ __forceinline__ void rank_list(const unsigned long long *list, uint32_t n, uint32_t k, unsigned long long *out) {
   for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
     const unsigned long long key = list[i];
@@ -152,16 +156,19 @@ __device__ __forceinline__ void rebase(float from, float to, float scale_log2, f
   sum *= f;
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(kThreads, 6) k_token_logprobs(const LogprobParams p) {
+// kThreads: 128 where rows fill the machine (1024 rows, seven to an SM, are all there at once, and the CTA's ends take half of what they take with 256), 512
+// for few rows.
+template <bool BF16, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads == 128 ? 8 : 2) k_token_logprobs(const LogprobParams p) {
   ptx::pdl_wait();
+  constexpr int kWarps = kThreads / 32, kNamed = 32 / kWarps;
   constexpr int E = RowSplit<BF16>::kElements;
-  __shared__ SliceSmem sm;
+  __shared__ SliceSmem<kThreads> sm;
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const uint32_t row = blockIdx.x / p.slices, slice = blockIdx.x - row * p.slices;
   if (p.slices > 1) cluster.barrier_arrive();  // waited for before the first write to another CTA's shared memory
-  if (t == 0) sm.n_list = 0;
+  if (t == 0) sm.n_list = sm.n_look = 0;
   const void *grow = row_at<BF16>(p.logits, row, p.stride);
   const RowSplit<BF16> split(grow, p.cols);
   // this CTA: groups [g0, g1) of the row's body; the first also has its head, the last its tail
@@ -177,11 +184,21 @@ __global__ void __launch_bounds__(kThreads, 6) k_token_logprobs(const LogprobPar
   // ---- one walk: maximum (NaN apart) and sums of this thread's elements
   const float x_extra = extra < p.cols ? load1<BF16>(grow, extra) : -INFINITY;
   float mine = -INFINITY, sum = 0.0f, weighted = 0.0f;
+  constexpr uint32_t kNone = BF16 ? 0xff80ff80u : 0xff800000u;  // -inf
+  uint4 ahead[kChunk];  // the next chunk is on its way while one is worked on
+  auto load = [&](uint32_t g) {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) ahead[i] = g + i * kThreads < g1 ? __ldg(body + g + i * kThreads) : make_uint4(kNone, kNone, kNone, kNone);
+  };
+  load(g0 + t);
+  const uint32_t chunks = (g1 - g0 + kChunk * kThreads - 1) / (kChunk * kThreads), chunks_per_part = (chunks + kParts - 1) / kParts;
+  uint32_t at_part = 0, chunk_of_part = 0;
+  float part_most = -INFINITY;
   for (uint32_t g = g0 + t; g < g1; g += kChunk * kThreads) {
-    constexpr uint32_t kNone = BF16 ? 0xff80ff80u : 0xff800000u;  // -inf
     uint4 v[kChunk];
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) v[i] = g + i * kThreads < g1 ? __ldg(body + g + i * kThreads) : make_uint4(kNone, kNone, kNone, kNone);
+    for (int i = 0; i < kChunk; ++i) v[i] = ahead[i];
+    load(g + kChunk * kThreads);
     float top = -INFINITY;
     if (BF16) {
       __nv_bfloat162 top2 = pair_of(kNone);
@@ -194,6 +211,13 @@ __global__ void __launch_bounds__(kThreads, 6) k_token_logprobs(const LogprobPar
       for (int i = 0; i < kChunk; ++i)
 #pragma unroll
         for (int e = 0; e < E; ++e) top = fmaxf(top, element<BF16>(v[i], e));
+    }
+    part_most = fmaxf(part_most, top);
+    sm.most[at_part][t] = part_most;
+    if (++chunk_of_part == chunks_per_part) {
+      ++at_part;
+      chunk_of_part = 0;
+      part_most = -INFINITY;
     }
     if (top > mine) {
       rebase(mine, top, scale_log2, sum, weighted);
@@ -228,14 +252,14 @@ __global__ void __launch_bounds__(kThreads, 6) k_token_logprobs(const LogprobPar
   const uint32_t full_warps = min((g1 - g0) / 32, (uint32_t)kWarps);  // every lane of them has a maximum
   const uint32_t named = full_warps == 0 ? 0u : full_warps == kWarps ? (uint32_t)kNamed : (p.top_k + full_warps - 1) / full_warps;
   if (p.top_k && warp < full_warps) {  // this warp's largest lane maxima
-    uint32_t left = order_of(body_most) | 1u, bound = 0;  // (the last bit off: a lane that is out has 0)
+    uint32_t left = order_of(body_most), bound = 0;  // no value's order is 0: a lane that is out
     for (uint32_t n = 0; n < named; ++n) {
       bound = __reduce_max_sync(0xffffffffu, left);
       const uint32_t holds = __ballot_sync(0xffffffffu, left == bound);
       if (lane == __ffs(holds) - 1) left = 0;
-      if (lane == 0 && n < kNamed) sm.bound[n * kWarps + warp] = bound & ~1u;
+      if (lane == 0 && n < kNamed) sm.bound[n * kWarps + warp] = bound;
     }
-    if (lane == 0 && full_warps < kWarps) sm.bound[warp] = bound & ~1u;
+    if (lane == 0 && full_warps < kWarps) sm.bound[warp] = bound;
   }
   __syncthreads();
   top = sm.red[0][lane % kWarps];
@@ -249,36 +273,25 @@ __global__ void __launch_bounds__(kThreads, 6) k_token_logprobs(const LogprobPar
   }
   if (lane == 0) { sm.red[1][warp] = sum; sm.red[2][warp] = weighted; }
 
-  // ---- the slice's best
+  // ---- the slice's best: which parts of which threads reach the bound
+  float bound = -INFINITY;  // fewer than 32 groups: everything
   if (p.top_k) {
-    float bound = -INFINITY;  // fewer than 32 groups: everything
     if (full_warps == kWarps) {  // the k-th largest of 32: the smallest that fewer than k are above
       const uint32_t order = sm.bound[lane];
       uint32_t above = 0;
 #pragma unroll 8
       for (int j = 0; j < 32; ++j) above += sm.bound[j] > order ? 1u : 0u;
-      bound = bound_of(__reduce_min_sync(0xffffffffu, above < p.top_k ? order : 0xffffffffu));
+      bound = value_of(__reduce_min_sync(0xffffffffu, above < p.top_k ? order : 0xffffffffu));
     } else if (full_warps) {  // at least k lanes have a maximum that reaches the smallest of these
-      bound = bound_of(__reduce_min_sync(0xffffffffu, lane < full_warps ? sm.bound[lane] : 0xffffffffu));
+      bound = value_of(__reduce_min_sync(0xffffffffu, lane < full_warps ? sm.bound[lane] : 0xffffffffu));
     }
-    auto consider = [&](float x, uint32_t i) {
-      if (!(x < bound)) {  // a NaN is nobody's maximum, but comes first
-        const uint32_t at = atomicAdd(&sm.n_list, 1u);
-        if (at < kList) sm.list[at] = key_of(x, i);
+    if (any && (body_most >= bound || nan_here)) {
+      const uint32_t my_parts = at_part + (chunk_of_part ? 1 : 0);
+      for (uint32_t i = 0; i < my_parts; ++i) {
+        if (!(sm.most[i][t] >= bound) && !nan_here) continue;
+        const uint32_t at = atomicAdd(&sm.n_look, 1u);
+        if (at < kLook) sm.look[at] = i << 16 | t;
       }
-    };
-    if (extra < p.cols) consider(x_extra, extra);
-    // the warp's lanes over all groups of the lanes to be looked through at once: one after another they cost a trip to L2 each
-    const bool look = any && (body_most >= bound || nan_here);
-    const uint32_t looking = __ballot_sync(0xffffffffu, look), turns = (g1 - g0 + kThreads - 1) / kThreads;
-    if (look) sm.owner[warp][__popc(looking & ((1u << lane) - 1))] = (uint8_t)lane;
-    __syncwarp();
-    for (uint32_t i = lane; i < __popc(looking) * turns; i += 32) {
-      const uint32_t n = i / turns, g = g0 + warp * 32 + sm.owner[warp][n] + (i - n * turns) * kThreads;
-      if (g >= g1) continue;
-      const uint4 v = __ldg(body + g);
-#pragma unroll
-      for (int e = 0; e < E; ++e) consider(element<BF16>(v, e), split.head + g * E + e);
     }
   }
   __syncthreads();
@@ -292,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 6) k_token_logprobs(const LogprobPar
   const bool bad = isnan(sum) || top == INFINITY;  // a NaN or +inf reaches the sum
 
   // ---- to the first CTA
-  SliceSmem *first = &sm;
+  SliceSmem<kThreads> *first = &sm;
   if (p.slices > 1) {
     cluster.barrier_wait();
     first = cluster.map_shared_rank(&sm, 0);
@@ -300,11 +313,76 @@ __global__ void __launch_bounds__(kThreads, 6) k_token_logprobs(const LogprobPar
   if (t == 0) first->part[slice] = make_float4(top, sum, weighted, bad ? 1.0f : 0.0f);
   unsigned long long *best = first->best + slice * p.top_k;
   if (p.top_k) {
-    const uint32_t n = sm.n_list;
+    auto note = [&](float x, uint32_t i) {
+      const uint32_t at = atomicAdd(&sm.n_list, 1u);
+      if (at < kList) sm.list[at] = key_of(x, i);
+    };
+    const uint32_t n_look = sm.n_look, per_part = chunks_per_part * kChunk;
+    if (n_look <= kLook) {
+      if (extra < p.cols && !(x_extra < bound)) note(x_extra, extra);  // a NaN is nobody's maximum, but comes first
+      for (uint32_t i = t; i < n_look * per_part; i += kThreads) {
+        const uint32_t n = i / per_part, what = sm.look[n], g = g0 + (what & 0xffffu) + ((what >> 16) * per_part + (i - n * per_part)) * kThreads;
+        if (g >= g1) continue;
+        const uint4 v = __ldg(body + g);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (!(element<BF16>(v, e) < bound)) note(element<BF16>(v, e), split.head + g * E + e);
+      }
+    }
+    __syncthreads();
+    uint32_t n = sm.n_list;
+    if (n_look > kLook || n > kList) {
+      // Many equal the bound (equal logits, columns masked out): the larger ones, and of the equal ones the first, in their order.
+      __syncthreads();
+      if (t == 0) sm.n_list = 0;
+      __syncthreads();
+      if (extra < p.cols && !(x_extra <= bound)) note(x_extra, extra);
+      for (uint32_t g = g0 + t; g < g1; g += kThreads) {
+        const uint4 v = __ldg(body + g);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (!(element<BF16>(v, e) <= bound)) note(element<BF16>(v, e), split.head + g * E + e);
+      }
+      __syncthreads();
+      n = sm.n_list;
+      auto take = [&](uint32_t mine, auto &&value_at) {  // this thread's `mine` equal elements stand behind those of the threads before it
+        uint32_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= (uint32_t)o) upto += x;
+        }
+        if (lane == 31) sm.taken[warp] = upto;
+        __syncthreads();
+        uint32_t before = 0, all = 0;
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < (int)warp) before += sm.taken[w];
+          all += sm.taken[w];
+        }
+        for (uint32_t i = 0, at = n + before + upto - mine; i < mine && at < p.top_k; ++i, ++at) sm.list[at] = value_at(i);
+        __syncthreads();
+        n = min(n + all, max(n, p.top_k));
+      };
+      if (n < p.top_k) {
+        const bool in_head = extra < split.head;
+        take(in_head && x_extra == bound ? 1u : 0u, [&](uint32_t) { return key_of(x_extra, extra); });
+        for (uint32_t gb = g0; gb < g1 && n < p.top_k; gb += kThreads) {
+          const uint32_t g = gb + t;
+          uint32_t equal = 0;
+          if (g < g1) {
+            const uint4 v = __ldg(body + g);
+#pragma unroll
+            for (int e = 0; e < E; ++e) equal |= element<BF16>(v, e) == bound ? 1u << e : 0u;
+          }
+          take(__popc(equal), [&](uint32_t i) { return key_of(bound, split.head + g * E + __fns(equal, 0, i + 1)); });
+        }
+        if (n < p.top_k) take(!in_head && extra < p.cols && x_extra == bound ? 1u : 0u, [&](uint32_t) { return key_of(x_extra, extra); });
+      }
+    }
     if (n <= kList) {
       for (uint32_t k = n + t; k < p.top_k; k += kThreads) best[k] = 0;  // a slice with fewer elements than k
-      rank_list(sm.list, n, p.top_k, best);
-    } else {  // one after another
+      rank_list<kThreads>(sm.list, n, p.top_k, best);
+    } else {  // more than the list holds are larger than the bound: one after another
       unsigned long long last = ~0ull;
       for (uint32_t k = 0; k < p.top_k; ++k) {
         unsigned long long most = 0;
@@ -335,7 +413,6 @@ __global__ void __launch_bounds__(kThreads, 6) k_token_logprobs(const LogprobPar
   } else {
     __syncthreads();
   }
-  if (t >= max(32u, p.slices * p.top_k)) return;
   RowResult r = {-INFINITY, 0.0f, 0.0f, false};
   for (uint32_t s = 0; s < p.slices; ++s) {
     r.top = fmaxf(r.top, sm.part[s].x);
@@ -355,11 +432,12 @@ __global__ void __launch_bounds__(kThreads, 6) k_token_logprobs(const LogprobPar
       if (t < p.top_k) r.write_top(p, row, t, sm.best[t]);
     } else {  // keys that are not there are 0 and differ from each other in nothing: they are never among the k best, which exist
       const uint32_t n = p.slices * p.top_k;
-      const unsigned long long key = t < n ? sm.best[t] : 0ull;
-      uint32_t rank = 0;
-      if (key)
+      for (uint32_t i = t; i < n; i += kThreads) {
+        const unsigned long long key = sm.best[i];
+        uint32_t rank = key ? 0u : n;
         for (uint32_t j = 0; j < n; ++j) rank += sm.best[j] > key ? 1u : 0u;
-      if (key && rank < p.top_k) r.write_top(p, row, rank, key);
+        if (rank < p.top_k) r.write_top(p, row, rank, key);
+      }
     }
   }
 }
@@ -376,9 +454,9 @@ struct LogprobGradParams {
 
 // A CTA takes kGradGroups groups a thread of one row, all loaded before the first is worked on. SAME_PHASE: gradient rows lie at the same place between
 // 16-byte boundaries as logits rows, so that they are stored in groups too.
-constexpr int kGradGroups = 4;
+constexpr int kGradGroups = 4, kGradThreads = 256;
 template <bool BF16, bool SAME_PHASE>
-__global__ void __launch_bounds__(kThreads) k_token_logprobs_backward(const LogprobGradParams p) {
+__global__ void __launch_bounds__(kGradThreads) k_token_logprobs_backward(const LogprobGradParams p) {
   ptx::pdl_wait();
   constexpr int E = RowSplit<BF16>::kElements;
   const uint32_t row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks, t = threadIdx.x;
@@ -386,11 +464,11 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs_backward(const Logp
   uint8_t *drow = static_cast<uint8_t *>(p.d_logits) + (size_t)row * p.d_stride * (16 / E);
   const RowSplit<BF16> split(grow, p.cols);
   const uint4 *body = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(grow) + (size_t)split.head * (16 / E));
-  const uint32_t g0 = chunk * (kGradGroups * kThreads) + t;
+  const uint32_t g0 = chunk * (kGradGroups * kGradThreads) + t;
   uint4 v[kGradGroups];
 #pragma unroll
   for (int i = 0; i < kGradGroups; ++i)
-    if (g0 + i * kThreads < split.groups) v[i] = __ldcs(body + g0 + i * kThreads);
+    if (g0 + i * kGradThreads < split.groups) v[i] = __ldcs(body + g0 + i * kGradThreads);
   const int32_t target = __ldg(p.targets + row);
   const bool has = target >= 0 && (uint32_t)target < p.cols;
   const float lse = __ldg(p.lse + row), entropy = __ldg(p.entropy + row);
@@ -413,7 +491,7 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs_backward(const Logp
   }
 #pragma unroll
   for (int i = 0; i < kGradGroups; ++i) {
-    const uint32_t group = g0 + i * kThreads, c0 = split.head + group * E;
+    const uint32_t group = g0 + i * kGradThreads, c0 = split.head + group * E;
     if (group >= split.groups) break;
     float d[E];
 #pragma unroll
@@ -441,31 +519,32 @@ int finish(int st) {
   return st;
 }
 
-// One CTA a row; more, up to eight, while the rows alone do not give every SM three and a CTA still has a chunk.
+// Rows that give every SM three CTAs of 128 threads get one each; fewer are cut among up to eight of 512 while a CTA still has a chunk.
 template <bool BF16>
 int launch_forward(LogprobParams &p, cudaStream_t s) {
   const uint32_t n = p.cols / RowSplit<BF16>::kElements + 1;
   const int n_sm = sm_count();
   if (n_sm == 0) return DF_ERR_CUDA;
-  uint32_t slices = 1;
-  while (slices < kMaxSlices && (uint64_t)p.rows * slices < 3u * (uint64_t)n_sm && n > slices * (kChunk * kThreads)) slices *= 2;
-  p.slices = slices;
-  p.groups = (n + slices * kThreads - 1) / (slices * kThreads);
-  if ((uint64_t)p.rows * slices > 0x7fffffffull) return DF_ERR_UNSUPPORTED;
-  const int st = check_cuda(launch_clusters(k_token_logprobs<BF16>, slices, dim3(p.rows * slices), dim3(kThreads), 0, s, p));
+  const bool many = p.rows >= 3u * (uint32_t)n_sm || n <= kChunk * 128;
+  const uint32_t threads = many ? 128 : 512;
+  p.slices = 1;
+  while (!many && p.slices < kMaxSlices && (uint64_t)p.rows * p.slices < 2u * (uint64_t)n_sm && n > p.slices * (kChunk * threads)) p.slices *= 2;
+  p.groups = (n + p.slices * threads - 1) / (p.slices * threads);
+  const int st = check_cuda(launch_clusters(many ? k_token_logprobs<BF16, 128> : k_token_logprobs<BF16, 512>, p.slices, dim3(p.rows * p.slices),
+                                            dim3(threads), 0, s, p));
   note_launch();
   return st;
 }
 
 template <bool BF16>
 int launch_backward(LogprobGradParams &p, cudaStream_t s) {
-  constexpr uint32_t per = kGradGroups * kThreads * RowSplit<BF16>::kElements;
+  constexpr uint32_t per = kGradGroups * kGradThreads * RowSplit<BF16>::kElements;
   p.chunks = (p.cols + per - 1) / per;
   if ((uint64_t)p.rows * p.chunks > 0x7fffffffull) return DF_ERR_UNSUPPORTED;
   const uint64_t elt = BF16 ? 2 : 4;
   const bool same_phase = (((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.d_logits)) | (p.stride * elt ^ p.d_stride * elt)) & 15u) == 0;
   const int st = check_cuda(launch_kernel(same_phase ? k_token_logprobs_backward<BF16, true> : k_token_logprobs_backward<BF16, false>,
-                                          dim3(p.rows * p.chunks), dim3(kThreads), 0, s, p));
+                                          dim3(p.rows * p.chunks), dim3(kGradThreads), 0, s, p));
   note_launch();
   return st;
 }
