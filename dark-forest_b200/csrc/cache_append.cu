@@ -19,7 +19,7 @@
 namespace df {
 namespace {
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 128;
 
 struct AppendParams {
   const void *src[2];  // k, v
@@ -32,25 +32,41 @@ struct AppendParams {
   uint32_t aligned[2]; // rows start on boundaries of four elements
 };
 
-// four elements of a row
+// Four elements of a row, as they lie there (half the registers for bf16) and as numbers.
 template <bool BF16>
-__device__ __forceinline__ float4 load4(const void *base, unsigned long long e, bool aligned) {
-  if (BF16) {
+struct Raw4 {
+  uint32_t w[BF16 ? 2 : 4];
+};
+template <bool BF16>
+__device__ __forceinline__ Raw4<BF16> load4(const void *base, unsigned long long e, bool aligned) {
+  Raw4<BF16> r;
+  if constexpr (BF16) {
     const uint16_t *p = static_cast<const uint16_t *>(base) + e;
-    uint32_t lo, hi;
     if (aligned) {
-      const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
-      lo = w.x;
-      hi = w.y;
+      const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+      r.w[0] = v.x; r.w[1] = v.y;
     } else {
-      lo = __ldg(p) | ((uint32_t)__ldg(p + 1) << 16);
-      hi = __ldg(p + 2) | ((uint32_t)__ldg(p + 3) << 16);
+      r.w[0] = __ldg(p) | ((uint32_t)__ldg(p + 1) << 16);
+      r.w[1] = __ldg(p + 2) | ((uint32_t)__ldg(p + 3) << 16);
     }
-    return make_float4(__uint_as_float(lo << 16), __uint_as_float(lo & 0xffff0000u), __uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u));
+  } else {
+    const uint32_t *p = static_cast<const uint32_t *>(base) + e;
+    if (aligned) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+      r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.w[i] = __ldg(p + i);
+    }
   }
-  const float *p = static_cast<const float *>(base) + e;
-  if (aligned) return __ldg(reinterpret_cast<const float4 *>(p));
-  return make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ float4 numbers(const Raw4<BF16> &r) {
+  if constexpr (BF16)
+    return make_float4(__uint_as_float(r.w[0] << 16), __uint_as_float(r.w[0] & 0xffff0000u), __uint_as_float(r.w[1] << 16), __uint_as_float(r.w[1] & 0xffff0000u));
+  else
+    return make_float4(__uint_as_float(r.w[0]), __uint_as_float(r.w[1]), __uint_as_float(r.w[2]), __uint_as_float(r.w[3]));
 }
 
 __device__ __forceinline__ uint32_t largest(uint32_t m, const float4 &x) {  // of the magnitudes, as bits: infinities and NaN come out on top
@@ -81,10 +97,10 @@ __device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d)
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
-template <bool BF16, int FORMAT>
-__global__ void __launch_bounds__(kAppendThreads) k_cache_append(const AppendParams p) {
+// kHeld: turns of the warp whose elements stay in registers: those of 16 tokens (two to a turn up to 64 dims, one beyond).
+template <bool BF16, int FORMAT, int kHeld>
+__global__ void __launch_bounds__(kAppendThreads, BF16 ? (kHeld == 8 ? 8 : 6) : (kHeld == 8 ? 6 : 4)) k_cache_append(const AppendParams p) {
   ptx::pdl_wait();
-  constexpr int kHeld = 16;  // turns of the warp whose elements stay in registers
   const uint32_t lane = threadIdx.x & 31;
   const unsigned long long warp = (unsigned long long)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
   const uint32_t which = (uint32_t)(warp % (2 * p.H)), h = which >> 1, kv = which & 1;
@@ -102,13 +118,48 @@ __global__ void __launch_bounds__(kAppendThreads) k_cache_append(const AppendPar
   float *scales = kv ? p.scale[1] : p.scale[0];
   const unsigned long long stride = kv ? p.stride[1] : p.stride[0];
   const bool aligned = (kv ? p.aligned[1] : p.aligned[0]) != 0;
-  for (uint32_t t = (uint32_t)first; t < t_end; ++t) {
-    const int32_t slot = __ldg(p.slots + t);
-    if (slot < 0 || slot >= n_slots) continue;
-    const uint32_t page = (uint32_t)slot / p.P, row = (uint32_t)slot % p.P;
-    if (t > 0 && row > 0 && __ldg(p.slots + t - 1) == slot - 1) continue;  // not the first of its run
-    uint32_t n = 1;
-    for (;;) {  // the run's length
+  // the warp's window of slots, one to a lane, and the beginnings of runs in it
+  const uint32_t t0 = (uint32_t)first, window = t_end - t0;
+  const bool in_window = lane < window;
+  const int32_t my_slot = in_window ? __ldg(p.slots + t0 + lane) : -1;
+  int32_t before = __shfl_up_sync(0xffffffffu, my_slot, 1);
+  if (lane == 0) before = t0 > 0 ? __ldg(p.slots + t0 - 1) : -2;
+  const bool valid = my_slot >= 0 && my_slot < n_slots;
+  const uint32_t my_page = (uint32_t)my_slot / p.P, my_row = (uint32_t)my_slot - my_page * p.P;
+  const bool goes_on = valid && my_row > 0 && before == my_slot - 1;
+  const uint32_t going_on = __ballot_sync(0xffffffffu, goes_on);
+  // A run's first turn and the scale that its page has are loaded while the run before it is worked on: a decode step's runs are of
+  // one token each, and their loads would otherwise follow one another (4096 tokens of 8 heads of 128: 57 us, XX this way).
+  struct Run {
+    uint32_t at, page, row, n;
+    int32_t slot;
+    float old;
+    Raw4<BF16> first;
+  };
+  const unsigned long long e0 = (unsigned long long)h * p.D + x;
+  auto begin = [&](uint32_t at) {
+    Run r;
+    r.at = at;
+    r.slot = __shfl_sync(0xffffffffu, my_slot, at);
+    r.page = __shfl_sync(0xffffffffu, my_page, at);
+    r.row = __shfl_sync(0xffffffffu, my_row, at);
+    r.n = 1 + (at == 31 ? 0u : __ffs(~(going_on >> (at + 1))) - 1);  // (bits above the window are 0)
+    r.old = r.row > 0 ? scales[(size_t)r.page * p.H + h] : 0.0f;
+    r.first = Raw4<BF16>{};
+    if (in_row && sub < r.n) r.first = load4<BF16>(src, (unsigned long long)(t0 + at + sub) * stride + e0, aligned);
+    return r;
+  };
+  uint32_t begins = __ballot_sync(0xffffffffu, valid && !goes_on);
+  if (!begins) return;
+  Run next = begin(__ffs(begins) - 1);
+  while (begins) {
+    const Run run = next;
+    begins &= begins - 1;
+    if (begins) next = begin(__ffs(begins) - 1);
+    const uint32_t at = run.at, t = t0 + at, page = run.page, row = run.row;
+    const int32_t slot = run.slot;
+    uint32_t n = run.n;
+    while (at + n >= window) {  // the run may go on behind the window
       const uint32_t i = n + lane;
       const bool in = row + i < p.P && t + i < p.n_tokens && __ldg(p.slots + t + i) == slot + (int32_t)i;
       const uint32_t together = __ballot_sync(0xffffffffu, in);
@@ -118,25 +169,30 @@ __global__ void __launch_bounds__(kAppendThreads) k_cache_append(const AppendPar
       }
       n += 32;
     }
-    const unsigned long long e0 = (unsigned long long)h * p.D + x;
     auto element = [&](uint32_t i) { return (unsigned long long)(t + i) * stride + e0; };
-    float4 held[kHeld];
+    Raw4<BF16> held[kHeld];
+    held[0] = run.first;
+    if (sub >= run.n && sub < n && in_row) held[0] = load4<BF16>(src, element(sub), aligned);
     uint32_t amax = 0;
+    if (n > turn) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const uint32_t r = i * turn + sub;
-      held[i] = in_row && r < n ? load4<BF16>(src, element(r), aligned) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int i = 1; i < kHeld; ++i) {
+        const uint32_t r = i * turn + sub;
+        if (in_row && r < n) held[i] = load4<BF16>(src, element(r), aligned);
+        else held[i] = Raw4<BF16>{};
+      }
+#pragma unroll
+      for (int i = 1; i < kHeld; ++i) amax = largest(amax, numbers(held[i]));
     }
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) amax = largest(amax, held[i]);
+    amax = largest(amax, numbers(held[0]));
     for (uint32_t r = kHeld * turn + sub; r < n; r += turn)
-      if (in_row) amax = largest(amax, load4<BF16>(src, element(r), aligned));
+      if (in_row) amax = largest(amax, numbers(load4<BF16>(src, element(r), aligned)));
     amax = __reduce_max_sync(0xffffffffu, amax);
     float *scale_at = scales + (size_t)page * p.H + h;
     uint8_t *slice = cache + ((size_t)page * p.H + h) * p.P * p.D;
     float scale = scale_for<FORMAT>(amax);
     if (row > 0) {
-      const float old = *scale_at;
+      const float old = run.old;
       if (!(old <= scale)) scale = isnan(scale) ? scale : old;  // larger already, or NaN
       if (old < scale) {                                        // the older rows' codes, in steps of the new scale
         const float ratio = old / scale;
@@ -147,19 +203,27 @@ __global__ void __launch_bounds__(kAppendThreads) k_cache_append(const AppendPar
                                       cache_value<FORMAT>((w >> 16) & 0xff) * ratio, cache_value<FORMAT>(w >> 24) * ratio);
         }
       }
-      __syncwarp();  // every lane has read the old scale
     }
     if (lane == 0) *scale_at = scale;
     const bool poisoned = isnan(scale);
+    // Dividing by a power of two is multiplying by its inverse; a scale of the caller's own may be another number.
+    const uint32_t scale_bits = __float_as_uint(scale);
+    const bool power = (scale_bits & 0x7fffffu) == 0 && scale_bits >= 0x00800000u && scale_bits < 0x7f000000u;
+    const float inverse = __uint_as_float(0x7f000000u - scale_bits);
     auto put = [&](uint32_t r, const float4 &v) {
-      const uint32_t w = poisoned ? 0u : to_codes<FORMAT>(v.x / scale, v.y / scale, v.z / scale, v.w / scale);
+      uint32_t w = 0u;
+      if (power) w = to_codes<FORMAT>(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
+      else if (!poisoned) w = to_codes<FORMAT>(v.x / scale, v.y / scale, v.z / scale, v.w / scale);
       *reinterpret_cast<uint32_t *>(slice + (size_t)(row + r) * p.D + x) = w;
     };
+    if (in_row && sub < n) put(sub, numbers(held[0]));
+    if (n > turn) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-      if (in_row && i * turn + sub < n) put(i * turn + sub, held[i]);
+      for (int i = 1; i < kHeld; ++i)
+        if (in_row && i * turn + sub < n) put(i * turn + sub, numbers(held[i]));
+    }
     for (uint32_t r = kHeld * turn + sub; r < n; r += turn)
-      if (in_row) put(r, load4<BF16>(src, element(r), aligned));
+      if (in_row) put(r, numbers(load4<BF16>(src, element(r), aligned)));
   }
 }
 
@@ -170,11 +234,17 @@ int finish(int st) {
 
 template <bool BF16, int FORMAT>
 int launch(AppendParams &p, cudaStream_t s) {
-  const unsigned long long warps = (unsigned long long)p.n_tokens * 2 * p.H;
-  p.per_warp = 1;
+  // A slot to a warp while that leaves no more than two rounds of resident warps (16 an SM: registers), else windows of up to 32 slots: in a
+  // prompt only every 16th slot or so begins a run, and warps that find none cost more than the others' work (8205 tokens of 12 heads: 110 us with a slot
+  // to a warp, XX with windows).
+  const int n_sm = sm_count();
+  if (n_sm == 0) return DF_ERR_CUDA;
+  const unsigned long long all = (unsigned long long)p.n_tokens * 2 * p.H, two_rounds = 32ull * (unsigned)n_sm;
+  p.per_warp = all <= two_rounds ? 1u : all >= 32 * two_rounds ? 32u : (uint32_t)((all + two_rounds - 1) / two_rounds);
+  const unsigned long long warps = (p.n_tokens + p.per_warp - 1ull) / p.per_warp * 2 * p.H;
   const unsigned long long blocks = (warps + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
   if (blocks > 0x7fffffffull) return DF_ERR_UNSUPPORTED;
-  const int st = check_cuda(launch_kernel(k_cache_append<BF16, FORMAT>, dim3((unsigned)blocks), dim3(kAppendThreads), 0, s, p));
+  const int st = check_cuda(launch_kernel(p.D <= 64 ? k_cache_append<BF16, FORMAT, 8> : k_cache_append<BF16, FORMAT, 16>, dim3((unsigned)blocks), dim3(kAppendThreads), 0, s, p));
   note_launch();
   return st;
 }
