@@ -58,12 +58,12 @@ struct AttendParams {
   float scale_log2;
 };
 
-// How query rows fill the 16 rows of an instruction: 8 fp32 rows and their second parts; 8 bf16 rows, the other half empty (few rows: what
-// the kernel waits for is latency, and half the accumulators let more warps in); 16 bf16 rows.
-enum Mode { kFp32, kBf16Few, kBf16 };
+// How query rows fill the 16 rows of an instruction: 8 fp32 rows and their second parts, or 16 bf16 rows. A warp takes 16 rows (fp32: two instructions' worth,
+// which share the widened codes), or, where requests have few, 8: half the accumulators and operands then let more of its work overlap.
+enum Mode { kFp32Few, kFp32, kBf16Few, kBf16 };
 // Rows that one warp takes, and the size of a partial state.
 template <Mode MODE>
-constexpr uint32_t kRows = MODE == kBf16 ? 16 : 8;
+constexpr uint32_t kRows = MODE == kBf16 || MODE == kFp32 ? 16 : 8;
 template <Mode MODE, int DP>
 constexpr uint32_t kPartialFloats = kComputeWarps * kRows<MODE> * (DP + 2);
 
@@ -294,20 +294,25 @@ template <int DP>
 constexpr uint32_t kSubBytes = 16 * DP;  // a box of 16 tokens, or less where D < DP: whole swizzle periods
 // CTAs of an SM, by the registers that they need, and stages of the ring, by the shared memory that is left to each.
 template <Mode MODE>
-constexpr int kCtas = MODE == kBf16 ? 2 : 3;
+constexpr int kCtas = MODE == kFp32Few ? 3 : 2;
 template <Mode MODE, int DP>
-constexpr uint32_t kStagesOf = MODE == kBf16 ? (DP == 128 ? 5 : 8) : (DP == 128 ? 3 : 6);
+constexpr uint32_t kStagesOf = MODE == kFp32Few ? (DP == 128 ? 3 : 6) : MODE == kFp32 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 5 : 8);
+// A warp's region of shared memory: its rows of q as operands (16 bytes a lane and k-step, for each instruction that shares a code), later 8 rows of sums.
+template <Mode MODE>
+constexpr uint32_t kTiles = MODE == kFp32 ? 2 : 1;
+template <Mode MODE, int DP>
+constexpr uint32_t kWarpBytes = kTiles<MODE> * 8 * DP * 4;
 template <Mode MODE, int DP>
 constexpr uint32_t kRingBytes = kStagesOf<MODE, DP> * 2 * (kStageTokens / 16) * kSubBytes<DP>;
 template <Mode MODE, int DP>
-constexpr uint32_t kSmemBytes = 1024 + kRingBytes<MODE, DP> + kComputeWarps * 8 * DP * 4;
+constexpr uint32_t kSmemBytes = 1024 + kRingBytes<MODE, DP> + kComputeWarps * kWarpBytes<MODE, DP>;
 
 template <Mode MODE, int FORMAT, int DP>
 __global__ void __launch_bounds__(kThreads, kCtas<MODE>)
 k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttendParams p) {
   constexpr uint32_t ROWS = kRows<MODE>, kStages = kStagesOf<MODE, DP>;
-  constexpr bool BF16 = MODE != kFp32;
-  constexpr int KT = DP / 16, NT = DP / 8, RW = MODE == kBf16 ? 2 : 1;  // k-steps, n-tiles, rows of a lane
+  constexpr bool BF16 = MODE == kBf16Few || MODE == kBf16;
+  constexpr int KT = DP / 16, NT = DP / 8, RW = ROWS / 8, MT = kTiles<MODE>;  // k-steps, n-tiles, rows of a lane
   extern __shared__ uint8_t smem_raw[];
   __shared__ float2 s_scale[kStages][kStageTokens / 16];  // k_scale, v_scale of a stage's boxes
   __shared__ float s_m[kComputeWarps][8], s_l[kComputeWarps][8];
@@ -417,13 +422,13 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       gr.slice = in ? (uint32_t)gr.page * p.kv_heads + head : p.n_pages * p.kv_heads;  // behind the last slice: zeros
       gr.scale = in ? make_float2(__ldg(p.k_scale + gr.slice), __ldg(p.v_scale + gr.slice)) : make_float2(0.0f, 0.0f);
     };
+    uint32_t slot = 0, phase = 1;  // (the phase that a slot's second use waits for is the first, 0: see the flip at the ring's end)
     look_up(now);
     look_up_scales(now);
     while (now.stages) {
       look_up(then);
-      for (uint32_t s = 0; s < now.stages; ++s, ++stage) {
-        const uint32_t slot = stage % kStages;
-        if (stage >= kStages && !ptx::mbar_wait_warp(a_empty + 8 * slot, (stage / kStages - 1) & 1, &s_abort)) {
+      for (uint32_t s = 0; s < now.stages; ++s) {
+        if (stage >= kStages && !ptx::mbar_wait_warp(a_empty + 8 * slot, phase, &s_abort)) {
           if (lane == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
           goto loaded;
         }
@@ -436,6 +441,11 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           const uint32_t dst = ring + (slot * 2 * 4 + lane % 4) * kSubBytes<DP>;
           ptx::tma_load_3d(dst, &k_map, a_full + 8 * slot, 0, (int)now.line, (int)now.slice);
           ptx::tma_load_3d(dst + 4 * kSubBytes<DP>, &v_map, a_full + 8 * slot, 0, (int)now.line, (int)now.slice);
+        }
+        ++stage;
+        if (++slot == kStages) {
+          slot = 0;
+          phase ^= 1;
         }
       }
       if (then.stages) look_up_scales(then);
@@ -453,7 +463,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   // ---------------------------------------------------------------- the computing warps
   const uint32_t g = lane >> 2, c = lane & 3;
   bool ok = true;
-  uint8_t *q_at = ring_bytes + kRingBytes<MODE, DP> + warp * (8 * DP * 4) + lane * 16;
+  uint32_t slot = 0, phase = 0;  // of the next stage
+  uint8_t *q_at = ring_bytes + kRingBytes<MODE, DP> + warp * kWarpBytes<MODE, DP> + lane * 16;
   // Tokens of a lane's accumulators: tile j, columns 2c and 2c + 1. With 64-byte rows the order below keeps two rows of a 128-byte
   // line together, which the swizzle then spreads over all banks.
   auto token_of = [&](uint32_t j, uint32_t col) { return DP == 128 ? 8 * j + col : 4 * (col >> 1) + 2 * j + (col & 1); };
@@ -538,7 +549,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         } else {
           split_halves(raw[i][kt].at(0) * down, raw[i][kt].at(1) * down, a[0][0], a[0][1]);
           split_halves(raw[i][kt].at(2) * down, raw[i][kt].at(3) * down, a[1][0], a[1][1]);
-          *reinterpret_cast<uint4 *>(q_at + kt * 512) = make_uint4(a[0][0], a[0][1], a[1][0], a[1][1]);
+          *reinterpret_cast<uint4 *>(q_at + (kt * MT + i) * 512) = make_uint4(a[0][0], a[0][1], a[1][0], a[1][1]);
         }
       }
       m[i] = -FLT_MAX;
@@ -556,24 +567,32 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     // takes a half. Every warp waits for every stage and gives it back, also one that has nothing to do with it: a wait names its phase by a
     // parity, and a warp that had passed over a stage of a slot would take that stage for the next one.
     const uint32_t pair0 = weight == kComputeWarps ? 0u : token_warp & 1, pair1 = weight == kComputeWarps ? 2u : pair0 + 1;
-    for (uint32_t tile = tile0; tile < tile1; ++tile, ++stage) {
-      const uint32_t slot = stage % kStages;
-      ok = ok && ptx::mbar_wait_warp(a_full + 8 * slot, (stage / kStages) & 1, &s_abort);
-      if (!ok) continue;
-      const uint8_t *stage_at = ring_bytes + slot * 2 * 4 * kSubBytes<DP>;
+    bool idle = weight == 1 && token_warp >> 1 != 0;
+    for (uint32_t tile = tile0; ok && tile < tile1; ++tile) {
+      ok = ptx::mbar_wait_warp(a_full + 8 * slot, phase, &s_abort);
+      const uint32_t here = slot;
+      if (++slot == kStages) {
+        slot = 0;
+        phase ^= 1;
+      }
       auto give_back = [&]() {
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(a_empty + 8 * slot);
+        if (lane == 0) ptx::mbar_arrive(a_empty + 8 * here);
       };
+      if (idle || !ok) {
+        if (ok) give_back();
+        idle = false;
+        continue;
+      }
+      idle = weight == 1;
+      const uint8_t *stage_at = ring_bytes + here * 2 * 4 * kSubBytes<DP>;
       bool given_back = false;
-      const bool idle = weight == 1 && ((tile - tile0) & 1) != token_warp >> 1;
-      for (uint32_t pair = idle ? pair1 : pair0; pair < pair1; ++pair) {
+      for (uint32_t pair = pair0; pair < pair1; ++pair) {
         const uint32_t token0 = tile * kStageTokens + pair * 32;
         if (token0 >= see_any) break;
-        const float2 scale[2] = {s_scale[slot][2 * pair], s_scale[slot][2 * pair + 1]};
+        const float2 scale[2] = {s_scale[here][2 * pair], s_scale[here][2 * pair + 1]};
         const uint8_t *k_at = stage_at + 2 * pair * kSubBytes<DP>, *v_at = k_at + 4 * kSubBytes<DP>;
         // ---- scores
-        float acc[4][4];
+        float acc[MT][4][4];
 #pragma unroll
         for (int k4 = 0; k4 < KT / 4; ++k4) {
           uint32_t w[4][4];
@@ -584,68 +603,96 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           }
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
-            uint32_t a[4];
-            if (MODE == kBf16Few) {
-              const uint2 q2 = *reinterpret_cast<const uint2 *>(q_at + (k4 * 4 + kk) * 512);
-              a[0] = q2.x; a[1] = 0u; a[2] = q2.y; a[3] = 0u;
-            } else {
-              const uint4 q4 = *reinterpret_cast<const uint4 *>(q_at + (k4 * 4 + kk) * 512);
-              a[0] = q4.x; a[1] = q4.y; a[2] = q4.z; a[3] = q4.w;
+            uint32_t a[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              if (MODE == kBf16Few) {
+                const uint2 q2 = *reinterpret_cast<const uint2 *>(q_at + (k4 * 4 + kk) * 512);
+                a[mt][0] = q2.x; a[mt][1] = 0u; a[mt][2] = q2.y; a[mt][3] = 0u;
+              } else {
+                const uint4 q4 = *reinterpret_cast<const uint4 *>(q_at + ((k4 * 4 + kk) * MT + mt) * 512);
+                a[mt][0] = q4.x; a[mt][1] = q4.y; a[mt][2] = q4.z; a[mt][3] = q4.w;
+              }
             }
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt) {
               uint32_t b0, b1;
               widen_word<FORMAT>(w[nt][kk], b0, b1);
-              if (k4 == 0 && kk == 0) mma_half_first(acc[nt], a, b0, b1);
-              else mma_half(acc[nt], a, b0, b1);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                if (k4 == 0 && kk == 0) mma_half_first(acc[mt][nt], a[mt], b0, b1);
+                else mma_half(acc[mt][nt], a[mt], b0, b1);
+              }
             }
           }
         }
-        // ---- V's bytes: the stage is given back before the longer half of the work on it
+        // ---- V's bytes. Where registers allow (kEarly) all of them now, so that the stage is given back before the longer half of the work on
+        // it; else two words of a lane's piece at a time, when they are used.
         const bool masked = token0 + 32 > see_all;
-        uint32_t w[2][4][NT / 4];
+        constexpr bool kEarly = RW == 1;
+        constexpr int kWords = kEarly ? NT / 4 : 2;
+        uint32_t w[2][4][kWords];
+        auto load_v = [&](int part) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+          for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint8_t *at = v_at + b * kSubBytes<DP> + v_off[k];
-            if constexpr (DP == 128) {
-              const uint4 v = *reinterpret_cast<const uint4 *>(at);
-              w[b][k][0] = v.x; w[b][k][1] = v.y; w[b][k][2] = v.z; w[b][k][3] = v.w;
-            } else {
-              const uint2 v = *reinterpret_cast<const uint2 *>(at);
-              w[b][k][0] = v.x; w[b][k][1] = v.y;
+            for (int k = 0; k < 4; ++k) {
+              const uint8_t *at = v_at + b * kSubBytes<DP> + v_off[k] + 8 * part;
+              if constexpr (kWords == 4) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(at);
+                w[b][k][0] = v.x; w[b][k][1] = v.y; w[b][k][2] = v.z; w[b][k][3] = v.w;
+              } else {
+                const uint2 v = *reinterpret_cast<const uint2 *>(at);
+                w[b][k][0] = v.x; w[b][k][1] = v.y;
+              }
             }
-            // behind the last token that a row sees a box may hold any bytes, and an 8-bit float may be NaN
-            if (FORMAT == DF_CACHE_E4M3 && masked && token0 + 16 * b + token_of(k >> 1, 2 * c + (k & 1)) >= see_any) {
+          if (FORMAT == DF_CACHE_E4M3 && masked) {  // behind the last token that a row sees a box may hold any bytes, and an 8-bit float may be NaN
 #pragma unroll
-              for (int n4 = 0; n4 < NT / 4; ++n4) w[b][k][n4] = 0u;
-            }
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const bool behind_all = token0 + 16 * b + token_of(k >> 1, 2 * c + (k & 1)) >= see_any;
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) w[b][k][i] = behind_all ? 0u : w[b][k][i];
+              }
           }
-        if (pair + 1 == pair1) {
-          give_back();
-          given_back = true;
+        };
+        if (kEarly) {
+          load_v(0);
+          if (pair + 1 == pair1) {
+            __syncwarp();
+            give_back();
+            given_back = true;
+          }
         }
         // ---- weights
         // The two boxes' weights meet one scale of V, the larger one; a row that sees none of a box's tokens takes nothing of
         // it, whatever its scale is (it may be NaN).
         const float v_scale = fmaxf(scale[0].y, scale[1].y);
         const bool v_alike = scale[0].y == scale[1].y && !masked;
-        uint32_t pa[2][4];
+        uint32_t pa[MT][2][4];
         float v_row[RW], before[RW];
         bool grew = false;
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
           before[i] = m[i];
           v_row[i] = 0.0f;
-          if (MODE == kBf16Few || (i == 1 && !second_rows)) pa[0][1] = pa[0][3] = pa[1][1] = pa[1][3] = 0u;
-          if (i == 1 && !second_rows) continue;
+          if (MODE == kBf16Few || (BF16 && i == 1 && !second_rows)) pa[0][0][1] = pa[0][0][3] = pa[0][1][1] = pa[0][1][3] = 0u;
+          if (i == 1 && !second_rows) {
+            if (!BF16) {
+#pragma unroll
+              for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) pa[MT - 1][b][k] = 0u;
+            }
+            continue;
+          }
           const float f[2] = {scale[0].x * norm[i], scale[1].x * norm[i]};
           float s[4][2];
 #pragma unroll
           for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) s[nt][k] = (BF16 ? acc[nt][2 * i + k] : acc[nt][k] + acc[nt][2 + k]) * f[nt >> 1];
+            for (int k = 0; k < 2; ++k) s[nt][k] = (BF16 ? acc[0][nt][2 * i + k] : acc[i % MT][nt][k] + acc[i % MT][nt][2 + k]) * f[nt >> 1];
           if (masked) {
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt)
@@ -678,11 +725,11 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             if (BF16) {
-              pa[b][i] = halves(s[2 * b][0], s[2 * b][1]);
-              pa[b][2 + i] = halves(s[2 * b + 1][0], s[2 * b + 1][1]);
+              pa[0][b][i] = halves(s[2 * b][0], s[2 * b][1]);
+              pa[0][b][2 + i] = halves(s[2 * b + 1][0], s[2 * b + 1][1]);
             } else {
-              split_halves(s[2 * b][0], s[2 * b][1], pa[b][0], pa[b][1]);
-              split_halves(s[2 * b + 1][0], s[2 * b + 1][1], pa[b][2], pa[b][3]);
+              split_halves(s[2 * b][0], s[2 * b][1], pa[i % MT][b][0], pa[i % MT][b][1]);
+              split_halves(s[2 * b + 1][0], s[2 * b + 1][1], pa[i % MT][b][2], pa[i % MT][b][3]);
             }
           }
         }
@@ -697,28 +744,36 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         // ---- output
 #pragma unroll
         for (int n4 = 0; n4 < NT / 4; ++n4) {
+          if (!kEarly && n4 % 2 == 0) load_v(n4 / 2);
+          const int i4 = kEarly ? n4 : n4 % 2;
           uint32_t b0[2][4], b1[2][4];
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            widen_pairs<FORMAT>(w[b][0][n4], w[b][1][n4], b0[b]);
-            widen_pairs<FORMAT>(w[b][2][n4], w[b][3][n4], b1[b]);
+            widen_pairs<FORMAT>(w[b][0][i4], w[b][1][i4], b0[b]);
+            widen_pairs<FORMAT>(w[b][2][i4], w[b][3][i4], b1[b]);
           }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < 4; ++k) {
+            const int n = n4 * 4 + k;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
               float d[4];
-              mma_half_first(d, pa[0], b0[0][k], b1[0][k]);
-              mma_half(d, pa[1], b0[1][k], b1[1][k]);
-              const int n = n4 * 4 + k;
+              mma_half_first(d, pa[mt][0], b0[0][k], b1[0][k]);
+              mma_half(d, pa[mt][1], b0[1][k], b1[1][k]);
               if (BF16) {
                 o[0][n] = ptx::fma2(make_float2(v_row[0], v_row[0]), make_float2(d[0], d[1]), o[0][n]);
-                if (RW == 2 && second_rows) o[RW - 1][n] = ptx::fma2(make_float2(v_row[RW - 1], v_row[RW - 1]), make_float2(d[2], d[3]), o[RW - 1][n]);
+                if (RW == 2) o[RW - 1][n] = ptx::fma2(make_float2(v_row[RW - 1], v_row[RW - 1]), make_float2(d[2], d[3]), o[RW - 1][n]);
               } else {
-                o[0][n] = ptx::fma2(make_float2(v_row[0], v_row[0]), ptx::add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])), o[0][n]);
+                o[mt][n] = ptx::fma2(make_float2(v_row[mt], v_row[mt]), ptx::add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])), o[mt][n]);
               }
             }
+          }
         }
       }
-      if (!given_back) give_back();
+      if (!given_back) {
+        __syncwarp();
+        give_back();
+      }
     }
     if (!ok && lane == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
 #pragma unroll
@@ -773,7 +828,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         if (valid[i]) {
           if (c == 0) { s_m[warp][g] = m[i]; s_l[warp][g] = l[i]; }
 #pragma unroll
-          for (int n = 0; n < DP / 16; ++n) *reinterpret_cast<float4 *>(merge + (warp * 8 + g) * DP + 4 * spread(g, c * (DP / 16) + n)) = four(i, 4 * n);
+          for (int n = 0; n < DP / 16; ++n) *reinterpret_cast<float4 *>(merge + warp * (kWarpBytes<MODE, DP> / 4) + g * DP + 4 * spread(g, c * (DP / 16) + n)) = four(i, 4 * n);
         }
         compute_barrier();
         for (uint32_t e = t; e < weight * 8 * (DP / 4); e += 32 * kComputeWarps) {
@@ -781,7 +836,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           if (row >= rows) break;
           Running sum;
           for (uint32_t w = w0; w < kComputeWarps; w += weight)
-            sum.add(s_m[w][r8], s_l[w][r8], *reinterpret_cast<const float4 *>(merge + (w * 8 + r8) * DP + 4 * spread(r8, dim / 4)));
+            sum.add(s_m[w][r8], s_l[w][r8], *reinterpret_cast<const float4 *>(merge + w * (kWarpBytes<MODE, DP> / 4) + r8 * DP + 4 * spread(r8, dim / 4)));
           const float4 x = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
           if (!split) {
             finish_row(global_row(row), dim, x, sum.m, sum.l);
@@ -954,12 +1009,11 @@ extern "C" int df_cache_attention(const void *q, const void *k_cache, const void
   p.out_aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
   p.scale_log2 = scale * kLog2e;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // Eight bf16 rows to a warp while requests have no more on average: what the kernel is then bound by is the latency of a
-  // warp's steps, and with half the accumulators twice the warps fit an SM.
+  // Eight rows to a warp while requests have no more on average.
   const bool few = (uint64_t)n_tokens * p.group <= 8ull * n_requests;
   auto run = [&](auto format_constant) {
     constexpr int FORMAT = decltype(format_constant)::value;
-    if (!q_bf16) return launch_for_head<kFp32, FORMAT>(p, k_cache, v_cache, s);
+    if (!q_bf16) return few ? launch_for_head<kFp32Few, FORMAT>(p, k_cache, v_cache, s) : launch_for_head<kFp32, FORMAT>(p, k_cache, v_cache, s);
     return few ? launch_for_head<kBf16Few, FORMAT>(p, k_cache, v_cache, s) : launch_for_head<kBf16, FORMAT>(p, k_cache, v_cache, s);
   };
   return finish(format == DF_CACHE_INT8 ? run(std::integral_constant<int, DF_CACHE_INT8>{}) : run(std::integral_constant<int, DF_CACHE_E4M3>{}));
