@@ -293,10 +293,10 @@ __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 12
 template <int DP>
 constexpr uint32_t kSubBytes = 16 * DP;  // a box of 16 tokens, or less where D < DP: whole swizzle periods
 // CTAs of an SM, by the registers that they need, and stages of the ring, by the shared memory that is left to each.
-template <Mode MODE>
-constexpr int kCtas = MODE == kFp32Few ? 3 : 2;
 template <Mode MODE, int DP>
-constexpr uint32_t kStagesOf = MODE == kFp32Few ? (DP == 128 ? 3 : 6) : MODE == kFp32 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 5 : 8);
+constexpr int kCtas = DP == 64 ? (kRows<MODE> == 8 ? 4 : 3) : MODE == kFp32Few ? 3 : 2;
+template <Mode MODE, int DP>
+constexpr uint32_t kStagesOf = DP == 64 ? (kRows<MODE> == 8 ? 5 : 6) : MODE == kFp32Few ? 3 : MODE == kFp32 ? 4 : 5;
 // A warp's region of shared memory: its rows of q as operands (16 bytes a lane and k-step, for each instruction that shares a code), later 8 rows of sums.
 template <Mode MODE>
 constexpr uint32_t kTiles = MODE == kFp32 ? 2 : 1;
@@ -308,7 +308,7 @@ template <Mode MODE, int DP>
 constexpr uint32_t kSmemBytes = 1024 + kRingBytes<MODE, DP> + kComputeWarps * kWarpBytes<MODE, DP>;
 
 template <Mode MODE, int FORMAT, int DP>
-__global__ void __launch_bounds__(kThreads, kCtas<MODE>)
+__global__ void __launch_bounds__(kThreads, kCtas<MODE, DP>)
 k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttendParams p) {
   constexpr uint32_t ROWS = kRows<MODE>, kStages = kStagesOf<MODE, DP>;
   constexpr bool BF16 = MODE == kBf16Few || MODE == kBf16;

@@ -45,7 +45,7 @@ PARTS = [[(1, 1)], [(1, 9)], [(4, 7)], [(2, 3), (1, 8), (4, 5), (1, 0), (1, 2)],
 def stage_counts():
     with open(SOURCE) as f:
         text = f.read()
-    return sorted({int(n) for n in re.findall(r"\d+", re.search(r"kStagesOf = (.*?);", text).group(1).replace("DP == 128", "").replace("kBf16", "").replace("kFp32", ""))})
+    return sorted({int(n) for n in re.findall(r"[?:] (\d+)\b(?! \?)", re.search(r"kStagesOf = (.*?);", text).group(1).replace("(", "").replace("kRows<MODE> == 8", "few"))})
 
 
 @pytest.mark.parametrize("parts", PARTS)
