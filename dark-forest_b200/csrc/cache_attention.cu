@@ -20,16 +20,20 @@
 // Work. A CTA is one warp that loads (tensor-map copies of 16 tokens, 128-byte swizzle: the reads above are then free of bank conflicts at
 // head sizes 64 and 128) and four that compute, over a ring of stages of 64 tokens. A request with no more rows (query tokens times heads per K/V head)
 // than a warp takes is computed with its tokens dealt to the four warps; one with more has its rows dealt to them, and every warp goes over
-// all tokens. The whole step is one line of units (64 tokens of one head and row tile; four units where rows are dealt, which takes four times as
-// long); the grid's CTAs take equal parts of it, whatever the requests' lengths. A segment (request, row tile, head) that is cut leaves partial (m, l, out)
-// states in the workspace, and the CTA that finishes its last part adds them in their order. Every CTA forms the sums over the requests itself.
+// all tokens. Work is dealt out as cache_line.cuh says; a stage where rows are dealt counts four units, since it takes four times as long. Calls of many rows go
+// to cache_attention_many.cu.
+//
+// What it reaches. 32 requests of 200 to 16000 tokens, one new each, 32 heads on 8 of 128, bf16 and e4m3: 73 us for 342 MB, 4.7 TB/s, 70 % of a copy's rate. One request of
+// 131073 tokens, 16 heads of 128, fp32 and int8: 112 us for 537 MB, 4.8 TB/s. One of 300 tokens, 12 heads of 64: 6.7 us, of which 2.4 are a launch. The copies
+// alone (no arithmetic) took 92 us of the second. What is left is issue: 800 instructions per warp for 32 tokens, 350 of them widening (two per clock
+// and SM), the others softmax and products; and 8 to 10 us for a segment's beginning, its end and the addition of its parts.
 #include <float.h>
 #include <math.h>
 
 #include <mutex>
 #include <type_traits>
 
-#include "cache_codes.cuh"
+#include "cache_line.cuh"
 #include "sm100_ptx.cuh"
 
 namespace df {
@@ -37,26 +41,8 @@ namespace {
 
 using ptx::ex2_approx;
 
-constexpr uint32_t kStageTokens = 64, kComputeWarps = 4, kThreads = 32 * (kComputeWarps + 1);
+constexpr uint32_t kComputeWarps = 4, kThreads = 32 * (kComputeWarps + 1);
 constexpr float kWeightBits = 15.0f;  // weights are held times 2^15, so that halves reach down to 2^-39 of the largest one
-constexpr uint32_t kMaxGrid = 640;
-constexpr uint32_t kCounterBytes = 4096;  // a counter per CTA, at the workspace's beginning
-
-struct AttendParams {
-  const void *q;
-  const float *k_scale, *v_scale;
-  const int32_t *table, *lens, *starts;
-  void *out;
-  float *lse;
-  unsigned int *counters;
-  float *partial;
-  unsigned int *status;
-  unsigned long long q_stride;
-  uint32_t n_requests, n_tokens, heads, kv_heads, group, D, P, n_pages, width;
-  uint32_t q_aligned, out_aligned;  // 16-byte boundaries
-  uint32_t whole;  // the line would be too long in units
-  float scale_log2;
-};
 
 // How query rows fill the 16 rows of an instruction: 8 fp32 rows and their second parts, or 16 bf16 rows. A warp takes 16 rows (fp32: two instructions' worth,
 // which share the widened codes), or, where requests have few, 8: half the accumulators and operands then let more of its work overlap.
@@ -64,130 +50,15 @@ enum Mode { kFp32Few, kFp32, kBf16Few, kBf16 };
 // Rows that one warp takes, and the size of a partial state.
 template <Mode MODE>
 constexpr uint32_t kRows = MODE == kBf16 || MODE == kFp32 ? 16 : 8;
+// What a segment costs besides its stages: 5 to 8 us beside 1.2 us for a stage of 128-byte tokens with every SM busy. Without it CTAs with several short
+// segments ended 20 us after the others (32 ragged requests: 94 us, 77 with it).
+template <Mode MODE, int DP>
+struct Work {
+  static constexpr uint32_t kRows = df::kRows<MODE>, kSegmentUnits = DP == 128 ? 6 : 10, kThreads = df::kThreads;
+  static constexpr bool kDeal = true;
+};
 template <Mode MODE, int DP>
 constexpr uint32_t kPartialFloats = kComputeWarps * kRows<MODE> * (DP + 2);
-
-struct Request {
-  uint32_t first, rows, q_len, len, tiles, row_tiles;
-  uint32_t weight_log2;  // warps that the rows of a tile are dealt to (1, 2, 4; the tokens to the others): units of a stage
-};
-
-template <uint32_t ROWS>
-__device__ __forceinline__ Request request_of(const AttendParams &p, uint32_t r) {
-  Request q;
-  const long long most = (long long)p.width * p.P;
-  q.len = (uint32_t)min((long long)max(__ldg(p.lens + r), 0), most);
-  const int b = max(0, min(__ldg(p.starts + r), (int)p.n_tokens)), e = max(b, min(__ldg(p.starts + r + 1), (int)p.n_tokens));
-  q.first = (uint32_t)b;
-  q.q_len = (uint32_t)(e - b);
-  q.rows = q.q_len * p.group;
-  q.weight_log2 = q.rows <= ROWS ? 0u : q.rows <= 2 * ROWS ? 1u : 2u;
-  q.row_tiles = (q.rows + (ROWS << q.weight_log2) - 1) / ROWS >> q.weight_log2;
-  q.tiles = max(1u, (q.len + kStageTokens - 1) / kStageTokens);
-  return q;
-}
-
-// What a CTA does of one segment.
-struct Part {
-  Request rq;
-  uint32_t r, h, row0;           // K/V head; first row of the row tile
-  uint32_t t0, t1;               // stages [t0, t1)
-  uint32_t limit;                // tokens that the tile's last row sees
-  uint32_t parts, first_cta;     // of the whole segment
-};
-
-// What a segment costs besides its stages (its rows of q, the sums over warps, its results), in units: 5 to 8 us beside 1.2 us for a stage of 128-byte
-// tokens with every SM busy. Counted at the segment's beginning; without it CTAs with several short segments ended 20 us after the others
-// (32 ragged requests: 94 us, 77 with it).
-template <int DP>
-constexpr uint32_t kSegmentUnits = DP == 128 ? 6 : 10;
-template <int DP>
-__device__ __forceinline__ uint32_t span_of(const Request &q) { return (q.tiles << q.weight_log2) + kSegmentUnits<DP>; }
-template <int DP>
-__device__ __forceinline__ uint32_t tile_at(const Request &q, uint32_t x) {  // stages of a segment in front of its unit x
-  return x <= kSegmentUnits<DP> ? 0u : (x - kSegmentUnits<DP>) >> q.weight_log2;
-}
-
-// The line of units (or, where no segment is cut, of segments) and this CTA's place on it. Its length is below 2^31 (the launcher sees to
-// it), so that its divisions are of 32 bits: those of 64 took a part's first microseconds.
-struct Line {
-  uint32_t at, end, base;  // base: of request r
-  uint32_t per_cta, r;
-  bool whole;  // counted in segments
-};
-
-template <uint32_t ROWS, int DP>
-__device__ __forceinline__ bool next_part(const AttendParams &p, Line &line, Part &part) {
-  while (line.at < line.end) {
-    Request q = request_of<ROWS>(p, line.r);
-    uint32_t span = line.whole ? 1u : span_of<DP>(q);
-    while (line.at >= line.base + span * q.row_tiles * p.kv_heads) {  // on to the request that holds line.at (it is below the line's end)
-      line.base += span * q.row_tiles * p.kv_heads;
-      q = request_of<ROWS>(p, ++line.r);
-      span = line.whole ? 1u : span_of<DP>(q);
-    }
-    const uint32_t idx = line.whole ? line.at - line.base : (line.at - line.base) / span;
-    const uint32_t s0 = line.base + idx * span, s1 = s0 + span;
-    const uint32_t row_tile = q.row_tiles == 1 ? 0u : idx / p.kv_heads;
-    part.rq = q;
-    part.r = line.r;
-    part.h = idx - row_tile * p.kv_heads;
-    part.row0 = row_tile * (ROWS << q.weight_log2);
-    part.parts = 1;
-    part.first_cta = blockIdx.x;
-    part.t0 = 0;
-    part.t1 = q.tiles;
-    const uint32_t from = line.at, stop = min(s1, line.end);
-    line.at = stop;
-    if (from != s0 || stop != s1) {  // cut
-      part.t0 = tile_at<DP>(q, from - s0);
-      if (stop < s1) part.t1 = tile_at<DP>(q, stop - s0);
-      // A boundary between CTAs counts down to whole stages; so the first CTA that a segment reaches may have none of it, every other one has
-      // some (a CTA has at least four units more than a segment's beginning takes).
-      uint32_t c0 = s0 / line.per_cta;
-      const uint32_t c1 = (s1 - 1) / line.per_cta;
-      if (tile_at<DP>(q, (c0 + 1) * line.per_cta - s0) == 0) ++c0;
-      part.first_cta = c0;
-      part.parts = c1 - c0 + 1;
-      if (part.t1 <= part.t0) continue;
-    }
-    const uint32_t last_row = min(q.rows, part.row0 + (ROWS << q.weight_log2)) - 1;
-    const int see = (int)q.len - (int)q.q_len + (int)(p.group == 1 ? last_row : last_row / p.group) + 1;
-    part.limit = (uint32_t)max(0, min(see, (int)q.len));
-    part.t1 = max(part.t0, min(part.t1, (part.limit + kStageTokens - 1) / kStageTokens));
-    return true;
-  }
-  return false;
-}
-
-// ---------------------------------------------------------------- widening codes to pairs of halves
-// int8: 1024 + (code + 128) is a half with the code in its last bits. e4m3: an instruction.
-__device__ __forceinline__ uint32_t half_of_biased(uint32_t biased) {  // two halves 1024 + (code + 128)
-  const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
-  const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&biased), bias);
-  return *reinterpret_cast<const uint32_t *>(&x);
-}
-__device__ __forceinline__ void halves_of_e4m3(uint32_t w, uint32_t &low, uint32_t &high) {  // bytes (0, 1) and (2, 3)
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(low), "=r"(high) : "r"(w));
-}
-// The four codes of a word as two pairs: bytes (0, 1) and (2, 3).
-template <int FORMAT>
-__device__ __forceinline__ void widen_word(uint32_t w, uint32_t &first, uint32_t &second) {
-  if (FORMAT == DF_CACHE_INT8) {
-    const uint32_t u = w ^ 0x80808080u;
-    first = half_of_biased(__byte_perm(u, 0x64646464u, 0x4140));
-    second = half_of_biased(__byte_perm(u, 0x64646464u, 0x4342));
-  } else {
-    halves_of_e4m3(w, first, second);
-  }
-}
-// Byte i of two words each, for the four i: pair[i] = (a.byte i, b.byte i).
-template <int FORMAT>
-__device__ __forceinline__ void widen_pairs(uint32_t a, uint32_t b, uint32_t (&pair)[4]) {
-  const uint32_t lo = __byte_perm(a, b, 0x5140), hi = __byte_perm(a, b, 0x7362);  // a0 b0 a1 b1, a2 b2 a3 b3
-  widen_word<FORMAT>(lo, pair[0], pair[1]);
-  widen_word<FORMAT>(hi, pair[2], pair[3]);
-}
 
 __device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
@@ -202,91 +73,6 @@ __device__ __forceinline__ void mma_half_first(float (&d)[4], const uint32_t (&a
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
-
-__device__ __forceinline__ uint32_t halves(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-// a pair of floats as halves and what they leave
-__device__ __forceinline__ void split_halves(float x, float y, uint32_t &first, uint32_t &second) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  first = *reinterpret_cast<const uint32_t *>(&h);
-  second = halves(x - f.x, y - f.y);
-}
-
-// Four elements of a row of q, as they lie there.
-template <bool BF16>
-struct Raw4 {
-  uint32_t w[BF16 ? 2 : 4];
-  __device__ __forceinline__ void load(const void *q, unsigned long long e, bool aligned) {
-    if constexpr (BF16) {
-      const uint16_t *p = static_cast<const uint16_t *>(q) + e;
-      if (aligned) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-        w[0] = v.x; w[1] = v.y;
-      } else {
-        w[0] = __ldg(p) | ((uint32_t)__ldg(p + 1) << 16);
-        w[1] = __ldg(p + 2) | ((uint32_t)__ldg(p + 3) << 16);
-      }
-    } else {
-      const uint32_t *p = static_cast<const uint32_t *>(q) + e;
-      if (aligned) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __ldg(p + i);
-      }
-    }
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (uint32_t &x : w) x = 0u;
-  }
-  __device__ __forceinline__ float at(int i) const {
-    if constexpr (BF16) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-    else return __uint_as_float(w[i]);
-  }
-};
-
-template <bool BF16>
-__device__ __forceinline__ void store_row4(void *out, size_t e, bool aligned, const float (&x)[4]) {
-  if (BF16) {
-    uint32_t w[2];
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[0]) : "f"(x[1]), "f"(x[0]));
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[1]) : "f"(x[3]), "f"(x[2]));
-    uint16_t *p = static_cast<uint16_t *>(out) + e;
-    if (aligned) {
-      *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-    }
-  } else {
-    float *p = static_cast<float *>(out) + e;
-    if (aligned) {
-      *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = x[i];
-    }
-  }
-}
-
-// Sums (m, l, o[4]) states one after another.
-struct Running {
-  float m = -FLT_MAX, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  __device__ __forceinline__ void add(float m2, float l2, const float4 &o2) {
-    const float top = fmaxf(m, m2), a = ex2_approx(m - top), b = ex2_approx(m2 - top);
-    m = top;
-    l = l * a + l2 * b;
-    o[0] = o[0] * a + o2.x * b;
-    o[1] = o[1] * a + o2.y * b;
-    o[2] = o[2] * a + o2.z * b;
-    o[3] = o[3] * a + o2.w * b;
-  }
-};
 
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // the compute warps; all of them come to each
 
@@ -310,6 +96,7 @@ constexpr uint32_t kSmemBytes = 1024 + kRingBytes<MODE, DP> + kComputeWarps * kW
 template <Mode MODE, int FORMAT, int DP>
 __global__ void __launch_bounds__(kThreads, kCtas<MODE, DP>)
 k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttendParams p) {
+  using W = Work<MODE, DP>;
   constexpr uint32_t ROWS = kRows<MODE>, kStages = kStagesOf<MODE, DP>;
   constexpr bool BF16 = MODE == kBf16Few || MODE == kBf16;
   constexpr int KT = DP / 16, NT = DP / 8, RW = ROWS / 8, MT = kTiles<MODE>;  // k-steps, n-tiles, rows of a lane
@@ -319,7 +106,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   __shared__ Line s_line[kComputeWarps];
   __shared__ Part s_part[kComputeWarps];
   __shared__ uint64_t s_full[kStages], s_empty[kStages];
-  __shared__ uint32_t s_units[kThreads], s_segments[kThreads], s_most[kThreads / 32], s_last, s_abort;
+  __shared__ LineSmem<W> s_sums;
+  __shared__ uint32_t s_last, s_abort;
   const uint32_t t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const uint32_t ring = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t *ring_bytes = smem_raw + (ring - ptx::smem_u32(smem_raw));
@@ -336,53 +124,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   }
   ptx::pdl_wait();
 
-  // ---- the line: sums over the requests, and the request at which this CTA begins
-  const uint32_t per = (p.n_requests + kThreads - 1) / kThreads, r0 = min(p.n_requests, t * per), r1 = min(p.n_requests, r0 + per);
-  uint32_t units = 0, segments = 0, most = 0;
-  for (uint32_t r = r0; r < r1; ++r) {
-    const Request q = request_of<ROWS>(p, r);
-    const uint32_t n = q.row_tiles * p.kv_heads;
-    segments += n;
-    units += n * span_of<DP>(q);
-    if (n) most = max(most, span_of<DP>(q));
-  }
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t a = __shfl_up_sync(0xffffffffu, units, o), b = __shfl_up_sync(0xffffffffu, segments, o);
-    if (lane >= (uint32_t)o) { units += a; segments += b; }
-  }
-  most = __reduce_max_sync(0xffffffffu, most);
-  s_units[t] = units;
-  s_segments[t] = segments;
-  if (lane == 0) s_most[warp] = most;
-  __syncthreads();
-  uint32_t all_units = 0, all_segments = 0;
-  most = 0;
-#pragma unroll
-  for (uint32_t w = 0; w < kThreads / 32; ++w) {
-    all_units += s_units[32 * w + 31];
-    all_segments += s_segments[32 * w + 31];
-    most = max(most, s_most[w]);
-  }
   Line line;
-  const uint32_t G = gridDim.x, seg_per = (all_segments + G - 1) / G, unit_per = max(kSegmentUnits<DP> + 8u, (all_units + G - 1) / G);
-  line.whole = p.whole || (unsigned long long)seg_per * most <= unit_per + kSegmentUnits<DP>;  // cutting costs another end
-  line.per_cta = line.whole ? seg_per : unit_per;
-  const uint32_t total = line.whole ? all_segments : all_units;
-  if ((unsigned long long)line.per_cta * blockIdx.x >= total) return;  // (the whole CTA)
-  line.at = line.per_cta * blockIdx.x;
-  line.end = min(total, line.at + line.per_cta);
-  // the warp, then the lane, then the request of those lane's that line.at falls to: every warp looks for itself
-  {
-    const uint32_t *sums = line.whole ? s_segments : s_units;
-    uint32_t base = 0, w = 0;
-    while (line.at >= base + sums[32 * w + 31]) base += sums[32 * w++ + 31];
-    const uint32_t mine = base + sums[32 * w + lane];
-    const uint32_t owner = __ffs(__ballot_sync(0xffffffffu, line.at < mine)) - 1;
-    const uint32_t before = __shfl_sync(0xffffffffu, mine, max(owner, 1u) - 1);
-    line.base = owner == 0 ? base : before;
-    line.r = (32 * w + owner) * per;  // next_part goes on to the request
-  }
+  if (!begin_line<W>(p, s_sums, line)) return;
 
   const uint32_t a_full = ptx::smem_u32(&s_full[0]), a_empty = ptx::smem_u32(&s_empty[0]);
   const uint32_t chunks = p.D / 16;  // 16-byte pieces of a row
@@ -404,7 +147,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       gr.stages = 0;
       if (tile >= part.t1) {
         do {
-          if (!next_part<ROWS, DP>(p, line, part)) return;
+          if (!next_part<W>(p, line, part)) return;
         } while (part.t0 >= part.t1);  // a part that sees nothing
         tile = part.t0;
       }
@@ -488,7 +231,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     Line next = s_line[warp];
     __syncwarp();
     Part found;
-    if (!next_part<ROWS, DP>(p, next, found)) break;
+    if (!next_part<W>(p, next, found)) break;
     if (lane == 0) {
       s_line[warp] = next;
       s_part[warp] = found;
@@ -793,12 +536,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     auto state_of = [&](uint32_t cta) {  // the first CTA of a segment has it last, every other one first
       return p.partial + (size_t)(2 * cta + (cta == part.first_cta ? 1 : 0)) * kPartialFloats<MODE, DP>;
     };
-    auto finish_row = [&](size_t row, uint32_t dim, const float4 &x, float mm, float ll) {  // four dims of a finished row
-      const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-      const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
-      if (dim < p.D) store_row4<BF16>(p.out, row * p.D + dim, p.out_aligned, y);
-      if (dim == 0 && p.lse) p.lse[row] = ll == 0.0f ? -INFINITY : (mm - kWeightBits + log2f(ll)) * kLn2;
-    };
+    auto finish_row = [&](size_t row, uint32_t dim, const float4 &x, float mm, float ll) { finish_row4<BF16>(p, row, dim, x, mm, ll, kWeightBits); };
     auto global_row = [&](uint32_t row) {
       const uint32_t rr = part.row0 + row;
       const uint32_t j = p.group == 1 ? rr : rr / p.group;
@@ -920,22 +658,10 @@ uint32_t resident_ctas() {
   return d.grid;
 }
 
-// The pool as lines of 128 bytes: a slice (page, head) is P * D / 128 of them, 16 tokens D / 8.
-bool encode_pool_map(CUtensorMap *map, const void *pool, const AttendParams &p) {
-  PFN_encodeTiled encode = get_encode_tiled();
-  if (!encode) return false;
-  const cuuint64_t lines = (cuuint64_t)p.P * p.D / 128;
-  const cuuint64_t dims[3] = {128, lines, (cuuint64_t)p.n_pages * p.kv_heads};
-  const cuuint64_t strides[2] = {128, lines * 128};
-  const cuuint32_t box[3] = {128, p.D / 8, 1}, step[3] = {1, 1, 1};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <Mode MODE, int FORMAT, int DP>
 int launch(AttendParams &p, const void *k_cache, const void *v_cache, cudaStream_t s) {
   constexpr uint32_t kFits = (DF_CACHE_WORKSPACE_BYTES - kCounterBytes) / (2 * kPartialFloats<MODE, DP> * 4);
-  static_assert(kFits >= 2 * 148 && kMaxGrid * 4 <= kCounterBytes, "workspace");
+  static_assert(kFits >= 2 * 148, "workspace");
   uint32_t grid = resident_ctas<MODE, FORMAT, DP>();
   if (grid == 0) return DF_ERR_CUDA;
   grid = grid < kFits ? grid : kFits;
@@ -1009,8 +735,13 @@ extern "C" int df_cache_attention(const void *q, const void *k_cache, const void
   p.out_aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
   p.scale_log2 = scale * kLog2e;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // Eight rows to a warp while requests have no more on average.
-  const bool few = (uint64_t)n_tokens * p.group <= 8ull * n_requests;
+  // How many rows requests have on average decides who multiplies. Up to 8: a warp's few. Up to 32: 16 rows a warp. Above: tiles of 128 rows on tcgen05, which
+  // take the same time for 9 rows as for 32. Measured over 3000 to 6000 cached tokens, mma.sync to tcgen05, bf16 and fp32: 16 requests of 12 heads of 64, 16
+  // rows 37 to 81 us, 52 to 97; 32 rows 56 to 82, 80 to 98; 64 rows 97 to 83, 142 to 102. 16 requests of 8 heads of 128, 20 rows 68 to 77, 105 to 90;
+  // 32 rows 74 to 78, 113 to 91; 64 rows 133 to 84, 198 to 102. One request of 12 heads of 64, 24 rows 27 to 23, 31 to 27; 40 rows 53 to 24, 59 to 28.
+  const uint64_t rows = (uint64_t)n_tokens * p.group;
+  if (rows > 32ull * n_requests) return finish(cache_attention_many(p, k_cache, v_cache, q_bf16 != 0, format, s));
+  const bool few = rows <= 8ull * n_requests;
   auto run = [&](auto format_constant) {
     constexpr int FORMAT = decltype(format_constant)::value;
     if (!q_bf16) return few ? launch_for_head<kFp32Few, FORMAT>(p, k_cache, v_cache, s) : launch_for_head<kFp32, FORMAT>(p, k_cache, v_cache, s);

@@ -63,7 +63,99 @@ def test_a_warp_that_passes_over_stages_comes_early():
     assert phases_early(roles) != set()
 
 
-def test_whole_warps_wait_as_warps():
-    with open(SOURCE) as f:
+def many(parts, ring):
+    """k_cache_attention_many over parts of n stages, `ring` stages of codes. Four widening warps do the same: two stand for them; a row role for the even stages and one for
+    the odd ones."""
+    load, mma, widen, rows = Role(), Role(), [Role(), Role()], [Role(), Role()]
+    at = 0
+    for n_part, n in enumerate(parts):
+        for role in rows:
+            role.mark("q written", n_part)
+            role.arrive("Q_FULL")
+        mma.wait("Q_FULL", n_part)
+
+        def scores(j):
+            mma.wait("K_FULL%d" % (j % 2), j // 2)
+            if j >= 2:
+                mma.wait("S_FREE%d" % (j % 2), j // 2 - 1)
+            mma.mark("scores", j)
+            mma.arrive("S_FULL%d" % (j % 2))
+            mma.arrive("K_FREE%d" % (j % 2))
+
+        for j in range(at, at + min(n, 2)):
+            scores(j)
+        for i in range(n):
+            j = at + i
+            if i + 2 < n:
+                scores(j + 2)
+            mma.wait("V_FULL%d" % (j % 2), j // 2)
+            mma.wait("P_FULL%d" % (j % 2), j // 2)
+            if i == 0 and n_part:
+                mma.wait("O_FREE", n_part - 1)
+            mma.mark("product", j)
+            if i == 0:
+                mma.mark("output begun", n_part)
+            mma.arrive("PV_DONE%d" % (j % 2))
+
+        def keys(role, j):
+            role.wait("FULL%d" % (j % ring), j // ring)
+            if j >= 2:
+                role.wait("K_FREE%d" % (j % 2), j // 2 - 1)
+            role.mark("scale written", j)
+            role.arrive("K_FULL%d" % (j % 2))
+
+        for role in widen:
+            for j in range(at, at + min(n, 2)):
+                keys(role, j)
+            for j in range(at, at + n):
+                if j + 2 < at + n:
+                    keys(role, j + 2)
+                if j >= 2:
+                    role.wait("PV_DONE%d" % (j % 2), j // 2 - 1)
+                role.mark("codes read", j)
+                role.arrive("V_FULL%d" % (j % 2))
+                role.arrive("EMPTY%d" % (j % ring))
+        for j in range(at, at + n):
+            b, use, slot = j % 2, j // 2, j % ring
+            if j >= ring:
+                load.wait("EMPTY%d" % slot, j // ring - 1)
+            load.mark("codes", j)
+            load.arrive("FULL%d" % slot)
+            role = rows[b]  # even stages, odd stages
+            role.wait("S_FULL%d" % b, use)
+            role.mark("scale read", j)
+            role.arrive("S_FREE%d" % b)
+            if use:
+                role.wait("PV_DONE%d" % b, use - 1)
+            role.mark("weights written", j)
+            role.arrive("P_FULL%d" % b)
+        at += n
+        for b, role in enumerate(rows):
+            last = at - 1 - (at - 1 - b) % 2
+            if last >= at - n:
+                role.wait("PV_DONE%d" % b, last // 2)
+            role.arrive("ROWS")
+            role.wait("ROWS", n_part)
+            role.mark("output read", n_part)
+            role.arrive("O_FREE")
+    return {"load": load, "mma": mma, **{"widen %d" % i: r for i, r in enumerate(widen)}, **{"rows %d" % i: r for i, r in enumerate(rows)}}
+
+
+@pytest.mark.parametrize("parts", [[1], [2], [7], [1, 1, 1], [3, 1, 4, 2], [10, 9]])
+@pytest.mark.parametrize("stages", [4, 8])
+def test_every_wait_of_the_many_row_kernel_sees_its_phase(parts, stages):
+    roles = many(parts, stages)
+    assert phases_missed(roles) == [] and phases_early(roles) == set()
+    assert out_of_order(roles, "scale written", "scale read") == set()
+    assert out_of_order(roles, "scale read", "scale written", 4) == set()          # four places
+    assert out_of_order(roles, "codes read", "codes", stages) == set()
+    assert out_of_order(roles, "product", "weights written", 2) == set()           # two buffers of weights
+    assert out_of_order(roles, "weights written", "product") == set()
+    assert out_of_order(roles, "output read", "output begun", 1) == set()
+
+
+@pytest.mark.parametrize("source", [SOURCE, SOURCE.replace(".cu", "_many.cu")])
+def test_whole_warps_wait_as_warps(source):
+    with open(source) as f:
         src = f.read()
     assert "mbar_wait_warp" in src and lone_waits(src) == []
