@@ -12,14 +12,15 @@
 // Precision: as there. An fp32 row is two halves (two K-steps for one, into the same accumulators), and so are its weights; they are held times 2^7, and the
 // maximum that they refer to is moved when a row's has grown by 2^8 (the accumulators are then rescaled by the row's thread), so that they stay in
 // the halves' range either way. v_scale enters the weights, relative to the largest so far.
-// What bounds it. Two requests of 500 tokens over 6000 to 9000 cached ones, 12 heads of 64, fp32, int8: 99 us, 252 TFLOP/s of the formula's operations (twice as
+// What bounds it. Two requests of 500 tokens over 6000 to 9000 cached ones, 12 heads of 64, fp32, int8: 99 us, 254 TFLOP/s of the formula's operations (twice as
 // many are done). A stage takes 1.1 us; of that the tensor pipe works a quarter, and the issuing warp is busy for 1300 cycles (waits apart; one
-// instruction of 64 columns costs it 70), nearly as long as a row's warp is (2800 cycles for every second stage, with two of them and a
-// widening warp on each scheduler). 128-wide heads, 2000 tokens of 32 heads: 359 us in bf16, 468 TFLOP/s.
+// instruction of 64 columns costs it 70), nearly as long as a row's warp is (2500 cycles for every second stage, with two of them and a
+// widening warp on each scheduler). One request of 2000 tokens, 32 heads on 8 of 128: 343 us in bf16, 476 us in fp32.
 // What it came from: row tiles on mma.sync 244 us; four row warps 152; eight, each with every second stage 133; a score's factor and the shift of its exponent in one
 // operation 125; one branch around the products of a stage 114; masks and rescaling in tensor memory, without spilling the scores 108; scores two stages
-// ahead 99. Measured and left out: more registers for the row warps by setmaxnreg (more spills in all), segments counted as 2 or 4 stages more (the same, and 7 %
-// more where CTAs have two), keys widened one stage ahead only (113).
+// ahead 99; outputs added up every 16 stages, which all precision above 5.9e-6 needs, 106 (32 heads of 128 636), with states that a warp reads and writes side by side 99
+// (476). Measured and left out: more registers for the row warps by setmaxnreg (more spills in all), segments counted as 2 or 4 stages more (the
+// same, and 7 % more where CTAs have two), keys widened one stage ahead only (113).
 #include "cache_line.cuh"
 
 #include <mutex>
@@ -33,6 +34,13 @@ constexpr uint32_t kRowWarps = 8, kLoadWarp = 12, kMmaWarp = 13;  // (warps 8 to
 constexpr uint32_t kTileRows = 128;
 constexpr float kManyWeightBits = 7.0f, kRescale = 8.0f;
 constexpr uint32_t kTmemColumns = 512, kScoreColumn = 0, kWeightColumn = 128, kOutColumn = 256;  // scores 2 x 64, weights 2 x (32 + 32), outputs 2 x DP
+// Stages whose output products add up in place. The tensor cores cut their sums off, they do not round them, at every step of 16 tokens: 9000 tokens one after another
+// left an error of 6e-6 where fp32 sums leave 2e-6. So a row's thread adds an fp32 output up, rounded, every 16 stages (8 of its half), in tensor memory where there is room
+// (heads of up to 64 dims), else in the workspace. bf16 results have 8 bits: all stages.
+template <bool BF16>
+constexpr uint32_t kChunk = BF16 ? 0x40000000u : 16u;
+template <bool BF16, int DP>
+constexpr bool kSumsOutside = !BF16 && DP == 128;
 
 template <int DP>
 struct ManyWork {
@@ -41,6 +49,8 @@ struct ManyWork {
 };
 template <int DP>
 constexpr uint32_t kManyPartialFloats = kTileRows * (DP + 2);
+template <bool BF16, int DP>
+constexpr uint32_t kManyCtaFloats = 2 * kManyPartialFloats<DP> + (kSumsOutside<BF16, DP> ? kTileRows * DP : 0);  // two states; sums of the second half
 
 template <bool BF16, int DP>
 struct ManySmem {
@@ -66,7 +76,7 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
   __shared__ float2 s_box_scale[kStages][4];  // k_scale, v_scale of the boxes in the ring
   __shared__ float2 s_scale[4][4];            // and of the last four stages widened
   __shared__ uint64_t s_bars[NUM_BARS];
-  __shared__ float s_state[2][3][kTileRows];  // maximum, sum and scale of the two halves' rows
+  __shared__ float s_state[2][4][kTileRows];  // of the two halves' rows: maximum, sum, scale of the output in place and of that added up before
   __shared__ Line s_line[kRowWarps];
   __shared__ Part s_part[kRowWarps];
   __shared__ uint32_t s_last, s_abort, s_tmem;
@@ -194,7 +204,7 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
     };
     auto output = [&](uint32_t j, uint32_t i) {  // stage j, the i-th of its part
       const uint32_t b = j & 1;
-      const bool first = i < 2;  // of its half
+      const bool first = i % kChunk<BF16> < 2;  // of its half of a chunk
       if (!mbar_wait_warp(bar(V_FULL + b), (j >> 1) & 1, &s_abort)) return false;
       if (!mbar_wait_warp(bar(P_FULL + b), (j >> 1) & 1, &s_abort)) return false;
       if (i == 0 && n_part > 0 && !mbar_wait_warp(bar(O_FREE), (n_part - 1) & 1, &s_abort)) return false;
@@ -359,6 +369,15 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
       float m = -FLT_MAX, l = 0.0f, v_most = 0.0f;  // the maximum that the weights refer to; the scale that the output is in units of
       bool started = false;                         // this half has had a stage
+      float m_sum = -FLT_MAX, v_sum = -1.0f;        // of the chunks before, as m and v_most; below 0: there are none
+      const bool split = part.parts > 1;
+      auto state_of = [&](uint32_t cta) { return p.partial + (size_t)(2 * cta + (cta == part.first_cta ? 1 : 0)) * kManyPartialFloats<DP>; };
+      float *mine = state_of(blockIdx.x);  // (of no other segment while this one lasts, cut or not)
+      // A state's outputs lie as [dim / 4][row][4]: a warp's rows side by side. Where halves add up outside: the first in the segment's own state.
+      auto at_dim = [&](float *outputs, uint32_t d) { return reinterpret_cast<float4 *>(outputs) + d / 4 * kTileRows + row; };
+      auto sums_of = [&](uint32_t half) {
+        return half == 0 ? mine + 2 * kTileRows : p.partial + (size_t)gridDim.x * 2 * kManyPartialFloats<DP> + (size_t)blockIdx.x * kTileRows * DP;
+      };
       const uint32_t first_stage = stage;
       for (; ok && stage < first_stage + n; ++stage) {
         if ((stage & 1) != b) continue;
@@ -422,11 +441,18 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
           if (!ok) break;
           tc_fence_after_sync();
         }
+        const bool fresh = started && (stage - first_stage) % kChunk<BF16> < 2;  // a chunk's first of this half: what is there is added up
+        const float factor = !BF16 && fresh && v_sum > 0.0f && v_most > 0.0f ? ex2_approx(m_sum - m) * __fdividef(v_sum, v_most) : 0.0f;
+        const bool had_sum = !(v_sum < 0.0f);
+        if (fresh) {
+          m_sum = m;
+          v_sum = v_most;
+        }
         const float v_now = fmaxf(fmaxf(fmaxf(scale[0].y, scale[1].y), fmaxf(scale[2].y, scale[3].y)), v_most);
         const bool grow = top > m + kRescale;  // (also the first that a row sees)
-        const bool rescale = started && (__any_sync(0xffffffffu, grow) || v_now != v_most);
+        const bool rescale = started && !fresh && (__any_sync(0xffffffffu, grow) || v_now != v_most);
         float down_out = 1.0f;
-        if (rescale || !started) {  // (v_now is the same in all rows)
+        if (rescale || fresh || !started) {  // (v_now is the same in all rows)
           const float to = fmaxf(m, top), alpha = ex2_approx(m - to);
           m = to;
           l *= alpha;
@@ -455,6 +481,34 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
         }
         sums[0] = add2(sums[0], sums[1]);
         l += sums[0].x + sums[0].y;
+        if (!BF16 && fresh) {
+          float *outside = sums_of(b);
+#pragma unroll 1
+          for (uint32_t d = 0; d < DP; d += 16) {
+            uint32_t o[16];
+            tmem_ld16(t_out + d, o);
+            if (kSumsOutside<BF16, DP>) {
+              float4 *at = at_dim(outside, d);
+              float4 before[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) before[x] = had_sum ? at[x * kTileRows] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              tmem_wait_ld();
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                at[x * kTileRows] = make_float4(fmaf(before[x].x, factor, __uint_as_float(o[4 * x])), fmaf(before[x].y, factor, __uint_as_float(o[4 * x + 1])),
+                                    fmaf(before[x].z, factor, __uint_as_float(o[4 * x + 2])), fmaf(before[x].w, factor, __uint_as_float(o[4 * x + 3])));
+            } else {
+              uint32_t before[16];
+              if (had_sum) tmem_ld16(t_out + 2 * DP + d, before);
+              tmem_wait_ld();
+              if (had_sum) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(fmaf(__uint_as_float(before[x]), factor, __uint_as_float(o[x])));
+              }
+              tmem_st16(t_out + 2 * DP + d, o);
+            }
+          }
+        }
         if (rescale) {
 #pragma unroll 1
           for (uint32_t d = 0; d < DP; d += 16) {
@@ -480,32 +534,52 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
       s_state[b][0][row] = m;
       s_state[b][1][row] = l;
       s_state[b][2][row] = started && ok ? v_most : -1.0f;  // below 0: there is no output
+      s_state[b][3][row] = v_sum < 0.0f ? -1.0f : ex2_approx(m_sum - m) * v_sum;
       tc_fence_before_sync();
       row_barrier();
       tc_fence_after_sync();
       const float m_all = fmaxf(s_state[0][0][row], s_state[1][0][row]);
       const float w0 = ex2_approx(s_state[0][0][row] - m_all), w1 = ex2_approx(s_state[1][0][row] - m_all);
       const float l_all = s_state[0][1][row] * w0 + s_state[1][1][row] * w1, u0 = s_state[0][2][row], u1 = s_state[1][2][row];
-      const bool has0 = !(u0 < 0.0f), has1 = !(u1 < 0.0f);  // the same in all rows
-      const bool split = part.parts > 1;
-      auto state_of = [&](uint32_t cta) { return p.partial + (size_t)(2 * cta + (cta == part.first_cta ? 1 : 0)) * kManyPartialFloats<DP>; };
-      float *mine = state_of(blockIdx.x);
+      const float g0 = s_state[0][3][row], g1 = s_state[1][3][row];
+      const bool has0 = !(u0 < 0.0f), has1 = !(u1 < 0.0f), sum0 = !BF16 && !(g0 < 0.0f), sum1 = !BF16 && !(g1 < 0.0f);  // the same in all rows
       const size_t out_row = valid ? global_row(row) : 0;
 #pragma unroll 1
       for (uint32_t d = b * (DP / 2); d < (b + 1) * (DP / 2); d += 16) {  // half of the dims each
-        uint32_t o0[16], o1[16];
-        if (has0) tmem_ld16(tmem + kOutColumn + lane_base + d, o0);
-        if (has1) tmem_ld16(tmem + kOutColumn + DP + lane_base + d, o1);
-        tmem_wait_ld();
-        const float f0 = has0 ? w0 * u0 : 0.0f, f1 = has1 ? w1 * u1 : 0.0f;
+        float y[16];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) y[x] = 0.0f;
+        auto add = [&](uint32_t column, float f) {
+          uint32_t o[16];
+          tmem_ld16(tmem + column + d + lane_base, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int x = 0; x < 16; ++x) y[x] = fmaf(__uint_as_float(o[x]), f, y[x]);
+        };
+        auto add_outside = [&](float *sums, float f) {
+#pragma unroll
+          for (int x = 0; x < 16; x += 4) {
+            const float4 o = *at_dim(sums, d + x);
+            y[x] = fmaf(o.x, f, y[x]);
+            y[x + 1] = fmaf(o.y, f, y[x + 1]);
+            y[x + 2] = fmaf(o.z, f, y[x + 2]);
+            y[x + 3] = fmaf(o.w, f, y[x + 3]);
+          }
+        };
+        if (has0) add(kOutColumn, w0 * u0);
+        if (has1) add(kOutColumn + DP, w1 * u1);
+        if (kSumsOutside<BF16, DP>) {
+          if (sum0) add_outside(sums_of(0), w0 * g0);
+          if (sum1) add_outside(sums_of(1), w1 * g1);
+        } else {
+          if (sum0) add(kOutColumn + 2 * DP, w0 * g0);
+          if (sum1) add(kOutColumn + 3 * DP, w1 * g1);
+        }
         if (valid) {
 #pragma unroll
           for (int x = 0; x < 16; x += 4) {
-            float y[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = (has0 ? __uint_as_float(o0[x + k]) * f0 : 0.0f) + (has1 ? __uint_as_float(o1[x + k]) * f1 : 0.0f);
-            const float4 v = make_float4(y[0], y[1], y[2], y[3]);
-            if (split) *reinterpret_cast<float4 *>(mine + 2 * kTileRows + row * DP + d + x) = v;
+            const float4 v = make_float4(y[x], y[x + 1], y[x + 2], y[x + 3]);
+            if (split) *at_dim(mine + 2 * kTileRows, d + x) = v;
             else finish_row4<BF16>(p, out_row, d + x, v, m_all, l_all, kManyWeightBits);
           }
         }
@@ -536,18 +610,18 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
               float4 o[kAtOnce];
 #pragma unroll
               for (uint32_t k = 0; k < kAtOnce; ++k) {
-                const uint32_t at = e + k * 32 * kRowWarps, r = min(at / kPieces, rows - 1);
+                const uint32_t at = min(e + k * 32 * kRowWarps, rows * kPieces - 1), piece = at / rows, r = at - piece * rows;
                 ml[k] = __ldcg(reinterpret_cast<const float2 *>(state + 2 * r));
-                o[k] = __ldcg(reinterpret_cast<const float4 *>(state + 2 * kTileRows + r * DP + at % kPieces * 4));
+                o[k] = __ldcg(reinterpret_cast<const float4 *>(state + 2 * kTileRows) + piece * kTileRows + r);
               }
 #pragma unroll
               for (uint32_t k = 0; k < kAtOnce; ++k) sum[k].add(ml[k].x, ml[k].y, o[k]);
             }
 #pragma unroll
             for (uint32_t k = 0; k < kAtOnce; ++k) {
-              const uint32_t at = e + k * 32 * kRowWarps, r = at / kPieces;
-              if (r < rows)
-                finish_row4<BF16>(p, global_row(r), at % kPieces * 4, make_float4(sum[k].o[0], sum[k].o[1], sum[k].o[2], sum[k].o[3]), sum[k].m, sum[k].l,
+              const uint32_t at = e + k * 32 * kRowWarps, piece = at / rows, r = at - piece * rows;
+              if (piece < kPieces)
+                finish_row4<BF16>(p, global_row(r), piece * 4, make_float4(sum[k].o[0], sum[k].o[1], sum[k].o[2], sum[k].o[3]), sum[k].m, sum[k].l,
                                   kManyWeightBits);
             }
           }
@@ -573,7 +647,7 @@ template <bool BF16, int FORMAT, int DP>
 int launch(AttendParams &p, const void *k_cache, const void *v_cache, cudaStream_t s) {
   static DeviceInfo table[64];
   constexpr uint32_t smem = ManySmem<BF16, DP>::kTotal;
-  constexpr uint32_t kFits = (DF_CACHE_WORKSPACE_BYTES - kCounterBytes) / (2 * kManyPartialFloats<DP> * 4);
+  constexpr uint32_t kFits = (DF_CACHE_WORKSPACE_BYTES - kCounterBytes) / (kManyCtaFloats<BF16, DP> * 4);
   static_assert(kFits >= 160, "workspace");
   auto kernel = k_cache_attention_many<BF16, FORMAT, DP>;
   int dev = 0;
