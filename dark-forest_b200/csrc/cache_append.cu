@@ -10,7 +10,8 @@
 //
 // The tokens of one page form a run of the slot map (row, row + 1, ... of one page). A warp takes a run, one head, and K or V, so that everything that
 // shares a scale is one warp's and nothing is exchanged; its first slot says how many rows the page had. Bound by HBM: rows are read once (up to
-// kHeld rows' elements stay in registers between the maximum and the rounding), codes written once.
+// kHeld rows' elements stay in registers between the maximum and the rounding), codes written once: 8205 tokens of 12 heads of 64, fp32 to int8, 63 MB in 17 us, 3.7
+// TB/s (56 % of a copy's rate; what is missing is the start and the end of one round of warps).
 #include <math.h>
 
 #include "cache_codes.cuh"
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(kAppendThreads, BF16 ? (kHeld == 8 ? 8 : 6) : 
   const bool goes_on = valid && my_row > 0 && before == my_slot - 1;
   const uint32_t going_on = __ballot_sync(0xffffffffu, goes_on);
   // A run's first turn and the scale that its page has are loaded while the run before it is worked on: a decode step's runs are of
-  // one token each, and their loads would otherwise follow one another (4096 tokens of 8 heads of 128: 57 us, XX this way).
+  // one token each, and their loads would otherwise follow one another (4096 tokens of 8 heads of 128: 57 us, 23 this way).
   struct Run {
     uint32_t at, page, row, n;
     int32_t slot;
@@ -236,7 +237,7 @@ template <bool BF16, int FORMAT>
 int launch(AppendParams &p, cudaStream_t s) {
   // A slot to a warp while that leaves no more than two rounds of resident warps (16 an SM: registers), else windows of up to 32 slots: in a
   // prompt only every 16th slot or so begins a run, and warps that find none cost more than the others' work (8205 tokens of 12 heads: 110 us with a slot
-  // to a warp, XX with windows).
+  // to a warp, 18 with windows).  64 tokens of 8 heads, a warp each: 3.0 us, of which 2.4 are a launch.
   const int n_sm = sm_count();
   if (n_sm == 0) return DF_ERR_CUDA;
   const unsigned long long all = (unsigned long long)p.n_tokens * 2 * p.H, two_rounds = 32ull * (unsigned)n_sm;

@@ -18,7 +18,8 @@ inline bool cache_shape_valid(uint32_t n_kv_heads, uint32_t d_head, uint32_t pag
 }
 
 // The value of one code. An 8-bit float has the fields s eeee fff (bias 7): its seven low bits moved up by seven are those of a half with bias 15, i.e.
-// the value times 2^-8, subnormals included, so that no table and no special case is needed (and 0x7f reads as 480, not NaN).
+// the value times 2^-8, subnormals included, so that no table and no special case is needed (and 0x7f reads as 480, not NaN:
+// df_cache_append never writes it; the attention kernels' own conversion gives NaN).
 template <int FORMAT>
 __device__ __forceinline__ float cache_value(uint32_t code) {
   if (FORMAT == DF_CACHE_INT8) return (float)(int8_t)(uint8_t)code;
