@@ -237,7 +237,7 @@ template <bool BF16, int FORMAT>
 int launch(AppendParams &p, cudaStream_t s) {
   // A slot to a warp while that leaves no more than two rounds of resident warps (16 an SM: registers), else windows of up to 32 slots: in a
   // prompt only every 16th slot or so begins a run, and warps that find none cost more than the others' work (8205 tokens of 12 heads: 110 us with a slot
-  // to a warp, 18 with windows).  64 tokens of 8 heads, a warp each: 3.0 us, of which 2.4 are a launch.
+  // to a warp, 18 with windows). 64 tokens of 8 heads, a warp each: 3.0 us, of which 2.4 are a launch.
   const int n_sm = sm_count();
   if (n_sm == 0) return DF_ERR_CUDA;
   const unsigned long long all = (unsigned long long)p.n_tokens * 2 * p.H, two_rounds = 32ull * (unsigned)n_sm;

@@ -736,9 +736,9 @@ extern "C" int df_cache_attention(const void *q, const void *k_cache, const void
   p.scale_log2 = scale * kLog2e;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   // How many rows requests have on average decides who multiplies. Up to 8: a warp's few. Up to 32: 16 rows a warp. Above: tiles of 128 rows on tcgen05, which
-  // take the same time for 9 rows as for 32. Measured over 3000 to 6000 cached tokens, mma.sync to tcgen05, bf16 and fp32: 16 requests of 12 heads of 64, 16
-  // rows 37 to 81 us, 52 to 97; 32 rows 56 to 82, 80 to 98; 64 rows 97 to 83, 142 to 102. 16 requests of 8 heads of 128, 20 rows 68 to 77, 105 to 90;
-  // 32 rows 74 to 78, 113 to 91; 64 rows 133 to 84, 198 to 102. One request of 12 heads of 64, 24 rows 27 to 23, 31 to 27; 40 rows 53 to 24, 59 to 28.
+  // take the same time for 9 rows as for 32. Measured over 3000 to 6000 cached tokens, mma.sync to tcgen05, us, bf16 and fp32: 16 requests of 12 heads of
+  // 64, 16 rows 37 to 79, 52 to 97; 32 rows 56 to 80, 80 to 98; 64 rows 97 to 78, 142 to 102. 16 requests of 8 heads of 128, 20 rows 68 to 75, 105 to
+  // 100; 32 rows 74 to 75, 113 to 99; 64 rows 133 to 79, 198 to 106. One request of 12 heads of 64, 24 rows 27 to 22, 31 to 26; 40 rows 53 to 23, 59 to 27.
   const uint64_t rows = (uint64_t)n_tokens * p.group;
   if (rows > 32ull * n_requests) return finish(cache_attention_many(p, k_cache, v_cache, q_bf16 != 0, format, s));
   const bool few = rows <= 8ull * n_requests;

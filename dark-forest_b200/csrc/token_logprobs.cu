@@ -520,13 +520,16 @@ int finish(int st) {
   return st;
 }
 
-// Rows that give every SM three CTAs of 128 threads get one each; fewer are cut among up to eight of 512 while a CTA still has a chunk.
+// Rows that give every SM three CTAs of 128 threads get one each, and so do rows that give it one where they are short; fewer or longer ones are cut among up to eight of
+// 512 while a CTA still has a chunk. Measured, 128 threads to 512, us: 50257 fp32 columns 74 rows 12.8 to 13.5, 148 16.7 to 11.3, 296 24.5 to 15.9, 400 25.9
+// to 25.2, 592 29.5 to 29.9, 1024 39.7 to 53.5; bf16 296 13.6 to 11.8, 400 16.7 to 18.9, 1024 27.5 to 38.2. 4000 groups of 16 bytes: 8 rows 6.9 to 6.0, 64 rows 7.2 to
+// 6.3, 148 7.3 to 8.0, 300 8.5 to 11.8; 1100 groups: 8 rows 5.4 to 5.0, 300 6.0 to 10.0.
 template <bool BF16>
 int launch_forward(LogprobParams &p, cudaStream_t s) {
   const uint32_t n = p.cols / RowSplit<BF16>::kElements + 1;
   const int n_sm = sm_count();
   if (n_sm == 0) return DF_ERR_CUDA;
-  const bool many = p.rows >= 3u * (uint32_t)n_sm || n <= kChunk * 128;
+  const bool many = p.rows >= 3u * (uint32_t)n_sm || (p.rows >= (uint32_t)n_sm && n <= 4096) || n <= kChunk * 128;
   const uint32_t threads = many ? 128 : 512;
   p.slices = 1;
   while (!many && p.slices < kMaxSlices && (uint64_t)p.rows * p.slices < 2u * (uint64_t)n_sm && n > p.slices * (kChunk * threads)) p.slices *= 2;
