@@ -284,7 +284,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           a[0][0] = halves(raw[i][kt].at(0) * down, raw[i][kt].at(1) * down);
           a[0][1] = halves(raw[i][kt].at(2) * down, raw[i][kt].at(3) * down);
           if (MODE == kBf16Few) {
-            *reinterpret_cast<uint2 *>(q_at + kt * 512) = make_uint2(a[0][0], a[0][1]);
+            *reinterpret_cast<uint4 *>(q_at + kt * 512) = make_uint4(a[0][0], 0u, a[0][1], 0u);  // with the zeros of rows 8 .. 15: read as an operand's four words
           } else {
             *reinterpret_cast<uint32_t *>(q_at + kt * 512 + 4 * i) = a[0][0];
             *reinterpret_cast<uint32_t *>(q_at + kt * 512 + 4 * (2 + i)) = a[0][1];
@@ -349,13 +349,8 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             uint32_t a[MT][4];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              if (MODE == kBf16Few) {
-                const uint2 q2 = *reinterpret_cast<const uint2 *>(q_at + (k4 * 4 + kk) * 512);
-                a[mt][0] = q2.x; a[mt][1] = 0u; a[mt][2] = q2.y; a[mt][3] = 0u;
-              } else {
-                const uint4 q4 = *reinterpret_cast<const uint4 *>(q_at + ((k4 * 4 + kk) * MT + mt) * 512);
-                a[mt][0] = q4.x; a[mt][1] = q4.y; a[mt][2] = q4.z; a[mt][3] = q4.w;
-              }
+              const uint4 q4 = *reinterpret_cast<const uint4 *>(q_at + ((k4 * 4 + kk) * MT + mt) * 512);
+              a[mt][0] = q4.x; a[mt][1] = q4.y; a[mt][2] = q4.z; a[mt][3] = q4.w;
             }
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt) {
