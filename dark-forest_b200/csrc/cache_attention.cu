@@ -25,8 +25,8 @@
 //
 // What it reaches. 32 requests of 200 to 16000 tokens, one new each, 32 heads on 8 of 128, bf16 and e4m3: 73 us for 342 MB, 4.7 TB/s, 70 % of a copy's rate. One request of
 // 131073 tokens, 16 heads of 128, fp32 and int8: 112 us for 537 MB, 4.8 TB/s. One of 300 tokens, 12 heads of 64: 6.7 us, of which 2.4 are a launch. The copies
-// alone (no arithmetic) took 92 us of the second. What is left is issue: 800 instructions per warp for 32 tokens, 350 of them widening (two per clock
-// and SM), the others softmax and products; and 8 to 10 us for a segment's beginning, its end and the addition of its parts.
+// alone (no arithmetic) took 92 us of the second. What is left is issue: 700 instructions per 32 tokens (waits and the
+// loading warp's included), 310 of them in the ALU pipe, which widens (two per clock and SM), 64 products; and 8 to 10 us for a segment's beginning, its end and the addition of its parts.
 #include <float.h>
 #include <math.h>
 
