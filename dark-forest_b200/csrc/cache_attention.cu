@@ -14,7 +14,8 @@
 //            n-tile i is its byte i. The accumulators of lane (g, c) are then row g's dims c * DP/4 ..., like its part of q.
 // Precision. An fp32 query row, times a power of two that brings its largest element to 1 .. 2, enters as two halves (22 bits), and so do the
 // weights exp(s - m) * 2^15: the 16 rows of an instruction are then 8 rows and their second parts, and the two accumulators are added. A bf16 row
-// fits one half, its weights are rounded to 11 bits (the result has 8): 16 rows. The products of 16 tokens, which share one v_scale, are
+// fits one half; in tiles of 16 rows its weights are rounded to 11 bits (the result has 8), in tiles of 8 the second halves take the other 8 rows (as zeros they
+// cost registers: 2 CTAs an SM, and 72 us instead of 69 in the first case below). The products of 16 tokens, which share one v_scale, are
 // added to the row's fp32 sums.
 //
 // Work. A CTA is one warp that loads (tensor-map copies of 16 tokens, 128-byte swizzle: the reads above are then free of bank conflicts at
@@ -23,7 +24,7 @@
 // all tokens. Work is dealt out as cache_line.cuh says; a stage where rows are dealt counts four units, since it takes four times as long. Calls of many rows go
 // to cache_attention_many.cu.
 //
-// What it reaches. 32 requests of 200 to 16000 tokens, one new each, 32 heads on 8 of 128, bf16 and e4m3: 73 us for 342 MB, 4.7 TB/s, 70 % of a copy's rate. One request of
+// What it reaches. 32 requests of 200 to 16000 tokens, one new each, 32 heads on 8 of 128, bf16 and e4m3: 69 us for 342 MB, 4.9 TB/s, 75 % of a copy's rate. One request of
 // 131073 tokens, 16 heads of 128, fp32 and int8: 112 us for 537 MB, 4.8 TB/s. One of 300 tokens, 12 heads of 64: 6.7 us, of which 2.4 are a launch. The copies
 // alone (no arithmetic) took 92 us of the second. What is left is issue: 700 instructions per 32 tokens (waits and the
 // loading warp's included), 310 of them in the ALU pipe, which widens (two per clock and SM), 64 products; and 8 to 10 us for a segment's beginning, its end and the addition of its parts.
@@ -80,9 +81,9 @@ template <int DP>
 constexpr uint32_t kSubBytes = 16 * DP;  // a box of 16 tokens, or less where D < DP: whole swizzle periods
 // CTAs of an SM, by the registers that they need, and stages of the ring, by the shared memory that is left to each.
 template <Mode MODE, int DP>
-constexpr int kCtas = DP == 64 ? (kRows<MODE> == 8 ? 4 : 3) : MODE == kFp32Few ? 3 : 2;
+constexpr int kCtas = DP == 64 ? (kRows<MODE> == 8 ? 4 : 3) : kRows<MODE> == 8 ? 3 : 2;
 template <Mode MODE, int DP>
-constexpr uint32_t kStagesOf = DP == 64 ? (kRows<MODE> == 8 ? 5 : 6) : MODE == kFp32Few ? 3 : MODE == kFp32 ? 4 : 5;
+constexpr uint32_t kStagesOf = DP == 64 ? (kRows<MODE> == 8 ? 5 : 6) : kRows<MODE> == 8 ? 3 : MODE == kFp32 ? 4 : 5;
 // A warp's region of shared memory: its rows of q as operands (16 bytes a lane and k-step, for each instruction that shares a code), later 8 rows of sums.
 template <Mode MODE>
 constexpr uint32_t kTiles = MODE == kFp32 ? 2 : 1;
@@ -415,7 +416,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         for (int i = 0; i < RW; ++i) {
           before[i] = m[i];
           v_row[i] = 0.0f;
-          if (MODE == kBf16Few || (BF16 && i == 1 && !second_rows)) pa[0][0][1] = pa[0][0][3] = pa[0][1][1] = pa[0][1][3] = 0u;
+          if (BF16 && i == 1 && !second_rows) pa[0][0][1] = pa[0][0][3] = pa[0][1][1] = pa[0][1][3] = 0u;
           if (i == 1 && !second_rows) {
             if (!BF16) {
 #pragma unroll
@@ -462,7 +463,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           }
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            if (BF16) {
+            if (BF16 && RW == 2) {
               pa[0][b][i] = halves(s[2 * b][0], s[2 * b][1]);
               pa[0][b][2 + i] = halves(s[2 * b + 1][0], s[2 * b + 1][1]);
             } else {
@@ -498,7 +499,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
               float d[4];
               mma_half_first(d, pa[mt][0], b0[0][k], b1[0][k]);
               mma_half(d, pa[mt][1], b0[1][k], b1[1][k]);
-              if (BF16) {
+              if (BF16 && RW == 2) {
                 o[0][n] = ptx::fma2(make_float2(v_row[0], v_row[0]), make_float2(d[0], d[1]), o[0][n]);
                 if (RW == 2) o[RW - 1][n] = ptx::fma2(make_float2(v_row[RW - 1], v_row[RW - 1]), make_float2(d[2], d[3]), o[RW - 1][n]);
               } else {
