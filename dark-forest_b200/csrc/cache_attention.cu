@@ -14,8 +14,9 @@
 //            n-tile i is its byte i. The accumulators of lane (g, c) are then row g's dims c * DP/4 ..., like its part of q.
 // Precision. An fp32 query row, times a power of two that brings its largest element to 1 .. 2, enters as two halves (22 bits), and so do the
 // weights exp(s - m) * 2^15: the 16 rows of an instruction are then 8 rows and their second parts, and the two accumulators are added. A bf16 row
-// fits one half; in tiles of 16 rows its weights are rounded to 11 bits (the result has 8), in tiles of 8 the second halves take the other 8 rows (as zeros they
-// cost registers: 2 CTAs an SM, and 72 us instead of 69 in the first case below). The products of 16 tokens, which share one v_scale, are
+// fits one half; its weights are two as well: in tiles of 8 rows the second halves take the other 8 (as zeros they cost registers: 2 CTAs an SM, and 72
+// us instead of 69 in the first case below), in tiles of 16 they are multiplied behind the first ones (16 requests of 20 rows, 8 heads of 128: 59 us;
+// rounded to 11 bits 54, and a result of 8 bits then comes out as its neighbour now and then: 6e-4 of it in the 2-norm). The products of 16 tokens, which share one v_scale, are
 // added to the row's fp32 sums.
 //
 // Work. A CTA is one warp that loads (tensor-map copies of 16 tokens, 128-byte swizzle: the reads above are then free of bank conflicts at
@@ -101,6 +102,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   constexpr uint32_t ROWS = kRows<MODE>, kStages = kStagesOf<MODE, DP>;
   constexpr bool BF16 = MODE == kBf16Few || MODE == kBf16;
   constexpr int KT = DP / 16, NT = DP / 8, RW = ROWS / 8, MT = kTiles<MODE>;  // k-steps, n-tiles, rows of a lane
+  constexpr int PT = RW;  // operands that a box's weights fill: two where 16 rows have two halves each
   extern __shared__ uint8_t smem_raw[];
   __shared__ float2 s_scale[kStages][kStageTokens / 16];  // k_scale, v_scale of a stage's boxes
   __shared__ float s_m[kComputeWarps][8], s_l[kComputeWarps][8];
@@ -409,21 +411,21 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         // it, whatever its scale is (it may be NaN).
         const float v_scale = fmaxf(scale[0].y, scale[1].y);
         const bool v_alike = scale[0].y == scale[1].y && !masked;
-        uint32_t pa[MT][2][4];
+        uint32_t pa[PT][2][4];
         float v_row[RW], before[RW];
         bool grew = false;
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
           before[i] = m[i];
           v_row[i] = 0.0f;
-          if (BF16 && i == 1 && !second_rows) pa[0][0][1] = pa[0][0][3] = pa[0][1][1] = pa[0][1][3] = 0u;
           if (i == 1 && !second_rows) {
-            if (!BF16) {
 #pragma unroll
-              for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) pa[MT - 1][b][k] = 0u;
-            }
+              for (int k = 0; k < 2; ++k) {
+                if (BF16) pa[0][b][2 * k + 1] = pa[PT - 1][b][2 * k + 1] = 0u;
+                else pa[PT - 1][b][2 * k] = pa[PT - 1][b][2 * k + 1] = 0u;
+              }
             continue;
           }
           const float f[2] = {scale[0].x * norm[i], scale[1].x * norm[i]};
@@ -463,9 +465,9 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           }
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            if (BF16 && RW == 2) {
-              pa[0][b][i] = halves(s[2 * b][0], s[2 * b][1]);
-              pa[0][b][2 + i] = halves(s[2 * b + 1][0], s[2 * b + 1][1]);
+            if (BF16 && RW == 2) {  // first halves of 16 rows, then their second ones
+              split_halves(s[2 * b][0], s[2 * b][1], pa[0][b][i], pa[PT - 1][b][i]);
+              split_halves(s[2 * b + 1][0], s[2 * b + 1][1], pa[0][b][2 + i], pa[PT - 1][b][2 + i]);
             } else {
               split_halves(s[2 * b][0], s[2 * b][1], pa[i % MT][b][0], pa[i % MT][b][1]);
               split_halves(s[2 * b + 1][0], s[2 * b + 1][1], pa[i % MT][b][2], pa[i % MT][b][3]);
@@ -500,8 +502,10 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
               mma_half_first(d, pa[mt][0], b0[0][k], b1[0][k]);
               mma_half(d, pa[mt][1], b0[1][k], b1[1][k]);
               if (BF16 && RW == 2) {
+                mma_half(d, pa[PT - 1][0], b0[0][k], b1[0][k]);
+                mma_half(d, pa[PT - 1][1], b0[1][k], b1[1][k]);
                 o[0][n] = ptx::fma2(make_float2(v_row[0], v_row[0]), make_float2(d[0], d[1]), o[0][n]);
-                if (RW == 2) o[RW - 1][n] = ptx::fma2(make_float2(v_row[RW - 1], v_row[RW - 1]), make_float2(d[2], d[3]), o[RW - 1][n]);
+                o[RW - 1][n] = ptx::fma2(make_float2(v_row[RW - 1], v_row[RW - 1]), make_float2(d[2], d[3]), o[RW - 1][n]);
               } else {
                 o[mt][n] = ptx::fma2(make_float2(v_row[mt], v_row[mt]), ptx::add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])), o[mt][n]);
               }

@@ -9,13 +9,13 @@
 //   warps 8-11  codes -> halves: K [token][dim] (K-major), V [token][dim] (MN-major), 128-byte swizzled slabs of 64 dims, two buffers each
 //   warp 12     copies of the codes, 16 tokens a box, and the scales of their pages
 //   warp 13     issues: scores of stage j + 2 ahead of the output product of stage j
-// Precision: as there. An fp32 row is two halves (two K-steps for one, into the same accumulators), and so are its weights; they are held times 2^7, and the
+// Precision: as there. An fp32 row is two halves (two K-steps for one, into the same accumulators), a bf16 row one; weights are two either way, and are held times 2^7, and the
 // maximum that they refer to is moved when a row's has grown by 2^8 (the accumulators are then rescaled by the row's thread), so that they stay in
 // the halves' range either way. v_scale enters the weights, relative to the largest so far.
 // What bounds it. Two requests of 500 tokens over 6000 to 9000 cached ones, 12 heads of 64, fp32, int8: 99 us, 254 TFLOP/s of the formula's operations (twice as
 // many are done). A stage takes 1.1 us; of that the tensor pipe works a quarter, and the issuing warp is busy for 1300 cycles (waits apart; one
 // instruction of 64 columns costs it 70), nearly as long as a row's warp is (2500 cycles for every second stage, with two of them and a
-// widening warp on each scheduler). One request of 2000 tokens, 32 heads on 8 of 128: 343 us in bf16, 476 us in fp32.
+// widening warp on each scheduler). One request of 2000 tokens over 8000, 32 heads on 8 of 128: 485 us in bf16, 605 us in fp32.
 // What it came from: row tiles on mma.sync 244 us; four row warps 152; eight, each with every second stage 133; a score's factor and the shift of its exponent in one
 // operation 125; one branch around the products of a stage 114; masks and rescaling in tensor memory, without spilling the scores 108; scores two stages
 // ahead 99; outputs added up every 16 stages, which all precision above 5.9e-6 needs, 106 (32 heads of 128 636), with states that a warp reads and writes side by side 99
@@ -54,7 +54,7 @@ constexpr uint32_t kManyCtaFloats = 2 * kManyPartialFloats<DP> + (kSumsOutside<B
 
 template <bool BF16, int DP>
 struct ManySmem {
-  static constexpr uint32_t kStages = DP == 128 ? 4 : 8, kParts = BF16 ? 1 : 2, kSlabs = DP / 64;
+  static constexpr uint32_t kStages = DP == 128 ? 4 : 8, kParts = BF16 ? 1 : 2, kSlabs = DP / 64;  // kParts: of q (weights have two)
   static constexpr uint32_t kBoxBytes = 16 * DP, kStageBytes = 8 * kBoxBytes;         // codes: K boxes, V boxes
   static constexpr uint32_t kTileBytes = kSlabs * 64 * 128, kQBytes = kSlabs * 128 * 128;  // 64 tokens, 128 rows of halves
   static constexpr uint32_t kK = kStages * kStageBytes, kV = kK + 2 * kTileBytes, kQ = kV + 2 * kTileBytes;
@@ -211,7 +211,7 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
       tc_fence_after_sync();
       if (elect_one()) {
 #pragma unroll
-        for (uint32_t part_of_w = 0; part_of_w < kParts; ++part_of_w)
+        for (uint32_t part_of_w = 0; part_of_w < 2; ++part_of_w)
 #pragma unroll
           for (uint32_t kk = 0; kk < 4; ++kk)
             mma_f16_ts(tmem + kOutColumn + b * DP, tmem + kWeightColumn + b * 64 + part_of_w * 32 + kk * 8, d_v + ((b * M::kTileBytes + kk * 2048) >> 4), idesc_o,
@@ -473,11 +473,10 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
             w = make_float2(ex2_approx(w.x), ex2_approx(w.y));
             sums[x / 2 & 1] = add2(sums[x / 2 & 1], w);
             w = mul2(w, make_float2(share, share));
-            if (BF16) first[x / 2] = halves(w.x, w.y);
-            else split_halves(w.x, w.y, first[x / 2], second[x / 2]);
+            split_halves(w.x, w.y, first[x / 2], second[x / 2]);
           }
           tmem_st16(tmem + kWeightColumn + b * 64 + 16 * half + lane_base, first);
-          if (!BF16) tmem_st16(tmem + kWeightColumn + b * 64 + 32 + 16 * half + lane_base, second);
+          tmem_st16(tmem + kWeightColumn + b * 64 + 32 + 16 * half + lane_base, second);
         }
         sums[0] = add2(sums[0], sums[1]);
         l += sums[0].x + sums[0].y;
