@@ -16,8 +16,8 @@
 // weights exp(s - m) * 2^15: the 16 rows of an instruction are then 8 rows and their second parts, and the two accumulators are added. A bf16 row
 // fits one half; its weights are two as well: in tiles of 8 rows the second halves take the other 8 (as zeros they cost registers: 2 CTAs an SM, and 72
 // us instead of 69 in the first case below), in tiles of 16 they are multiplied behind the first ones (16 requests of 20 rows, 8 heads of 128: 59 us;
-// rounded to 11 bits 54, and a result of 8 bits then comes out as its neighbour now and then: 6e-4 of it in the 2-norm). The products of 16 tokens, which share one v_scale, are
-// added to the row's fp32 sums.
+// rounded to 11 bits 54, and a result of 8 bits then comes out as its neighbour now and then: 6e-4 of it in the 2-norm). V's scales enter the weights as
+// cache_line.cuh says (unit_exponent). The products of 32 tokens are added to the row's fp32 sums.
 //
 // Work. A CTA is one warp that loads (tensor-map copies of 16 tokens, 128-byte swizzle: the reads above are then free of bank conflicts at
 // head sizes 64 and 128) and four that compute, over a ring of stages of 64 tokens. A request with no more rows (query tokens times heads per K/V head)
@@ -249,7 +249,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     // rows of this lane
     uint32_t see[RW];
     bool valid[RW];
-    float norm[RW], m[RW], l[RW];
+    float norm[RW], m[RW], l[RW], excess[RW];  // (excess: d of unit_exponent)
     float2 o[RW][NT];  // columns 2c, 2c + 1 of n-tile n: dims 2c * DP/8 + n and (2c + 1) * DP/8 + n
     __syncwarp();  // the region below was read as a merge buffer by this warp's lanes alone, behind a barrier
     Raw4<BF16> raw[RW][KT];  // all loads first: they come from DRAM
@@ -300,6 +300,7 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       }
       m[i] = -FLT_MAX;
       l[i] = 0.0f;
+      excess[i] = kLeastExcess;
 #pragma unroll
       for (int n2 = 0; n2 < NT; ++n2) o[i][n2] = make_float2(0.0f, 0.0f);
     }
@@ -407,17 +408,14 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           }
         }
         // ---- weights
-        // The two boxes' weights meet one scale of V, the larger one; a row that sees none of a box's tokens takes nothing of
-        // it, whatever its scale is (it may be NaN).
-        const float v_scale = fmaxf(scale[0].y, scale[1].y);
-        const bool v_alike = scale[0].y == scale[1].y && !masked;
+        const bool v_alike = scale[0].y == scale[1].y;
+        const float v_log[2] = {scale_log(scale[0].y), scale_log(scale[1].y)};
         uint32_t pa[PT][2][4];
-        float v_row[RW], before[RW];
+        float down[RW];
         bool grew = false;
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
-          before[i] = m[i];
-          v_row[i] = 0.0f;
+          down[i] = 1.0f;
           if (i == 1 && !second_rows) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -441,27 +439,38 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
               for (int k = 0; k < 2; ++k)
                 if (token0 + 16 * (nt >> 1) + token_of(nt & 1, 2 * c + k) >= see[i]) s[nt][k] = -INFINITY;
           }
-          float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          grew |= top > m[i];
-          m[i] = fmaxf(m[i], top);
+          float tops[2];  // of the boxes
+#pragma unroll
+          for (int b = 0; b < 2; ++b) tops[b] = fmaxf(fmaxf(s[2 * b][0], s[2 * b][1]), fmaxf(s[2 * b + 1][0], s[2 * b + 1][1]));
+          if (v_alike) tops[0] = tops[1] = fmaxf(tops[0], tops[1]);
+          tops[0] = fmaxf(tops[0], __shfl_xor_sync(0xffffffffu, tops[0], 1));
+          tops[0] = fmaxf(tops[0], __shfl_xor_sync(0xffffffffu, tops[0], 2));
+          if (v_alike) {
+            tops[1] = tops[0];
+          } else {
+            tops[1] = fmaxf(tops[1], __shfl_xor_sync(0xffffffffu, tops[1], 1));
+            tops[1] = fmaxf(tops[1], __shfl_xor_sync(0xffffffffu, tops[1], 2));
+          }
+          const float before = m[i], e_before = unit_exponent(excess[i]);
+          m[i] = fmaxf(before, fmaxf(tops[0], tops[1]));
+          excess[i] = fmaxf(excess[i] + (before - m[i]), fmaxf(tops[0] - m[i] + v_log[0], tops[1] - m[i] + v_log[1]));
+          const float e_now = unit_exponent(excess[i]), units = ex2_approx(-e_now);
+          grew |= m[i] > before || e_now != e_before;
+          down[i] = ex2_approx((before - m[i]) + (e_before - e_now));
           const float shift = m[i] - kWeightBits;
 #pragma unroll
           for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
             for (int k = 0; k < 2; ++k) s[nt][k] = ex2_approx(s[nt][k] - shift);
-          l[i] = fmaf(l[i], ex2_approx(before[i] - m[i]), ((s[0][0] + s[0][1]) + (s[1][0] + s[1][1])) + ((s[2][0] + s[2][1]) + (s[3][0] + s[3][1])));
-          v_row[i] = token0 < see[i] ? v_scale : 0.0f;
-          if (!v_alike) {
+          l[i] = fmaf(l[i], ex2_approx(before - m[i]), ((s[0][0] + s[0][1]) + (s[1][0] + s[1][1])) + ((s[2][0] + s[2][1]) + (s[3][0] + s[3][1])));
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              const float share = token0 + 16 * b < see[i] && v_scale != 0.0f ? __fdividef(scale[b].y, v_scale) : 0.0f;
+          for (int b = 0; b < 2; ++b) {
+            // a row that sees none of a box's tokens takes nothing of it, whatever its scale is (it may be NaN)
+            const float share = masked && token0 + 16 * b >= see[i] ? 0.0f : share_of(scale[b].y, units);
 #pragma unroll
-              for (int nt = 2 * b; nt < 2 * b + 2; ++nt)
+            for (int nt = 2 * b; nt < 2 * b + 2; ++nt)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) s[nt][k] *= share;
-            }
+              for (int k = 0; k < 2; ++k) s[nt][k] *= share;
           }
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
@@ -476,11 +485,9 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-          for (int i = 0; i < RW; ++i) {
-            const float f = ex2_approx(before[i] - m[i]);
+          for (int i = 0; i < RW; ++i)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) o[i][n] = make_float2(o[i][n].x * f, o[i][n].y * f);
-          }
+            for (int n = 0; n < NT; ++n) o[i][n] = make_float2(o[i][n].x * down[i], o[i][n].y * down[i]);
         }
         // ---- output
 #pragma unroll
@@ -504,10 +511,10 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
               if (BF16 && RW == 2) {
                 mma_half(d, pa[PT - 1][0], b0[0][k], b1[0][k]);
                 mma_half(d, pa[PT - 1][1], b0[1][k], b1[1][k]);
-                o[0][n] = ptx::fma2(make_float2(v_row[0], v_row[0]), make_float2(d[0], d[1]), o[0][n]);
-                o[RW - 1][n] = ptx::fma2(make_float2(v_row[RW - 1], v_row[RW - 1]), make_float2(d[2], d[3]), o[RW - 1][n]);
+                o[0][n] = ptx::add2(make_float2(d[0], d[1]), o[0][n]);
+                o[RW - 1][n] = ptx::add2(make_float2(d[2], d[3]), o[RW - 1][n]);
               } else {
-                o[mt][n] = ptx::fma2(make_float2(v_row[mt], v_row[mt]), ptx::add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])), o[mt][n]);
+                o[mt][n] = ptx::add2(ptx::add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])), o[mt][n]);
               }
             }
           }
@@ -523,6 +530,9 @@ k_cache_attention(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     for (int i = 0; i < RW; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      const float unit = ex2_approx(unit_exponent(excess[i]));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[i][n] = make_float2(o[i][n].x * unit, o[i][n].y * unit);
     }
     // four of the lane's DP / 4 dims of row i, from the n-th on
     auto four = [&](int i, int n) {

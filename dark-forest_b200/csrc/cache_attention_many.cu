@@ -9,9 +9,9 @@
 //   warps 8-11  codes -> halves: K [token][dim] (K-major), V [token][dim] (MN-major), 128-byte swizzled slabs of 64 dims, two buffers each
 //   warp 12     copies of the codes, 16 tokens a box, and the scales of their pages
 //   warp 13     issues: scores of stage j + 2 ahead of the output product of stage j
-// Precision: as there. An fp32 row is two halves (two K-steps for one, into the same accumulators), a bf16 row one; weights are two either way, and are held times 2^7, and the
-// maximum that they refer to is moved when a row's has grown by 2^8 (the accumulators are then rescaled by the row's thread), so that they stay in
-// the halves' range either way. v_scale enters the weights, relative to the largest so far.
+// Precision: as there. An fp32 row is two halves (two K-steps for one, into the same accumulators), a bf16 row one; weights are two either way, and are held
+// times 2^7; what they refer to (the maximum m, and the unit 2^(m + e) of cache_line.cuh that V's scales need) is moved when a row's own weights have grown by 2^8 (the
+// accumulators are then rescaled by the row's thread), so that they stay in the halves' range either way.
 // What bounds it. Two requests of 500 tokens over 6000 to 9000 cached ones, 12 heads of 64, fp32, int8: 99 us, 254 TFLOP/s of the formula's operations (twice as
 // many are done). A stage takes 1.1 us; of that the tensor pipe works a quarter, and the issuing warp is busy for 1300 cycles (waits apart; one
 // instruction of 64 columns costs it 70), nearly as long as a row's warp is (2500 cycles for every second stage, with two of them and a
@@ -32,7 +32,7 @@ using namespace ptx;
 
 constexpr uint32_t kRowWarps = 8, kLoadWarp = 12, kMmaWarp = 13;  // (warps 8 to 11 widen)
 constexpr uint32_t kTileRows = 128;
-constexpr float kManyWeightBits = 7.0f, kRescale = 8.0f;
+constexpr float kManyWeightBits = 7.0f, kRescale = 8.0f, kRescaleV = 7.0f;  // (room for the rounding of s + log2 v_scale)
 constexpr uint32_t kTmemColumns = 512, kScoreColumn = 0, kWeightColumn = 128, kOutColumn = 256;  // scores 2 x 64, weights 2 x (32 + 32), outputs 2 x DP
 // Stages whose output products add up in place. The tensor cores cut their sums off, they do not round them, at every step of 16 tokens: 9000 tokens one after another
 // left an error of 6e-6 where fp32 sums leave 2e-6. So a row's thread adds an fp32 output up, rounded, every 16 stages (8 of its half), in tensor memory where there is room
@@ -74,9 +74,9 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
   extern __shared__ uint8_t smem_raw[];
   __shared__ LineSmem<W> s_sums;
   __shared__ float2 s_box_scale[kStages][4];  // k_scale, v_scale of the boxes in the ring
-  __shared__ float2 s_scale[4][4];            // and of the last four stages widened
+  __shared__ float4 s_scale[4][4];            // and of the last four stages widened, with log2 v_scale
   __shared__ uint64_t s_bars[NUM_BARS];
-  __shared__ float s_state[2][4][kTileRows];  // of the two halves' rows: maximum, sum, scale of the output in place and of that added up before
+  __shared__ float s_state[2][4][kTileRows];  // of the two halves' rows: maximum, sum, units of the output in place and of that added up before
   __shared__ Line s_line[kRowWarps];
   __shared__ Part s_part[kRowWarps];
   __shared__ uint32_t s_last, s_abort, s_tmem;
@@ -266,7 +266,10 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
       const uint32_t b = j & 1, slot = j % kStages;
       if (!mbar_wait_warp(bar(FULL + slot), (j / kStages) & 1, &s_abort)) return false;
       if (j >= 2 && !mbar_wait_warp(bar(K_FREE + b), ((j >> 1) - 1) & 1, &s_abort)) return false;
-      if (wt < 4) s_scale[j & 3][wt] = s_box_scale[slot][wt];
+      if (wt < 4) {
+        const float2 scale = s_box_scale[slot][wt];
+        s_scale[j & 3][wt] = make_float4(scale.x, scale.y, scale_log(scale.y), 0.0f);
+      }
       widen(smem + slot * M::kStageBytes, smem + M::kK + b * M::kTileBytes, 64);
       if (lane == 0) mbar_arrive(bar(K_FULL + b));
       return true;
@@ -367,9 +370,10 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(Q_FULL));
       }
-      float m = -FLT_MAX, l = 0.0f, v_most = 0.0f;  // the maximum that the weights refer to; the scale that the output is in units of
-      bool started = false;                         // this half has had a stage
-      float m_sum = -FLT_MAX, v_sum = -1.0f;        // of the chunks before, as m and v_most; below 0: there are none
+      // The maximum that the weights refer to, and d and e of unit_exponent with it: the output is in units of 2^(m + e).
+      float m = -FLT_MAX, l = 0.0f, excess = kLeastExcess, e = kLeastExcess;
+      bool started = false, had_sum = false;  // this half has had a stage; chunks before this one
+      float m_sum = -FLT_MAX, e_sum = 0.0f;   // m and e of what those add up to
       const bool split = part.parts > 1;
       auto state_of = [&](uint32_t cta) { return p.partial + (size_t)(2 * cta + (cta == part.first_cta ? 1 : 0)) * kManyPartialFloats<DP>; };
       float *mine = state_of(blockIdx.x);  // (of no other segment while this one lasts, cut or not)
@@ -416,24 +420,30 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
           tmem_ld32(tmem + kScoreColumn + b * 64 + 32 + lane_base, s1);
           tmem_wait_ld();
         }
-        float2 scale[4];
+        float v_scale[4], f[4], v_log[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) scale[i] = s_scale[stage & 3][i];
+        for (int i = 0; i < 4; ++i) {
+          const float4 scale = s_scale[stage & 3][i];
+          f[i] = scale.x * norm;
+          v_scale[i] = scale.y;
+          v_log[i] = scale.z;
+        }
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(S_FREE + b));  // scores and scales are in registers
-        float top = -INFINITY;
-        float f[4];  // what a box's scores are multiplied by; above 0 (or NaN, for rows that see the box), so that -inf stays -inf
+        float top = -INFINITY, top_v = -INFINITY;  // of the scores, and with log2 v_scale
+        // f: what a box's scores are multiplied by; above 0 (or NaN, for rows that see the box), so that -inf stays -inf
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          f[i] = scale[i].x * norm;
           if (f[i] < 0x1p-120f || 16 * i >= seen) f[i] = 0x1p-120f;
           float most[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             most[k] = fmaxf(fmaxf(__uint_as_float(s[16 * i + 4 * k]), __uint_as_float(s[16 * i + 4 * k + 1])),
                             fmaxf(__uint_as_float(s[16 * i + 4 * k + 2]), __uint_as_float(s[16 * i + 4 * k + 3])));
-          top = fmaxf(top, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * f[i]);
+          const float top_i = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * f[i];
+          top = fmaxf(top, top_i);
+          top_v = fmaxf(top_v, top_i + v_log[i]);
         }
         // the product of two stages ago has read the weights' buffer and written this half's output
         if (stage >= 2) {
@@ -442,25 +452,26 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
           tc_fence_after_sync();
         }
         const bool fresh = started && (stage - first_stage) % kChunk<BF16> < 2;  // a chunk's first of this half: what is there is added up
-        const float factor = !BF16 && fresh && v_sum > 0.0f && v_most > 0.0f ? ex2_approx(m_sum - m) * __fdividef(v_sum, v_most) : 0.0f;
-        const bool had_sum = !(v_sum < 0.0f);
+        const bool add_sum = had_sum;
+        const float factor = ex2_approx((m_sum - m) + (e_sum - e));
         if (fresh) {
           m_sum = m;
-          v_sum = v_most;
+          e_sum = e;
+          had_sum = true;
         }
-        const float v_now = fmaxf(fmaxf(fmaxf(scale[0].y, scale[1].y), fmaxf(scale[2].y, scale[3].y)), v_most);
-        const bool grow = top > m + kRescale;  // (also the first that a row sees)
-        const bool rescale = started && !fresh && (__any_sync(0xffffffffu, grow) || v_now != v_most);
+        const bool grow_m = top > m + kRescale, grow = grow_m || top_v - m > e + kRescaleV;  // (also the first that a row sees)
+        const bool rescale = started && !fresh && __any_sync(0xffffffffu, grow);
         float down_out = 1.0f;
-        if (rescale || fresh || !started) {  // (v_now is the same in all rows)
-          const float to = fmaxf(m, top), alpha = ex2_approx(m - to);
+        if (grow || fresh || !started) {  // (a row for itself: what others see changes nothing of it)
+          const float to = grow_m || fresh || !started ? fmaxf(m, top) : m, before = e;  // (V has no part in the sum of the weights)
+          excess = fmaxf(excess + (m - to), top_v - to);
+          e = unit_exponent(excess);
+          down_out = ex2_approx((m - to) + (before - e));
+          l *= ex2_approx(m - to);
           m = to;
-          l *= alpha;
-          down_out = v_now > 0.0f ? alpha * __fdividef(v_most, v_now) : 0.0f;
-          v_most = v_now;
         }
         started = true;
-        const float minus_shift = kManyWeightBits - m, v_down = v_most > 0.0f ? __fdividef(1.0f, v_most) : 0.0f;
+        const float minus_shift = kManyWeightBits - m, units = ex2_approx(-e);
         float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {  // 32 tokens at a time: fewer registers
@@ -468,7 +479,7 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #pragma unroll
           for (int x = 0; x < 32; x += 2) {
             const int i = 2 * half + x / 16;
-            const float share = 16 * i < seen ? scale[i].y * v_down : 0.0f;  // a row takes nothing of a box that it sees nothing of
+            const float share = 16 * i < seen ? share_of(v_scale[i], units) : 0.0f;  // a row takes nothing of a box that it sees nothing of
             float2 w = fma2(as_float2(s[32 * half + x], s[32 * half + x + 1]), make_float2(f[i], f[i]), make_float2(minus_shift, minus_shift));
             w = make_float2(ex2_approx(w.x), ex2_approx(w.y));
             sums[x / 2 & 1] = add2(sums[x / 2 & 1], w);
@@ -490,7 +501,7 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
               float4 *at = at_dim(outside, d);
               float4 before[4];
 #pragma unroll
-              for (int x = 0; x < 4; ++x) before[x] = had_sum ? at[x * kTileRows] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              for (int x = 0; x < 4; ++x) before[x] = add_sum ? at[x * kTileRows] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
               tmem_wait_ld();
 #pragma unroll
               for (int x = 0; x < 4; ++x)
@@ -498,9 +509,9 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
                                     fmaf(before[x].z, factor, __uint_as_float(o[4 * x + 2])), fmaf(before[x].w, factor, __uint_as_float(o[4 * x + 3])));
             } else {
               uint32_t before[16];
-              if (had_sum) tmem_ld16(t_out + 2 * DP + d, before);
+              if (add_sum) tmem_ld16(t_out + 2 * DP + d, before);
               tmem_wait_ld();
-              if (had_sum) {
+              if (add_sum) {
 #pragma unroll
                 for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(fmaf(__uint_as_float(before[x]), factor, __uint_as_float(o[x])));
               }
@@ -532,8 +543,8 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
       s_state[b][0][row] = m;
       s_state[b][1][row] = l;
-      s_state[b][2][row] = started && ok ? v_most : -1.0f;  // below 0: there is no output
-      s_state[b][3][row] = v_sum < 0.0f ? -1.0f : ex2_approx(m_sum - m) * v_sum;
+      s_state[b][2][row] = started && ok ? ex2_approx(e) : -1.0f;  // below 0: there is no output
+      s_state[b][3][row] = had_sum ? ex2_approx((m_sum - m) + e_sum) : -1.0f;
       tc_fence_before_sync();
       row_barrier();
       tc_fence_after_sync();

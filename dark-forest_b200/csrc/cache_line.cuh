@@ -282,6 +282,21 @@ __device__ __forceinline__ void store_row4(void *out, size_t e, bool aligned, co
   }
 }
 
+// Weights of V. Pages have scales of their own, so the largest weight exp(s - m) need not belong to the largest part of the result; half-precision weights
+// must reach down from that part, and nothing that a row does not see may move them. So a row keeps, besides its maximum m,
+//   d = max (s - m) + log2 v_scale   over the tokens that it sees (units of log 2),
+// and its output in units of 2^e, e the whole number next to d: a weight is exp(s - m) * (v_scale 2^-e), at most 2^(1/2), exact in all bits that exp(s - m)
+// has where scales are powers of two. The logarithm is bounded, so that 2^e and 2^-e are numbers; a row that has seen nothing has the lowest d.
+constexpr float kLeastExcess = -126.0f;
+__device__ __forceinline__ float scale_log(float v_scale) { return fminf(fmaxf(__log2f(v_scale), kLeastExcess), 126.0f); }
+__device__ __forceinline__ float unit_exponent(float d) { return (d + 12582912.0f) - 12582912.0f; }  // 1.5 * 2^23: rounds to a whole number
+// v_scale 2^-e, given 2^-e. Bounded, so that a weight of zero stays one beside any scale; NaN stays NaN.
+__device__ __forceinline__ float share_of(float v_scale, float units) {
+  float share;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(share) : "f"(v_scale * units), "f"(0x1p126f));
+  return share;
+}
+
 // Sums (m, l, o[4]) states one after another.
 struct Running {
   float m = -FLT_MAX, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
