@@ -76,6 +76,7 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
   __shared__ float2 s_box_scale[kStages][4];  // k_scale, v_scale of the boxes in the ring
   __shared__ float4 s_scale[4][4];            // and of the last four stages widened, with log2 v_scale
   __shared__ uint64_t s_bars[NUM_BARS];
+  __shared__ float s_top[2][kTileRows];       // largest elements of the halves of q's rows; no other use: a half without stages may be at its state already
   __shared__ float s_state[2][4][kTileRows];  // of the two halves' rows: maximum, sum, units of the output in place and of that added up before
   __shared__ Line s_line[kRowWarps];
   __shared__ Part s_part[kRowWarps];
@@ -339,9 +340,9 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
         for (uint32_t i = 0; i < DP / 8; ++i)
 #pragma unroll
           for (int k = 0; k < 4; ++k) top = fmaxf(top, fabsf(x[i].at(k)));
-        s_state[b][0][row] = top;
+        s_top[b][row] = top;
         row_barrier();
-        top = fmaxf(top, s_state[1 - b][0][row]);
+        top = fmaxf(top, s_top[1 - b][row]);
         const uint32_t exponent = min(max(__float_as_uint(top) >> 23, 1u), 253u);
         const bool keep = top == 0.0f || top == INFINITY;
         // (the scale's sign goes into q: what multiplies a score is then not negative, and a maximum stays one)
@@ -637,7 +638,7 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
           }
         }
       }
-      row_barrier();  // s_last and s_state are free again
+      row_barrier();  // s_last, s_top and s_state are free again
     }
   }
   // ---- teardown: every role comes here, also when a wait has run out
