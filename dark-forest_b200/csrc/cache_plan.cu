@@ -9,6 +9,8 @@
 // waiting for another block, and then writes its share of tokens and pages, whose request it finds by bisection in the
 // sums, which lie in shared memory. No block reads what another writes: a table entry that a token needs is an old one, or is taken from
 // the free pages again.
+#include <initializer_list>
+
 #include "df_common.cuh"
 #include "sm100_ptx.cuh"
 
@@ -183,6 +185,25 @@ int prepare(K kernel, size_t smem) {
   return smem > 48 * 1024 ? check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) : DF_OK;
 }
 
+// Blocks read all inputs while others write: what a kernel writes may be nothing that it reads, and no two results the same.
+struct Entries {
+  const int32_t *at;
+  uint64_t n;
+};
+bool apart(std::initializer_list<Entries> written, std::initializer_list<Entries> read) {
+  auto meet = [](const Entries &a, const Entries &b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    return a.n != 0 && b.n != 0 && x < y + 4 * b.n && y < x + 4 * a.n;
+  };
+  for (const Entries *a = written.begin(); a != written.end(); ++a) {
+    for (const Entries *b = written.begin(); b != a; ++b)
+      if (meet(*a, *b)) return false;
+    for (const Entries &b : read)
+      if (meet(*a, b)) return false;
+  }
+  return true;
+}
+
 bool page_layout_valid(uint32_t page_size, uint32_t n_pages) { return page_size != 0 && (uint64_t)page_size * n_pages < (1ull << 31); }
 
 }  // namespace
@@ -199,7 +220,11 @@ int df_cache_plan(const int32_t *lens, const int32_t *new_tokens, int *block_tab
   if (!page_layout_valid(page_size, n_pages) || n_tokens >= (1u << 31)) return finish(DF_ERR_INVALID_ARG);
   if (n_requests > kMaxRequests) return finish(DF_ERR_UNSUPPORTED);
   if (!free_count || !starts || !state || (n_pages && !free_pages) || (n_tokens && (!slots || !positions))) return finish(DF_ERR_INVALID_ARG);
-  if (n_requests && (!lens || !new_tokens || !lens_out || lens_out == lens || (table_width && !block_table))) return finish(DF_ERR_INVALID_ARG);
+  if (n_requests && (!lens || !new_tokens || !lens_out || (table_width && !block_table))) return finish(DF_ERR_INVALID_ARG);
+  const uint64_t R = n_requests;
+  if (!apart({{lens_out, R}, {starts, R + 1}, {slots, n_tokens}, {positions, n_tokens}, {state, 2}, {block_table, R * table_width}},
+             {{lens, R}, {new_tokens, R}, {free_pages, n_pages}, {free_count, 1}}))
+    return finish(DF_ERR_INVALID_ARG);
   const PlanParams p = {lens, new_tokens, free_pages, free_count, block_table, lens_out, starts, slots, positions, state,
                         n_requests, n_tokens, table_width, page_size, n_pages};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -222,8 +247,11 @@ int df_cache_release(const int32_t *lens, const int32_t *finished, const int32_t
   DF_RANGE("df_cache_release");
   if (!page_layout_valid(page_size, n_pages)) return finish(DF_ERR_INVALID_ARG);
   if (n_requests > kMaxRequests) return finish(DF_ERR_UNSUPPORTED);
-  if (!free_count || !count_out || count_out == free_count || (n_pages && !free_pages)) return finish(DF_ERR_INVALID_ARG);
-  if (n_requests && (!lens || !finished || !lens_out || lens_out == lens || (table_width && !block_table))) return finish(DF_ERR_INVALID_ARG);
+  if (!free_count || !count_out || (n_pages && !free_pages)) return finish(DF_ERR_INVALID_ARG);
+  if (n_requests && (!lens || !finished || !lens_out || (table_width && !block_table))) return finish(DF_ERR_INVALID_ARG);
+  const uint64_t R = n_requests;
+  if (!apart({{lens_out, R}, {count_out, 1}, {free_pages, n_pages}}, {{lens, R}, {finished, R}, {block_table, R * table_width}, {free_count, 1}}))
+    return finish(DF_ERR_INVALID_ARG);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const size_t smem = sizeof(uint32_t) * (size_t)n_requests;
   int st;

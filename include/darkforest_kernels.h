@@ -402,10 +402,12 @@ DF_API int df_chunked_logit_ce(float *logits, const uint32_t *targets, float *gr
  *       starts[n_requests + 1]: exclusive sums of new_tokens; slots, positions [n_tokens]: the new tokens' slots and places in their
  *       sequences, request after request (-1 behind the last one). state[0]: free pages left, state[1]: 0. All or nothing: where the pages do not suffice
  *       (state[1] = pages missing), or a request outgrows its table row or n_tokens (state[1] = -1 - r, the first such request), nothing is
- *       granted: lens_out = lens, slots and positions -1, table and free pages as before. At most 16384 requests. lens_out must
- *       not be lens. free_pages has n_pages entries.
+ *       granted: lens_out = lens, slots and positions -1, table and free pages as before. At most 16384 requests. free_pages
+ *       has n_pages entries. No output may overlap an input or another output (DF_ERR_INVALID_ARG): state holds the next step's count, so a program that keeps its buffers
+ *       has two of them that it swaps, as for the lengths.
  *   df_cache_release    Requests with finished[r] != 0 give their ceil(lens[r] / page_size) pages back: they are appended to free_pages behind
- *       *free_count, in order; lens_out[r] = 0, *count_out = the new count. The others keep their length. Outputs must not be inputs, free_pages aside.
+ *       *free_count, in order; lens_out[r] = 0, *count_out = the new count. The others keep their length. No output may overlap an input or another output,
+ *       free_pages (which is both) included: DF_ERR_INVALID_ARG.
  *   df_cache_append     Rows k, v [n_tokens] of n_kv_heads * d_head elements (fp32, or bf16 with kv_bf16; row strides in elements) go to slots[n_tokens];
  *       slots outside the cache (-1) are left out. The tokens of a page lie together and in order, and behind the rows that the page already has (as
  *       df_cache_plan lays them out). The scale of a page and head is the smallest power of two, 2^-126 or above, that holds its
