@@ -10,6 +10,7 @@
 // sums, which lie in shared memory. No block reads what another writes: a table entry that a token needs is an old one, or is taken from
 // the free pages again.
 #include <initializer_list>
+#include <mutex>
 
 #include "df_common.cuh"
 #include "sm100_ptx.cuh"
@@ -180,9 +181,16 @@ unsigned blocks_for(uint32_t work, uint32_t threads) {
   return n < 1 ? 1 : n < kMaxBlocks ? n : kMaxBlocks;
 }
 
-template <typename K>
-int prepare(K kernel, size_t smem) {
-  return smem > 48 * 1024 ? check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) : DF_OK;
+// Shared memory for the most requests, asked for once per kernel and device: a launch may have 48 KB without, what the kernel holds itself included, and
+// a limit that followed each call's size could be lowered by another thread's call.
+template <auto K>
+int prepare(size_t bytes) {
+  static std::once_flag once[64];
+  static bool ok[64];
+  int dev = 0;
+  if (check_cuda(cudaGetDevice(&dev)) != DF_OK || dev < 0 || dev >= 64) return DF_ERR_CUDA;
+  std::call_once(once[dev], [&]() { ok[dev] = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess; });
+  return ok[dev] ? DF_OK : DF_ERR_CUDA;
 }
 
 // Blocks read all inputs while others write: what a kernel writes may be nothing that it reads, and no two results the same.
@@ -234,7 +242,7 @@ int df_cache_plan(const int32_t *lens, const int32_t *new_tokens, int *block_tab
   if (n_requests <= kSmallWork) {
     st = check_cuda(launch_kernel(k_cache_plan<kSmall>, dim3(blocks_for(work, kSmall)), dim3(kSmall), smem, s, p));
   } else {
-    st = prepare(k_cache_plan<kLarge>, smem);
+    st = prepare<k_cache_plan<kLarge>>(2 * sizeof(uint32_t) * kMaxRequests);
     if (st == DF_OK) st = check_cuda(launch_kernel(k_cache_plan<kLarge>, dim3(blocks_for(work, kLarge)), dim3(kLarge), smem, s, p));
   }
   note_launch();
@@ -259,7 +267,7 @@ int df_cache_release(const int32_t *lens, const int32_t *finished, const int32_t
     st = check_cuda(launch_kernel(k_cache_release<kSmall>, dim3(blocks_for(n_requests, kSmall)), dim3(kSmall), smem, s, lens, finished, block_table, free_pages, free_count,
                                   lens_out, count_out, n_requests, table_width, page_size, n_pages));
   } else {
-    st = prepare(k_cache_release<kLarge>, smem);
+    st = prepare<k_cache_release<kLarge>>(sizeof(uint32_t) * kMaxRequests);
     if (st == DF_OK)
       st = check_cuda(launch_kernel(k_cache_release<kLarge>, dim3(blocks_for(n_requests, kLarge)), dim3(kLarge), smem, s, lens, finished,
                                     block_table, free_pages, free_count, lens_out, count_out, n_requests, table_width, page_size, n_pages));
