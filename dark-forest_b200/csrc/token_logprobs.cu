@@ -471,8 +471,10 @@ __global__ void __launch_bounds__(kGradThreads) k_token_logprobs_backward(const 
   for (int i = 0; i < kGradGroups; ++i)
     if (g0 + i * kGradThreads < split.groups) v[i] = __ldcs(body + g0 + i * kGradThreads);
   const int32_t target = __ldg(p.targets + row);
-  const bool has = target >= 0 && (uint32_t)target < p.cols;
-  const float lse = __ldg(p.lse + row), entropy = __ldg(p.entropy + row);
+  // A row that nothing can come of (lse -inf) has no part of anything: p = 0 throughout, as if lse were +inf, and no target.
+  const float lse_row = __ldg(p.lse + row), entropy = __ldg(p.entropy + row);
+  const float lse = lse_row == -INFINITY ? INFINITY : lse_row;
+  const bool has = target >= 0 && (uint32_t)target < p.cols && lse_row != -INFINITY;
   const float g = has && p.grad_logp ? __ldg(p.grad_logp + row) : 0.0f, h = p.grad_entropy ? __ldg(p.grad_entropy + row) : 0.0f;
   const float g_all = -p.scale * fmaf(h, entropy, g), h_all = -p.scale * h, g_one = p.scale * g;
   const uint32_t one = has ? (uint32_t)target : 0xffffffffu;

@@ -447,7 +447,8 @@ DF_API int df_cache_attention(const void *q, const void *k_cache, const void *v_
  *       nothing else has lse -inf, entropy 0 and log probabilities of -inf; a NaN or +inf in a row makes its results NaN (NaN and +inf
  *       stand first among the alternatives).
  *   df_token_logprobs_backward   d_logits = scale * (grad_logp * (onehot(target) - p) - grad_entropy * p * (log p + entropy)), from lse and entropy as
- *       above; grad_logp and grad_entropy [rows] may each be NULL. A row with a target outside the columns has no part of grad_logp. d_logits has
+ *       above; grad_logp and grad_entropy [rows] may each be NULL. A row with a target outside the columns has no part of grad_logp;
+ *       a row that nothing can come of (lse -inf) has gradient 0. d_logits has
  *       the logits' type and may be the logits themselves (with the same row stride). */
 #define DF_LOGPROBS_MAX_TOP 32
 DF_API int df_token_logprobs(const void *logits, const int32_t *targets, float *logp, float *entropy, float *lse, int *top_ids,
