@@ -777,7 +777,7 @@ const char *df_attn_status_string(int status) {
     case DF_ERR_UNSUPPORTED: return "shape not supported by the selected variant";
     case DF_ERR_CUDA: return "CUDA call failed";
     case DF_ERR_DEVICE_TIMEOUT: return "a bounded wait inside a kernel ran out";
-    case DF_ERR_DEVICE_BOUNDS: return "a kernel of a DF_BOUNDS_CHECK build computed an index outside its tensor";
+    case DF_ERR_DEVICE_BOUNDS: return "a kernel met an index outside its tensor (cache attention: starts that fall)";
     case DF_ERR_WORKSPACE: return "caller scratch too small";
     case DF_ERR_STATIC_SCRATCH:
       return "batch*heads*seq_len exceeds DF_STATIC_SCRATCH_MAX_ROWS, the size of the built-in scratch array";

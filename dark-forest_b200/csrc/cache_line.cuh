@@ -126,7 +126,7 @@ __device__ __forceinline__ bool next_part(const AttendParams &p, Line &line, Par
 }
 
 // Sums over the requests, in shared memory, and this CTA's place on the line. All threads of the CTA call it; false: nothing is left for this CTA. The barrier in
-// it is the only one.
+// it is the only one. Starts that fall somewhere let rows belong to several requests: their units could pass what the line counts to, so nothing is done then.
 template <class W>
 struct LineSmem {
   uint32_t units[W::kThreads], segments[W::kThreads], most[W::kThreads / 32];
@@ -136,8 +136,10 @@ __device__ __forceinline__ bool begin_line(const AttendParams &p, LineSmem<W> &s
   const uint32_t t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const uint32_t per = (p.n_requests + W::kThreads - 1) / W::kThreads, r0 = min(p.n_requests, t * per), r1 = min(p.n_requests, r0 + per);
   uint32_t units = 0, segments = 0, most = 0;
+  bool falls = false;
   for (uint32_t r = r0; r < r1; ++r) {
     const Request q = request_of<W>(p, r);
+    falls |= __ldg(p.starts + r + 1) < __ldg(p.starts + r);
     const uint32_t n = q.row_tiles * p.kv_heads;
     segments += n;
     units += n * span_of<W>(q);
@@ -152,7 +154,10 @@ __device__ __forceinline__ bool begin_line(const AttendParams &p, LineSmem<W> &s
   sm.units[t] = units;
   sm.segments[t] = segments;
   if (lane == 0) sm.most[warp] = most;
-  __syncthreads();
+  if (__syncthreads_or(falls)) {
+    if (blockIdx.x == 0 && t == 0 && p.status) atomicOr(p.status, DEV_STATUS_BOUNDS);
+    return false;
+  }
   uint32_t all_units = 0, all_segments = 0;
   most = 0;
 #pragma unroll

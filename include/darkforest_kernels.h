@@ -53,7 +53,7 @@ extern "C" {
 #define DF_ERR_STATIC_SCRATCH 6 /* problem larger than the library's built-in scratch array  */
 #define DF_ERR_RING_TIMEOUT 7  /* darkforest_ring.h: a host-side wait on the communicator ran out; it was aborted */
 #define DF_ERR_NCCL 8          /* darkforest_ring.h: NCCL reported an error (df_ring_last_nccl_result)          */
-#define DF_ERR_DEVICE_BOUNDS 9 /* DF_BOUNDS_CHECK builds only: a kernel computed an index outside its tensor (see df_sync_status) */
+#define DF_ERR_DEVICE_BOUNDS 9 /* a kernel met an index outside its tensor (df_cache_attention: starts that fall; others: DF_BOUNDS_CHECK builds only; see df_sync_status) */
 
 /* ---- legacy symbols: signatures identical to the reference ---- */
 
@@ -418,6 +418,7 @@ DF_API int df_chunked_logit_ce(float *logits, const uint32_t *targets, float *gr
  *       says, against the requests' cached tokens: with q_len = starts[r + 1] - starts[r], row j of request r sees its tokens 0 .. lens[r] - q_len + j
  *       (its own is in the cache already). Query head h reads K/V head h / (n_heads / n_kv_heads). lse [n_tokens][n_heads]: natural logsumexp of the
  *       scaled scores, may be NULL. Rows that see nothing: out = 0, lse = -inf. Rows outside every request are left as they are.
+ *       Where starts falls from one request to the next nothing is computed and df_sync_status returns DF_ERR_DEVICE_BOUNDS.
  *       workspace: DF_CACHE_WORKSPACE_BYTES, 16-byte aligned, zeroed once by the caller; every call leaves it ready for the next.
  *       Calls that can overlap need a workspace each. */
 #define DF_CACHE_INT8 0
@@ -498,7 +499,8 @@ DF_API const char *df_attn_status_string(int status);
 DF_API int df_attn_selftest_wait_expiry(uint32_t budget_ms, void *stream);
 
 /* Checked builds (make EXTRA=-DDF_BOUNDS_CHECK; no counterpart in the reference, which runs unchecked): the
- * SIMT kernels and the split fp32 kernels range-check every global-memory index; an index outside its tensor sets a bit in the device status word
+ * SIMT kernels and the split fp32 kernels range-check every global-memory index (not the kernels of the paged cache and the log probabilities, which in every
+ * build compare what they read on the GPU, slots, pages, lengths and starts, with the sizes that they were given); an index outside its tensor sets a bit in the device status word
  * and is replaced by 0, so nothing outside the tensor is touched and the context stays usable, and df_sync_status
  * returns DF_ERR_DEVICE_BOUNDS once. This call makes one thread ask the checker for an out-of-range element, which is
  * how a test sees the path work without a bad access. In a normal build it returns DF_ERR_UNSUPPORTED. */
