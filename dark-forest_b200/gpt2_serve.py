@@ -4,7 +4,7 @@ A `Server` holds the model of gpt2_step.build and one cache per layer that share
 bring (a piece of) a prompt and the others one token: pages of finished requests go back (cache_release), the new tokens get their pages and slots
 (cache_plan, once for all layers), and per layer LayerNorm -> Q, K, V projections -> cache_append -> cache_attention -> output projection with
 residual -> LayerNorm -> MLP, all of this library but the MLP's second projection and the tied LM head (stock torch). The tokens that come out carry their log
-probability, the entropy and the alternatives (token_logprobs). The host reads nothing but those, once per step.
+probability, the entropy and the alternatives (token_logprobs). generate() reads those five results and the plan's state, once per step, and nothing else.
 
 `policy_step` is the training side: the model's ordinary forward over the served sequences, the log probabilities of their tokens with token_logprobs
 and its gradient, and an optimizer step on -advantage * log p - bonus * entropy.
@@ -39,6 +39,7 @@ class Server:
             self.caches.append((k, v, k_scale, v_scale))
         self.workspace = torch.zeros(pkg.CACHE_WORKSPACE_BYTES, dtype=torch.uint8, device=self.device)
         self.lens = torch.zeros(slots, dtype=torch.int32, device=self.device)
+        self.held = [0] * slots  # the same on the host, so that a step that does not fit is refused before anything runs
         self.table = torch.zeros(slots, width, dtype=torch.int32, device=self.device)
         self.free = torch.arange(self.n_pages - 1, -1, -1, dtype=torch.int32, device=self.device)
         self.count = torch.full((1,), self.n_pages, dtype=torch.int32, device=self.device)
@@ -60,12 +61,29 @@ class Server:
             x = x + block.w2(up)
         return x
 
+    def _lengths_after(self, new, finished):
+        """The slots' lengths behind a step; ValueError for one that the cache or the model has no place for (their kernels would index behind it)."""
+        if len(new) != len(self.held) or (finished is not None and len(finished) != len(self.held)):
+            raise ValueError(f"a step has an entry for each of the {len(self.held)} slots")
+        if not any(new):
+            raise ValueError("a step needs a token of some slot (release() gives pages back without one)")
+        vocab = self.model.tok.num_embeddings
+        if any(not 0 <= t < vocab for tokens in new for t in tokens):
+            raise ValueError(f"token ids are 0 to {vocab - 1}")
+        after = [(0 if finished is not None and finished[s] else n) + len(new[s]) for s, n in enumerate(self.held)]
+        if max(after) > self.max_len:
+            raise ValueError(f"slot {after.index(max(after))}: {max(after)} tokens, {self.max_len} at most")
+        pages = sum(-(-n // self.page_size) for n in after)
+        if pages > self.n_pages:
+            raise ValueError(f"the step needs {pages} pages, there are {self.n_pages}")
+        return after
+
     def step(self, new, finished=None):
-        """One step: `new` is a list, for each slot the tokens that it brings (possibly none); `finished` flags the slots whose request has left.
-        Returns (tokens, logp, entropy, top_ids, top_logp), a row per slot, sampled behind the slot's last new token (rows of slots
-        without any mean nothing)."""
+        """One step: `new` is a list, for each slot the tokens that it brings (possibly none, but not all of them); `finished` flags the slots whose request has
+        left. Returns (tokens, logp, entropy, top_ids, top_logp), a row per slot, sampled behind the slot's last new token (rows of slots
+        without any mean nothing). ValueError, and nothing changed, where the tokens or their pages do not fit."""
         import torch
-        pkg = self.pkg
+        pkg, after = self.pkg, self._lengths_after(new, finished)
         with torch.no_grad():
             if finished is not None and any(finished):
                 flags = torch.tensor([int(f) for f in finished], dtype=torch.int32, device=self.device)
@@ -74,7 +92,7 @@ class Server:
             tokens = torch.tensor([t for n in new for t in n], dtype=torch.int64, device=self.device)
             self.lens, starts, slots, positions, state = pkg.cache_plan(self.lens, counts, self.table, self.free, self.count, self.page_size,
                                                                         tokens.numel())
-            self.count = state[:1]
+            self.count, self.held = state[:1], after
             x = self._forward(tokens, positions.long(), starts, slots)
             last = x[(starts[1:].long() - 1).clamp_(min=0)]
             logits = self.model.ln_f(last) @ self.model.tok.weight.t()
@@ -90,6 +108,8 @@ class Server:
         slots = self.lens.numel()
         answers = [{"tokens": [], "logp": [], "entropy": [], "alternatives": []} for _ in prompts]
         waiting, owner = list(range(len(prompts))), [None] * slots
+        if max_new < 1:
+            raise ValueError("max_new is 1 or more")
         todo, pages, finished = [[] for _ in range(slots)], [0] * slots, [False] * slots
 
         def needs(i):
@@ -132,6 +152,7 @@ class Server:
         import torch
         flags = torch.tensor([int(f) for f in finished], dtype=torch.int32, device=self.device)
         self.lens, self.count = self.pkg.cache_release(self.lens, flags, self.table, self.free, self.count, self.page_size)
+        self.held = [0 if f else n for f, n in zip(finished, self.held)]
 
 
 def token_logprobs_function(pkg):
