@@ -175,16 +175,20 @@ def token_logprobs_function(pkg):
     return TokenLogprobs
 
 
-def policy_step(pkg, model, opt, sequences, prompt_lens, advantages, bonus=0.0, temperature=1.0):
+def policy_step(pkg, model, opt, sequences, prompt_lens, advantages, bonus=0.0, temperature=1.0, lens=None):
     """One policy gradient step over sequences [batch, S] (int64 token ids, prompts first), of which the tokens behind prompt_lens [batch] were
-    sampled; advantages [batch]. Returns (loss, logp [batch, S - 1], 0 where a token is the prompt's)."""
+    sampled; advantages [batch]. lens [batch]: the sequences' lengths where they differ, what lies behind is padding (no token attends to what comes
+    after it, so every log probability is under the context that was served). Returns (loss, logp [batch, S - 1], 0 where a token is the prompt's or padding)."""
     import torch
     batch, S = sequences.shape
     x = model.tok(sequences) + model.pos(torch.arange(S, device=sequences.device))[None]
     for block in model.blocks:
         x = block(x)
     logits = model.ln_f(x)[:, :-1].reshape(batch * (S - 1), -1) @ model.tok.weight.t()
-    sampled = torch.arange(1, S, device=sequences.device)[None] >= prompt_lens[:, None]
+    place = torch.arange(1, S, device=sequences.device)[None]
+    sampled = place >= prompt_lens[:, None]
+    if lens is not None:
+        sampled &= place < lens[:, None]
     targets = torch.where(sampled, sequences[:, 1:], -1).to(torch.int32).reshape(-1)  # -1: no log probability, and no gradient of one
     logp, entropy = token_logprobs_function(pkg).apply(logits, targets, 1.0 / temperature)
     logp, entropy = logp.view(batch, S - 1), entropy.view(batch, S - 1)
@@ -193,6 +197,16 @@ def policy_step(pkg, model, opt, sequences, prompt_lens, advantages, bonus=0.0, 
     loss.backward()
     opt.step()
     return loss.detach(), logp.detach()
+
+
+def sequences_of(prompts, answers, device):
+    """policy_step's sequences (padded behind with 0), prompt_lens and lens of prompts and what generate() answered to them."""
+    import torch
+    rows = [list(p) + a["tokens"] for p, a in zip(prompts, answers)]
+    sequences = torch.zeros(len(rows), max(len(r) for r in rows), dtype=torch.int64)
+    for i, row in enumerate(rows):
+        sequences[i, :len(row)] = torch.tensor(row)
+    return sequences.to(device), torch.tensor([len(p) for p in prompts], device=device), torch.tensor([len(r) for r in rows], device=device)
 
 
 def main():
@@ -225,13 +239,8 @@ def main():
     n = sum(len(a["tokens"]) for a in answers)
     print(f"{n} tokens of {args.requests} requests in {seconds * 1e3:.0f} ms, {n / seconds:.0f} a second; "
           f"mean log probability {sum(sum(a['logp']) for a in answers) / n:.3f}, mean entropy {sum(sum(a['entropy']) for a in answers) / n:.3f}")
-    length = max(len(p) for p in prompts) + args.new
-    sequences = torch.zeros(args.requests, length, dtype=torch.int64, device="cuda")
-    for i, (p, a) in enumerate(zip(prompts, answers)):
-        row = ([0] * (length - len(p) - len(a["tokens"]))) + p + a["tokens"]  # padded in front, so that all answers end alike
-        sequences[i] = torch.tensor(row, device="cuda")
-    prompt_lens = torch.full((args.requests,), length - args.new, device="cuda")
-    loss, _ = policy_step(pkg, model, opt, sequences, prompt_lens, torch.randn(args.requests, device="cuda"), bonus=0.01)
+    sequences, prompt_lens, lens = sequences_of(prompts, answers, "cuda")
+    loss, _ = policy_step(pkg, model, opt, sequences, prompt_lens, torch.randn(args.requests, device="cuda"), bonus=0.01, lens=lens)
     print(f"policy step: loss {float(loss):.4f}")
 
 
