@@ -156,7 +156,8 @@ class Server:
 
 
 def token_logprobs_function(pkg):
-    """token_logprobs as an autograd.Function: apply(logits, targets, scale) -> (logp, entropy)."""
+    """token_logprobs as an autograd.Function: apply(logits, targets, scale) -> (logp, entropy). Its gradient has none of its own: a second derivative
+    raises instead of being left out."""
     import torch
 
     class TokenLogprobs(torch.autograd.Function):
@@ -168,6 +169,7 @@ def token_logprobs_function(pkg):
             return logp, entropy
 
         @staticmethod
+        @torch.autograd.function.once_differentiable
         def backward(ctx, d_logp, d_entropy):
             logits, targets, lse, entropy = ctx.saved_tensors
             return pkg.token_logprobs_backward(logits, targets, lse, entropy, d_logp.contiguous(), d_entropy.contiguous(), ctx.scale), None, None
