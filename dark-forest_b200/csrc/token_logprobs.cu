@@ -479,7 +479,10 @@ __global__ void __launch_bounds__(kGradThreads) k_token_logprobs_backward(const 
   const float g_all = -p.scale * fmaf(h, entropy, g), h_all = -p.scale * h, g_one = p.scale * g;
   const uint32_t one = has ? (uint32_t)target : 0xffffffffu;
   auto gradient = [&](float x, uint32_t i) {  // -scale p (g + h (log p + entropy)), and scale g at the target; p = 0 has no part (log p = -inf)
-    const float y = fmaf(x, p.scale, -lse), prob = ex2_approx(y * kLog2e);
+    // log p is at most 0: the rounding of an lse of 10^30 (a row masked with the type's lowest value) must not become an exponent. NaN stays NaN.
+    float y = fmaf(x, p.scale, -lse);
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(0.0f));
+    const float prob = ex2_approx(y * kLog2e);
     const float d = prob == 0.0f ? 0.0f : prob * fmaf(h_all, y, g_all);
     return i == one ? d + g_one : d;
   };
