@@ -9,9 +9,12 @@
 // new largest element.
 //
 // The tokens of one page form a run of the slot map (row, row + 1, ... of one page). A warp takes a run, one head, and K or V, so that everything that
-// shares a scale is one warp's and nothing is exchanged; its first slot says how many rows the page had. Bound by HBM: rows are read once (up to
-// kHeld rows' elements stay in registers between the maximum and the rounding), codes written once: 8205 tokens of 12 heads of 64, fp32 to int8, 63 MB in 17 us, 3.7
-// TB/s (56 % of a copy's rate; what is missing is the start and the end of one round of warps).
+// shares a scale is one warp's and nothing is exchanged; its first slot says how many rows the page had. Rows are read once (up to
+// kHeld rows' elements stay in registers between the maximum and the rounding), codes written once: 8205 tokens of 12 heads of 64, fp32 to int8, 63 MB in 18 us, 3.5
+// TB/s (53 % of a copy's rate). What is missing is the second round: 6168 warps of which 24 an SM are there at once are 1.7 rounds of a chain slots ->
+// rows -> maximum -> codes (56 % of the issue slots in use, an instruction waits for loads three times as long as for its slot). bf16: 1.3 rounds, the same time for
+// 38 MB. A page whose scale grows has its older codes rounded again, word after word of a lane: 4096 single tokens of 8 heads of 128 take 25 us (floor 4), 130 if all
+// of their pages' scales grow in the same call.
 #include <math.h>
 
 #include "cache_codes.cuh"
@@ -130,7 +133,7 @@ __global__ void __launch_bounds__(kAppendThreads, BF16 ? (kHeld == 8 ? 8 : 6) : 
   const bool goes_on = valid && my_row > 0 && before == my_slot - 1;
   const uint32_t going_on = __ballot_sync(0xffffffffu, goes_on);
   // A run's first turn and the scale that its page has are loaded while the run before it is worked on: a decode step's runs are of
-  // one token each, and their loads would otherwise follow one another (4096 tokens of 8 heads of 128: 57 us, 23 this way).
+  // one token each, and their loads would otherwise follow one another (4096 tokens of 8 heads of 128: 57 us, 25 this way).
   struct Run {
     uint32_t at, page, row, n;
     int32_t slot;
@@ -235,9 +238,9 @@ int finish(int st) {
 
 template <bool BF16, int FORMAT>
 int launch(AppendParams &p, cudaStream_t s) {
-  // A slot to a warp while that leaves no more than two rounds of resident warps (16 an SM: registers), else windows of up to 32 slots: in a
+  // A slot to a warp while that leaves no more than 32 warps an SM (16 to 32 of them are there at once, by the variant's registers), else windows of up to 32 slots: in a
   // prompt only every 16th slot or so begins a run, and warps that find none cost more than the others' work (8205 tokens of 12 heads: 110 us with a slot
-  // to a warp, 18 with windows). 64 tokens of 8 heads, a warp each: 3.0 us, of which 2.4 are a launch.
+  // to a warp, 18 with windows). 64 tokens of 8 heads, a warp each: 3.4 us, of which 2.4 are a launch.
   const int n_sm = sm_count();
   if (n_sm == 0) return DF_ERR_CUDA;
   const unsigned long long all = (unsigned long long)p.n_tokens * 2 * p.H, two_rounds = 32ull * (unsigned)n_sm;

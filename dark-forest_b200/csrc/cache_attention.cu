@@ -15,20 +15,22 @@
 // Precision. An fp32 query row, times a power of two that brings its largest element to 1 .. 2, enters as two halves (22 bits), and so do the
 // weights exp(s - m) * 2^15: the 16 rows of an instruction are then 8 rows and their second parts, and the two accumulators are added. A bf16 row
 // fits one half; its weights are two as well: in tiles of 8 rows the second halves take the other 8 (as zeros they cost registers: 2 CTAs an SM, and 72
-// us instead of 69 in the first case below), in tiles of 16 they are multiplied behind the first ones (16 requests of 20 rows, 8 heads of 128: 59 us;
-// rounded to 11 bits 54, and a result of 8 bits then comes out as its neighbour now and then: 6e-4 of it in the 2-norm). V's scales enter the weights as
-// cache_line.cuh says (unit_exponent). The products of 32 tokens are added to the row's fp32 sums.
+// us instead of 69 at 32 requests of bf16), in tiles of 16 they are multiplied behind the first ones (16 requests of 20 rows, 8 heads of 128:
+// 54 to 59 us; with weights rounded to 11 bits a result of 8 bits comes out as its neighbour now and then, 6e-4 of it in the 2-norm). V's scales enter the weights as
+// cache_line.cuh says (unit_exponent; 59 to 63 us there, 1 to 2 % with few rows). The products of 32 tokens are added to the row's fp32 sums.
 //
 // Work. A CTA is one warp that loads (tensor-map copies of 16 tokens, 128-byte swizzle: the reads above are then free of bank conflicts at
-// head sizes 64 and 128) and four that compute, over a ring of stages of 64 tokens. A request with no more rows (query tokens times heads per K/V head)
-// than a warp takes is computed with its tokens dealt to the four warps; one with more has its rows dealt to them, and every warp goes over
-// all tokens. Work is dealt out as cache_line.cuh says; a stage where rows are dealt counts four units, since it takes four times as long. Calls of many rows go
-// to cache_attention_many.cu.
+// head sizes 64 and 128) and four that compute, over a ring of stages of 64 tokens. Of a request with no more rows (query tokens times heads per K/V
+// head) than a warp takes, the tokens are dealt to the four warps; with up to twice as many, the rows to two pairs of warps and the tokens to the two of a
+// pair; with more, the rows to all four, and every warp goes over all tokens. A stage then counts one, two or four units of the line on which work is dealt out (cache_line.cuh),
+// since it takes a warp as much longer. Calls of many rows go to cache_attention_many.cu.
 //
-// What it reaches. 32 requests of 200 to 16000 tokens, one new each, 32 heads on 8 of 128, bf16 and e4m3: 69 us for 342 MB, 4.9 TB/s, 75 % of a copy's rate. One request of
-// 131073 tokens, 16 heads of 128, fp32 and int8: 112 us for 537 MB, 4.8 TB/s. One of 300 tokens, 12 heads of 64: 6.7 us, of which 2.4 are a launch. The copies
-// alone (no arithmetic) took 92 us of the second. What is left is issue: 700 instructions per 32 tokens (waits and the
-// loading warp's included), 310 of them in the ALU pipe, which widens (two per clock and SM), 64 products; and 8 to 10 us for a segment's beginning, its end and the addition of its parts.
+// What it reaches. 32 requests of 200 to 16000 tokens, one new each, 32 heads on 8 of 128, bf16 and e4m3: 66 us for 342 MB, 5.2 TB/s, 79 % of a copy's rate. One request of
+// 131073 tokens, 16 heads of 128, fp32 and int8: 107 us for 537 MB, 5.0 TB/s. One of 300 tokens, 12 heads of 64: 7.2 us, of which 2.4 are a launch. The copies
+// alone (no arithmetic) took 92 us of the second. What is left is latency with few warps to hide it: twelve computing warps an SM, 3.5 warps a scheduler of which 0.75 (first case) and 0.98 (second)
+// can issue, 47 and 55 % of the issue slots in use; for each slot that a warp issues in it waits 2.3 and 1.7 for fixed latencies, 1.2 and 0.7 for memory; the ALU pipe,
+// which widens, is 42 and 48 % busy, the tensor pipe a third. 735 instructions per 32 tokens (waits and the loading warp's included), 325 of them in the ALU pipe, 64
+// products. A segment's beginning, its end and the addition of its parts take 8 to 10 us. 16 rows a warp: two CTAs an SM, 2.3 warps a scheduler, 0.43 of them able to issue, 35 % of the slots.
 #include <float.h>
 #include <math.h>
 
@@ -747,8 +749,10 @@ extern "C" int df_cache_attention(const void *q, const void *k_cache, const void
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   // How many rows requests have on average decides who multiplies. Up to 8: a warp's few. Up to 32: 16 rows a warp. Above: tiles of 128 rows on tcgen05, which
   // take the same time for 9 rows as for 32. Measured over 3000 to 6000 cached tokens, mma.sync to tcgen05, us, bf16 and fp32: 16 requests of 12 heads of
-  // 64, 16 rows 37 to 79, 52 to 97; 32 rows 56 to 80, 80 to 98; 64 rows 97 to 78, 142 to 102. 16 requests of 8 heads of 128, 20 rows 68 to 75, 105 to
-  // 100; 32 rows 74 to 75, 113 to 99; 64 rows 133 to 79, 198 to 106. One request of 12 heads of 64, 24 rows 27 to 22, 31 to 26; 40 rows 53 to 23, 59 to 27.
+  // 64, 16 rows 47 to 100, 54 to 101; 32 rows 74 to 100, 84 to 102; 64 rows 129 to 100, 148 to 103. 16 requests of 8 heads of 128, 20 rows 89 to 88, 102 to
+  // 96; 32 rows 96 to 89, 111 to 97; 64 rows 171 to 91, 195 to 102. One request of 12 heads of 64, 24 rows 30 to 26, 32 to 27; 40 rows 58 to 27, 60 to 28.
+  // These are requests alike. The mean decides for the whole call, so requests unlike each other cost more together than apart: 31 single tokens beside
+  // a piece of 500 tokens, 12 heads of 64 in fp32, 134 us (49 and 40 by themselves); 24 beside 8 pieces of 128, 32 heads on 8 of 128 in bf16, 232 (43 and 138).
   const uint64_t rows = (uint64_t)n_tokens * p.group;
   if (rows > 32ull * n_requests) return finish(cache_attention_many(p, k_cache, v_cache, q_bf16 != 0, format, s));
   const bool few = rows <= 8ull * n_requests;

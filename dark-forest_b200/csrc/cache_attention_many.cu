@@ -12,14 +12,14 @@
 // Precision: as there. An fp32 row is two halves (two K-steps for one, into the same accumulators), a bf16 row one; weights are two either way, and are held
 // times 2^7; what they refer to (the maximum m, and the unit 2^(m + e) of cache_line.cuh that V's scales need) is moved when a row's own weights have grown by 2^8 (the
 // accumulators are then rescaled by the row's thread), so that they stay in the halves' range either way.
-// What bounds it. Two requests of 500 tokens over 6000 to 9000 cached ones, 12 heads of 64, fp32, int8: 99 us, 254 TFLOP/s of the formula's operations (twice as
+// What bounds it. Two requests of 500 tokens over 6000 to 9000 cached ones, 12 heads of 64, fp32, int8: 100 us, 250 TFLOP/s of the formula's operations (twice as
 // many are done). A stage takes 1.1 us; of that the tensor pipe works a quarter, and the issuing warp is busy for 1300 cycles (waits apart; one
 // instruction of 64 columns costs it 70), nearly as long as a row's warp is (2500 cycles for every second stage, with two of them and a
-// widening warp on each scheduler). One request of 2000 tokens over 8000, 32 heads on 8 of 128: 485 us in bf16, 605 us in fp32.
+// widening warp on each scheduler: 53 % of the issue slots, 0.8 of 3.5 warps able to issue). One request of 2000 tokens over 8000, 32 heads on 8 of 128: 485 us in bf16, 605 us in fp32.
 // What it came from: row tiles on mma.sync 244 us; four row warps 152; eight, each with every second stage 133; a score's factor and the shift of its exponent in one
 // operation 125; one branch around the products of a stage 114; masks and rescaling in tensor memory, without spilling the scores 108; scores two stages
-// ahead 99; outputs added up every 16 stages, which all precision above 5.9e-6 needs, 106 (32 heads of 128 636), with states that a warp reads and writes side by side 99
-// (476). Measured and left out: more registers for the row warps by setmaxnreg (more spills in all), segments counted as 2 or 4 stages more (the
+// ahead 99; outputs added up every 16 stages, which all precision above 5.9e-6 needs, 106, with states that a warp reads and writes side by side 99; V's scales by what a
+// row sees 100. Measured and left out: more registers for the row warps by setmaxnreg (more spills in all), segments counted as 2 or 4 stages more (the
 // same, and 7 % more where CTAs have two), keys widened one stage ahead only (113).
 #include "cache_line.cuh"
 
@@ -188,7 +188,7 @@ k_cache_attention_many(const __grid_constant__ CUtensorMap k_map, const __grid_c
       if (!mbar_wait_warp(bar(K_FULL + b), (j >> 1) & 1, &s_abort)) return false;
       if (j >= 2 && !mbar_wait_warp(bar(S_FREE + b), ((j >> 1) - 1) & 1, &s_abort)) return false;
       tc_fence_after_sync();
-      if (elect_one()) {  // one branch for all: see above
+      if (elect_one()) {  // one election for all products of a stage: one for each cost 114 us where this takes 108
 #pragma unroll
         for (uint32_t part_of_q = 0; part_of_q < kParts; ++part_of_q)
 #pragma unroll

@@ -67,7 +67,9 @@ constexpr unsigned int DEV_STATUS_BOUNDS = 2u;
 // so the access itself stays inside the tensor and the context stays usable; df_sync_status then returns
 // DF_ERR_DEVICE_BOUNDS. In the normal build the macro is the index itself. (The other tensor-core
 // kernels move their tiles with TMA, whose tensor maps bound every copy in hardware; the row statistics, and the results of the one-tile kernels and of
-// the forward, they move by plain accesses behind a comparison with the number of rows, which no build checks.)
+// the forward, they move by plain accesses behind a comparison with the number of rows, which no build checks. Nor do the kernels of the paged cache and
+// the log probabilities go through DF_IDX: what they read on the GPU to index by, slots, pages, lengths, starts and targets, they compare with the sizes that they were
+// given in every build.)
 #ifdef DF_BOUNDS_CHECK
 #ifdef __CUDACC__
 __device__ __forceinline__ size_t df_checked_index(size_t i, size_t n, unsigned int *status) {

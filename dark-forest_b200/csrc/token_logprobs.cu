@@ -9,8 +9,9 @@
 // Both directions are bound by HBM: the forward reads every logit once, the gradient reads and writes it once. In the forward a CTA, or where there are few
 // rows a cluster of them, walks a row once, kChunk 16-byte groups a thread at a time, with a running maximum and sums per thread; the CTAs' parts
 // (maximum, sums, best keys) meet in the shared memory of the cluster's first. Holding the row in shared memory instead (four CTAs or two of an SM) took
-// 50 to 66 us at 1024 x 50257 bf16, 27 this way (3.8 TB/s): loads of one row then ran beside the sums of one other at best. What is left is issue: in bf16 an
-// element costs some 5 instructions (widening, exponential, two sums, maximum). fp32: 40 us, 5.2 TB/s.
+// 50 to 66 us at 1024 x 50257 bf16, 27 this way (3.8 TB/s): loads of one row then ran beside the sums of one other at best. fp32: 40 us, 5.2 TB/s. What is left in
+// bf16: all rows are there at once and in the same phase, and looking for alternatives, when memory idles, takes 3 to 5 us of it; the walk takes 24 (floor 15.7), with 60 % of
+// the issue slots in use (some 5 instructions an element) and the exponentials' pipe half busy. The gradient, 512 x 50257: fp32 34 us (floor 31.5), bf16 19 (15.7; 80 % of the issue slots).
 // Alternatives without sorting a row: each of the 4 (16) warps names its 8 (2) largest lane maxima; the k-th largest of these 32 is a bound that at
 // least k elements reach, and for logits in no particular order few others do. A thread also keeps the maxima of up to kParts parts of
 // its elements; only parts that reach the bound are read again (out of L2), and what is found is put in a list and ranked by counting (key: the value's

@@ -390,7 +390,7 @@ DF_API int df_chunked_logit_ce(float *logits, const uint32_t *targets, float *gr
 /* ---- serving a batch of requests over a paged cache held in 8 bits (no counterpart in the reference, whose decode forms
  * above read one sequence's fp32 or bf16 cache) ----
  * Cache: k_cache, v_cache are codes [n_pages][n_kv_heads][page_size][d_head], one byte each, k_scale, v_scale [n_pages][n_kv_heads]
- * fp32; an element is code * scale of its page and head. `format` DF_CACHE_INT8: the code is a signed byte; DF_CACHE_E4M3: an 8-bit float
+ * fp32, not negative (NaN: a page that holds a NaN or infinity); an element is code * scale of its page and head. `format` DF_CACHE_INT8: the code is a signed byte; DF_CACHE_E4M3: an 8-bit float
  * (1 sign, 4 exponent and 3 fraction bits, finite up to 448; the codes 0x7f and 0xff, which df_cache_append never writes, are NaN).
  * Token t of request r lies in page block_table[r * table_width + t / page_size], row t % page_size; its slot is page * page_size + row.
  * d_head is a multiple of 16 up to 128, page_size a multiple of 16 up to 256 (anything else: DF_ERR_UNSUPPORTED), n_pages * page_size below 2^31.
@@ -417,7 +417,9 @@ DF_API int df_chunked_logit_ce(float *logits, const uint32_t *targets, float *gr
  *   df_cache_attention  Rows of q [n_tokens][n_heads * d_head] (fp32, or bf16 with q_bf16; out alike), request after request as starts[n_requests + 1]
  *       says, against the requests' cached tokens: with q_len = starts[r + 1] - starts[r], row j of request r sees its tokens 0 .. lens[r] - q_len + j
  *       (its own is in the cache already). Query head h reads K/V head h / (n_heads / n_kv_heads). lse [n_tokens][n_heads]: natural logsumexp of the
- *       scaled scores, may be NULL. Rows that see nothing: out = 0, lse = -inf. Rows outside every request are left as they are.
+ *       scaled scores, may be NULL. Precision: q enters the products in 22 bits (bf16: its own 8), codes exactly, weights in 22 bits relative to the row's largest
+ *       weight times V scale; sums in fp32, those of up to 512 tokens (bf16 calls of many rows: of a CTA's whole share) in the tensor cores, which cut them off instead
+ *       of rounding; bf16 results are rounded once. Rows that see nothing: out = 0, lse = -inf. Rows outside every request are left as they are.
  *       Where starts falls from one request to the next nothing is computed and df_sync_status returns DF_ERR_DEVICE_BOUNDS.
  *       workspace: DF_CACHE_WORKSPACE_BYTES, 16-byte aligned, zeroed once by the caller; every call leaves it ready for the next.
  *       Calls that can overlap need a workspace each. */
