@@ -127,6 +127,7 @@ __device__ __forceinline__ bool next_part(const AttendParams &p, Line &line, Par
 
 // Sums over the requests, in shared memory, and this CTA's place on the line. All threads of the CTA call it; false: nothing is left for this CTA. The barrier in
 // it is the only one. Starts that fall somewhere let rows belong to several requests: their units could pass what the line counts to, so nothing is done then.
+constexpr uint32_t kFalls = 0xffffffffu;  // in the place of the longest segment's units (below 2^31)
 template <class W>
 struct LineSmem {
   uint32_t units[W::kThreads], segments[W::kThreads], most[W::kThreads / 32];
@@ -136,14 +137,13 @@ __device__ __forceinline__ bool begin_line(const AttendParams &p, LineSmem<W> &s
   const uint32_t t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const uint32_t per = (p.n_requests + W::kThreads - 1) / W::kThreads, r0 = min(p.n_requests, t * per), r1 = min(p.n_requests, r0 + per);
   uint32_t units = 0, segments = 0, most = 0;
-  bool falls = false;
   for (uint32_t r = r0; r < r1; ++r) {
     const Request q = request_of<W>(p, r);
-    falls |= __ldg(p.starts + r + 1) < __ldg(p.starts + r);
     const uint32_t n = q.row_tiles * p.kv_heads;
     segments += n;
     units += n * span_of<W>(q);
     if (n) most = max(most, span_of<W>(q));
+    if (__ldg(p.starts + r + 1) < __ldg(p.starts + r)) most = kFalls;
   }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -154,10 +154,7 @@ __device__ __forceinline__ bool begin_line(const AttendParams &p, LineSmem<W> &s
   sm.units[t] = units;
   sm.segments[t] = segments;
   if (lane == 0) sm.most[warp] = most;
-  if (__syncthreads_or(falls)) {
-    if (blockIdx.x == 0 && t == 0 && p.status) atomicOr(p.status, DEV_STATUS_BOUNDS);
-    return false;
-  }
+  __syncthreads();
   uint32_t all_units = 0, all_segments = 0;
   most = 0;
 #pragma unroll
@@ -165,6 +162,10 @@ __device__ __forceinline__ bool begin_line(const AttendParams &p, LineSmem<W> &s
     all_units += sm.units[32 * w + 31];
     all_segments += sm.segments[32 * w + 31];
     most = max(most, sm.most[w]);
+  }
+  if (most == kFalls) {
+    if (blockIdx.x == 0 && t == 0 && p.status) atomicOr(p.status, DEV_STATUS_BOUNDS);
+    return false;
   }
   const uint32_t G = gridDim.x, seg_per = (all_segments + G - 1) / G, unit_per = max(W::kSegmentUnits + 8u, (all_units + G - 1) / G);
   line.whole = p.whole || (unsigned long long)seg_per * most <= unit_per + W::kSegmentUnits;  // cutting costs another end
