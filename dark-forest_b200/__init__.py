@@ -100,6 +100,12 @@ PROTOTYPES = {
     "df_cache_attention": (ctypes.c_int, [_P] * 11 + [_U64] + [_U32] * 8 + [_U64, _F32, _U32, _U32, _P]),
     "df_token_logprobs": (ctypes.c_int, [_P] * 7 + [_U32] * 2 + [_U64, _U32, _F32, _U32, _P]),
     "df_token_logprobs_backward": (ctypes.c_int, [_P] * 7 + [_U32] * 2 + [_U64] * 2 + [_F32, _U32, _P]),
+    "df_linear_cross_entropy_workspace_bytes": (_U64, [_U32] * 5),
+    "df_linear_cross_entropy": (ctypes.c_int, [_P] * 6 + [_U64] + [_U32] * 3 + [_U64] * 2 + [_F32, _U32, _P]),
+    "df_linear_cross_entropy_backward": (ctypes.c_int, [_P] * 8 + [_U64] + [_U32] * 3 + [_U64] * 4 + [_F32, _U32, _P]),
+    "df_orthogonalize_workspace_bytes": (_U64, [_U32] * 3),
+    "df_orthogonalize": (ctypes.c_int, [_P] * 3 + [_U64] + [_U32] * 3 + [_U64] * 4 + [_U32] + [_F32] * 4 + [_U32, _P]),
+    "df_muon_update": (ctypes.c_int, [_P] + [_U32] * 3 + [_F32] * 3 + [_U32, _F32, _U32] + [_F32] * 4 + [_P, _U64, _P]),
     "df_attn_init": (ctypes.c_int, []),
     "df_attn_backward_profile": (ctypes.c_int, [_P] * 10 + [_U32] * 4 + [_F32, _U32, _P, _P, _P]),
     "df_attn_set_option": (ctypes.c_int, [ctypes.c_int, ctypes.c_int]),
@@ -359,6 +365,48 @@ def token_logprobs(logits, targets, scale=1.0, top_k=0, logp=None, entropy=None,
 def token_logprobs_backward(logits, targets, lse, entropy, grad_logp, grad_entropy=None, scale=1.0, d_logits=None, stream=None):
     """Gradient of token_logprobs' logp and entropy with respect to the logits, in their type (grad_logp or grad_entropy may be None)."""
     return _calls.token_logprobs_backward(logits, targets, lse, entropy, grad_logp, grad_entropy, scale, d_logits, stream)
+
+
+# ------------------------------------------------------------------------------------------
+# Loss from hidden states and orthogonalised updates: what a training step does behind its last block (no counterpart in the reference).
+# workspace: a tensor of at least the bytes that the *_workspace_bytes function names, aligned to 256, kept by the program; None takes one from
+# torch's allocator for the call.
+# ------------------------------------------------------------------------------------------
+def linear_cross_entropy_workspace_bytes(rows, vocab, width, bf16, backward):
+    return int(lib().df_linear_cross_entropy_workspace_bytes(rows, vocab, width, int(bf16), int(backward)))
+
+
+def linear_cross_entropy(x, weight, targets, scale=1.0, loss=None, lse=None, workspace=None, stream=None):
+    """Softmax cross entropy of targets [rows] (int32; outside 0 .. vocab - 1: the row is left out) under scale * x weight^T, x [rows, width], weight [vocab, width]
+    (both fp32 or both bf16; rows may be strided). The logits are not kept. Returns (loss [rows], lse [rows]), 0 for rows that are left out."""
+    return _calls.linear_cross_entropy(x, weight, targets, scale, loss, lse, workspace, stream)
+
+
+def linear_cross_entropy_backward(x, weight, targets, lse, grad_loss, scale=1.0, d_x=None, d_weight=None, want_x=True, want_weight=True, workspace=None,
+                                  stream=None):
+    """Gradients of linear_cross_entropy's losses, weighted by grad_loss [rows], with respect to x and weight, in their type. Returns (d_x, d_weight);
+    None in the place of one that is not wanted."""
+    return _calls.linear_cross_entropy_backward(x, weight, targets, lse, grad_loss, scale, d_x, d_weight, want_x, want_weight, workspace, stream)
+
+
+MUON_COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # the polynomial that brings singular values near 1 in five steps
+
+
+def orthogonalize_workspace_bytes(n, rows, cols):
+    return int(lib().df_orthogonalize_workspace_bytes(n, rows, cols))
+
+
+def orthogonalize(update, steps=5, coefficients=MUON_COEFFICIENTS, eps=1e-7, out=None, workspace=None, stream=None):
+    """Matrices [rows, cols] or [n, rows, cols] (fp32 or bf16; rows and matrices may be strided), each divided by its Frobenius norm + eps and orthogonalised by
+    Newton-Schulz steps X <- a X + (b X X^T + c (X X^T)^2) X. Returns out, in the update's type; out may be the update."""
+    return _calls.orthogonalize(update, steps, coefficients, eps, out, workspace, stream)
+
+
+def muon_update(parameters, momenta, gradients, lr, momentum=0.95, weight_decay=0.0, nesterov=True, update_scale=1.0, steps=5, coefficients=MUON_COEFFICIENTS,
+                eps=1e-7, workspace=None, stream=None):
+    """One step on lists of matrices of one shape (fp32, contiguous), in place: momenta <- momentum * momenta + gradients, and parameters <- parameters (1 - lr
+    weight_decay) - lr update_scale * orthogonalize(gradients + momentum * momenta, or the momenta themselves without nesterov)."""
+    _calls.muon_update(parameters, momenta, gradients, lr, momentum, weight_decay, nesterov, update_scale, steps, coefficients, eps, workspace, stream)
 
 
 # ------------------------------------------------------------------------------------------

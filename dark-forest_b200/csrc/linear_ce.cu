@@ -1,0 +1,835 @@
+// linear_ce.cu — softmax cross entropy from hidden states and the output weight, without keeping the logits (sm_100a):
+//   z = scale * x w^T [R, V],  lse_r = log sum_v exp z_rv,  loss_r = lse_r - z_r,target
+//   G = exp(z - lse) - onehot,  d_x = (grad * scale) G w,  d_w = G^T (grad * scale) x
+// Rows whose target is outside 0 .. V - 1 are left out: loss, lse and gradients 0, whatever x holds there.
+//
+// Forward: one product with an epilogue that keeps of every row and 128 columns the largest logit and the sum of exponentials, and
+// the target's logit; a second kernel joins them. bf16 operands enter as they are (products exact, sums fp32). fp32 operands are cut
+// into two fp16 parts (product_sm100.cuh), x scaled row by row, w as a whole.
+// Backward, per piece of the vocabulary: the logits again with an epilogue that writes G in fp16 (one part for bf16 calls: 11 bits, where a
+// bf16 result has 8; two for fp32 calls: 22), then d_w = G^T x' with x' = grad * x, complete for its piece, and d_x += G w in fp32, its
+// contraction split where there are few tiles. grad is not in G, so that a row's G keeps its bits however small its weight is.
+#include <math.h>
+
+#include "product_sm100.cuh"
+
+namespace df {
+namespace {
+
+using namespace ptx;
+
+constexpr float kGScale = 16384.0f;  // G is stored times 2^14
+constexpr uint64_t kPieceBytes = 128ull << 20;  // of G, or of a piece's weight in parts
+constexpr int kChunkBlocks = 1;                 // of 64: between takings out of an fp32 call's sums (measured: see k_product's users)
+
+int finish(int st) {
+  note_status(st);
+  return st;
+}
+
+struct Words {  // at the head of the workspace
+  uint32_t largest_w, largest_x;  // bits of the largest finite |w|, and |grad x| over the rows that count
+};
+
+__device__ __forceinline__ float load_f(const void *p, bool bf16, size_t i) {
+  return bf16 ? __uint_as_float((uint32_t)static_cast<const uint16_t *>(p)[i] << 16) : static_cast<const float *>(p)[i];
+}
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+// What a product is times for the logit: the call's scale and, for fp32 calls, the scales of the row's parts and of the weight's.
+__device__ __forceinline__ float logit_factor(float scale, const float *row_factor, const uint32_t *largest_w, uint32_t row, bool in) {
+  if (!row_factor) return scale;
+  float inv;
+  part_scale(*largest_w, &inv);
+  return scale * (in ? row_factor[row] : 1.0f) * inv;
+}
+
+// ---------------------------------------------------------------- epilogues
+struct LseEpi {
+  struct Params {
+    const int32_t *targets;
+    const float *row_factor;     // fp32 calls: 1 / scale of a row's parts
+    const uint32_t *largest_w;   // fp32 calls
+    float2 *parts;               // [slots][rows_pad]: largest logit (as the product has it), sum of e^(z - largest)
+    float *picked;               // [rows]: the target's logit (as the product has it)
+    float scale;
+    uint32_t rows, cols, rows_pad, col_base, slot_base;  // col_base: first column of the piece; cols: of the piece
+  };
+  const Params &p;
+  float c, m, s;
+  uint32_t row, col0;
+  int target;
+  bool in;
+  __device__ __forceinline__ LseEpi(const Params &q, uint8_t *, int) : p(q) {}
+  __device__ __forceinline__ void begin(const ProductTile &, uint32_t r, uint32_t c0) {
+    row = r;
+    col0 = c0;
+    in = r < p.rows;
+    target = in ? p.targets[r] - (int)p.col_base : -1;
+    c = logit_factor(p.scale, p.row_factor, p.largest_w, r, in) * kLog2e;
+    m = -INFINITY;
+    s = 0.0f;
+  }
+  // Differences are formed before they are scaled: the target's logit and the largest may agree in most of their bits.
+  __device__ __forceinline__ void block(int cg, float (&v)[32]) {
+    const uint32_t first = col0 + cg * 32;
+    if (first >= p.cols) return;
+    const uint32_t at = (uint32_t)target - first;
+    if (__any_sync(0xffffffffu, at < 32u)) {
+      float z = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 32; ++x) z = at == (uint32_t)x ? v[x] : z;
+      if (in && at < 32u && (uint32_t)target < p.cols) p.picked[row] = z;
+    }
+    if (first + 32 > p.cols) {
+#pragma unroll
+      for (int x = 0; x < 32; ++x) v[x] = first + x < p.cols ? v[x] : -INFINITY;
+    }
+    float top = v[0];
+#pragma unroll
+    for (int x = 1; x < 32; ++x) top = fmaxf(top, v[x]);
+    top = fmaxf(m, top);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float2 add = make_float2(0.0f, 0.0f);
+    const float2 minus = make_float2(-ref, -ref), cc = make_float2(c, c);
+#pragma unroll
+    for (int x = 0; x < 32; x += 2) {
+      const float2 d = mul2(add2(make_float2(v[x], v[x + 1]), minus), cc);
+      add = add2(add, make_float2(ex2_approx(d.x), ex2_approx(d.y)));
+    }
+    s = s * ex2_approx((m - ref) * c) + (add.x + add.y);
+    m = top;
+  }
+  __device__ __forceinline__ void end() {
+    if (in && col0 < p.cols) p.parts[(size_t)(p.slot_base + col0 / 128) * p.rows_pad + row] = make_float2(m, s);
+  }
+};
+
+template <int PARTS>
+struct GradEpi {
+  struct Params {
+    const int32_t *targets;
+    const float *lse, *row_factor;
+    const uint32_t *largest_w;
+    __half *g, *g_lo;  // [rows][pitch]
+    float scale;
+    uint32_t rows, cols, pitch, col_base, all_cols;
+  };
+  const Params &p;
+  uint4 *slab;
+  int lane;
+  float c, off;
+  uint32_t row, col0;
+  int target;
+  bool counts;
+  __device__ __forceinline__ GradEpi(const Params &q, uint8_t *sl, int l) : p(q), slab(reinterpret_cast<uint4 *>(sl)), lane(l) {}
+  __device__ __forceinline__ void begin(const ProductTile &, uint32_t r, uint32_t c0) {
+    row = r;
+    col0 = c0;
+    const bool in = r < p.rows;
+    const int t = in ? p.targets[r] : -1;
+    counts = (uint32_t)t < p.all_cols;
+    target = counts ? t - (int)p.col_base : -1;
+    c = logit_factor(p.scale, p.row_factor, p.largest_w, r, in);
+    off = counts ? p.lse[r] : 0.0f;
+  }
+  // 64 bytes of a row a lane: turned over in halves of the slab, then 8 rows of 64 bytes at a time
+  __device__ __forceinline__ void store(__half *dst, uint32_t first, const uint32_t (&h)[16], int half) {
+    uint4 *sl = slab + half * 128;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) sl[lane * 4 + (x ^ ((lane >> 1) & 3))] = make_uint4(h[4 * x], h[4 * x + 1], h[4 * x + 2], h[4 * x + 3]);
+    __syncwarp();
+    const uint32_t row0 = row - lane;
+    const int lrow = lane >> 2, chunk = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int rr = 8 * i + lrow;
+      const uint4 q = sl[rr * 4 + (chunk ^ ((rr >> 1) & 3))];
+      if (row0 + rr < p.rows) *reinterpret_cast<uint4 *>(dst + (size_t)(row0 + rr) * p.pitch + first + 8 * chunk) = q;
+    }
+  }
+  __device__ __forceinline__ void block(int cg, float (&v)[32]) {
+    const uint32_t first = col0 + cg * 32;
+    if (first >= p.cols) return;  // the pitch is a multiple of 32, so a block that begins inside may be written whole
+    const uint32_t at = (uint32_t)target - first;
+    // the logarithm of the probability first: where it is near 0 it has all its bits, and p - 1 at the target is e^log p - 1
+    const bool here = __any_sync(0xffffffffu, at < 32u);
+    float one = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 32; ++x) {
+      float z = fmaf(v[x], c, -off);
+      z = z > 0.0f ? 0.0f : z;  // a probability is at most 1, also under an lse that is rounded; a NaN stays
+      v[x] = z;
+    }
+    if (here) {
+#pragma unroll
+      for (int x = 0; x < 32; ++x) one = at == (uint32_t)x ? v[x] : one;
+      one = expm1f(one) * kGScale;
+    }
+#pragma unroll
+    for (int x = 0; x < 32; ++x) v[x] = counts ? ex2_approx(v[x] * kLog2e) * kGScale : 0.0f;
+    if (here) {
+#pragma unroll
+      for (int x = 0; x < 32; ++x) v[x] = at == (uint32_t)x ? one : v[x];
+    }
+    uint32_t hi[16], lo[16];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      if constexpr (PARTS == 2) split_half2(v[2 * x], v[2 * x + 1], hi[x], lo[x]);
+      else hi[x] = pack_half2(v[2 * x], v[2 * x + 1]);
+    }
+    __syncwarp();
+    store(p.g, first, hi, 0);
+    if constexpr (PARTS == 2) store(p.g_lo, first, lo, 1);
+  }
+  __device__ __forceinline__ void end() {}
+};
+
+// Sums into fp32 planes, one per slice of the contraction (d_x), or results of a whole contraction in the caller's type (d_w).
+struct OutEpi {
+  struct Params {
+    float *planes;              // d_x: [splits][rows][plane_pitch]
+    uint64_t plane_rows;
+    uint32_t plane_pitch;
+    int add;                    // the planes hold the pieces before this one
+    void *out;                  // d_w (planes null): row r of the product is row row_base + r of out
+    uint64_t out_stride;
+    uint32_t out_bf16, vec;     // vec: rows can be written 16 bytes (fp32) or 8 (bf16) at a time
+    const uint32_t *largest_x;  // d_w: its factor is scale / (2^14 s_x)
+    float scale;
+    uint32_t rows, cols;
+  };
+  const Params &p;
+  float4 *slab;
+  int lane;
+  float f;
+  float *plane;
+  uint32_t row0, col0;
+  __device__ __forceinline__ OutEpi(const Params &q, uint8_t *sl, int l) : p(q), slab(reinterpret_cast<float4 *>(sl)), lane(l) {}
+  __device__ __forceinline__ void begin(const ProductTile &t, uint32_t r, uint32_t c0) {
+    row0 = r - lane;
+    col0 = c0;
+    f = 1.0f;
+    if (p.planes) {
+      plane = p.planes + (size_t)t.split * p.plane_rows * p.plane_pitch;
+    } else {
+      float inv;
+      part_scale(*p.largest_x, &inv);
+      f = inv * (p.scale / kGScale);
+    }
+  }
+  __device__ __forceinline__ void block(int cg, float (&v)[32]) {
+    const uint32_t first = col0 + cg * 32;
+    if (first >= p.cols) return;
+    float4 q[8];
+    turn_over(slab, lane, v, q);
+    const uint32_t col = first + 4 * (lane & 7);
+    if (col >= p.cols) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t r = row0 + 4 * i + (lane >> 3);
+      if (r >= p.rows) continue;
+      if (p.planes) {
+        float4 *at = reinterpret_cast<float4 *>(plane + (size_t)r * p.plane_pitch + col);
+        if (p.add) {
+          const float4 old = *at;
+          q[i].x += old.x; q[i].y += old.y; q[i].z += old.z; q[i].w += old.w;
+        }
+        *at = q[i];
+        continue;
+      }
+      const float w[4] = {q[i].x * f, q[i].y * f, q[i].z * f, q[i].w * f};
+      const size_t at = (size_t)r * p.out_stride + col;
+      if (p.vec && col + 4 <= p.cols) {
+        if (p.out_bf16) {
+          uint2 b;
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.x) : "f"(w[1]), "f"(w[0]));
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.y) : "f"(w[3]), "f"(w[2]));
+          *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) = b;
+        } else {
+          *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = make_float4(w[0], w[1], w[2], w[3]);
+        }
+        continue;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (col + x >= p.cols) break;
+        if (p.out_bf16) {
+          uint32_t b;
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(0.0f), "f"(w[x]));
+          static_cast<uint16_t *>(p.out)[at + x] = (uint16_t)b;
+        } else {
+          static_cast<float *>(p.out)[at + x] = w[x];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void end() {}
+};
+
+// ---------------------------------------------------------------- around the products
+// The largest finite magnitude of w (first `w_blocks` blocks) and of grad * x over the rows that count (the others), a warp a row.
+struct RangeParams {
+  const void *w, *x;
+  const float *grad;
+  const int32_t *targets;
+  Words *words;
+  uint64_t w_stride, x_stride;
+  uint32_t vocab, rows, width, w_blocks, bf16;
+};
+__global__ void __launch_bounds__(256) k_ranges(const RangeParams p) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool is_w = blockIdx.x < p.w_blocks;
+  const uint32_t n = is_w ? p.vocab : p.rows, step = (is_w ? p.w_blocks : gridDim.x - p.w_blocks) * 8;
+  const void *src = is_w ? p.w : p.x;
+  const uint64_t stride = is_w ? p.w_stride : p.x_stride;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(src) | (stride * (p.bf16 ? 2 : 4));
+  uint32_t top = 0;
+  for (uint32_t r = (is_w ? blockIdx.x : blockIdx.x - p.w_blocks) * 8 + warp; r < n; r += step) {
+    float g = 1.0f;
+    if (!is_w) {
+      if ((uint32_t)p.targets[r] >= p.vocab) continue;
+      g = p.grad ? p.grad[r] : 1.0f;
+    }
+    const size_t at = (size_t)r * stride;
+    uint32_t k = 0;
+    if ((bits & 15u) == 0) {
+      const uint32_t per = p.bf16 ? 8 : 4, n16 = p.width / per;
+      const uint4 *row = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(src) + at * (p.bf16 ? 2 : 4));
+#pragma unroll 4
+      for (uint32_t i = lane; i < n16; i += 32) {
+        const uint4 q = row[i];
+        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (p.bf16) {
+            top = max(top, finite_bits(__uint_as_float(u[x] << 16) * g));
+            top = max(top, finite_bits(__uint_as_float(u[x] & 0xffff0000u) * g));
+          } else {
+            top = max(top, finite_bits(__uint_as_float(u[x]) * g));
+          }
+        }
+      }
+      k = n16 * per;
+    }
+    for (k += lane; k < p.width; k += 32) top = max(top, finite_bits(load_f(src, p.bf16, at + k) * g));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  __shared__ uint32_t tops[8];
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = max(top, tops[i]);
+    atomicMax(is_w ? &p.words->largest_w : &p.words->largest_x, top);  // a maximum does not depend on the order
+  }
+}
+
+// Rows cut into parts (or, for bf16 calls, copied): a warp a row. scale_from: the word that the whole tensor's scale follows from; null: every
+// row its own, its inverse written to row_factor. grad: rows times grad, rows that do not count as zeros.
+struct PackParams {
+  const void *src;
+  const uint32_t *scale_from;
+  float *row_factor;
+  const float *grad;
+  const int32_t *targets;  // null: every row counts
+  uint16_t *hi, *lo;       // lo null: one part; raw: bf16 as they are (operands that cannot be copied in place)
+  uint64_t stride;
+  uint32_t rows, width, pitch, vocab, bf16, raw;
+};
+__global__ void __launch_bounds__(256) k_pack(const PackParams p) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const uint32_t r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= p.rows) return;
+  const bool counts = !p.targets || (uint32_t)p.targets[r] < p.vocab;
+  const float g = p.grad && counts ? p.grad[r] : 1.0f;
+  const size_t at = (size_t)r * p.stride, to = (size_t)r * p.pitch;
+  const bool wide = ((reinterpret_cast<uintptr_t>(p.src) | (p.stride * (p.bf16 ? 2 : 4))) & 15u) == 0;
+  // four elements at a time, zeros behind the end (the pitch is a multiple of 64)
+  auto four = [&](uint32_t k) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!counts) return v;
+    if (wide && k + 4 <= p.width) {
+      if (p.bf16) {
+        const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.src) + at + k);
+        v = make_float4(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u));
+      } else {
+        v = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.src) + at + k);
+      }
+    } else {
+      if (k < p.width) v.x = load_f(p.src, p.bf16, at + k);
+      if (k + 1 < p.width) v.y = load_f(p.src, p.bf16, at + k + 1);
+      if (k + 2 < p.width) v.z = load_f(p.src, p.bf16, at + k + 2);
+      if (k + 3 < p.width) v.w = load_f(p.src, p.bf16, at + k + 3);
+    }
+    if (p.grad) v = make_float4(v.x * g, v.y * g, v.z * g, v.w * g);
+    return v;
+  };
+  float s = 1.0f, inv;
+  if (!p.raw) {
+    uint32_t top = 0;
+    if (p.scale_from) {
+      top = *p.scale_from;
+    } else {
+#pragma unroll 4
+      for (uint32_t k = lane * 4; k < p.width; k += 128) {
+        const float4 v = four(k);
+        top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+    }
+    s = part_scale(top, &inv);
+    if (p.row_factor && lane == 0) p.row_factor[r] = inv;
+  }
+#pragma unroll 4
+  for (uint32_t k = lane * 4; k < p.width; k += 128) {
+    const float4 v = four(k);
+    uint2 hi, lo;
+    if (p.raw) {
+      hi = make_uint2((__float_as_uint(v.x) >> 16) | (__float_as_uint(v.y) & 0xffff0000u), (__float_as_uint(v.z) >> 16) | (__float_as_uint(v.w) & 0xffff0000u));
+    } else {
+      split_half2(v.x * s, v.y * s, hi.x, lo.x);
+      split_half2(v.z * s, v.w * s, hi.y, lo.y);
+    }
+    *reinterpret_cast<uint2 *>(p.hi + to + k) = hi;
+    if (p.lo) *reinterpret_cast<uint2 *>(p.lo + to + k) = lo;
+  }
+}
+
+// loss and lse of 32 rows a block: lanes are rows, warps share the slots
+struct JoinParams {
+  const float2 *parts;
+  const float *picked, *row_factor;
+  const uint32_t *largest_w;
+  const int32_t *targets;
+  float *loss, *lse;
+  uint32_t rows, cols, rows_pad, slots;
+  float scale;
+};
+__global__ void __launch_bounds__(1024) k_join(const JoinParams p) {
+  pdl_wait();
+  __shared__ float2 s_part[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t row = blockIdx.x * 32 + lane;
+  const float cn = logit_factor(p.scale, p.row_factor, p.largest_w, row, row < p.rows), c = cn * kLog2e;
+  float m = -INFINITY, s = 0.0f;
+  auto join = [&](float2 q) {
+    const float top = fmaxf(m, q.x), ref = top == -INFINITY ? 0.0f : top;
+    s = s * ex2_approx((m - ref) * c) + q.y * ex2_approx((q.x - ref) * c);
+    m = top;
+  };
+  if (row < p.rows) {
+#pragma unroll 4
+    for (uint32_t i = warp; i < p.slots; i += 32) join(p.parts[(size_t)i * p.rows_pad + row]);
+  }
+  s_part[warp][lane] = make_float2(m, s);
+  __syncthreads();
+  if (warp != 0 || row >= p.rows) return;
+#pragma unroll 1
+  for (int i = 1; i < 32; ++i) join(s_part[i][lane]);
+  const bool counts = (uint32_t)p.targets[row] < p.cols;
+  const float l = logf(s);
+  p.lse[row] = counts ? fmaf(m, cn, l) : 0.0f;
+  p.loss[row] = counts ? fmaf(m - p.picked[row], cn, l) : 0.0f;
+}
+
+// d_x = factor * sum of the planes, in the caller's type; rows that do not count get zeros
+struct SumParams {
+  const float *planes, *grad;
+  const int32_t *targets;
+  const uint32_t *largest_w;
+  void *out;
+  uint64_t out_stride, plane_size;
+  uint32_t rows, width, pitch, splits, vocab, out_bf16, vec;
+  float scale;
+};
+__global__ void __launch_bounds__(256) k_sum_planes(const SumParams p) {
+  pdl_wait();
+  const uint32_t per_row = (p.width + 3) / 4;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (uint64_t)per_row * p.rows) return;
+  const uint32_t r = (uint32_t)(i / per_row), col = (uint32_t)(i % per_row) * 4;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if ((uint32_t)p.targets[r] < p.vocab) {
+    float inv;
+    part_scale(*p.largest_w, &inv);
+    const float f = inv * (p.scale / kGScale) * p.grad[r];
+    const float *at = p.planes + (size_t)r * p.pitch + col;
+    for (uint32_t k = 0; k < p.splits; ++k) {
+      const float4 a = *reinterpret_cast<const float4 *>(at + k * p.plane_size);
+      v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+    }
+    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+  }
+  const size_t to = (size_t)r * p.out_stride + col;
+  const float w[4] = {v.x, v.y, v.z, v.w};
+  if (p.vec && col + 4 <= p.width) {
+    if (p.out_bf16) {
+      uint2 b;
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.x) : "f"(w[1]), "f"(w[0]));
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.y) : "f"(w[3]), "f"(w[2]));
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + to) = b;
+    } else {
+      *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to) = v;
+    }
+    return;
+  }
+  for (int x = 0; x < 4 && col + x < p.width; ++x) {
+    if (p.out_bf16) {
+      uint32_t b;
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(0.0f), "f"(w[x]));
+      static_cast<uint16_t *>(p.out)[to + x] = (uint16_t)b;
+    } else {
+      static_cast<float *>(p.out)[to + x] = w[x];
+    }
+  }
+}
+
+// ---------------------------------------------------------------- sizes
+uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+
+// What a call uses of its workspace, in bytes from its start (all of it multiples of 256).
+struct Layout {
+  uint64_t row_factor, x_parts, x_grad, w_parts, w_raw, parts, picked, g, planes, total;
+  uint32_t pitch;           // of rows of `width` 16-bit elements or floats
+  uint32_t piece, n_pieces; // columns of the vocabulary at a time
+  uint32_t slots, rows_pad;
+  int splits;               // of d_x's contraction
+};
+
+constexpr int kMaxSplits = 16;
+
+bool in_place(const void *p, uint64_t stride) { return ((reinterpret_cast<uintptr_t>(p) | (stride * 2)) & 15u) == 0; }
+
+Layout layout(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool backward) {
+  Layout l = {};
+  const uint64_t parts = bf16 ? 1 : 2;
+  l.pitch = (uint32_t)up(width, 64);
+  l.rows_pad = (uint32_t)up(rows, 32);
+  uint64_t per_col = (uint64_t)l.pitch * 2 * parts;
+  if (backward && (uint64_t)rows * 2 * parts > per_col) per_col = (uint64_t)rows * 2 * parts;
+  uint64_t most = kPieceBytes / per_col / 256 * 256;
+  if (most < 256) most = 256;
+  l.n_pieces = (uint32_t)((vocab + most - 1) / most);
+  if (bf16 && !backward) l.n_pieces = 1;  // nothing is kept per column but what joins the rows
+  l.piece = (uint32_t)up((vocab + l.n_pieces - 1) / l.n_pieces, 256);
+  l.n_pieces = (vocab + l.piece - 1) / l.piece;
+  uint64_t at = 256;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t here = at;
+    at += up(bytes, 256);
+    return here;
+  };
+  l.row_factor = take((uint64_t)rows * 4);
+  l.x_parts = take((uint64_t)rows * l.pitch * 2 * parts);
+  l.w_parts = take((uint64_t)l.piece * l.pitch * 2 * parts);
+  if (!backward) {
+    l.slots = (vocab + 127) / 128 + l.n_pieces;
+    l.parts = take((uint64_t)l.slots * l.rows_pad * 8);
+    l.picked = take((uint64_t)rows * 4);
+  } else {
+    l.x_grad = take((uint64_t)rows * l.pitch * 2 * parts);
+    if (bf16) l.w_raw = take((uint64_t)l.piece * l.pitch * 2);
+    l.g = take((uint64_t)rows * l.piece * 2 * parts);
+    // d_x has (rows / 256) (width / 256) tiles for some 74 pairs of SMs: its contraction is split until they are busy
+    const uint64_t tiles = ((rows + 255) / 256) * ((width + 255) / 256), blocks = l.piece / 64;
+    uint64_t n = (74 + tiles - 1) / tiles;
+    if (n > (uint64_t)kMaxSplits) n = kMaxSplits;
+    if (n > blocks) n = blocks;
+    l.splits = (int)(n < 1 ? 1 : n);
+    l.planes = take((uint64_t)l.splits * rows * l.pitch * 4);
+  }
+  l.total = at;
+  return l;
+}
+
+bool sizes_ok(uint32_t rows, uint32_t vocab, uint32_t width) {
+  return vocab > 0 && width > 0 && vocab < (1u << 30) && width < (1u << 24) && rows < (1u << 30);
+}
+
+// How many slices have blocks when n are cut into `wanted` of the same length. Asked again with the answer and no more blocks, it is no more.
+int slices(uint32_t n, int wanted) {
+  const uint32_t each = (n + (uint32_t)wanted - 1) / (uint32_t)wanted;
+  return (int)((n + each - 1) / each);
+}
+
+template <bool A_MN, bool B_MN, int PARTS, class Epi>
+int product(const Operand &a, const Operand &b, uint32_t M, uint32_t N, uint32_t K, int splits, bool bf16, const typename Epi::Params &e, cudaStream_t s) {
+  ProductParams p = {};
+  p.M = M;
+  p.N = N;
+  p.batch = 1;
+  p.n_kb = (int)((K + kProdK - 1) / kProdK);
+  p.splits = slices(p.n_kb, splits);
+  p.kb_per_split = (p.n_kb + splits - 1) / splits;
+  p.chunk = kChunkBlocks;
+  p.fmt = bf16 ? (uint32_t)kFmtBF16 : (uint32_t)kFmtF16;
+  return launch_product<ProdCfg<true, A_MN, B_MN, PARTS>, Epi>(a, b, p, e, s);
+}
+
+struct HeadCall {
+  const void *x, *w;
+  const int32_t *targets;
+  uint64_t x_stride, w_stride;
+  uint32_t rows, vocab, width;
+  bool bf16;
+  float scale;
+  uint8_t *ws;
+  Layout l;
+  cudaStream_t s;
+
+  const uint8_t *row_of_w(uint32_t v) const { return static_cast<const uint8_t *>(w) + (size_t)v * w_stride * (bf16 ? 2 : 4); }
+  uint16_t *at16(uint64_t offset) const { return reinterpret_cast<uint16_t *>(ws + offset); }
+
+  int pack(const void *src, uint64_t stride, uint32_t n, uint64_t to, bool raw, const uint32_t *scale_from, float *row_factor, const float *grad,
+           const int32_t *which) const {
+    PackParams p = {};
+    p.src = src;
+    p.scale_from = scale_from;
+    p.row_factor = row_factor;
+    p.grad = grad;
+    p.targets = which;
+    p.hi = at16(to);
+    p.lo = bf16 ? nullptr : at16(to) + (size_t)n * l.pitch;
+    p.stride = stride;
+    p.rows = n;
+    p.width = width;
+    p.pitch = l.pitch;
+    p.vocab = vocab;
+    p.bf16 = bf16;
+    p.raw = raw;
+    const int st = check_cuda(launch_kernel(k_pack, dim3((n + 7) / 8), dim3(256), 0, s, p));
+    note_launch();
+    return st;
+  }
+  Operand packed(uint64_t at, uint32_t n, bool is_bf16) const {
+    return {at16(at), at16(at) + (size_t)n * l.pitch, is_bf16, n, width, l.pitch, 0};
+  }
+  int ranges(const float *grad, bool of_x) const {
+    RangeParams p = {w, x, grad, targets, reinterpret_cast<Words *>(ws), w_stride, x_stride, vocab, rows, width, 0, bf16};
+    const uint32_t n_sm = (uint32_t)sm_count();
+    p.w_blocks = (vocab + 7) / 8 < 8 * n_sm ? (vocab + 7) / 8 : 8 * n_sm;
+    const uint32_t x_blocks = !of_x ? 0 : ((rows + 7) / 8 < 2 * n_sm ? (rows + 7) / 8 : 2 * n_sm);
+    int st = check_cuda(cudaMemsetAsync(ws, 0, sizeof(Words), s));
+    if (st != DF_OK) return st;
+    st = check_cuda(launch_kernel(k_ranges, dim3(p.w_blocks + x_blocks), dim3(256), 0, s, p));
+    note_launch();
+    return st;
+  }
+  // operands of the logits: bf16 in place where a copy can start there, else copied; fp32 in parts (x once, w piece by piece)
+  int logits_x(Operand *o) const {
+    if (bf16 && in_place(x, x_stride)) {
+      *o = {x, x, true, rows, width, x_stride, 0};
+      return DF_OK;
+    }
+    *o = packed(l.x_parts, rows, bf16);
+    return pack(x, x_stride, rows, l.x_parts, bf16, nullptr, bf16 ? nullptr : reinterpret_cast<float *>(ws + l.row_factor), nullptr, nullptr);
+  }
+
+  int forward(float *loss, float *lse) const {
+    const Words *words = reinterpret_cast<const Words *>(ws);
+    int st = DF_OK;
+    if (!bf16) st = ranges(nullptr, false);
+    Operand a;
+    if (st == DF_OK) st = logits_x(&a);
+    uint32_t slots = 0;
+    for (uint32_t c0 = 0; st == DF_OK && c0 < vocab; c0 += l.piece) {
+      const uint32_t n = vocab - c0 < l.piece ? vocab - c0 : l.piece;
+      Operand b = {row_of_w(c0), nullptr, true, n, width, w_stride, 0};
+      if (!(bf16 && in_place(w, w_stride))) {
+        st = pack(row_of_w(c0), w_stride, n, l.w_parts, bf16, &words->largest_w, nullptr, nullptr, nullptr);
+        b = packed(l.w_parts, n, bf16);
+      }
+      LseEpi::Params e = {};
+      e.targets = targets;
+      e.row_factor = bf16 ? nullptr : reinterpret_cast<const float *>(ws + l.row_factor);
+      e.largest_w = &words->largest_w;
+      e.parts = reinterpret_cast<float2 *>(ws + l.parts);
+      e.picked = reinterpret_cast<float *>(ws + l.picked);
+      e.scale = scale;
+      e.rows = rows;
+      e.cols = n;
+      e.rows_pad = l.rows_pad;
+      e.col_base = c0;
+      e.slot_base = slots;
+      slots += (n + 127) / 128;
+      if (st == DF_OK)
+        st = bf16 ? product<false, false, 1, LseEpi>(a, b, rows, n, width, 1, true, e, s) : product<false, false, 2, LseEpi>(a, b, rows, n, width, 1, false, e, s);
+    }
+    if (st != DF_OK) return st;
+    JoinParams j = {reinterpret_cast<const float2 *>(ws + l.parts), reinterpret_cast<const float *>(ws + l.picked),
+                    bf16 ? nullptr : reinterpret_cast<const float *>(ws + l.row_factor), &words->largest_w, targets, loss, lse, rows, vocab, l.rows_pad, slots, scale};
+    st = check_cuda(launch_kernel(k_join, dim3((rows + 31) / 32), dim3(1024), 0, s, j));
+    note_launch();
+    return st;
+  }
+
+  template <int PARTS>
+  int backward(const float *lse, const float *grad, void *d_x, uint64_t dx_stride, void *d_w, uint64_t dw_stride) const {
+    const Words *words = reinterpret_cast<const Words *>(ws);
+    const uint32_t elt = bf16 ? 2 : 4, wide = bf16 ? 7 : 15;
+    int st = ranges(grad, d_w != nullptr);
+    Operand a;
+    if (st == DF_OK) st = logits_x(&a);
+    if (st == DF_OK && d_w) st = pack(x, x_stride, rows, l.x_grad, false, &words->largest_x, nullptr, grad, targets);
+    int splits = l.splits;
+    for (uint32_t c0 = 0; st == DF_OK && c0 < vocab; c0 += l.piece) {
+      const uint32_t n = vocab - c0 < l.piece ? vocab - c0 : l.piece;
+      // w in fp16 parts, for d_x and for the logits of fp32 calls
+      st = pack(row_of_w(c0), w_stride, n, l.w_parts, false, &words->largest_w, nullptr, nullptr, nullptr);
+      const Operand wp = packed(l.w_parts, n, false);
+      Operand b = wp;
+      if (bf16) {
+        b = {row_of_w(c0), nullptr, true, n, width, w_stride, 0};
+        if (!in_place(w, w_stride)) {
+          if (st == DF_OK) st = pack(row_of_w(c0), w_stride, n, l.w_raw, true, nullptr, nullptr, nullptr, nullptr);
+          b = packed(l.w_raw, n, true);
+        }
+      }
+      typename GradEpi<PARTS>::Params e = {};
+      e.targets = targets;
+      e.lse = lse;
+      e.row_factor = bf16 ? nullptr : reinterpret_cast<const float *>(ws + l.row_factor);
+      e.largest_w = &words->largest_w;
+      e.g = reinterpret_cast<__half *>(ws + l.g);
+      e.g_lo = e.g + (size_t)rows * l.piece;
+      e.scale = scale;
+      e.rows = rows;
+      e.cols = n;
+      e.pitch = l.piece;
+      e.col_base = c0;
+      e.all_cols = vocab;
+      if (st == DF_OK) st = product<false, false, PARTS, GradEpi<PARTS>>(a, b, rows, n, width, 1, bf16, e, s);
+      const Operand g = {e.g, e.g_lo, false, rows, n, l.piece, 0};
+      if (st == DF_OK && d_x) {
+        if (c0 == 0) splits = slices((n + kProdK - 1) / kProdK, splits);
+        OutEpi::Params o = {};
+        o.planes = reinterpret_cast<float *>(ws + l.planes);
+        o.plane_rows = rows;
+        o.plane_pitch = l.pitch;
+        o.add = c0 > 0;
+        o.rows = rows;
+        o.cols = width;
+        st = product<false, true, PARTS, OutEpi>(g, wp, rows, width, n, splits, false, o, s);
+      }
+      if (st == DF_OK && d_w) {
+        OutEpi::Params o = {};
+        o.out = static_cast<uint8_t *>(d_w) + (size_t)c0 * dw_stride * elt;
+        o.out_stride = dw_stride;
+        o.out_bf16 = bf16;
+        o.vec = ((reinterpret_cast<uintptr_t>(o.out) | (dw_stride * elt)) & wide) == 0;
+        o.largest_x = &words->largest_x;
+        o.scale = scale;
+        o.rows = n;
+        o.cols = width;
+        st = product<true, true, PARTS, OutEpi>(g, packed(l.x_grad, rows, false), n, width, rows, 1, false, o, s);
+      }
+    }
+    if (st != DF_OK || !d_x) return st;
+    SumParams q = {};
+    q.planes = reinterpret_cast<const float *>(ws + l.planes);
+    q.grad = grad;
+    q.targets = targets;
+    q.largest_w = &words->largest_w;
+    q.out = d_x;
+    q.out_stride = dx_stride;
+    q.plane_size = (uint64_t)rows * l.pitch;
+    q.rows = rows;
+    q.width = width;
+    q.pitch = l.pitch;
+    q.splits = (uint32_t)splits;
+    q.vocab = vocab;
+    q.out_bf16 = bf16;
+    q.vec = ((reinterpret_cast<uintptr_t>(d_x) | (dx_stride * elt)) & wide) == 0;
+    q.scale = scale;
+    st = check_cuda(launch_kernel(k_sum_planes, dim3((unsigned)(((uint64_t)rows * ((width + 3) / 4) + 255) / 256)), dim3(256), 0, s, q));
+    note_launch();
+    return st;
+  }
+};
+
+// Whether [rows][stride] elements from a and those from b share memory.
+struct Span {
+  uintptr_t from, to;
+  Span(const void *p, uint64_t rows, uint64_t stride, uint64_t width, uint64_t elt) {
+    from = reinterpret_cast<uintptr_t>(p);
+    to = from + ((rows - 1) * stride + width) * elt;
+  }
+  bool meets(const Span &o) const { return from < o.to && o.from < to; }
+};
+
+int check_call(const void *x, const void *w, const int32_t *targets, uint32_t rows, uint32_t vocab, uint32_t width, uint64_t x_stride, uint64_t w_stride,
+               float scale) {
+  if (!sizes_ok(rows, vocab, width) || !(scale > 0.0f) || !isfinite(scale)) return DF_ERR_INVALID_ARG;
+  if ((rows > 1 && x_stride < width) || (vocab > 1 && w_stride < width) || x_stride >= (1ull << 32) || w_stride >= (1ull << 32)) return DF_ERR_INVALID_ARG;
+  if (rows && (!x || !targets)) return DF_ERR_INVALID_ARG;
+  return w ? DF_OK : DF_ERR_INVALID_ARG;
+}
+
+}  // namespace
+}  // namespace df
+
+using namespace df;
+
+extern "C" {
+
+uint64_t df_linear_cross_entropy_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t width, uint32_t bf16, uint32_t backward) {
+  if (rows == 0 || !sizes_ok(rows, vocab, width)) return 0;
+  return layout(rows, vocab, width, bf16 != 0, backward != 0).total;
+}
+
+int df_linear_cross_entropy(const void *x, const void *weight, const int32_t *targets, float *loss, float *lse, void *workspace, uint64_t workspace_bytes,
+                            uint32_t rows, uint32_t vocab, uint32_t width, uint64_t x_stride, uint64_t weight_stride, float scale, uint32_t bf16,
+                            void *stream) {
+  DF_RANGE("df_linear_cross_entropy");
+  int st = check_call(x, weight, targets, rows, vocab, width, x_stride, weight_stride, scale);
+  if (st != DF_OK) return finish(st);
+  if (rows == 0) return DF_OK;
+  if (!loss || !lse) return finish(DF_ERR_INVALID_ARG);
+  const Layout l = layout(rows, vocab, width, bf16 != 0, false);
+  if (!workspace || workspace_bytes < l.total || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return finish(DF_ERR_WORKSPACE);
+  const HeadCall call = {x, weight, targets, rows > 1 ? x_stride : up(width, 8), vocab > 1 ? weight_stride : up(width, 8), rows, vocab, width, bf16 != 0, scale,
+                         static_cast<uint8_t *>(workspace), l, static_cast<cudaStream_t>(stream)};
+  return finish(call.forward(loss, lse));
+}
+
+int df_linear_cross_entropy_backward(const void *x, const void *weight, const int32_t *targets, const float *lse, const float *grad_loss, void *d_x,
+                                     void *d_weight, void *workspace, uint64_t workspace_bytes, uint32_t rows, uint32_t vocab, uint32_t width,
+                                     uint64_t x_stride, uint64_t weight_stride, uint64_t dx_stride, uint64_t dw_stride, float scale, uint32_t bf16,
+                                     void *stream) {
+  DF_RANGE("df_linear_cross_entropy_backward");
+  int st = check_call(x, weight, targets, rows, vocab, width, x_stride, weight_stride, scale);
+  if (st != DF_OK) return finish(st);
+  if ((d_x && rows > 1 && dx_stride < width) || (d_weight && vocab > 1 && dw_stride < width) || dx_stride >= (1ull << 32) || dw_stride >= (1ull << 32))
+    return finish(DF_ERR_INVALID_ARG);
+  const uint64_t elt = bf16 ? 2 : 4;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {  // a sum over no rows
+    if (d_weight) st = check_cuda(cudaMemset2DAsync(d_weight, (vocab > 1 ? dw_stride : width) * elt, 0, width * elt, vocab, s));
+    return finish(st);
+  }
+  if (!lse || !grad_loss) return finish(DF_ERR_INVALID_ARG);
+  if (!d_x && !d_weight) return DF_OK;
+  const Span sx(x, rows, x_stride, width, elt), sw(weight, vocab, weight_stride, width, elt);
+  if (d_x) {
+    const Span o(d_x, rows, dx_stride, width, elt);
+    if (o.meets(sx) || o.meets(sw)) return finish(DF_ERR_INVALID_ARG);
+    if (d_weight && o.meets(Span(d_weight, vocab, dw_stride, width, elt))) return finish(DF_ERR_INVALID_ARG);
+  }
+  if (d_weight) {
+    const Span o(d_weight, vocab, dw_stride, width, elt);
+    if (o.meets(sx) || o.meets(sw)) return finish(DF_ERR_INVALID_ARG);
+  }
+  const Layout l = layout(rows, vocab, width, bf16 != 0, true);
+  if (!workspace || workspace_bytes < l.total || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return finish(DF_ERR_WORKSPACE);
+  const HeadCall call = {x, weight, targets, rows > 1 ? x_stride : up(width, 8), vocab > 1 ? weight_stride : up(width, 8), rows, vocab, width, bf16 != 0, scale,
+                         static_cast<uint8_t *>(workspace), l, s};
+  return finish(bf16 ? call.backward<1>(lse, grad_loss, d_x, dx_stride, d_weight, dw_stride) : call.backward<2>(lse, grad_loss, d_x, dx_stride, d_weight, dw_stride));
+}
+
+}  // extern "C"

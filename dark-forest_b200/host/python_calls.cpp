@@ -13,11 +13,13 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <string>
+#include <vector>
 
 #include "../../include/darkforest_kernels.h"
 
@@ -32,7 +34,8 @@ namespace {
   X(df_adamw_update) X(df_adamw_update_multi) X(launch_fused_attention) X(launch_fused_mha_forward)                          \
   X(launch_attention_backward) X(launch_fused_mha_backward) X(df_attn_last_status) X(df_attn_status_string)                  \
   X(df_cache_plan) X(df_cache_release) X(df_cache_append) X(df_cache_attention) X(df_token_logprobs)                        \
-  X(df_token_logprobs_backward)
+  X(df_token_logprobs_backward) X(df_linear_cross_entropy_workspace_bytes) X(df_linear_cross_entropy)                       \
+  X(df_linear_cross_entropy_backward) X(df_orthogonalize_workspace_bytes) X(df_orthogonalize) X(df_muon_update)
 
 struct Functions {
 #define X(name) decltype(&::name) name = nullptr;
@@ -527,6 +530,188 @@ PyObject *token_logprobs_backward(Args a) {  // logits targets lse entropy grad_
   return d.release();
 }
 
+// ---------------------------------------------------------------- loss from hidden states, orthogonalised updates
+// For the length of a call: its tensors' device, which becomes the current one, and every other tensor of the call has to be there.
+class OnDevice {
+ public:
+  explicit OnDevice(PyObject *first, const char *what) : device_(of(first, what)), guard_(device_) {}
+  void same(PyObject *o, const char *what) const {
+    if (o != Py_None && of(o, what) != device_) refuse(what, "on another device than the others");
+  }
+  // A workspace: the caller's, or one from the allocator that belongs to the call's stream, so that it is not given to another before the call is through.
+  void *workspace(Out &held, PyObject *given, PyObject *stream_arg, uint64_t bytes, uint64_t *size) const {
+    if (given != Py_None) {
+      same(given, "workspace");
+      if (!tensor(given).is_contiguous()) refuse("workspace", "must be contiguous");
+      *size = tensor(given).nbytes();
+      return tensor(given).data_ptr();
+    }
+    c10::cuda::OptionalCUDAStreamGuard there;
+    if (stream_arg != Py_None) there.reset_stream(c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(stream(stream_arg)), device_.index()));
+    held.wrap(at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(device_)));
+    *size = bytes;
+    return tensor(held.get()).data_ptr();
+  }
+
+ private:
+  static c10::Device of(PyObject *o, const char *what) {
+    const at::Tensor &t = tensor(o);
+    if (!t.is_cuda()) refuse(what, "must live on a CUDA device (no CPU path)");
+    return t.device();
+  }
+  c10::Device device_;
+  c10::cuda::CUDAGuard guard_;
+};
+
+struct Head {
+  Rows x, w;
+  int32_t *targets;
+};
+Head head(const OnDevice &on, Args a) {  // x weight targets
+  on.same(a[1], "weight");
+  on.same(a[2], "targets");
+  const Rows x = strided_rows(a[0], "x"), w = strided_rows(a[1], "weight");
+  if (w.cols != x.cols || w.bf16 != x.bf16) refuse("weight", "width or dtype differs from x");
+  return {x, w, ints(a[2], {x.rows}, "targets")};
+}
+
+PyObject *linear_cross_entropy(Args a) {  // x weight targets scale loss lse workspace stream
+  const OnDevice on(a[0], "x");
+  const Head h = head(on, a);
+  Out loss, lse, ws;
+  given_or_floats(loss, a[4], a[0], {h.x.rows}, "loss");
+  given_or_floats(lse, a[5], a[0], {h.x.rows}, "lse");
+  on.same(loss.get(), "loss");
+  on.same(lse.get(), "lse");
+  uint64_t size = 0;
+  void *work = on.workspace(ws, a[6], a[7], fn.df_linear_cross_entropy_workspace_bytes(h.x.rows, h.w.rows, h.x.cols, h.x.bf16, 0), &size);
+  call(fn.df_linear_cross_entropy, a[7], h.x.data, h.w.data, h.targets, ptr(loss.get()), ptr(lse.get()), work, size, h.x.rows, h.w.rows, h.x.cols, h.x.stride,
+       h.w.stride, real(a[3]), h.x.bf16);
+  return tuple_of({&loss, &lse});
+}
+
+PyObject *linear_cross_entropy_backward(Args a) {  // x weight targets lse grad_loss scale d_x d_weight want_x want_weight workspace stream
+  const OnDevice on(a[0], "x");
+  const Head h = head(on, a);
+  on.same(a[3], "lse");
+  on.same(a[4], "grad_loss");
+  float *lse = floats(a[3], {h.x.rows}, "lse"), *grad = floats(a[4], {h.x.rows}, "grad_loss");
+  const at::ScalarType type = h.x.bf16 ? at::kBFloat16 : at::kFloat;
+  Out d[2], ws;
+  Rows to[2] = {};
+  const Rows *like[2] = {&h.x, &h.w};
+  const char *names[2] = {"d_x", "d_weight"};
+  for (int i = 0; i < 2; ++i) {
+    if (!truth(a[8 + i])) {
+      d[i].keep(Py_None);
+      continue;
+    }
+    given_or_empty(d[i], a[6 + i], a[0], {static_cast<int64_t>(like[i]->rows), static_cast<int64_t>(like[i]->cols)}, type);
+    on.same(d[i].get(), names[i]);
+    to[i] = strided_rows(d[i].get(), names[i]);
+    if (to[i].rows != like[i]->rows || to[i].cols != like[i]->cols || to[i].bf16 != h.x.bf16) refuse(names[i], "shape or dtype differs from what it is the gradient of");
+  }
+  uint64_t size = 0;
+  void *work = on.workspace(ws, a[10], a[11], fn.df_linear_cross_entropy_workspace_bytes(h.x.rows, h.w.rows, h.x.cols, h.x.bf16, 1), &size);
+  call(fn.df_linear_cross_entropy_backward, a[11], h.x.data, h.w.data, h.targets, lse, grad, const_cast<void *>(to[0].data), const_cast<void *>(to[1].data), work,
+       size, h.x.rows, h.w.rows, h.x.cols, h.x.stride, h.w.stride, to[0].stride, to[1].stride, real(a[5]), h.x.bf16);
+  return tuple_of({&d[0], &d[1]});
+}
+
+struct Matrices {
+  void *data;
+  uint32_t n, rows, cols, bf16;
+  uint64_t matrix_stride, row_stride;
+};
+Matrices matrices(PyObject *o, const char *what) {
+  const at::Tensor &t = tensor(o);
+  const int64_t d = t.dim();
+  if (d != 2 && d != 3) refuse(what, "expected [rows, cols] or [n, rows, cols]");
+  if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16) refuse(what, "expected float32 or bfloat16");
+  if (t.size(d - 1) > 1 && t.stride(d - 1) != 1) refuse(what, "the elements of a row must lie together");
+  const int64_t rows = t.size(d - 2), cols = t.size(d - 1);
+  const int64_t row_stride = rows > 1 ? t.stride(d - 2) : cols;
+  if (row_stride < cols) refuse(what, "rows overlap");
+  return {t.data_ptr(), d == 3 ? below_2_31(t.size(0), what) : 1u, below_2_31(rows, what), below_2_31(cols, what), t.scalar_type() == at::kBFloat16 ? 1u : 0u,
+          d == 3 && t.size(0) > 1 ? static_cast<uint64_t>(t.stride(0)) : 0, static_cast<uint64_t>(row_stride)};
+}
+
+struct Polynomial {
+  float a, b, c;
+};
+Polynomial polynomial(PyObject *o) {
+  PyObject *s = PySequence_Tuple(o);
+  if (!s) throw PythonError();
+  float v[3] = {};
+  const bool three = PyTuple_GET_SIZE(s) == 3;
+  try {
+    for (int i = 0; three && i < 3; ++i) v[i] = real(PyTuple_GET_ITEM(s, i));
+  } catch (...) {
+    Py_DECREF(s);
+    throw;
+  }
+  Py_DECREF(s);
+  if (!three) refuse("coefficients", "expected three numbers");
+  return {v[0], v[1], v[2]};
+}
+
+PyObject *orthogonalize(Args a) {  // update steps coefficients eps out workspace stream
+  const OnDevice on(a[0], "update");
+  const Matrices u = matrices(a[0], "update");
+  const Polynomial q = polynomial(a[2]);
+  Out out, ws;
+  given_or_empty(out, a[4], a[0], tensor(a[0]).sizes(), u.bf16 ? at::kBFloat16 : at::kFloat);
+  on.same(out.get(), "out");
+  const Matrices o = matrices(out.get(), "out");
+  if (!tensor(out.get()).sizes().equals(tensor(a[0]).sizes()) || o.bf16 != u.bf16) refuse("out", "shape or dtype differs from update");
+  uint64_t size = 0;
+  void *work = on.workspace(ws, a[5], a[6], fn.df_orthogonalize_workspace_bytes(u.n, u.rows, u.cols), &size);
+  call(fn.df_orthogonalize, a[6], static_cast<const void *>(u.data), o.data, work, size, u.n, u.rows, u.cols, u.matrix_stride, u.row_stride, o.matrix_stride,
+       o.row_stride, u32(a[1]), q.a, q.b, q.c, real(a[3]), u.bf16);
+  return out.release();
+}
+
+class Sequence {  // a list or tuple of tensors
+ public:
+  Sequence(PyObject *o, const char *what) : s_(PySequence_Tuple(o)) {
+    if (!s_) throw PythonError();
+    (void)what;
+  }
+  Sequence(const Sequence &) = delete;
+  Sequence &operator=(const Sequence &) = delete;
+  ~Sequence() { Py_DECREF(s_); }
+  Py_ssize_t size() const { return PyTuple_GET_SIZE(s_); }
+  PyObject *operator[](Py_ssize_t i) const { return PyTuple_GET_ITEM(s_, i); }
+
+ private:
+  PyObject *s_;
+};
+
+PyObject *muon_update(Args a) {  // parameters momenta gradients lr momentum weight_decay nesterov update_scale steps coefficients eps workspace stream
+  const Sequence p(a[0], "parameters"), m(a[1], "momenta"), g(a[2], "gradients");
+  if (m.size() != p.size() || g.size() != p.size()) refuse("parameters", "as many parameters, momenta and gradients are expected");
+  if (p.size() == 0) Py_RETURN_NONE;
+  const OnDevice on(p[0], "parameters");
+  const at::Tensor &first = tensor(p[0]);
+  if (first.dim() != 2) refuse("parameters", "expected matrices");
+  const int64_t rows = first.size(0), cols = first.size(1);
+  std::vector<df_muon_tensor_t> table;
+  for (Py_ssize_t i = 0; i < p.size(); ++i) {
+    on.same(p[i], "parameters");
+    on.same(m[i], "momenta");
+    on.same(g[i], "gradients");
+    table.push_back({floats(p[i], {rows, cols}, "parameters"), floats(m[i], {rows, cols}, "momenta"), floats(g[i], {rows, cols}, "gradients")});
+  }
+  const Polynomial q = polynomial(a[9]);
+  const uint32_t n = below_2_31(p.size(), "parameters"), r = below_2_31(rows, "parameters"), c = below_2_31(cols, "parameters");
+  Out ws;
+  uint64_t size = 0;
+  void *work = on.workspace(ws, a[11], a[12], fn.df_orthogonalize_workspace_bytes(n, r, c), &size);
+  call(fn.df_muon_update, a[12], static_cast<const void *>(table.data()), n, r, c, real(a[3]), real(a[4]), real(a[5]), truth(a[6]), real(a[7]), u32(a[8]), q.a, q.b,
+       q.c, real(a[10]), work, size);
+  Py_RETURN_NONE;
+}
+
 // ---------------------------------------------------------------- LayerNorm, GELU, AdamW
 PyObject *layernorm(Args a) {  // x gamma beta out means rstds stream
   const Shape2 x = shape2(a[0]);
@@ -665,7 +850,8 @@ PyMethodDef methods[] = {
     ENTRY(merge_partials, 6), ENTRY(accumulate, 3), ENTRY(linear_qkv, 11), ENTRY(linear, 6), ENTRY(linear_gelu, 7), ENTRY(chunked_logit_ce, 6),
     ENTRY(layernorm, 7), ENTRY(layernorm_backward, 9), ENTRY(gelu, 3), ENTRY(gelu_backward, 4), ENTRY(adamw_update, 12), ENTRY(adamw_step, 11),
     ENTRY(cache_plan, 13), ENTRY(cache_release, 9), ENTRY(cache_append, 8), ENTRY(cache_attention, 14), ENTRY(token_logprobs, 10),
-    ENTRY(token_logprobs_backward, 9),
+    ENTRY(token_logprobs_backward, 9), ENTRY(linear_cross_entropy, 8), ENTRY(linear_cross_entropy_backward, 12), ENTRY(orthogonalize, 7),
+    ENTRY(muon_update, 13),
     ENTRY(context_forward, 9), ENTRY(context_backward, 13), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "df_python_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

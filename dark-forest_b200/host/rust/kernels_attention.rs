@@ -217,6 +217,32 @@ extern "C" {
         grad_entropy: *const f32, d_logits: *mut c_void, rows: u32, cols: u32, row_stride: u64, d_row_stride:
         u64, scale: f32, logits_bf16: u32, stream: *mut c_void
     ) -> i32;
+    pub fn df_linear_cross_entropy_workspace_bytes(
+        rows: u32, vocab: u32, width: u32, bf16: u32, backward: u32
+    ) -> u64;
+    pub fn df_linear_cross_entropy(
+        x: *const c_void, weight: *const c_void, targets: *const i32, loss: *mut f32, lse: *mut f32, workspace: *mut
+        c_void, workspace_bytes: u64, rows: u32, vocab: u32, width: u32, x_stride: u64, weight_stride: u64, scale:
+        f32, bf16: u32, stream: *mut c_void
+    ) -> i32;
+    pub fn df_linear_cross_entropy_backward(
+        x: *const c_void, weight: *const c_void, targets: *const i32, lse: *const f32, grad_loss: *const f32, d_x:
+        *mut c_void, d_weight: *mut c_void, workspace: *mut c_void, workspace_bytes: u64, rows: u32, vocab: u32,
+        width: u32, x_stride: u64, weight_stride: u64, dx_stride: u64, dw_stride: u64, scale: f32, bf16: u32,
+        stream: *mut c_void
+    ) -> i32;
+    pub fn df_orthogonalize_workspace_bytes(n: u32, rows: u32, cols: u32) -> u64;
+    pub fn df_orthogonalize(
+        update: *const c_void, out: *mut c_void, workspace: *mut c_void, workspace_bytes: u64, n: u32, rows: u32,
+        cols: u32, update_matrix_stride: u64, update_row_stride: u64, out_matrix_stride: u64, out_row_stride: u64,
+        steps: u32, a: f32, b: f32, c: f32, eps: f32, bf16: u32, stream: *mut c_void
+    ) -> i32;
+    /// `tensors_host`: `n` entries of three device pointers (parameter, momentum, gradient), read before the call returns.
+    pub fn df_muon_update(
+        tensors_host: *const c_void, n: u32, rows: u32, cols: u32, lr: f32, beta: f32, weight_decay: f32, nesterov:
+        u32, update_scale: f32, steps: u32, a: f32, b: f32, c: f32, eps: f32, workspace: *mut c_void,
+        workspace_bytes: u64, stream: *mut c_void
+    ) -> i32;
     pub fn launch_layernorm(
         x: *const f32, gamma: *const f32, beta: *const f32, out: *mut f32, means: *mut f32, rstds: *mut f32, batch: u32,
         features: u32

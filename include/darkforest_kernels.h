@@ -461,6 +461,50 @@ DF_API int df_token_logprobs_backward(const void *logits, const int32_t *targets
                                const float *grad_logp, const float *grad_entropy, void *d_logits, uint32_t rows, uint32_t cols,
                                uint64_t row_stride, uint64_t d_row_stride, float scale, uint32_t logits_bf16, void *stream);
 
+/* ---- softmax cross entropy from hidden states and the output weight, without keeping the logits (no counterpart in the reference, whose loss head
+ * above takes logits) ----
+ * x [rows] of `width` elements, weight [vocab] of `width` (both fp32, or both bf16 with bf16 != 0; row strides in elements), z = scale * x weight^T (scale > 0).
+ *   df_linear_cross_entropy            lse = log sum exp z, loss = lse - z[target], both [rows] fp32. The caller sums or averages.
+ *   df_linear_cross_entropy_backward   with G = exp(z - lse) - onehot(target): d_x = scale * grad_loss * G weight and d_weight = scale * (grad_loss * G)^T x,
+ *       overwritten, in the inputs' type; lse as above, grad_loss [rows]; d_x or d_weight may be NULL (not wanted). Neither may overlap x, weight or the other.
+ * A row whose target is outside 0 .. vocab - 1 is left out: loss 0, lse 0, no part of any gradient, whatever x holds there (NaN included). Infinities and NaN
+ * elsewhere make the results that they enter NaN. rows = 0: nothing, or d_weight = 0.
+ * Precision: products of bf16 are exact, G enters them in 11 bits; fp32 operands enter in 22 bits relative to their row's largest element (x), or the weight's
+ * and grad_loss * x's largest (elements 2^18 below that in fewer), G in 22. Sums in fp32; results rounded once. Nothing depends on the order of execution.
+ * The logits' gradient exists piece by piece of the vocabulary in the workspace (up to 128 MB at a time, at least 256 columns).
+ * workspace: df_linear_cross_entropy_workspace_bytes, 256-byte aligned, contents undefined before and after. Calls that can overlap need one each. */
+DF_API uint64_t df_linear_cross_entropy_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t width, uint32_t bf16, uint32_t backward);
+DF_API int df_linear_cross_entropy(const void *x, const void *weight, const int32_t *targets, float *loss, float *lse, void *workspace,
+                            uint64_t workspace_bytes, uint32_t rows, uint32_t vocab, uint32_t width, uint64_t x_stride, uint64_t weight_stride,
+                            float scale, uint32_t bf16, void *stream);
+DF_API int df_linear_cross_entropy_backward(const void *x, const void *weight, const int32_t *targets, const float *lse, const float *grad_loss, void *d_x,
+                                     void *d_weight, void *workspace, uint64_t workspace_bytes, uint32_t rows, uint32_t vocab, uint32_t width,
+                                     uint64_t x_stride, uint64_t weight_stride, uint64_t dx_stride, uint64_t dw_stride, float scale, uint32_t bf16,
+                                     void *stream);
+
+/* ---- orthogonalised updates of matrices, next to AdamW (no counterpart in the reference) ----
+ * O(U): X = U / (|U|_F + eps); `steps` (1 .. 64) times X <- a X + (b X X^T + c (X X^T)^2) X. rows, cols up to 65536, rows * cols below 2^31, any of the two larger.
+ *   df_orthogonalize   n matrices [rows][cols] (fp32, or bf16 with bf16 != 0; strides in elements): out = O(update). out may be the update itself.
+ *   df_muon_update     n tensors [rows][cols] fp32, contiguous, described by df_muon_tensor_t entries in HOST memory, read before the call returns (up to 1024):
+ *       momentum <- beta momentum + gradient; U = gradient + beta momentum (nesterov != 0) or momentum;
+ *       parameter <- parameter (1 - lr weight_decay) - lr update_scale O(U). No tensor may overlap another.
+ * Precision: factors in 22 bits relative to 1 (elements below 2^-26 in fewer, none below 2^-37), sums in fp32, the norm in double, results rounded once.
+ * |a| + |b| + |c| below 15 (else DF_ERR_UNSUPPORTED); singular values that a step brings above 3.8 make the matrix's results infinite or NaN. A zero matrix gives 0
+ * (eps > 0), an infinity or NaN NaN, both without touching the other matrices. Nothing depends on the order of execution.
+ * workspace: df_orthogonalize_workspace_bytes (for both calls; at most 512 MB or one matrix), 256-byte aligned, contents undefined before and after. Calls that can overlap need one each. */
+typedef struct df_muon_tensor {
+  float *parameter;
+  float *momentum;
+  const float *gradient;
+} df_muon_tensor_t;
+DF_API uint64_t df_orthogonalize_workspace_bytes(uint32_t n, uint32_t rows, uint32_t cols);
+DF_API int df_orthogonalize(const void *update, void *out, void *workspace, uint64_t workspace_bytes, uint32_t n, uint32_t rows, uint32_t cols,
+                     uint64_t update_matrix_stride, uint64_t update_row_stride, uint64_t out_matrix_stride, uint64_t out_row_stride, uint32_t steps,
+                     float a, float b, float c, float eps, uint32_t bf16, void *stream);
+DF_API int df_muon_update(const void *tensors_host, uint32_t n, uint32_t rows, uint32_t cols, float lr, float beta, float weight_decay,
+                   uint32_t nesterov, float update_scale, uint32_t steps, float a, float b, float c, float eps, void *workspace,
+                   uint64_t workspace_bytes, void *stream);
+
 /* ---- variant selection and status ---- */
 #define DF_VARIANT_AUTO 0     /* tensor-core kernel where the shape allows (TF32 at d_head 64, full fp32 by bf16 parts at others), SIMT otherwise */
 #define DF_VARIANT_SIMT 1     /* force the shape-generic SIMT kernels                      */
