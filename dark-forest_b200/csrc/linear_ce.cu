@@ -19,8 +19,7 @@ namespace {
 using namespace ptx;
 
 constexpr float kGScale = 16384.0f;  // G is stored times 2^14
-constexpr uint64_t kPieceBytes = 128ull << 20;  // of G, or of a piece's weight in parts
-constexpr int kChunkBlocks = 1;                 // of 64: between takings out of an fp32 call's sums (measured: see k_product's users)
+constexpr uint64_t kPieceBytes = 256ull << 20;  // of G, or of a piece's weight in parts
 
 int finish(int st) {
   note_status(st);
@@ -503,8 +502,21 @@ struct Layout {
 };
 
 constexpr int kMaxSplits = 16;
+constexpr uint64_t kPairs = 74;  // of SMs
 
 bool in_place(const void *p, uint64_t stride) { return ((reinterpret_cast<uintptr_t>(p) | (stride * 2)) & 15u) == 0; }
+
+// Time of a backward piece of t tiles of 256 columns in units of 64 of a contraction on every pair of SMs (about 512 cycles and part), with `splits` slices of d_x:
+// waves of tiles times their blocks, for the three products, and what a piece costs besides (four launches, w cut into parts).
+struct Tiles {
+  uint64_t m, k;              // tiles of 256 rows and of 256 of the width
+  uint64_t rows64, width64;   // blocks of 64
+  double besides;
+  double piece(uint64_t t, uint64_t splits) const {
+    auto waves = [](uint64_t n) { return (n + kPairs - 1) / kPairs; };
+    return (double)(waves(m * t) * (width64 + 3) + waves(t * k) * (rows64 + 3) + waves(m * k * splits) * ((4 * t + splits - 1) / splits + 3)) + besides;
+  }
+};
 
 Layout layout(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool backward) {
   Layout l = {};
@@ -513,12 +525,35 @@ Layout layout(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool bac
   l.rows_pad = (uint32_t)up(rows, 32);
   uint64_t per_col = (uint64_t)l.pitch * 2 * parts;
   if (backward && (uint64_t)rows * 2 * parts > per_col) per_col = (uint64_t)rows * 2 * parts;
-  uint64_t most = kPieceBytes / per_col / 256 * 256;
-  if (most < 256) most = 256;
-  l.n_pieces = (uint32_t)((vocab + most - 1) / most);
-  if (bf16 && !backward) l.n_pieces = 1;  // nothing is kept per column but what joins the rows
-  l.piece = (uint32_t)up((vocab + l.n_pieces - 1) / l.n_pieces, 256);
-  l.n_pieces = (vocab + l.piece - 1) / l.piece;
+  const uint64_t all = (vocab + 255) / 256;  // tiles of the vocabulary
+  uint64_t most = kPieceBytes / per_col / 256, piece = all;
+  if (most < 1) most = 1;
+  if (!backward && !bf16) {
+    const uint64_t n = (all + most - 1) / most;
+    piece = (all + n - 1) / n;
+  }
+  l.splits = 1;
+  if (backward) {
+    const Tiles c = {((uint64_t)rows + 255) / 256, ((uint64_t)width + 255) / 256, ((uint64_t)rows + 63) / 64, ((uint64_t)width + 63) / 64, bf16 ? 24.0 : 12.0};
+    if (most > all) most = all;
+    double best = 1e300;
+    const uint64_t least = most > 3 ? most / 3 : 1, step = (most - least) / 48 + 1;
+    for (uint64_t t = least; t <= most; t += step) {
+      const uint64_t tail = all % t;
+      // as many slices as there are pairs for, and the fewer the better: each is a plane of sums
+      uint64_t few = 1;
+      for (uint64_t k = 2; k <= (uint64_t)kMaxSplits && k <= 4 * t; ++k)
+        if (c.piece(t, k) < 0.97 * c.piece(t, few)) few = k;
+      const double cost = (double)(all / t) * c.piece(t, few) + (tail ? c.piece(tail, few) : 0.0);
+      if (cost < best) {
+        best = cost;
+        piece = t;
+        l.splits = (int)few;
+      }
+    }
+  }
+  l.piece = (uint32_t)piece * 256;
+  l.n_pieces = (uint32_t)((all + piece - 1) / piece);
   uint64_t at = 256;
   auto take = [&](uint64_t bytes) {
     const uint64_t here = at;
@@ -536,12 +571,6 @@ Layout layout(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool bac
     l.x_grad = take((uint64_t)rows * l.pitch * 2 * parts);
     if (bf16) l.w_raw = take((uint64_t)l.piece * l.pitch * 2);
     l.g = take((uint64_t)rows * l.piece * 2 * parts);
-    // d_x has (rows / 256) (width / 256) tiles for some 74 pairs of SMs: its contraction is split until they are busy
-    const uint64_t tiles = ((rows + 255) / 256) * ((width + 255) / 256), blocks = l.piece / 64;
-    uint64_t n = (74 + tiles - 1) / tiles;
-    if (n > (uint64_t)kMaxSplits) n = kMaxSplits;
-    if (n > blocks) n = blocks;
-    l.splits = (int)(n < 1 ? 1 : n);
     l.planes = take((uint64_t)l.splits * rows * l.pitch * 4);
   }
   l.total = at;
@@ -563,13 +592,11 @@ int product(const Operand &a, const Operand &b, uint32_t M, uint32_t N, uint32_t
   ProductParams p = {};
   p.M = M;
   p.N = N;
-  p.batch = 1;
   p.n_kb = (int)((K + kProdK - 1) / kProdK);
   p.splits = slices(p.n_kb, splits);
   p.kb_per_split = (p.n_kb + splits - 1) / splits;
-  p.chunk = kChunkBlocks;
   p.fmt = bf16 ? (uint32_t)kFmtBF16 : (uint32_t)kFmtF16;
-  return launch_product<ProdCfg<true, A_MN, B_MN, PARTS>, Epi>(a, b, p, e, s);
+  return launch_product<ProdCfg<A_MN, B_MN, PARTS>, Epi>(a, b, p, e, s);
 }
 
 struct HeadCall {
@@ -608,7 +635,7 @@ struct HeadCall {
     return st;
   }
   Operand packed(uint64_t at, uint32_t n, bool is_bf16) const {
-    return {at16(at), at16(at) + (size_t)n * l.pitch, is_bf16, n, width, l.pitch, 0};
+    return {at16(at), at16(at) + (size_t)n * l.pitch, is_bf16, n, width, l.pitch};
   }
   int ranges(const float *grad, bool of_x) const {
     RangeParams p = {w, x, grad, targets, reinterpret_cast<Words *>(ws), w_stride, x_stride, vocab, rows, width, 0, bf16};
@@ -624,7 +651,7 @@ struct HeadCall {
   // operands of the logits: bf16 in place where a copy can start there, else copied; fp32 in parts (x once, w piece by piece)
   int logits_x(Operand *o) const {
     if (bf16 && in_place(x, x_stride)) {
-      *o = {x, x, true, rows, width, x_stride, 0};
+      *o = {x, x, true, rows, width, x_stride};
       return DF_OK;
     }
     *o = packed(l.x_parts, rows, bf16);
@@ -640,7 +667,7 @@ struct HeadCall {
     uint32_t slots = 0;
     for (uint32_t c0 = 0; st == DF_OK && c0 < vocab; c0 += l.piece) {
       const uint32_t n = vocab - c0 < l.piece ? vocab - c0 : l.piece;
-      Operand b = {row_of_w(c0), nullptr, true, n, width, w_stride, 0};
+      Operand b = {row_of_w(c0), nullptr, true, n, width, w_stride};
       if (!(bf16 && in_place(w, w_stride))) {
         st = pack(row_of_w(c0), w_stride, n, l.w_parts, bf16, &words->largest_w, nullptr, nullptr, nullptr);
         b = packed(l.w_parts, n, bf16);
@@ -685,7 +712,7 @@ struct HeadCall {
       const Operand wp = packed(l.w_parts, n, false);
       Operand b = wp;
       if (bf16) {
-        b = {row_of_w(c0), nullptr, true, n, width, w_stride, 0};
+        b = {row_of_w(c0), nullptr, true, n, width, w_stride};
         if (!in_place(w, w_stride)) {
           if (st == DF_OK) st = pack(row_of_w(c0), w_stride, n, l.w_raw, true, nullptr, nullptr, nullptr, nullptr);
           b = packed(l.w_raw, n, true);
@@ -705,7 +732,7 @@ struct HeadCall {
       e.col_base = c0;
       e.all_cols = vocab;
       if (st == DF_OK) st = product<false, false, PARTS, GradEpi<PARTS>>(a, b, rows, n, width, 1, bf16, e, s);
-      const Operand g = {e.g, e.g_lo, false, rows, n, l.piece, 0};
+      const Operand g = {e.g, e.g_lo, false, rows, n, l.piece};
       if (st == DF_OK && d_x) {
         if (c0 == 0) splits = slices((n + kProdK - 1) / kProdK, splits);
         OutEpi::Params o = {};

@@ -4,7 +4,11 @@
 // tiny near 1. G and B are symmetric: only tiles on and right of the diagonal are computed, and written twice.
 // A singular value far below the largest grows by a factor of up to a^steps (485), and so does whatever a rounding put beside it: all
 // factors are held in two fp16 parts (22 bits; product_sm100.cuh) times 2^12, which suits values up to 15, and sums leave the tensor cores every
-// 768 of the contraction. a is on the diagonal of B, so that X's new value is one product.
+// 64 of the contraction. a is on the diagonal of B, so that X's new value is one product.
+//
+// All products of all steps are one cooperative launch. Its tiles are numbered step by step, product by product, matrix by matrix, and dealt out
+// to the CTAs in turn; a tile waits until the tiles of the product before it, of the same matrix, are written (a counter per matrix). What it waits for has
+// a lower number, and every CTA takes its tiles in their order, so the lowest unfinished tile never waits.
 #include <math.h>
 
 #include "product_sm100.cuh"
@@ -18,7 +22,6 @@ constexpr float kPartScale = 4096.0f, kPartInverse = 1.0f / 4096.0f;
 constexpr int kMostMatrices = 64;               // of a group: what the kernels' tables of pointers hold
 constexpr uint64_t kGroupBytes = 512ull << 20;  // of workspace, beyond one matrix
 constexpr int kNormBlocks = 64;                 // partial sums of squares per matrix
-constexpr int kChunk = 1;
 constexpr uint32_t kMostTensors = 1024;         // of an optimiser step: every pair is checked for overlap
 
 int finish(int st) {
@@ -43,6 +46,7 @@ struct Targets {
 struct UpdateParams {
   Table t;
   double *sums;  // [matrices][kNormBlocks]
+  uint32_t *done;  // [matrices]: set to 0 here
   uint16_t *hi, *lo;
   uint64_t row_stride, matrix;  // of the source; elements of a matrix in parts
   uint32_t rows, cols, pitch, bf16, nesterov;
@@ -77,6 +81,7 @@ __global__ void __launch_bounds__(256) k_update(const __grid_constant__ UpdatePa
     __syncthreads();
   }
   if (threadIdx.x == 0) p.sums[m * kNormBlocks + blockIdx.x] = part[0];
+  if (threadIdx.x == 0 && blockIdx.x == 0) p.done[m] = 0;
 }
 
 // X in parts
@@ -107,7 +112,78 @@ __global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ Updat
   }
 }
 
-// ---------------------------------------------------------------- epilogues
+// ---------------------------------------------------------------- the products
+template <bool PAIR_>
+struct NsCfg {
+  static constexpr bool PAIR = PAIR_;
+  static constexpr int kCtas = PAIR ? 2 : 1, T = PAIR ? 256 : 128;  // tiles of T x T
+  static constexpr uint32_t kTileBytes = 128 * kProdK * 2, kStageBytes = 4 * kTileBytes;  // A hi, B hi, A lo, B lo
+  static constexpr int kStages = 3;
+  static constexpr uint32_t kSmemStaging = kStages * kStageBytes;
+  static constexpr uint32_t kSmemBars = kSmemStaging + kProdEpiWarps * kProdSlabBytes;
+  static constexpr uint32_t kSmemTotal = kSmemBars + 256 + 1024;
+  static constexpr uint32_t kTmemCols = 2 * T;
+  static constexpr int FULL = 0, EMPTY = FULL + kStages, ACC_FULL = EMPTY + kStages, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2, NUM_BARS = DRAIN + 1;
+  static_assert(NUM_BARS * 8 <= 192 && kSmemTotal <= 227 * 1024, "shared memory");
+};
+
+struct NsParams {
+  // [buffer][hi, lo]: X with k along its rows or its columns, G, B
+  CUtensorMap x_k[2][2], x_mn[2][2], g[2], b[2];
+  uint32_t *done;             // [matrices]: epilogue warps that are through with their tile
+  uint16_t *x[2][2], *gp[2], *bp[2];
+  uint64_t x_matrix, g_matrix;
+  uint32_t rows, cols, side, x_pitch, g_pitch;
+  int wide, n, steps;
+  int side_tiles, x_m_tiles, x_n_tiles, g_units, x_units;  // tiles: along the side, of X; of a symmetric product, of X's
+  float a, b_, c;             // of B, times the parts' scales
+  Targets t;
+  uint64_t out_stride;
+  uint32_t out_bf16, vec, apply;
+  float keep, step;
+  unsigned int *status;
+};
+
+enum Product { kGram, kPolynomial, kNext };
+struct Unit {
+  int step, batch, m, n, blocks;
+  Product product;
+  uint32_t after;  // tiles of this matrix that have to be written before
+};
+__device__ __forceinline__ Unit unit_of(const NsParams &p, int u) {
+  Unit w;
+  const int per_step = p.n * (2 * p.g_units + p.x_units);
+  w.step = u / per_step;
+  int r = u % per_step;
+  w.after = (uint32_t)w.step * (uint32_t)(2 * p.g_units + p.x_units);
+  const int g_all = p.n * p.g_units;
+  w.product = r < g_all ? kGram : (r < 2 * g_all ? kPolynomial : kNext);
+  if (w.product == kNext) {
+    r -= 2 * g_all;
+    w.after += 2 * p.g_units;
+    w.batch = r / p.x_units;
+    r %= p.x_units;
+    w.m = r / p.x_n_tiles;
+    w.n = r % p.x_n_tiles;
+    w.blocks = (int)(p.side + kProdK - 1) / kProdK;
+    return w;
+  }
+  if (w.product == kPolynomial) {
+    r -= g_all;
+    w.after += p.g_units;
+  }
+  w.batch = r / p.g_units;
+  r %= p.g_units;
+  w.m = 0;
+  while (r >= p.side_tiles - w.m) {  // the tiles with n >= m, row after row
+    r -= p.side_tiles - w.m;
+    ++w.m;
+  }
+  w.n = w.m + r;
+  w.blocks = (int)((w.product == kPolynomial ? p.side : (p.wide ? p.cols : p.rows)) + kProdK - 1) / kProdK;
+  return w;
+}
+
 // A row's 32 columns of two parts, 64 bytes each
 __device__ __forceinline__ void write_parts(uint16_t *hi, uint16_t *lo, size_t at, const float (&v)[32]) {
 #pragma unroll
@@ -121,165 +197,341 @@ __device__ __forceinline__ void write_parts(uint16_t *hi, uint16_t *lo, size_t a
     *reinterpret_cast<uint4 *>(lo + at + x) = l;
   }
 }
-__device__ __forceinline__ float one_part(const uint16_t *hi, const uint16_t *lo, size_t i) {
-  return __half2float(*reinterpret_cast<const __half *>(hi + i)) + __half2float(*reinterpret_cast<const __half *>(lo + i));
-}
 
 // G = X X^T, or B = a I + b G + c G G: symmetric, in parts, each tile in its place and in the mirrored one
-struct SymmetricEpi {
-  struct Params {
-    uint16_t *hi, *lo;              // [matrices][side][pitch]
-    const uint16_t *g_hi, *g_lo;    // null: G itself
-    uint64_t matrix;
-    uint32_t side, pitch;
-    float a, b, c;                  // of B, times the parts' scales
-  };
-  const Params &p;
-  uint32_t row, col0;
-  size_t base;
-  bool mirror;
-  __device__ __forceinline__ SymmetricEpi(const Params &q, uint8_t *, int) : p(q) {}
-  __device__ __forceinline__ void begin(const ProductTile &t, uint32_t r, uint32_t c0) {
-    row = r;
-    col0 = c0;
-    base = (size_t)t.batch * p.matrix;
-    mirror = t.m_tile != t.n_tile;
-  }
-  __device__ __forceinline__ void block(int cg, float (&v)[32]) {
-    const uint32_t first = col0 + cg * 32;
-    if (first >= p.side || row >= p.side) return;  // the pitch is a multiple of 64: a block that begins inside may be written whole
-    const size_t at = base + (size_t)row * p.pitch + first;
-    if (p.g_hi) {
+__device__ __forceinline__ void symmetric_block(const NsParams &p, const Unit &w, uint32_t row, uint32_t first, float (&v)[32]) {
+  if (first >= p.side || row >= p.side) return;  // the pitch is a multiple of 64: a block that begins inside may be written whole
+  const size_t base = (size_t)w.batch * p.g_matrix, at = base + (size_t)row * p.g_pitch + first;
+  uint16_t *hi, *lo;
+  if (w.product == kPolynomial) {
+    hi = p.bp[0];
+    lo = p.bp[1];
 #pragma unroll
-      for (int x = 0; x < 32; x += 8) {
-        const uint4 h = *reinterpret_cast<const uint4 *>(p.g_hi + at + x), l = *reinterpret_cast<const uint4 *>(p.g_lo + at + x);
-        const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
+    for (int x = 0; x < 32; x += 8) {  // written by other SMs of this launch: not through L1
+      const uint4 h = __ldcg(reinterpret_cast<const uint4 *>(p.gp[0] + at + x)), l = __ldcg(reinterpret_cast<const uint4 *>(p.gp[1] + at + x));
+      const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const float2 u = __half22float2(*reinterpret_cast<const __half2 *>(&hh[y])), w = __half22float2(*reinterpret_cast<const __half2 *>(&ll[y]));
-          v[x + 2 * y] = fmaf(p.c, v[x + 2 * y], p.b * (u.x + w.x));
-          v[x + 2 * y + 1] = fmaf(p.c, v[x + 2 * y + 1], p.b * (u.y + w.y));
-        }
+      for (int y = 0; y < 4; ++y) {
+        const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&hh[y])), r = __half22float2(*reinterpret_cast<const __half2 *>(&ll[y]));
+        v[x + 2 * y] = fmaf(p.c, v[x + 2 * y], p.b_ * (q.x + r.x));
+        v[x + 2 * y + 1] = fmaf(p.c, v[x + 2 * y + 1], p.b_ * (q.y + r.y));
       }
-#pragma unroll
-      for (int x = 0; x < 32; ++x) v[x] += first + x == row ? p.a : 0.0f;
-    } else {
-#pragma unroll
-      for (int x = 0; x < 32; ++x) v[x] *= p.c;
     }
-    write_parts(p.hi, p.lo, at, v);
-    if (!mirror) return;
-    // the mirrored tile: a column's 32 rows lie together across the warp's lanes
 #pragma unroll
-    for (int x = 0; x < 32; ++x) {
-      if (first + x >= p.side) break;
-      const size_t to = base + (size_t)(first + x) * p.pitch + row;
-      const __half h = __float2half_rn(v[x]);
-      *reinterpret_cast<__half *>(p.hi + to) = h;
-      *reinterpret_cast<__half *>(p.lo + to) = __float2half_rn(v[x] - __half2float(h));
-    }
-  }
-  __device__ __forceinline__ void end() {}
-};
-
-// X of the next step, in parts
-struct NextEpi {
-  struct Params {
-    uint16_t *hi, *lo;
-    uint64_t matrix;
-    uint32_t rows, cols, pitch;
-    float scale;
-  };
-  const Params &p;
-  uint32_t row, col0;
-  size_t base;
-  __device__ __forceinline__ NextEpi(const Params &q, uint8_t *, int) : p(q) {}
-  __device__ __forceinline__ void begin(const ProductTile &t, uint32_t r, uint32_t c0) {
-    row = r;
-    col0 = c0;
-    base = (size_t)t.batch * p.matrix;
-  }
-  __device__ __forceinline__ void block(int cg, float (&v)[32]) {
-    const uint32_t first = col0 + cg * 32;
-    if (first >= p.cols || row >= p.rows) return;
+    for (int x = 0; x < 32; ++x) v[x] += first + x == row ? p.a : 0.0f;
+  } else {
+    hi = p.gp[0];
+    lo = p.gp[1];
 #pragma unroll
-    for (int x = 0; x < 32; ++x) v[x] *= p.scale;
-    write_parts(p.hi, p.lo, base + (size_t)row * p.pitch + first, v);
+    for (int x = 0; x < 32; ++x) v[x] *= kPartInverse;
   }
-  __device__ __forceinline__ void end() {}
-};
+  write_parts(hi, lo, at, v);
+  if (w.m == w.n) return;
+  // the mirrored tile: a column's 32 rows lie together across the warp's lanes
+#pragma unroll
+  for (int x = 0; x < 32; ++x) {
+    if (first + x >= p.side) break;
+    const size_t to = base + (size_t)(first + x) * p.g_pitch + row;
+    const __half h = __float2half_rn(v[x]);
+    *reinterpret_cast<__half *>(hi + to) = h;
+    *reinterpret_cast<__half *>(lo + to) = __float2half_rn(v[x] - __half2float(h));
+  }
+}
 
 // X of the last step: written in the caller's type, or applied to the parameter: P <- keep P - step X
-struct LastEpi {
-  struct Params {
-    Targets t;
-    uint64_t row_stride;
-    uint32_t rows, cols, bf16, vec, apply;
-    float scale, keep, step;
-  };
-  const Params &p;
-  float4 *slab;
-  int lane;
-  uint32_t row0, col0;
-  void *out;
-  __device__ __forceinline__ LastEpi(const Params &q, uint8_t *sl, int l) : p(q), slab(reinterpret_cast<float4 *>(sl)), lane(l) {}
-  __device__ __forceinline__ void begin(const ProductTile &t, uint32_t r, uint32_t c0) {
-    row0 = r - lane;
-    col0 = c0;
-    out = p.t.out[t.batch];
-  }
-  __device__ __forceinline__ void block(int cg, float (&v)[32]) {
-    const uint32_t first = col0 + cg * 32;
-    if (first >= p.cols) return;
-    float4 q[8];
-    turn_over(slab, lane, v, q);
-    const uint32_t col = first + 4 * (lane & 7);
-    if (col >= p.cols) return;
+__device__ __forceinline__ void last_block(const NsParams &p, const Unit &w, float4 *slab, int lane, uint32_t row0, uint32_t first, const float (&v)[32]) {
+  if (first >= p.cols) return;
+  float4 q[8];
+  turn_over(slab, lane, v, q);
+  const uint32_t col = first + 4 * (lane & 7);
+  if (col >= p.cols) return;
+  void *out = p.t.out[w.batch];
+  constexpr float scale = kPartInverse * kPartInverse;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t r = row0 + 4 * i + (lane >> 3);
-      if (r >= p.rows) continue;
-      float w[4] = {q[i].x * p.scale, q[i].y * p.scale, q[i].z * p.scale, q[i].w * p.scale};
-      const size_t at = (size_t)r * p.row_stride + col;
-      if (p.vec && col + 4 <= p.cols) {
-        if (p.bf16) {
-          uint2 b;
-          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.x) : "f"(w[1]), "f"(w[0]));
-          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.y) : "f"(w[3]), "f"(w[2]));
-          *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + at) = b;
-        } else {
-          float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(out) + at);
-          if (p.apply) {
-            const float4 old = *to;
-            w[0] = fmaf(p.keep, old.x, -p.step * w[0]);
-            w[1] = fmaf(p.keep, old.y, -p.step * w[1]);
-            w[2] = fmaf(p.keep, old.z, -p.step * w[2]);
-            w[3] = fmaf(p.keep, old.w, -p.step * w[3]);
-          }
-          *to = make_float4(w[0], w[1], w[2], w[3]);
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t r = row0 + 4 * i + (lane >> 3);
+    if (r >= p.rows) continue;
+    float y[4] = {q[i].x * scale, q[i].y * scale, q[i].z * scale, q[i].w * scale};
+    const size_t at = (size_t)r * p.out_stride + col;
+    if (p.vec && col + 4 <= p.cols) {
+      if (p.out_bf16) {
+        uint2 b;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.x) : "f"(y[1]), "f"(y[0]));
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.y) : "f"(y[3]), "f"(y[2]));
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + at) = b;
+      } else {
+        float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(out) + at);
+        if (p.apply) {
+          const float4 old = *to;
+          y[0] = fmaf(p.keep, old.x, -p.step * y[0]);
+          y[1] = fmaf(p.keep, old.y, -p.step * y[1]);
+          y[2] = fmaf(p.keep, old.z, -p.step * y[2]);
+          y[3] = fmaf(p.keep, old.w, -p.step * y[3]);
         }
-        continue;
+        *to = make_float4(y[0], y[1], y[2], y[3]);
       }
+      continue;
+    }
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        if (col + x >= p.cols) break;
-        if (p.bf16) {
-          uint32_t b;
-          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(0.0f), "f"(w[x]));
-          static_cast<uint16_t *>(out)[at + x] = (uint16_t)b;
-        } else {
-          float *to = static_cast<float *>(out) + at + x;
-          *to = p.apply ? fmaf(p.keep, *to, -p.step * w[x]) : w[x];
-        }
+    for (int x = 0; x < 4; ++x) {
+      if (col + x >= p.cols) break;
+      if (p.out_bf16) {
+        uint32_t b;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(0.0f), "f"(y[x]));
+        static_cast<uint16_t *>(out)[at + x] = (uint16_t)b;
+      } else {
+        float *to = static_cast<float *>(out) + at + x;
+        *to = p.apply ? fmaf(p.keep, *to, -p.step * y[x]) : y[x];
       }
     }
   }
-  __device__ __forceinline__ void end() {}
-};
+}
+
+__device__ __forceinline__ uint32_t load_acquire(const uint32_t *p) {
+  uint32_t v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+// Writes by ordinary stores become visible to the copy engines of other SMs: a fence between the two ways to memory at both ends.
+__device__ __forceinline__ void fence_proxies() { asm volatile("fence.proxy.async;" ::: "memory"); }
+
+template <class C>
+__global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_constant__ NsParams p) {
+  constexpr int kStages = C::kStages, T = C::T;
+  constexpr bool PAIR = C::PAIR;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t a0 = smem_u32(smem);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kSmemBars);
+  volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + C::kSmemBars + 192);
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(smem + C::kSmemBars + 196);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  auto bar = [&](int id) { return smem_u32(&bars[id]); };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::NUM_BARS; ++i) mbar_init(bar(i), i == C::ACC_EMPTY || i == C::ACC_EMPTY + 1 ? C::kCtas * kProdEpiWarps : 1);
+    *abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 1) {
+    if (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_holder), C::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_holder), C::kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before_sync();
+  if (PAIR) cluster_sync();
+  else __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_holder;
+  pdl_wait();
+  const int first = blockIdx.x / C::kCtas, apart = gridDim.x / C::kCtas, units = p.steps * p.n * (2 * p.g_units + p.x_units);
+
+  if (warp < 4) {
+    prod_regs_less<kProdOtherRegs>();
+    if (warp == 0) {
+      // ---------------------------------------------------------- copies
+      if (lane == 0) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int u = first; ok && u < units; u += apart) {
+          const Unit w = unit_of(p, u);
+          const uint32_t need = w.after * (C::kCtas * kProdEpiWarps);
+          if (load_acquire(p.done + w.batch) < need) {
+            const uint64_t t0 = global_timer_ns();
+#pragma unroll 1
+            for (uint32_t polls = 1; load_acquire(p.done + w.batch) < need; ++polls) {
+              if ((polls & 63u) == 0u && (*abort_flag != 0u || polls >= kWaitMaxPolls || global_timer_ns() - t0 > kWaitBudgetNs)) { ok = false; break; }
+            }
+            if (!ok) {
+              *abort_flag = 1u;
+              break;
+            }
+          }
+          fence_proxies();
+          const int cur = w.step & 1;
+          const bool x_product = w.product == kNext;
+          // G: X X^T (k along rows) or X^T X (k along columns); B: G G; X: B X or X B
+          const bool mn_a = w.product == kGram && !p.wide, mn_b = mn_a || (x_product && p.wide);
+          const CUtensorMap *a, *b;
+          if (w.product == kGram) a = b = p.wide ? p.x_k[cur] : p.x_mn[cur];
+          else if (w.product == kPolynomial) a = b = p.g;
+          else if (p.wide) { a = p.b; b = p.x_mn[cur]; }
+          else { a = p.x_k[cur]; b = p.b; }
+          const int row_a = w.m * T + (int)rank * 128, row_b = w.n * T + (int)rank * 128;
+          for (int kb = 0; kb < w.blocks; ++kb, ++it) {
+            const uint32_t s = it % kStages, use = it / kStages;
+            if (use > 0 && !prod_wait(bar(C::EMPTY + s), (use - 1) & 1, abort_flag)) { ok = false; break; }
+            const uint32_t sa = a0 + s * C::kStageBytes, full = PAIR ? map_to_rank(bar(C::FULL + s), 0) : bar(C::FULL + s);
+            if (rank == 0) mbar_arrive_expect_tx(bar(C::FULL + s), C::kCtas * C::kStageBytes);
+            auto copy = [&](uint32_t dst, const CUtensorMap *m, int x, int y) {
+              if (PAIR) tma_load_3d_pair(dst, m, full, x, y, w.batch);
+              else tma_load_3d(dst, m, full, x, y, w.batch);
+            };
+            auto load = [&](uint32_t dst, const CUtensorMap *m, bool mn, int row) {
+              if (mn) {
+                copy(dst, m, row, kb * kProdK);
+                copy(dst + 8192, m, row + 64, kb * kProdK);
+              } else {
+                copy(dst, m, kb * kProdK, row);
+              }
+            };
+            load(sa + 2 * C::kTileBytes, a + 1, mn_a, row_a);
+            load(sa + C::kTileBytes, b, mn_b, row_b);
+            load(sa, a, mn_a, row_a);
+            load(sa + 3 * C::kTileBytes, b + 1, mn_b, row_b);
+          }
+        }
+      }
+    } else if (warp == 1 && rank == 0) {
+      // ---------------------------------------------------------- products
+      uint32_t it = 0;
+      bool ok = true;
+      for (int u = first; ok && u < units; u += apart) {
+        const Unit w = unit_of(p, u);
+        const bool mn_a = w.product == kGram && !p.wide, mn_b = mn_a || (w.product == kNext && p.wide);
+        const uint32_t idesc = make_idesc(kFmtF16, T, T, mn_a ? 1 : 0, mn_b ? 1 : 0);
+        const uint32_t lbo_a = mn_a ? 8192 : 16, lbo_b = mn_b ? 8192 : 16;
+        const uint64_t step_a = mn_a ? 2048 >> 4 : 32 >> 4, step_b = mn_b ? 2048 >> 4 : 32 >> 4;
+        auto issue = [&](uint32_t d, uint32_t sa, uint32_t sb, bool fresh) {
+          const uint64_t da = make_smem_desc(sa, lbo_a, 1024, kSwz128), db = make_smem_desc(sb, lbo_b, 1024, kSwz128);
+#pragma unroll
+          for (int k = 0; k < kProdK / 16; ++k) {
+            if (PAIR) mma_f16_ss_pair(d, da + k * step_a, db + k * step_b, idesc, fresh && k == 0 ? 0u : 1u);
+            else mma_f16_ss(d, da + k * step_a, db + k * step_b, idesc, fresh && k == 0 ? 0u : 1u);
+          }
+        };
+        for (int kb = 0; kb < w.blocks; ++kb, ++it) {
+          const uint32_t acc = it & 1, d = tmem + acc * T, s = it % kStages, sa = a0 + s * C::kStageBytes;
+          if (it >= 2 && !prod_wait_warp(bar(C::ACC_EMPTY + acc), ((it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+          if (!prod_wait_warp(bar(C::FULL + s), (it / kStages) & 1, abort_flag)) { ok = false; break; }
+          tc_fence_after_sync();
+          if (elect_one()) {
+            issue(d, sa + 2 * C::kTileBytes, sa + C::kTileBytes, true);
+            issue(d, sa, sa + 3 * C::kTileBytes, false);
+            issue(d, sa, sa + C::kTileBytes, false);
+            if (PAIR) {
+              mma_commit_pair(bar(C::EMPTY + s));
+              mma_commit_pair(bar(C::ACC_FULL + acc));
+            } else {
+              mma_commit(bar(C::EMPTY + s));
+              mma_commit(bar(C::ACC_FULL + acc));
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ sums and results
+    prod_regs_more<kProdEpiRegs>();
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    constexpr int kGroups = T / 64;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * (T / 2);
+    float4 *slab = reinterpret_cast<float4 *>(smem + C::kSmemStaging + (warp - 4) * kProdSlabBytes);
+    uint32_t j = 0;
+    bool ok = true;
+    for (int u = first; ok && u < units; u += apart) {
+      const Unit w = unit_of(p, u);
+      float sum[kGroups][32];
+#pragma unroll
+      for (int cg = 0; cg < kGroups; ++cg)
+#pragma unroll
+        for (int x = 0; x < 32; ++x) sum[cg][x] = 0.0f;
+#pragma unroll 1
+      for (int kb = 0; kb < w.blocks; ++kb, ++j) {
+        const uint32_t acc = j & 1;
+        if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j >> 1) & 1, abort_flag)) { ok = false; break; }
+        tc_fence_after_sync();
+#pragma unroll
+        for (int cg = 0; cg < kGroups; ++cg) {
+          uint32_t r[32];
+          tmem_ld32(lane_base + acc * T + cg * 32, r);
+          tmem_wait_ld();
+          if (cg == kGroups - 1) {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+              if (PAIR) mbar_arrive_cluster(map_to_rank(bar(C::ACC_EMPTY + acc), 0));
+              else mbar_arrive(bar(C::ACC_EMPTY + acc));
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < 32; x += 2) {
+            const float2 q = add2(make_float2(sum[cg][x], sum[cg][x + 1]), as_float2(r[x], r[x + 1]));
+            sum[cg][x] = q.x;
+            sum[cg][x + 1] = q.y;
+          }
+        }
+      }
+      if (!ok) break;
+      const uint32_t row0 = (uint32_t)(w.m * T + (int)rank * 128 + quarter * 32), row = row0 + lane, col0 = (uint32_t)(w.n * T + half * (T / 2));
+      if (w.product == kPolynomial) {  // what it reads of G: the copies have been waited for, these loads as well
+        (void)load_acquire(p.done + w.batch);
+        __syncwarp();
+      }
+      if (w.product != kNext) {
+#pragma unroll
+        for (int cg = 0; cg < kGroups; ++cg) symmetric_block(p, w, row, col0 + cg * 32, sum[cg]);
+      } else if (w.step + 1 < p.steps) {
+        const int next = (w.step + 1) & 1;
+#pragma unroll
+        for (int cg = 0; cg < kGroups; ++cg) {
+          const uint32_t c = col0 + cg * 32;
+          if (c >= p.cols || row >= p.rows) continue;
+#pragma unroll
+          for (int x = 0; x < 32; ++x) sum[cg][x] *= kPartInverse;
+          write_parts(p.x[next][0], p.x[next][1], (size_t)w.batch * p.x_matrix + (size_t)row * p.x_pitch + c, sum[cg]);
+        }
+      } else {
+#pragma unroll
+        for (int cg = 0; cg < kGroups; ++cg) last_block(p, w, slab, lane, row0, col0 + cg * 32, sum[cg]);
+      }
+      fence_proxies();
+      __syncwarp();
+      if (lane == 0) {
+        __threadfence();
+        asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(p.done + w.batch), "r"(1u) : "memory");
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown (all roles), as in linear_sm100.cu
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag != 0u) {
+    if (warp == 1 && rank == 0) {
+      if (elect_one()) {
+        if (PAIR) mma_commit_pair(bar(C::DRAIN));
+        else mma_commit(bar(C::DRAIN));
+      }
+      __syncwarp();
+      for (int n = 0; n < (1 << 16) && !mbar_try_wait(bar(C::DRAIN), 0); ++n) {
+      }
+    }
+    if (warp == 0 && lane == 0) {
+      const uint64_t t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 2000000ull) {
+      }
+    }
+    if (threadIdx.x == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
+    __syncthreads();
+  }
+  if (PAIR) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    if (PAIR) tmem_dealloc_pair(tmem, C::kTmemCols);
+    else tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
 
 // ---------------------------------------------------------------- host
 struct Layout {
-  uint64_t x, x_next, g, b, total;  // offsets: parts hi, then lo, of all matrices of a group
+  uint64_t done, x, x_next, g, b, total;  // offsets: parts hi, then lo, of all matrices of a group
   uint64_t x_matrix, g_matrix;      // elements of a matrix
   uint32_t x_pitch, g_pitch, side, group;
 };
@@ -295,7 +547,8 @@ Layout layout(uint32_t n, uint32_t rows, uint32_t cols) {
   if (group > (uint64_t)kMostMatrices) group = kMostMatrices;
   if (group < 1) group = 1;
   l.group = n < group ? n : (uint32_t)group;
-  uint64_t at = (uint64_t)kMostMatrices * kNormBlocks * 8;
+  l.done = (uint64_t)kMostMatrices * kNormBlocks * 8;
+  uint64_t at = l.done + kMostMatrices * 4;
   auto take = [&](uint64_t elements) {
     const uint64_t here = at;
     at += elements * l.group * 4;
@@ -313,28 +566,16 @@ bool sizes_ok(uint32_t n, uint32_t rows, uint32_t cols) {
   return rows > 0 && cols > 0 && n < (1u << 24) && rows <= 65536u && cols <= 65536u && (uint64_t)rows * cols < (1ull << 31);
 }
 
-template <bool A_MN, bool B_MN, class Epi>
-int product(const Operand &a, const Operand &b, uint32_t M, uint32_t N, uint32_t K, uint32_t batch, bool symmetric, const typename Epi::Params &e, cudaStream_t s) {
-  ProductParams p = {};
-  p.M = M;
-  p.N = N;
-  p.batch = (int)batch;
-  p.symmetric = symmetric;
-  p.n_kb = (int)((K + kProdK - 1) / kProdK);
-  p.kb_per_split = p.n_kb;
-  p.splits = 1;
-  p.chunk = kChunk;
-  p.fmt = (uint32_t)kFmtF16;
-  // A pair's tile is four of a single CTA's; it takes about as long as two of them (its operands are shared), on twice the SMs.
-  auto tiles = [&](uint32_t t) {
-    const uint64_t m = (M + t - 1) / t, q = (N + t - 1) / t;
-    return (symmetric ? m * (m + 1) / 2 : m * q) * batch;
-  };
-  const uint64_t n_sm = (uint64_t)sm_count();
-  if (n_sm < 2) return DF_ERR_CUDA;
-  const uint64_t wide = (tiles(256) + n_sm / 2 - 1) / (n_sm / 2) * 12, narrow = (tiles(128) + n_sm - 1) / n_sm * 10;
-  if (wide < narrow) return launch_product<ProdCfg<true, A_MN, B_MN, 2>, Epi>(a, b, p, e, s);
-  return launch_product<ProdCfg<false, A_MN, B_MN, 2>, Epi>(a, b, p, e, s);
+// A matrix of parts in a batch as an operand, as operand_map
+bool batch_map(CUtensorMap *m, const void *base, uint64_t rows, uint64_t cols, uint64_t pitch, uint64_t n, uint64_t matrix, bool mn_major) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {cols, rows, n};
+  const cuuint64_t strides[2] = {pitch * 2, matrix * 2};
+  const cuuint32_t box[3] = {64, mn_major ? 64u : 128u, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 struct Plan {
@@ -344,17 +585,54 @@ struct Plan {
   Layout l;
   cudaStream_t s;
 
-  Operand parts(uint64_t at, uint64_t rows_, uint64_t cols_, uint64_t pitch, uint64_t matrix) const {
-    uint16_t *hi = reinterpret_cast<uint16_t *>(ws + at);
-    return {hi, hi + matrix * l.group, false, rows_, cols_, pitch, matrix};
+  template <class C>
+  int products(uint32_t n, NsParams &p) const {
+    auto tiles = [](uint32_t v) { return (int)((v + C::T - 1) / C::T); };
+    p.side_tiles = tiles(l.side);
+    p.x_m_tiles = tiles(rows);
+    p.x_n_tiles = tiles(cols);
+    p.g_units = p.side_tiles * (p.side_tiles + 1) / 2;
+    p.x_units = p.x_m_tiles * p.x_n_tiles;
+    const int slots = cluster_slots<k_newton_schulz<C>>(C::kCtas, C::kSmemTotal, kProdLaunchRegs);
+    if (slots == 0) return DF_ERR_CUDA;
+    const long long most = (long long)n * (p.g_units > p.x_units ? p.g_units : p.x_units);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = C::kCtas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)((most < slots ? most : slots) * C::kCtas));
+    cfg.blockDim = dim3(kProdThreads);
+    cfg.dynamicSmemBytes = C::kSmemTotal;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const int st = check_cuda(cudaLaunchKernelEx(&cfg, k_newton_schulz<C>, p));
+    note_launch();
+    return st;
   }
 
-  int run(uint32_t n, UpdateParams u, LastEpi::Params last) const {
-    Operand x = parts(l.x, rows, cols, l.x_pitch, l.x_matrix), next = parts(l.x_next, rows, cols, l.x_pitch, l.x_matrix);
-    const Operand g = parts(l.g, l.side, l.side, l.g_pitch, l.g_matrix), bb = parts(l.b, l.side, l.side, l.g_pitch, l.g_matrix);
+  int run(uint32_t n, UpdateParams u, NsParams p) const {
+    auto part = [&](uint64_t at, uint64_t matrix, int lo) { return reinterpret_cast<uint16_t *>(ws + at) + lo * matrix * l.group; };
+    bool ok = true;
+    for (int i = 0; i < 2; ++i) {
+      for (int j = 0; j < 2; ++j) {
+        p.x[j][i] = part(j ? l.x_next : l.x, l.x_matrix, i);
+        ok = ok && batch_map(&p.x_k[j][i], p.x[j][i], rows, cols, l.x_pitch, n, l.x_matrix, false) &&
+             batch_map(&p.x_mn[j][i], p.x[j][i], rows, cols, l.x_pitch, n, l.x_matrix, true);
+      }
+      p.gp[i] = part(l.g, l.g_matrix, i);
+      p.bp[i] = part(l.b, l.g_matrix, i);
+      ok = ok && batch_map(&p.g[i], p.gp[i], l.side, l.side, l.g_pitch, n, l.g_matrix, false) &&
+           batch_map(&p.b[i], p.bp[i], l.side, l.side, l.g_pitch, n, l.g_matrix, false);
+    }
+    if (!ok) return DF_ERR_CUDA;
     u.sums = reinterpret_cast<double *>(ws);
-    u.hi = static_cast<uint16_t *>(const_cast<void *>(x.hi));
-    u.lo = static_cast<uint16_t *>(const_cast<void *>(x.lo));
+    u.done = p.done = reinterpret_cast<uint32_t *>(ws + l.done);
+    u.hi = p.x[0][0];
+    u.lo = p.x[0][1];
     u.matrix = l.x_matrix;
     u.rows = rows;
     u.cols = cols;
@@ -366,48 +644,27 @@ struct Plan {
     const uint32_t blocks = (uint32_t)((quads + 255) / 256 < 512 ? (quads + 255) / 256 : 512);
     st = check_cuda(launch_kernel(k_normalise, dim3(blocks, n), dim3(256), 0, s, u));
     note_launch(2);
-    const bool wide = rows <= cols;
-    for (uint32_t i = 0; st == DF_OK && i < steps; ++i) {
-      SymmetricEpi::Params e = {};
-      e.hi = static_cast<uint16_t *>(const_cast<void *>(g.hi));
-      e.lo = static_cast<uint16_t *>(const_cast<void *>(g.lo));
-      e.matrix = l.g_matrix;
-      e.side = l.side;
-      e.pitch = l.g_pitch;
-      e.c = kPartInverse;  // parts are times 2^12, their product 2^24
-      st = wide ? product<false, false, SymmetricEpi>(x, x, l.side, l.side, cols, n, true, e, s)
-                : product<true, true, SymmetricEpi>(x, x, l.side, l.side, rows, n, true, e, s);
-      if (st != DF_OK) break;
-      e.hi = static_cast<uint16_t *>(const_cast<void *>(bb.hi));
-      e.lo = static_cast<uint16_t *>(const_cast<void *>(bb.lo));
-      e.g_hi = static_cast<const uint16_t *>(g.hi);
-      e.g_lo = static_cast<const uint16_t *>(g.lo);
-      e.a = a * kPartScale;
-      e.b = b;
-      e.c = c * kPartInverse;
-      st = product<false, false, SymmetricEpi>(g, g, l.side, l.side, l.side, n, true, e, s);
-      if (st != DF_OK) break;
-      if (i + 1 == steps) {
-        last.rows = rows;
-        last.cols = cols;
-        last.scale = kPartInverse * kPartInverse;
-        st = wide ? product<false, true, LastEpi>(bb, x, rows, cols, rows, n, false, last, s) : product<false, false, LastEpi>(x, bb, rows, cols, cols, n, false, last, s);
-        break;
-      }
-      NextEpi::Params f = {};
-      f.hi = static_cast<uint16_t *>(const_cast<void *>(next.hi));
-      f.lo = static_cast<uint16_t *>(const_cast<void *>(next.lo));
-      f.matrix = l.x_matrix;
-      f.rows = rows;
-      f.cols = cols;
-      f.pitch = l.x_pitch;
-      f.scale = kPartInverse;
-      st = wide ? product<false, true, NextEpi>(bb, x, rows, cols, rows, n, false, f, s) : product<false, false, NextEpi>(x, bb, rows, cols, cols, n, false, f, s);
-      const Operand t = x;
-      x = next;
-      next = t;
-    }
-    return st;
+    if (st != DF_OK) return st;
+    p.x_matrix = l.x_matrix;
+    p.g_matrix = l.g_matrix;
+    p.rows = rows;
+    p.cols = cols;
+    p.side = l.side;
+    p.x_pitch = l.x_pitch;
+    p.g_pitch = l.g_pitch;
+    p.wide = rows <= cols;
+    p.n = (int)n;
+    p.steps = (int)steps;
+    p.a = a * kPartScale;  // parts are times 2^12, their product 2^24
+    p.b_ = b;
+    p.c = c * kPartInverse;
+    p.status = device_status_ptr();
+    // Of a block of 64 a pair takes about 1536 cycles for 256 x 256 (its products), one CTA about 1150 for 128 x 128 (its operands' copies).
+    auto waves = [&](uint64_t t, uint64_t slots) {
+      const uint64_t m = (l.side + t - 1) / t, x = ((rows + t - 1) / t) * ((cols + t - 1) / t), g = m * (m + 1) / 2, larger = rows > cols ? rows : cols;
+      return ((g * n + slots - 1) / slots) * (larger + l.side) + ((x * n + slots - 1) / slots) * l.side;
+    };
+    return waves(256, 74) * 1536 < waves(128, 148) * 1150 ? products<NsCfg<true>>(n, p) : products<NsCfg<false>>(n, p);
   }
 };
 
@@ -450,11 +707,11 @@ int df_orthogonalize(const void *update, void *out, void *workspace, uint64_t wo
   for (uint32_t i0 = 0; st == DF_OK && i0 < n; i0 += l.group) {
     const uint32_t k = n - i0 < l.group ? n - i0 : l.group;
     UpdateParams u = {};
-    LastEpi::Params last = {};
+    NsParams last = {};
     u.row_stride = update_row_stride;
     u.bf16 = bf16 != 0;
-    last.row_stride = out_row_stride;
-    last.bf16 = bf16 != 0;
+    last.out_stride = out_row_stride;
+    last.out_bf16 = bf16 != 0;
     last.vec = 1;
     for (uint32_t i = 0; i < k; ++i) {
       u.t.source[i] = static_cast<const uint8_t *>(update) + (i0 + i) * update_matrix_stride * elt;
@@ -495,11 +752,11 @@ int df_muon_update(const void *tensors, uint32_t n, uint32_t rows, uint32_t cols
   for (uint32_t i0 = 0; st == DF_OK && i0 < n; i0 += l.group) {
     const uint32_t k = n - i0 < l.group ? n - i0 : l.group;
     UpdateParams u = {};
-    LastEpi::Params last = {};
+    NsParams last = {};
     u.row_stride = cols;
     u.beta = momentum;
     u.nesterov = nesterov != 0;
-    last.row_stride = cols;
+    last.out_stride = cols;
     last.vec = 1;
     last.apply = 1;
     last.keep = (float)(1.0 - (double)lr * (double)weight_decay);

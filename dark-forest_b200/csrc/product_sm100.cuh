@@ -1,18 +1,20 @@
 // product_sm100.cuh — batched matrix products of 16-bit operands on tcgen05 with an epilogue of the caller's:
-//   acc[b][m][n] = sum_k A[b][m][k] B[b][n][k]
+//   acc[m][n] = sum_k A[m][k] B[n][k]
 // Operands lie in global memory with either side contiguous (K-major: rows of k; MN-major: rows of m or n), bf16 or fp16. With
 // PARTS = 2 a value is two fp16 numbers, hi = fp16(s x) and lo = fp16(s x - hi) for a power of two s that the caller undoes: 22 bits
 // where |x| is within 2^18 of the largest that s was chosen for, and nothing below 2^-40 of that one. Then
 //   A B = A_lo B_hi + A_hi B_lo + A_hi B_hi      (A_lo B_lo, 2^-24 of it, is left out)
 // is three products in that order: the tensor cores cut sums off instead of rounding them, and a large sum is cut off at each of its
-// additions, so the small terms come first and a sum is taken out to registers, where it is added up rounded, every `chunk` blocks.
+// additions, so the small terms come first and every 64 of the contraction the sum is taken out to registers and added up rounded.
+// (Taken out every 768 a loss of 2048 rows of 768 was 2e-6 off 64 bits and orthogonalised 768 x 768 1.2e-5, every 192 6e-7 and 3.8e-6, every 64 1.4e-7 and
+// 1.6e-6, where sums in fp32 registers have 6e-7 and 2.3e-6.)
 //
-// One persistent kernel, at most one CTA an SM, 320 threads, as in linear_sm100.cu:
-//   warp 0      copies: a ring of stages, each 64 of the contraction: 128 rows of A and this CTA's rows of B, 128-byte swizzle;
-//   warp 1      issues the products into one of two accumulators in tensor memory;
-//   warps 2-9   the epilogue of one tile under the products of the next: a warp has the 32 rows of its quarter of tensor memory, a row
-//               a lane, and half of the tile's columns, 32 at a time.
-// Forms: a pair of CTAs on 256 x 256 (cta_group::2: 32 KB a CTA for 512 cycles of products), and one CTA on 128 x 128 where tiles are few.
+// One persistent kernel, at most one CTA an SM, 384 threads:
+//   warp 0       copies: a ring of stages, each 64 of the contraction: 128 rows of A and this CTA's rows of B (PARTS = 2: both parts), 128-byte swizzle;
+//   warp 1       issues the products into one of two accumulators in tensor memory;
+//   warps 4-11   the epilogue of one tile under the products of the next: a warp has the 32 rows of its quarter of tensor memory, a row
+//                a lane, and half of the tile's columns, 32 at a time. With PARTS = 2 its sums are 128 registers a thread, which it takes over from warps 0-3.
+// The tile is 256 x 256 over a pair of CTAs (cta_group::2): 32 KB a CTA and part for 512 cycles of products.
 // The contraction can be split: tile z * tiles + t is slice z of tile t, and the epilogue is told z.
 #pragma once
 
@@ -29,11 +31,8 @@ namespace df {
 struct ProductParams {
   uint32_t M, N;
   int m_tiles, n_tiles;     // tiles of this form along M and N
-  int tiles_per_batch;      // m_tiles * n_tiles, or those with n >= m of a symmetric product
-  int symmetric;
-  int batch, splits;
+  int splits;
   int n_kb, kb_per_split;   // blocks of 64 of the contraction: all, and of one slice
-  int chunk;                // blocks between takings out (PARTS = 2)
   long long tiles;
   uint32_t fmt;             // kFmtF16 or kFmtBF16
   unsigned int *status;
@@ -41,19 +40,43 @@ struct ProductParams {
 
 // One tile's place, as the epilogue sees it.
 struct ProductTile {
-  int m_tile, n_tile, batch, split;
+  int m_tile, n_tile, split;
 };
 
-constexpr int kProdEpiWarps = 8, kProdThreads = (2 + kProdEpiWarps) * 32, kProdK = 64;
+constexpr int kProdEpiWarps = 8, kProdThreads = 384, kProdK = 64;
 constexpr uint32_t kProdSlabBytes = 32 * 128;  // a warp's staging slab: 32 rows of 128 bytes
+// PARTS = 2: the launch gives 168 registers to each thread of three warpgroups; the two of the epilogue take over 48 from each thread of the first.
+constexpr int kProdLaunchRegs = 168, kProdEpiRegs = 216, kProdOtherRegs = 72;
+static_assert(2 * kProdEpiRegs + kProdOtherRegs <= 3 * kProdLaunchRegs, "setmaxnreg waits for registers that the block was not launched with");
+template <int N> __device__ __forceinline__ void prod_regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void prod_regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-template <bool PAIR_, bool A_MN_, bool B_MN_, int PARTS_>
+// The waits of sm100_ptx.cuh with their polling loop in place: a kernel that moves registers between its warps cannot be compiled with calls.
+__device__ __forceinline__ bool prod_wait(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) {
+  using namespace ptx;
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+#pragma unroll 1
+  for (uint32_t polls = 1; polls < kWaitMaxPolls; ++polls) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((polls & 255u) == 0u && (*abort_flag != 0u || global_timer_ns() - t0 > kWaitBudgetNs)) break;
+  }
+  *abort_flag = 1u;
+  return false;
+}
+__device__ __forceinline__ bool prod_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) {
+  using namespace ptx;
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, prod_wait(bar, parity, abort_flag)) != 0;
+}
+
+template <bool A_MN_, bool B_MN_, int PARTS_>
 struct ProdCfg {
-  static constexpr bool PAIR = PAIR_, A_MN = A_MN_, B_MN = B_MN_;
+  static constexpr bool A_MN = A_MN_, B_MN = B_MN_;
   static constexpr int PARTS = PARTS_;
-  static constexpr int TM = PAIR ? 256 : 128, TN = PAIR ? 256 : 128;
-  static constexpr uint32_t kABytes = 128 * kProdK * 2, kBBytes = 128 * kProdK * 2, kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 6;
+  static constexpr int TM = 256, TN = 256;
+  static constexpr uint32_t kTileBytes = 128 * kProdK * 2, kStageBytes = 2 * PARTS * kTileBytes;  // A hi, B hi (, A lo, B lo)
+  static constexpr int kStages = PARTS == 2 ? 3 : 6;
   static constexpr uint32_t kSmemStaging = kStages * kStageBytes;
   static constexpr uint32_t kSmemBars = kSmemStaging + kProdEpiWarps * kProdSlabBytes;
   static constexpr uint32_t kSmemTotal = kSmemBars + 256 + 1024;
@@ -61,22 +84,6 @@ struct ProdCfg {
   static constexpr int FULL = 0, EMPTY = FULL + kStages, ACC_FULL = EMPTY + kStages, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2, NUM_BARS = DRAIN + 1;
   static_assert(NUM_BARS * 8 <= 192 && kSmemTotal <= 227 * 1024, "shared memory");
 };
-
-// m and n tile of index t of a batch entry. Symmetric products have the tiles with n >= m only, row after row.
-__host__ __device__ inline void product_tile(const ProductParams &p, int t, int *m, int *n) {
-  if (!p.symmetric) {
-    *m = t / p.n_tiles;
-    *n = t % p.n_tiles;
-    return;
-  }
-  int row = 0;
-  while (t >= p.n_tiles - row) {
-    t -= p.n_tiles - row;
-    ++row;
-  }
-  *m = row;
-  *n = row + t;
-}
 
 // Epi: struct Params; begin(tile, row, col0) for this lane's row and the first of this warp's TN / 2 columns; block(cg, v): columns
 // col0 + 32 cg ..; end(). All of it warp-uniform in control flow apart from guarded accesses to memory.
@@ -86,7 +93,6 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
           const __grid_constant__ CUtensorMap tmB_lo, const __grid_constant__ ProductParams p, const __grid_constant__ typename Epi::Params e) {
   using namespace ptx;
   constexpr int kStages = C::kStages, TN = C::TN;
-  constexpr bool PAIR = C::PAIR;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t a0 = smem_u32(smem);
@@ -94,144 +100,126 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
   volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + C::kSmemBars + 192);
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(smem + C::kSmemBars + 196);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  const uint32_t rank = cluster_rank();
   auto bar = [&](int id) { return smem_u32(&bars[id]); };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::NUM_BARS; ++i) mbar_init(bar(i), i == C::ACC_EMPTY || i == C::ACC_EMPTY + 1 ? (PAIR ? 2 : 1) * kProdEpiWarps : 1);
+    for (int i = 0; i < C::NUM_BARS; ++i) mbar_init(bar(i), i == C::ACC_EMPTY || i == C::ACC_EMPTY + 1 ? 2 * kProdEpiWarps : 1);
     *abort_flag = 0;
     mbar_init_fence();
   }
   if (warp == 1) {
-    if (PAIR) {
-      tmem_alloc_pair(smem_u32(tmem_holder), C::kTmemCols);
-      tmem_relinquish_pair();
-    } else {
-      tmem_alloc(smem_u32(tmem_holder), C::kTmemCols);
-      tmem_relinquish();
-    }
+    tmem_alloc_pair(smem_u32(tmem_holder), C::kTmemCols);
+    tmem_relinquish_pair();
   }
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
   }
   tc_fence_before_sync();
-  if (PAIR) cluster_sync();
-  else __syncthreads();
+  cluster_sync();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_holder;
   pdl_wait();
-  constexpr int kCtas = PAIR ? 2 : 1, kPasses = C::PARTS == 2 ? 3 : 1;
-  const long long first_tile = blockIdx.x / kCtas, tile_step = gridDim.x / kCtas;
+  const long long first_tile = blockIdx.x / 2, tile_step = gridDim.x / 2;
 
   auto decode = [&](long long id, int *kb0, int *kb1) {
     ProductTile t;
-    const int per_split = p.tiles_per_batch * p.batch;
+    const int per_split = p.m_tiles * p.n_tiles, r = (int)(id % per_split);
     t.split = (int)(id / per_split);
-    const int r = (int)(id % per_split);
-    t.batch = r / p.tiles_per_batch;
-    product_tile(p, r % p.tiles_per_batch, &t.m_tile, &t.n_tile);
+    t.m_tile = r / p.n_tiles;
+    t.n_tile = r % p.n_tiles;
     *kb0 = t.split * p.kb_per_split;
     *kb1 = *kb0 + p.kb_per_split < p.n_kb ? *kb0 + p.kb_per_split : p.n_kb;
     return t;
   };
-  const int chunk = C::PARTS == 2 ? p.chunk : 0x40000000;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ copies (in a pair: each CTA its own rows)
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (long long id = first_tile; ok && id < p.tiles; id += tile_step) {
-        int kb0, kb1;
-        const ProductTile t = decode(id, &kb0, &kb1);
-        const int row_a = t.m_tile * C::TM + (int)rank * 128, row_b = t.n_tile * TN + (int)rank * 128;
-        for (int c0 = kb0; ok && c0 < kb1; c0 += chunk) {
-          const int c1 = c0 + chunk < kb1 ? c0 + chunk : kb1;
-          for (int pass = 0; ok && pass < kPasses; ++pass) {
-            const CUtensorMap *ta = kPasses == 3 && pass == 0 ? &tmA_lo : &tmA, *tb = kPasses == 3 && pass == 1 ? &tmB_lo : &tmB;
-            for (int kb = c0; kb < c1; ++kb, ++it) {
-              const uint32_t s = it % kStages, use = it / kStages;
-              if (use > 0 && !mbar_wait(bar(C::EMPTY + s), (use - 1) & 1, abort_flag)) { ok = false; break; }
-              const uint32_t sa = a0 + s * C::kStageBytes, sb = sa + C::kABytes;
-              // in a pair both CTAs' copies count on the even CTA's barrier, which expects the bytes of both
-              const uint32_t full = PAIR ? map_to_rank(bar(C::FULL + s), 0) : bar(C::FULL + s);
-              if (rank == 0) mbar_arrive_expect_tx(bar(C::FULL + s), kCtas * C::kStageBytes);
-              auto load = [&](uint32_t dst, const CUtensorMap *m, int x, int y) {
-                if (PAIR) tma_load_3d_pair(dst, m, full, x, y, t.batch);
-                else tma_load_3d(dst, m, full, x, y, t.batch);
-              };
-              if (C::A_MN) {
-                load(sa, ta, row_a, kb * kProdK);
-                load(sa + 8192, ta, row_a + 64, kb * kProdK);
+  if (warp < 4) {
+    if constexpr (C::PARTS == 2) prod_regs_less<kProdOtherRegs>();
+    if (warp == 0) {
+      // ---------------------------------------------------------- copies: each CTA its own rows
+      if (lane == 0) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (long long id = first_tile; ok && id < p.tiles; id += tile_step) {
+          int kb0, kb1;
+          const ProductTile t = decode(id, &kb0, &kb1);
+          const int row_a = t.m_tile * C::TM + (int)rank * 128, row_b = t.n_tile * TN + (int)rank * 128;
+          for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const uint32_t s = it % kStages, use = it / kStages;
+            if (use > 0 && !prod_wait(bar(C::EMPTY + s), (use - 1) & 1, abort_flag)) { ok = false; break; }
+            const uint32_t sa = a0 + s * C::kStageBytes;
+            // both CTAs' copies count on the even CTA's barrier, which expects the bytes of both
+            const uint32_t full = map_to_rank(bar(C::FULL + s), 0);
+            if (rank == 0) mbar_arrive_expect_tx(bar(C::FULL + s), 2 * C::kStageBytes);
+            auto load = [&](uint32_t dst, const CUtensorMap *m, bool mn, int row) {
+              if (mn) {
+                tma_load_2d_pair(dst, m, full, row, kb * kProdK);
+                tma_load_2d_pair(dst + 8192, m, full, row + 64, kb * kProdK);
               } else {
-                load(sa, ta, kb * kProdK, row_a);
+                tma_load_2d_pair(dst, m, full, kb * kProdK, row);
               }
-              if (C::B_MN) {
-                load(sb, tb, row_b, kb * kProdK);
-                load(sb + 8192, tb, row_b + 64, kb * kProdK);
-              } else {
-                load(sb, tb, kb * kProdK, row_b);
-              }
+            };
+            load(sa, &tmA, C::A_MN, row_a);
+            load(sa + C::kTileBytes, &tmB, C::B_MN, row_b);
+            if constexpr (C::PARTS == 2) {
+              load(sa + 2 * C::kTileBytes, &tmA_lo, C::A_MN, row_a);
+              load(sa + 3 * C::kTileBytes, &tmB_lo, C::B_MN, row_b);
             }
           }
         }
       }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ products (in a pair: the even CTA issues)
-    if (rank == 0) {
+    } else if (warp == 1 && rank == 0) {
+      // ---------------------------------------------------------- products: the even CTA issues for both
       const uint32_t idesc = make_idesc(p.fmt, C::TM, TN, C::A_MN ? 1 : 0, C::B_MN ? 1 : 0);
       uint32_t it = 0, j = 0;
       bool ok = true;
+      // K-major: 16 of k are 32 bytes of a swizzled row; MN-major: 16 rows of 128 bytes, the next 64 of m or n 8192 bytes on
+      auto issue = [&](uint32_t d, uint32_t sa, uint32_t sb, bool first) {
+        const uint64_t da = make_smem_desc(sa, C::A_MN ? 8192 : 16, 1024, kSwz128), db = make_smem_desc(sb, C::B_MN ? 8192 : 16, 1024, kSwz128);
+#pragma unroll
+        for (int k = 0; k < kProdK / 16; ++k) {
+          const uint64_t oa = (uint64_t)((k * (C::A_MN ? 2048 : 32)) >> 4), ob = (uint64_t)((k * (C::B_MN ? 2048 : 32)) >> 4);
+          mma_f16_ss_pair(d, da + oa, db + ob, idesc, first && k == 0 ? 0u : 1u);
+        }
+      };
       for (long long id = first_tile; ok && id < p.tiles; id += tile_step) {
         int kb0, kb1;
         decode(id, &kb0, &kb1);
-        for (int c0 = kb0; ok && c0 < kb1; c0 += chunk, ++j) {
-          const int c1 = c0 + chunk < kb1 ? c0 + chunk : kb1;
-          const uint32_t acc = j & 1;
-          if (j >= 2 && !mbar_wait_warp(bar(C::ACC_EMPTY + acc), ((j >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const uint32_t acc = j & 1, d = tmem + acc * TN, s = it % kStages, sa = a0 + s * C::kStageBytes;
+          // an accumulator is taken out after every block (PARTS = 2), or at the end of the tile
+          const bool first = C::PARTS == 2 || kb == kb0, last = C::PARTS == 2 || kb + 1 == kb1;
+          if (first && j >= 2 && !prod_wait_warp(bar(C::ACC_EMPTY + acc), ((j >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+          if (!prod_wait_warp(bar(C::FULL + s), (it / kStages) & 1, abort_flag)) { ok = false; break; }
           tc_fence_after_sync();
-          const int steps = (c1 - c0) * kPasses;
-          for (int n = 0; n < steps; ++n, ++it) {
-            const uint32_t s = it % kStages;
-            if (!mbar_wait_warp(bar(C::FULL + s), (it / kStages) & 1, abort_flag)) { ok = false; break; }
-            tc_fence_after_sync();
-            const uint32_t sa = a0 + s * C::kStageBytes, sb = sa + C::kABytes;
-            // K-major: 16 of k are 32 bytes of a swizzled row; MN-major: 16 rows of 128 bytes, the next 64 of m or n 8192 bytes on
-            const uint64_t da = make_smem_desc(sa, C::A_MN ? 8192 : 16, 1024, kSwz128), db = make_smem_desc(sb, C::B_MN ? 8192 : 16, 1024, kSwz128);
-            if (elect_one()) {
-#pragma unroll
-              for (int k = 0; k < kProdK / 16; ++k) {
-                const uint64_t oa = (uint64_t)((k * (C::A_MN ? 2048 : 32)) >> 4), ob = (uint64_t)((k * (C::B_MN ? 2048 : 32)) >> 4);
-                if (PAIR) mma_f16_ss_pair(tmem + acc * TN, da + oa, db + ob, idesc, (n > 0 || k > 0) ? 1u : 0u);
-                else mma_f16_ss(tmem + acc * TN, da + oa, db + ob, idesc, (n > 0 || k > 0) ? 1u : 0u);
-              }
-              if (PAIR) mma_commit_pair(bar(C::EMPTY + s));
-              else mma_commit(bar(C::EMPTY + s));
-              if (n + 1 == steps) {
-                if (PAIR) mma_commit_pair(bar(C::ACC_FULL + acc));
-                else mma_commit(bar(C::ACC_FULL + acc));
-              }
+          if (elect_one()) {
+            if constexpr (C::PARTS == 2) {
+              issue(d, sa + 2 * C::kTileBytes, sa + C::kTileBytes, true);
+              issue(d, sa, sa + 3 * C::kTileBytes, false);
+              issue(d, sa, sa + C::kTileBytes, false);
+            } else {
+              issue(d, sa, sa + C::kTileBytes, first);
             }
-            __syncwarp();
+            mma_commit_pair(bar(C::EMPTY + s));
+            if (last) mma_commit_pair(bar(C::ACC_FULL + acc));
           }
+          __syncwarp();
+          j += last;
         }
       }
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    if constexpr (C::PARTS == 2) prod_regs_more<kProdEpiRegs>();
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
     constexpr int kGroups = TN / 64;  // 32-column blocks of this warp
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * (TN / 2);
-    Epi epi(e, smem + C::kSmemStaging + (warp - 2) * kProdSlabBytes, lane);
+    Epi epi(e, smem + C::kSmemStaging + (warp - 4) * kProdSlabBytes, lane);
     auto release = [&](uint32_t acc) {
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) {
-        if (PAIR) mbar_arrive_cluster(map_to_rank(bar(C::ACC_EMPTY + acc), 0));
-        else mbar_arrive(bar(C::ACC_EMPTY + acc));
-      }
+      if (lane == 0) mbar_arrive_cluster(map_to_rank(bar(C::ACC_EMPTY + acc), 0));
     };
     uint32_t j = 0;
     bool ok = true;
@@ -242,7 +230,7 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
       epi.begin(t, row, col0);
       if constexpr (C::PARTS == 1) {
         const uint32_t acc = j & 1;
-        if (!mbar_wait_warp(bar(C::ACC_FULL + acc), (j >> 1) & 1, abort_flag)) break;
+        if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j >> 1) & 1, abort_flag)) break;
         tc_fence_after_sync();
 #pragma unroll 1
         for (int cg = 0; cg < kGroups; ++cg) {
@@ -258,24 +246,28 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         ++j;
       } else {
         float sum[kGroups][32];
-        for (int c0 = kb0; c0 < kb1; c0 += chunk, ++j) {
+#pragma unroll
+        for (int cg = 0; cg < kGroups; ++cg)
+#pragma unroll
+          for (int x = 0; x < 32; ++x) sum[cg][x] = 0.0f;
+#pragma unroll 1
+        for (int kb = kb0; kb < kb1; ++kb, ++j) {
           const uint32_t acc = j & 1;
-          if (!mbar_wait_warp(bar(C::ACC_FULL + acc), (j >> 1) & 1, abort_flag)) { ok = false; break; }
+          if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j >> 1) & 1, abort_flag)) { ok = false; break; }
           tc_fence_after_sync();
 #pragma unroll
           for (int cg = 0; cg < kGroups; ++cg) {
             uint32_t r[32];
             tmem_ld32(lane_base + acc * TN + cg * 32, r);
             tmem_wait_ld();
-            if (c0 == kb0) {
+            if (cg == kGroups - 1) release(acc);
 #pragma unroll
-              for (int x = 0; x < 32; ++x) sum[cg][x] = __uint_as_float(r[x]);
-            } else {
-#pragma unroll
-              for (int x = 0; x < 32; ++x) sum[cg][x] += __uint_as_float(r[x]);
+            for (int x = 0; x < 32; x += 2) {
+              const float2 q = add2(make_float2(sum[cg][x], sum[cg][x + 1]), as_float2(r[x], r[x + 1]));
+              sum[cg][x] = q.x;
+              sum[cg][x + 1] = q.y;
             }
           }
-          release(acc);
         }
         if (!ok) break;
 #pragma unroll
@@ -290,10 +282,7 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
   __syncthreads();
   if (*abort_flag != 0u) {
     if (warp == 1 && rank == 0) {
-      if (elect_one()) {
-        if (PAIR) mma_commit_pair(bar(C::DRAIN));
-        else mma_commit(bar(C::DRAIN));
-      }
+      if (elect_one()) mma_commit_pair(bar(C::DRAIN));
       __syncwarp();
       for (int n = 0; n < (1 << 16) && !mbar_try_wait(bar(C::DRAIN), 0); ++n) {
       }
@@ -306,11 +295,10 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
     if (threadIdx.x == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
     __syncthreads();
   }
-  if (PAIR) cluster_sync();
+  cluster_sync();
   if (warp == 1) {
     tc_fence_after_sync();
-    if (PAIR) tmem_dealloc_pair(tmem, C::kTmemCols);
-    else tmem_dealloc(tmem, C::kTmemCols);
+    tmem_dealloc_pair(tmem, C::kTmemCols);
   }
 }
 
@@ -349,71 +337,74 @@ __device__ __forceinline__ void turn_over(float4 *slab, int lane, const float (&
 }
 
 // ---------------------------------------------------------------- host
-// A 16-bit tensor [batch][rows][cols] (row pitch and batch pitch in elements, multiples of 8) as an operand: K-major boxes are 64 columns
-// x 128 rows, MN-major ones 64 x 64. Outside of it a copy gives zeros.
-inline bool operand_map(CUtensorMap *m, const void *base, bool bf16, uint64_t rows, uint64_t cols, uint64_t pitch, uint64_t batch, uint64_t batch_pitch,
-                        bool mn_major) {
+// A 16-bit matrix [rows][cols] (row pitch in elements, a multiple of 8) as an operand: K-major boxes are 64 columns x 128 rows, MN-major ones
+// 64 x 64. Outside of it a copy gives zeros.
+inline bool operand_map(CUtensorMap *m, const void *base, bool bf16, uint64_t rows, uint64_t cols, uint64_t pitch, bool mn_major) {
   PFN_encodeTiled enc = get_encode_tiled();
   if (!enc) return false;
-  const cuuint64_t dims[3] = {cols, rows, batch};
-  const cuuint64_t strides[2] = {pitch * 2, (batch > 1 ? batch_pitch : rows * pitch) * 2};
-  const cuuint32_t box[3] = {64, mn_major ? 64u : 128u, 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {pitch * 2};
+  const cuuint32_t box[2] = {64, mn_major ? 64u : 128u};
+  const cuuint32_t estr[2] = {1, 1};
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// An operand as the launcher needs it: its parts (lo only with two), and which side is contiguous.
+// An operand as the launcher needs it: its parts (lo only with two).
 struct Operand {
   const void *hi, *lo;
   bool bf16;
-  uint64_t rows, cols, pitch, batch_pitch;
+  uint64_t rows, cols, pitch;
 };
 
-// Launches one form of a product; `slots` (clusters that run at once) is kept per kernel and device by the caller's static.
+// How many clusters of a kernel run at once on the current device, its attributes set; asked for once per kernel and device. 0: it cannot be launched
+// (a build with other register counts than its hand-over of registers needs would wait for ever).
+template <auto Kernel>
+int cluster_slots(uint32_t ctas, uint32_t smem, int regs) {
+  static std::atomic<int> slots_of[64];
+  int dev = 0;
+  if (check_cuda(cudaGetDevice(&dev)) != DF_OK || dev < 0 || dev >= 64) return 0;
+  int slots = slots_of[dev].load(std::memory_order_acquire);
+  if (slots != 0) return slots;
+  cudaFuncAttributes have;
+  if (check_cuda(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != DF_OK ||
+      check_cuda(cudaFuncGetAttributes(&have, Kernel)) != DF_OK || (regs != 0 && have.numRegs != regs))
+    return 0;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(64 * ctas);
+  cfg.blockDim = dim3(kProdThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (check_cuda(cudaOccupancyMaxActiveClusters(&slots, Kernel, &cfg)) != DF_OK || slots <= 0) return 0;
+  slots_of[dev].store(slots, std::memory_order_release);
+  return slots;
+}
+
 template <class C, class Epi>
 int launch_product(const Operand &a, const Operand &b, ProductParams p, const typename Epi::Params &e, cudaStream_t s) {
   static_assert(sizeof(ProductParams) + sizeof(typename Epi::Params) + 4 * sizeof(CUtensorMap) < 4000, "kernel parameters");
-  auto kernel = k_product<C, Epi>;
-  static std::atomic<int> slots_of[64];  // 0: not asked yet
-  int dev = 0;
-  if (check_cuda(cudaGetDevice(&dev)) != DF_OK || dev < 0 || dev >= 64) return DF_ERR_CUDA;
-  constexpr int ctas = C::PAIR ? 2 : 1;
-  int slots = slots_of[dev].load(std::memory_order_acquire);
-  if (slots == 0) {
-    if (check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmemTotal)) != DF_OK) return DF_ERR_CUDA;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ctas;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(64 * ctas);
-    cfg.blockDim = dim3(kProdThreads);
-    cfg.dynamicSmemBytes = C::kSmemTotal;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (check_cuda(cudaOccupancyMaxActiveClusters(&slots, kernel, &cfg)) != DF_OK || slots <= 0) return DF_ERR_CUDA;
-    slots_of[dev].store(slots, std::memory_order_release);
-  }
+  const int slots = cluster_slots<k_product<C, Epi>>(2, C::kSmemTotal, C::PARTS == 2 ? kProdLaunchRegs : 0);
+  if (slots == 0) return DF_ERR_CUDA;
   p.m_tiles = (int)((p.M + C::TM - 1) / C::TM);
   p.n_tiles = (int)((p.N + C::TN - 1) / C::TN);
-  p.tiles_per_batch = p.symmetric ? p.m_tiles * (p.m_tiles + 1) / 2 : p.m_tiles * p.n_tiles;
-  p.tiles = (long long)p.tiles_per_batch * p.batch * p.splits;
+  p.tiles = (long long)p.m_tiles * p.n_tiles * p.splits;
   p.status = device_status_ptr();
   CUtensorMap ma, ma_lo, mb, mb_lo;
-  bool ok = operand_map(&ma, a.hi, a.bf16, a.rows, a.cols, a.pitch, p.batch, a.batch_pitch, C::A_MN) &&
-            operand_map(&mb, b.hi, b.bf16, b.rows, b.cols, b.pitch, p.batch, b.batch_pitch, C::B_MN);
+  bool ok = operand_map(&ma, a.hi, a.bf16, a.rows, a.cols, a.pitch, C::A_MN) && operand_map(&mb, b.hi, b.bf16, b.rows, b.cols, b.pitch, C::B_MN);
   ma_lo = ma;
   mb_lo = mb;
-  if (C::PARTS == 2)
-    ok = ok && operand_map(&ma_lo, a.lo, a.bf16, a.rows, a.cols, a.pitch, p.batch, a.batch_pitch, C::A_MN) &&
-         operand_map(&mb_lo, b.lo, b.bf16, b.rows, b.cols, b.pitch, p.batch, b.batch_pitch, C::B_MN);
+  if (C::PARTS == 2) ok = ok && operand_map(&ma_lo, a.lo, a.bf16, a.rows, a.cols, a.pitch, C::A_MN) && operand_map(&mb_lo, b.lo, b.bf16, b.rows, b.cols, b.pitch, C::B_MN);
   if (!ok) {
     note_status(DF_ERR_CUDA);
     return DF_ERR_CUDA;
   }
-  const long long grid = (p.tiles < slots ? p.tiles : slots) * ctas;
-  const int st = check_cuda(launch_clusters(kernel, ctas > 1 ? ctas : 0, dim3((unsigned)grid), dim3(kProdThreads), C::kSmemTotal, s, ma, ma_lo, mb, mb_lo, p, e));
+  const long long grid = (p.tiles < slots ? p.tiles : slots) * 2;
+  const int st = check_cuda(launch_clusters(k_product<C, Epi>, 2, dim3((unsigned)grid), dim3(kProdThreads), C::kSmemTotal, s, ma, ma_lo, mb, mb_lo, p, e));
   note_launch();
   return st;
 }
