@@ -21,7 +21,7 @@ using namespace ptx;
 constexpr float kPartScale = 4096.0f, kPartInverse = 1.0f / 4096.0f;
 constexpr int kMostMatrices = 64;               // of a group: what the kernels' tables of pointers hold
 constexpr uint64_t kGroupBytes = 512ull << 20;  // of workspace, beyond one matrix
-constexpr int kNormBlocks = 64;                 // partial sums of squares per matrix
+constexpr int kNormBlocks = 256;                // partial sums of squares per matrix, at most
 constexpr uint32_t kMostTensors = 1024;         // of an optimiser step: every pair is checked for overlap
 
 int finish(int st) {
@@ -45,86 +45,126 @@ struct Targets {
 // ---------------------------------------------------------------- before the products
 struct UpdateParams {
   Table t;
-  double *sums;  // [matrices][kNormBlocks]
+  double *sums;    // [matrices][kNormBlocks]
   uint32_t *done;  // [matrices]: set to 0 here
   uint16_t *hi, *lo;
   uint64_t row_stride, matrix;  // of the source; elements of a matrix in parts
-  uint32_t rows, cols, pitch, bf16, nesterov;
+  uint32_t rows, cols, pitch, bf16, nesterov, vec;  // vec: four elements of a row at a time
   float beta, eps;
 };
 
-// U at (row, col): the source itself, or the momentum with or without a look ahead (the momentum has been moved already)
-__device__ __forceinline__ float update_at(const UpdateParams &p, int m, uint32_t r, uint32_t c) {
-  const float g = load_f(p.t.source[m], p.bf16, (size_t)r * p.row_stride + c);
-  if (!p.t.momentum[m]) return g;
-  const float v = p.t.momentum[m][(size_t)r * p.cols + c];
-  return p.nesterov ? fmaf(p.beta, v, g) : v;
+__device__ __forceinline__ float4 load_four(const void *p, bool bf16, size_t i) {
+  if (!bf16) return *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+  const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i);
+  return make_float4(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u));
 }
 
-// Moves the momentum, and adds up squares: blocks of a matrix take rows in turn. Squares in double: a gradient of 1e-30 is none of 0.
+// Moves the momentum, and adds up the squares of U: a warp a row, or all of a matrix that lies in one piece by 128 elements a warp. Squares in double: a
+// gradient of 1e-30 is none of 0.
 __global__ void __launch_bounds__(256) k_update(const __grid_constant__ UpdateParams p) {
   pdl_wait();
-  const int m = blockIdx.y;
+  const int m = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const void *source = p.t.source[m];
+  float *momentum = p.t.momentum[m];
+  const bool flat = p.rows == 1 || p.row_stride == p.cols;  // rows * cols below 2^31
+  const uint32_t rows = flat ? 1 : p.rows, cols = flat ? p.rows * p.cols : p.cols;
+  const uint32_t workers = gridDim.x * 8, me = blockIdx.x * 8 + warp;
   double sum = 0.0;
-  const uint64_t n = (uint64_t)p.rows * p.cols;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)kNormBlocks * 256) {
-    const uint32_t r = (uint32_t)(i / p.cols), c = (uint32_t)(i % p.cols);
-    if (p.t.momentum[m]) p.t.momentum[m][i] = fmaf(p.beta, p.t.momentum[m][i], load_f(p.t.source[m], p.bf16, (size_t)r * p.row_stride + c));
-    const double u = update_at(p, m, r, c);
-    sum += u * u;
+  for (uint32_t r = flat ? 0 : me; r < rows; r += flat ? 1 : workers) {
+    const size_t at = (size_t)r * p.row_stride, at_m = (size_t)r * p.cols;
+    const uint32_t whole = p.vec ? cols & ~3u : 0, step = flat ? workers : 1;
+#pragma unroll 4
+    for (uint32_t c = ((flat ? me : 0) * 32 + lane) * 4; c < whole; c += step * 128) {
+      float4 u = load_four(source, p.bf16, at + c);
+      if (momentum) {
+        float4 v = *reinterpret_cast<const float4 *>(momentum + at_m + c);
+        v = make_float4(fmaf(p.beta, v.x, u.x), fmaf(p.beta, v.y, u.y), fmaf(p.beta, v.z, u.z), fmaf(p.beta, v.w, u.w));
+        *reinterpret_cast<float4 *>(momentum + at_m + c) = v;
+        u = p.nesterov ? make_float4(fmaf(p.beta, v.x, u.x), fmaf(p.beta, v.y, u.y), fmaf(p.beta, v.z, u.z), fmaf(p.beta, v.w, u.w)) : v;
+      }
+      sum += ((double)u.x * u.x + (double)u.y * u.y) + ((double)u.z * u.z + (double)u.w * u.w);
+    }
+    for (uint32_t c = whole + (flat ? me : 0) * 32 + lane; c < cols; c += step * 32) {
+      float u = load_f(source, p.bf16, at + c);
+      if (momentum) {
+        const float v = fmaf(p.beta, momentum[at_m + c], u);
+        momentum[at_m + c] = v;
+        u = p.nesterov ? fmaf(p.beta, v, u) : v;
+      }
+      sum += (double)u * u;
+    }
   }
-  __shared__ double part[256];
-  part[threadIdx.x] = sum;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  __shared__ double part[8];
+  if (lane == 0) part[warp] = sum;
   __syncthreads();
-  for (int half = 128; half > 0; half >>= 1) {
-    if ((int)threadIdx.x < half) part[threadIdx.x] += part[threadIdx.x + half];
-    __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) sum += part[i];
+    p.sums[m * kNormBlocks + blockIdx.x] = sum;
+    if (blockIdx.x == 0) p.done[m] = 0;
   }
-  if (threadIdx.x == 0) p.sums[m * kNormBlocks + blockIdx.x] = part[0];
-  if (threadIdx.x == 0 && blockIdx.x == 0) p.done[m] = 0;
 }
 
-// X in parts
-__global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ UpdateParams p) {
+// X in parts, a warp a row
+__global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ UpdateParams p, int blocks) {
   pdl_wait();
-  const int m = blockIdx.y;
-  __shared__ float factor;
-  if (threadIdx.x == 0) {
-    double sum = 0.0;
-    for (int i = 0; i < kNormBlocks; ++i) sum += p.sums[m * kNormBlocks + i];
-    factor = (float)((double)kPartScale / (sqrt(sum) + (double)p.eps));
-  }
-  __syncthreads();
-  const float f = factor;
-  const uint32_t quads = p.pitch / 4;
-  const uint64_t n = (uint64_t)p.rows * quads;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) {
-    const uint32_t r = (uint32_t)(i / quads), c = (uint32_t)(i % quads) * 4;
-    float v[4];
+  const int m = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double sum = 0.0;
+  for (int i = lane; i < blocks; i += 32) sum += p.sums[m * kNormBlocks + i];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) v[x] = c + x < p.cols ? update_at(p, m, r, c + x) * f : 0.0f;
-    uint2 hi, lo;
-    split_half2(v[0], v[1], hi.x, lo.x);
-    split_half2(v[2], v[3], hi.y, lo.y);
-    const size_t to = (size_t)m * p.matrix + (size_t)r * p.pitch + c;
-    *reinterpret_cast<uint2 *>(p.hi + to) = hi;
-    *reinterpret_cast<uint2 *>(p.lo + to) = lo;
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  const float f = (float)((double)kPartScale / (sqrt(sum) + (double)p.eps));
+  const void *source = p.t.source[m];
+  const float *momentum = p.t.momentum[m];
+  for (uint32_t r = blockIdx.x * 8 + warp; r < p.rows; r += gridDim.x * 8) {
+    const size_t at = (size_t)r * p.row_stride, at_m = (size_t)r * p.cols, to = (size_t)m * p.matrix + (size_t)r * p.pitch;
+#pragma unroll 2
+    for (uint32_t c = lane * 4; c < p.pitch; c += 128) {
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (p.vec && c + 4 <= p.cols) {
+        const float4 u = load_four(source, p.bf16, at + c);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+        if (momentum) {
+          const float4 q = *reinterpret_cast<const float4 *>(momentum + at_m + c);
+          const float g[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int x = 0; x < 4; ++x) v[x] = p.nesterov ? fmaf(p.beta, g[x], v[x]) : g[x];
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (c + x >= p.cols) continue;
+          v[x] = load_f(source, p.bf16, at + c + x);
+          if (momentum) v[x] = p.nesterov ? fmaf(p.beta, momentum[at_m + c + x], v[x]) : momentum[at_m + c + x];
+        }
+      }
+      uint2 hi, lo;
+      split_half2(v[0] * f, v[1] * f, hi.x, lo.x);
+      split_half2(v[2] * f, v[3] * f, hi.y, lo.y);
+      *reinterpret_cast<uint2 *>(p.hi + to + c) = hi;
+      *reinterpret_cast<uint2 *>(p.lo + to + c) = lo;
+    }
   }
 }
 
 // ---------------------------------------------------------------- the products
-template <bool PAIR_>
+// PAIR: tiles of 256 x 256 over two CTAs. Else 128 x 128, the contraction cut among KS CTAs of a cluster.
+template <bool PAIR_, int KS_>
 struct NsCfg {
   static constexpr bool PAIR = PAIR_;
-  static constexpr int kCtas = PAIR ? 2 : 1, T = PAIR ? 256 : 128;  // tiles of T x T
-  static constexpr uint32_t kTileBytes = 128 * kProdK * 2, kStageBytes = 4 * kTileBytes;  // A hi, B hi, A lo, B lo
-  static constexpr int kStages = 3;
-  static constexpr uint32_t kSmemStaging = kStages * kStageBytes;
-  static constexpr uint32_t kSmemBars = kSmemStaging + kProdEpiWarps * kProdSlabBytes;
+  static constexpr int KS = KS_, kCtas = PAIR ? 2 : KS, T = PAIR ? 256 : 128;
+  static constexpr int kOwned = T / KS, W = kOwned / 2 < 32 ? kOwned / 2 : 32, kGroups = kOwned / 2 / W;  // columns of a CTA's results; of a warp, W at a time
+  static constexpr uint32_t kTileBytes = 128 * kProdK * 2, kSlotBytes = 2 * kTileBytes;  // a slot: A and B, low or high parts, in turn
+  static constexpr int kSlots = KS > 1 ? 5 : 6;
+  // the other half of shared memory: slabs of the epilogue's warps, or the partial sums [KS][128][kOwned] of the columns that this CTA owns
+  static constexpr uint32_t kSmemStaging = kSlots * kSlotBytes, kStagingBytes = KS > 1 ? 128 * 128 * 4 : kProdEpiWarps * kProdSlabBytes;
+  static constexpr uint32_t kSmemBars = kSmemStaging + kStagingBytes;
   static constexpr uint32_t kSmemTotal = kSmemBars + 256 + 1024;
   static constexpr uint32_t kTmemCols = 2 * T;
-  static constexpr int FULL = 0, EMPTY = FULL + kStages, ACC_FULL = EMPTY + kStages, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2, NUM_BARS = DRAIN + 1;
-  static_assert(NUM_BARS * 8 <= 192 && kSmemTotal <= 227 * 1024, "shared memory");
+  static constexpr int FULL = 0, EMPTY = FULL + kSlots, ACC_FULL = EMPTY + kSlots, ACC_EMPTY = ACC_FULL + 2, RED_FULL = ACC_EMPTY + 2, RED_FREE = RED_FULL + 1,
+                       DRAIN = RED_FREE + 1, NUM_BARS = DRAIN + 1;
+  static_assert(NUM_BARS * 8 <= 192 && kSmemTotal <= 227 * 1024 && (!PAIR || KS == 1), "shared memory");
 };
 
 struct NsParams {
@@ -135,6 +175,8 @@ struct NsParams {
   uint64_t x_matrix, g_matrix;
   uint32_t rows, cols, side, x_pitch, g_pitch;
   int wide, n, steps;
+  int from, to;               // units of this launch
+  int ordered;                // 1: what a unit needs was written by launches before this one
   int side_tiles, x_m_tiles, x_n_tiles, g_units, x_units;  // tiles: along the side, of X; of a symmetric product, of X's
   float a, b_, c;             // of B, times the parts' scales
   Targets t;
@@ -184,10 +226,11 @@ __device__ __forceinline__ Unit unit_of(const NsParams &p, int u) {
   return w;
 }
 
-// A row's 32 columns of two parts, 64 bytes each
-__device__ __forceinline__ void write_parts(uint16_t *hi, uint16_t *lo, size_t at, const float (&v)[32]) {
+// W columns of a row in two parts
+template <int W>
+__device__ __forceinline__ void write_parts(uint16_t *hi, uint16_t *lo, size_t at, const float (&v)[W]) {
 #pragma unroll
-  for (int x = 0; x < 32; x += 8) {
+  for (int x = 0; x < W; x += 8) {
     uint4 h, l;
     split_half2(v[x], v[x + 1], h.x, l.x);
     split_half2(v[x + 2], v[x + 3], h.y, l.y);
@@ -199,7 +242,8 @@ __device__ __forceinline__ void write_parts(uint16_t *hi, uint16_t *lo, size_t a
 }
 
 // G = X X^T, or B = a I + b G + c G G: symmetric, in parts, each tile in its place and in the mirrored one
-__device__ __forceinline__ void symmetric_block(const NsParams &p, const Unit &w, uint32_t row, uint32_t first, float (&v)[32]) {
+template <int W>
+__device__ __forceinline__ void symmetric_block(const NsParams &p, const Unit &w, uint32_t row, uint32_t first, float (&v)[W]) {
   if (first >= p.side || row >= p.side) return;  // the pitch is a multiple of 64: a block that begins inside may be written whole
   const size_t base = (size_t)w.batch * p.g_matrix, at = base + (size_t)row * p.g_pitch + first;
   uint16_t *hi, *lo;
@@ -207,7 +251,7 @@ __device__ __forceinline__ void symmetric_block(const NsParams &p, const Unit &w
     hi = p.bp[0];
     lo = p.bp[1];
 #pragma unroll
-    for (int x = 0; x < 32; x += 8) {  // written by other SMs of this launch: not through L1
+    for (int x = 0; x < W; x += 8) {  // written by other SMs of this launch: not through L1
       const uint4 h = __ldcg(reinterpret_cast<const uint4 *>(p.gp[0] + at + x)), l = __ldcg(reinterpret_cast<const uint4 *>(p.gp[1] + at + x));
       const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
@@ -218,18 +262,18 @@ __device__ __forceinline__ void symmetric_block(const NsParams &p, const Unit &w
       }
     }
 #pragma unroll
-    for (int x = 0; x < 32; ++x) v[x] += first + x == row ? p.a : 0.0f;
+    for (int x = 0; x < W; ++x) v[x] += first + x == row ? p.a : 0.0f;
   } else {
     hi = p.gp[0];
     lo = p.gp[1];
 #pragma unroll
-    for (int x = 0; x < 32; ++x) v[x] *= kPartInverse;
+    for (int x = 0; x < W; ++x) v[x] *= kPartInverse;
   }
-  write_parts(hi, lo, at, v);
+  write_parts<W>(hi, lo, at, v);
   if (w.m == w.n) return;
   // the mirrored tile: a column's 32 rows lie together across the warp's lanes
 #pragma unroll
-  for (int x = 0; x < 32; ++x) {
+  for (int x = 0; x < W; ++x) {
     if (first + x >= p.side) break;
     const size_t to = base + (size_t)(first + x) * p.g_pitch + row;
     const __half h = __float2half_rn(v[x]);
@@ -238,51 +282,147 @@ __device__ __forceinline__ void symmetric_block(const NsParams &p, const Unit &w
   }
 }
 
-// X of the last step: written in the caller's type, or applied to the parameter: P <- keep P - step X
+// Four columns of X of the last step: written in the caller's type, or applied to the parameter: P <- keep P - step X
+__device__ __forceinline__ void last_four(const NsParams &p, void *out, uint32_t r, uint32_t col, float4 q) {
+  constexpr float scale = kPartInverse * kPartInverse;
+  float y[4] = {q.x * scale, q.y * scale, q.z * scale, q.w * scale};
+  const size_t at = (size_t)r * p.out_stride + col;
+  if (p.vec && col + 4 <= p.cols) {
+    if (p.out_bf16) {
+      uint2 b;
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.x) : "f"(y[1]), "f"(y[0]));
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.y) : "f"(y[3]), "f"(y[2]));
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + at) = b;
+    } else {
+      float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(out) + at);
+      if (p.apply) {
+        const float4 old = *to;
+        y[0] = fmaf(p.keep, old.x, -p.step * y[0]);
+        y[1] = fmaf(p.keep, old.y, -p.step * y[1]);
+        y[2] = fmaf(p.keep, old.z, -p.step * y[2]);
+        y[3] = fmaf(p.keep, old.w, -p.step * y[3]);
+      }
+      *to = make_float4(y[0], y[1], y[2], y[3]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    if (col + x >= p.cols) break;
+    if (p.out_bf16) {
+      uint32_t b;
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(0.0f), "f"(y[x]));
+      static_cast<uint16_t *>(out)[at + x] = (uint16_t)b;
+    } else {
+      float *to = static_cast<float *>(out) + at + x;
+      *to = p.apply ? fmaf(p.keep, *to, -p.step * y[x]) : y[x];
+    }
+  }
+}
+// 32 columns of a warp's rows, turned over so that memory moves in whole lines
 __device__ __forceinline__ void last_block(const NsParams &p, const Unit &w, float4 *slab, int lane, uint32_t row0, uint32_t first, const float (&v)[32]) {
   if (first >= p.cols) return;
   float4 q[8];
   turn_over(slab, lane, v, q);
   const uint32_t col = first + 4 * (lane & 7);
   if (col >= p.cols) return;
-  void *out = p.t.out[w.batch];
-  constexpr float scale = kPartInverse * kPartInverse;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint32_t r = row0 + 4 * i + (lane >> 3);
-    if (r >= p.rows) continue;
-    float y[4] = {q[i].x * scale, q[i].y * scale, q[i].z * scale, q[i].w * scale};
-    const size_t at = (size_t)r * p.out_stride + col;
-    if (p.vec && col + 4 <= p.cols) {
-      if (p.out_bf16) {
-        uint2 b;
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.x) : "f"(y[1]), "f"(y[0]));
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.y) : "f"(y[3]), "f"(y[2]));
-        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + at) = b;
-      } else {
-        float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(out) + at);
-        if (p.apply) {
-          const float4 old = *to;
-          y[0] = fmaf(p.keep, old.x, -p.step * y[0]);
-          y[1] = fmaf(p.keep, old.y, -p.step * y[1]);
-          y[2] = fmaf(p.keep, old.z, -p.step * y[2]);
-          y[3] = fmaf(p.keep, old.w, -p.step * y[3]);
+    if (r < p.rows) last_four(p, p.t.out[w.batch], r, col, q[i]);
+  }
+}
+
+// Blocks of 32 rows x 64 columns of a warp, v[0 .. 63] a lane's row: they go through the warp's slab, so that global memory moves in whole lines (a lane's own
+// row as it is: 32 lines an instruction, 8 us for a tile's 128 x 256; turned over 4).
+__device__ __forceinline__ void store_block(uint4 *slab, int lane, uint16_t *dst, size_t pitch, uint32_t rows, const uint4 (&q)[8]) {
+  __syncwarp();
+#pragma unroll
+  for (int x = 0; x < 8; ++x) slab[lane * 8 + (x ^ (lane & 7))] = q[x];
+  __syncwarp();
+  const int lrow = lane >> 3, chunk = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint4 v = slab[(4 * i + lrow) * 8 + (chunk ^ ((4 * i + lrow) & 7))];
+    if ((uint32_t)(4 * i + lrow) < rows) *reinterpret_cast<uint4 *>(dst + (size_t)(4 * i + lrow) * pitch + 8 * chunk) = v;
+  }
+}
+__device__ __forceinline__ void split_block(const float (&v)[64], uint4 (&q)[8], bool low) {
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) split_half2(v[8 * x + 2 * y], v[8 * x + 2 * y + 1], h[y], l[y]);
+    q[x] = low ? make_uint4(l[0], l[1], l[2], l[3]) : make_uint4(h[0], h[1], h[2], h[3]);
+  }
+}
+// `rows`: how many of the warp's 32 are in the matrix
+__device__ __forceinline__ void next_block(uint16_t *const (&dst)[2], size_t at, uint32_t pitch, uint4 *slab, int lane, uint32_t rows, float (&v)[64]) {
+#pragma unroll
+  for (int low = 0; low < 2; ++low) {
+    uint4 q[8];
+    split_block(v, q, low != 0);
+    store_block(slab, lane, dst[low] + at, pitch, rows, q);
+  }
+}
+__device__ __forceinline__ void symmetric_64(const NsParams &p, const Unit &w, uint4 *slab, int lane, uint32_t row0, uint32_t first, float (&v)[64]) {
+  if (first >= p.side || row0 >= p.side) return;
+  const size_t base = (size_t)w.batch * p.g_matrix, at = base + (size_t)row0 * p.g_pitch + first;
+  const uint32_t rows = p.side - row0;
+  if (w.product == kPolynomial) {
+    const int lrow = lane >> 3, chunk = lane & 7;
+#pragma unroll
+    for (int low = 0; low < 2; ++low) {
+      uint4 q[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)  // written by other SMs of this launch: not through L1
+        q[i] = (uint32_t)(4 * i + lrow) < rows ? __ldcg(reinterpret_cast<const uint4 *>(p.gp[low] + at + (size_t)(4 * i + lrow) * p.g_pitch + 8 * chunk))
+                                               : make_uint4(0u, 0u, 0u, 0u);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) slab[(4 * i + lrow) * 8 + (chunk ^ ((4 * i + lrow) & 7))] = q[i];
+      __syncwarp();
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const uint4 g = slab[lane * 8 + (x ^ (lane & 7))];
+        const uint32_t gg[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&gg[y]));
+          float &v0 = v[8 * x + 2 * y], &v1 = v[8 * x + 2 * y + 1];
+          v0 = low == 0 ? fmaf(p.c, v0, p.b_ * f.x) : fmaf(p.b_, f.x, v0);
+          v1 = low == 0 ? fmaf(p.c, v1, p.b_ * f.y) : fmaf(p.b_, f.y, v1);
         }
-        *to = make_float4(y[0], y[1], y[2], y[3]);
       }
-      continue;
     }
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      if (col + x >= p.cols) break;
-      if (p.out_bf16) {
-        uint32_t b;
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(0.0f), "f"(y[x]));
-        static_cast<uint16_t *>(out)[at + x] = (uint16_t)b;
-      } else {
-        float *to = static_cast<float *>(out) + at + x;
-        *to = p.apply ? fmaf(p.keep, *to, -p.step * y[x]) : y[x];
-      }
+    for (int x = 0; x < 64; ++x) v[x] += first + x == row0 + lane ? p.a : 0.0f;
+  } else {
+#pragma unroll
+    for (int x = 0; x < 64; ++x) v[x] *= kPartInverse;
+  }
+  uint16_t *const(&dst)[2] = w.product == kPolynomial ? p.bp : p.gp;
+  next_block(dst, at, p.g_pitch, slab, lane, rows, v);
+  if (w.m == w.n) return;
+  // the mirrored tile: column x of the block is row first + x, 32 elements from row0 on. Two lanes make a pair of rows of a column each.
+  const uint32_t columns = p.side - first;
+#pragma unroll
+  for (int low = 0; low < 2; ++low) {
+    uint32_t *words = reinterpret_cast<uint32_t *>(slab);
+    __syncwarp();
+#pragma unroll
+    for (int x = 0; x < 64; x += 2) {
+      uint32_t h, l;
+      split_half2(v[x], v[x + 1], h, l);
+      const uint32_t mine = low ? l : h, other = __shfl_xor_sync(0xffffffffu, mine, 1);
+      words[(x + (lane & 1)) * 16 + (lane >> 1)] = lane & 1 ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t c = 8 * i + (lane >> 2);
+      const uint4 q = slab[c * 4 + (lane & 3)];
+      if (c < columns) *reinterpret_cast<uint4 *>(dst[low] + base + (size_t)(first + c) * p.g_pitch + row0 + 8 * (lane & 3)) = q;
     }
   }
 }
@@ -295,9 +435,33 @@ __device__ __forceinline__ uint32_t load_acquire(const uint32_t *p) {
 // Writes by ordinary stores become visible to the copy engines of other SMs: a fence between the two ways to memory at both ends.
 __device__ __forceinline__ void fence_proxies() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
+// As prod_wait_warp, for a barrier on which other CTAs of the cluster arrive behind their writes to this one's shared memory.
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) {
+  auto there = [&]() {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+  };
+  bool done = there();
+  if (!done) {
+    const uint64_t t0 = global_timer_ns();
+#pragma unroll 1
+    for (uint32_t polls = 1; !done && polls < kWaitMaxPolls; ++polls) {
+      done = there();
+      if ((polls & 255u) == 0u && (*abort_flag != 0u || global_timer_ns() - t0 > kWaitBudgetNs)) break;
+    }
+    if (!done) *abort_flag = 1u;
+  }
+  return __all_sync(0xffffffffu, done) != 0;
+}
+
 template <class C>
 __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_constant__ NsParams p) {
-  constexpr int kStages = C::kStages, T = C::T;
+  constexpr int kSlots = C::kSlots, T = C::T, KS = C::KS;
   constexpr bool PAIR = C::PAIR;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -306,11 +470,16 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
   volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + C::kSmemBars + 192);
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(smem + C::kSmemBars + 196);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  const uint32_t rank = PAIR ? cluster_rank() : 0, part = KS > 1 ? cluster_rank() : 0;
   auto bar = [&](int id) { return smem_u32(&bars[id]); };
+  auto first_block = [&](int blocks) { return (int)part * blocks / KS; };
+  auto my_blocks = [&](int blocks) { return ((int)part + 1) * blocks / KS - (int)part * blocks / KS; };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::NUM_BARS; ++i) mbar_init(bar(i), i == C::ACC_EMPTY || i == C::ACC_EMPTY + 1 ? C::kCtas * kProdEpiWarps : 1);
+    for (int i = 0; i < C::NUM_BARS; ++i)
+      mbar_init(bar(i), i == C::ACC_EMPTY || i == C::ACC_EMPTY + 1 ? (PAIR ? 2 : 1) * kProdEpiWarps
+                        : i == C::RED_FULL || i == C::RED_FREE     ? KS * kProdEpiWarps
+                                                                   : 1);
     *abort_flag = 0;
     mbar_init_fence();
   }
@@ -324,12 +493,12 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
     }
   }
   tc_fence_before_sync();
-  if (PAIR) cluster_sync();
+  if (C::kCtas > 1) cluster_sync();
   else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_holder;
   pdl_wait();
-  const int first = blockIdx.x / C::kCtas, apart = gridDim.x / C::kCtas, units = p.steps * p.n * (2 * p.g_units + p.x_units);
+  const int first = p.from + blockIdx.x / C::kCtas, apart = gridDim.x / C::kCtas, units = p.to;
 
   if (warp < 4) {
     prod_regs_less<kProdOtherRegs>();
@@ -340,7 +509,7 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
         bool ok = true;
         for (int u = first; ok && u < units; u += apart) {
           const Unit w = unit_of(p, u);
-          const uint32_t need = w.after * (C::kCtas * kProdEpiWarps);
+          const uint32_t need = p.ordered ? 0 : w.after * (C::kCtas * kProdEpiWarps);
           if (load_acquire(p.done + w.batch) < need) {
             const uint64_t t0 = global_timer_ns();
 #pragma unroll 1
@@ -363,27 +532,29 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
           else if (p.wide) { a = p.b; b = p.x_mn[cur]; }
           else { a = p.x_k[cur]; b = p.b; }
           const int row_a = w.m * T + (int)rank * 128, row_b = w.n * T + (int)rank * 128;
-          for (int kb = 0; kb < w.blocks; ++kb, ++it) {
-            const uint32_t s = it % kStages, use = it / kStages;
-            if (use > 0 && !prod_wait(bar(C::EMPTY + s), (use - 1) & 1, abort_flag)) { ok = false; break; }
-            const uint32_t sa = a0 + s * C::kStageBytes, full = PAIR ? map_to_rank(bar(C::FULL + s), 0) : bar(C::FULL + s);
-            if (rank == 0) mbar_arrive_expect_tx(bar(C::FULL + s), C::kCtas * C::kStageBytes);
-            auto copy = [&](uint32_t dst, const CUtensorMap *m, int x, int y) {
-              if (PAIR) tma_load_3d_pair(dst, m, full, x, y, w.batch);
-              else tma_load_3d(dst, m, full, x, y, w.batch);
-            };
-            auto load = [&](uint32_t dst, const CUtensorMap *m, bool mn, int row) {
-              if (mn) {
-                copy(dst, m, row, kb * kProdK);
-                copy(dst + 8192, m, row + 64, kb * kProdK);
-              } else {
-                copy(dst, m, kb * kProdK, row);
-              }
-            };
-            load(sa + 2 * C::kTileBytes, a + 1, mn_a, row_a);
-            load(sa + C::kTileBytes, b, mn_b, row_b);
-            load(sa, a, mn_a, row_a);
-            load(sa + 3 * C::kTileBytes, b + 1, mn_b, row_b);
+          const int kb0 = first_block(w.blocks), kb1 = kb0 + my_blocks(w.blocks);
+          for (int kb = kb0; ok && kb < kb1; ++kb) {
+#pragma unroll
+            for (int lo = 1; lo >= 0; --lo, ++it) {
+              const uint32_t s = it % kSlots, use = it / kSlots;
+              if (use > 0 && !prod_wait(bar(C::EMPTY + s), (use - 1) & 1, abort_flag)) { ok = false; break; }
+              const uint32_t sa = a0 + s * C::kSlotBytes, full = PAIR ? map_to_rank(bar(C::FULL + s), 0) : bar(C::FULL + s);
+              if (rank == 0) mbar_arrive_expect_tx(bar(C::FULL + s), (PAIR ? 2 : 1) * C::kSlotBytes);
+              auto copy = [&](uint32_t dst, const CUtensorMap *m, int x, int y) {
+                if (PAIR) tma_load_3d_pair(dst, m, full, x, y, w.batch);
+                else tma_load_3d(dst, m, full, x, y, w.batch);
+              };
+              auto load = [&](uint32_t dst, const CUtensorMap *m, bool mn, int row) {
+                if (mn) {
+                  copy(dst, m, row, kb * kProdK);
+                  copy(dst + 8192, m, row + 64, kb * kProdK);
+                } else {
+                  copy(dst, m, kb * kProdK, row);
+                }
+              };
+              load(sa, a + lo, mn_a, row_a);
+              load(sa + C::kTileBytes, b + lo, mn_b, row_b);
+            }
           }
         }
       }
@@ -405,22 +576,25 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
             else mma_f16_ss(d, da + k * step_a, db + k * step_b, idesc, fresh && k == 0 ? 0u : 1u);
           }
         };
-        for (int kb = 0; kb < w.blocks; ++kb, ++it) {
-          const uint32_t acc = it & 1, d = tmem + acc * T, s = it % kStages, sa = a0 + s * C::kStageBytes;
+        const int blocks = my_blocks(w.blocks);
+        for (int kb = 0; kb < blocks; ++kb, ++it) {
+          const uint32_t acc = it & 1, d = tmem + acc * T, s_lo = (2 * it) % kSlots, s_hi = (2 * it + 1) % kSlots;
+          const uint32_t lo = a0 + s_lo * C::kSlotBytes, hi = a0 + s_hi * C::kSlotBytes;
+          auto commit = [&](int id) {
+            if (PAIR) mma_commit_pair(bar(id));
+            else mma_commit(bar(id));
+          };
           if (it >= 2 && !prod_wait_warp(bar(C::ACC_EMPTY + acc), ((it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
-          if (!prod_wait_warp(bar(C::FULL + s), (it / kStages) & 1, abort_flag)) { ok = false; break; }
+          if (!prod_wait_warp(bar(C::FULL + s_lo), ((2 * it) / kSlots) & 1, abort_flag) ||
+              !prod_wait_warp(bar(C::FULL + s_hi), ((2 * it + 1) / kSlots) & 1, abort_flag)) { ok = false; break; }
           tc_fence_after_sync();
           if (elect_one()) {
-            issue(d, sa + 2 * C::kTileBytes, sa + C::kTileBytes, true);
-            issue(d, sa, sa + 3 * C::kTileBytes, false);
-            issue(d, sa, sa + C::kTileBytes, false);
-            if (PAIR) {
-              mma_commit_pair(bar(C::EMPTY + s));
-              mma_commit_pair(bar(C::ACC_FULL + acc));
-            } else {
-              mma_commit(bar(C::EMPTY + s));
-              mma_commit(bar(C::ACC_FULL + acc));
-            }
+            issue(d, lo, hi + C::kTileBytes, true);
+            issue(d, hi, lo + C::kTileBytes, false);
+            commit(C::EMPTY + s_lo);
+            issue(d, hi, hi + C::kTileBytes, false);
+            commit(C::EMPTY + s_hi);
+            commit(C::ACC_FULL + acc);
           }
           __syncwarp();
         }
@@ -430,29 +604,31 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
     // ------------------------------------------------------------ sums and results
     prod_regs_more<kProdEpiRegs>();
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    constexpr int kGroups = T / 64;
+    constexpr int kSums = T / 64, W = C::W, kGroups = C::kGroups;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * (T / 2);
-    float4 *slab = reinterpret_cast<float4 *>(smem + C::kSmemStaging + (warp - 4) * kProdSlabBytes);
-    uint32_t j = 0;
+    float4 *slab = reinterpret_cast<float4 *>(smem + C::kSmemStaging + (KS > 1 ? 0 : (warp - 4) * kProdSlabBytes));
+    const int local = quarter * 32 + lane;  // row of the tile's 128
+    uint32_t j = 0, turn = 0;
     bool ok = true;
-    for (int u = first; ok && u < units; u += apart) {
+    for (int u = first; ok && u < units; u += apart, ++turn) {
       const Unit w = unit_of(p, u);
-      float sum[kGroups][32];
+      float sum[kSums][32];
 #pragma unroll
-      for (int cg = 0; cg < kGroups; ++cg)
+      for (int cg = 0; cg < kSums; ++cg)
 #pragma unroll
         for (int x = 0; x < 32; ++x) sum[cg][x] = 0.0f;
+      const int blocks = my_blocks(w.blocks);
 #pragma unroll 1
-      for (int kb = 0; kb < w.blocks; ++kb, ++j) {
+      for (int kb = 0; kb < blocks; ++kb, ++j) {
         const uint32_t acc = j & 1;
         if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j >> 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after_sync();
 #pragma unroll
-        for (int cg = 0; cg < kGroups; ++cg) {
+        for (int cg = 0; cg < kSums; ++cg) {
           uint32_t r[32];
           tmem_ld32(lane_base + acc * T + cg * 32, r);
           tmem_wait_ld();
-          if (cg == kGroups - 1) {
+          if (cg == kSums - 1) {
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
@@ -469,34 +645,93 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
         }
       }
       if (!ok) break;
-      const uint32_t row0 = (uint32_t)(w.m * T + (int)rank * 128 + quarter * 32), row = row0 + lane, col0 = (uint32_t)(w.n * T + half * (T / 2));
+      if constexpr (KS > 1) {
+        // ---------------------------------------------------------- partial sums meet at the CTAs that own their columns, and are added in the order of the slices
+        constexpr int OW = C::kOwned, kQuads = OW / 4;
+        auto place = [&](int slice, int quad) {  // of 16 bytes; 8 lanes' places fall into different banks
+          const int s = OW >= 32 ? (local & 7) : ((local >> 1) & 3);
+          return (slice * 128 + local) * kQuads + (quad ^ s);
+        };
+        const uint32_t in_rows = (w.product == kNext ? p.rows : p.side) - (uint32_t)(w.m * T), in_cols = (w.product == kNext ? p.cols : p.side) - (uint32_t)(w.n * T);
+        if (turn > 0 && !wait_cluster(bar(C::RED_FREE), (turn - 1) & 1, abort_flag)) { ok = false; break; }
+#pragma unroll
+        for (int cg = 0; cg < kSums; ++cg)
+#pragma unroll
+          for (int x = 0; x < 32; x += 4) {
+            const int c = half * (T / 2) + cg * 32 + x, owner = c / OW;
+            if ((uint32_t)local >= in_rows || (uint32_t)c >= in_cols) continue;  // zeros that nobody writes
+            const uint32_t dst = map_to_rank(a0 + C::kSmemStaging + place((int)part, (c - owner * OW) / 4) * 16, (uint32_t)owner);
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(sum[cg][x]), "f"(sum[cg][x + 1]), "f"(sum[cg][x + 2]), "f"(sum[cg][x + 3])
+                         : "memory");
+          }
+        __syncwarp();
+        if (lane < KS) mbar_arrive_cluster(map_to_rank(bar(C::RED_FULL), lane));
+        if (!wait_cluster(bar(C::RED_FULL), turn & 1, abort_flag)) { ok = false; break; }
+#pragma unroll
+        for (int cg = 0; cg < kGroups; ++cg)
+#pragma unroll
+          for (int x = 0; x < W; x += 4) {
+            const int quad = (half * (OW / 2) + cg * W + x) / 4;
+            float4 v = slab[place(0, quad)];
+#pragma unroll
+            for (int k = 1; k < KS; ++k) {
+              const float4 q = slab[place(k, quad)];
+              v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+            }
+            sum[cg][x] = v.x;
+            sum[cg][x + 1] = v.y;
+            sum[cg][x + 2] = v.z;
+            sum[cg][x + 3] = v.w;
+          }
+        __syncwarp();
+        if (lane < KS) mbar_arrive_cluster(map_to_rank(bar(C::RED_FREE), lane));
+      }
+      const uint32_t row0 = (uint32_t)(w.m * T + (int)rank * 128 + quarter * 32), row = row0 + lane;
+      const uint32_t col0 = (uint32_t)(w.n * T + (int)part * C::kOwned + half * (C::kOwned / 2));
       if (w.product == kPolynomial) {  // what it reads of G: the copies have been waited for, these loads as well
         (void)load_acquire(p.done + w.batch);
         __syncwarp();
       }
-      if (w.product != kNext) {
+      const bool last = w.product == kNext && w.step + 1 == p.steps;
+      const int next = (w.step + 1) & 1;
+      if constexpr (KS == 1) {
+        uint4 *slab16 = reinterpret_cast<uint4 *>(slab);
 #pragma unroll
-        for (int cg = 0; cg < kGroups; ++cg) symmetric_block(p, w, row, col0 + cg * 32, sum[cg]);
-      } else if (w.step + 1 < p.steps) {
-        const int next = (w.step + 1) & 1;
+        for (int cg = 0; cg < kGroups; cg += 2) {
+          const uint32_t c = col0 + cg * W;
+          float(&v)[64] = reinterpret_cast<float(&)[64]>(sum[cg]);
+          if (w.product != kNext) {
+            symmetric_64(p, w, slab16, lane, row0, c, v);
+          } else if (!last) {
+            if (c < p.cols && row0 < p.rows) {
 #pragma unroll
-        for (int cg = 0; cg < kGroups; ++cg) {
-          const uint32_t c = col0 + cg * 32;
-          if (c >= p.cols || row >= p.rows) continue;
-#pragma unroll
-          for (int x = 0; x < 32; ++x) sum[cg][x] *= kPartInverse;
-          write_parts(p.x[next][0], p.x[next][1], (size_t)w.batch * p.x_matrix + (size_t)row * p.x_pitch + c, sum[cg]);
+              for (int x = 0; x < 64; ++x) v[x] *= kPartInverse;
+              next_block(p.x[next], (size_t)w.batch * p.x_matrix + (size_t)row0 * p.x_pitch + c, p.x_pitch, slab16, lane, p.rows - row0, v);
+            }
+          } else {
+            last_block(p, w, slab, lane, row0, c, sum[cg]);
+            last_block(p, w, slab, lane, row0, c + W, sum[cg + 1]);
+          }
         }
       } else {
+        float(&v)[W] = reinterpret_cast<float(&)[W]>(sum[0]);
+        if (w.product != kNext) {
+          symmetric_block<W>(p, w, row, col0, v);
+        } else if (!last) {
+          if (col0 < p.cols && row < p.rows) {
 #pragma unroll
-        for (int cg = 0; cg < kGroups; ++cg) last_block(p, w, slab, lane, row0, col0 + cg * 32, sum[cg]);
+            for (int x = 0; x < W; ++x) v[x] *= kPartInverse;
+            write_parts<W>(p.x[next][0], p.x[next][1], (size_t)w.batch * p.x_matrix + (size_t)row * p.x_pitch + col0, v);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < W; x += 4)
+            if (row < p.rows && col0 + x < p.cols) last_four(p, p.t.out[w.batch], row, col0 + x, make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]));
+        }
       }
       fence_proxies();
       __syncwarp();
-      if (lane == 0) {
-        __threadfence();
-        asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(p.done + w.batch), "r"(1u) : "memory");
-      }
+      if (lane == 0) asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(p.done + w.batch), "r"(1u) : "memory");
     }
   }
 
@@ -521,7 +756,7 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
     if (threadIdx.x == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
     __syncthreads();
   }
-  if (PAIR) cluster_sync();
+  if (C::kCtas > 1) cluster_sync();  // no CTA leaves while another may still signal its barriers or write to its shared memory
   if (warp == 1) {
     tc_fence_after_sync();
     if (PAIR) tmem_dealloc_pair(tmem, C::kTmemCols);
@@ -585,8 +820,9 @@ struct Plan {
   Layout l;
   cudaStream_t s;
 
+  // All products of all steps in one launch (step < 0), or one product of a step.
   template <class C>
-  int products(uint32_t n, NsParams &p) const {
+  int products(uint32_t n, NsParams &p, int step, Product which) const {
     auto tiles = [](uint32_t v) { return (int)((v + C::T - 1) / C::T); };
     p.side_tiles = tiles(l.side);
     p.x_m_tiles = tiles(rows);
@@ -595,14 +831,28 @@ struct Plan {
     p.x_units = p.x_m_tiles * p.x_n_tiles;
     const int slots = cluster_slots<k_newton_schulz<C>>(C::kCtas, C::kSmemTotal, kProdLaunchRegs);
     if (slots == 0) return DF_ERR_CUDA;
-    const long long most = (long long)n * (p.g_units > p.x_units ? p.g_units : p.x_units);
+    const int per_step = (int)n * (2 * p.g_units + p.x_units);
+    long long most = (long long)n * (p.g_units > p.x_units ? p.g_units : p.x_units);
+    p.from = 0;
+    p.to = (int)steps * per_step;
+    p.ordered = step >= 0;
+    if (step >= 0) {
+      p.from = step * per_step + (which == kGram ? 0 : which == kPolynomial ? 1 : 2) * (int)n * p.g_units;
+      p.to = p.from + (int)n * (which == kNext ? p.x_units : p.g_units);
+      most = p.to - p.from;
+    }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeCooperative;
-    attr[0].val.cooperative = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = C::kCtas;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C::kCtas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    if (step < 0) {
+      attr[1].id = cudaLaunchAttributeCooperative;
+      attr[1].val.cooperative = 1;
+    } else {
+      attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[1].val.programmaticStreamSerializationAllowed = option(DF_OPT_PDL) != 0;
+    }
     cfg.gridDim = dim3((unsigned)((most < slots ? most : slots) * C::kCtas));
     cfg.blockDim = dim3(kProdThreads);
     cfg.dynamicSmemBytes = C::kSmemTotal;
@@ -612,6 +862,23 @@ struct Plan {
     const int st = check_cuda(cudaLaunchKernelEx(&cfg, k_newton_schulz<C>, p));
     note_launch();
     return st;
+  }
+  int products(int form, uint32_t n, NsParams &p, int step, Product which) const {
+    switch (form) {
+      case 0: return products<NsCfg<true, 1>>(n, p, step, which);
+      case 1: return products<NsCfg<false, 1>>(n, p, step, which);
+      case 2: return products<NsCfg<false, 2>>(n, p, step, which);
+      default: return products<NsCfg<false, 4>>(n, p, step, which);
+    }
+  }
+
+  // Time of a product in us in a form (tiles of t x t on clusters of `ctas`, the contraction cut in ks), without what comes between products.
+  double estimate(uint32_t n, int form, Product which) const {
+    const uint64_t t = form == 0 ? 256 : 128, ks = form < 2 ? 1 : (form == 2 ? 2 : 4), ctas = form == 0 ? 2 : ks, slots = 148 / ctas;
+    const uint64_t m = (l.side + t - 1) / t, x = ((rows + t - 1) / t) * ((cols + t - 1) / t), g = m * (m + 1) / 2;
+    const uint64_t k = which == kGram ? (rows > cols ? rows : cols) : l.side, blocks = ((k + 63) / 64 + ks - 1) / ks;
+    const uint64_t waves = ((which == kNext ? x : g) * n + slots - 1) / slots;
+    return (double)waves * ((double)blocks * (form == 0 ? 1.4 : 0.9) + (form == 0 ? 4.0 : ks > 1 ? 5.0 : 1.0));
   }
 
   int run(uint32_t n, UpdateParams u, NsParams p) const {
@@ -638,11 +905,11 @@ struct Plan {
     u.cols = cols;
     u.pitch = l.x_pitch;
     u.eps = eps;
-    int st = check_cuda(launch_kernel(k_update, dim3(kNormBlocks, n), dim3(256), 0, s, u));
+    const uint32_t each = (uint32_t)(1184 / n), quarter = (uint32_t)(((uint64_t)rows * cols + 4095) / 4096), sums = quarter < each ? quarter : each;
+    const uint32_t blocks = sums < 1 ? 1 : (sums < (uint32_t)kNormBlocks ? sums : (uint32_t)kNormBlocks);
+    int st = check_cuda(launch_kernel(k_update, dim3(blocks, n), dim3(256), 0, s, u));
     if (st != DF_OK) return st;
-    const uint64_t quads = (uint64_t)rows * (l.x_pitch / 4);
-    const uint32_t blocks = (uint32_t)((quads + 255) / 256 < 512 ? (quads + 255) / 256 : 512);
-    st = check_cuda(launch_kernel(k_normalise, dim3(blocks, n), dim3(256), 0, s, u));
+    st = check_cuda(launch_kernel(k_normalise, dim3((rows + 7) / 8 < 4 * each ? (rows + 7) / 8 : 4 * each, n), dim3(256), 0, s, u, (int)blocks));
     note_launch(2);
     if (st != DF_OK) return st;
     p.x_matrix = l.x_matrix;
@@ -659,12 +926,34 @@ struct Plan {
     p.b_ = b;
     p.c = c * kPartInverse;
     p.status = device_status_ptr();
-    // Of a block of 64 a pair takes about 1536 cycles for 256 x 256 (its products), one CTA about 1150 for 128 x 128 (its operands' copies).
-    auto waves = [&](uint64_t t, uint64_t slots) {
-      const uint64_t m = (l.side + t - 1) / t, x = ((rows + t - 1) / t) * ((cols + t - 1) / t), g = m * (m + 1) / 2, larger = rows > cols ? rows : cols;
-      return ((g * n + slots - 1) / slots) * (larger + l.side) + ((x * n + slots - 1) / slots) * l.side;
-    };
-    return waves(256, 74) * 1536 < waves(128, 148) * 1150 ? products<NsCfg<true>>(n, p) : products<NsCfg<false>>(n, p);
+    // One launch with one form for everything, about 5 us between products (fences, a counter, first copies), or a launch a product with the form that suits
+    // each, about 8 between.
+    const Product all[3] = {kGram, kPolynomial, kNext};
+    double one = 1e300, own = 0.0;
+    int one_form = 0, own_form[3] = {0, 0, 0};
+    for (int f = 0; f < 4; ++f) {
+      double t = 0.0;
+      for (Product q : all) t += estimate(n, f, q) + 5.0;
+      if (t < one) {
+        one = t;
+        one_form = f;
+      }
+    }
+    for (int i = 0; i < 3; ++i) {
+      double best = 1e300;
+      for (int f = 0; f < 4; ++f) {
+        const double t = estimate(n, f, all[i]) + 8.0;
+        if (t < best) {
+          best = t;
+          own_form[i] = f;
+        }
+      }
+      own += best;
+    }
+    if (one <= own) return products(one_form, n, p, -1, kGram);
+    for (uint32_t i = 0; st == DF_OK && i < steps; ++i)
+      for (int q = 0; st == DF_OK && q < 3; ++q) st = products(own_form[q], n, p, (int)i, all[q]);
+    return st;
   }
 };
 
@@ -710,13 +999,15 @@ int df_orthogonalize(const void *update, void *out, void *workspace, uint64_t wo
     NsParams last = {};
     u.row_stride = update_row_stride;
     u.bf16 = bf16 != 0;
+    u.vec = 1;
     last.out_stride = out_row_stride;
     last.out_bf16 = bf16 != 0;
     last.vec = 1;
     for (uint32_t i = 0; i < k; ++i) {
       u.t.source[i] = static_cast<const uint8_t *>(update) + (i0 + i) * update_matrix_stride * elt;
       last.t.out[i] = static_cast<uint8_t *>(out) + (i0 + i) * out_matrix_stride * elt;
-      if (!aligned(last.t.out[i], out_row_stride * elt, bf16 ? 8 : 16)) last.vec = 0;
+      if (!aligned(last.t.out[i], rows > 1 ? out_row_stride * elt : 0, bf16 ? 8 : 16)) last.vec = 0;
+      if (!aligned(u.t.source[i], rows > 1 ? update_row_stride * elt : 0, bf16 ? 8 : 16)) u.vec = 0;
     }
     st = plan.run(k, u, last);
   }
@@ -754,6 +1045,7 @@ int df_muon_update(const void *tensors, uint32_t n, uint32_t rows, uint32_t cols
     UpdateParams u = {};
     NsParams last = {};
     u.row_stride = cols;
+    u.vec = 1;
     u.beta = momentum;
     u.nesterov = nesterov != 0;
     last.out_stride = cols;
@@ -765,7 +1057,9 @@ int df_muon_update(const void *tensors, uint32_t n, uint32_t rows, uint32_t cols
       u.t.source[i] = t[i0 + i].gradient;
       u.t.momentum[i] = t[i0 + i].momentum;
       last.t.out[i] = t[i0 + i].parameter;
-      if (!aligned(last.t.out[i], (uint64_t)cols * 4, 16)) last.vec = 0;
+      if (!aligned(last.t.out[i], rows > 1 ? (uint64_t)cols * 4 : 0, 16)) last.vec = 0;
+      if (!aligned(u.t.source[i], 0, 16) || !aligned(u.t.momentum[i], 0, 16)) u.vec = 0;
+      if (rows > 1 && cols % 4 != 0) u.vec = 0;
     }
     st = plan.run(k, u, last);
   }

@@ -5,16 +5,16 @@
 // where |x| is within 2^18 of the largest that s was chosen for, and nothing below 2^-40 of that one. Then
 //   A B = A_lo B_hi + A_hi B_lo + A_hi B_hi      (A_lo B_lo, 2^-24 of it, is left out)
 // is three products in that order: the tensor cores cut sums off instead of rounding them, and a large sum is cut off at each of its
-// additions, so the small terms come first and every 64 of the contraction the sum is taken out to registers and added up rounded.
-// (Taken out every 768 a loss of 2048 rows of 768 was 2e-6 off 64 bits and orthogonalised 768 x 768 1.2e-5, every 192 6e-7 and 3.8e-6, every 64 1.4e-7 and
-// 1.6e-6, where sums in fp32 registers have 6e-7 and 2.3e-6.)
+// additions, so the small terms come first and every CHUNK blocks of 64 the sum is taken out to registers and added up rounded.
 //
 // One persistent kernel, at most one CTA an SM, 384 threads:
 //   warp 0       copies: a ring of stages, each 64 of the contraction: 128 rows of A and this CTA's rows of B (PARTS = 2: both parts), 128-byte swizzle;
 //   warp 1       issues the products into one of two accumulators in tensor memory;
 //   warps 4-11   the epilogue of one tile under the products of the next: a warp has the 32 rows of its quarter of tensor memory, a row
-//                a lane, and half of the tile's columns, 32 at a time. With PARTS = 2 its sums are 128 registers a thread, which it takes over from warps 0-3.
+//                a lane, and half of the tile's columns, 32 at a time. With CHUNK its sums are 128 registers a thread, which it takes over from warps 0-3.
 // The tile is 256 x 256 over a pair of CTAs (cta_group::2): 32 KB a CTA and part for 512 cycles of products.
+// Tiles that run at the same time share the operand with the more rows (K-major B: the output weight, by the tiles of all rows; MN-major B: the gradient of the
+// logits, by the tiles of the width): it is read from HBM once.
 // The contraction can be split: tile z * tiles + t is slice z of tile t, and the epilogue is told z.
 #pragma once
 
@@ -45,7 +45,7 @@ struct ProductTile {
 
 constexpr int kProdEpiWarps = 8, kProdThreads = 384, kProdK = 64;
 constexpr uint32_t kProdSlabBytes = 32 * 128;  // a warp's staging slab: 32 rows of 128 bytes
-// PARTS = 2: the launch gives 168 registers to each thread of three warpgroups; the two of the epilogue take over 48 from each thread of the first.
+// Sums in registers: the launch gives 168 registers to each thread of three warpgroups; the two of the epilogue take over 48 from each thread of the first.
 constexpr int kProdLaunchRegs = 168, kProdEpiRegs = 216, kProdOtherRegs = 72;
 static_assert(2 * kProdEpiRegs + kProdOtherRegs <= 3 * kProdLaunchRegs, "setmaxnreg waits for registers that the block was not launched with");
 template <int N> __device__ __forceinline__ void prod_regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -70,11 +70,13 @@ __device__ __forceinline__ bool prod_wait_warp(uint32_t bar, uint32_t parity, vo
   return __all_sync(0xffffffffu, prod_wait(bar, parity, abort_flag)) != 0;
 }
 
-template <bool A_MN_, bool B_MN_, int PARTS_>
+template <bool A_MN_, bool B_MN_, int PARTS_, int CHUNK_>
 struct ProdCfg {
   static constexpr bool A_MN = A_MN_, B_MN = B_MN_;
   static constexpr int PARTS = PARTS_;
   static constexpr int TM = 256, TN = 256;
+  static constexpr bool kSums = CHUNK_ > 0;                        // sums in registers
+  static constexpr int kChunk = kSums ? CHUNK_ : 0x40000000;  // blocks between takings out
   static constexpr uint32_t kTileBytes = 128 * kProdK * 2, kStageBytes = 2 * PARTS * kTileBytes;  // A hi, B hi (, A lo, B lo)
   static constexpr int kStages = PARTS == 2 ? 3 : 6;
   static constexpr uint32_t kSmemStaging = kStages * kStageBytes;
@@ -127,15 +129,15 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
     ProductTile t;
     const int per_split = p.m_tiles * p.n_tiles, r = (int)(id % per_split);
     t.split = (int)(id / per_split);
-    t.m_tile = r / p.n_tiles;
-    t.n_tile = r % p.n_tiles;
+    t.m_tile = C::B_MN ? r / p.n_tiles : r % p.m_tiles;
+    t.n_tile = C::B_MN ? r % p.n_tiles : r / p.m_tiles;
     *kb0 = t.split * p.kb_per_split;
     *kb1 = *kb0 + p.kb_per_split < p.n_kb ? *kb0 + p.kb_per_split : p.n_kb;
     return t;
   };
 
   if (warp < 4) {
-    if constexpr (C::PARTS == 2) prod_regs_less<kProdOtherRegs>();
+    if constexpr (C::kSums) prod_regs_less<kProdOtherRegs>();
     if (warp == 0) {
       // ---------------------------------------------------------- copies: each CTA its own rows
       if (lane == 0) {
@@ -188,14 +190,14 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         decode(id, &kb0, &kb1);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const uint32_t acc = j & 1, d = tmem + acc * TN, s = it % kStages, sa = a0 + s * C::kStageBytes;
-          // an accumulator is taken out after every block (PARTS = 2), or at the end of the tile
-          const bool first = C::PARTS == 2 || kb == kb0, last = C::PARTS == 2 || kb + 1 == kb1;
+          // an accumulator is taken out after every kChunk blocks, or at the end of the tile
+          const bool first = (kb - kb0) % C::kChunk == 0, last = (kb - kb0) % C::kChunk == C::kChunk - 1 || kb + 1 == kb1;
           if (first && j >= 2 && !prod_wait_warp(bar(C::ACC_EMPTY + acc), ((j >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
           if (!prod_wait_warp(bar(C::FULL + s), (it / kStages) & 1, abort_flag)) { ok = false; break; }
           tc_fence_after_sync();
           if (elect_one()) {
             if constexpr (C::PARTS == 2) {
-              issue(d, sa + 2 * C::kTileBytes, sa + C::kTileBytes, true);
+              issue(d, sa + 2 * C::kTileBytes, sa + C::kTileBytes, first);
               issue(d, sa, sa + 3 * C::kTileBytes, false);
               issue(d, sa, sa + C::kTileBytes, false);
             } else {
@@ -211,7 +213,7 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    if constexpr (C::PARTS == 2) prod_regs_more<kProdEpiRegs>();
+    if constexpr (C::kSums) prod_regs_more<kProdEpiRegs>();
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     constexpr int kGroups = TN / 64;  // 32-column blocks of this warp
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * (TN / 2);
@@ -228,7 +230,7 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
       const ProductTile t = decode(id, &kb0, &kb1);
       const uint32_t row = (uint32_t)(t.m_tile * C::TM + (int)rank * 128 + quarter * 32 + lane), col0 = (uint32_t)(t.n_tile * TN + half * (TN / 2));
       epi.begin(t, row, col0);
-      if constexpr (C::PARTS == 1) {
+      if constexpr (!C::kSums) {
         const uint32_t acc = j & 1;
         if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j >> 1) & 1, abort_flag)) break;
         tc_fence_after_sync();
@@ -251,7 +253,7 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
 #pragma unroll
           for (int x = 0; x < 32; ++x) sum[cg][x] = 0.0f;
 #pragma unroll 1
-        for (int kb = kb0; kb < kb1; ++kb, ++j) {
+        for (int kb = kb0; kb < kb1; kb += C::kChunk, ++j) {
           const uint32_t acc = j & 1;
           if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j >> 1) & 1, abort_flag)) { ok = false; break; }
           tc_fence_after_sync();
@@ -388,7 +390,7 @@ int cluster_slots(uint32_t ctas, uint32_t smem, int regs) {
 template <class C, class Epi>
 int launch_product(const Operand &a, const Operand &b, ProductParams p, const typename Epi::Params &e, cudaStream_t s) {
   static_assert(sizeof(ProductParams) + sizeof(typename Epi::Params) + 4 * sizeof(CUtensorMap) < 4000, "kernel parameters");
-  const int slots = cluster_slots<k_product<C, Epi>>(2, C::kSmemTotal, C::PARTS == 2 ? kProdLaunchRegs : 0);
+  const int slots = cluster_slots<k_product<C, Epi>>(2, C::kSmemTotal, C::kSums ? kProdLaunchRegs : 0);
   if (slots == 0) return DF_ERR_CUDA;
   p.m_tiles = (int)((p.M + C::TM - 1) / C::TM);
   p.n_tiles = (int)((p.N + C::TN - 1) / C::TN);
