@@ -19,10 +19,9 @@ namespace {
 using namespace ptx;
 
 constexpr float kGScale = 16384.0f;  // G is stored times 2^14
-// Blocks of 64 between takings out of sums. fp32 calls: 3 (the loss of 2048 rows, width 768: every 2 409 us and 3.8e-7 off 64 bits, every 3 390 and 6.6e-7, where fp32
-// registers have 6.1e-7). The loss of bf16 calls: none up to a width of 768 (4096 rows: 198 us, 1.0e-6; every 6 blocks 244, every 4 289 and 3.2e-7), 12 above
-// (210 us at 768).
-constexpr int kChunk = 3, kChunkBf16 = 12;
+// Blocks of 64 between takings out of the sums of a bf16 call's logits where the loss is wanted: none up to a width of 768 (4096 rows: 198 us, 1.0e-6 off 64 bits; every
+// 6 blocks 244, every 4 289 and 3.2e-7), 12 above (210 us at 768).
+constexpr int kChunkBf16 = 12;
 constexpr uint64_t kPieceBytes = 256ull << 20;  // of G, or of a piece's weight in parts
 
 int finish(int st) {
@@ -690,7 +689,7 @@ struct HeadCall {
       e.slot_base = slots;
       slots += (n + 127) / 128;
       if (st == DF_OK)
-        st = !bf16 ? product<false, false, 2, kChunk, LseEpi>(a, b, rows, n, width, 1, false, e, s)
+        st = !bf16 ? product<false, false, 2, 0, LseEpi>(a, b, rows, n, width, 1, false, e, s)
              : width <= kChunkBf16 * kProdK ? product<false, false, 1, 0, LseEpi>(a, b, rows, n, width, 1, true, e, s)
                                             : product<false, false, 1, kChunkBf16, LseEpi>(a, b, rows, n, width, 1, true, e, s);
     }
@@ -737,7 +736,7 @@ struct HeadCall {
       e.pitch = l.piece;
       e.col_base = c0;
       e.all_cols = vocab;
-      if (st == DF_OK) st = product<false, false, PARTS, PARTS == 2 ? kChunk : 0, GradEpi<PARTS>>(a, b, rows, n, width, 1, bf16, e, s);
+      if (st == DF_OK) st = product<false, false, PARTS, 0, GradEpi<PARTS>>(a, b, rows, n, width, 1, bf16, e, s);
       const Operand g = {e.g, e.g_lo, false, rows, n, l.piece};
       if (st == DF_OK && d_x) {
         if (c0 == 0) splits = slices((n + kProdK - 1) / kProdK, splits);
@@ -748,7 +747,7 @@ struct HeadCall {
         o.add = c0 > 0;
         o.rows = rows;
         o.cols = width;
-        st = product<false, true, PARTS, PARTS == 2 ? kChunk : 0, OutEpi>(g, wp, rows, width, n, splits, false, o, s);
+        st = product<false, true, PARTS, 0, OutEpi>(g, wp, rows, width, n, splits, false, o, s);
       }
       if (st == DF_OK && d_w) {
         OutEpi::Params o = {};
@@ -760,7 +759,7 @@ struct HeadCall {
         o.scale = scale;
         o.rows = n;
         o.cols = width;
-        st = product<true, true, PARTS, PARTS == 2 ? kChunk : 0, OutEpi>(g, packed(l.x_grad, rows, false), n, width, rows, 1, false, o, s);
+        st = product<true, true, PARTS, 0, OutEpi>(g, packed(l.x_grad, rows, false), n, width, rows, 1, false, o, s);
       }
     }
     if (st != DF_OK || !d_x) return st;

@@ -20,7 +20,7 @@ using namespace ptx;
 
 constexpr float kPartScale = 4096.0f, kPartInverse = 1.0f / 4096.0f;
 constexpr int kMostMatrices = 64;               // of a group: what the kernels' tables of pointers hold
-constexpr uint64_t kGroupBytes = 512ull << 20;  // of workspace, beyond one matrix
+constexpr uint64_t kGroupBytes = 192ull << 20;  // of workspace, beyond one matrix: what L2 loses between products is read again
 constexpr int kNormBlocks = 256;                // partial sums of squares per matrix, at most
 constexpr uint32_t kMostTensors = 1024;         // of an optimiser step: every pair is checked for overlap
 
@@ -149,11 +149,12 @@ __global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ Updat
 }
 
 // ---------------------------------------------------------------- the products
-// PAIR: tiles of 256 x 256 over two CTAs. Else 128 x 128, the contraction cut among KS CTAs of a cluster.
-template <bool PAIR_, int KS_>
+// Tiles of 128 x 128, the contraction cut among KS CTAs of a cluster. (Tiles of 256 x 256 over a pair of CTAs, whose operands are half the bytes, took 119 us for
+// 64 x 64 where these take 79, 371 and 242 for 768 x 768, 1839 and 1923 for 48 of them: a tile's 128 sums a thread leave no room to write one tile's results
+// while the next is added up.)
+template <int KS_>
 struct NsCfg {
-  static constexpr bool PAIR = PAIR_;
-  static constexpr int KS = KS_, kCtas = PAIR ? 2 : KS, T = PAIR ? 256 : 128;
+  static constexpr int KS = KS_, T = 128;
   static constexpr int kOwned = T / KS, W = kOwned / 2 < 32 ? kOwned / 2 : 32, kGroups = kOwned / 2 / W;  // columns of a CTA's results; of a warp, W at a time
   static constexpr uint32_t kTileBytes = 128 * kProdK * 2, kSlotBytes = 2 * kTileBytes;  // a slot: A and B, low or high parts, in turn
   static constexpr int kSlots = KS > 1 ? 5 : 6;
@@ -161,10 +162,10 @@ struct NsCfg {
   static constexpr uint32_t kSmemStaging = kSlots * kSlotBytes, kStagingBytes = KS > 1 ? 128 * 128 * 4 : kProdEpiWarps * kProdSlabBytes;
   static constexpr uint32_t kSmemBars = kSmemStaging + kStagingBytes;
   static constexpr uint32_t kSmemTotal = kSmemBars + 256 + 1024;
-  static constexpr uint32_t kTmemCols = 2 * T;
-  static constexpr int FULL = 0, EMPTY = FULL + kSlots, ACC_FULL = EMPTY + kSlots, ACC_EMPTY = ACC_FULL + 2, RED_FULL = ACC_EMPTY + 2, RED_FREE = RED_FULL + 1,
+  static constexpr int kAccs = 4;  // accumulators of 128 columns: so many blocks of the next tile run while results of this one are written
+  static constexpr int FULL = 0, EMPTY = FULL + kSlots, ACC_FULL = EMPTY + kSlots, ACC_EMPTY = ACC_FULL + kAccs, RED_FULL = ACC_EMPTY + kAccs, RED_FREE = RED_FULL + 1,
                        DRAIN = RED_FREE + 1, NUM_BARS = DRAIN + 1;
-  static_assert(NUM_BARS * 8 <= 192 && kSmemTotal <= 227 * 1024 && (!PAIR || KS == 1), "shared memory");
+  static_assert(NUM_BARS * 8 <= 240 && kSmemTotal <= 227 * 1024, "shared memory");
 };
 
 struct NsParams {
@@ -462,43 +463,37 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, vola
 template <class C>
 __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_constant__ NsParams p) {
   constexpr int kSlots = C::kSlots, T = C::T, KS = C::KS;
-  constexpr bool PAIR = C::PAIR;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t a0 = smem_u32(smem);
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kSmemBars);
-  volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + C::kSmemBars + 192);
-  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(smem + C::kSmemBars + 196);
+  volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + C::kSmemBars + 240);
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(smem + C::kSmemBars + 244);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_rank() : 0, part = KS > 1 ? cluster_rank() : 0;
+  const uint32_t part = KS > 1 ? cluster_rank() : 0;
   auto bar = [&](int id) { return smem_u32(&bars[id]); };
   auto first_block = [&](int blocks) { return (int)part * blocks / KS; };
   auto my_blocks = [&](int blocks) { return ((int)part + 1) * blocks / KS - (int)part * blocks / KS; };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::NUM_BARS; ++i)
-      mbar_init(bar(i), i == C::ACC_EMPTY || i == C::ACC_EMPTY + 1 ? (PAIR ? 2 : 1) * kProdEpiWarps
+      mbar_init(bar(i), i >= C::ACC_EMPTY && i < C::RED_FULL ? kProdEpiWarps
                         : i == C::RED_FULL || i == C::RED_FREE     ? KS * kProdEpiWarps
                                                                    : 1);
     *abort_flag = 0;
     mbar_init_fence();
   }
   if (warp == 1) {
-    if (PAIR) {
-      tmem_alloc_pair(smem_u32(tmem_holder), C::kTmemCols);
-      tmem_relinquish_pair();
-    } else {
-      tmem_alloc(smem_u32(tmem_holder), C::kTmemCols);
-      tmem_relinquish();
-    }
+    tmem_alloc(smem_u32(tmem_holder), 512);
+    tmem_relinquish();
   }
   tc_fence_before_sync();
-  if (C::kCtas > 1) cluster_sync();
+  if (KS > 1) cluster_sync();
   else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_holder;
   pdl_wait();
-  const int first = p.from + blockIdx.x / C::kCtas, apart = gridDim.x / C::kCtas, units = p.to;
+  const int first = p.from + blockIdx.x / KS, apart = gridDim.x / KS, units = p.to;
 
   if (warp < 4) {
     prod_regs_less<kProdOtherRegs>();
@@ -509,7 +504,7 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
         bool ok = true;
         for (int u = first; ok && u < units; u += apart) {
           const Unit w = unit_of(p, u);
-          const uint32_t need = p.ordered ? 0 : w.after * (C::kCtas * kProdEpiWarps);
+          const uint32_t need = p.ordered ? 0 : w.after * (KS * kProdEpiWarps);
           if (load_acquire(p.done + w.batch) < need) {
             const uint64_t t0 = global_timer_ns();
 #pragma unroll 1
@@ -531,19 +526,16 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
           else if (w.product == kPolynomial) a = b = p.g;
           else if (p.wide) { a = p.b; b = p.x_mn[cur]; }
           else { a = p.x_k[cur]; b = p.b; }
-          const int row_a = w.m * T + (int)rank * 128, row_b = w.n * T + (int)rank * 128;
+          const int row_a = w.m * T, row_b = w.n * T;
           const int kb0 = first_block(w.blocks), kb1 = kb0 + my_blocks(w.blocks);
           for (int kb = kb0; ok && kb < kb1; ++kb) {
 #pragma unroll
             for (int lo = 1; lo >= 0; --lo, ++it) {
               const uint32_t s = it % kSlots, use = it / kSlots;
               if (use > 0 && !prod_wait(bar(C::EMPTY + s), (use - 1) & 1, abort_flag)) { ok = false; break; }
-              const uint32_t sa = a0 + s * C::kSlotBytes, full = PAIR ? map_to_rank(bar(C::FULL + s), 0) : bar(C::FULL + s);
-              if (rank == 0) mbar_arrive_expect_tx(bar(C::FULL + s), (PAIR ? 2 : 1) * C::kSlotBytes);
-              auto copy = [&](uint32_t dst, const CUtensorMap *m, int x, int y) {
-                if (PAIR) tma_load_3d_pair(dst, m, full, x, y, w.batch);
-                else tma_load_3d(dst, m, full, x, y, w.batch);
-              };
+              const uint32_t sa = a0 + s * C::kSlotBytes, full = bar(C::FULL + s);
+              mbar_arrive_expect_tx(full, C::kSlotBytes);
+              auto copy = [&](uint32_t dst, const CUtensorMap *m, int x, int y) { tma_load_3d(dst, m, full, x, y, w.batch); };
               auto load = [&](uint32_t dst, const CUtensorMap *m, bool mn, int row) {
                 if (mn) {
                   copy(dst, m, row, kb * kProdK);
@@ -558,7 +550,7 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
           }
         }
       }
-    } else if (warp == 1 && rank == 0) {
+    } else if (warp == 1) {
       // ---------------------------------------------------------- products
       uint32_t it = 0;
       bool ok = true;
@@ -571,30 +563,23 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
         auto issue = [&](uint32_t d, uint32_t sa, uint32_t sb, bool fresh) {
           const uint64_t da = make_smem_desc(sa, lbo_a, 1024, kSwz128), db = make_smem_desc(sb, lbo_b, 1024, kSwz128);
 #pragma unroll
-          for (int k = 0; k < kProdK / 16; ++k) {
-            if (PAIR) mma_f16_ss_pair(d, da + k * step_a, db + k * step_b, idesc, fresh && k == 0 ? 0u : 1u);
-            else mma_f16_ss(d, da + k * step_a, db + k * step_b, idesc, fresh && k == 0 ? 0u : 1u);
-          }
+          for (int k = 0; k < kProdK / 16; ++k) mma_f16_ss(d, da + k * step_a, db + k * step_b, idesc, fresh && k == 0 ? 0u : 1u);
         };
         const int blocks = my_blocks(w.blocks);
         for (int kb = 0; kb < blocks; ++kb, ++it) {
-          const uint32_t acc = it & 1, d = tmem + acc * T, s_lo = (2 * it) % kSlots, s_hi = (2 * it + 1) % kSlots;
+          const uint32_t acc = it % C::kAccs, d = tmem + acc * T, s_lo = (2 * it) % kSlots, s_hi = (2 * it + 1) % kSlots;
           const uint32_t lo = a0 + s_lo * C::kSlotBytes, hi = a0 + s_hi * C::kSlotBytes;
-          auto commit = [&](int id) {
-            if (PAIR) mma_commit_pair(bar(id));
-            else mma_commit(bar(id));
-          };
-          if (it >= 2 && !prod_wait_warp(bar(C::ACC_EMPTY + acc), ((it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+          if (it >= C::kAccs && !prod_wait_warp(bar(C::ACC_EMPTY + acc), (it / C::kAccs - 1) & 1, abort_flag)) { ok = false; break; }
           if (!prod_wait_warp(bar(C::FULL + s_lo), ((2 * it) / kSlots) & 1, abort_flag) ||
               !prod_wait_warp(bar(C::FULL + s_hi), ((2 * it + 1) / kSlots) & 1, abort_flag)) { ok = false; break; }
           tc_fence_after_sync();
           if (elect_one()) {
             issue(d, lo, hi + C::kTileBytes, true);
             issue(d, hi, lo + C::kTileBytes, false);
-            commit(C::EMPTY + s_lo);
+            mma_commit(bar(C::EMPTY + s_lo));
             issue(d, hi, hi + C::kTileBytes, false);
-            commit(C::EMPTY + s_hi);
-            commit(C::ACC_FULL + acc);
+            mma_commit(bar(C::EMPTY + s_hi));
+            mma_commit(bar(C::ACC_FULL + acc));
           }
           __syncwarp();
         }
@@ -620,8 +605,8 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
       const int blocks = my_blocks(w.blocks);
 #pragma unroll 1
       for (int kb = 0; kb < blocks; ++kb, ++j) {
-        const uint32_t acc = j & 1;
-        if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j >> 1) & 1, abort_flag)) { ok = false; break; }
+        const uint32_t acc = j % C::kAccs;
+        if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j / C::kAccs) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after_sync();
 #pragma unroll
         for (int cg = 0; cg < kSums; ++cg) {
@@ -631,10 +616,7 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
           if (cg == kSums - 1) {
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) {
-              if (PAIR) mbar_arrive_cluster(map_to_rank(bar(C::ACC_EMPTY + acc), 0));
-              else mbar_arrive(bar(C::ACC_EMPTY + acc));
-            }
+            if (lane == 0) mbar_arrive(bar(C::ACC_EMPTY + acc));
           }
 #pragma unroll
           for (int x = 0; x < 32; x += 2) {
@@ -686,7 +668,7 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
         __syncwarp();
         if (lane < KS) mbar_arrive_cluster(map_to_rank(bar(C::RED_FREE), lane));
       }
-      const uint32_t row0 = (uint32_t)(w.m * T + (int)rank * 128 + quarter * 32), row = row0 + lane;
+      const uint32_t row0 = (uint32_t)(w.m * T + quarter * 32), row = row0 + lane;
       const uint32_t col0 = (uint32_t)(w.n * T + (int)part * C::kOwned + half * (C::kOwned / 2));
       if (w.product == kPolynomial) {  // what it reads of G: the copies have been waited for, these loads as well
         (void)load_acquire(p.done + w.batch);
@@ -739,11 +721,8 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
   tc_fence_before_sync();
   __syncthreads();
   if (*abort_flag != 0u) {
-    if (warp == 1 && rank == 0) {
-      if (elect_one()) {
-        if (PAIR) mma_commit_pair(bar(C::DRAIN));
-        else mma_commit(bar(C::DRAIN));
-      }
+    if (warp == 1) {
+      if (elect_one()) mma_commit(bar(C::DRAIN));
       __syncwarp();
       for (int n = 0; n < (1 << 16) && !mbar_try_wait(bar(C::DRAIN), 0); ++n) {
       }
@@ -756,11 +735,247 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
     if (threadIdx.x == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
     __syncthreads();
   }
-  if (C::kCtas > 1) cluster_sync();  // no CTA leaves while another may still signal its barriers or write to its shared memory
+  if (KS > 1) cluster_sync();  // no CTA leaves while another may still signal its barriers or write to its shared memory
   if (warp == 1) {
     tc_fence_after_sync();
-    if (PAIR) tmem_dealloc_pair(tmem, C::kTmemCols);
-    else tmem_dealloc(tmem, C::kTmemCols);
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------- small matrices, a CTA each
+// A matrix of at most 128 x 256 (seen with its rows the smaller side; a taller one is turned over on the way in and out) stays in shared memory as two fp16 parts
+// from its first product to its last: G, B and the new X go from tensor memory through registers to where the next product reads them, and nothing
+// between products leaves the SM (64 x 64: 79 us with a counter in global memory between products, see DESIGN for what this takes).
+// Slabs of 64 columns, 128 bytes a row, 128-byte swizzle: K-major for the products over columns, and the same bytes MN-major for B X, which contracts X's rows.
+constexpr uint32_t kSmallRows = 128, kSmallCols = 256;
+constexpr uint32_t kSlab = 128 * 128;                                       // bytes: 128 rows x 64 columns of one part
+constexpr uint32_t kSmallX = 0, kSmallG = 8 * kSlab, kSmallBars = 12 * kSlab;  // X: 4 slabs high, 4 low; G, then B: 2 high, 2 low
+constexpr uint32_t kSmallSmem = kSmallBars + 128 + 1024;
+constexpr uint32_t kSmallPitch = kSmallCols + 1;  // of the result in fp32, over all of it
+static_assert(kSmallRows * kSmallPitch * 4 <= kSmallBars, "the result does not fit");
+
+struct SmallParams {
+  Table t;
+  Targets o;
+  uint64_t source_stride, out_stride;
+  uint32_t rows, cols, bf16, nesterov, apply, steps;
+  float beta, eps, a, b, c, keep, step;
+  unsigned int *status;
+};
+
+__device__ __forceinline__ uint32_t small_at(uint32_t row, uint32_t col) {  // byte of an element in its part
+  return (col >> 6) * kSlab + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
+}
+// 64 columns of a row in parts: a slab's row
+__device__ __forceinline__ void small_store(uint8_t *hi, uint8_t *lo, uint32_t row, const float (&v)[64]) {
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    uint4 h, l;
+    split_half2(v[8 * x], v[8 * x + 1], h.x, l.x);
+    split_half2(v[8 * x + 2], v[8 * x + 3], h.y, l.y);
+    split_half2(v[8 * x + 4], v[8 * x + 5], h.z, l.z);
+    split_half2(v[8 * x + 6], v[8 * x + 7], h.w, l.w);
+    const uint32_t at = row * 128 + ((x ^ (row & 7)) << 4);
+    *reinterpret_cast<uint4 *>(hi + at) = h;
+    *reinterpret_cast<uint4 *>(lo + at) = l;
+  }
+}
+
+__global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_constant__ SmallParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t a0 = smem_u32(smem);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kSmallBars);
+  volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + kSmallBars + 40);
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(smem + kSmallBars + 44);
+  __shared__ double part[8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  if (tid == 0) {
+    for (int i = 0; i < 4; ++i) mbar_init(bar(i), 1);
+    *abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(tmem_holder), 512);
+    tmem_relinquish();
+  }
+  const bool wide = p.rows <= p.cols;
+  const uint32_t side = wide ? p.rows : p.cols, large = wide ? p.cols : p.rows, slabs = (large + 63) / 64, side_blocks = (side + 63) / 64, halves = (large + 127) / 128;
+  for (uint32_t i = tid; i < 8 * kSlab / 16; i += 256) reinterpret_cast<uint4 *>(smem + kSmallX)[i] = make_uint4(0u, 0u, 0u, 0u);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_holder;
+  pdl_wait();
+  const int m = blockIdx.x;
+  const void *source = p.t.source[m];
+  float *momentum = p.t.momentum[m];
+
+  // ---------------------------------------------------------------- U, its norm, X. A warp a row of the source, its lanes the columns, the same ones in both passes.
+  double sum = 0.0;
+  for (uint32_t r = warp; r < p.rows; r += 8) {
+#pragma unroll 4
+    for (uint32_t c = lane; c < p.cols; c += 32) {
+      float u = load_f(source, p.bf16, (size_t)r * p.source_stride + c);
+      if (momentum) {
+        const float v = fmaf(p.beta, momentum[r * p.cols + c], u);
+        momentum[r * p.cols + c] = v;
+        u = p.nesterov ? fmaf(p.beta, v, u) : v;
+      }
+      sum += (double)u * u;
+    }
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) part[warp] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (int i = 0; i < 8; ++i) sum += part[i];
+  const float f = (float)((double)kPartScale / (sqrt(sum) + (double)p.eps));
+  for (uint32_t r = warp; r < p.rows; r += 8) {
+#pragma unroll 4
+    for (uint32_t c = lane; c < p.cols; c += 32) {
+      float u = load_f(source, p.bf16, (size_t)r * p.source_stride + c);
+      if (momentum) {
+        const float v = momentum[r * p.cols + c];
+        u = p.nesterov ? fmaf(p.beta, v, u) : v;
+      }
+      u *= f;
+      const __half h = __float2half_rn(u);
+      const uint32_t at = wide ? small_at(r, c) : small_at(c, r);
+      *reinterpret_cast<__half *>(smem + kSmallX + at) = h;
+      *reinterpret_cast<__half *>(smem + kSmallX + 4 * kSlab + at) = __float2half_rn(u - __half2float(h));
+    }
+  }
+
+  // ---------------------------------------------------------------- the products: block i of 64 of a contraction into accumulator i, its end on barrier i
+  uint32_t phases = 0;  // bit i: the phase of barrier i that ends next
+  bool ok = true;
+  const int quarter = warp & 3, half = warp >> 2;
+  const uint32_t row = quarter * 32 + lane, lanes = tmem + ((uint32_t)(quarter * 32) << 16) + half * 64;
+  // block `acc`: A's slab at a (K-major), B at b: K-major slab, or MN-major rows with the next 64 columns a slab further
+  auto issue = [&](int acc, uint32_t a, uint32_t a_lo, uint32_t b, uint32_t b_lo, bool b_mn) {
+    const uint32_t idesc = make_idesc(kFmtF16, 128, 128, 0, b_mn ? 1 : 0);
+    auto product = [&](uint32_t x, uint32_t y, bool fresh) {
+      const uint64_t dx = make_smem_desc(a0 + x, 16, 1024, kSwz128), dy = make_smem_desc(a0 + y, b_mn ? kSlab : 16, 1024, kSwz128);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        mma_f16_ss(tmem + acc * 128, dx + (uint64_t)(k * 32 >> 4), dy + (uint64_t)(k * (b_mn ? 2048 : 32) >> 4), idesc, fresh && k == 0 ? 0u : 1u);
+    };
+    if (elect_one()) {
+      product(a_lo, b, true);
+      product(a, b_lo, false);
+      product(a, b, false);
+      mma_commit(bar(acc));
+    }
+    __syncwarp();
+  };
+  auto take = [&](int acc, float (&v)[64]) {  // adds this lane's 64 columns
+    if (!ok || !mbar_wait_warp(bar(acc), (phases >> acc) & 1, abort_flag)) {
+      ok = false;
+      return;
+    }
+    phases ^= 1u << acc;
+    tc_fence_after_sync();
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      uint32_t r[32];
+      tmem_ld32(lanes + acc * 128 + g * 32, r);
+      tmem_wait_ld();
+#pragma unroll
+      for (int x = 0; x < 32; ++x) v[32 * g + x] += __uint_as_float(r[x]);
+    }
+  };
+  auto meet = [&]() {  // what was written to shared memory is there for the tensor cores, and their results have been read
+    fence_proxy_async_smem();
+    tc_fence_before_sync();
+    const bool stop = __syncthreads_or(!ok) != 0;
+    tc_fence_after_sync();
+    return !stop;
+  };
+  auto clear = [](float (&v)[64]) {
+#pragma unroll
+    for (int x = 0; x < 64; ++x) v[x] = 0.0f;
+  };
+  bool go = meet();
+  for (uint32_t step = 0; go && step < p.steps; ++step) {
+    float g[64], v[64];
+    if (warp == 0)
+      for (uint32_t c = 0; c < slabs; ++c) issue((int)c, kSmallX + c * kSlab, kSmallX + (4 + c) * kSlab, kSmallX + c * kSlab, kSmallX + (4 + c) * kSlab, false);
+    clear(g);
+    for (uint32_t c = 0; c < slabs; ++c) take((int)c, g);
+#pragma unroll
+    for (int x = 0; x < 64; ++x) g[x] *= kPartInverse;
+    small_store(smem + kSmallG + half * kSlab, smem + kSmallG + (2 + half) * kSlab, row, g);
+    if (!(go = meet())) break;
+    if (warp == 0)
+      for (uint32_t c = 0; c < side_blocks; ++c) issue((int)c, kSmallG + c * kSlab, kSmallG + (2 + c) * kSlab, kSmallG + c * kSlab, kSmallG + (2 + c) * kSlab, false);
+    clear(v);
+    for (uint32_t c = 0; c < side_blocks; ++c) take((int)c, v);
+#pragma unroll
+    for (int x = 0; x < 64; ++x) v[x] = fmaf(p.c, v[x], p.b * g[x]) + ((uint32_t)(half * 64 + x) == row ? p.a : 0.0f);
+    small_store(smem + kSmallG + half * kSlab, smem + kSmallG + (2 + half) * kSlab, row, v);
+    if (!(go = meet())) break;
+    if (warp == 0)
+      for (uint32_t h = 0; h < halves; ++h)
+        for (uint32_t c = 0; c < side_blocks; ++c)
+          issue((int)(2 * h + c), kSmallG + c * kSlab, kSmallG + (2 + c) * kSlab, kSmallX + 2 * h * kSlab + c * 8192, kSmallX + (4 + 2 * h) * kSlab + c * 8192, true);
+    if (step + 1 < p.steps) {
+      for (uint32_t h = 0; h < halves; ++h) {
+        clear(v);
+        for (uint32_t c = 0; c < side_blocks; ++c) take((int)(2 * h + c), v);
+#pragma unroll
+        for (int x = 0; x < 64; ++x) v[x] *= kPartInverse;
+        // only the products that have just ended read these slabs of X
+        small_store(smem + kSmallX + (2 * h + half) * kSlab, smem + kSmallX + (4 + 2 * h + half) * kSlab, row, v);
+      }
+      go = meet();
+      continue;
+    }
+    // the last: in fp32 over everything in shared memory, once no product reads it
+    clear(g);
+    clear(v);
+    for (uint32_t c = 0; c < side_blocks; ++c) take((int)c, g);
+    if (halves > 1)
+      for (uint32_t c = 0; c < side_blocks; ++c) take((int)(2 + c), v);
+    if (!(go = meet())) break;
+    float *x = reinterpret_cast<float *>(smem) + row * kSmallPitch + half * 64;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+      x[i] = g[i] * (kPartInverse * kPartInverse);
+      x[128 + i] = v[i] * (kPartInverse * kPartInverse);
+    }
+  }
+  __syncthreads();
+  if (go) {
+    const float *x = reinterpret_cast<const float *>(smem);
+    for (uint32_t r = warp; r < p.rows; r += 8) {
+#pragma unroll 4
+      for (uint32_t c = lane; c < p.cols; c += 32) {
+        const float y = wide ? x[r * kSmallPitch + c] : x[c * kSmallPitch + r];
+        const size_t at = (size_t)r * p.out_stride + c;
+        if (p.bf16) {
+          uint32_t b;
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(0.0f), "f"(y));
+          static_cast<uint16_t *>(p.o.out[m])[at] = (uint16_t)b;
+        } else {
+          float *to = static_cast<float *>(p.o.out[m]) + at;
+          *to = p.apply ? fmaf(p.keep, *to, -p.step * y) : y;
+        }
+      }
+    }
+  } else if (tid == 0 && p.status) {  // a wait ran out: the products in flight are given time to end before the memory goes
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 2000000ull) {
+    }
+    atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -769,10 +984,17 @@ struct Layout {
   uint64_t done, x, x_next, g, b, total;  // offsets: parts hi, then lo, of all matrices of a group
   uint64_t x_matrix, g_matrix;      // elements of a matrix
   uint32_t x_pitch, g_pitch, side, group;
+  bool small;  // k_newton_schulz_small
 };
 Layout layout(uint32_t n, uint32_t rows, uint32_t cols) {
   Layout l = {};
   l.side = rows < cols ? rows : cols;
+  l.small = l.side <= kSmallRows && (rows < cols ? cols : rows) <= kSmallCols;
+  if (l.small) {
+    l.group = kMostMatrices;
+    l.total = 256;
+    return l;
+  }
   l.x_pitch = (uint32_t)up(cols, 64);
   l.g_pitch = (uint32_t)up(l.side, 64);
   l.x_matrix = up((uint64_t)rows * l.x_pitch, 128);
@@ -829,7 +1051,7 @@ struct Plan {
     p.x_n_tiles = tiles(cols);
     p.g_units = p.side_tiles * (p.side_tiles + 1) / 2;
     p.x_units = p.x_m_tiles * p.x_n_tiles;
-    const int slots = cluster_slots<k_newton_schulz<C>>(C::kCtas, C::kSmemTotal, kProdLaunchRegs);
+    const int slots = cluster_slots<k_newton_schulz<C>>(C::KS, C::kSmemTotal, kProdLaunchRegs);
     if (slots == 0) return DF_ERR_CUDA;
     const int per_step = (int)n * (2 * p.g_units + p.x_units);
     long long most = (long long)n * (p.g_units > p.x_units ? p.g_units : p.x_units);
@@ -844,7 +1066,7 @@ struct Plan {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = C::kCtas;
+    attr[0].val.clusterDim.x = C::KS;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     if (step < 0) {
       attr[1].id = cudaLaunchAttributeCooperative;
@@ -853,7 +1075,7 @@ struct Plan {
       attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
       attr[1].val.programmaticStreamSerializationAllowed = option(DF_OPT_PDL) != 0;
     }
-    cfg.gridDim = dim3((unsigned)((most < slots ? most : slots) * C::kCtas));
+    cfg.gridDim = dim3((unsigned)((most < slots ? most : slots) * C::KS));
     cfg.blockDim = dim3(kProdThreads);
     cfg.dynamicSmemBytes = C::kSmemTotal;
     cfg.stream = s;
@@ -865,23 +1087,55 @@ struct Plan {
   }
   int products(int form, uint32_t n, NsParams &p, int step, Product which) const {
     switch (form) {
-      case 0: return products<NsCfg<true, 1>>(n, p, step, which);
-      case 1: return products<NsCfg<false, 1>>(n, p, step, which);
-      case 2: return products<NsCfg<false, 2>>(n, p, step, which);
-      default: return products<NsCfg<false, 4>>(n, p, step, which);
+      case 0: return products<NsCfg<1>>(n, p, step, which);
+      case 1: return products<NsCfg<2>>(n, p, step, which);
+      default: return products<NsCfg<4>>(n, p, step, which);
     }
   }
 
-  // Time of a product in us in a form (tiles of t x t on clusters of `ctas`, the contraction cut in ks), without what comes between products.
+  // Time of a product in us with its contraction cut in 1 << form, without what comes between products: operands of 64 of the contraction are 64 KB a CTA, which
+  // arrive in about 1 us; results take 3, the exchange of partial sums 5.
   double estimate(uint32_t n, int form, Product which) const {
-    const uint64_t t = form == 0 ? 256 : 128, ks = form < 2 ? 1 : (form == 2 ? 2 : 4), ctas = form == 0 ? 2 : ks, slots = 148 / ctas;
-    const uint64_t m = (l.side + t - 1) / t, x = ((rows + t - 1) / t) * ((cols + t - 1) / t), g = m * (m + 1) / 2;
+    const uint64_t ks = 1ull << form, slots = 148 / ks, m = (l.side + 127) / 128, x = (uint64_t)((rows + 127) / 128) * ((cols + 127) / 128), g = m * (m + 1) / 2;
     const uint64_t k = which == kGram ? (rows > cols ? rows : cols) : l.side, blocks = ((k + 63) / 64 + ks - 1) / ks;
-    const uint64_t waves = ((which == kNext ? x : g) * n + slots - 1) / slots;
-    return (double)waves * ((double)blocks * (form == 0 ? 1.4 : 0.9) + (form == 0 ? 4.0 : ks > 1 ? 5.0 : 1.0));
+    return (double)(((which == kNext ? x : g) * n + slots - 1) / slots) * ((double)blocks + (form > 0 ? 5.0 : 1.0));
+  }
+
+  // Matrices that fit one CTA's shared memory. As many at a time as there are SMs take what one takes.
+  int small(uint32_t n, const UpdateParams &u, const NsParams &q) const {
+    static std::atomic<bool> ready[64];
+    int dev = 0;
+    if (check_cuda(cudaGetDevice(&dev)) != DF_OK || dev < 0 || dev >= 64) return DF_ERR_CUDA;
+    if (!ready[dev].load(std::memory_order_acquire)) {
+      if (check_cuda(cudaFuncSetAttribute(k_newton_schulz_small, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmallSmem)) != DF_OK) return DF_ERR_CUDA;
+      ready[dev].store(true, std::memory_order_release);
+    }
+    SmallParams p = {};
+    p.t = u.t;
+    p.o = q.t;
+    p.source_stride = u.row_stride;
+    p.out_stride = q.out_stride;
+    p.rows = rows;
+    p.cols = cols;
+    p.bf16 = u.bf16;
+    p.nesterov = u.nesterov;
+    p.apply = q.apply;
+    p.steps = steps;
+    p.beta = u.beta;
+    p.eps = eps;
+    p.a = a * kPartScale;
+    p.b = b;
+    p.c = c * kPartInverse;
+    p.keep = q.keep;
+    p.step = q.step;
+    p.status = device_status_ptr();
+    const int st = check_cuda(launch_kernel(k_newton_schulz_small, dim3(n), dim3(256), kSmallSmem, s, p));
+    note_launch();
+    return st;
   }
 
   int run(uint32_t n, UpdateParams u, NsParams p) const {
+    if (l.small) return small(n, u, p);
     auto part = [&](uint64_t at, uint64_t matrix, int lo) { return reinterpret_cast<uint16_t *>(ws + at) + lo * matrix * l.group; };
     bool ok = true;
     for (int i = 0; i < 2; ++i) {
@@ -927,11 +1181,11 @@ struct Plan {
     p.c = c * kPartInverse;
     p.status = device_status_ptr();
     // One launch with one form for everything, about 5 us between products (fences, a counter, first copies), or a launch a product with the form that suits
-    // each, about 8 between.
+    // each, about 7 between (1200 x 3000: one launch 527 at best, three a step 446; 64 x 64: 79 and 101).
     const Product all[3] = {kGram, kPolynomial, kNext};
     double one = 1e300, own = 0.0;
     int one_form = 0, own_form[3] = {0, 0, 0};
-    for (int f = 0; f < 4; ++f) {
+    for (int f = 0; f < 3; ++f) {
       double t = 0.0;
       for (Product q : all) t += estimate(n, f, q) + 5.0;
       if (t < one) {
@@ -941,8 +1195,8 @@ struct Plan {
     }
     for (int i = 0; i < 3; ++i) {
       double best = 1e300;
-      for (int f = 0; f < 4; ++f) {
-        const double t = estimate(n, f, all[i]) + 8.0;
+      for (int f = 0; f < 3; ++f) {
+        const double t = estimate(n, f, all[i]) + 7.0;
         if (t < best) {
           best = t;
           own_form[i] = f;
@@ -989,6 +1243,13 @@ int df_orthogonalize(const void *update, void *out, void *workspace, uint64_t wo
   if (update_matrix_stride >= most || update_row_stride >= most || out_matrix_stride >= most || out_row_stride >= most) return finish(DF_ERR_INVALID_ARG);
   if (rows > 1 && (update_row_stride < cols || out_row_stride < cols)) return finish(DF_ERR_INVALID_ARG);
   if (n > 1 && out_matrix_stride < (uint64_t)(rows - 1) * out_row_stride + cols) return finish(DF_ERR_INVALID_ARG);
+  {  // out is the update, element by element, or shares nothing with it
+    const uint64_t e = bf16 ? 2 : 4, in_rows = rows - 1, in_all = (uint64_t)(n - 1);
+    const uintptr_t u0 = reinterpret_cast<uintptr_t>(update), u1 = u0 + (in_all * update_matrix_stride + in_rows * update_row_stride + cols) * e;
+    const uintptr_t o0 = reinterpret_cast<uintptr_t>(out), o1 = o0 + (in_all * out_matrix_stride + in_rows * out_row_stride + cols) * e;
+    const bool same = u0 == o0 && (rows == 1 || update_row_stride == out_row_stride) && (n == 1 || update_matrix_stride == out_matrix_stride);
+    if (!same && u0 < o1 && o0 < u1) return finish(DF_ERR_INVALID_ARG);
+  }
   const Layout l = layout(n, rows, cols);
   if (!workspace || workspace_bytes < l.total || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return finish(DF_ERR_WORKSPACE);
   const Plan plan = {rows, cols, steps, a, b, c, eps, static_cast<uint8_t *>(workspace), l, static_cast<cudaStream_t>(stream)};

@@ -5,10 +5,12 @@
 // where |x| is within 2^18 of the largest that s was chosen for, and nothing below 2^-40 of that one. Then
 //   A B = A_lo B_hi + A_hi B_lo + A_hi B_hi      (A_lo B_lo, 2^-24 of it, is left out)
 // is three products in that order: the tensor cores cut sums off instead of rounding them, and a large sum is cut off at each of its
-// additions, so the small terms come first and every CHUNK blocks of 64 the sum is taken out to registers and added up rounded.
+// additions, so the small terms come first and every 128 of the contraction the sum is taken out to registers and added up rounded. (More often costs time: a
+// tile's sums are 128 KB a CTA, which tensor memory gives out in about 2000 cycles, and 64 of the contraction are 1536 cycles of products.)
 //
 // One persistent kernel, at most one CTA an SM, 384 threads:
-//   warp 0       copies: a ring of stages, each 64 of the contraction: 128 rows of A and this CTA's rows of B (PARTS = 2: both parts), 128-byte swizzle;
+//   warp 0       copies: a ring of slots, each 64 of the contraction: 128 rows of A and this CTA's rows of B (PARTS = 2: of the low parts, of the high parts, in
+//                turn), 128-byte swizzle;
 //   warp 1       issues the products into one of two accumulators in tensor memory;
 //   warps 4-11   the epilogue of one tile under the products of the next: a warp has the 32 rows of its quarter of tensor memory, a row
 //                a lane, and half of the tile's columns, 32 at a time. With CHUNK its sums are 128 registers a thread, which it takes over from warps 0-3.
@@ -44,6 +46,7 @@ struct ProductTile {
 };
 
 constexpr int kProdEpiWarps = 8, kProdThreads = 384, kProdK = 64;
+constexpr int kProdChunk = 2;  // products of parts: blocks of 64 between takings out of the sums
 constexpr uint32_t kProdSlabBytes = 32 * 128;  // a warp's staging slab: 32 rows of 128 bytes
 // Sums in registers: the launch gives 168 registers to each thread of three warpgroups; the two of the epilogue take over 48 from each thread of the first.
 constexpr int kProdLaunchRegs = 168, kProdEpiRegs = 216, kProdOtherRegs = 72;
@@ -70,15 +73,16 @@ __device__ __forceinline__ bool prod_wait_warp(uint32_t bar, uint32_t parity, vo
   return __all_sync(0xffffffffu, prod_wait(bar, parity, abort_flag)) != 0;
 }
 
+// CHUNK (bf16 only): blocks between takings out of sums, 0: none before the end of the tile.
 template <bool A_MN_, bool B_MN_, int PARTS_, int CHUNK_>
 struct ProdCfg {
   static constexpr bool A_MN = A_MN_, B_MN = B_MN_;
   static constexpr int PARTS = PARTS_;
   static constexpr int TM = 256, TN = 256;
-  static constexpr bool kSums = CHUNK_ > 0;                        // sums in registers
-  static constexpr int kChunk = kSums ? CHUNK_ : 0x40000000;  // blocks between takings out
-  static constexpr uint32_t kTileBytes = 128 * kProdK * 2, kStageBytes = 2 * PARTS * kTileBytes;  // A hi, B hi (, A lo, B lo)
-  static constexpr int kStages = PARTS == 2 ? 3 : 6;
+  static constexpr bool kSums = PARTS == 2 || CHUNK_ > 0;  // sums in registers
+  static constexpr int kChunk = PARTS == 2 ? kProdChunk : CHUNK_ > 0 ? CHUNK_ : 0x40000000;
+  static constexpr uint32_t kTileBytes = 128 * kProdK * 2, kStageBytes = 2 * kTileBytes;
+  static constexpr int kStages = 6;
   static constexpr uint32_t kSmemStaging = kStages * kStageBytes;
   static constexpr uint32_t kSmemBars = kSmemStaging + kProdEpiWarps * kProdSlabBytes;
   static constexpr uint32_t kSmemTotal = kSmemBars + 256 + 1024;
@@ -147,26 +151,25 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
           int kb0, kb1;
           const ProductTile t = decode(id, &kb0, &kb1);
           const int row_a = t.m_tile * C::TM + (int)rank * 128, row_b = t.n_tile * TN + (int)rank * 128;
-          for (int kb = kb0; kb < kb1; ++kb, ++it) {
-            const uint32_t s = it % kStages, use = it / kStages;
-            if (use > 0 && !prod_wait(bar(C::EMPTY + s), (use - 1) & 1, abort_flag)) { ok = false; break; }
-            const uint32_t sa = a0 + s * C::kStageBytes;
-            // both CTAs' copies count on the even CTA's barrier, which expects the bytes of both
-            const uint32_t full = map_to_rank(bar(C::FULL + s), 0);
-            if (rank == 0) mbar_arrive_expect_tx(bar(C::FULL + s), 2 * C::kStageBytes);
-            auto load = [&](uint32_t dst, const CUtensorMap *m, bool mn, int row) {
-              if (mn) {
-                tma_load_2d_pair(dst, m, full, row, kb * kProdK);
-                tma_load_2d_pair(dst + 8192, m, full, row + 64, kb * kProdK);
-              } else {
-                tma_load_2d_pair(dst, m, full, kb * kProdK, row);
-              }
-            };
-            load(sa, &tmA, C::A_MN, row_a);
-            load(sa + C::kTileBytes, &tmB, C::B_MN, row_b);
-            if constexpr (C::PARTS == 2) {
-              load(sa + 2 * C::kTileBytes, &tmA_lo, C::A_MN, row_a);
-              load(sa + 3 * C::kTileBytes, &tmB_lo, C::B_MN, row_b);
+          for (int kb = kb0; ok && kb < kb1; ++kb) {
+#pragma unroll
+            for (int lo = C::PARTS - 1; lo >= 0; --lo, ++it) {
+              const uint32_t s = it % kStages, use = it / kStages;
+              if (use > 0 && !prod_wait(bar(C::EMPTY + s), (use - 1) & 1, abort_flag)) { ok = false; break; }
+              const uint32_t sa = a0 + s * C::kStageBytes;
+              // both CTAs' copies count on the even CTA's barrier, which expects the bytes of both
+              const uint32_t full = map_to_rank(bar(C::FULL + s), 0);
+              if (rank == 0) mbar_arrive_expect_tx(bar(C::FULL + s), 2 * C::kStageBytes);
+              auto load = [&](uint32_t dst, const CUtensorMap *m, bool mn, int row) {
+                if (mn) {
+                  tma_load_2d_pair(dst, m, full, row, kb * kProdK);
+                  tma_load_2d_pair(dst + 8192, m, full, row + 64, kb * kProdK);
+                } else {
+                  tma_load_2d_pair(dst, m, full, kb * kProdK, row);
+                }
+              };
+              load(sa, lo ? &tmA_lo : &tmA, C::A_MN, row_a);
+              load(sa + C::kTileBytes, lo ? &tmB_lo : &tmB, C::B_MN, row_b);
             }
           }
         }
@@ -188,26 +191,50 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
       for (long long id = first_tile; ok && id < p.tiles; id += tile_step) {
         int kb0, kb1;
         decode(id, &kb0, &kb1);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const uint32_t acc = j & 1, d = tmem + acc * TN, s = it % kStages, sa = a0 + s * C::kStageBytes;
-          // an accumulator is taken out after every kChunk blocks, or at the end of the tile
-          const bool first = (kb - kb0) % C::kChunk == 0, last = (kb - kb0) % C::kChunk == C::kChunk - 1 || kb + 1 == kb1;
-          if (first && j >= 2 && !prod_wait_warp(bar(C::ACC_EMPTY + acc), ((j >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
-          if (!prod_wait_warp(bar(C::FULL + s), (it / kStages) & 1, abort_flag)) { ok = false; break; }
-          tc_fence_after_sync();
-          if (elect_one()) {
-            if constexpr (C::PARTS == 2) {
-              issue(d, sa + 2 * C::kTileBytes, sa + C::kTileBytes, first);
-              issue(d, sa, sa + 3 * C::kTileBytes, false);
-              issue(d, sa, sa + C::kTileBytes, false);
-            } else {
-              issue(d, sa, sa + C::kTileBytes, first);
+        for (int kb = kb0; ok && kb < kb1;) {
+          const uint32_t acc = j & 1, d = tmem + acc * TN;
+          const int n = kb1 - kb < C::kChunk ? kb1 - kb : C::kChunk;
+          if (j >= 2 && !prod_wait_warp(bar(C::ACC_EMPTY + acc), ((j >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+          if constexpr (C::PARTS == 2) {
+            // the small terms of the chunk's blocks, then the large ones
+            for (int i = 0; ok && i < n; ++i) {
+              const uint32_t t = it + 2 * i, s_lo = t % kStages, s_hi = (t + 1) % kStages;
+              if (!prod_wait_warp(bar(C::FULL + s_lo), (t / kStages) & 1, abort_flag) ||
+                  !prod_wait_warp(bar(C::FULL + s_hi), ((t + 1) / kStages) & 1, abort_flag)) { ok = false; break; }
+              tc_fence_after_sync();
+              if (elect_one()) {
+                const uint32_t lo = a0 + s_lo * C::kStageBytes, hi = a0 + s_hi * C::kStageBytes;
+                issue(d, lo, hi + C::kTileBytes, i == 0);
+                issue(d, hi, lo + C::kTileBytes, false);
+                mma_commit_pair(bar(C::EMPTY + s_lo));
+              }
+              __syncwarp();
             }
-            mma_commit_pair(bar(C::EMPTY + s));
-            if (last) mma_commit_pair(bar(C::ACC_FULL + acc));
+            if (ok && elect_one()) {
+              for (int i = 0; i < n; ++i) {
+                const uint32_t s_hi = (it + 2 * i + 1) % kStages, hi = a0 + s_hi * C::kStageBytes;
+                issue(d, hi, hi + C::kTileBytes, false);
+                mma_commit_pair(bar(C::EMPTY + s_hi));
+              }
+              mma_commit_pair(bar(C::ACC_FULL + acc));
+            }
+            __syncwarp();
+            it += 2 * n;
+          } else {
+            for (int i = 0; i < n; ++i, ++it) {
+              const uint32_t s = it % kStages, sa = a0 + s * C::kStageBytes;
+              if (!prod_wait_warp(bar(C::FULL + s), (it / kStages) & 1, abort_flag)) { ok = false; break; }
+              tc_fence_after_sync();
+              if (elect_one()) {
+                issue(d, sa, sa + C::kTileBytes, i == 0);
+                mma_commit_pair(bar(C::EMPTY + s));
+                if (i + 1 == n) mma_commit_pair(bar(C::ACC_FULL + acc));
+              }
+              __syncwarp();
+            }
           }
-          __syncwarp();
-          j += last;
+          kb += n;
+          ++j;
         }
       }
     }

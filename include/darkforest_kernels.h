@@ -484,14 +484,15 @@ DF_API int df_linear_cross_entropy_backward(const void *x, const void *weight, c
 
 /* ---- orthogonalised updates of matrices, next to AdamW (no counterpart in the reference) ----
  * O(U): X = U / (|U|_F + eps); `steps` (1 .. 64) times X <- a X + (b X X^T + c (X X^T)^2) X. rows, cols up to 65536, rows * cols below 2^31, any of the two larger.
- *   df_orthogonalize   n matrices [rows][cols] (fp32, or bf16 with bf16 != 0; strides in elements): out = O(update). out may be the update itself.
+ *   df_orthogonalize   n matrices [rows][cols] (fp32, or bf16 with bf16 != 0; strides in elements): out = O(update). out may be the update itself, and may not
+ *       overlap it otherwise.
  *   df_muon_update     n tensors [rows][cols] fp32, contiguous, described by df_muon_tensor_t entries in HOST memory, read before the call returns (up to 1024):
  *       momentum <- beta momentum + gradient; U = gradient + beta momentum (nesterov != 0) or momentum;
  *       parameter <- parameter (1 - lr weight_decay) - lr update_scale O(U). No tensor may overlap another.
  * Precision: factors in 22 bits relative to 1 (elements below 2^-26 in fewer, none below 2^-37), sums in fp32, the norm in double, results rounded once.
  * |a| + |b| + |c| below 15 (else DF_ERR_UNSUPPORTED); singular values that a step brings above 3.8 make the matrix's results infinite or NaN. A zero matrix gives 0
  * (eps > 0), an infinity or NaN NaN, both without touching the other matrices. Nothing depends on the order of execution.
- * workspace: df_orthogonalize_workspace_bytes (for both calls; at most 512 MB or one matrix), 256-byte aligned, contents undefined before and after. Calls that can overlap need one each. */
+ * workspace: df_orthogonalize_workspace_bytes (for both calls; at most 192 MB or one matrix), 256-byte aligned, contents undefined before and after. Calls that can overlap need one each. */
 typedef struct df_muon_tensor {
   float *parameter;
   float *momentum;
