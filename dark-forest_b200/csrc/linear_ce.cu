@@ -49,6 +49,9 @@ __device__ __forceinline__ float logit_factor(float scale, const float *row_fact
   return scale * (in ? row_factor[row] : 1.0f) * inv;
 }
 
+// The same for the exponent of 2, above 0 also where operands are so small that it vanishes: -inf, the largest of no columns, times it stays -inf.
+__device__ __forceinline__ float exponent_factor(float c) { return fmaxf(c * kLog2e, 1.17549435e-38f); }
+
 // ---------------------------------------------------------------- epilogues
 struct LseEpi {
   struct Params {
@@ -71,7 +74,7 @@ struct LseEpi {
     col0 = c0;
     in = r < p.rows;
     target = in ? p.targets[r] - (int)p.col_base : -1;
-    c = logit_factor(p.scale, p.row_factor, p.largest_w, r, in) * kLog2e;
+    c = exponent_factor(logit_factor(p.scale, p.row_factor, p.largest_w, r, in));
     m = -INFINITY;
     s = 0.0f;
   }
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(1024) k_join(const JoinParams p) {
   __shared__ float2 s_part[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t row = blockIdx.x * 32 + lane;
-  const float cn = logit_factor(p.scale, p.row_factor, p.largest_w, row, row < p.rows), c = cn * kLog2e;
+  const float cn = logit_factor(p.scale, p.row_factor, p.largest_w, row, row < p.rows), c = exponent_factor(cn);
   float m = -INFINITY, s = 0.0f;
   auto join = [&](float2 q) {
     const float top = fmaxf(m, q.x), ref = top == -INFINITY ? 0.0f : top;
@@ -785,15 +788,24 @@ struct HeadCall {
   }
 };
 
-// Whether [rows][stride] elements from a and those from b share memory.
+// Memory of a call: [rows] of width elements, stride apart; null: none.
 struct Span {
-  uintptr_t from, to;
+  uintptr_t from = 0, to = 0;
   Span(const void *p, uint64_t rows, uint64_t stride, uint64_t width, uint64_t elt) {
+    if (!p) return;
     from = reinterpret_cast<uintptr_t>(p);
     to = from + ((rows - 1) * stride + width) * elt;
   }
+  Span(const void *p, uint64_t bytes) : Span(p, 1, 0, bytes, 1) {}
   bool meets(const Span &o) const { return from < o.to && o.from < to; }
 };
+// Whether one of the first `written` shares memory with another.
+bool overlap(const Span *spans, int n, int written) {
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < n; ++j)
+      if (spans[i].meets(spans[j])) return true;
+  return false;
+}
 
 int check_call(const void *x, const void *w, const int32_t *targets, uint32_t rows, uint32_t vocab, uint32_t width, uint64_t x_stride, uint64_t w_stride,
                float scale) {
@@ -825,6 +837,10 @@ int df_linear_cross_entropy(const void *x, const void *weight, const int32_t *ta
   if (!loss || !lse) return finish(DF_ERR_INVALID_ARG);
   const Layout l = layout(rows, vocab, width, bf16 != 0, false);
   if (!workspace || workspace_bytes < l.total || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return finish(DF_ERR_WORKSPACE);
+  const uint64_t elt = bf16 ? 2 : 4;
+  const Span all[] = {Span(loss, 4ull * rows), Span(lse, 4ull * rows), Span(workspace, l.total), Span(x, rows, x_stride, width, elt),
+                      Span(weight, vocab, weight_stride, width, elt), Span(targets, 4ull * rows)};
+  if (overlap(all, 6, 3)) return finish(DF_ERR_INVALID_ARG);
   const HeadCall call = {x, weight, targets, rows > 1 ? x_stride : up(width, 8), vocab > 1 ? weight_stride : up(width, 8), rows, vocab, width, bf16 != 0, scale,
                          static_cast<uint8_t *>(workspace), l, static_cast<cudaStream_t>(stream)};
   return finish(call.forward(loss, lse));
@@ -847,18 +863,11 @@ int df_linear_cross_entropy_backward(const void *x, const void *weight, const in
   }
   if (!lse || !grad_loss) return finish(DF_ERR_INVALID_ARG);
   if (!d_x && !d_weight) return DF_OK;
-  const Span sx(x, rows, x_stride, width, elt), sw(weight, vocab, weight_stride, width, elt);
-  if (d_x) {
-    const Span o(d_x, rows, dx_stride, width, elt);
-    if (o.meets(sx) || o.meets(sw)) return finish(DF_ERR_INVALID_ARG);
-    if (d_weight && o.meets(Span(d_weight, vocab, dw_stride, width, elt))) return finish(DF_ERR_INVALID_ARG);
-  }
-  if (d_weight) {
-    const Span o(d_weight, vocab, dw_stride, width, elt);
-    if (o.meets(sx) || o.meets(sw)) return finish(DF_ERR_INVALID_ARG);
-  }
   const Layout l = layout(rows, vocab, width, bf16 != 0, true);
   if (!workspace || workspace_bytes < l.total || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return finish(DF_ERR_WORKSPACE);
+  const Span all[] = {Span(d_x, rows, dx_stride, width, elt), Span(d_weight, vocab, dw_stride, width, elt), Span(workspace, l.total), Span(x, rows, x_stride, width, elt),
+                      Span(weight, vocab, weight_stride, width, elt), Span(targets, 4ull * rows), Span(lse, 4ull * rows), Span(grad_loss, 4ull * rows)};
+  if (overlap(all, 8, 3)) return finish(DF_ERR_INVALID_ARG);
   const HeadCall call = {x, weight, targets, rows > 1 ? x_stride : up(width, 8), vocab > 1 ? weight_stride : up(width, 8), rows, vocab, width, bf16 != 0, scale,
                          static_cast<uint8_t *>(workspace), l, s};
   return finish(bf16 ? call.backward<1>(lse, grad_loss, d_x, dx_stride, d_weight, dw_stride) : call.backward<2>(lse, grad_loss, d_x, dx_stride, d_weight, dw_stride));

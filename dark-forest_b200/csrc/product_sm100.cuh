@@ -3,7 +3,7 @@
 // Operands lie in global memory with either side contiguous (K-major: rows of k; MN-major: rows of m or n), bf16 or fp16. With
 // PARTS = 2 a value is two fp16 numbers, hi = fp16(s x) and lo = fp16(s x - hi) for a power of two s that the caller undoes: 22 bits
 // where |x| is within 2^18 of the largest that s was chosen for, and nothing below 2^-40 of that one. Then
-//   A B = A_lo B_hi + A_hi B_lo + A_hi B_hi      (A_lo B_lo, 2^-24 of it, is left out)
+//   A B = A_lo B_hi + A_hi B_lo + A_hi B_hi      (A_lo B_lo, 2^-22 of it at most, is left out)
 // is three products in that order: the tensor cores cut sums off instead of rounding them, and a large sum is cut off at each of its
 // additions, so the small terms come first and every 128 of the contraction the sum is taken out to registers and added up rounded. (More often costs time: a
 // tile's sums are 128 KB a CTA, which tensor memory gives out in about 2000 cycles, and 64 of the contraction are 1536 cycles of products.)
