@@ -11,8 +11,10 @@ df_attn_backward on caller-owned q, k, v, attn_out, lse, delta, d_q, d_k, d_v bu
 fused_projections - the forward of the projections on either side of it (df_linear_qkv_forward: Q, K, V
 in one launch; df_linear_forward: output projection + bias + residual; with step_kernels also
 df_linear_gelu_forward: the MLP's first projection with GELU in its epilogue), each inside a
-torch.autograd.Function whose backward uses torch matmuls. Everything else (the other cuBLAS TF32
-GEMMs, cross-entropy; with step_kernels=False also LayerNorm, GELU and AdamW) is stock torch and stands in for the reference's own
+torch.autograd.Function whose backward uses torch matmuls. With linear_loss the tied LM head and its cross-entropy are one operator of the library that keeps no logits (df_linear_cross_entropy and its
+backward, full fp32 precision), with optimizer="muon" the blocks' matrices are updated by df_muon_update, a call per shape, and everything else by
+AdamW as before. Everything else (the other cuBLAS TF32
+GEMMs, cross-entropy unless linear_loss is set; with step_kernels=False also LayerNorm, GELU and AdamW) is stock torch and stands in for the reference's own
 kernels, which are outside the path; the purpose is to measure what share of a step the attention
 takes. Weights are N(0, 0.02) from a seed, tokens uniform in [0, vocab).
 """
@@ -22,7 +24,7 @@ import math
 
 
 def build(pkg, n_layers=12, d_model=768, n_heads=12, d_ff=3072, vocab=50257, max_pos=4096, device="cuda", seed=0,
-          fused_projections=True, optimizer=True, step_kernels=True):
+          fused_projections=True, optimizer=True, step_kernels=True, linear_loss=False):
     import torch
     import torch.nn as nn
     import torch.nn.functional as F
@@ -127,6 +129,23 @@ def build(pkg, n_layers=12, d_model=768, n_heads=12, d_ff=3072, vocab=50257, max
             d_pre = pkg.gelu_backward(d_act.reshape(pre.shape).contiguous(), pre)
             return (d_pre @ w).view(*d_act.shape[:-1], w.shape[1]), d_pre.t() @ x2, d_pre.sum(0)
 
+    class LinearCrossEntropy(torch.autograd.Function):
+        """Per-row cross-entropy of targets under rows weight^T; the logits are formed again for the gradient."""
+
+        @staticmethod
+        def forward(ctx, rows, weight, targets):
+            loss, lse = pkg.linear_cross_entropy(rows, weight, targets)
+            ctx.save_for_backward(rows, weight, targets, lse)
+            return loss
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad):
+            rows, weight, targets, lse = ctx.saved_tensors
+            d_rows, d_weight = pkg.linear_cross_entropy_backward(rows, weight, targets, lse, grad.contiguous(), want_x=ctx.needs_input_grad[0],
+                                                                 want_weight=ctx.needs_input_grad[1])
+            return d_rows, d_weight, None
+
     class LayerNorm(nn.LayerNorm):
         def forward(self, x):
             return LayerNormFn.apply(x, self.weight, self.bias) if step_kernels else super().forward(x)
@@ -176,6 +195,8 @@ def build(pkg, n_layers=12, d_model=768, n_heads=12, d_ff=3072, vocab=50257, max
             loss = x.new_zeros(())
             rows = x.reshape(B * S, d_model)
             tgt = targets.reshape(-1)
+            if linear_loss:
+                return LinearCrossEntropy.apply(rows, self.tok.weight, tgt.to(torch.int32)).sum() / (B * S)
             chunk = 8192
             for r0 in range(0, B * S, chunk):
                 logits = rows[r0:r0 + chunk] @ self.tok.weight.t()
@@ -192,7 +213,9 @@ def build(pkg, n_layers=12, d_model=768, n_heads=12, d_ff=3072, vocab=50257, max
             nn.init.zeros_(prm)
     if not optimizer:
         return model, None, timers
-    if step_kernels:
+    if optimizer == "muon":
+        opt = MuonWithAdamW(pkg, list(model.blocks.parameters()), [p for n, p in model.named_parameters() if not n.startswith("blocks.")])
+    elif step_kernels:
         opt = MultiTensorAdamW(pkg, list(model.parameters()), lr=3e-4, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
     else:
         opt = torch.optim.AdamW(model.parameters(), lr=3e-4, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1, fused=True)
@@ -221,6 +244,38 @@ class MultiTensorAdamW:
     def step(self):
         self.t += 1
         self.plan.step(self.lr, self.b1, self.b2, self.eps, self.wd, 1.0 - self.b1 ** self.t, 1.0 - self.b2 ** self.t)
+
+
+class MuonWithAdamW:
+    """Matrices among `inner` are updated by momentum and Newton-Schulz products (df_muon_update, one call per shape over all layers); the others of them, and
+    `outer` (embeddings, the head that shares their weight, final norm), by AdamW in one launch."""
+
+    def __init__(self, pkg, inner, outer, lr=0.02, momentum=0.95, weight_decay=0.1, adamw_lr=3e-4):
+        import torch
+        self.pkg, self.lr, self.momentum, self.wd = pkg, lr, momentum, weight_decay
+        matrices = [p for p in inner if p.dim() == 2]
+        self.adamw = MultiTensorAdamW(pkg, [p for p in inner if p.dim() != 2] + list(outer), lr=adamw_lr, betas=(0.9, 0.95), eps=1e-8, weight_decay=weight_decay)
+        self.groups = []  # (parameters, momenta) of one shape
+        for shape in sorted({tuple(p.shape) for p in matrices}):
+            of = [p for p in matrices if tuple(p.shape) == shape]
+            for p in of:
+                p.grad = torch.zeros_like(p)
+            self.groups.append((of, [torch.zeros_like(p) for p in of]))
+        most = max((pkg.orthogonalize_workspace_bytes(len(g[0]), *g[0][0].shape) for g in self.groups), default=0)
+        self.workspace = torch.empty(most, dtype=torch.uint8, device=matrices[0].device) if matrices else None
+
+    def zero_grad(self, set_to_none=False):
+        import torch
+        self.adamw.zero_grad()
+        for parameters, _ in self.groups:
+            torch._foreach_zero_([p.grad for p in parameters])
+
+    def step(self):
+        self.adamw.step()
+        for parameters, momenta in self.groups:
+            rows, cols = parameters[0].shape
+            self.pkg.muon_update([p.data for p in parameters], momenta, [p.grad for p in parameters], self.lr, self.momentum, self.wd,
+                                 update_scale=max(1.0, rows / cols) ** 0.5, workspace=self.workspace)
 
 
 def run(pkg, batch=8, seq=4096, steps=3, warmup=1, device="cuda", **model_kw):
