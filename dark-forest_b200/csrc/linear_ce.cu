@@ -19,9 +19,6 @@ namespace {
 using namespace ptx;
 
 constexpr float kGScale = 16384.0f;  // G is stored times 2^14
-// Blocks of 64 between takings out of the sums of a bf16 call's logits where the loss is wanted: none up to a width of 768 (4096 rows: 198 us, 1.0e-6 off 64 bits; every
-// 6 blocks 244, every 4 289 and 3.2e-7), 12 above (210 us at 768).
-constexpr int kChunkBf16 = 12;
 constexpr uint64_t kPieceBytes = 256ull << 20;  // of G, or of a piece's weight in parts
 
 int finish(int st) {
@@ -61,7 +58,7 @@ struct LseEpi {
     float2 *parts;               // [slots][rows_pad]: largest logit (as the product has it), sum of e^(z - largest)
     float *picked;               // [rows]: the target's logit (as the product has it)
     float scale;
-    uint32_t rows, cols, rows_pad, col_base, slot_base;  // col_base: first column of the piece; cols: of the piece
+    uint32_t rows, cols, rows_pad, col_base, slot_base, slot_cols;  // col_base: first column of the piece; cols: of the piece; slot_cols: of a warp
   };
   const Params &p;
   float c, m, s;
@@ -109,7 +106,7 @@ struct LseEpi {
     m = top;
   }
   __device__ __forceinline__ void end() {
-    if (in && col0 < p.cols) p.parts[(size_t)(p.slot_base + col0 / 128) * p.rows_pad + row] = make_float2(m, s);
+    if (in && col0 < p.cols) p.parts[(size_t)(p.slot_base + col0 / p.slot_cols) * p.rows_pad + row] = make_float2(m, s);
   }
 };
 
@@ -406,22 +403,55 @@ __global__ void __launch_bounds__(256) k_pack(const PackParams p) {
   }
 }
 
-// loss and lse of 32 rows a block: lanes are rows, warps share the slots
+// loss and lse of 32 rows a block: lanes are rows, warps share the slots. For bf16 calls a warp also takes a row's target again, in fp32 sums that are rounded: the tensor
+// cores cut the sum of a whole row off at each 16 of it, which a target's logit, a sum of terms of one sign where the model has learned something, feels most (4096
+// rows of 768: the loss 1.0e-6 off 64 bits without). With d what the logit lacks, sum e^z grows by p (e^d - 1) of itself.
 struct JoinParams {
   const float2 *parts;
   const float *picked, *row_factor;
   const uint32_t *largest_w;
   const int32_t *targets;
+  const uint16_t *x, *w;  // bf16 calls
+  uint64_t x_stride, w_stride;
   float *loss, *lse;
-  uint32_t rows, cols, rows_pad, slots;
+  uint32_t rows, cols, rows_pad, slots, width;
   float scale;
 };
 __global__ void __launch_bounds__(1024) k_join(const JoinParams p) {
   pdl_wait();
   __shared__ float2 s_part[32][33];
+  __shared__ float s_target[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t row = blockIdx.x * 32 + lane;
   const float cn = logit_factor(p.scale, p.row_factor, p.largest_w, row, row < p.rows), c = exponent_factor(cn);
+  if (p.x) {
+    const uint32_t r = blockIdx.x * 32 + warp, t = r < p.rows ? (uint32_t)p.targets[r] : ~0u;
+    float sum = 0.0f;
+    if (t < p.cols) {
+      const uint16_t *x = p.x + (size_t)r * p.x_stride, *w = p.w + (size_t)t * p.w_stride;
+      uint32_t done = 0;
+      if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15u) == 0) {
+        float other = 0.0f;
+        done = p.width & ~7u;
+#pragma unroll 4
+        for (uint32_t k = lane * 8; k < done; k += 256) {
+          const uint4 a = *reinterpret_cast<const uint4 *>(x + k), b = *reinterpret_cast<const uint4 *>(w + k);
+          const uint32_t aa[4] = {a.x, a.y, a.z, a.w}, bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sum = fmaf(__uint_as_float(aa[i] << 16), __uint_as_float(bb[i] << 16), sum);
+            other = fmaf(__uint_as_float(aa[i] & 0xffff0000u), __uint_as_float(bb[i] & 0xffff0000u), other);
+          }
+        }
+        sum += other;
+      }
+#pragma unroll 4
+      for (uint32_t k = done + lane; k < p.width; k += 32) sum = fmaf(load_f(x, true, k), load_f(w, true, k), sum);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) s_target[warp] = sum;
+  }
   float m = -INFINITY, s = 0.0f;
   auto join = [&](float2 q) {
     const float top = fmaxf(m, q.x), ref = top == -INFINITY ? 0.0f : top;
@@ -437,10 +467,21 @@ __global__ void __launch_bounds__(1024) k_join(const JoinParams p) {
   if (warp != 0 || row >= p.rows) return;
 #pragma unroll 1
   for (int i = 1; i < 32; ++i) join(s_part[i][lane]);
-  const bool counts = (uint32_t)p.targets[row] < p.cols;
-  const float l = logf(s);
-  p.lse[row] = counts ? fmaf(m, cn, l) : 0.0f;
-  p.loss[row] = counts ? fmaf(m - p.picked[row], cn, l) : 0.0f;
+  if ((uint32_t)p.targets[row] >= p.cols) {
+    p.lse[row] = 0.0f;
+    p.loss[row] = 0.0f;
+    return;
+  }
+  float target = p.picked[row], l = logf(s);
+  if (p.x) {
+    const float d = (s_target[lane] - target) * cn;
+    if (fabsf(d) < 1.0f) {  // above, all of it is rounding of logits of 2^20 and more: what was computed stays together. A NaN stays as well.
+      l += log1pf(expf((target - m) * cn - l) * expm1f(d));
+      target = s_target[lane];
+    }
+  }
+  p.lse[row] = fmaf(m, cn, l);
+  p.loss[row] = fmaf(m - target, cn, l);
 }
 
 // d_x = factor * sum of the planes, in the caller's type; rows that do not count get zeros
@@ -570,7 +611,7 @@ Layout layout(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool bac
   l.x_parts = take((uint64_t)rows * l.pitch * 2 * parts);
   l.w_parts = take((uint64_t)l.piece * l.pitch * 2 * parts);
   if (!backward) {
-    l.slots = (vocab + 127) / 128 + l.n_pieces;
+    l.slots = (vocab + 63) / 64 + l.n_pieces;
     l.parts = take((uint64_t)l.slots * l.rows_pad * 8);
     l.picked = take((uint64_t)rows * 4);
   } else {
@@ -593,7 +634,21 @@ int slices(uint32_t n, int wanted) {
   return (int)((n + each - 1) / each);
 }
 
-template <bool A_MN, bool B_MN, int PARTS, int CHUNK, class Epi>
+// Time in us of a product's waves of tiles with n blocks of 64 of the contraction each: a pair of CTAs takes about `PAIR` a block and writes results of parts while
+// no sums are added up, one CTA its operands' bytes, under which results are written.
+double tile_time(int parts, bool pair, uint64_t tiles, uint64_t n) {
+  const double block = parts == 2 ? (pair ? 1.2 : 1.0) : (pair ? 0.4 : 0.5), results = pair ? 4.0 : 2.5;
+  const double each = parts == 2 && pair ? block * (double)n + results : block * (double)n > results ? block * (double)n : results;
+  return (double)((tiles + (pair ? kPairs : 2 * kPairs) - 1) / (pair ? kPairs : 2 * kPairs)) * each;
+}
+
+bool pairs(int parts, uint32_t M, uint32_t N, uint32_t K, int splits) {
+  const uint32_t n_kb = (K + kProdK - 1) / kProdK, each = (n_kb + splits - 1) / splits;
+  auto tiles = [&](uint64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t) * (uint64_t)slices(n_kb, splits); };
+  return tile_time(parts, true, tiles(256), each) < tile_time(parts, false, tiles(128), each);
+}
+
+template <bool A_MN, bool B_MN, int PARTS, class Epi>
 int product(const Operand &a, const Operand &b, uint32_t M, uint32_t N, uint32_t K, int splits, bool bf16, const typename Epi::Params &e, cudaStream_t s) {
   ProductParams p = {};
   p.M = M;
@@ -602,7 +657,8 @@ int product(const Operand &a, const Operand &b, uint32_t M, uint32_t N, uint32_t
   p.splits = slices(p.n_kb, splits);
   p.kb_per_split = (p.n_kb + splits - 1) / splits;
   p.fmt = bf16 ? (uint32_t)kFmtBF16 : (uint32_t)kFmtF16;
-  return launch_product<ProdCfg<A_MN, B_MN, PARTS, CHUNK>, Epi>(a, b, p, e, s);
+  return pairs(PARTS, M, N, K, splits) ? launch_product<ProdCfg<true, A_MN, B_MN, PARTS>, Epi>(a, b, p, e, s)
+                                       : launch_product<ProdCfg<false, A_MN, B_MN, PARTS>, Epi>(a, b, p, e, s);
 }
 
 struct HeadCall {
@@ -690,15 +746,30 @@ struct HeadCall {
       e.rows_pad = l.rows_pad;
       e.col_base = c0;
       e.slot_base = slots;
-      slots += (n + 127) / 128;
+      e.slot_cols = pairs(bf16 ? 1 : 2, rows, n, width, 1) ? 128 : 64;
+      slots += (n + e.slot_cols - 1) / e.slot_cols;
       if (st == DF_OK)
-        st = !bf16 ? product<false, false, 2, 0, LseEpi>(a, b, rows, n, width, 1, false, e, s)
-             : width <= kChunkBf16 * kProdK ? product<false, false, 1, 0, LseEpi>(a, b, rows, n, width, 1, true, e, s)
-                                            : product<false, false, 1, kChunkBf16, LseEpi>(a, b, rows, n, width, 1, true, e, s);
+        st = bf16 ? product<false, false, 1, LseEpi>(a, b, rows, n, width, 1, true, e, s) : product<false, false, 2, LseEpi>(a, b, rows, n, width, 1, false, e, s);
     }
     if (st != DF_OK) return st;
-    JoinParams j = {reinterpret_cast<const float2 *>(ws + l.parts), reinterpret_cast<const float *>(ws + l.picked),
-                    bf16 ? nullptr : reinterpret_cast<const float *>(ws + l.row_factor), &words->largest_w, targets, loss, lse, rows, vocab, l.rows_pad, slots, scale};
+    JoinParams j = {};
+    j.parts = reinterpret_cast<const float2 *>(ws + l.parts);
+    j.picked = reinterpret_cast<const float *>(ws + l.picked);
+    j.row_factor = bf16 ? nullptr : reinterpret_cast<const float *>(ws + l.row_factor);
+    j.largest_w = &words->largest_w;
+    j.targets = targets;
+    j.x = bf16 ? static_cast<const uint16_t *>(x) : nullptr;
+    j.w = static_cast<const uint16_t *>(w);
+    j.x_stride = x_stride;
+    j.w_stride = w_stride;
+    j.loss = loss;
+    j.lse = lse;
+    j.rows = rows;
+    j.cols = vocab;
+    j.rows_pad = l.rows_pad;
+    j.slots = slots;
+    j.width = width;
+    j.scale = scale;
     st = check_cuda(launch_kernel(k_join, dim3((rows + 31) / 32), dim3(1024), 0, s, j));
     note_launch();
     return st;
@@ -739,7 +810,7 @@ struct HeadCall {
       e.pitch = l.piece;
       e.col_base = c0;
       e.all_cols = vocab;
-      if (st == DF_OK) st = product<false, false, PARTS, 0, GradEpi<PARTS>>(a, b, rows, n, width, 1, bf16, e, s);
+      if (st == DF_OK) st = product<false, false, PARTS, GradEpi<PARTS>>(a, b, rows, n, width, 1, bf16, e, s);
       const Operand g = {e.g, e.g_lo, false, rows, n, l.piece};
       if (st == DF_OK && d_x) {
         if (c0 == 0) splits = slices((n + kProdK - 1) / kProdK, splits);
@@ -750,7 +821,7 @@ struct HeadCall {
         o.add = c0 > 0;
         o.rows = rows;
         o.cols = width;
-        st = product<false, true, PARTS, 0, OutEpi>(g, wp, rows, width, n, splits, false, o, s);
+        st = product<false, true, PARTS, OutEpi>(g, wp, rows, width, n, splits, false, o, s);
       }
       if (st == DF_OK && d_w) {
         OutEpi::Params o = {};
@@ -762,7 +833,7 @@ struct HeadCall {
         o.scale = scale;
         o.rows = n;
         o.cols = width;
-        st = product<true, true, PARTS, 0, OutEpi>(g, packed(l.x_grad, rows, false), n, width, rows, 1, false, o, s);
+        st = product<true, true, PARTS, OutEpi>(g, packed(l.x_grad, rows, false), n, width, rows, 1, false, o, s);
       }
     }
     if (st != DF_OK || !d_x) return st;

@@ -13,8 +13,8 @@
 //                turn), 128-byte swizzle;
 //   warp 1       issues the products into one of two accumulators in tensor memory;
 //   warps 4-11   the epilogue of one tile under the products of the next: a warp has the 32 rows of its quarter of tensor memory, a row
-//                a lane, and half of the tile's columns, 32 at a time. With CHUNK its sums are 128 registers a thread, which it takes over from warps 0-3.
-// The tile is 256 x 256 over a pair of CTAs (cta_group::2): 32 KB a CTA and part for 512 cycles of products.
+//                a lane, and half of the tile's columns, 32 at a time. With PARTS = 2 its sums are 128 registers a thread, which it takes over from warps 0-3.
+// The tile is 256 x 256 over a pair of CTAs (cta_group::2: 32 KB a CTA and part for 512 cycles of products), or 128 x 128 of one.
 // Tiles that run at the same time share the operand with the more rows (K-major B: the output weight, by the tiles of all rows; MN-major B: the gradient of the
 // logits, by the tiles of the width): it is read from HBM once.
 // The contraction can be split: tile z * tiles + t is slice z of tile t, and the epilogue is told z.
@@ -73,21 +73,21 @@ __device__ __forceinline__ bool prod_wait_warp(uint32_t bar, uint32_t parity, vo
   return __all_sync(0xffffffffu, prod_wait(bar, parity, abort_flag)) != 0;
 }
 
-// CHUNK (bf16 only): blocks between takings out of sums, 0: none before the end of the tile.
-template <bool A_MN_, bool B_MN_, int PARTS_, int CHUNK_>
+// PAIR: tiles of 256 x 256 over two CTAs, else 128 x 128 of one: twice the operands' bytes for the same products, but a quarter of the tile, and with half the sums a
+// thread four accumulators, so that results are written under the next tile's products.
+template <bool PAIR_, bool A_MN_, bool B_MN_, int PARTS_>
 struct ProdCfg {
-  static constexpr bool A_MN = A_MN_, B_MN = B_MN_;
-  static constexpr int PARTS = PARTS_;
-  static constexpr int TM = 256, TN = 256;
-  static constexpr bool kSums = PARTS == 2 || CHUNK_ > 0;  // sums in registers
-  static constexpr int kChunk = PARTS == 2 ? kProdChunk : CHUNK_ > 0 ? CHUNK_ : 0x40000000;
+  static constexpr bool PAIR = PAIR_, A_MN = A_MN_, B_MN = B_MN_;
+  static constexpr int PARTS = PARTS_, kCtas = PAIR ? 2 : 1, T = PAIR ? 256 : 128;
+  static constexpr bool kSums = PARTS == 2;  // sums in registers
+  static constexpr int kChunk = kSums ? kProdChunk : 0x40000000;
   static constexpr uint32_t kTileBytes = 128 * kProdK * 2, kStageBytes = 2 * kTileBytes;
   static constexpr int kStages = 6;
   static constexpr uint32_t kSmemStaging = kStages * kStageBytes;
   static constexpr uint32_t kSmemBars = kSmemStaging + kProdEpiWarps * kProdSlabBytes;
   static constexpr uint32_t kSmemTotal = kSmemBars + 256 + 1024;
-  static constexpr uint32_t kTmemCols = 2 * TN;
-  static constexpr int FULL = 0, EMPTY = FULL + kStages, ACC_FULL = EMPTY + kStages, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2, NUM_BARS = DRAIN + 1;
+  static constexpr int kAccs = 512 / T;
+  static constexpr int FULL = 0, EMPTY = FULL + kStages, ACC_FULL = EMPTY + kStages, ACC_EMPTY = ACC_FULL + kAccs, DRAIN = ACC_EMPTY + kAccs, NUM_BARS = DRAIN + 1;
   static_assert(NUM_BARS * 8 <= 192 && kSmemTotal <= 227 * 1024, "shared memory");
 };
 
@@ -98,7 +98,8 @@ __global__ void __launch_bounds__(kProdThreads, 1)
 k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA_lo, const __grid_constant__ CUtensorMap tmB,
           const __grid_constant__ CUtensorMap tmB_lo, const __grid_constant__ ProductParams p, const __grid_constant__ typename Epi::Params e) {
   using namespace ptx;
-  constexpr int kStages = C::kStages, TN = C::TN;
+  constexpr int kStages = C::kStages, T = C::T;
+  constexpr bool PAIR = C::PAIR;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t a0 = smem_u32(smem);
@@ -106,28 +107,34 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
   volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + C::kSmemBars + 192);
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(smem + C::kSmemBars + 196);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
   auto bar = [&](int id) { return smem_u32(&bars[id]); };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::NUM_BARS; ++i) mbar_init(bar(i), i == C::ACC_EMPTY || i == C::ACC_EMPTY + 1 ? 2 * kProdEpiWarps : 1);
+    for (int i = 0; i < C::NUM_BARS; ++i) mbar_init(bar(i), i >= C::ACC_EMPTY && i < C::DRAIN ? C::kCtas * kProdEpiWarps : 1);
     *abort_flag = 0;
     mbar_init_fence();
   }
   if (warp == 1) {
-    tmem_alloc_pair(smem_u32(tmem_holder), C::kTmemCols);
-    tmem_relinquish_pair();
+    if (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_holder), 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_holder), 512);
+      tmem_relinquish();
+    }
   }
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
   }
   tc_fence_before_sync();
-  cluster_sync();
+  if (PAIR) cluster_sync();
+  else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_holder;
   pdl_wait();
-  const long long first_tile = blockIdx.x / 2, tile_step = gridDim.x / 2;
+  const long long first_tile = blockIdx.x / C::kCtas, tile_step = gridDim.x / C::kCtas;
 
   auto decode = [&](long long id, int *kb0, int *kb1) {
     ProductTile t;
@@ -150,22 +157,26 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         for (long long id = first_tile; ok && id < p.tiles; id += tile_step) {
           int kb0, kb1;
           const ProductTile t = decode(id, &kb0, &kb1);
-          const int row_a = t.m_tile * C::TM + (int)rank * 128, row_b = t.n_tile * TN + (int)rank * 128;
+          const int row_a = t.m_tile * T + (int)rank * 128, row_b = t.n_tile * T + (int)rank * 128;
           for (int kb = kb0; ok && kb < kb1; ++kb) {
 #pragma unroll
             for (int lo = C::PARTS - 1; lo >= 0; --lo, ++it) {
               const uint32_t s = it % kStages, use = it / kStages;
               if (use > 0 && !prod_wait(bar(C::EMPTY + s), (use - 1) & 1, abort_flag)) { ok = false; break; }
               const uint32_t sa = a0 + s * C::kStageBytes;
-              // both CTAs' copies count on the even CTA's barrier, which expects the bytes of both
-              const uint32_t full = map_to_rank(bar(C::FULL + s), 0);
-              if (rank == 0) mbar_arrive_expect_tx(bar(C::FULL + s), 2 * C::kStageBytes);
+              // in a pair both CTAs' copies count on the even CTA's barrier, which expects the bytes of both
+              const uint32_t full = PAIR ? map_to_rank(bar(C::FULL + s), 0) : bar(C::FULL + s);
+              if (rank == 0) mbar_arrive_expect_tx(bar(C::FULL + s), C::kCtas * C::kStageBytes);
+              auto copy = [&](uint32_t dst, const CUtensorMap *m, int x, int y) {
+                if (PAIR) tma_load_2d_pair(dst, m, full, x, y);
+                else tma_load_2d(dst, m, full, x, y);
+              };
               auto load = [&](uint32_t dst, const CUtensorMap *m, bool mn, int row) {
                 if (mn) {
-                  tma_load_2d_pair(dst, m, full, row, kb * kProdK);
-                  tma_load_2d_pair(dst + 8192, m, full, row + 64, kb * kProdK);
+                  copy(dst, m, row, kb * kProdK);
+                  copy(dst + 8192, m, row + 64, kb * kProdK);
                 } else {
-                  tma_load_2d_pair(dst, m, full, kb * kProdK, row);
+                  copy(dst, m, kb * kProdK, row);
                 }
               };
               load(sa, lo ? &tmA_lo : &tmA, C::A_MN, row_a);
@@ -175,8 +186,8 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         }
       }
     } else if (warp == 1 && rank == 0) {
-      // ---------------------------------------------------------- products: the even CTA issues for both
-      const uint32_t idesc = make_idesc(p.fmt, C::TM, TN, C::A_MN ? 1 : 0, C::B_MN ? 1 : 0);
+      // ---------------------------------------------------------- products: in a pair the even CTA issues for both
+      const uint32_t idesc = make_idesc(p.fmt, T, T, C::A_MN ? 1 : 0, C::B_MN ? 1 : 0);
       uint32_t it = 0, j = 0;
       bool ok = true;
       // K-major: 16 of k are 32 bytes of a swizzled row; MN-major: 16 rows of 128 bytes, the next 64 of m or n 8192 bytes on
@@ -185,16 +196,21 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
 #pragma unroll
         for (int k = 0; k < kProdK / 16; ++k) {
           const uint64_t oa = (uint64_t)((k * (C::A_MN ? 2048 : 32)) >> 4), ob = (uint64_t)((k * (C::B_MN ? 2048 : 32)) >> 4);
-          mma_f16_ss_pair(d, da + oa, db + ob, idesc, first && k == 0 ? 0u : 1u);
+          if (PAIR) mma_f16_ss_pair(d, da + oa, db + ob, idesc, first && k == 0 ? 0u : 1u);
+          else mma_f16_ss(d, da + oa, db + ob, idesc, first && k == 0 ? 0u : 1u);
         }
+      };
+      auto commit = [&](int id) {
+        if (PAIR) mma_commit_pair(bar(id));
+        else mma_commit(bar(id));
       };
       for (long long id = first_tile; ok && id < p.tiles; id += tile_step) {
         int kb0, kb1;
         decode(id, &kb0, &kb1);
         for (int kb = kb0; ok && kb < kb1;) {
-          const uint32_t acc = j & 1, d = tmem + acc * TN;
+          const uint32_t acc = j % C::kAccs, d = tmem + acc * T;
           const int n = kb1 - kb < C::kChunk ? kb1 - kb : C::kChunk;
-          if (j >= 2 && !prod_wait_warp(bar(C::ACC_EMPTY + acc), ((j >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+          if (j >= C::kAccs && !prod_wait_warp(bar(C::ACC_EMPTY + acc), (j / C::kAccs - 1) & 1, abort_flag)) { ok = false; break; }
           if constexpr (C::PARTS == 2) {
             // the small terms of the chunk's blocks, then the large ones
             for (int i = 0; ok && i < n; ++i) {
@@ -206,7 +222,7 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
                 const uint32_t lo = a0 + s_lo * C::kStageBytes, hi = a0 + s_hi * C::kStageBytes;
                 issue(d, lo, hi + C::kTileBytes, i == 0);
                 issue(d, hi, lo + C::kTileBytes, false);
-                mma_commit_pair(bar(C::EMPTY + s_lo));
+                commit(C::EMPTY + s_lo);
               }
               __syncwarp();
             }
@@ -214,9 +230,9 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
               for (int i = 0; i < n; ++i) {
                 const uint32_t s_hi = (it + 2 * i + 1) % kStages, hi = a0 + s_hi * C::kStageBytes;
                 issue(d, hi, hi + C::kTileBytes, false);
-                mma_commit_pair(bar(C::EMPTY + s_hi));
+                commit(C::EMPTY + s_hi);
               }
-              mma_commit_pair(bar(C::ACC_FULL + acc));
+              commit(C::ACC_FULL + acc);
             }
             __syncwarp();
             it += 2 * n;
@@ -227,8 +243,8 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
               tc_fence_after_sync();
               if (elect_one()) {
                 issue(d, sa, sa + C::kTileBytes, i == 0);
-                mma_commit_pair(bar(C::EMPTY + s));
-                if (i + 1 == n) mma_commit_pair(bar(C::ACC_FULL + acc));
+                commit(C::EMPTY + s);
+                if (i + 1 == n) commit(C::ACC_FULL + acc);
               }
               __syncwarp();
             }
@@ -242,29 +258,32 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
     // ------------------------------------------------------------ epilogue
     if constexpr (C::kSums) prod_regs_more<kProdEpiRegs>();
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    constexpr int kGroups = TN / 64;  // 32-column blocks of this warp
-    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * (TN / 2);
+    constexpr int kGroups = T / 64;  // 32-column blocks of this warp
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * (T / 2);
     Epi epi(e, smem + C::kSmemStaging + (warp - 4) * kProdSlabBytes, lane);
     auto release = [&](uint32_t acc) {
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_rank(bar(C::ACC_EMPTY + acc), 0));
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_cluster(map_to_rank(bar(C::ACC_EMPTY + acc), 0));
+        else mbar_arrive(bar(C::ACC_EMPTY + acc));
+      }
     };
     uint32_t j = 0;
     bool ok = true;
     for (long long id = first_tile; ok && id < p.tiles; id += tile_step) {
       int kb0, kb1;
       const ProductTile t = decode(id, &kb0, &kb1);
-      const uint32_t row = (uint32_t)(t.m_tile * C::TM + (int)rank * 128 + quarter * 32 + lane), col0 = (uint32_t)(t.n_tile * TN + half * (TN / 2));
+      const uint32_t row = (uint32_t)(t.m_tile * T + (int)rank * 128 + quarter * 32 + lane), col0 = (uint32_t)(t.n_tile * T + half * (T / 2));
       epi.begin(t, row, col0);
       if constexpr (!C::kSums) {
-        const uint32_t acc = j & 1;
-        if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j >> 1) & 1, abort_flag)) break;
+        const uint32_t acc = j % C::kAccs;
+        if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j / C::kAccs) & 1, abort_flag)) break;
         tc_fence_after_sync();
 #pragma unroll 1
         for (int cg = 0; cg < kGroups; ++cg) {
           uint32_t r[32];
-          tmem_ld32(lane_base + acc * TN + cg * 32, r);
+          tmem_ld32(lane_base + acc * T + cg * 32, r);
           tmem_wait_ld();
           if (cg == kGroups - 1) release(acc);
           float v[32];
@@ -281,13 +300,13 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
           for (int x = 0; x < 32; ++x) sum[cg][x] = 0.0f;
 #pragma unroll 1
         for (int kb = kb0; kb < kb1; kb += C::kChunk, ++j) {
-          const uint32_t acc = j & 1;
-          if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j >> 1) & 1, abort_flag)) { ok = false; break; }
+          const uint32_t acc = j % C::kAccs;
+          if (!prod_wait_warp(bar(C::ACC_FULL + acc), (j / C::kAccs) & 1, abort_flag)) { ok = false; break; }
           tc_fence_after_sync();
 #pragma unroll
           for (int cg = 0; cg < kGroups; ++cg) {
             uint32_t r[32];
-            tmem_ld32(lane_base + acc * TN + cg * 32, r);
+            tmem_ld32(lane_base + acc * T + cg * 32, r);
             tmem_wait_ld();
             if (cg == kGroups - 1) release(acc);
 #pragma unroll
@@ -311,7 +330,10 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
   __syncthreads();
   if (*abort_flag != 0u) {
     if (warp == 1 && rank == 0) {
-      if (elect_one()) mma_commit_pair(bar(C::DRAIN));
+      if (elect_one()) {
+        if (PAIR) mma_commit_pair(bar(C::DRAIN));
+        else mma_commit(bar(C::DRAIN));
+      }
       __syncwarp();
       for (int n = 0; n < (1 << 16) && !mbar_try_wait(bar(C::DRAIN), 0); ++n) {
       }
@@ -324,10 +346,11 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
     if (threadIdx.x == 0 && p.status) atomicOr(p.status, DEV_STATUS_WAIT_EXPIRED);
     __syncthreads();
   }
-  cluster_sync();
+  if (PAIR) cluster_sync();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc_pair(tmem, C::kTmemCols);
+    if (PAIR) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
 }
 
@@ -417,10 +440,10 @@ int cluster_slots(uint32_t ctas, uint32_t smem, int regs) {
 template <class C, class Epi>
 int launch_product(const Operand &a, const Operand &b, ProductParams p, const typename Epi::Params &e, cudaStream_t s) {
   static_assert(sizeof(ProductParams) + sizeof(typename Epi::Params) + 4 * sizeof(CUtensorMap) < 4000, "kernel parameters");
-  const int slots = cluster_slots<k_product<C, Epi>>(2, C::kSmemTotal, C::kSums ? kProdLaunchRegs : 0);
+  const int slots = cluster_slots<k_product<C, Epi>>(C::kCtas, C::kSmemTotal, C::kSums ? kProdLaunchRegs : 0);
   if (slots == 0) return DF_ERR_CUDA;
-  p.m_tiles = (int)((p.M + C::TM - 1) / C::TM);
-  p.n_tiles = (int)((p.N + C::TN - 1) / C::TN);
+  p.m_tiles = (int)((p.M + C::T - 1) / C::T);
+  p.n_tiles = (int)((p.N + C::T - 1) / C::T);
   p.tiles = (long long)p.m_tiles * p.n_tiles * p.splits;
   p.status = device_status_ptr();
   CUtensorMap ma, ma_lo, mb, mb_lo;
@@ -432,8 +455,8 @@ int launch_product(const Operand &a, const Operand &b, ProductParams p, const ty
     note_status(DF_ERR_CUDA);
     return DF_ERR_CUDA;
   }
-  const long long grid = (p.tiles < slots ? p.tiles : slots) * 2;
-  const int st = check_cuda(launch_clusters(k_product<C, Epi>, 2, dim3((unsigned)grid), dim3(kProdThreads), C::kSmemTotal, s, ma, ma_lo, mb, mb_lo, p, e));
+  const long long grid = (p.tiles < slots ? p.tiles : slots) * C::kCtas;
+  const int st = check_cuda(launch_clusters(k_product<C, Epi>, C::PAIR ? 2 : 0, dim3((unsigned)grid), dim3(kProdThreads), C::kSmemTotal, s, ma, ma_lo, mb, mb_lo, p, e));
   note_launch();
   return st;
 }
