@@ -49,6 +49,33 @@ __device__ __forceinline__ float logit_factor(float scale, const float *row_fact
 // The same for the exponent of 2, above 0 also where operands are so small that it vanishes: -inf, the largest of no columns, times it stays -inf.
 __device__ __forceinline__ float exponent_factor(float c) { return fmaxf(c * kLog2e, 1.17549435e-38f); }
 
+// Four values of a row at element `at`, of which `left` are in the row: together where wide (16 bytes fp32, 8 bf16), else one by one.
+__device__ __forceinline__ void write_four(void *out, size_t at, float4 v, uint32_t left, bool bf16, bool wide) {
+  if (wide && left >= 4) {
+    if (bf16) {
+      uint2 b;
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.x) : "f"(v.y), "f"(v.x));
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.y) : "f"(v.w), "f"(v.z));
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + at) = b;
+    } else {
+      *reinterpret_cast<float4 *>(static_cast<float *>(out) + at) = v;
+    }
+    return;
+  }
+  const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (uint32_t x = 0; x < 4; ++x) {
+    if (x >= left) break;
+    if (bf16) {
+      uint32_t b;
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(0.0f), "f"(w[x]));
+      static_cast<uint16_t *>(out)[at + x] = (uint16_t)b;
+    } else {
+      static_cast<float *>(out)[at + x] = w[x];
+    }
+  }
+}
+
 // ---------------------------------------------------------------- epilogues
 struct LseEpi {
   struct Params {
@@ -243,30 +270,7 @@ struct OutEpi {
         *at = q[i];
         continue;
       }
-      const float w[4] = {q[i].x * f, q[i].y * f, q[i].z * f, q[i].w * f};
-      const size_t at = (size_t)r * p.out_stride + col;
-      if (p.vec && col + 4 <= p.cols) {
-        if (p.out_bf16) {
-          uint2 b;
-          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.x) : "f"(w[1]), "f"(w[0]));
-          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.y) : "f"(w[3]), "f"(w[2]));
-          *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) = b;
-        } else {
-          *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = make_float4(w[0], w[1], w[2], w[3]);
-        }
-        continue;
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        if (col + x >= p.cols) break;
-        if (p.out_bf16) {
-          uint32_t b;
-          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(0.0f), "f"(w[x]));
-          static_cast<uint16_t *>(p.out)[at + x] = (uint16_t)b;
-        } else {
-          static_cast<float *>(p.out)[at + x] = w[x];
-        }
-      }
+      write_four(p.out, (size_t)r * p.out_stride + col, make_float4(q[i].x * f, q[i].y * f, q[i].z * f, q[i].w * f), p.cols - col, p.out_bf16, p.vec);
     }
   }
   __device__ __forceinline__ void end() {}
@@ -484,7 +488,16 @@ __global__ void __launch_bounds__(1024) k_join(const JoinParams p) {
   p.loss[row] = fmaf(m - target, cn, l);
 }
 
-// d_x = factor * sum of the planes, in the caller's type; rows that do not count get zeros
+}  // namespace
+}  // namespace df
+
+#include "linear_ce_few.cuh"
+
+namespace df {
+namespace {
+
+// d_x = factor * sum of the planes, in the caller's type; rows that do not count get zeros. A CTA has 32 groups of four elements, and eight warps share the planes,
+// added in the order of the warps.
 struct SumParams {
   const float *planes, *grad;
   const int32_t *targets;
@@ -496,44 +509,38 @@ struct SumParams {
 };
 __global__ void __launch_bounds__(256) k_sum_planes(const SumParams p) {
   pdl_wait();
-  const uint32_t per_row = (p.width + 3) / 4;
-  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (uint64_t)per_row * p.rows) return;
+  __shared__ float4 s_sum[8][32];
+  const uint32_t per_row = (p.width + 3) / 4, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint64_t i = (uint64_t)blockIdx.x * 32 + lane;
+  const bool in = i < (uint64_t)per_row * p.rows;
   const uint32_t r = (uint32_t)(i / per_row), col = (uint32_t)(i % per_row) * 4;
+  const bool counts = in && (uint32_t)p.targets[r] < p.vocab;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if ((uint32_t)p.targets[r] < p.vocab) {
-    float inv;
-    part_scale(*p.largest_w, &inv);
-    const float f = inv * (p.scale / kGScale) * p.grad[r];
+  if (counts) {
     const float *at = p.planes + (size_t)r * p.pitch + col;
-    for (uint32_t k = 0; k < p.splits; ++k) {
+#pragma unroll 4
+    for (uint32_t k = warp; k < p.splits; k += 8) {
       const float4 a = *reinterpret_cast<const float4 *>(at + k * p.plane_size);
       v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
     }
+  }
+  s_sum[warp][lane] = v;
+  __syncthreads();
+  if (warp != 0 || !in) return;
+  for (int k = 1; k < 8; ++k) {
+    const float4 a = s_sum[k][lane];
+    v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+  }
+  if (counts) {
+    float f = p.scale * p.grad[r];
+    if (p.largest_w) {
+      float inv;
+      part_scale(*p.largest_w, &inv);
+      f = inv * (p.scale / kGScale) * p.grad[r];
+    }
     v.x *= f; v.y *= f; v.z *= f; v.w *= f;
   }
-  const size_t to = (size_t)r * p.out_stride + col;
-  const float w[4] = {v.x, v.y, v.z, v.w};
-  if (p.vec && col + 4 <= p.width) {
-    if (p.out_bf16) {
-      uint2 b;
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.x) : "f"(w[1]), "f"(w[0]));
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.y) : "f"(w[3]), "f"(w[2]));
-      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + to) = b;
-    } else {
-      *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to) = v;
-    }
-    return;
-  }
-  for (int x = 0; x < 4 && col + x < p.width; ++x) {
-    if (p.out_bf16) {
-      uint32_t b;
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(0.0f), "f"(w[x]));
-      static_cast<uint16_t *>(p.out)[to + x] = (uint16_t)b;
-    } else {
-      static_cast<float *>(p.out)[to + x] = w[x];
-    }
-  }
+  write_four(p.out, (size_t)r * p.out_stride + col, v, p.width - col, p.out_bf16, p.vec);
 }
 
 // ---------------------------------------------------------------- sizes
@@ -546,6 +553,7 @@ struct Layout {
   uint32_t piece, n_pieces; // columns of the vocabulary at a time
   uint32_t slots, rows_pad;
   int splits;               // of d_x's contraction
+  bool few;                 // linear_ce_few.cuh
 };
 
 constexpr int kMaxSplits = 16;
@@ -565,11 +573,43 @@ struct Tiles {
   }
 };
 
+constexpr uint32_t kFewBlocks = 592;
+
+// Whether the weight is better read as it is (linear_ce_few.cuh) than through the tensor cores. In us, 50257 columns of 768 in fp32: the loss of 1 row 36 against 165,
+// 8 rows 54 and 142, 16 rows 100 and 138, 24 rows 189 and 154; the gradient of 1 row 107 and 276, 8 rows 150 and 246. bf16 needs no parts: the loss of 8 rows 58 and 27; the
+// gradient of 8 rows 234 and 168, but 22 and 40 with 3000 columns of 512, where launches count (3 against 8).
+bool few_rows(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool backward) {
+  if (kFewMost * up(width, 128) * 4 > kFewSmem) return false;
+  if (!backward) return !bf16 && rows <= kFewMost;
+  return rows <= kFewGradMost && (uint64_t)rows * vocab <= (64u << 20) && (!bf16 || (uint64_t)vocab * width <= (8u << 20));
+}
+
 Layout layout(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool backward) {
   Layout l = {};
   const uint64_t parts = bf16 ? 1 : 2;
   l.pitch = (uint32_t)up(width, 64);
   l.rows_pad = (uint32_t)up(rows, 32);
+  uint64_t at = 256;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t here = at;
+    at += up(bytes, 256);
+    return here;
+  };
+  if (few_rows(rows, vocab, width, bf16, backward)) {
+    l.few = true;
+    l.slots = (vocab + 31) / 32 < kFewBlocks ? (vocab + 31) / 32 : kFewBlocks;  // CTAs of the logits
+    if (backward) {
+      l.piece = (vocab + kFewRanges - 1) / kFewRanges;  // rows of the weight of a range
+      l.splits = (int)((vocab + l.piece - 1) / l.piece);
+      l.g = take((uint64_t)rows * vocab * 4);
+      l.planes = take((uint64_t)l.splits * rows * l.pitch * 4);
+    } else {
+      l.parts = take((uint64_t)l.slots * l.rows_pad * 8);
+      l.picked = take((uint64_t)rows * 4);
+    }
+    l.total = at;
+    return l;
+  }
   uint64_t per_col = (uint64_t)l.pitch * 2 * parts;
   if (backward && (uint64_t)rows * 2 * parts > per_col) per_col = (uint64_t)rows * 2 * parts;
   const uint64_t all = (vocab + 255) / 256;  // tiles of the vocabulary
@@ -601,12 +641,6 @@ Layout layout(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool bac
   }
   l.piece = (uint32_t)piece * 256;
   l.n_pieces = (uint32_t)((all + piece - 1) / piece);
-  uint64_t at = 256;
-  auto take = [&](uint64_t bytes) {
-    const uint64_t here = at;
-    at += up(bytes, 256);
-    return here;
-  };
   l.row_factor = take((uint64_t)rows * 4);
   l.x_parts = take((uint64_t)rows * l.pitch * 2 * parts);
   l.w_parts = take((uint64_t)l.piece * l.pitch * 2 * parts);
@@ -634,18 +668,20 @@ int slices(uint32_t n, int wanted) {
   return (int)((n + each - 1) / each);
 }
 
-// Time in us of a product's waves of tiles with n blocks of 64 of the contraction each: a pair of CTAs takes about `PAIR` a block and writes results of parts while
-// no sums are added up, one CTA its operands' bytes, under which results are written.
-double tile_time(int parts, bool pair, uint64_t tiles, uint64_t n) {
-  const double block = parts == 2 ? (pair ? 1.2 : 1.0) : (pair ? 0.4 : 0.5), results = pair ? 4.0 : 2.5;
-  const double each = parts == 2 && pair ? block * (double)n + results : block * (double)n > results ? block * (double)n : results;
+// Time in us of waves of tiles of parts with n blocks of 64 of the contraction each. A pair of CTAs writes its results while no sums are added up; one CTA takes the time
+// that its operands' bytes take, and writes results meanwhile.
+double tile_time(bool pair, uint64_t tiles, uint64_t n) {
+  const double each = pair ? 1.2 * (double)n + 4.0 : n > 2 ? (double)n : 2.5;
   return (double)((tiles + (pair ? kPairs : 2 * kPairs) - 1) / (pair ? kPairs : 2 * kPairs)) * each;
 }
 
+// Which tiles. bf16: always pairs (1000 x 5000 rows of 768: 19 us and 21, 4096 x 50257: 204 and 304, the gradient 63 and 64, 8192 x 50257: 1739 and 2178). Parts: by the
+// estimate (777 x 10007 rows of 330, gradient: pairs 157 us, single CTAs 122; 2048 x 50257 of 768: 415 and 487).
 bool pairs(int parts, uint32_t M, uint32_t N, uint32_t K, int splits) {
+  if (parts == 1) return true;
   const uint32_t n_kb = (K + kProdK - 1) / kProdK, each = (n_kb + splits - 1) / splits;
   auto tiles = [&](uint64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t) * (uint64_t)slices(n_kb, splits); };
-  return tile_time(parts, true, tiles(256), each) < tile_time(parts, false, tiles(128), each);
+  return tile_time(true, tiles(256), each) < tile_time(false, tiles(128), each);
 }
 
 template <bool A_MN, bool B_MN, int PARTS, class Epi>
@@ -657,8 +693,9 @@ int product(const Operand &a, const Operand &b, uint32_t M, uint32_t N, uint32_t
   p.splits = slices(p.n_kb, splits);
   p.kb_per_split = (p.n_kb + splits - 1) / splits;
   p.fmt = bf16 ? (uint32_t)kFmtBF16 : (uint32_t)kFmtF16;
-  return pairs(PARTS, M, N, K, splits) ? launch_product<ProdCfg<true, A_MN, B_MN, PARTS>, Epi>(a, b, p, e, s)
-                                       : launch_product<ProdCfg<false, A_MN, B_MN, PARTS>, Epi>(a, b, p, e, s);
+  if constexpr (PARTS == 2)
+    if (!pairs(PARTS, M, N, K, splits)) return launch_product<ProdCfg<false, A_MN, B_MN, PARTS>, Epi>(a, b, p, e, s);
+  return launch_product<ProdCfg<true, A_MN, B_MN, PARTS>, Epi>(a, b, p, e, s);
 }
 
 struct HeadCall {
@@ -720,7 +757,108 @@ struct HeadCall {
     return pack(x, x_stride, rows, l.x_parts, bf16, nullptr, bf16 ? nullptr : reinterpret_cast<float *>(ws + l.row_factor), nullptr, nullptr);
   }
 
+  int join(float *loss, float *lse, uint32_t slots, bool again) const {  // again: targets' logits in rounded sums
+    const Words *words = reinterpret_cast<const Words *>(ws);
+    JoinParams j = {};
+    j.parts = reinterpret_cast<const float2 *>(ws + l.parts);
+    j.picked = reinterpret_cast<const float *>(ws + l.picked);
+    j.row_factor = bf16 || l.few ? nullptr : reinterpret_cast<const float *>(ws + l.row_factor);
+    j.largest_w = &words->largest_w;
+    j.targets = targets;
+    j.x = again ? static_cast<const uint16_t *>(x) : nullptr;
+    j.w = static_cast<const uint16_t *>(w);
+    j.x_stride = x_stride;
+    j.w_stride = w_stride;
+    j.loss = loss;
+    j.lse = lse;
+    j.rows = rows;
+    j.cols = vocab;
+    j.rows_pad = l.rows_pad;
+    j.slots = slots;
+    j.width = width;
+    j.scale = scale;
+    const int st = check_cuda(launch_kernel(k_join, dim3((rows + 31) / 32), dim3(1024), 0, s, j));
+    note_launch();
+    return st;
+  }
+  int sum_planes(const float *grad, void *d_x, uint64_t dx_stride, int splits, const uint32_t *largest_w) const {
+    const uint32_t elt = bf16 ? 2 : 4, wide = bf16 ? 7 : 15;
+    SumParams q = {};
+    q.planes = reinterpret_cast<const float *>(ws + l.planes);
+    q.grad = grad;
+    q.targets = targets;
+    q.largest_w = largest_w;
+    q.out = d_x;
+    q.out_stride = dx_stride;
+    q.plane_size = (uint64_t)rows * l.pitch;
+    q.rows = rows;
+    q.width = width;
+    q.pitch = l.pitch;
+    q.splits = (uint32_t)splits;
+    q.vocab = vocab;
+    q.out_bf16 = bf16;
+    q.vec = ((reinterpret_cast<uintptr_t>(d_x) | (dx_stride * elt)) & wide) == 0;
+    q.scale = scale;
+    const int st = check_cuda(launch_kernel(k_sum_planes, dim3((unsigned)(((uint64_t)rows * ((width + 3) / 4) + 31) / 32)), dim3(256), 0, s, q));
+    note_launch();
+    return st;
+  }
+
+  FewParams few() const {
+    FewParams p = {};
+    p.x = x;
+    p.w = w;
+    p.targets = targets;
+    p.x_stride = x_stride;
+    p.w_stride = w_stride;
+    p.rows = rows;
+    p.vocab = vocab;
+    p.width = width;
+    p.padded = (uint32_t)up(width, 128);
+    p.rows_pad = l.rows_pad;
+    const uint64_t elt = bf16 ? 2 : 4;
+    p.wide = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | (x_stride * elt) | (w_stride * elt)) & (bf16 ? 7u : 15u)) == 0;
+    p.scale = scale;
+    return p;
+  }
+  int forward_few(float *loss, float *lse) const {
+    FewParams p = few();
+    p.parts = reinterpret_cast<float2 *>(ws + l.parts);
+    p.picked = reinterpret_cast<float *>(ws + l.picked);
+    const int st = bf16 ? launch_few_logits<true, false>(p, l.slots, s) : launch_few_logits<false, false>(p, l.slots, s);
+    return st != DF_OK ? st : join(loss, lse, l.slots, false);
+  }
+  int backward_few(const float *lse, const float *grad, void *d_x, uint64_t dx_stride, void *d_w, uint64_t dw_stride) const {
+    FewParams p = few();
+    p.lse = lse;
+    p.g = reinterpret_cast<float *>(ws + l.g);
+    int st = bf16 ? launch_few_logits<true, true>(p, l.slots, s) : launch_few_logits<false, true>(p, l.slots, s);
+    if (st != DF_OK) return st;
+    FewGradParams q = {};
+    q.x = x;
+    q.w = w;
+    q.targets = targets;
+    q.g = p.g;
+    q.grad = grad;
+    q.d_w = d_w;
+    q.planes = d_x ? reinterpret_cast<float *>(ws + l.planes) : nullptr;
+    q.x_stride = x_stride;
+    q.w_stride = w_stride;
+    q.dw_stride = dw_stride;
+    q.rows = rows;
+    q.vocab = vocab;
+    q.width = width;
+    q.pitch = l.pitch;
+    q.range = l.piece;
+    q.wide = p.wide;
+    q.dw_wide = ((reinterpret_cast<uintptr_t>(d_w) | (dw_stride * (bf16 ? 2 : 4))) & (bf16 ? 7u : 15u)) == 0;
+    q.scale = scale;
+    st = bf16 ? launch_few_gradients<true>(q, s) : launch_few_gradients<false>(q, s);
+    return st != DF_OK || !d_x ? st : sum_planes(grad, d_x, dx_stride, l.splits, nullptr);
+  }
+
   int forward(float *loss, float *lse) const {
+    if (l.few) return forward_few(loss, lse);
     const Words *words = reinterpret_cast<const Words *>(ws);
     int st = DF_OK;
     if (!bf16) st = ranges(nullptr, false);
@@ -752,31 +890,12 @@ struct HeadCall {
         st = bf16 ? product<false, false, 1, LseEpi>(a, b, rows, n, width, 1, true, e, s) : product<false, false, 2, LseEpi>(a, b, rows, n, width, 1, false, e, s);
     }
     if (st != DF_OK) return st;
-    JoinParams j = {};
-    j.parts = reinterpret_cast<const float2 *>(ws + l.parts);
-    j.picked = reinterpret_cast<const float *>(ws + l.picked);
-    j.row_factor = bf16 ? nullptr : reinterpret_cast<const float *>(ws + l.row_factor);
-    j.largest_w = &words->largest_w;
-    j.targets = targets;
-    j.x = bf16 ? static_cast<const uint16_t *>(x) : nullptr;
-    j.w = static_cast<const uint16_t *>(w);
-    j.x_stride = x_stride;
-    j.w_stride = w_stride;
-    j.loss = loss;
-    j.lse = lse;
-    j.rows = rows;
-    j.cols = vocab;
-    j.rows_pad = l.rows_pad;
-    j.slots = slots;
-    j.width = width;
-    j.scale = scale;
-    st = check_cuda(launch_kernel(k_join, dim3((rows + 31) / 32), dim3(1024), 0, s, j));
-    note_launch();
-    return st;
+    return join(loss, lse, slots, bf16);
   }
 
   template <int PARTS>
   int backward(const float *lse, const float *grad, void *d_x, uint64_t dx_stride, void *d_w, uint64_t dw_stride) const {
+    if (l.few) return backward_few(lse, grad, d_x, dx_stride, d_w, dw_stride);
     const Words *words = reinterpret_cast<const Words *>(ws);
     const uint32_t elt = bf16 ? 2 : 4, wide = bf16 ? 7 : 15;
     int st = ranges(grad, d_w != nullptr);
@@ -836,26 +955,7 @@ struct HeadCall {
         st = product<true, true, PARTS, OutEpi>(g, packed(l.x_grad, rows, false), n, width, rows, 1, false, o, s);
       }
     }
-    if (st != DF_OK || !d_x) return st;
-    SumParams q = {};
-    q.planes = reinterpret_cast<const float *>(ws + l.planes);
-    q.grad = grad;
-    q.targets = targets;
-    q.largest_w = &words->largest_w;
-    q.out = d_x;
-    q.out_stride = dx_stride;
-    q.plane_size = (uint64_t)rows * l.pitch;
-    q.rows = rows;
-    q.width = width;
-    q.pitch = l.pitch;
-    q.splits = (uint32_t)splits;
-    q.vocab = vocab;
-    q.out_bf16 = bf16;
-    q.vec = ((reinterpret_cast<uintptr_t>(d_x) | (dx_stride * elt)) & wide) == 0;
-    q.scale = scale;
-    st = check_cuda(launch_kernel(k_sum_planes, dim3((unsigned)(((uint64_t)rows * ((width + 3) / 4) + 255) / 256)), dim3(256), 0, s, q));
-    note_launch();
-    return st;
+    return st != DF_OK || !d_x ? st : sum_planes(grad, d_x, dx_stride, splits, &words->largest_w);
   }
 };
 

@@ -111,7 +111,7 @@ def check_gradient(torch, x, w, targets, lse, grad, scale, d_x, d_w):
 
 
 SHAPES = [(1, 1, 1), (1, 2, 7), (2, 31, 8), (3, 32, 63), (5, 33, 64), (127, 255, 65), (128, 256, 128), (129, 257, 129), (300, 1000, 330), (257, 129, 768), (40, 3001, 777), (64, 513, 1600),
-          (9, 50257, 96), (700, 2053, 72)]
+          (9, 50257, 96), (700, 2053, 72), (4, 301, 515), (8, 9001, 130), (16, 777, 200), (17, 777, 200), (3, 12000, 770), (12, 400, 3300), (6, 300, 3300)]
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
