@@ -5,10 +5,10 @@
 //
 // Forward: one product with an epilogue that keeps of every row and 128 columns the largest logit and the sum of exponentials, and
 // the target's logit; a second kernel joins them. bf16 operands enter as they are (products exact, sums fp32). fp32 operands are cut
-// into two fp16 parts (product_sm100.cuh), x scaled row by row, w as a whole.
+// into two fp16 parts (product_sm100.cuh), both scaled row by row.
 // Backward, per piece of the vocabulary: the logits again with an epilogue that writes G in fp16 (one part for bf16 calls: 11 bits, where a
 // bf16 result has 8; two for fp32 calls: 22), then d_w = G^T x' with x' = grad * x, complete for its piece, and d_x += G w in fp32, its
-// contraction split where there are few tiles. grad is not in G, so that a row's G keeps its bits however small its weight is.
+// contraction split where there are few tiles. w and x' are contracted row by row there, so that each has one scale for all of it. grad is not in G, so that a row's G keeps its bits however small its weight is.
 #include <math.h>
 
 #include "product_sm100.cuh"
@@ -38,12 +38,11 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
   return b < 0x7f800000u ? b : 0u;
 }
 
-// What a product is times for the logit: the call's scale and, for fp32 calls, the scales of the row's parts and of the weight's.
+// What a product is times for the logit: the call's scale and, for fp32 calls, the scale of the row's parts and, where the weight has one for all of it, the weight's.
 __device__ __forceinline__ float logit_factor(float scale, const float *row_factor, const uint32_t *largest_w, uint32_t row, bool in) {
-  if (!row_factor) return scale;
-  float inv;
-  part_scale(*largest_w, &inv);
-  return scale * (in ? row_factor[row] : 1.0f) * inv;
+  float inv = 1.0f;
+  if (largest_w) part_scale(*largest_w, &inv);
+  return (row_factor && in ? scale * row_factor[row] : scale) * inv;
 }
 
 // The same for the exponent of 2, above 0 also where operands are so small that it vanishes: -inf, the largest of no columns, times it stays -inf.
@@ -80,8 +79,7 @@ __device__ __forceinline__ void write_four(void *out, size_t at, float4 v, uint3
 struct LseEpi {
   struct Params {
     const int32_t *targets;
-    const float *row_factor;     // fp32 calls: 1 / scale of a row's parts
-    const uint32_t *largest_w;   // fp32 calls
+    const float *row_factor, *col_factor;  // fp32 calls: 1 / scale of a row's parts, of x and of the weight
     float2 *parts;               // [slots][rows_pad]: largest logit (as the product has it), sum of e^(z - largest)
     float *picked;               // [rows]: the target's logit (as the product has it)
     float scale;
@@ -98,7 +96,7 @@ struct LseEpi {
     col0 = c0;
     in = r < p.rows;
     target = in ? p.targets[r] - (int)p.col_base : -1;
-    c = exponent_factor(logit_factor(p.scale, p.row_factor, p.largest_w, r, in));
+    c = exponent_factor(logit_factor(p.scale, p.row_factor, nullptr, r, in));
     m = -INFINITY;
     s = 0.0f;
   }
@@ -106,6 +104,16 @@ struct LseEpi {
   __device__ __forceinline__ void block(int cg, float (&v)[32]) {
     const uint32_t first = col0 + cg * 32;
     if (first >= p.cols) return;
+    if (p.col_factor) {
+#pragma unroll
+      for (int x = 0; x < 32; x += 4) {
+        const float4 q = __ldg(reinterpret_cast<const float4 *>(p.col_factor + first + x));  // the same for all lanes
+        v[x] *= q.x;
+        v[x + 1] *= q.y;
+        v[x + 2] *= q.z;
+        v[x + 3] *= q.w;
+      }
+    }
     const uint32_t at = (uint32_t)target - first;
     if (__any_sync(0xffffffffu, at < 32u)) {
       float z = 0.0f;
@@ -162,7 +170,7 @@ struct GradEpi {
     const int t = in ? p.targets[r] : -1;
     counts = (uint32_t)t < p.all_cols;
     target = counts ? t - (int)p.col_base : -1;
-    c = logit_factor(p.scale, p.row_factor, p.largest_w, r, in);
+    c = logit_factor(p.scale, p.row_factor, p.row_factor ? p.largest_w : nullptr, r, in);
     off = counts ? p.lse[r] : 0.0f;
   }
   // 64 bytes of a row a lane: turned over in halves of the slab, then 8 rows of 64 bytes at a time
@@ -413,7 +421,6 @@ __global__ void __launch_bounds__(256) k_pack(const PackParams p) {
 struct JoinParams {
   const float2 *parts;
   const float *picked, *row_factor;
-  const uint32_t *largest_w;
   const int32_t *targets;
   const uint16_t *x, *w;  // bf16 calls
   uint64_t x_stride, w_stride;
@@ -427,7 +434,7 @@ __global__ void __launch_bounds__(1024) k_join(const JoinParams p) {
   __shared__ float s_target[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t row = blockIdx.x * 32 + lane;
-  const float cn = logit_factor(p.scale, p.row_factor, p.largest_w, row, row < p.rows), c = exponent_factor(cn);
+  const float cn = logit_factor(p.scale, p.row_factor, nullptr, row, row < p.rows), c = exponent_factor(cn);
   if (p.x) {
     const uint32_t r = blockIdx.x * 32 + warp, t = r < p.rows ? (uint32_t)p.targets[r] : ~0u;
     float sum = 0.0f;
@@ -548,7 +555,7 @@ uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
 // What a call uses of its workspace, in bytes from its start (all of it multiples of 256).
 struct Layout {
-  uint64_t row_factor, x_parts, x_grad, w_parts, w_raw, parts, picked, g, planes, total;
+  uint64_t row_factor, col_factor, x_parts, x_grad, w_parts, w_raw, parts, picked, g, planes, total;
   uint32_t pitch;           // of rows of `width` 16-bit elements or floats
   uint32_t piece, n_pieces; // columns of the vocabulary at a time
   uint32_t slots, rows_pad;
@@ -645,6 +652,7 @@ Layout layout(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool bac
   l.x_parts = take((uint64_t)rows * l.pitch * 2 * parts);
   l.w_parts = take((uint64_t)l.piece * l.pitch * 2 * parts);
   if (!backward) {
+    l.col_factor = take((uint64_t)l.piece * 4);
     l.slots = (vocab + 63) / 64 + l.n_pieces;
     l.parts = take((uint64_t)l.slots * l.rows_pad * 8);
     l.picked = take((uint64_t)rows * 4);
@@ -758,12 +766,10 @@ struct HeadCall {
   }
 
   int join(float *loss, float *lse, uint32_t slots, bool again) const {  // again: targets' logits in rounded sums
-    const Words *words = reinterpret_cast<const Words *>(ws);
     JoinParams j = {};
     j.parts = reinterpret_cast<const float2 *>(ws + l.parts);
     j.picked = reinterpret_cast<const float *>(ws + l.picked);
     j.row_factor = bf16 || l.few ? nullptr : reinterpret_cast<const float *>(ws + l.row_factor);
-    j.largest_w = &words->largest_w;
     j.targets = targets;
     j.x = again ? static_cast<const uint16_t *>(x) : nullptr;
     j.w = static_cast<const uint16_t *>(w);
@@ -859,9 +865,7 @@ struct HeadCall {
 
   int forward(float *loss, float *lse) const {
     if (l.few) return forward_few(loss, lse);
-    const Words *words = reinterpret_cast<const Words *>(ws);
     int st = DF_OK;
-    if (!bf16) st = ranges(nullptr, false);
     Operand a;
     if (st == DF_OK) st = logits_x(&a);
     uint32_t slots = 0;
@@ -869,13 +873,13 @@ struct HeadCall {
       const uint32_t n = vocab - c0 < l.piece ? vocab - c0 : l.piece;
       Operand b = {row_of_w(c0), nullptr, true, n, width, w_stride};
       if (!(bf16 && in_place(w, w_stride))) {
-        st = pack(row_of_w(c0), w_stride, n, l.w_parts, bf16, &words->largest_w, nullptr, nullptr, nullptr);
+        st = pack(row_of_w(c0), w_stride, n, l.w_parts, bf16, nullptr, bf16 ? nullptr : reinterpret_cast<float *>(ws + l.col_factor), nullptr, nullptr);
         b = packed(l.w_parts, n, bf16);
       }
       LseEpi::Params e = {};
       e.targets = targets;
       e.row_factor = bf16 ? nullptr : reinterpret_cast<const float *>(ws + l.row_factor);
-      e.largest_w = &words->largest_w;
+      e.col_factor = bf16 ? nullptr : reinterpret_cast<const float *>(ws + l.col_factor);
       e.parts = reinterpret_cast<float2 *>(ws + l.parts);
       e.picked = reinterpret_cast<float *>(ws + l.picked);
       e.scale = scale;
