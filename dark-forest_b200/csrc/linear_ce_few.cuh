@@ -112,8 +112,7 @@ __global__ void __launch_bounds__(256) k_few_logits(const FewParams p) {
       const uint32_t r = row0 + first + o;
       if (r >= p.rows) continue;
       if constexpr (GRAD) {
-        float t = fmaf(acc[o], p.scale, -off[o]);
-        t = t > 0.0f ? 0.0f : t;  // as in linear_ce.cu
+        const float t = at_most_0(fmaf(acc[o], p.scale, -off[o]));  // as in linear_ce.cu
         const float e = (uint32_t)target[o] == v ? expm1f(t) : ex2_approx(t * kLog2e);
         p.g[(size_t)r * p.vocab + v] = (uint32_t)target[o] < p.vocab ? e : 0.0f;
       } else {
