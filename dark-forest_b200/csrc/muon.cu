@@ -742,12 +742,13 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
   }
 }
 
-// ---------------------------------------------------------------- small matrices, a CTA each
-// A matrix of at most 128 x 256 (seen with its rows the smaller side; a taller one is turned over on the way in and out) stays in shared memory as two fp16 parts
-// from its first product to its last: G, B and the new X go from tensor memory through registers to where the next product reads them, and nothing
-// between products leaves the SM (64 x 64: 33 us, where tiles that wait for a counter in global memory take 79; 128 x 128: 59 and 116).
+// ---------------------------------------------------------------- matrices with a small side, a CTA or a cluster each
+// A matrix of at most 128 rows (its smaller side; a taller one is turned over on the way in and out) stays in shared memory as two fp16 parts from its first product to
+// its last, up to 256 columns in a CTA, up to 2048 in a cluster of up to eight: G, B and the new X go from tensor memory through registers to where the next product
+// reads them. In a cluster every CTA adds up G from all CTAs' parts of it, which lie in global memory between two cluster barriers, and the rest is its own columns'.
+// Nothing else between products leaves the SM (64 x 64: 33 us, where tiles that wait for a counter in global memory take 79; 128 x 128: 59 and 116).
 // Slabs of 64 columns, 128 bytes a row, 128-byte swizzle: K-major for the products over columns, and the same bytes MN-major for B X, which contracts X's rows.
-constexpr uint32_t kSmallRows = 128, kSmallCols = 256;
+constexpr uint32_t kSmallRows = 128, kSmallCols = 256, kSmallCtas = 8;
 constexpr uint32_t kSlab = 128 * 128;                                       // bytes: 128 rows x 64 columns of one part
 constexpr uint32_t kSmallX = 0, kSmallG = 8 * kSlab, kSmallBars = 12 * kSlab;  // X: 4 slabs high, 4 low; G, then B: 2 high, 2 low
 constexpr uint32_t kSmallSmem = kSmallBars + 128 + 1024;
@@ -758,8 +759,10 @@ struct SmallParams {
   Table t;
   Targets o;
   uint64_t source_stride, out_stride;
-  uint32_t rows, cols, bf16, nesterov, apply, steps;
+  uint32_t rows, cols, bf16, nesterov, apply, steps, ctas, share;  // share: columns of a CTA
   float beta, eps, a, b, c, keep, step;
+  double *sums;   // [matrices][ctas]
+  float4 *grams;  // [matrices][2][ctas][32][128]: four columns of a row each, for odd and even steps
   unsigned int *status;
 };
 
@@ -800,23 +803,26 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
     tmem_alloc(smem_u32(tmem_holder), 512);
     tmem_relinquish();
   }
+  const int m = blockIdx.x / p.ctas, rank = blockIdx.x % p.ctas;
   const bool wide = p.rows <= p.cols;
-  const uint32_t side = wide ? p.rows : p.cols, large = wide ? p.cols : p.rows, slabs = (large + 63) / 64, side_blocks = (side + 63) / 64, halves = (large + 127) / 128;
+  const uint32_t side = wide ? p.rows : p.cols, all = wide ? p.cols : p.rows, off = rank * p.share, large = all - off < p.share ? all - off : p.share;
+  const uint32_t slabs = (large + 63) / 64, side_blocks = (side + 63) / 64, halves = (large + 127) / 128;
+  // this CTA's part of the source
+  const uint32_t rows = wide ? p.rows : large, cols = wide ? large : p.cols, row_off = wide ? 0 : off, col_off = wide ? off : 0;
   for (uint32_t i = tid; i < 8 * kSlab / 16; i += 256) reinterpret_cast<uint4 *>(smem + kSmallX)[i] = make_uint4(0u, 0u, 0u, 0u);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_holder;
   pdl_wait();
-  const int m = blockIdx.x;
   const void *source = p.t.source[m];
   float *momentum = p.t.momentum[m];
 
   // ---------------------------------------------------------------- U, its norm, X. A warp a row of the source, its lanes the columns, the same ones in both passes.
   double sum = 0.0;
-  for (uint32_t r = warp; r < p.rows; r += 8) {
+  for (uint32_t r = row_off + warp; r < row_off + rows; r += 8) {
 #pragma unroll 4
-    for (uint32_t c = lane; c < p.cols; c += 32) {
+    for (uint32_t c = col_off + lane; c < col_off + cols; c += 32) {
       float u = load_f(source, p.bf16, (size_t)r * p.source_stride + c);
       if (momentum) {
         const float v = fmaf(p.beta, momentum[r * p.cols + c], u);
@@ -832,10 +838,16 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
   __syncthreads();
   sum = 0.0;
   for (int i = 0; i < 8; ++i) sum += part[i];
+  if (p.ctas > 1) {
+    if (tid == 0) p.sums[blockIdx.x] = sum;
+    cluster_sync();
+    sum = 0.0;
+    for (uint32_t i = 0; i < p.ctas; ++i) sum += __ldcg(p.sums + m * p.ctas + i);
+  }
   const float f = (float)((double)kPartScale / (sqrt(sum) + (double)p.eps));
-  for (uint32_t r = warp; r < p.rows; r += 8) {
+  for (uint32_t r = row_off + warp; r < row_off + rows; r += 8) {
 #pragma unroll 4
-    for (uint32_t c = lane; c < p.cols; c += 32) {
+    for (uint32_t c = col_off + lane; c < col_off + cols; c += 32) {
       float u = load_f(source, p.bf16, (size_t)r * p.source_stride + c);
       if (momentum) {
         const float v = momentum[r * p.cols + c];
@@ -843,7 +855,7 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
       }
       u *= f;
       const __half h = __float2half_rn(u);
-      const uint32_t at = wide ? small_at(r, c) : small_at(c, r);
+      const uint32_t at = wide ? small_at(r, c - off) : small_at(c, r - off);
       *reinterpret_cast<__half *>(smem + kSmallX + at) = h;
       *reinterpret_cast<__half *>(smem + kSmallX + 4 * kSlab + at) = __float2half_rn(u - __half2float(h));
     }
@@ -899,16 +911,37 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
     for (int x = 0; x < 64; ++x) v[x] = 0.0f;
   };
   bool go = meet();
-  for (uint32_t step = 0; go && step < p.steps; ++step) {
+  for (uint32_t step = 0; step < p.steps; ++step) {  // to the end also where a wait has run out: the cluster's barriers are met by all
     float g[64], v[64];
-    if (warp == 0)
-      for (uint32_t c = 0; c < slabs; ++c) issue((int)c, kSmallX + c * kSlab, kSmallX + (4 + c) * kSlab, kSmallX + c * kSlab, kSmallX + (4 + c) * kSlab, false);
     clear(g);
-    for (uint32_t c = 0; c < slabs; ++c) take((int)c, g);
+    if (go) {
+      if (warp == 0)
+        for (uint32_t c = 0; c < slabs; ++c) issue((int)c, kSmallX + c * kSlab, kSmallX + (4 + c) * kSlab, kSmallX + c * kSlab, kSmallX + (4 + c) * kSlab, false);
+      for (uint32_t c = 0; c < slabs; ++c) take((int)c, g);
+    }
+    if (p.ctas > 1) {
+      // a part of step s is written when every CTA has read those of step s - 2: it has been at the barrier of step s - 1 since
+      float4 *parts = p.grams + (size_t)(m * 2 + (step & 1)) * p.ctas * 4096 + (half * 16) * 128 + row;
+#pragma unroll
+      for (int q = 0; q < 16; ++q) parts[(size_t)rank * 4096 + q * 128] = make_float4(g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]);
+      cluster_sync();
+      clear(g);
+      for (uint32_t k = 0; k < p.ctas; ++k) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const float4 x = __ldcg(parts + (size_t)k * 4096 + q * 128);
+          g[4 * q] += x.x;
+          g[4 * q + 1] += x.y;
+          g[4 * q + 2] += x.z;
+          g[4 * q + 3] += x.w;
+        }
+      }
+    }
+    if (!go) continue;
 #pragma unroll
     for (int x = 0; x < 64; ++x) g[x] *= kPartInverse;
     small_store(smem + kSmallG + half * kSlab, smem + kSmallG + (2 + half) * kSlab, row, g);
-    if (!(go = meet())) break;
+    if (!(go = meet())) continue;
     if (warp == 0)
       for (uint32_t c = 0; c < side_blocks; ++c) issue((int)c, kSmallG + c * kSlab, kSmallG + (2 + c) * kSlab, kSmallG + c * kSlab, kSmallG + (2 + c) * kSlab, false);
     clear(v);
@@ -916,7 +949,7 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
 #pragma unroll
     for (int x = 0; x < 64; ++x) v[x] = fmaf(p.c, v[x], p.b * g[x]) + ((uint32_t)(half * 64 + x) == row ? p.a : 0.0f);
     small_store(smem + kSmallG + half * kSlab, smem + kSmallG + (2 + half) * kSlab, row, v);
-    if (!(go = meet())) break;
+    if (!(go = meet())) continue;
     if (warp == 0)
       for (uint32_t h = 0; h < halves; ++h)
         for (uint32_t c = 0; c < side_blocks; ++c)
@@ -939,7 +972,7 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
     for (uint32_t c = 0; c < side_blocks; ++c) take((int)c, g);
     if (halves > 1)
       for (uint32_t c = 0; c < side_blocks; ++c) take((int)(2 + c), v);
-    if (!(go = meet())) break;
+    if (!(go = meet())) continue;
     float *x = reinterpret_cast<float *>(smem) + row * kSmallPitch + half * 64;
 #pragma unroll
     for (int i = 0; i < 64; ++i) {
@@ -950,10 +983,10 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
   __syncthreads();
   if (go) {
     const float *x = reinterpret_cast<const float *>(smem);
-    for (uint32_t r = warp; r < p.rows; r += 8) {
+    for (uint32_t r = row_off + warp; r < row_off + rows; r += 8) {
 #pragma unroll 4
-      for (uint32_t c = lane; c < p.cols; c += 32) {
-        const float y = wide ? x[r * kSmallPitch + c] : x[c * kSmallPitch + r];
+      for (uint32_t c = col_off + lane; c < col_off + cols; c += 32) {
+        const float y = wide ? x[r * kSmallPitch + c - off] : x[c * kSmallPitch + r - off];
         const size_t at = (size_t)r * p.out_stride + c;
         if (p.bf16) {
           uint32_t b;
@@ -984,15 +1017,21 @@ struct Layout {
   uint64_t done, x, x_next, g, b, total;  // offsets: parts hi, then lo, of all matrices of a group
   uint64_t x_matrix, g_matrix;      // elements of a matrix
   uint32_t x_pitch, g_pitch, side, group;
-  bool small;  // k_newton_schulz_small
+  bool small;            // k_newton_schulz_small,
+  uint32_t ctas, share;  // on so many CTAs a matrix, with so many columns each
 };
 Layout layout(uint32_t n, uint32_t rows, uint32_t cols) {
   Layout l = {};
   l.side = rows < cols ? rows : cols;
-  l.small = l.side <= kSmallRows && (rows < cols ? cols : rows) <= kSmallCols;
+  const uint32_t larger = rows < cols ? cols : rows;
+  l.small = l.side <= kSmallRows && larger <= kSmallCtas * kSmallCols;
   if (l.small) {
-    l.group = kMostMatrices;
-    l.total = 256;
+    l.ctas = (larger + kSmallCols - 1) / kSmallCols;
+    l.share = (uint32_t)up((larger + l.ctas - 1) / l.ctas, 64);
+    l.ctas = (larger + l.share - 1) / l.share;
+    l.group = n < (uint32_t)kMostMatrices ? n : (uint32_t)kMostMatrices;
+    l.g = up((uint64_t)l.group * l.ctas * 8, 256);
+    l.total = l.g + (l.ctas > 1 ? (uint64_t)l.group * 2 * l.ctas * 65536 : 0);
     return l;
   }
   l.x_pitch = (uint32_t)up(cols, 64);
@@ -1101,7 +1140,6 @@ struct Plan {
     return (double)(((which == kNext ? x : g) * n + slots - 1) / slots) * ((double)blocks + (form > 0 ? 5.0 : 1.0));
   }
 
-  // Matrices that fit one CTA's shared memory. As many at a time as there are SMs take what one takes.
   int small(uint32_t n, const UpdateParams &u, const NsParams &q) const {
     static std::atomic<bool> ready[64];
     int dev = 0;
@@ -1128,8 +1166,12 @@ struct Plan {
     p.c = c * kPartInverse;
     p.keep = q.keep;
     p.step = q.step;
+    p.ctas = l.ctas;
+    p.share = l.share;
+    p.sums = reinterpret_cast<double *>(ws);
+    p.grams = reinterpret_cast<float4 *>(ws + l.g);
     p.status = device_status_ptr();
-    const int st = check_cuda(launch_kernel(k_newton_schulz_small, dim3(n), dim3(256), kSmallSmem, s, p));
+    const int st = check_cuda(launch_clusters(k_newton_schulz_small, l.ctas > 1 ? l.ctas : 0, dim3(n * l.ctas), dim3(256), kSmallSmem, s, p));
     note_launch();
     return st;
   }

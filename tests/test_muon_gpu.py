@@ -55,7 +55,7 @@ def updates(torch, seed, n, rows, cols, dtype="fp32", size=1e-3):
     return u.to(torch.bfloat16 if dtype == "bf16" else torch.float32)
 
 
-SMALL = [(1, 1, 1), (2, 1, 40), (1, 40, 1), (3, 16, 16), (2, 31, 65), (1, 64, 128), (2, 128, 129), (1, 127, 256), (2, 256, 128), (1, 255, 3)]
+SMALL = [(1, 1, 1), (2, 1, 40), (1, 40, 1), (3, 16, 16), (2, 31, 65), (1, 64, 128), (2, 128, 129), (1, 127, 256), (2, 256, 128), (1, 255, 3), (1, 128, 257), (3, 100, 700), (2, 513, 65), (1, 2048, 128), (70, 5, 300), (1, 1, 2048), (1, 77, 2049)]
 LARGE = [(1, 129, 129), (2, 130, 257), (1, 257, 130), (1, 3, 257), (1, 1000, 5), (3, 131, 515), (1, 515, 131), (1, 384, 384), (2, 300, 701), (1, 128, 2000), (1, 640, 129), (70, 130, 130)]
 
 
