@@ -627,7 +627,7 @@ Layout layout(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool bac
   const uint64_t all = (vocab + 255) / 256;  // tiles of the vocabulary
   uint64_t most = kPieceBytes / per_col / 256, piece = all;
   if (most < 1) most = 1;
-  if (!backward && !bf16) {
+  if (!backward) {
     const uint64_t n = (all + most - 1) / most;
     piece = (all + n - 1) / n;
   }
@@ -874,10 +874,12 @@ struct HeadCall {
     Operand a;
     if (st == DF_OK) st = logits_x(&a);
     uint32_t slots = 0;
-    for (uint32_t c0 = 0; st == DF_OK && c0 < vocab; c0 += l.piece) {
-      const uint32_t n = vocab - c0 < l.piece ? vocab - c0 : l.piece;
+    const bool as_it_is = bf16 && in_place(w, w_stride);  // then all of it at a time
+    const uint32_t piece = as_it_is ? vocab : l.piece;
+    for (uint32_t c0 = 0; st == DF_OK && c0 < vocab; c0 += piece) {
+      const uint32_t n = vocab - c0 < piece ? vocab - c0 : piece;
       Operand b = {row_of_w(c0), nullptr, true, n, width, w_stride};
-      if (!(bf16 && in_place(w, w_stride))) {
+      if (!as_it_is) {
         st = pack(row_of_w(c0), w_stride, n, l.w_parts, bf16, nullptr, bf16 ? nullptr : reinterpret_cast<float *>(ws + l.col_factor), nullptr, nullptr);
         b = packed(l.w_parts, n, bf16);
       }

@@ -337,3 +337,12 @@ def test_refusals(torch):
             call()
     again = p.linear_cross_entropy(x, w, targets)
     assert torch.equal(again[0], loss) and p.sync_status() == 0
+
+
+def test_pieces_of_a_weight_that_is_copied(torch):
+    p = pkg()
+    x, w, targets = case(torch, 77, 40, 70001, 2047, "bf16", padded=0.2, stride=2049, offset=1)  # 16-byte loads cannot start at its rows: 287 MB of copies
+    assert p.linear_cross_entropy_workspace_bytes(40, 70001, 2047, True, False) < 280 << 20
+    targets[:2] = torch.tensor([0, 70000], dtype=torch.int32, device="cuda")
+    loss, lse = p.linear_cross_entropy(x, w, targets)
+    check_loss(torch, x, w, targets, 1.0, loss, lse)
