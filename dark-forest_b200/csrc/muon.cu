@@ -11,6 +11,8 @@
 // a lower number, and every CTA takes its tiles in their order, so the lowest unfinished tile never waits.
 #include <math.h>
 
+#include <algorithm>
+
 #include "product_sm100.cuh"
 
 namespace df {
@@ -22,7 +24,7 @@ constexpr float kPartScale = 4096.0f, kPartInverse = 1.0f / 4096.0f;
 constexpr int kMostMatrices = 64;               // of a group: what the kernels' tables of pointers hold
 constexpr uint64_t kGroupBytes = 192ull << 20;  // of workspace, beyond one matrix: what L2 loses between products is read again
 constexpr int kNormBlocks = 256;                // partial sums of squares per matrix, at most
-constexpr uint32_t kMostTensors = 1024;         // of an optimiser step: every pair is checked for overlap
+constexpr uint32_t kMostTensors = 1024;         // of an optimiser step
 
 int finish(int st) {
   note_status(st);
@@ -1260,6 +1262,29 @@ int check_call(uint32_t n, uint32_t rows, uint32_t cols, uint32_t steps, float a
   return fabsf(a) + fabsf(b) + fabsf(c) < 15.0f ? DF_OK : DF_ERR_UNSUPPORTED;
 }
 
+bool meet(const void *x, uint64_t x_bytes, const void *y, uint64_t y_bytes) {  // whether they share memory
+  const uintptr_t u = reinterpret_cast<uintptr_t>(x), v = reinterpret_cast<uintptr_t>(y);
+  return u < v + y_bytes && v < u + x_bytes;
+}
+// Whether a parameter or a momentum, which are written, shares memory with anything else of the table. All are of the same size, so of two in order of their
+// addresses that meet, the first meets its successor and the second its predecessor.
+bool tensors_meet(const df_muon_tensor_t *t, uint32_t n, uint64_t bytes) {
+  struct Held {
+    uintptr_t at;
+    bool written;
+  } all[3 * kMostTensors];
+  uint32_t k = 0;
+  for (uint32_t i = 0; i < n; ++i) {
+    all[k++] = {reinterpret_cast<uintptr_t>(t[i].parameter), true};
+    all[k++] = {reinterpret_cast<uintptr_t>(t[i].momentum), true};
+    all[k++] = {reinterpret_cast<uintptr_t>(t[i].gradient), false};
+  }
+  std::sort(all, all + k, [](const Held &x, const Held &y) { return x.at < y.at; });
+  for (uint32_t i = 1; i < k; ++i)
+    if ((all[i].written || all[i - 1].written) && all[i].at - all[i - 1].at < bytes) return true;
+  return false;
+}
+
 bool aligned(const void *p, uint64_t row_bytes, uint64_t to) { return ((reinterpret_cast<uintptr_t>(p) | row_bytes) & (to - 1)) == 0; }
 
 }  // namespace
@@ -1285,15 +1310,14 @@ int df_orthogonalize(const void *update, void *out, void *workspace, uint64_t wo
   if (update_matrix_stride >= most || update_row_stride >= most || out_matrix_stride >= most || out_row_stride >= most) return finish(DF_ERR_INVALID_ARG);
   if (rows > 1 && (update_row_stride < cols || out_row_stride < cols)) return finish(DF_ERR_INVALID_ARG);
   if (n > 1 && out_matrix_stride < (uint64_t)(rows - 1) * out_row_stride + cols) return finish(DF_ERR_INVALID_ARG);
-  {  // out is the update, element by element, or shares nothing with it
-    const uint64_t e = bf16 ? 2 : 4, in_rows = rows - 1, in_all = (uint64_t)(n - 1);
-    const uintptr_t u0 = reinterpret_cast<uintptr_t>(update), u1 = u0 + (in_all * update_matrix_stride + in_rows * update_row_stride + cols) * e;
-    const uintptr_t o0 = reinterpret_cast<uintptr_t>(out), o1 = o0 + (in_all * out_matrix_stride + in_rows * out_row_stride + cols) * e;
-    const bool same = u0 == o0 && (rows == 1 || update_row_stride == out_row_stride) && (n == 1 || update_matrix_stride == out_matrix_stride);
-    if (!same && u0 < o1 && o0 < u1) return finish(DF_ERR_INVALID_ARG);
-  }
+  // out is the update, element by element, or shares nothing with it
+  const uint64_t in_elt = bf16 ? 2 : 4, in_bytes = ((uint64_t)(n - 1) * update_matrix_stride + (uint64_t)(rows - 1) * update_row_stride + cols) * in_elt;
+  const uint64_t out_bytes = ((uint64_t)(n - 1) * out_matrix_stride + (uint64_t)(rows - 1) * out_row_stride + cols) * in_elt;
+  const bool same = update == out && (rows == 1 || update_row_stride == out_row_stride) && (n == 1 || update_matrix_stride == out_matrix_stride);
+  if (!same && meet(update, in_bytes, out, out_bytes)) return finish(DF_ERR_INVALID_ARG);
   const Layout l = layout(n, rows, cols);
   if (!workspace || workspace_bytes < l.total || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return finish(DF_ERR_WORKSPACE);
+  if (meet(update, in_bytes, workspace, l.total) || meet(out, out_bytes, workspace, l.total)) return finish(DF_ERR_INVALID_ARG);
   const Plan plan = {rows, cols, steps, a, b, c, eps, static_cast<uint8_t *>(workspace), l, static_cast<cudaStream_t>(stream)};
   const uint64_t elt = bf16 ? 2 : 4;
   for (uint32_t i0 = 0; st == DF_OK && i0 < n; i0 += l.group) {
@@ -1329,19 +1353,12 @@ int df_muon_update(const void *tensors, uint32_t n, uint32_t rows, uint32_t cols
   if (n > kMostTensors) return finish(DF_ERR_UNSUPPORTED);
   for (uint32_t i = 0; i < n; ++i)
     if (!t[i].parameter || !t[i].momentum || !t[i].gradient) return finish(DF_ERR_INVALID_ARG);
-  const uint64_t bytes = (uint64_t)rows * cols * 4;
-  auto meet = [&](const void *x, const void *y) {
-    const uintptr_t u = reinterpret_cast<uintptr_t>(x), v = reinterpret_cast<uintptr_t>(y);
-    return u < v + bytes && v < u + bytes;
-  };
-  for (uint32_t i = 0; i < n; ++i) {  // what is written may not be anything else of the call
-    for (uint32_t j = 0; j < n; ++j)
-      if (meet(t[i].parameter, t[j].momentum) || meet(t[i].parameter, t[j].gradient) || meet(t[i].momentum, t[j].gradient) ||
-          (i < j && (meet(t[i].parameter, t[j].parameter) || meet(t[i].momentum, t[j].momentum))))
-        return finish(DF_ERR_INVALID_ARG);
-  }
+  if (tensors_meet(t, n, (uint64_t)rows * cols * 4)) return finish(DF_ERR_INVALID_ARG);
   const Layout l = layout(n, rows, cols);
   if (!workspace || workspace_bytes < l.total || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return finish(DF_ERR_WORKSPACE);
+  for (uint32_t i = 0; i < n; ++i)
+    for (const void *p : {static_cast<const void *>(t[i].parameter), static_cast<const void *>(t[i].momentum), static_cast<const void *>(t[i].gradient)})
+      if (meet(p, (uint64_t)rows * cols * 4, workspace, l.total)) return finish(DF_ERR_INVALID_ARG);
   const Plan plan = {rows, cols, steps, a, b, c, eps, static_cast<uint8_t *>(workspace), l, static_cast<cudaStream_t>(stream)};
   for (uint32_t i0 = 0; st == DF_OK && i0 < n; i0 += l.group) {
     const uint32_t k = n - i0 < l.group ? n - i0 : l.group;

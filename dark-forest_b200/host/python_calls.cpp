@@ -673,9 +673,8 @@ PyObject *orthogonalize(Args a) {  // update steps coefficients eps out workspac
 
 class Sequence {  // a list or tuple of tensors
  public:
-  Sequence(PyObject *o, const char *what) : s_(PySequence_Tuple(o)) {
+  explicit Sequence(PyObject *o) : s_(PySequence_Tuple(o)) {
     if (!s_) throw PythonError();
-    (void)what;
   }
   Sequence(const Sequence &) = delete;
   Sequence &operator=(const Sequence &) = delete;
@@ -688,7 +687,7 @@ class Sequence {  // a list or tuple of tensors
 };
 
 PyObject *muon_update(Args a) {  // parameters momenta gradients lr momentum weight_decay nesterov update_scale steps coefficients eps workspace stream
-  const Sequence p(a[0], "parameters"), m(a[1], "momenta"), g(a[2], "gradients");
+  const Sequence p(a[0]), m(a[1]), g(a[2]);
   if (m.size() != p.size() || g.size() != p.size()) refuse("parameters", "as many parameters, momenta and gradients are expected");
   if (p.size() == 0) Py_RETURN_NONE;
   const OnDevice on(p[0], "parameters");

@@ -489,11 +489,12 @@ DF_API int df_linear_cross_entropy_backward(const void *x, const void *weight, c
  *       overlap it otherwise.
  *   df_muon_update     n tensors [rows][cols] fp32, contiguous, described by df_muon_tensor_t entries in HOST memory, read before the call returns (up to 1024):
  *       momentum <- beta momentum + gradient; U = gradient + beta momentum (nesterov != 0) or momentum;
- *       parameter <- parameter (1 - lr weight_decay) - lr update_scale O(U). No tensor may overlap another.
+ *       parameter <- parameter (1 - lr weight_decay) - lr update_scale O(U). No parameter or momentum may overlap another tensor.
  * Precision: factors in 22 bits relative to 1 (elements below 2^-26 in fewer, none below 2^-37), sums in fp32, the norm in double, results rounded once.
  * |a| + |b| + |c| below 15 (else DF_ERR_UNSUPPORTED); singular values that a step brings above 3.8 make the matrix's results infinite or NaN. A zero matrix gives 0
  * (eps > 0), an infinity or NaN NaN, both without touching the other matrices. Nothing depends on the order of execution.
- * workspace: df_orthogonalize_workspace_bytes (for both calls; at most 192 MB or one matrix), 256-byte aligned, contents undefined before and after. Calls that can overlap need one each. */
+ * workspace: df_orthogonalize_workspace_bytes (for both calls; at most 192 MB or one matrix), 256-byte aligned, contents undefined before and after, apart
+ * from the call's tensors. Calls that can overlap need one each. */
 typedef struct df_muon_tensor {
   float *parameter;
   float *momentum;

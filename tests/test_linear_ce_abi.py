@@ -129,3 +129,31 @@ def test_optimiser_refuses(lib):
         assert muon(lib, **kw) == p.DF_ERR_INVALID_ARG, kw
     assert muon(lib, n=1025) == p.DF_ERR_UNSUPPORTED
     assert lib.df_muon_update(None, 1, 4, 8, 0.1, 0.9, 0.0, 1, 1.0, 5, 3.0, -4.0, 2.0, 1e-7, aligned(5), 1 << 40, None) == p.DF_ERR_INVALID_ARG
+
+
+def test_matrices_in_the_workspace(lib):
+    p = pkg()
+    inside = ctypes.c_void_p(aligned(5).value + 128)  # 4 x 8 in fp32 need more than that of it
+    assert orth(lib, u=inside) == p.DF_ERR_INVALID_ARG and orth(lib, out=inside) == p.DF_ERR_INVALID_ARG and orth(lib, u=inside, out=inside) == p.DF_ERR_INVALID_ARG
+    for t in ((inside, at(1), at(2)), (at(0), inside, at(2)), (at(0), at(1), inside)):
+        assert muon(lib, tensors=table(t)) == p.DF_ERR_INVALID_ARG
+
+
+def test_overlaps_among_many_tensors(lib):
+    p = pkg()
+    n, each = 341, 4 * 8 * 4
+    places = [ctypes.c_void_p(at(0).value + i * each) for i in range(3 * n)]
+    for i, j in ((0, 3 * n - 1), (3 * n - 1, 1), (4, 600), (302, 301)):  # a parameter or momentum moved onto the end of another tensor
+        moved = list(places)
+        k = i if i % 3 != 2 else j
+        moved[k] = ctypes.c_void_p(places[j if k == i else i].value + each - 4)
+        assert muon(lib, tensors=table(*[tuple(moved[3 * x:3 * x + 3]) for x in range(n)]), n=n) == p.DF_ERR_INVALID_ARG
+    # the same gradient for two parameters is none: what is refused is only the missing workspace
+    shared = [tuple(places[3 * x:3 * x + 3]) for x in range(n)]
+    shared[7] = shared[7][:2] + (shared[200][2],)
+    assert muon(lib, tensors=table(*shared), n=n, ws=None) == p.DF_ERR_WORKSPACE
+
+
+def test_a_weight_that_has_to_be_copied_is_so_in_pieces(lib):
+    size = lib.df_linear_cross_entropy_workspace_bytes
+    assert size(64, 1 << 18, 16384, 1, 0) < 300 << 20 and size(64, 1 << 18, 16384, 0, 0) < 300 << 20
