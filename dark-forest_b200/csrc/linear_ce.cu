@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(256) k_pack(const PackParams p) {
   }
 }
 
-// loss and lse of 32 rows a block: lanes are rows, warps share the slots. For bf16 calls a warp also takes a row's target again, in fp32 sums that are rounded: the tensor
+// loss and lse of `group` rows a block, 32 / group lanes of each of 32 warps and row: they share the slots, then a warp a row joins what the warps have. For bf16 calls it also takes a row's target again, in fp32 sums that are rounded: the tensor
 // cores cut the sum of a whole row off at each 16 of it, which a target's logit, a sum of terms of one sign where the model has learned something, feels most (4096
 // rows of 768: the loss 1.0e-6 off 64 bits without). With d what the logit lacks, sum e^z grows by p (e^d - 1) of itself.
 struct JoinParams {
@@ -430,21 +430,41 @@ struct JoinParams {
   const uint16_t *x, *w;  // bf16 calls
   uint64_t x_stride, w_stride;
   float *loss, *lse;
-  uint32_t rows, cols, rows_pad, slots, width;
+  uint32_t rows, cols, rows_pad, slots, width, group;  // group: a power of two, at most 32
   float scale;
 };
 __global__ void __launch_bounds__(1024) k_join(const JoinParams p) {
   pdl_wait();
   __shared__ float2 s_part[32][33];
-  __shared__ float s_target[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t row = blockIdx.x * 32 + lane;
-  const float cn = logit_factor(p.scale, p.row_factor, nullptr, row, row < p.rows), c = exponent_factor(cn);
-  if (p.x) {
-    const uint32_t r = blockIdx.x * 32 + warp, t = r < p.rows ? (uint32_t)p.targets[r] : ~0u;
+  float m = -INFINITY, s = 0.0f, c;
+  auto join = [&](float2 q) {
+    const float top = fmaxf(m, q.x), ref = top == -INFINITY ? 0.0f : top;
+    s = s * ex2_approx((m - ref) * c) + q.y * ex2_approx((q.x - ref) * c);
+    m = top;
+  };
+  auto join_lanes = [&](uint32_t from) {
+#pragma unroll 1
+    for (uint32_t d = from; d < 32; d <<= 1) join(make_float2(__shfl_xor_sync(0xffffffffu, m, d), __shfl_xor_sync(0xffffffffu, s, d)));
+  };
+  {
+    const uint32_t r = lane & (p.group - 1), first = blockIdx.x * p.group + r, lanes = 32 / p.group;
+    c = exponent_factor(logit_factor(p.scale, p.row_factor, nullptr, first, first < p.rows));
+    if (first < p.rows) {
+#pragma unroll 4
+      for (uint32_t i = warp * lanes + lane / p.group; i < p.slots; i += 32 * lanes) join(p.parts[(size_t)i * p.rows_pad + first]);
+    }
+    join_lanes(p.group);
+    if (lane == r) s_part[warp][r] = make_float2(m, s);
+  }
+  const uint32_t row = blockIdx.x * p.group + warp;
+  const bool mine = warp < (int)p.group && row < p.rows;
+  float again = 0.0f;
+  if (p.x && mine) {
+    const uint32_t t = (uint32_t)p.targets[row];
     float sum = 0.0f;
     if (t < p.cols) {
-      const uint16_t *x = p.x + (size_t)r * p.x_stride, *w = p.w + (size_t)t * p.w_stride;
+      const uint16_t *x = p.x + (size_t)row * p.x_stride, *w = p.w + (size_t)t * p.w_stride;
       uint32_t done = 0;
       if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15u) == 0) {
         float other = 0.0f;
@@ -466,23 +486,16 @@ __global__ void __launch_bounds__(1024) k_join(const JoinParams p) {
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) s_target[warp] = sum;
+    again = sum;
   }
-  float m = -INFINITY, s = 0.0f;
-  auto join = [&](float2 q) {
-    const float top = fmaxf(m, q.x), ref = top == -INFINITY ? 0.0f : top;
-    s = s * ex2_approx((m - ref) * c) + q.y * ex2_approx((q.x - ref) * c);
-    m = top;
-  };
-  if (row < p.rows) {
-#pragma unroll 4
-    for (uint32_t i = warp; i < p.slots; i += 32) join(p.parts[(size_t)i * p.rows_pad + row]);
-  }
-  s_part[warp][lane] = make_float2(m, s);
   __syncthreads();
-  if (warp != 0 || row >= p.rows) return;
-#pragma unroll 1
-  for (int i = 1; i < 32; ++i) join(s_part[i][lane]);
+  if (!mine) return;
+  const float cn = logit_factor(p.scale, p.row_factor, nullptr, row, true);
+  c = exponent_factor(cn);
+  m = s_part[lane][warp].x;
+  s = s_part[lane][warp].y;
+  join_lanes(1);
+  if (lane != 0) return;
   if ((uint32_t)p.targets[row] >= p.cols) {
     p.lse[row] = 0.0f;
     p.loss[row] = 0.0f;
@@ -490,10 +503,10 @@ __global__ void __launch_bounds__(1024) k_join(const JoinParams p) {
   }
   float target = p.picked[row], l = logf(s);
   if (p.x) {
-    const float d = (s_target[lane] - target) * cn;
+    const float d = (again - target) * cn;
     if (fabsf(d) < 1.0f) {  // above, all of it is rounding of logits of 2^20 and more: what was computed stays together. A NaN stays as well.
       l += log1pf(expf((target - m) * cn - l) * expm1f(d));
-      target = s_target[lane];
+      target = again;
     }
   }
   p.lse[row] = fmaf(m, cn, l);
@@ -788,7 +801,9 @@ struct HeadCall {
     j.slots = slots;
     j.width = width;
     j.scale = scale;
-    const int st = check_cuda(launch_kernel(k_join, dim3((rows + 31) / 32), dim3(1024), 0, s, j));
+    j.group = 1;  // as many blocks as there are SMs, while there are rows for them
+    while (j.group < 32 && (uint64_t)j.group * (uint64_t)sm_count() < rows) j.group *= 2;
+    const int st = check_cuda(launch_kernel(k_join, dim3((rows + j.group - 1) / j.group), dim3(1024), 0, s, j));
     note_launch();
     return st;
   }
