@@ -155,6 +155,7 @@ struct GradEpi {
   struct Params {
     const int32_t *targets;
     const float *lse, *row_factor;
+    const float *picked;  // fp32 calls: logarithm of the targets' probabilities
     const uint32_t *largest_w;
     __half *g, *g_lo;  // [rows][pitch]
     float scale;
@@ -205,6 +206,8 @@ struct GradEpi {
     if (here) {
 #pragma unroll
       for (int x = 0; x < 32; ++x) one = at == (uint32_t)x ? v[x] : one;
+      // the tensor cores cut sums off, which a sum of terms of one sign feels most, and p - 1 of a target of high probability
+      if (PARTS == 2 && at < 32u) one = at_most_0(p.picked[row]);
       one = expm1f(one) * kGScale;
     }
 #pragma unroll
@@ -356,6 +359,11 @@ struct PackParams {
   float *row_factor;
   const float *grad;
   const int32_t *targets;  // null: every row counts
+  const float *other, *lse;  // fp32: with the rows of `other` that `picks` names, `picked` becomes scale * product - lse, rounded once
+  const int32_t *picks;
+  float *picked;
+  uint64_t other_stride;
+  float scale;
   uint16_t *hi, *lo;       // lo null: one part; raw: bf16 as they are (operands that cannot be copied in place)
   uint64_t stride;
   uint32_t rows, width, pitch, vocab, bf16, raw;
@@ -369,6 +377,18 @@ __global__ void __launch_bounds__(256) k_pack(const PackParams p) {
   const float g = p.grad && counts ? p.grad[r] : 1.0f;
   const size_t at = (size_t)r * p.stride, to = (size_t)r * p.pitch;
   const bool wide = ((reinterpret_cast<uintptr_t>(p.src) | (p.stride * (p.bf16 ? 2 : 4))) & 15u) == 0;
+  if (p.picked) {
+    const uint32_t t = (uint32_t)p.picks[r];
+    if (t < p.vocab) {
+      const float *x = static_cast<const float *>(p.src) + at, *w = p.other + (size_t)t * p.other_stride;
+      double sum = 0.0;
+#pragma unroll 8
+      for (uint32_t k = lane; k < p.width; k += 32) sum = fma((double)x[k], (double)w[k], sum);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (lane == 0) p.picked[r] = (float)((double)p.scale * sum - (double)p.lse[r]);
+    }
+  }
   // four elements at a time, zeros behind the end (the pitch is a multiple of 64)
   auto four = [&](uint32_t k) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -677,6 +697,7 @@ Layout layout(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool bac
   } else {
     l.x_grad = take((uint64_t)rows * l.pitch * 2 * parts);
     if (bf16) l.w_raw = take((uint64_t)l.piece * l.pitch * 2);
+    else l.picked = take((uint64_t)rows * 4);
     l.g = take((uint64_t)rows * l.piece * 2 * parts);
     l.planes = take((uint64_t)l.splits * rows * l.pitch * 4);
   }
@@ -739,8 +760,14 @@ struct HeadCall {
   uint16_t *at16(uint64_t offset) const { return reinterpret_cast<uint16_t *>(ws + offset); }
 
   int pack(const void *src, uint64_t stride, uint32_t n, uint64_t to, bool raw, const uint32_t *scale_from, float *row_factor, const float *grad,
-           const int32_t *which) const {
+           const int32_t *which, float *picked = nullptr, const float *lse = nullptr) const {
     PackParams p = {};
+    p.other = static_cast<const float *>(w);
+    p.other_stride = w_stride;
+    p.picks = targets;
+    p.picked = picked;
+    p.lse = lse;
+    p.scale = scale;
     p.src = src;
     p.scale_from = scale_from;
     p.row_factor = row_factor;
@@ -774,13 +801,13 @@ struct HeadCall {
     return st;
   }
   // operands of the logits: bf16 in place where a copy can start there, else copied; fp32 in parts (x once, w piece by piece)
-  int logits_x(Operand *o) const {
+  int logits_x(Operand *o, float *picked = nullptr, const float *lse = nullptr) const {
     if (bf16 && in_place(x, x_stride)) {
       *o = {x, x, true, rows, width, x_stride};
       return DF_OK;
     }
     *o = packed(l.x_parts, rows, bf16);
-    return pack(x, x_stride, rows, l.x_parts, bf16, nullptr, bf16 ? nullptr : reinterpret_cast<float *>(ws + l.row_factor), nullptr, nullptr);
+    return pack(x, x_stride, rows, l.x_parts, bf16, nullptr, bf16 ? nullptr : reinterpret_cast<float *>(ws + l.row_factor), nullptr, nullptr, picked, lse);
   }
 
   int join(float *loss, float *lse, uint32_t slots, bool again) const {  // again: targets' logits in rounded sums
@@ -926,7 +953,8 @@ struct HeadCall {
     const uint32_t elt = bf16 ? 2 : 4, wide = bf16 ? 7 : 15;
     int st = ranges(grad, d_w != nullptr);
     Operand a;
-    if (st == DF_OK) st = logits_x(&a);
+    float *picked = bf16 ? nullptr : reinterpret_cast<float *>(ws + l.picked);
+    if (st == DF_OK) st = logits_x(&a, picked, lse);
     if (st == DF_OK && d_w) st = pack(x, x_stride, rows, l.x_grad, false, &words->largest_x, nullptr, grad, targets);
     int splits = l.splits;
     for (uint32_t c0 = 0; st == DF_OK && c0 < vocab; c0 += l.piece) {
@@ -947,6 +975,7 @@ struct HeadCall {
       e.lse = lse;
       e.row_factor = bf16 ? nullptr : reinterpret_cast<const float *>(ws + l.row_factor);
       e.largest_w = &words->largest_w;
+      e.picked = picked;
       e.g = reinterpret_cast<__half *>(ws + l.g);
       e.g_lo = e.g + (size_t)rows * l.piece;
       e.scale = scale;

@@ -1,10 +1,11 @@
 // muon.cu — matrices orthogonalised by Newton-Schulz products, and the optimiser step that applies them (sm_100a):
-//   X = U / (|U|_F + eps);  `steps` times:  G = X X^T (rows <= cols; else X^T X),  B = a I + b G + c G G,  X <- B X (else X B)
+//   X = U / (|U|_F + eps);  `steps` times:  G = X X^T (rows <= cols; else X^T X),  B = b G + c G G,  X <- a X + B X (else a X + X B)
 // Each singular value goes through s -> a s + b s^3 + c s^5 by itself; with the usual coefficients five steps bring those that are not
 // tiny near 1. G and B are symmetric: only tiles on and right of the diagonal are computed, and written twice.
 // A singular value far below the largest grows by a factor of up to a^steps (485), and so does whatever a rounding put beside it: all
 // factors are held in two fp16 parts (22 bits; product_sm100.cuh) times 2^12, which suits values up to 15, and sums leave the tensor cores every
-// 64 of the contraction. a is on the diagonal of B, so that X's new value is one product.
+// 64 of the contraction. a X is added to the sums that have left them, in fp32: as a I in B it would be the largest term of sums that the tensor cores cut off (36 x 59: 1.7e-6
+// off 64 bits with it there, 1.3e-6 so; 768 x 768: 1.5e-6 and 0.9e-6).
 //
 // All products of all steps are one cooperative launch. Its tiles are numbered step by step, product by product, matrix by matrix, and dealt out
 // to the CTAs in turn; a tile waits until the tiles of the product before it, of the same matrix, are written (a counter per matrix). What it waits for has
@@ -181,7 +182,7 @@ struct NsParams {
   int from, to;               // units of this launch
   int ordered;                // 1: what a unit needs was written by launches before this one
   int side_tiles, x_m_tiles, x_n_tiles, g_units, x_units;  // tiles: along the side, of X; of a symmetric product, of X's
-  float a, b_, c;             // of B, times the parts' scales
+  float a, b_, c;             // of the polynomial, times the parts' scales
   Targets t;
   uint64_t out_stride;
   uint32_t out_bf16, vec, apply;
@@ -244,7 +245,23 @@ __device__ __forceinline__ void write_parts(uint16_t *hi, uint16_t *lo, size_t a
   }
 }
 
-// G = X X^T, or B = a I + b G + c G G: symmetric, in parts, each tile in its place and in the mirrored one
+// v += factor * (hi + lo), W columns of a row. Written by other SMs of this launch: not through L1.
+template <int W>
+__device__ __forceinline__ void add_parts(const uint16_t *hi, const uint16_t *lo, size_t at, float factor, float (&v)[W]) {
+#pragma unroll
+  for (int x = 0; x < W; x += 8) {
+    const uint4 h = __ldcg(reinterpret_cast<const uint4 *>(hi + at + x)), l = __ldcg(reinterpret_cast<const uint4 *>(lo + at + x));
+    const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&hh[y])), r = __half22float2(*reinterpret_cast<const __half2 *>(&ll[y]));
+      v[x + 2 * y] = fmaf(factor, q.x + r.x, v[x + 2 * y]);
+      v[x + 2 * y + 1] = fmaf(factor, q.y + r.y, v[x + 2 * y + 1]);
+    }
+  }
+}
+
+// G = X X^T, or B = b G + c G G: symmetric, in parts, each tile in its place and in the mirrored one
 template <int W>
 __device__ __forceinline__ void symmetric_block(const NsParams &p, const Unit &w, uint32_t row, uint32_t first, float (&v)[W]) {
   if (first >= p.side || row >= p.side) return;  // the pitch is a multiple of 64: a block that begins inside may be written whole
@@ -254,18 +271,8 @@ __device__ __forceinline__ void symmetric_block(const NsParams &p, const Unit &w
     hi = p.bp[0];
     lo = p.bp[1];
 #pragma unroll
-    for (int x = 0; x < W; x += 8) {  // written by other SMs of this launch: not through L1
-      const uint4 h = __ldcg(reinterpret_cast<const uint4 *>(p.gp[0] + at + x)), l = __ldcg(reinterpret_cast<const uint4 *>(p.gp[1] + at + x));
-      const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&hh[y])), r = __half22float2(*reinterpret_cast<const __half2 *>(&ll[y]));
-        v[x + 2 * y] = fmaf(p.c, v[x + 2 * y], p.b_ * (q.x + r.x));
-        v[x + 2 * y + 1] = fmaf(p.c, v[x + 2 * y + 1], p.b_ * (q.y + r.y));
-      }
-    }
-#pragma unroll
-    for (int x = 0; x < W; ++x) v[x] += first + x == row ? p.a : 0.0f;
+    for (int x = 0; x < W; ++x) v[x] *= p.c;
+    add_parts<W>(p.gp[0], p.gp[1], at, p.b_, v);
   } else {
     hi = p.gp[0];
     lo = p.gp[1];
@@ -368,38 +375,40 @@ __device__ __forceinline__ void next_block(uint16_t *const (&dst)[2], size_t at,
     store_block(slab, lane, dst[low] + at, pitch, rows, q);
   }
 }
+// v += factor * (hi + lo) of such a block, which other SMs of this launch have written: not through L1
+__device__ __forceinline__ void add_block(uint16_t *const (&src)[2], size_t at, uint32_t pitch, uint4 *slab, int lane, uint32_t rows, float factor, float (&v)[64]) {
+  const int lrow = lane >> 3, chunk = lane & 7;
+#pragma unroll
+  for (int low = 0; low < 2; ++low) {
+    uint4 q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      q[i] = (uint32_t)(4 * i + lrow) < rows ? __ldcg(reinterpret_cast<const uint4 *>(src[low] + at + (size_t)(4 * i + lrow) * pitch + 8 * chunk)) : make_uint4(0u, 0u, 0u, 0u);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) slab[(4 * i + lrow) * 8 + (chunk ^ ((4 * i + lrow) & 7))] = q[i];
+    __syncwarp();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const uint4 g = slab[lane * 8 + (x ^ (lane & 7))];
+      const uint32_t gg[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&gg[y]));
+        v[8 * x + 2 * y] = fmaf(factor, f.x, v[8 * x + 2 * y]);
+        v[8 * x + 2 * y + 1] = fmaf(factor, f.y, v[8 * x + 2 * y + 1]);
+      }
+    }
+  }
+}
 __device__ __forceinline__ void symmetric_64(const NsParams &p, const Unit &w, uint4 *slab, int lane, uint32_t row0, uint32_t first, float (&v)[64]) {
   if (first >= p.side || row0 >= p.side) return;
   const size_t base = (size_t)w.batch * p.g_matrix, at = base + (size_t)row0 * p.g_pitch + first;
   const uint32_t rows = p.side - row0;
   if (w.product == kPolynomial) {
-    const int lrow = lane >> 3, chunk = lane & 7;
 #pragma unroll
-    for (int low = 0; low < 2; ++low) {
-      uint4 q[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)  // written by other SMs of this launch: not through L1
-        q[i] = (uint32_t)(4 * i + lrow) < rows ? __ldcg(reinterpret_cast<const uint4 *>(p.gp[low] + at + (size_t)(4 * i + lrow) * p.g_pitch + 8 * chunk))
-                                               : make_uint4(0u, 0u, 0u, 0u);
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) slab[(4 * i + lrow) * 8 + (chunk ^ ((4 * i + lrow) & 7))] = q[i];
-      __syncwarp();
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const uint4 g = slab[lane * 8 + (x ^ (lane & 7))];
-        const uint32_t gg[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&gg[y]));
-          float &v0 = v[8 * x + 2 * y], &v1 = v[8 * x + 2 * y + 1];
-          v0 = low == 0 ? fmaf(p.c, v0, p.b_ * f.x) : fmaf(p.b_, f.x, v0);
-          v1 = low == 0 ? fmaf(p.c, v1, p.b_ * f.y) : fmaf(p.b_, f.y, v1);
-        }
-      }
-    }
-#pragma unroll
-    for (int x = 0; x < 64; ++x) v[x] += first + x == row0 + lane ? p.a : 0.0f;
+    for (int x = 0; x < 64; ++x) v[x] *= p.c;
+    add_block(p.gp, at, p.g_pitch, slab, lane, rows, p.b_, v);
   } else {
 #pragma unroll
     for (int x = 0; x < 64; ++x) v[x] *= kPartInverse;
@@ -672,7 +681,7 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
       }
       const uint32_t row0 = (uint32_t)(w.m * T + quarter * 32), row = row0 + lane;
       const uint32_t col0 = (uint32_t)(w.n * T + (int)part * C::kOwned + half * (C::kOwned / 2));
-      if (w.product == kPolynomial) {  // what it reads of G: the copies have been waited for, these loads as well
+      if (w.product != kGram) {  // what it reads of G or X: the copies have been waited for, these loads as well
         (void)load_acquire(p.done + w.batch);
         __syncwarp();
       }
@@ -686,31 +695,35 @@ __global__ void __launch_bounds__(kProdThreads, 1) k_newton_schulz(const __grid_
           float(&v)[64] = reinterpret_cast<float(&)[64]>(sum[cg]);
           if (w.product != kNext) {
             symmetric_64(p, w, slab16, lane, row0, c, v);
-          } else if (!last) {
-            if (c < p.cols && row0 < p.rows) {
+          } else if (c < p.cols && row0 < p.rows) {
+            const size_t at = (size_t)w.batch * p.x_matrix + (size_t)row0 * p.x_pitch + c;
+            add_block(p.x[w.step & 1], at, p.x_pitch, slab16, lane, p.rows - row0, p.a, v);
+            if (!last) {
 #pragma unroll
               for (int x = 0; x < 64; ++x) v[x] *= kPartInverse;
-              next_block(p.x[next], (size_t)w.batch * p.x_matrix + (size_t)row0 * p.x_pitch + c, p.x_pitch, slab16, lane, p.rows - row0, v);
+              next_block(p.x[next], at, p.x_pitch, slab16, lane, p.rows - row0, v);
+            } else {
+              last_block(p, w, slab, lane, row0, c, sum[cg]);
+              last_block(p, w, slab, lane, row0, c + W, sum[cg + 1]);
             }
-          } else {
-            last_block(p, w, slab, lane, row0, c, sum[cg]);
-            last_block(p, w, slab, lane, row0, c + W, sum[cg + 1]);
           }
         }
       } else {
         float(&v)[W] = reinterpret_cast<float(&)[W]>(sum[0]);
         if (w.product != kNext) {
           symmetric_block<W>(p, w, row, col0, v);
-        } else if (!last) {
-          if (col0 < p.cols && row < p.rows) {
+        } else if (col0 < p.cols && row < p.rows) {
+          const size_t at = (size_t)w.batch * p.x_matrix + (size_t)row * p.x_pitch + col0;
+          add_parts<W>(p.x[w.step & 1][0], p.x[w.step & 1][1], at, p.a, v);
+          if (!last) {
 #pragma unroll
             for (int x = 0; x < W; ++x) v[x] *= kPartInverse;
-            write_parts<W>(p.x[next][0], p.x[next][1], (size_t)w.batch * p.x_matrix + (size_t)row * p.x_pitch + col0, v);
-          }
-        } else {
+            write_parts<W>(p.x[next][0], p.x[next][1], at, v);
+          } else {
 #pragma unroll
-          for (int x = 0; x < W; x += 4)
-            if (row < p.rows && col0 + x < p.cols) last_four(p, p.t.out[w.batch], row, col0 + x, make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]));
+            for (int x = 0; x < W; x += 4)
+              if (col0 + x < p.cols) last_four(p, p.t.out[w.batch], row, col0 + x, make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]));
+          }
         }
       }
       fence_proxies();
@@ -783,6 +796,22 @@ __device__ __forceinline__ void small_store(uint8_t *hi, uint8_t *lo, uint32_t r
     const uint32_t at = row * 128 + ((x ^ (row & 7)) << 4);
     *reinterpret_cast<uint4 *>(hi + at) = h;
     *reinterpret_cast<uint4 *>(lo + at) = l;
+  }
+}
+
+// v += factor * (hi + lo) of such a row
+__device__ __forceinline__ void small_add(const uint8_t *hi, const uint8_t *lo, uint32_t row, float factor, float (&v)[64]) {
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    const uint32_t at = row * 128 + ((x ^ (row & 7)) << 4);
+    const uint4 h = *reinterpret_cast<const uint4 *>(hi + at), l = *reinterpret_cast<const uint4 *>(lo + at);
+    const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&hh[y])), r = __half22float2(*reinterpret_cast<const __half2 *>(&ll[y]));
+      v[8 * x + 2 * y] = fmaf(factor, q.x + r.x, v[8 * x + 2 * y]);
+      v[8 * x + 2 * y + 1] = fmaf(factor, q.y + r.y, v[8 * x + 2 * y + 1]);
+    }
   }
 }
 
@@ -949,7 +978,7 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
     clear(v);
     for (uint32_t c = 0; c < side_blocks; ++c) take((int)c, v);
 #pragma unroll
-    for (int x = 0; x < 64; ++x) v[x] = fmaf(p.c, v[x], p.b * g[x]) + ((uint32_t)(half * 64 + x) == row ? p.a : 0.0f);
+    for (int x = 0; x < 64; ++x) v[x] = fmaf(p.c, v[x], p.b * g[x]);
     small_store(smem + kSmallG + half * kSlab, smem + kSmallG + (2 + half) * kSlab, row, v);
     if (!(go = meet())) continue;
     if (warp == 0)
@@ -960,6 +989,7 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
       for (uint32_t h = 0; h < halves; ++h) {
         clear(v);
         for (uint32_t c = 0; c < side_blocks; ++c) take((int)(2 * h + c), v);
+        small_add(smem + kSmallX + (2 * h + half) * kSlab, smem + kSmallX + (4 + 2 * h + half) * kSlab, row, p.a, v);
 #pragma unroll
         for (int x = 0; x < 64; ++x) v[x] *= kPartInverse;
         // only the products that have just ended read these slabs of X
@@ -972,8 +1002,11 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
     clear(g);
     clear(v);
     for (uint32_t c = 0; c < side_blocks; ++c) take((int)c, g);
-    if (halves > 1)
+    small_add(smem + kSmallX + half * kSlab, smem + kSmallX + (4 + half) * kSlab, row, p.a, g);
+    if (halves > 1) {
       for (uint32_t c = 0; c < side_blocks; ++c) take((int)(2 + c), v);
+      small_add(smem + kSmallX + (2 + half) * kSlab, smem + kSmallX + (6 + half) * kSlab, row, p.a, v);
+    }
     if (!(go = meet())) continue;
     float *x = reinterpret_cast<float *>(smem) + row * kSmallPitch + half * 64;
 #pragma unroll

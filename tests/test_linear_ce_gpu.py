@@ -346,3 +346,28 @@ def test_pieces_of_a_weight_that_is_copied(torch):
     targets[:2] = torch.tensor([0, 70000], dtype=torch.int32, device="cuda")
     loss, lse = p.linear_cross_entropy(x, w, targets)
     check_loss(torch, x, w, targets, 1.0, loss, lse)
+
+
+@pytest.mark.parametrize("rows,vocab,width", [(75, 364, 256), (600, 533, 768), (40, 300, 1000)])
+def test_gradient_of_targets_of_high_probability(torch, rows, vocab, width):
+    """p - 1 at the target. Its logit is a sum of terms of one sign, about 11 here: a product rounded to 24 bits and lanes' sums of width / 32 terms, then five more, are
+    off by (width / 32 + 6) 2^-24 of it at most, scale and lse's difference by 2^-24 of their own size, and expm1 by 2^-22 of its result."""
+    p = pkg()
+    x, w, targets = case(torch, 5, rows, vocab, width, "fp32")
+    x += 9.0 * w[targets.long()]
+    z = x.double() @ w.double().t()
+    lse = torch.logsumexp(z, 1).float()
+    d_x, _ = p.linear_cross_entropy_backward(x, w, targets, lse, torch.ones(rows, device="cuda"), want_weight=False)
+    picked = z.gather(1, targets.long()[:, None]).squeeze(1)
+    g = torch.exp(z - lse.double()[:, None])
+    g[torch.arange(rows, device="cuda"), targets.long()] = torch.expm1(picked - lse.double())
+    want = g @ w.double()
+    at_target = ((width / 32 + 6) * 2.0 ** -24 * (x.double() * w[targets.long()].double()).abs().sum(1) + 2.0 ** -24 * (picked.abs() + lse.double().abs())) \
+        * torch.exp(picked - lse.double()) + 2.0 ** -22 * g.abs().max(1).values
+    # the other logits, p each: sums cut off as in exact(), 22-bit operands
+    e = (16 + width / 128) * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t()) + width * 2.0 ** -38 * float(x.abs().max() * w.abs().max())
+    others = torch.exp(z - lse.double()[:, None]) * (e + (z.abs() + lse.double().abs()[:, None] + 4) * 2.0 ** -22)
+    others[torch.arange(rows, device="cuda"), targets.long()] = 0.0
+    wide = w.double().abs()
+    tol = at_target[:, None] * wide[targets.long()] + others @ wide + (16 + vocab / 128) * 2.0 ** -23 * (g.abs() @ wide) + vocab * 2.0 ** -38 * float(wide.max()) + want.abs() * 2.0 ** -23
+    assert bool(((d_x.double() - want).abs() <= tol).all())
