@@ -440,14 +440,15 @@ __global__ void __launch_bounds__(256) k_pack(const PackParams p) {
   }
 }
 
-// loss and lse of `group` rows a block, 32 / group lanes of each of 32 warps and row: they share the slots, then a warp a row joins what the warps have. For bf16 calls it also takes a row's target again, in fp32 sums that are rounded: the tensor
+// loss and lse of `group` rows a block, 32 / group lanes of each of 32 warps and row: they share the slots, then a warp a row joins what the warps have. It also takes a row's target again, in sums that are rounded: the tensor
 // cores cut the sum of a whole row off at each 16 of it, which a target's logit, a sum of terms of one sign where the model has learned something, feels most (4096
-// rows of 768: the loss 1.0e-6 off 64 bits without). With d what the logit lacks, sum e^z grows by p (e^d - 1) of itself.
+// rows of 768 in bf16: the loss 1.0e-6 off 64 bits without; 75 rows over 364 columns of 256 in fp32, the gradient from such an lse 2.8e-6). With d what the logit lacks, sum e^z grows by p (e^d - 1) of itself.
 struct JoinParams {
   const float2 *parts;
   const float *picked, *row_factor;
   const int32_t *targets;
-  const uint16_t *x, *w;  // bf16 calls
+  const uint16_t *x, *w;    // bf16 calls
+  const float *x32, *w32;   // fp32 calls on the tensor cores
   uint64_t x_stride, w_stride;
   float *loss, *lse;
   uint32_t rows, cols, rows_pad, slots, width, group;  // group: a power of two, at most 32
@@ -507,6 +508,17 @@ __global__ void __launch_bounds__(1024) k_join(const JoinParams p) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     again = sum;
+  } else if (p.x32 && mine) {  // in double, and in the unit that the product's row has
+    const uint32_t t = (uint32_t)p.targets[row];
+    double sum = 0.0;
+    if (t < p.cols) {
+      const float *x = p.x32 + (size_t)row * p.x_stride, *w = p.w32 + (size_t)t * p.w_stride;
+#pragma unroll 8
+      for (uint32_t k = lane; k < p.width; k += 32) sum = fma((double)x[k], (double)w[k], sum);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    again = (float)(sum / (double)p.row_factor[row]);
   }
   __syncthreads();
   if (!mine) return;
@@ -522,7 +534,7 @@ __global__ void __launch_bounds__(1024) k_join(const JoinParams p) {
     return;
   }
   float target = p.picked[row], l = logf(s);
-  if (p.x) {
+  if (p.x || p.x32) {
     const float d = (again - target) * cn;
     if (fabsf(d) < 1.0f) {  // above, all of it is rounding of logits of 2^20 and more: what was computed stays together. A NaN stays as well.
       l += log1pf(expf((target - m) * cn - l) * expm1f(d));
@@ -816,8 +828,10 @@ struct HeadCall {
     j.picked = reinterpret_cast<const float *>(ws + l.picked);
     j.row_factor = bf16 || l.few ? nullptr : reinterpret_cast<const float *>(ws + l.row_factor);
     j.targets = targets;
-    j.x = again ? static_cast<const uint16_t *>(x) : nullptr;
+    j.x = again && bf16 ? static_cast<const uint16_t *>(x) : nullptr;
     j.w = static_cast<const uint16_t *>(w);
+    j.x32 = again && !bf16 ? static_cast<const float *>(x) : nullptr;
+    j.w32 = static_cast<const float *>(w);
     j.x_stride = x_stride;
     j.w_stride = w_stride;
     j.loss = loss;
@@ -943,7 +957,7 @@ struct HeadCall {
         st = bf16 ? product<false, false, 1, LseEpi>(a, b, rows, n, width, 1, true, e, s) : product<false, false, 2, LseEpi>(a, b, rows, n, width, 1, false, e, s);
     }
     if (st != DF_OK) return st;
-    return join(loss, lse, slots, bf16);
+    return join(loss, lse, slots, true);
   }
 
   template <int PARTS>
