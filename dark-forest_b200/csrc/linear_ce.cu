@@ -18,7 +18,9 @@ namespace {
 
 using namespace ptx;
 
-constexpr float kGScale = 16384.0f, kGScaleLog2 = 14.0f;  // G is stored times 2^14
+// G is stored times 2^15, the most that fp16 holds of 1: one part (bf16 calls) has 11 bits for probabilities down to 2^-29 and steps of 2^-39 below, two have 22 bits down to 2^-28 and
+// steps of 2^-50. Columns that are unlikely in every row have nothing else in their row of d_w.
+constexpr float kGScale = 32768.0f, kGScaleLog2 = 15.0f;
 constexpr uint64_t kPieceBytes = 256ull << 20;  // of G, or of a piece's weight in parts
 
 int finish(int st) {
@@ -220,7 +222,7 @@ struct GradEpi {
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
       if constexpr (PARTS == 2) {
-        split_half2(v[2 * x], v[2 * x + 1], hi[x], lo[x]);
+        split_half2<kProdLowUp>(v[2 * x], v[2 * x + 1], hi[x], lo[x]);
         lo[x] = counts ? lo[x] : 0u;
       } else {
         hi[x] = pack_half2(v[2 * x], v[2 * x + 1]);
@@ -244,7 +246,7 @@ struct OutEpi {
     void *out;                  // d_w (planes null): row r of the product is row row_base + r of out
     uint64_t out_stride;
     uint32_t out_bf16, vec;     // vec: rows can be written 16 bytes (fp32) or 8 (bf16) at a time
-    const uint32_t *largest_x;  // d_w: its factor is scale / (2^14 s_x)
+    const uint32_t *largest_x;  // d_w: its factor is scale / (2^15 s_x)
     float scale;
     uint32_t rows, cols;
   };
@@ -432,8 +434,8 @@ __global__ void __launch_bounds__(256) k_pack(const PackParams p) {
     if (p.raw) {
       hi = make_uint2((__float_as_uint(v.x) >> 16) | (__float_as_uint(v.y) & 0xffff0000u), (__float_as_uint(v.z) >> 16) | (__float_as_uint(v.w) & 0xffff0000u));
     } else {
-      split_half2(v.x * s, v.y * s, hi.x, lo.x);
-      split_half2(v.z * s, v.w * s, hi.y, lo.y);
+      split_half2<kProdLowUp>(v.x * s, v.y * s, hi.x, lo.x);
+      split_half2<kProdLowUp>(v.z * s, v.w * s, hi.y, lo.y);
     }
     *reinterpret_cast<uint2 *>(p.hi + to + k) = hi;
     if (p.lo) *reinterpret_cast<uint2 *>(p.lo + to + k) = lo;

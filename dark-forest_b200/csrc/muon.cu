@@ -143,8 +143,8 @@ __global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ Updat
         }
       }
       uint2 hi, lo;
-      split_half2(v[0] * f, v[1] * f, hi.x, lo.x);
-      split_half2(v[2] * f, v[3] * f, hi.y, lo.y);
+      split_half2<0>(v[0] * f, v[1] * f, hi.x, lo.x);
+      split_half2<0>(v[2] * f, v[3] * f, hi.y, lo.y);
       *reinterpret_cast<uint2 *>(p.hi + to + c) = hi;
       *reinterpret_cast<uint2 *>(p.lo + to + c) = lo;
     }
@@ -236,10 +236,10 @@ __device__ __forceinline__ void write_parts(uint16_t *hi, uint16_t *lo, size_t a
 #pragma unroll
   for (int x = 0; x < W; x += 8) {
     uint4 h, l;
-    split_half2(v[x], v[x + 1], h.x, l.x);
-    split_half2(v[x + 2], v[x + 3], h.y, l.y);
-    split_half2(v[x + 4], v[x + 5], h.z, l.z);
-    split_half2(v[x + 6], v[x + 7], h.w, l.w);
+    split_half2<0>(v[x], v[x + 1], h.x, l.x);
+    split_half2<0>(v[x + 2], v[x + 3], h.y, l.y);
+    split_half2<0>(v[x + 4], v[x + 5], h.z, l.z);
+    split_half2<0>(v[x + 6], v[x + 7], h.w, l.w);
     *reinterpret_cast<uint4 *>(hi + at + x) = h;
     *reinterpret_cast<uint4 *>(lo + at + x) = l;
   }
@@ -362,7 +362,7 @@ __device__ __forceinline__ void split_block(const float (&v)[64], uint4 (&q)[8],
   for (int x = 0; x < 8; ++x) {
     uint32_t h[4], l[4];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) split_half2(v[8 * x + 2 * y], v[8 * x + 2 * y + 1], h[y], l[y]);
+    for (int y = 0; y < 4; ++y) split_half2<0>(v[8 * x + 2 * y], v[8 * x + 2 * y + 1], h[y], l[y]);
     q[x] = low ? make_uint4(l[0], l[1], l[2], l[3]) : make_uint4(h[0], h[1], h[2], h[3]);
   }
 }
@@ -425,7 +425,7 @@ __device__ __forceinline__ void symmetric_64(const NsParams &p, const Unit &w, u
 #pragma unroll
     for (int x = 0; x < 64; x += 2) {
       uint32_t h, l;
-      split_half2(v[x], v[x + 1], h, l);
+      split_half2<0>(v[x], v[x + 1], h, l);
       const uint32_t mine = low ? l : h, other = __shfl_xor_sync(0xffffffffu, mine, 1);
       words[(x + (lane & 1)) * 16 + (lane >> 1)] = lane & 1 ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
     }
@@ -789,10 +789,10 @@ __device__ __forceinline__ void small_store(uint8_t *hi, uint8_t *lo, uint32_t r
 #pragma unroll
   for (int x = 0; x < 8; ++x) {
     uint4 h, l;
-    split_half2(v[8 * x], v[8 * x + 1], h.x, l.x);
-    split_half2(v[8 * x + 2], v[8 * x + 3], h.y, l.y);
-    split_half2(v[8 * x + 4], v[8 * x + 5], h.z, l.z);
-    split_half2(v[8 * x + 6], v[8 * x + 7], h.w, l.w);
+    split_half2<0>(v[8 * x], v[8 * x + 1], h.x, l.x);
+    split_half2<0>(v[8 * x + 2], v[8 * x + 3], h.y, l.y);
+    split_half2<0>(v[8 * x + 4], v[8 * x + 5], h.z, l.z);
+    split_half2<0>(v[8 * x + 6], v[8 * x + 7], h.w, l.w);
     const uint32_t at = row * 128 + ((x ^ (row & 7)) << 4);
     *reinterpret_cast<uint4 *>(hi + at) = h;
     *reinterpret_cast<uint4 *>(lo + at) = l;

@@ -1,11 +1,12 @@
 // product_sm100.cuh — batched matrix products of 16-bit operands on tcgen05 with an epilogue of the caller's:
 //   acc[m][n] = sum_k A[m][k] B[n][k]
 // Operands lie in global memory with either side contiguous (K-major: rows of k; MN-major: rows of m or n), bf16 or fp16. With
-// PARTS = 2 a value is two fp16 numbers, hi = fp16(s x) and lo = fp16(s x - hi) for a power of two s that the caller undoes: 22 bits
-// where |x| is within 2^18 of the largest that s was chosen for, and nothing below 2^-40 of that one. Then
-//   A B = A_lo B_hi + A_hi B_lo + A_hi B_hi      (A_lo B_lo, 2^-22 of it at most, is left out)
+// PARTS = 2 a value is two fp16 numbers, hi = fp16(s x) and lo = fp16(2^11 (s x - hi)) for a power of two s that the caller undoes: 22 bits
+// where |x| is within 2^27 of the largest that s was chosen for (2^14 .. 2^15 after it), and nothing below 2^-50 of that one: without the 2^11, lo would leave fp16 that much earlier,
+// and a probability of 1e-9 among ones near 1 would have 9 bits. Then
+//   A B = 2^-11 (A_lo B_hi + A_hi B_lo) + A_hi B_hi      (A_lo B_lo, 2^-22 of it at most, is left out)
 // is three products in that order: the tensor cores cut sums off instead of rounding them, and a large sum is cut off at each of its
-// additions, so the small terms come first and every 128 of the contraction the sum is taken out to registers and added up rounded. (More often costs time: a
+// additions, so the small terms come first (the first large one scales their sum down by 2^11 as it adds to it) and every 128 of the contraction the sum is taken out to registers and added up rounded. (More often costs time: a
 // tile's sums are 128 KB a CTA, which tensor memory gives out in about 2000 cycles, and 64 of the contraction are 1536 cycles of products.)
 //
 // One persistent kernel, at most one CTA an SM, 384 threads:
@@ -47,6 +48,7 @@ struct ProductTile {
 
 constexpr int kProdEpiWarps = 8, kProdThreads = 384, kProdK = 64;
 constexpr int kProdChunk = 2;  // products of parts: blocks of 64 between takings out of the sums
+constexpr int kProdLowUp = 11;  // low parts are held times 2^11
 constexpr uint32_t kProdSlabBytes = 32 * 128;  // a warp's staging slab: 32 rows of 128 bytes
 // Sums in registers: the launch gives 168 registers to each thread of three warpgroups; the two of the epilogue take over 48 from each thread of the first.
 constexpr int kProdLaunchRegs = 168, kProdEpiRegs = 216, kProdOtherRegs = 72;
@@ -191,13 +193,15 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
       uint32_t it = 0, j = 0;
       bool ok = true;
       // K-major: 16 of k are 32 bytes of a swizzled row; MN-major: 16 rows of 128 bytes, the next 64 of m or n 8192 bytes on
-      auto issue = [&](uint32_t d, uint32_t sa, uint32_t sb, bool first) {
+      // fresh: the sum begins; down: it holds the small terms, 2^11 too large
+      auto issue = [&](uint32_t d, uint32_t sa, uint32_t sb, bool fresh, bool down = false) {
         const uint64_t da = make_smem_desc(sa, C::A_MN ? 8192 : 16, 1024, kSwz128), db = make_smem_desc(sb, C::B_MN ? 8192 : 16, 1024, kSwz128);
 #pragma unroll
         for (int k = 0; k < kProdK / 16; ++k) {
           const uint64_t oa = (uint64_t)((k * (C::A_MN ? 2048 : 32)) >> 4), ob = (uint64_t)((k * (C::B_MN ? 2048 : 32)) >> 4);
-          if (PAIR) mma_f16_ss_pair(d, da + oa, db + ob, idesc, first && k == 0 ? 0u : 1u);
-          else mma_f16_ss(d, da + oa, db + ob, idesc, first && k == 0 ? 0u : 1u);
+          if (C::PARTS == 2 && down && k == 0) mma_f16_ss_down<kProdLowUp, PAIR>(d, da, db, idesc);
+          else if (PAIR) mma_f16_ss_pair(d, da + oa, db + ob, idesc, fresh && k == 0 ? 0u : 1u);
+          else mma_f16_ss(d, da + oa, db + ob, idesc, fresh && k == 0 ? 0u : 1u);
         }
       };
       auto commit = [&](int id) {
@@ -229,7 +233,7 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
             if (ok && elect_one()) {
               for (int i = 0; i < n; ++i) {
                 const uint32_t s_hi = (it + 2 * i + 1) % kStages, hi = a0 + s_hi * C::kStageBytes;
-                issue(d, hi, hi + C::kTileBytes, false);
+                issue(d, hi, hi + C::kTileBytes, false, i == 0);
                 commit(C::EMPTY + s_hi);
               }
               commit(C::ACC_FULL + acc);
@@ -354,11 +358,13 @@ k_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
   }
 }
 
-// Two values as two fp16 parts each, packed: hi and lo of (x, y).
+// Two values as two fp16 parts each, packed: hi and lo of (x, y), lo times 2^UP.
+template <int UP>
 __device__ __forceinline__ void split_half2(float x, float y, uint32_t &hi, uint32_t &lo) {
+  constexpr float up = (float)(1 << UP);
   const __half2 h = __floats2half2_rn(x, y);
   const float2 back = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - back.x, y - back.y);
+  const __half2 l = __floats2half2_rn((x - back.x) * up, (y - back.y) * up);
   hi = *reinterpret_cast<const uint32_t *>(&h);
   lo = *reinterpret_cast<const uint32_t *>(&l);
 }

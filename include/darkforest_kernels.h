@@ -469,8 +469,9 @@ DF_API int df_token_logprobs_backward(const void *logits, const int32_t *targets
  *       overwritten, in the inputs' type; lse as above, grad_loss [rows]; d_x or d_weight may be NULL (not wanted). No output, and not the workspace, may overlap anything else of the call.
  * A row whose target is outside 0 .. vocab - 1 is left out: loss 0, lse 0, no part of any gradient, whatever x holds there (NaN included). Infinities and NaN
  * elsewhere make the results that they enter NaN. rows = 0: nothing, or d_weight = 0.
- * Precision: products of bf16 are exact, G enters them in 11 bits; fp32 operands enter in 22 bits relative to the largest element of their row (x, and the weight in the
- * loss; elements 2^18 below that in fewer), in the gradient the weight's and grad_loss * x's relative to the largest of all, G in 22. Sums in fp32; results rounded once.
+ * Precision: products of bf16 are exact, G and grad_loss * x enter them in 11 bits (G below 2^-29 in steps of 2^-39); fp32 operands enter in 22 bits relative to the largest element of
+ * their row (x, and the weight in the loss; elements 2^27 below that in fewer), in the gradient the weight's and grad_loss * x's relative to the largest of all, G in 22 (below 2^-28 in
+ * steps of 2^-50). Up to 16 rows (loss, fp32) and 8 (gradient) may be computed in fp32 throughout. Sums in fp32; results rounded once.
  * Nothing depends on the order of execution.
  * The logits' gradient exists piece by piece of the vocabulary in the workspace (up to 256 MB at a time, at least 256 columns).
  * workspace: df_linear_cross_entropy_workspace_bytes, 256-byte aligned, contents undefined before and after. Calls that can overlap need one each. */
