@@ -55,6 +55,21 @@ __device__ __forceinline__ float logit_factor(float scale, const float *row_fact
 // The same for the exponent of 2, above 0 also where operands are so small that it vanishes: -inf, the largest of no columns, times it stays -inf.
 __device__ __forceinline__ float exponent_factor(float c) { return fmaxf(c * kLog2e, 1.17549435e-38f); }
 
+// Elements k .. k + 3 of a row that begins at element `at`, 0 behind its end: together where wide (16 bytes fp32, 8 bf16), else one by one.
+__device__ __forceinline__ float4 load_four(const void *base, bool bf16, size_t at, uint32_t k, uint32_t width, bool wide) {
+  if (wide && k + 4 <= width) {
+    if (!bf16) return *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at + k);
+    const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(base) + at + k);
+    return make_float4(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u));
+  }
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (k < width) v.x = load_f(base, bf16, at + k);
+  if (k + 1 < width) v.y = load_f(base, bf16, at + k + 1);
+  if (k + 2 < width) v.z = load_f(base, bf16, at + k + 2);
+  if (k + 3 < width) v.w = load_f(base, bf16, at + k + 3);
+  return v;
+}
+
 // Four values of a row at element `at`, of which `left` are in the row: together where wide (16 bytes fp32, 8 bf16), else one by one.
 __device__ __forceinline__ void write_four(void *out, size_t at, float4 v, uint32_t left, bool bf16, bool wide) {
   if (wide && left >= 4) {
@@ -157,7 +172,7 @@ struct GradEpi {
   struct Params {
     const int32_t *targets;
     const float *lse, *row_factor;
-    const float *picked;  // fp32 calls: logarithm of the targets' probabilities
+    const float *picked;  // logarithm of the targets' probabilities
     const uint32_t *largest_w;
     __half *g, *g_lo;  // [rows][pitch]
     float scale;
@@ -206,11 +221,9 @@ struct GradEpi {
 #pragma unroll
     for (int x = 0; x < 32; ++x) v[x] = at_most_0(fmaf(v[x], c, -off));  // a probability is at most 1, also under an lse that is rounded; a NaN stays
     if (here) {
-#pragma unroll
-      for (int x = 0; x < 32; ++x) one = at == (uint32_t)x ? v[x] : one;
-      // the tensor cores cut sums off, which a sum of terms of one sign feels most, and p - 1 of a target of high probability
-      if (PARTS == 2 && at < 32u) one = at_most_0(p.picked[row]);
-      one = expm1f(one) * kGScale;
+      // the tensor cores cut sums off, which a sum of terms of one sign feels most, and p - 1 of a target of high probability: 40 rows of 1000 in bf16 whose targets
+      // have a logit of 16 and 1 - p of 5e-5 had p - 1 off by up to half of itself
+      one = expm1f(at < 32u ? at_most_0(p.picked[row]) : 0.0f) * kGScale;
     }
 #pragma unroll
     for (int x = 0; x < 32; ++x) v[x] = ex2_approx(fmaf(v[x], kLog2e, kGScaleLog2));
@@ -354,14 +367,15 @@ __global__ void __launch_bounds__(256) k_ranges(const RangeParams p) {
 }
 
 // Rows cut into parts (or, for bf16 calls, copied): a warp a row. scale_from: the word that the whole tensor's scale follows from; null: every
-// row its own, its inverse written to row_factor. grad: rows times grad, rows that do not count as zeros.
+// row its own, its inverse written to row_factor. grad: rows times grad, rows that do not count as zeros. hi null: only `picked` is wanted.
 struct PackParams {
   const void *src;
   const uint32_t *scale_from;
   float *row_factor;
   const float *grad;
   const int32_t *targets;  // null: every row counts
-  const float *other, *lse;  // fp32: with the rows of `other` that `picks` names, `picked` becomes scale * product - lse, rounded once
+  const void *other;         // with the rows of `other` that `picks` names, `picked` becomes scale * product - lse, in double and rounded once
+  const float *lse;
   const int32_t *picks;
   float *picked;
   uint64_t other_stride;
@@ -382,32 +396,23 @@ __global__ void __launch_bounds__(256) k_pack(const PackParams p) {
   if (p.picked) {
     const uint32_t t = (uint32_t)p.picks[r];
     if (t < p.vocab) {
-      const float *x = static_cast<const float *>(p.src) + at, *w = p.other + (size_t)t * p.other_stride;
+      const bool wide_w = ((reinterpret_cast<uintptr_t>(p.other) | (p.other_stride * (p.bf16 ? 2 : 4))) & 15u) == 0;
       double sum = 0.0;
-#pragma unroll 8
-      for (uint32_t k = lane; k < p.width; k += 32) sum = fma((double)x[k], (double)w[k], sum);
+#pragma unroll 4
+      for (uint32_t k = lane * 4; k < p.width; k += 128) {
+        const float4 x = load_four(p.src, p.bf16, at, k, p.width, wide), w = load_four(p.other, p.bf16, (size_t)t * p.other_stride, k, p.width, wide_w);
+        sum = fma((double)x.x, (double)w.x, fma((double)x.y, (double)w.y, fma((double)x.z, (double)w.z, fma((double)x.w, (double)w.w, sum))));
+      }
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       if (lane == 0) p.picked[r] = (float)((double)p.scale * sum - (double)p.lse[r]);
     }
   }
+  if (!p.hi) return;
   // four elements at a time, zeros behind the end (the pitch is a multiple of 64)
   auto four = [&](uint32_t k) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!counts) return v;
-    if (wide && k + 4 <= p.width) {
-      if (p.bf16) {
-        const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.src) + at + k);
-        v = make_float4(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u));
-      } else {
-        v = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.src) + at + k);
-      }
-    } else {
-      if (k < p.width) v.x = load_f(p.src, p.bf16, at + k);
-      if (k + 1 < p.width) v.y = load_f(p.src, p.bf16, at + k + 1);
-      if (k + 2 < p.width) v.z = load_f(p.src, p.bf16, at + k + 2);
-      if (k + 3 < p.width) v.w = load_f(p.src, p.bf16, at + k + 3);
-    }
+    if (!counts) return make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 v = load_four(p.src, p.bf16, at, k, p.width, wide);
     if (p.grad) v = make_float4(v.x * g, v.y * g, v.z * g, v.w * g);
     return v;
   };
@@ -711,7 +716,7 @@ Layout layout(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool bac
   } else {
     l.x_grad = take((uint64_t)rows * l.pitch * 2 * parts);
     if (bf16) l.w_raw = take((uint64_t)l.piece * l.pitch * 2);
-    else l.picked = take((uint64_t)rows * 4);
+    l.picked = take((uint64_t)rows * 4);
     l.g = take((uint64_t)rows * l.piece * 2 * parts);
     l.planes = take((uint64_t)l.splits * rows * l.pitch * 4);
   }
@@ -773,10 +778,11 @@ struct HeadCall {
   const uint8_t *row_of_w(uint32_t v) const { return static_cast<const uint8_t *>(w) + (size_t)v * w_stride * (bf16 ? 2 : 4); }
   uint16_t *at16(uint64_t offset) const { return reinterpret_cast<uint16_t *>(ws + offset); }
 
+  // to 0: only the targets' log probabilities are wanted
   int pack(const void *src, uint64_t stride, uint32_t n, uint64_t to, bool raw, const uint32_t *scale_from, float *row_factor, const float *grad,
            const int32_t *which, float *picked = nullptr, const float *lse = nullptr) const {
     PackParams p = {};
-    p.other = static_cast<const float *>(w);
+    p.other = w;
     p.other_stride = w_stride;
     p.picks = targets;
     p.picked = picked;
@@ -787,7 +793,7 @@ struct HeadCall {
     p.row_factor = row_factor;
     p.grad = grad;
     p.targets = which;
-    p.hi = at16(to);
+    p.hi = to ? at16(to) : nullptr;
     p.lo = bf16 ? nullptr : at16(to) + (size_t)n * l.pitch;
     p.stride = stride;
     p.rows = n;
@@ -969,9 +975,11 @@ struct HeadCall {
     const uint32_t elt = bf16 ? 2 : 4, wide = bf16 ? 7 : 15;
     int st = ranges(grad, d_w != nullptr);
     Operand a;
-    float *picked = bf16 ? nullptr : reinterpret_cast<float *>(ws + l.picked);
-    if (st == DF_OK) st = logits_x(&a, picked, lse);
-    if (st == DF_OK && d_w) st = pack(x, x_stride, rows, l.x_grad, false, &words->largest_x, nullptr, grad, targets);
+    // the targets' log probabilities come with the pass over x that there is: its parts (fp32), grad x, or one of its own
+    float *picked = reinterpret_cast<float *>(ws + l.picked), *in_parts = bf16 ? nullptr : picked, *in_grad = bf16 ? picked : nullptr;
+    if (st == DF_OK) st = logits_x(&a, in_parts, lse);
+    if (st == DF_OK && d_w) st = pack(x, x_stride, rows, l.x_grad, false, &words->largest_x, nullptr, grad, targets, in_grad, lse);
+    if (st == DF_OK && !d_w && bf16) st = pack(x, x_stride, rows, 0, false, nullptr, nullptr, nullptr, nullptr, picked, lse);
     int splits = l.splits;
     for (uint32_t c0 = 0; st == DF_OK && c0 < vocab; c0 += l.piece) {
       const uint32_t n = vocab - c0 < l.piece ? vocab - c0 : l.piece;

@@ -76,7 +76,7 @@ def test_columns_that_are_unlikely_in_every_row(torch, dtype, rows, vocab, width
 
 
 @pytest.mark.parametrize("rows,vocab,width,pull", [(75, 364, 256, 14.0), (600, 533, 768, 18.0), (40, 300, 1000, 16.0), (20, 9000, 2048, 20.0)])
-@pytest.mark.parametrize("dtype", ["fp32"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("both", [True, False])
 def test_targets_that_are_nearly_certain(torch, dtype, rows, vocab, width, pull, both):
     """1 - p of about 1e-4 and less: e^log p - 1 from a logit of terms of one sign. Its products are exact or rounded to 24 bits and added in double, log p is rounded once, and lse is the
