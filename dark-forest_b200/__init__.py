@@ -370,7 +370,7 @@ def token_logprobs_backward(logits, targets, lse, entropy, grad_logp, grad_entro
 # ------------------------------------------------------------------------------------------
 # Loss from hidden states and orthogonalised updates: what a training step does behind its last block (no counterpart in the reference).
 # workspace: a tensor of at least the bytes that the *_workspace_bytes function names, aligned to 256, kept by the program; None takes one from
-# torch's allocator for the call.
+# torch's allocator for the call. With stream given, workspaces and results that are not given belong to that stream.
 # ------------------------------------------------------------------------------------------
 def linear_cross_entropy_workspace_bytes(rows, vocab, width, bf16, backward):
     return int(lib().df_linear_cross_entropy_workspace_bytes(rows, vocab, width, int(bf16), int(backward)))

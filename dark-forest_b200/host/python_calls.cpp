@@ -13,6 +13,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
@@ -531,23 +532,30 @@ PyObject *token_logprobs_backward(Args a) {  // logits targets lse entropy grad_
 }
 
 // ---------------------------------------------------------------- loss from hidden states, orthogonalised updates
-// For the length of a call: its tensors' device, which becomes the current one, and every other tensor of the call has to be there.
+// For the length of a call: its tensors' device, which becomes the current one, and every other tensor of the call has to be there; and its stream, which becomes the
+// current one as well. So what the call allocates belongs to that stream and holds nothing that another one still uses.
 class OnDevice {
  public:
-  explicit OnDevice(PyObject *first, const char *what) : device_(of(first, what)), guard_(device_) {}
+  OnDevice(PyObject *first, const char *what, PyObject *stream_arg) : device_(of(first, what)), guard_(device_), caller_(c10::cuda::getCurrentCUDAStream()) {
+    if (stream_arg != Py_None) there_.reset_stream(c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(stream(stream_arg)), device_.index()));
+  }
+  // A result goes to a caller on another stream: when it is dropped there, its memory waits for what that stream does with it.
+  PyObject *result(Out &out, PyObject *given) const {
+    if (given == Py_None && out.get() != Py_None && caller_ != c10::cuda::getCurrentCUDAStream() && tensor(out.get()).nbytes() > 0)
+      c10::cuda::CUDACachingAllocator::recordStream(tensor(out.get()).storage().data_ptr(), caller_);
+    return out.get();
+  }
   void same(PyObject *o, const char *what) const {
     if (o != Py_None && of(o, what) != device_) refuse(what, "on another device than the others");
   }
-  // A workspace: the caller's, or one from the allocator that belongs to the call's stream, so that it is not given to another before the call is through.
-  void *workspace(Out &held, PyObject *given, PyObject *stream_arg, uint64_t bytes, uint64_t *size) const {
+  // A workspace: the caller's, or one from the allocator.
+  void *workspace(Out &held, PyObject *given, uint64_t bytes, uint64_t *size) const {
     if (given != Py_None) {
       same(given, "workspace");
       if (!tensor(given).is_contiguous()) refuse("workspace", "must be contiguous");
       *size = tensor(given).nbytes();
       return tensor(given).data_ptr();
     }
-    c10::cuda::OptionalCUDAStreamGuard there;
-    if (stream_arg != Py_None) there.reset_stream(c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(stream(stream_arg)), device_.index()));
     held.wrap(at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(device_)));
     *size = bytes;
     return tensor(held.get()).data_ptr();
@@ -561,6 +569,8 @@ class OnDevice {
   }
   c10::Device device_;
   c10::cuda::CUDAGuard guard_;
+  c10::cuda::CUDAStream caller_;
+  c10::cuda::OptionalCUDAStreamGuard there_;
 };
 
 struct Head {
@@ -576,22 +586,22 @@ Head head(const OnDevice &on, Args a) {  // x weight targets
 }
 
 PyObject *linear_cross_entropy(Args a) {  // x weight targets scale loss lse workspace stream
-  const OnDevice on(a[0], "x");
+  const OnDevice on(a[0], "x", a[7]);
   const Head h = head(on, a);
   Out loss, lse, ws;
   given_or_floats(loss, a[4], a[0], {h.x.rows}, "loss");
   given_or_floats(lse, a[5], a[0], {h.x.rows}, "lse");
-  on.same(loss.get(), "loss");
-  on.same(lse.get(), "lse");
+  on.same(on.result(loss, a[4]), "loss");
+  on.same(on.result(lse, a[5]), "lse");
   uint64_t size = 0;
-  void *work = on.workspace(ws, a[6], a[7], fn.df_linear_cross_entropy_workspace_bytes(h.x.rows, h.w.rows, h.x.cols, h.x.bf16, 0), &size);
+  void *work = on.workspace(ws, a[6], fn.df_linear_cross_entropy_workspace_bytes(h.x.rows, h.w.rows, h.x.cols, h.x.bf16, 0), &size);
   call(fn.df_linear_cross_entropy, a[7], h.x.data, h.w.data, h.targets, ptr(loss.get()), ptr(lse.get()), work, size, h.x.rows, h.w.rows, h.x.cols, h.x.stride,
        h.w.stride, real(a[3]), h.x.bf16);
   return tuple_of({&loss, &lse});
 }
 
 PyObject *linear_cross_entropy_backward(Args a) {  // x weight targets lse grad_loss scale d_x d_weight want_x want_weight workspace stream
-  const OnDevice on(a[0], "x");
+  const OnDevice on(a[0], "x", a[11]);
   const Head h = head(on, a);
   on.same(a[3], "lse");
   on.same(a[4], "grad_loss");
@@ -607,12 +617,12 @@ PyObject *linear_cross_entropy_backward(Args a) {  // x weight targets lse grad_
       continue;
     }
     given_or_empty(d[i], a[6 + i], a[0], {static_cast<int64_t>(like[i]->rows), static_cast<int64_t>(like[i]->cols)}, type);
-    on.same(d[i].get(), names[i]);
+    on.same(on.result(d[i], a[6 + i]), names[i]);
     to[i] = strided_rows(d[i].get(), names[i]);
     if (to[i].rows != like[i]->rows || to[i].cols != like[i]->cols || to[i].bf16 != h.x.bf16) refuse(names[i], "shape or dtype differs from what it is the gradient of");
   }
   uint64_t size = 0;
-  void *work = on.workspace(ws, a[10], a[11], fn.df_linear_cross_entropy_workspace_bytes(h.x.rows, h.w.rows, h.x.cols, h.x.bf16, 1), &size);
+  void *work = on.workspace(ws, a[10], fn.df_linear_cross_entropy_workspace_bytes(h.x.rows, h.w.rows, h.x.cols, h.x.bf16, 1), &size);
   call(fn.df_linear_cross_entropy_backward, a[11], h.x.data, h.w.data, h.targets, lse, grad, const_cast<void *>(to[0].data), const_cast<void *>(to[1].data), work,
        size, h.x.rows, h.w.rows, h.x.cols, h.x.stride, h.w.stride, to[0].stride, to[1].stride, real(a[5]), h.x.bf16);
   return tuple_of({&d[0], &d[1]});
@@ -656,16 +666,16 @@ Polynomial polynomial(PyObject *o) {
 }
 
 PyObject *orthogonalize(Args a) {  // update steps coefficients eps out workspace stream
-  const OnDevice on(a[0], "update");
+  const OnDevice on(a[0], "update", a[6]);
   const Matrices u = matrices(a[0], "update");
   const Polynomial q = polynomial(a[2]);
   Out out, ws;
   given_or_empty(out, a[4], a[0], tensor(a[0]).sizes(), u.bf16 ? at::kBFloat16 : at::kFloat);
-  on.same(out.get(), "out");
+  on.same(on.result(out, a[4]), "out");
   const Matrices o = matrices(out.get(), "out");
   if (!tensor(out.get()).sizes().equals(tensor(a[0]).sizes()) || o.bf16 != u.bf16) refuse("out", "shape or dtype differs from update");
   uint64_t size = 0;
-  void *work = on.workspace(ws, a[5], a[6], fn.df_orthogonalize_workspace_bytes(u.n, u.rows, u.cols), &size);
+  void *work = on.workspace(ws, a[5], fn.df_orthogonalize_workspace_bytes(u.n, u.rows, u.cols), &size);
   call(fn.df_orthogonalize, a[6], static_cast<const void *>(u.data), o.data, work, size, u.n, u.rows, u.cols, u.matrix_stride, u.row_stride, o.matrix_stride,
        o.row_stride, u32(a[1]), q.a, q.b, q.c, real(a[3]), u.bf16);
   return out.release();
@@ -690,7 +700,7 @@ PyObject *muon_update(Args a) {  // parameters momenta gradients lr momentum wei
   const Sequence p(a[0]), m(a[1]), g(a[2]);
   if (m.size() != p.size() || g.size() != p.size()) refuse("parameters", "as many parameters, momenta and gradients are expected");
   if (p.size() == 0) Py_RETURN_NONE;
-  const OnDevice on(p[0], "parameters");
+  const OnDevice on(p[0], "parameters", a[12]);
   const at::Tensor &first = tensor(p[0]);
   if (first.dim() != 2) refuse("parameters", "expected matrices");
   const int64_t rows = first.size(0), cols = first.size(1);
@@ -705,7 +715,7 @@ PyObject *muon_update(Args a) {  // parameters momenta gradients lr momentum wei
   const uint32_t n = below_2_31(p.size(), "parameters"), r = below_2_31(rows, "parameters"), c = below_2_31(cols, "parameters");
   Out ws;
   uint64_t size = 0;
-  void *work = on.workspace(ws, a[11], a[12], fn.df_orthogonalize_workspace_bytes(n, r, c), &size);
+  void *work = on.workspace(ws, a[11], fn.df_orthogonalize_workspace_bytes(n, r, c), &size);
   call(fn.df_muon_update, a[12], static_cast<const void *>(table.data()), n, r, c, real(a[3]), real(a[4]), real(a[5]), truth(a[6]), real(a[7]), u32(a[8]), q.a, q.b,
        q.c, real(a[10]), work, size);
   Py_RETURN_NONE;
