@@ -373,6 +373,7 @@ def token_logprobs_backward(logits, targets, lse, entropy, grad_logp, grad_entro
 # torch's allocator for the call. With stream given, workspaces and results that are not given belong to that stream.
 # ------------------------------------------------------------------------------------------
 def linear_cross_entropy_workspace_bytes(rows, vocab, width, bf16, backward):
+    """Bytes for linear_cross_entropy; with backward enough for linear_cross_entropy_backward as well."""
     return int(lib().df_linear_cross_entropy_workspace_bytes(rows, vocab, width, int(bf16), int(backward)))
 
 
