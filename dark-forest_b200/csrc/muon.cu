@@ -109,6 +109,14 @@ __global__ void __launch_bounds__(256) k_update(const __grid_constant__ UpdatePa
   }
 }
 
+// What brings a matrix's elements to its X times 2^12: multiplied by `first`, a power of two that is 1 for all but the smallest and largest norms, then by the result. A
+// norm below 2^-116 has a factor that fp32 does not hold (eps = 0, or as small), one above 2^138 one with fewer bits. A norm of 0 gives infinity, and 0 times that NaN.
+__device__ __forceinline__ float norm_factor(double sum_of_squares, float eps, float *first) {
+  const double f = (double)kPartScale / (sqrt(sum_of_squares) + (double)eps);
+  *first = f > 0x1p100 ? 0x1p64f : f < 0x1p-100 ? 0x1p-64f : 1.0f;
+  return (float)(f / (double)*first);
+}
+
 // X in parts, a warp a row
 __global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ UpdateParams p, int blocks) {
   pdl_wait();
@@ -117,7 +125,8 @@ __global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ Updat
   for (int i = lane; i < blocks; i += 32) sum += p.sums[m * kNormBlocks + i];
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  const float f = (float)((double)kPartScale / (sqrt(sum) + (double)p.eps));
+  float first;
+  const float f = norm_factor(sum, p.eps, &first);
   const void *source = p.t.source[m];
   const float *momentum = p.t.momentum[m];
   for (uint32_t r = blockIdx.x * 8 + warp; r < p.rows; r += gridDim.x * 8) {
@@ -143,8 +152,8 @@ __global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ Updat
         }
       }
       uint2 hi, lo;
-      split_half2<0>(v[0] * f, v[1] * f, hi.x, lo.x);
-      split_half2<0>(v[2] * f, v[3] * f, hi.y, lo.y);
+      split_half2<0>(v[0] * first * f, v[1] * first * f, hi.x, lo.x);
+      split_half2<0>(v[2] * first * f, v[3] * first * f, hi.y, lo.y);
       *reinterpret_cast<uint2 *>(p.hi + to + c) = hi;
       *reinterpret_cast<uint2 *>(p.lo + to + c) = lo;
     }
@@ -875,7 +884,8 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
     sum = 0.0;
     for (uint32_t i = 0; i < p.ctas; ++i) sum += __ldcg(p.sums + m * p.ctas + i);
   }
-  const float f = (float)((double)kPartScale / (sqrt(sum) + (double)p.eps));
+  float first;
+  const float f = norm_factor(sum, p.eps, &first);
   for (uint32_t r = row_off + warp; r < row_off + rows; r += 8) {
 #pragma unroll 4
     for (uint32_t c = col_off + lane; c < col_off + cols; c += 32) {
@@ -884,7 +894,7 @@ __global__ void __launch_bounds__(256, 1) k_newton_schulz_small(const __grid_con
         const float v = momentum[r * p.cols + c];
         u = p.nesterov ? fmaf(p.beta, v, u) : v;
       }
-      u *= f;
+      u = u * first * f;
       const __half h = __float2half_rn(u);
       const uint32_t at = wide ? small_at(r, c - off) : small_at(c, r - off);
       *reinterpret_cast<__half *>(smem + kSmallX + at) = h;
