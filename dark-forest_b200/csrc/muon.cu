@@ -1301,7 +1301,7 @@ struct Plan {
 int check_call(uint32_t n, uint32_t rows, uint32_t cols, uint32_t steps, float a, float b, float c, float eps) {
   if (!sizes_ok(n, rows, cols) || steps < 1 || steps > 64) return DF_ERR_INVALID_ARG;
   if (!isfinite(a) || !isfinite(b) || !isfinite(c) || !isfinite(eps) || eps < 0.0f) return DF_ERR_INVALID_ARG;
-  // the parts hold values up to 15; |B| is at most this for singular values up to 1
+  // the parts hold values up to 15; |B|, and X after a step, are at most this for singular values up to 1. What later steps bring follows from the data.
   return fabsf(a) + fabsf(b) + fabsf(c) < 15.0f ? DF_OK : DF_ERR_UNSUPPORTED;
 }
 

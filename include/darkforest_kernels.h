@@ -493,7 +493,9 @@ DF_API int df_linear_cross_entropy_backward(const void *x, const void *weight, c
  *       momentum <- beta momentum + gradient; U = gradient + beta momentum (nesterov != 0) or momentum;
  *       parameter <- parameter (1 - lr weight_decay) - lr update_scale O(U). No parameter or momentum may overlap another tensor.
  * Precision: factors in 22 bits relative to 1 (elements below 2^-26 in fewer, none below 2^-37), sums in fp32, the norm in double, results rounded once.
- * |a| + |b| + |c| below 15 (else DF_ERR_UNSUPPORTED); singular values that a step brings above 3.8 make the matrix's results infinite or NaN. A zero matrix gives 0
+ * |a| + |b| + |c| below 15 (else DF_ERR_UNSUPPORTED), so that the first step's factors, of singular values up to 1, stay in range. Factors are held up to 15: X X^T, b X X^T + c (X X^T)^2 and,
+ * before the last step, X. They fit while s^2, |b s^2 + c s^4| and |a s + b s^3 + c s^5| are below 15 for all singular values s that occur (with the usual coefficients s up to 2; they
+ * stay below 1.3); an element above becomes infinite or NaN, and so does every result that it enters. A zero matrix gives 0
  * (eps > 0), an infinity or NaN NaN, both without touching the other matrices. Nothing depends on the order of execution.
  * workspace: df_orthogonalize_workspace_bytes (for both calls; at most 192 MB or one matrix), 256-byte aligned, contents undefined before and after, apart
  * from the call's tensors. Calls that can overlap need one each. */
