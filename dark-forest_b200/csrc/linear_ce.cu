@@ -1112,6 +1112,7 @@ int df_linear_cross_entropy_backward(const void *x, const void *weight, const in
   const uint64_t elt = bf16 ? 2 : 4;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (rows == 0) {  // a sum over no rows
+    if (Span(d_weight, vocab, dw_stride, width, elt).meets(Span(weight, vocab, weight_stride, width, elt))) return finish(DF_ERR_INVALID_ARG);
     if (d_weight) st = check_cuda(cudaMemset2DAsync(d_weight, (vocab > 1 ? dw_stride : width) * elt, 0, width * elt, vocab, s));
     return finish(st);
   }
