@@ -266,20 +266,18 @@ struct OutEpi {
   const Params &p;
   float4 *slab;
   int lane;
-  float f;
+  float f, inv;  // inv, a power of two, by itself: where x is near the smallest numbers their product leaves fp32
   float *plane;
   uint32_t row0, col0;
   __device__ __forceinline__ OutEpi(const Params &q, uint8_t *sl, int l) : p(q), slab(reinterpret_cast<float4 *>(sl)), lane(l) {}
   __device__ __forceinline__ void begin(const ProductTile &t, uint32_t r, uint32_t c0) {
     row0 = r - lane;
     col0 = c0;
-    f = 1.0f;
     if (p.planes) {
       plane = p.planes + (size_t)t.split * p.plane_rows * p.plane_pitch;
     } else {
-      float inv;
       part_scale(*p.largest_x, &inv);
-      f = inv * (p.scale / kGScale);
+      f = p.scale / kGScale;
     }
   }
   __device__ __forceinline__ void block(int cg, float (&v)[32]) {
@@ -301,7 +299,7 @@ struct OutEpi {
           *at = q[i];
         continue;
       }
-      write_four(p.out, (size_t)r * p.out_stride + col, make_float4(q[i].x * f, q[i].y * f, q[i].z * f, q[i].w * f), p.cols - col, p.out_bf16, p.vec);
+      write_four(p.out, (size_t)r * p.out_stride + col, make_float4(q[i].x * f * inv, q[i].y * f * inv, q[i].z * f * inv, q[i].w * f * inv), p.cols - col, p.out_bf16, p.vec);
     }
   }
   __device__ __forceinline__ void end() {}
@@ -596,13 +594,13 @@ __global__ void __launch_bounds__(256) k_sum_planes(const SumParams p) {
     v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
   }
   if (counts) {
-    float f = p.scale * p.grad[r];
+    float f = p.scale, inv = 1.0f;  // one after the other: their product may leave fp32
     if (p.largest_w) {
-      float inv;
       part_scale(*p.largest_w, &inv);
-      f = inv * (p.scale / kGScale) * p.grad[r];
+      f /= kGScale;
     }
-    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+    const float g = p.grad[r];
+    v.x = v.x * f * g * inv; v.y = v.y * f * g * inv; v.z = v.z * f * g * inv; v.w = v.w * f * g * inv;
   }
   write_four(p.out, (size_t)r * p.out_stride + col, v, p.width - col, p.out_bf16, p.vec);
 }
