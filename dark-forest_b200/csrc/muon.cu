@@ -1352,7 +1352,10 @@ int df_orthogonalize(const void *update, void *out, void *workspace, uint64_t wo
   const uint64_t most = 1ull << 40;
   if (update_matrix_stride >= most || update_row_stride >= most || out_matrix_stride >= most || out_row_stride >= most) return finish(DF_ERR_INVALID_ARG);
   if (rows > 1 && (update_row_stride < cols || out_row_stride < cols)) return finish(DF_ERR_INVALID_ARG);
-  if (n > 1 && out_matrix_stride < (uint64_t)(rows - 1) * out_row_stride + cols) return finish(DF_ERR_INVALID_ARG);
+  // results lie apart: one matrix behind the other, or row by row of all of them
+  if (n > 1 && out_matrix_stride < (uint64_t)(rows - 1) * out_row_stride + cols &&
+      (out_matrix_stride < cols || (rows > 1 && out_row_stride < (uint64_t)(n - 1) * out_matrix_stride + cols)))
+    return finish(DF_ERR_INVALID_ARG);
   // out is the update, element by element, or shares nothing with it
   const uint64_t in_elt = bf16 ? 2 : 4, in_bytes = ((uint64_t)(n - 1) * update_matrix_stride + (uint64_t)(rows - 1) * update_row_stride + cols) * in_elt;
   const uint64_t out_bytes = ((uint64_t)(n - 1) * out_matrix_stride + (uint64_t)(rows - 1) * out_row_stride + cols) * in_elt;

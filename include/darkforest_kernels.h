@@ -487,8 +487,8 @@ DF_API int df_linear_cross_entropy_backward(const void *x, const void *weight, c
 
 /* ---- orthogonalised updates of matrices, next to AdamW (no counterpart in the reference) ----
  * O(U): X = U / (|U|_F + eps); `steps` (1 .. 64) times X <- a X + (b X X^T + c (X X^T)^2) X. rows, cols up to 65536, rows * cols below 2^31, any of the two larger.
- *   df_orthogonalize   n matrices [rows][cols] (fp32, or bf16 with bf16 != 0; strides in elements): out = O(update). out may be the update itself, and may not
- *       overlap it otherwise.
+ *   df_orthogonalize   n matrices [rows][cols] (fp32, or bf16 with bf16 != 0; strides in elements): out = O(update). out may be the update itself, with its strides, and may not
+ *       lie between its first and last element otherwise. Results lie one matrix behind the other or row by row of all matrices.
  *   df_muon_update     n tensors [rows][cols] fp32, contiguous, described by df_muon_tensor_t entries in HOST memory, read before the call returns (up to 1024):
  *       momentum <- beta momentum + gradient; U = gradient + beta momentum (nesterov != 0) or momentum;
  *       parameter <- parameter (1 - lr weight_decay) - lr update_scale O(U). No parameter or momentum may overlap another tensor.
