@@ -466,7 +466,7 @@ DF_API int df_token_logprobs_backward(const void *logits, const int32_t *targets
  * x [rows] of `width` elements, weight [vocab] of `width` (both fp32, or both bf16 with bf16 != 0; row strides in elements), z = scale * x weight^T (scale > 0).
  *   df_linear_cross_entropy            lse = log sum exp z, loss = lse - z[target], both [rows] fp32. The caller sums or averages.
  *   df_linear_cross_entropy_backward   with G = exp(z - lse) - onehot(target): d_x = scale * grad_loss * G weight and d_weight = scale * (grad_loss * G)^T x,
- *       overwritten, in the inputs' type; lse as above, grad_loss [rows]; d_x or d_weight may be NULL (not wanted). No output, and not the workspace, may overlap anything else of the call.
+ *       overwritten, in the inputs' type; lse as above, grad_loss [rows]; d_x or d_weight may be NULL (not wanted). No output, and not the workspace, may overlap anything else of the call (a tensor counts from its first to its last element, gaps between its rows included).
  * A row whose target is outside 0 .. vocab - 1 is left out: loss 0, lse 0, no part of any gradient, whatever x holds there (NaN included). Infinities and NaN
  * elsewhere make the results that they enter NaN. rows = 0: nothing, or d_weight = 0.
  * Precision: products of bf16 are exact, G and grad_loss * x enter them in 11 bits (G below 2^-29 in steps of 2^-39); fp32 operands enter in 22 bits relative to the largest element of
