@@ -19,6 +19,7 @@
 #include <cuda_runtime_api.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <string>
 #include <vector>
 
@@ -646,6 +647,17 @@ Matrices matrices(PyObject *o, const char *what) {
           d == 3 && t.size(0) > 1 ? static_cast<uint64_t>(t.stride(0)) : 0, static_cast<uint64_t>(row_stride)};
 }
 
+// A count: a whole number, not what is left of one in 32 bits.
+uint32_t count(PyObject *o, const char *what) {
+  PyObject *n = PyFloat_Check(o) && PyFloat_AS_DOUBLE(o) == std::floor(PyFloat_AS_DOUBLE(o)) ? PyNumber_Long(o) : PyNumber_Index(o);  // 5.0 is one
+  if (!n) throw PythonError();
+  int overflow = 0;
+  const long long v = PyLong_AsLongLongAndOverflow(n, &overflow);
+  Py_DECREF(n);
+  if (overflow != 0 || v < 0 || v > 0x7fffffffll) refuse(what, "out of range");
+  return static_cast<uint32_t>(v);
+}
+
 struct Polynomial {
   float a, b, c;
 };
@@ -677,7 +689,7 @@ PyObject *orthogonalize(Args a) {  // update steps coefficients eps out workspac
   uint64_t size = 0;
   void *work = on.workspace(ws, a[5], fn.df_orthogonalize_workspace_bytes(u.n, u.rows, u.cols), &size);
   call(fn.df_orthogonalize, a[6], static_cast<const void *>(u.data), o.data, work, size, u.n, u.rows, u.cols, u.matrix_stride, u.row_stride, o.matrix_stride,
-       o.row_stride, u32(a[1]), q.a, q.b, q.c, real(a[3]), u.bf16);
+       o.row_stride, count(a[1], "steps"), q.a, q.b, q.c, real(a[3]), u.bf16);
   return out.release();
 }
 
@@ -716,7 +728,7 @@ PyObject *muon_update(Args a) {  // parameters momenta gradients lr momentum wei
   Out ws;
   uint64_t size = 0;
   void *work = on.workspace(ws, a[11], fn.df_orthogonalize_workspace_bytes(n, r, c), &size);
-  call(fn.df_muon_update, a[12], static_cast<const void *>(table.data()), n, r, c, real(a[3]), real(a[4]), real(a[5]), truth(a[6]), real(a[7]), u32(a[8]), q.a, q.b,
+  call(fn.df_muon_update, a[12], static_cast<const void *>(table.data()), n, r, c, real(a[3]), real(a[4]), real(a[5]), truth(a[6]), real(a[7]), count(a[8], "steps"), q.a, q.b,
        q.c, real(a[10]), work, size);
   Py_RETURN_NONE;
 }

@@ -1,4 +1,4 @@
-"""Matrices to orthogonalise that lie row by row of all of them, as the heads' parts of a projection do: in, out and in place."""
+"""Matrices to orthogonalise that lie row by row of all of them, as the heads' parts of a projection do: in, out and in place. Counts of steps."""
 import pytest
 
 from helpers import pkg
@@ -39,3 +39,17 @@ def test_results_that_would_overlap(torch):
         with pytest.raises(p.AttentionError):
             p.orthogonalize(u, out=held.as_strided((3, 6, 8), strides))
     assert not held.any()
+
+
+def test_steps_are_whole_numbers(torch):
+    """Not what 32 bits leave of them, nor what lies in front of a decimal point."""
+    p = pkg()
+    u = torch.randn(6, 8, device="cuda")
+    three = [[torch.randn(6, 8, device="cuda")] for _ in range(3)]
+    kept = three[0][0].clone()
+    for steps in (2 ** 32 + 5, 2 ** 64 + 5, -2 ** 64 + 5, -1, 0, 65, 2.5, float("inf"), float("nan")):
+        with pytest.raises((p.AttentionError, TypeError, OverflowError)):
+            p.orthogonalize(u, steps)
+        with pytest.raises((p.AttentionError, TypeError, OverflowError)):
+            p.muon_update(*three, 0.1, steps=steps)
+    assert torch.equal(three[0][0], kept) and torch.equal(p.orthogonalize(u, torch.tensor(5)), p.orthogonalize(u, 5.0))
