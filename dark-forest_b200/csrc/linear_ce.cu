@@ -637,9 +637,10 @@ struct Tiles {
 
 constexpr uint32_t kFewBlocks = 592;
 
-// Whether the weight is better read as it is (linear_ce_few.cuh) than through the tensor cores. In us, 50257 columns of 768 in fp32: the loss of 1 row 36 against 165,
-// 8 rows 54 and 142, 16 rows 100 and 138, 24 rows 189 and 154; the gradient of 1 row 107 and 276, 8 rows 150 and 246. bf16 needs no parts: the loss of 8 rows 58 and 27; the
-// gradient of 8 rows 234 and 168, but 22 and 40 with 3000 columns of 512, where launches count (3 against 8).
+// Whether the weight is better read as it is (linear_ce_few.cuh) than through the tensor cores. In us, 50257 columns of 768 in fp32, weights out of cache: the loss of 1 row 44 against
+// 151, 8 rows 60 and 126, 16 rows 108 and 133, 24 rows 189 (on the same weight again) and 133; 130000 columns of 2000: 16 rows 560 and 876. The gradient of 1 row 112 and 283, 8 rows 155
+// and 258. bf16 needs no parts: the loss of 8 rows 58 and 27; the gradient of 8 rows of 50257 x 768 234 and 168 (the same weight again), but 34 and 49 with 3000 columns of 512, where launches
+// count (3 against 8), and 56 and 63 with 5000 of 1024.
 bool few_rows(uint32_t rows, uint32_t vocab, uint32_t width, bool bf16, bool backward) {
   if (kFewMost * up(width, 128) * 4 > kFewSmem) return false;
   if (!backward) return !bf16 && rows <= kFewMost;
@@ -739,7 +740,8 @@ double tile_time(bool pair, uint64_t tiles, uint64_t n) {
   return (double)((tiles + (pair ? kPairs : 2 * kPairs) - 1) / (pair ? kPairs : 2 * kPairs)) * each;
 }
 
-// Which tiles. bf16: always pairs (1000 x 5000 rows of 768: 19 us and 21, 4096 x 50257: 204 and 304, the gradient 63 and 64, 8192 x 50257: 1739 and 2178). Parts: by the
+// Which tiles (times on the same inputs again; new ones cost more, 4096 x 50257 250). bf16: always pairs (1000 x 5000 rows of 768: 19 us and 21, 4096 x 50257: 204 and 304, the gradient 63
+// and 64, 8192 x 50257: 1739 and 2178). Parts: by the
 // estimate (777 x 10007 rows of 330, gradient: pairs 157 us, single CTAs 122; 2048 x 50257 of 768: 415 and 487).
 bool pairs(int parts, uint32_t M, uint32_t N, uint32_t K, int splits) {
   if (parts == 1) return true;

@@ -474,8 +474,8 @@ DF_API int df_token_logprobs_backward(const void *logits, const int32_t *targets
  * steps of 2^-50). Up to 16 rows (loss, fp32) and 8 (gradient) may be computed in fp32 throughout. Sums in fp32; results rounded once.
  * Nothing depends on the order of execution.
  * The logits' gradient exists piece by piece of the vocabulary in the workspace (up to 256 MB at a time, at least 256 columns).
- * workspace: df_linear_cross_entropy_workspace_bytes, with backward != 0 enough for either direction (the forward alone may need more than the backward), 256-byte aligned, contents
- * undefined before and after. Calls that can overlap need one each. */
+ * workspace: df_linear_cross_entropy_workspace_bytes of the call's sizes (fewer rows can need more: 2048 rows of 50257 x 768 in fp32 233 MB, 1024 rows 368), with backward != 0 enough
+ * for either direction (the forward alone may need more than the backward), 256-byte aligned, contents undefined before and after. Calls that can overlap need one each. */
 DF_API uint64_t df_linear_cross_entropy_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t width, uint32_t bf16, uint32_t backward);
 DF_API int df_linear_cross_entropy(const void *x, const void *weight, const int32_t *targets, float *loss, float *lse, void *workspace,
                             uint64_t workspace_bytes, uint32_t rows, uint32_t vocab, uint32_t width, uint64_t x_stride, uint64_t weight_stride,
