@@ -1177,8 +1177,8 @@ struct Plan {
     }
   }
 
-  // Time of a product in us with its contraction cut in 1 << form, without what comes between products: operands of 64 of the contraction are 64 KB a CTA, which
-  // arrive in about 1 us; results take 3, the exchange of partial sums 5.
+  // Time of a product in us with its contraction cut in 1 << form, without what comes between products: 64 of the contraction, 64 KB of operands a CTA,
+  // take about 1 us; results take 3, the exchange of partial sums 5.
   double estimate(uint32_t n, int form, Product which) const {
     const uint64_t ks = 1ull << form, slots = 148 / ks, m = (l.side + 127) / 128, x = (uint64_t)((rows + 127) / 128) * ((cols + 127) / 128), g = m * (m + 1) / 2;
     const uint64_t k = which == kGram ? (rows > cols ? rows : cols) : l.side, blocks = ((k + 63) / 64 + ks - 1) / ks;
